@@ -258,6 +258,101 @@ int ssd_paged_verify_attention(ssd_stream_t stream, const void* q, const void* p
                                float scale, int B, int T, int num_heads, int max_seq_len,
                                void* workspace, size_t workspace_bytes);
 
+/* ------------------------------------------------------- 8-bit paged KV cache */
+/*
+ * A paged cache that holds K and V in 8 bits (no counterpart in the reference, whose cache is
+ * bf16/fp32, jax_ssd/kernels/kv_cache.py:13): half the bytes of bf16 to store and to read.
+ *   pages  [2, num_layers, num_blocks, block_size, Hkv, D] e4m3
+ *   scales [2, num_layers, num_blocks, Hkv] fp32, powers of two: an element is its e4m3 value times
+ *          the scale of its plane, layer, page and KV head
+ * head_dim is 64, 128 or 256; pages, k, v, q, qkv and the outputs are 16-byte aligned
+ * (else SSD_ERR_UNSUPPORTED).  num_blocks * block_size < 2^31.
+ * A page's scale is the smallest power of two (at least 2^-118) under which its largest finite
+ * magnitude stays within e4m3's 448.  Rounding is to nearest even; infinities and NaN are stored as
+ * NaN and do not count for the scale.
+ * B = 0 or T = 0 is allowed and does nothing.
+ */
+
+/*
+ * Append new rows: token t < q_lens[b] (NULL: T) of sequence b enters at position
+ * seq_lens[b] - q_lens[b] + t, seq_lens counting the new tokens -- the positions
+ * ssd_kv8_attention gives them.  k, v [B, T, Hkv, D] in `dtype`.
+ * A page whose first row is among the new ones starts over.  In any other page the rows before
+ * the new ones keep their values: where a new row needs a larger scale they are rewritten under
+ * it (exactly, but for values below 2^-14 of the page's largest).  Rows behind the last new one
+ * keep their bytes.  A page written by the call belongs to one sequence; positions below 0, past
+ * max_blocks pages, or whose table entry is no block are skipped.
+ */
+int ssd_kv8_append(ssd_stream_t stream, void* pages, float* scales, int num_layers, int num_blocks, int block_size,
+                   int num_kv_heads, int head_dim, int layer, const int32_t* block_tables, int max_blocks,
+                   const int32_t* seq_lens, const int32_t* q_lens, const void* k, const void* v, int dtype, int B,
+                   int T);
+
+/*
+ * The same from a QKV projection's rows, qkv [B*T, (Hq+2Hkv)*D], with RoPE as ssd_rope_kv_write
+ * applies it: rotated q to q_out [B*T, Hq, D] (zeros for t >= q_lens[b]), rotated k and v into the
+ * pages with one rounding.  rope_cos, rope_sin [rope_max_pos, D/2] fp32.
+ */
+int ssd_kv8_rope_append(ssd_stream_t stream, const void* qkv, void* q_out, void* pages, float* scales, int dtype,
+                        int num_layers, int num_blocks, int block_size, int num_heads, int num_kv_heads, int head_dim,
+                        int layer, const int32_t* block_tables, int max_blocks, const int32_t* seq_lens,
+                        const int32_t* q_lens, const float* rope_cos, const float* rope_sin, int rope_max_pos, int B,
+                        int T);
+
+/* K and V rows k, v [B, N, Hkv, D] (`dtype`) of positions [B, N]; zeros where a position is negative, past
+ * the table or without a block. */
+int ssd_kv8_gather(ssd_stream_t stream, const void* pages, const float* scales, int num_layers, int num_blocks,
+                   int block_size, int num_kv_heads, int head_dim, int layer, const int32_t* block_tables,
+                   int max_blocks, const int32_t* positions, void* k, void* v, int dtype, int B, int N);
+
+size_t ssd_kv8_attention_workspace_size(int B, int T, int num_heads, int num_kv_heads, int head_dim,
+                                        int max_seq_len);
+
+/*
+ * ssd_paged_verify_attention over an 8-bit cache: same rows, positions, lengths and zero rows.
+ * q and out [B, T, Hq, D] in `dtype`; scores, softmax statistics and sums in fp32.  What a row does
+ * not see (positions past its own, rows behind seq_lens) does not reach it, NaN included.
+ */
+int ssd_kv8_attention(ssd_stream_t stream, const void* q, const void* pages, const float* scales, int dtype,
+                      int num_layers, int num_blocks, int block_size, int num_kv_heads, int head_dim, int layer,
+                      const int32_t* block_tables, int max_blocks, const int32_t* seq_lens, const int32_t* q_lens,
+                      void* out, float scale, int B, int T, int num_heads, int max_seq_len, void* workspace,
+                      size_t workspace_bytes);
+
+/* ---------------------------------------------------------------- page moves */
+/*
+ * Copy page src_ids[i * src_step] of one pool to page dst_ids[i * dst_step] of another (or the
+ * same) pool, i < n, in each of `planes` planes (2 * num_layers): `page_bytes` per page and plane,
+ * and, with scales_per_page > 0, that many fp32 scales (an 8-bit cache's Hkv).  A pool's plane is
+ * its block count times page_bytes.  Pairs with an id out of range on either side (-1) are skipped.
+ * count (device, may be NULL): number of pairs, at most n.  Within one pool no page may be both
+ * copied from and copied to, nor copied to twice: the pairs move in no particular order.
+ */
+int ssd_page_copy(ssd_stream_t stream, const void* src_pages, const float* src_scales, int src_blocks,
+                  void* dst_pages, float* dst_scales, int dst_blocks, int planes, size_t page_bytes,
+                  int scales_per_page, const int32_t* src_ids, int64_t src_step, const int32_t* dst_ids,
+                  int64_t dst_step, int n, const int32_t* count);
+
+/*
+ * Plan the compaction of a pool whose free list is free_list[0 : *free_top].  With U blocks in use
+ * (not on the list), the k-th used block at U or above moves to the k-th free block below U, both
+ * in ascending order: afterwards blocks 0 .. U-1 are in use.
+ *   remap [num_blocks]        new id of every block in use (its own where it stays), -1 for free ones
+ *   move_src, move_dst [num_blocks / 2, at least 1], num_moves [1]  the moves, for ssd_page_copy
+ *   ref_counts_out            the counts under the new ids
+ *   free_list_out, free_top_out  num_blocks - U free blocks, handed out from U upwards
+ * The *_out arrays may be the inputs themselves.  Pages and tables do not change: ssd_page_copy and
+ * ssd_page_remap carry the plan out.
+ */
+int ssd_page_compact(ssd_stream_t stream, const int32_t* free_list, const int32_t* free_top,
+                     const int32_t* ref_counts, int num_blocks, int32_t* free_list_out, int32_t* free_top_out,
+                     int32_t* ref_counts_out, int32_t* remap, int32_t* move_src, int32_t* move_dst,
+                     int32_t* num_moves);
+
+/* tables_out[b][i] = remap[tables[b][i]] for i < lens[b], else -1; tables_out may be tables. */
+int ssd_page_remap(ssd_stream_t stream, const int32_t* tables, int32_t* tables_out, const int32_t* lens,
+                   int max_blocks, int B, const int32_t* remap, int num_blocks);
+
 /* ------------------------------------------------------- K3: skinny projections */
 
 enum {

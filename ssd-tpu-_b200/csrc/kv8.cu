@@ -1,0 +1,412 @@
+// 8-bit paged KV cache: quantised append (plain, and fused with the rotary embedding) and read-back.
+//
+// Append.  New rows enter at the end of each sequence, at the positions the attention calls use: token t
+// of row b at n0 + t, n0 = seq_lens[b] - q_lens[b].  For one page, KV head and plane let R be the new rows:
+//   e = smallest exponent with max |R| <= 448 2^e;   if rows before R are in the page: e = max(e, e_page)
+//   stored = e4m3(R 2^-e),   earlier rows = e4m3(old 2^(e_page - e))  where e grew, else untouched.
+// A page whose first row is among the new ones starts over: what it held counts for nothing.  Rows behind
+// the last new one keep their bytes.
+//
+// One CTA per (sequence, touched page, KV head, plane): the page's scale has one owner, no atomics, and the
+// result does not depend on scheduling.  The rows stay in registers between the maximum and the rounding, so
+// each input byte is read once; old rows are read only when the scale grows.  Bound: HBM bytes for prompts,
+// launch latency for single tokens.
+#include "kv8.cuh"
+
+namespace ssd {
+namespace {
+
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, float* f);
+template <>
+__device__ __forceinline__ void load8<bf16>(const bf16* p, float* f) { unpack8(ld_act_v4(p), f); }
+template <>
+__device__ __forceinline__ void load8<float>(const float* p, float* f) {
+  const uint4 a = ld_act_v4(p), b = ld_act_v4(p + 4);
+  f[0] = __uint_as_float(a.x); f[1] = __uint_as_float(a.y); f[2] = __uint_as_float(a.z); f[3] = __uint_as_float(a.w);
+  f[4] = __uint_as_float(b.x); f[5] = __uint_as_float(b.y); f[6] = __uint_as_float(b.z); f[7] = __uint_as_float(b.w);
+}
+__device__ __forceinline__ void store8(bf16* p, const float* f) {
+  uint4 u;
+  __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&u);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) h[i] = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+  *reinterpret_cast<uint4*>(p) = u;
+}
+__device__ __forceinline__ void store8(float* p, const float* f) {
+  *reinterpret_cast<float4*>(p) = make_float4(f[0], f[1], f[2], f[3]);
+  *reinterpret_cast<float4*>(p + 4) = make_float4(f[4], f[5], f[6], f[7]);
+}
+
+struct AppendArgs {
+  Kv8Cache c;
+  const int32_t* tables;
+  int max_blocks;
+  const int32_t* seq_lens;
+  const int32_t* q_lens;
+  const void* k;        // row m, head h at k + m * row + h * D
+  const void* v;
+  int64_t row;          // elements between token rows
+  int T, pages_per_seq, kv_ctas;
+  // rotary embedding (nullptr cos: none)
+  const void* q;
+  void* q_out;          // [B*T, hq, D]
+  const float* cos_t;   // [rope_max_pos, D/2]
+  const float* sin_t;
+  int hq, rope_max_pos, total_rows;
+};
+
+// y1 = x1 c - x2 s, y2 = x2 c + x1 s, the products rounded one by one (as ssd_rope_kv_write does)
+__device__ __forceinline__ void rotate8(float* x1, float* x2, const float* c, const float* s) {
+#pragma unroll
+  for (int i = 0; i < 8; i += 4) {
+    const float4 cv = *reinterpret_cast<const float4*>(c + i), sv = *reinterpret_cast<const float4*>(s + i);
+    const float cc[4] = {cv.x, cv.y, cv.z, cv.w}, ss[4] = {sv.x, sv.y, sv.z, sv.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float a = x1[i + j], b = x2[i + j];
+      x1[i + j] = __fsub_rn(__fmul_rn(a, cc[j]), __fmul_rn(b, ss[j]));
+      x2[i + j] = __fadd_rn(__fmul_rn(b, cc[j]), __fmul_rn(a, ss[j]));
+    }
+  }
+}
+
+// Values of one item: 8 dims of V (or of K without rotation), or a rotation pair 8 + 8 of K.
+template <typename T, int D>
+struct Rows {
+  const AppendArgs& a;
+  int64_t m0;   // token row of position `first`
+  int first;    // first new position in the page
+  int head, plane;
+  __device__ __forceinline__ bool rotated() const { return a.cos_t != nullptr && plane == 0; }
+  // item i of the page's rows: local row r, 16 dims as two groups of 8 (d0, d1)
+  __device__ __forceinline__ void get(int i, int& r, int& d0, int& d1, float* x0, float* x1) const {
+    constexpr int PER = D / 16;
+    r = i / PER;
+    const int c = i % PER;
+    const T* base = reinterpret_cast<const T*>(plane ? a.v : a.k) + (m0 + r) * a.row + (int64_t)head * D;
+    if (rotated()) {
+      d0 = c * 8;
+      d1 = d0 + D / 2;
+    } else {
+      d0 = c * 16;
+      d1 = d0 + 8;
+    }
+    load8<T>(base + d0, x0);
+    load8<T>(base + d1, x1);
+    if (rotated()) {
+      const int p = min(first + r, a.rope_max_pos - 1);
+      rotate8(x0, x1, a.cos_t + (int64_t)p * (D / 2) + d0, a.sin_t + (int64_t)p * (D / 2) + d0);
+    }
+  }
+};
+
+template <typename T, int D>
+__device__ __forceinline__ void rope_q_cta(const AppendArgs& a, int cta) {
+  // one warp per token row and CTA-strided heads: items of 16 dims
+  constexpr int PER = D / 16;
+  const int items = a.hq * PER;
+  const int64_t m = cta;
+  const int b = (int)(m / a.T), t = (int)(m % a.T);
+  const int seq = a.seq_lens[b];
+  const int ql = a.q_lens ? min(max(a.q_lens[b], 0), a.T) : a.T;
+  const int pos = seq - ql + t;
+  const bool real = t < ql && pos >= 0;
+  const int p = real ? min(pos, a.rope_max_pos - 1) : 0;
+  const T* src = reinterpret_cast<const T*>(a.q) + m * a.row;
+  T* dst = reinterpret_cast<T*>(a.q_out) + m * a.hq * D;
+  for (int i = threadIdx.x; i < items; i += blockDim.x) {
+    const int h = i / PER, d = (i % PER) * 8;
+    float x0[8], x1[8];
+    if (real) {
+      load8<T>(src + h * D + d, x0);
+      load8<T>(src + h * D + d + D / 2, x1);
+      rotate8(x0, x1, a.cos_t + (int64_t)p * (D / 2) + d, a.sin_t + (int64_t)p * (D / 2) + d);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x0[j] = x1[j] = 0.f;
+    }
+    store8(dst + h * D + d, x0);
+    store8(dst + h * D + d + D / 2, x1);
+  }
+}
+
+// KEEP: items (of 16 values) a thread holds in registers between the two passes; rows of a page beyond
+// KEEP * blockDim.x items are read a second time (through L2).
+template <typename T, int D, int KEEP>
+__global__ void __launch_bounds__(256) kv8_append_kernel(const AppendArgs a) {
+  __shared__ float red[32];
+  pdl_wait();
+  pdl_trigger();
+  if ((int)blockIdx.x >= a.kv_ctas) {
+    rope_q_cta<T, D>(a, blockIdx.x - a.kv_ctas);
+    return;
+  }
+  int u = blockIdx.x;
+  const int plane = u & 1;
+  u >>= 1;
+  const int head = u % a.c.hkv;
+  u /= a.c.hkv;
+  const int i = u % a.pages_per_seq, b = u / a.pages_per_seq;
+  const int bs = a.c.block_size;
+  const int seq = a.seq_lens[b];
+  const int ql = a.q_lens ? min(max(a.q_lens[b], 0), a.T) : a.T;
+  const int n0 = seq - ql;
+  const int start = max(n0, 0);
+  const int page = start / bs + i;
+  const int64_t p0 = (int64_t)page * bs;
+  if (p0 >= seq || page >= a.max_blocks) return;
+  const int first = max(start, (int)p0);
+  const int rows = (int)min((int64_t)seq, p0 + bs) - first;
+  if (rows <= 0) return;
+  const int blk = ld_act(a.tables + (int64_t)b * a.max_blocks + page);
+  if ((unsigned)blk >= (unsigned)a.c.num_blocks) return;
+
+  constexpr int PER = D / 16;
+  const Rows<T, D> src{a, (int64_t)b * a.T + (first - n0), first, head, plane};
+  const int items = rows * PER;
+  float x[KEEP][16];
+  float amax = 0.f;
+#pragma unroll
+  for (int k = 0; k < KEEP; ++k) {
+    const int it = threadIdx.x + k * blockDim.x;
+    if (it < items) {
+      int r, d0, d1;
+      src.get(it, r, d0, d1, x[k], x[k] + 8);
+#pragma unroll
+      for (int j = 0; j < 16; ++j) amax = fmaxf(amax, finite_abs(x[k][j]));
+    }
+  }
+  for (int it = threadIdx.x + KEEP * blockDim.x; it < items; it += blockDim.x) {
+    int r, d0, d1;
+    float y[16];
+    src.get(it, r, d0, d1, y, y + 8);
+#pragma unroll
+    for (int j = 0; j < 16; ++j) amax = fmaxf(amax, finite_abs(y[j]));
+  }
+  amax = block_reduce(amax, red, OpMax());
+
+  float* scale = a.c.scales + plane * a.c.scale_plane + a.c.scale_layer + (int64_t)blk * a.c.hkv + head;
+  uint8_t* base = a.c.pages + plane * a.c.plane + a.c.layer + ((int64_t)blk * bs * a.c.hkv + head) * D;
+  const int64_t rstride = (int64_t)a.c.hkv * D;
+  const int r0 = first - (int)p0;  // first new row of the page
+  int e = kv8_exponent(amax);
+  if (r0 > 0) {
+    const int eo = scale_exponent(ld_act(scale));
+    if (e > eo) {
+      // the earlier rows move to the larger scale; exp2i's range holds the difference down to 2^-126, below
+      // which every value rounds to zero anyway
+      const float f = exp2i(max(eo - e, -126));
+      for (int it = threadIdx.x; it < r0 * PER; it += blockDim.x) {
+        uint4* p = reinterpret_cast<uint4*>(base + (it / PER) * rstride + (it % PER) * 16);
+        const uint4 w = ld_act_v4(p);
+        const uint32_t in[4] = {w.x, w.y, w.z, w.w};
+        uint32_t out[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float2 lo = e4m3_pair(in[j]), hi = e4m3_pair(in[j] >> 16);
+          const float v[4] = {lo.x, lo.y, hi.x, hi.y};
+          out[j] = e4m3x4(v, f);
+        }
+        *p = make_uint4(out[0], out[1], out[2], out[3]);
+      }
+    } else {
+      e = eo;
+    }
+  }
+  // every thread of the CTA has read the old scale only if r0 > 0; the barrier keeps the new one behind those reads
+  __syncthreads();
+  if (threadIdx.x == 0) *scale = exp2i(e);
+  const float inv = exp2i(-e);
+  auto put = [&](int r, int d0, int d1, const float* y) {
+    uint8_t* p = base + (r0 + r) * rstride;
+    *reinterpret_cast<uint2*>(p + d0) = make_uint2(e4m3x4(y, inv), e4m3x4(y + 4, inv));
+    *reinterpret_cast<uint2*>(p + d1) = make_uint2(e4m3x4(y + 8, inv), e4m3x4(y + 12, inv));
+  };
+#pragma unroll
+  for (int k = 0; k < KEEP; ++k) {
+    const int it = threadIdx.x + k * blockDim.x;
+    if (it < items) {
+      const int r = it / PER, c = it % PER;
+      if (src.rotated())
+        put(r, c * 8, c * 8 + D / 2, x[k]);
+      else
+        put(r, c * 16, c * 16 + 8, x[k]);
+    }
+  }
+  for (int it = threadIdx.x + KEEP * blockDim.x; it < items; it += blockDim.x) {
+    int r, d0, d1;
+    float y[16];
+    src.get(it, r, d0, d1, y, y + 8);
+    put(r, d0, d1, y);
+  }
+}
+
+template <typename T, int D>
+int launch_append_d(cudaStream_t st, const AppendArgs& a, int B) {
+  constexpr int KEEP = 2;
+  // two items (32 values) a thread, the block size a power of two between one warp and 256 threads
+  const int64_t items = (int64_t)a.c.block_size * (D / 16);
+  int threads = 32;
+  while (threads < 256 && (int64_t)threads * KEEP < items) threads *= 2;
+  const int64_t q_ctas = a.cos_t ? (int64_t)a.total_rows : 0;
+  if (a.kv_ctas + q_ctas > 0x7fffffff) return SSD_ERR_UNSUPPORTED;
+  SSD_PDL((kv8_append_kernel<T, D, KEEP>), (unsigned)(a.kv_ctas + q_ctas), threads, 0, st, a);
+  return SSD_OK;
+}
+
+template <typename T>
+int launch_append(cudaStream_t st, const AppendArgs& a, int B, int D) {
+  if (D == 256) return launch_append_d<T, 256>(st, a, B);
+  if (D == 128) return launch_append_d<T, 128>(st, a, B);
+  return launch_append_d<T, 64>(st, a, B);
+}
+
+int append_common(ssd_stream_t stream, AppendArgs a, int dtype, int B, int T, int D) {
+  const int bs = a.c.block_size;
+  const int64_t pages = ((int64_t)T + bs - 2) / bs + 1;  // pages that T consecutive rows can touch
+  const int64_t ctas = (int64_t)B * pages * a.c.hkv * 2;
+  if (ctas > 0x7fffffff || (int64_t)B * T > 0x7fffffff) return SSD_ERR_UNSUPPORTED;
+  a.T = T;
+  a.total_rows = B * T;
+  a.pages_per_seq = (int)pages;
+  a.kv_ctas = (int)ctas;
+  cudaStream_t st = (cudaStream_t)stream;
+  if (dtype == SSD_DTYPE_BF16) return launch_append<bf16>(st, a, B, D);
+  return launch_append<float>(st, a, B, D);
+}
+
+// K and V rows of positions [B][N] (-1: zeros): one warp per position, lanes over 16-byte pieces of its
+// heads in both planes.  Bound: HBM (1 byte in, 2 or 4 out).
+template <typename T, int D>
+__global__ void __launch_bounds__(256) kv8_gather_kernel(const Kv8Cache c, const int32_t* tables, int max_blocks,
+                                                         const int32_t* positions, int64_t rows, int N, T* k, T* v) {
+  pdl_wait();
+  pdl_trigger();
+  constexpr int PER = D / 16;
+  const int lane = threadIdx.x & 31;
+  const int64_t m = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (m >= rows) return;
+  const int b = (int)(m / N);
+  const int pos = ld_act(positions + m);
+  int blk = -1;
+  if (pos >= 0 && pos / c.block_size < max_blocks)
+    blk = ld_act(tables + (int64_t)b * max_blocks + pos / c.block_size);
+  const bool ok = (unsigned)blk < (unsigned)c.num_blocks;
+  const int items = c.hkv * PER;
+  const int64_t row = ok ? (int64_t)blk * c.block_size + pos % c.block_size : 0;
+  for (int i = lane; i < 2 * items; i += 32) {
+    const int plane = i >= items, j = plane ? i - items : i;
+    uint4 w = make_uint4(0, 0, 0, 0);
+    float s = 0.f;
+    if (ok) {
+      w = ld_act_v4(c.pages + plane * c.plane + c.layer + row * c.hkv * D + (int64_t)j * 16);
+      s = ld_act(c.scales + plane * c.scale_plane + c.scale_layer + (int64_t)blk * c.hkv + j / PER);
+    }
+    const uint32_t in[4] = {w.x, w.y, w.z, w.w};
+    float f[16];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const float2 lo = e4m3_pair(in[q]), hi = e4m3_pair(in[q] >> 16);
+      f[4 * q] = lo.x * s; f[4 * q + 1] = lo.y * s; f[4 * q + 2] = hi.x * s; f[4 * q + 3] = hi.y * s;
+    }
+    T* o = (plane ? v : k) + m * c.hkv * D + (int64_t)j * 16;
+    store8(o, f);
+    store8(o + 8, f + 8);
+  }
+}
+
+template <typename T>
+int launch_gather(cudaStream_t st, const Kv8Cache& c, const int32_t* tables, int max_blocks, const int32_t* positions,
+                  int64_t rows, int N, void* k, void* v, int D) {
+  const unsigned grid = (unsigned)((rows + 7) / 8);
+  T* ko = reinterpret_cast<T*>(k);
+  T* vo = reinterpret_cast<T*>(v);
+  if (D == 256)
+    SSD_PDL((kv8_gather_kernel<T, 256>), grid, 256, 0, st, c, tables, max_blocks, positions, rows, N, ko, vo);
+  else if (D == 128)
+    SSD_PDL((kv8_gather_kernel<T, 128>), grid, 256, 0, st, c, tables, max_blocks, positions, rows, N, ko, vo);
+  else
+    SSD_PDL((kv8_gather_kernel<T, 64>), grid, 256, 0, st, c, tables, max_blocks, positions, rows, N, ko, vo);
+  return SSD_OK;
+}
+
+}  // namespace
+}  // namespace ssd
+
+using namespace ssd;
+
+extern "C" int ssd_kv8_append(ssd_stream_t stream, void* pages, float* scales, int num_layers, int num_blocks,
+                              int block_size, int num_kv_heads, int head_dim, int layer, const int32_t* block_tables,
+                              int max_blocks, const int32_t* seq_lens, const int32_t* q_lens, const void* k,
+                              const void* v, int dtype, int B, int T) {
+  if (int rc = kv8_check(pages, scales, num_layers, num_blocks, block_size, num_kv_heads, head_dim, layer)) return rc;
+  if (B < 0 || T < 0 || max_blocks <= 0 || !block_tables || !seq_lens ||
+      (dtype != SSD_DTYPE_BF16 && dtype != SSD_DTYPE_F32))
+    return SSD_ERR_INVALID;
+  if (B == 0 || T == 0) return SSD_OK;
+  if (!k || !v) return SSD_ERR_INVALID;
+  if (!kv8_aligned(k) || !kv8_aligned(v)) return SSD_ERR_UNSUPPORTED;
+  AppendArgs a{};
+  a.c = kv8_cache(pages, scales, num_layers, num_blocks, block_size, num_kv_heads, head_dim, layer);
+  a.tables = block_tables;
+  a.max_blocks = max_blocks;
+  a.seq_lens = seq_lens;
+  a.q_lens = q_lens;
+  a.k = k;
+  a.v = v;
+  a.row = (int64_t)num_kv_heads * head_dim;
+  return append_common(stream, a, dtype, B, T, head_dim);
+}
+
+extern "C" int ssd_kv8_rope_append(ssd_stream_t stream, const void* qkv, void* q_out, void* pages, float* scales,
+                                   int dtype, int num_layers, int num_blocks, int block_size, int num_heads,
+                                   int num_kv_heads, int head_dim, int layer, const int32_t* block_tables,
+                                   int max_blocks, const int32_t* seq_lens, const int32_t* q_lens,
+                                   const float* rope_cos, const float* rope_sin, int rope_max_pos, int B, int T) {
+  if (int rc = kv8_check(pages, scales, num_layers, num_blocks, block_size, num_kv_heads, head_dim, layer)) return rc;
+  if (B < 0 || T < 0 || max_blocks <= 0 || num_heads <= 0 || rope_max_pos <= 0 || !block_tables || !seq_lens ||
+      !rope_cos || !rope_sin || (dtype != SSD_DTYPE_BF16 && dtype != SSD_DTYPE_F32))
+    return SSD_ERR_INVALID;
+  if (B == 0 || T == 0) return SSD_OK;
+  if (!qkv || !q_out) return SSD_ERR_INVALID;
+  if (!kv8_aligned(qkv) || !kv8_aligned(q_out) || !kv8_aligned(rope_cos) || !kv8_aligned(rope_sin))
+    return SSD_ERR_UNSUPPORTED;
+  const size_t es = dtype == SSD_DTYPE_BF16 ? 2 : 4;
+  AppendArgs a{};
+  a.c = kv8_cache(pages, scales, num_layers, num_blocks, block_size, num_kv_heads, head_dim, layer);
+  a.tables = block_tables;
+  a.max_blocks = max_blocks;
+  a.seq_lens = seq_lens;
+  a.q_lens = q_lens;
+  a.q = qkv;
+  a.k = reinterpret_cast<const char*>(qkv) + es * (size_t)num_heads * head_dim;
+  a.v = reinterpret_cast<const char*>(qkv) + es * (size_t)(num_heads + num_kv_heads) * head_dim;
+  a.row = (int64_t)(num_heads + 2 * num_kv_heads) * head_dim;
+  a.q_out = q_out;
+  a.cos_t = rope_cos;
+  a.sin_t = rope_sin;
+  a.hq = num_heads;
+  a.rope_max_pos = rope_max_pos;
+  return append_common(stream, a, dtype, B, T, head_dim);
+}
+
+extern "C" int ssd_kv8_gather(ssd_stream_t stream, const void* pages, const float* scales, int num_layers,
+                              int num_blocks, int block_size, int num_kv_heads, int head_dim, int layer,
+                              const int32_t* block_tables, int max_blocks, const int32_t* positions, void* k, void* v,
+                              int dtype, int B, int N) {
+  if (int rc = kv8_check(pages, scales, num_layers, num_blocks, block_size, num_kv_heads, head_dim, layer)) return rc;
+  if (B < 0 || N < 0 || max_blocks <= 0 || !block_tables || (dtype != SSD_DTYPE_BF16 && dtype != SSD_DTYPE_F32))
+    return SSD_ERR_INVALID;
+  if (B == 0 || N == 0) return SSD_OK;
+  if (!positions || !k || !v) return SSD_ERR_INVALID;
+  if (!kv8_aligned(k) || !kv8_aligned(v)) return SSD_ERR_UNSUPPORTED;
+  const int64_t rows = (int64_t)B * N;
+  if ((rows + 7) / 8 > 0x7fffffff) return SSD_ERR_UNSUPPORTED;
+  const Kv8Cache c = kv8_cache(const_cast<void*>(pages), const_cast<float*>(scales), num_layers, num_blocks,
+                               block_size, num_kv_heads, head_dim, layer);
+  cudaStream_t st = (cudaStream_t)stream;
+  if (dtype == SSD_DTYPE_BF16)
+    return launch_gather<bf16>(st, c, block_tables, max_blocks, positions, rows, N, k, v, head_dim);
+  return launch_gather<float>(st, c, block_tables, max_blocks, positions, rows, N, k, v, head_dim);
+}

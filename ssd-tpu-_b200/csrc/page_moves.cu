@@ -1,0 +1,241 @@
+// Page moves of a paged cache: whole pages copied inside a pool (or into another of the same page shape), and
+// a fragmented pool compacted.
+//
+// A page is a run of `page_bytes` at a fixed stride in each of `planes` arrays (K and V of every layer), so
+// the copies know nothing of the element type; an 8-bit cache's scales are a second, small set of runs.
+#include "common.cuh"
+
+namespace ssd {
+namespace {
+
+constexpr int kCopyThreads = 256;
+
+struct PageRuns {
+  const char* src;
+  char* dst;
+  int64_t bytes;                 // of one page in one plane; multiple of `vec`
+  int64_t src_plane, dst_plane;  // bytes between planes
+};
+
+struct CopyArgs {
+  PageRuns data, scales;         // scales.bytes = 0: none
+  const int32_t* src_ids;
+  const int32_t* dst_ids;
+  int64_t src_step, dst_step;    // elements between ids (0: the same id for every pair)
+  const int32_t* count;          // pairs on the device, or NULL (= n)
+  int n, planes;
+  int src_blocks, dst_blocks;
+  int parts;                     // CTAs a page of one plane is cut into
+};
+
+// One CTA per (pair, plane, part).  Pairs with an id out of range on either side (-1) are skipped.
+template <typename V>
+__global__ void __launch_bounds__(kCopyThreads) page_copy_kernel(const CopyArgs a) {
+  pdl_wait();
+  pdl_trigger();
+  const int n = a.count ? min(ld_act(a.count), a.n) : a.n;
+  const int64_t work = (int64_t)n * a.planes * a.parts;
+  for (int64_t w = blockIdx.x; w < work; w += gridDim.x) {
+    const int part = (int)(w % a.parts);
+    const int64_t pp = w / a.parts;
+    const int plane = (int)(pp % a.planes), i = (int)(pp / a.planes);
+    const int s = ld_act(a.src_ids + i * a.src_step), d = ld_act(a.dst_ids + i * a.dst_step);
+    if ((unsigned)s >= (unsigned)a.src_blocks || (unsigned)d >= (unsigned)a.dst_blocks) continue;
+    const V* from = reinterpret_cast<const V*>(a.data.src + plane * a.data.src_plane + s * a.data.bytes);
+    V* to = reinterpret_cast<V*>(a.data.dst + plane * a.data.dst_plane + d * a.data.bytes);
+    if (from == to) continue;
+    const int64_t items = a.data.bytes / (int64_t)sizeof(V);
+    const int64_t per = (items + a.parts - 1) / a.parts;
+    const int64_t end = min(items, (part + 1) * per);
+    for (int64_t k = part * per + threadIdx.x; k < end; k += kCopyThreads) to[k] = __ldcg(from + k);
+    if (part == 0 && a.scales.bytes) {
+      const float* fs = reinterpret_cast<const float*>(a.scales.src + plane * a.scales.src_plane + s * a.scales.bytes);
+      float* ts = reinterpret_cast<float*>(a.scales.dst + plane * a.scales.dst_plane + d * a.scales.bytes);
+      for (int k = threadIdx.x; k < a.scales.bytes / 4; k += kCopyThreads) ts[k] = __ldcg(fs + k);
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------- compaction
+// U = blocks not on the free list.  The k-th of them at U or above (ascending) moves to the k-th free block
+// below U: the fewest moves there can be, and no block is both read and written.  One CTA: the pool's state
+// is a few integers per block; each thread owns a run of blocks, ranks come from one block-wide scan.
+constexpr int kPlanThreads = 1024;
+
+struct CompactArgs {
+  const int32_t *free_list, *free_top, *ref_counts;
+  int32_t *free_list_out, *free_top_out, *ref_counts_out;
+  int32_t *remap, *src, *dst, *moves;  // [num_blocks], [num_blocks / 2], [num_blocks / 2], [1]
+  int num_blocks;
+};
+
+__device__ __forceinline__ int2 block_scan2(int2 v, int2* tmp, int2* total) {
+  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
+  int2 x = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int a = __shfl_up_sync(0xffffffffu, x.x, o), b = __shfl_up_sync(0xffffffffu, x.y, o);
+    if (lane >= o) { x.x += a; x.y += b; }
+  }
+  if (lane == 31) tmp[wid] = x;
+  __syncthreads();
+  if (wid == 0) {
+    int2 y = tmp[lane];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int a = __shfl_up_sync(0xffffffffu, y.x, o), b = __shfl_up_sync(0xffffffffu, y.y, o);
+      if (lane >= o) { y.x += a; y.y += b; }
+    }
+    tmp[lane] = y;
+  }
+  __syncthreads();
+  const int2 base = wid ? tmp[wid - 1] : make_int2(0, 0);
+  *total = tmp[31];
+  __syncthreads();
+  return make_int2(base.x + x.x - v.x, base.y + x.y - v.y);  // exclusive
+}
+
+__global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(const CompactArgs a) {
+  __shared__ int2 tmp[32];
+  pdl_wait();
+  const int nb = a.num_blocks, tid = threadIdx.x;
+  const int top = min(max(ld_act(a.free_top), 0), nb);
+  for (int i = tid; i < nb; i += kPlanThreads) a.remap[i] = i;
+  __syncthreads();
+  for (int i = tid; i < top; i += kPlanThreads) {
+    const int f = ld_act(a.free_list + i);
+    if ((unsigned)f < (unsigned)nb) a.remap[f] = -1;
+  }
+  __syncthreads();
+  const int per = (nb + kPlanThreads - 1) / kPlanThreads;
+  const int i0 = min(nb, tid * per), i1 = min(nb, i0 + per);
+  int used = 0;
+  for (int i = i0; i < i1; ++i) used += a.remap[i] >= 0;
+  int2 total;
+  block_scan2(make_int2(used, 0), tmp, &total);
+  const int U = total.x;
+  // free blocks below U, used blocks at or above it
+  int2 mine = make_int2(0, 0);
+  for (int i = i0; i < i1; ++i) {
+    const bool u = a.remap[i] >= 0;
+    mine.x += !u && i < U;
+    mine.y += u && i >= U;
+  }
+  int2 at = block_scan2(mine, tmp, &total);
+  for (int i = i0; i < i1; ++i) {
+    const bool u = a.remap[i] >= 0;
+    if (!u && i < U) a.dst[at.x++] = i;
+    if (u && i >= U) a.src[at.y++] = i;
+  }
+  __syncthreads();
+  const int n = total.y;  // == total.x: both count U minus the used blocks below U
+  for (int i = tid; i < nb; i += kPlanThreads)
+    a.free_list_out[i] = i < nb - U ? nb - 1 - i : -1;  // pops hand out U, U + 1, ...
+  if (a.ref_counts_out != a.ref_counts)
+    for (int i = tid; i < nb; i += kPlanThreads) a.ref_counts_out[i] = ld_act(a.ref_counts + i);
+  __syncthreads();
+  for (int k = tid; k < n; k += kPlanThreads) {
+    const int s = a.src[k], d = a.dst[k];
+    a.remap[s] = d;
+    a.ref_counts_out[d] = ld_act(a.ref_counts + s);
+    a.ref_counts_out[s] = 0;
+  }
+  if (tid == 0) {
+    *a.moves = n;
+    *a.free_top_out = nb - U;
+  }
+  pdl_trigger();
+}
+
+// out[b][i] = remap[in[b][i]] for i < lens[b], -1 behind (ids out of range become -1).
+__global__ void table_remap_kernel(const int32_t* in, int32_t* out, const int32_t* lens, int64_t entries,
+                                   int max_blocks, const int32_t* remap, int num_blocks) {
+  pdl_wait();
+  pdl_trigger();
+  for (int64_t e = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; e < entries; e += (int64_t)gridDim.x * blockDim.x) {
+    const int b = (int)(e / max_blocks), i = (int)(e % max_blocks);
+    const int blk = i < ld_act(lens + b) ? ld_act(in + e) : -1;
+    out[e] = (unsigned)blk < (unsigned)num_blocks ? ld_act(remap + blk) : -1;
+  }
+}
+
+template <typename V>
+int launch_copy(cudaStream_t st, CopyArgs a) {
+  const int64_t items = a.data.bytes / (int64_t)sizeof(V);
+  // a CTA moves up to 16 vectors a thread; small pages take one CTA
+  a.parts = (int)((items + kCopyThreads * 16 - 1) / (kCopyThreads * 16));
+  const int64_t work = (int64_t)a.n * a.planes * a.parts;
+  SSD_PDL(page_copy_kernel<V>, (unsigned)(work < (1 << 20) ? work : (1 << 20)), kCopyThreads, 0, st, a);
+  return SSD_OK;
+}
+
+inline bool aligned_to(const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+
+int copy_common(cudaStream_t st, const CopyArgs& a) {
+  auto fits = [&](size_t v) {
+    return a.data.bytes % v == 0 && a.data.src_plane % v == 0 && a.data.dst_plane % v == 0 &&
+           aligned_to(a.data.src, v) && aligned_to(a.data.dst, v);
+  };
+  if (fits(16)) return launch_copy<uint4>(st, a);
+  if (fits(4)) return launch_copy<uint32_t>(st, a);
+  return launch_copy<uint8_t>(st, a);
+}
+
+}  // namespace
+}  // namespace ssd
+
+using namespace ssd;
+
+extern "C" int ssd_page_copy(ssd_stream_t stream, const void* src_pages, const float* src_scales, int src_blocks,
+                             void* dst_pages, float* dst_scales, int dst_blocks, int planes, size_t page_bytes,
+                             int scales_per_page, const int32_t* src_ids, int64_t src_step, const int32_t* dst_ids,
+                             int64_t dst_step, int n, const int32_t* count) {
+  if (n < 0 || planes <= 0 || page_bytes == 0 || src_blocks <= 0 || dst_blocks <= 0 || scales_per_page < 0 ||
+      src_step < 0 || dst_step < 0 || !src_pages || !dst_pages)
+    return SSD_ERR_INVALID;
+  if (scales_per_page > 0 && (!src_scales || !dst_scales)) return SSD_ERR_INVALID;
+  if (n == 0) return SSD_OK;
+  if (!src_ids || !dst_ids) return SSD_ERR_INVALID;
+  if (page_bytes > (size_t)1 << 31) return SSD_ERR_UNSUPPORTED;
+  CopyArgs a{};
+  a.data = {reinterpret_cast<const char*>(src_pages), reinterpret_cast<char*>(dst_pages), (int64_t)page_bytes,
+            (int64_t)page_bytes * src_blocks, (int64_t)page_bytes * dst_blocks};
+  const int64_t sb = (int64_t)scales_per_page * (int64_t)sizeof(float);
+  a.scales = {reinterpret_cast<const char*>(src_scales), reinterpret_cast<char*>(dst_scales), sb, sb * src_blocks,
+              sb * dst_blocks};
+  a.src_ids = src_ids;
+  a.dst_ids = dst_ids;
+  a.src_step = src_step;
+  a.dst_step = dst_step;
+  a.count = count;
+  a.n = n;
+  a.planes = planes;
+  a.src_blocks = src_blocks;
+  a.dst_blocks = dst_blocks;
+  return copy_common((cudaStream_t)stream, a);
+}
+
+extern "C" int ssd_page_compact(ssd_stream_t stream, const int32_t* free_list, const int32_t* free_top,
+                                const int32_t* ref_counts, int num_blocks, int32_t* free_list_out,
+                                int32_t* free_top_out, int32_t* ref_counts_out, int32_t* remap, int32_t* move_src,
+                                int32_t* move_dst, int32_t* num_moves) {
+  if (num_blocks <= 0 || !free_list || !free_top || !ref_counts || !free_list_out || !free_top_out ||
+      !ref_counts_out || !remap || !move_src || !move_dst || !num_moves)
+    return SSD_ERR_INVALID;
+  const CompactArgs a{free_list, free_top, ref_counts, free_list_out, free_top_out, ref_counts_out,
+                      remap, move_src, move_dst, num_moves, num_blocks};
+  SSD_PDL(compact_plan_kernel, 1, kPlanThreads, 0, (cudaStream_t)stream, a);
+  return SSD_OK;
+}
+
+extern "C" int ssd_page_remap(ssd_stream_t stream, const int32_t* tables, int32_t* tables_out, const int32_t* lens,
+                              int max_blocks, int B, const int32_t* remap, int num_blocks) {
+  if (B < 0 || max_blocks <= 0 || num_blocks <= 0) return SSD_ERR_INVALID;
+  if (B == 0) return SSD_OK;
+  if (!tables || !tables_out || !lens || !remap) return SSD_ERR_INVALID;
+  const int64_t entries = (int64_t)B * max_blocks;
+  const int64_t ctas = (entries + 255) / 256;
+  SSD_PDL(table_remap_kernel, (unsigned)(ctas < 1184 ? ctas : 1184), 256, 0, (cudaStream_t)stream, tables, tables_out,
+          lens, entries, max_blocks, remap, num_blocks);
+  return SSD_OK;
+}

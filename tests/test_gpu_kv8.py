@@ -1,0 +1,439 @@
+"""GPU: the 8-bit paged KV cache against the oracle in 64 bits -- append, RoPE append, read-back, attention."""
+
+from __future__ import annotations
+
+import math
+
+import numpy as np
+import pytest
+
+from oracle import kv8 as o
+
+pytestmark = pytest.mark.gpu
+
+EPS = {"bf16": 2.0 ** -8, "f32": 2.0 ** -24}  # half a step, relative
+
+
+def _torch():
+    import torch
+
+    return torch, {"bf16": torch.bfloat16, "f32": torch.float32}
+
+
+def _round(x, dtype):
+    torch, dts = _torch()
+    return torch.tensor(np.asarray(x, np.float32)).to(dts[dtype]).float().numpy().astype(np.float64)
+
+
+class Pool:
+    """A one-layer (layer 1 of 2) cache with tables, on both sides; dead bytes are NaN and dead scales garbage."""
+
+    def __init__(self, rng, b, bs, hkv, d, cols):
+        from ssd_b200.kernels.kv8_cache import KV8CacheState
+
+        torch, _ = _torch()
+        nb = b * cols + 3
+        self.bs, self.hkv, self.d = bs, hkv, d
+        self.cache = KV8CacheState.allocate(2, nb, bs, hkv, d)
+        self.cache.pages.view(torch.uint8).fill_(0x7F)
+        self.cache.scales.fill_(float("nan"))
+        self.vals = np.full((2, nb, bs, hkv, d), np.nan)
+        self.exps = np.full((2, nb, hkv), 120, np.int64)
+        self.tables = np.full((b, cols), -1, np.int32)
+        perm = rng.permutation(nb)
+        for i in range(b):
+            self.tables[i] = perm[i * cols:(i + 1) * cols]
+        self.dev_tables = torch.tensor(self.tables, device="cuda")
+
+    def append(self, seq_lens, k, v, q_lens, dtype):
+        from ssd_b200.kernels.kv8_cache import append_kv8
+
+        torch, dts = _torch()
+        t = lambda a: torch.tensor(np.asarray(a, np.float32)).to(dts[dtype]).cuda()  # noqa: E731
+        i = lambda a: torch.tensor(np.asarray(a, np.int32), device="cuda")  # noqa: E731
+        k, v = _round(k, dtype), _round(v, dtype)  # what the device is given, on both sides
+        append_kv8(self.cache, 1, self.dev_tables, i(seq_lens), t(k), t(v), q_lens=i(q_lens))
+        for r, (n, m) in enumerate(zip(seq_lens, q_lens)):
+            m = min(max(int(m), 0), k.shape[1])
+            o.append(self.vals, self.exps, self.tables[r], int(n), k[r, :m], v[r, :m])
+
+    def check(self):
+        """The whole layer, dead rows included, byte for byte; the other layer untouched."""
+        torch, _ = _torch()
+        got = self.cache.pages[:, 1].float().cpu().numpy().astype(np.float64)
+        np.testing.assert_array_equal(got, self.vals)
+        live = ~np.isnan(self.vals).all(axis=(2, 4))  # pages and heads that hold something
+        sc = self.cache.scales[:, 1].cpu().numpy()
+        np.testing.assert_array_equal(sc[live], np.exp2(self.exps[live].astype(np.float64)))
+        assert (self.cache.pages[:, 0].view(torch.uint8) == 0x7F).all() and self.cache.scales[:, 0].isnan().all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("bs,hkv,d", [(16, 1, 256), (16, 4, 64), (4, 2, 128), (32, 3, 256), (1, 2, 64), (7, 2, 128),
+                                      (100, 1, 256)])
+def test_append_in_steps_of_every_size(cuda, dtype, bs, hkv, d):
+    """Prompts, then single tokens and short runs whose magnitudes rise and fall; rows with nothing new; then a
+    rollback: the sequence goes on from a shorter length."""
+    rng = np.random.default_rng(bs * d + hkv)
+    b = 4
+    p = Pool(rng, b, bs, hkv, d, cols=3 + 60 // bs)
+    lens = np.zeros(b, int)
+    for step, (t, mag) in enumerate([(37, 1.0), (1, 0.01), (1, 900.0), (5, 1.0), (0, 1.0), (3, 2.0 ** -30), (2, 1e30),
+                                     (1, 0.0), (4, 1.0)]):
+        if step == 6:
+            lens = np.maximum(lens - np.arange(b) * 3, 0)  # rolled back by 0, 3, 6, 9 tokens
+        ql = np.array([t, max(t - 1, 0), 0 if step % 2 else t, t])
+        lens = lens + ql
+        k = _round(mag * rng.standard_normal((b, max(t, 1), hkv, d)), dtype)
+        v = _round(rng.standard_normal((b, max(t, 1), hkv, d)) * np.exp2(rng.integers(-6, 6, (b, 1, hkv, 1))), dtype)
+        p.append(lens, k, v, ql, dtype)
+        p.check()
+
+
+def test_append_skips_what_it_cannot_place(cuda):
+    """Tables without a block, pages past the table, q_lens above T and above the length: no write there."""
+    torch, _ = _torch()
+    rng = np.random.default_rng(5)
+    p = Pool(rng, 3, 16, 2, 64, cols=3)
+    p.tables[0, 1], p.tables[1, 0] = -1, 10 ** 6
+    p.dev_tables = torch.tensor(p.tables, device="cuda")
+    k = _round(rng.standard_normal((3, 40, 2, 64)), "bf16")
+    p.append([40, 60, 8], k, 2 * k, [40, 99, 40], "bf16")  # row 2: positions -32 .. 7
+    p.check()
+
+
+def test_append_of_non_finite_rows(cuda):
+    """Infinities and NaN are stored as NaN and leave the scale to the finite values."""
+    rng = np.random.default_rng(6)
+    p = Pool(rng, 1, 16, 1, 64, cols=2)
+    k = _round(rng.standard_normal((1, 20, 1, 64)), "bf16")
+    k[0, 3, 0, 5], k[0, 3, 0, 6], k[0, 17, 0, 0] = np.inf, np.nan, -np.inf
+    p.append([20], k, k[:, ::-1].copy(), [20], "bf16")
+    p.check()
+
+
+@pytest.mark.parametrize("bs,hkv,d,n", [(16, 1, 64, 5), (16, 16, 256, 33), (4, 3, 128, 1), (32, 2, 64, 70)])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_gather_returns_the_stored_values(cuda, dtype, bs, hkv, d, n):
+    from ssd_b200.kernels.kv8_cache import gather_kv8
+
+    torch, dts = _torch()
+    rng = np.random.default_rng(n)
+    p = Pool(rng, 2, bs, hkv, d, cols=80 // bs + 1)
+    k = _round(rng.standard_normal((2, 75, hkv, d)), "bf16")
+    p.append([75, 40], k, 3 * k, [75, 40], "bf16")
+    pos = rng.integers(-2, 40, (2, n)).astype(np.int32)
+    pos[0, 0] = 10 ** 6
+    gk, gv = gather_kv8(p.cache, 1, p.dev_tables, torch.tensor(pos, device="cuda"), dtype=dts[dtype])
+    for r in range(2):
+        rk, rv = o.rows_of(p.vals, p.exps, p.tables[r], pos[r])
+        np.testing.assert_array_equal(gk[r].float().cpu().numpy(), rk)
+        np.testing.assert_array_equal(gv[r].float().cpu().numpy(), rv)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("hq,hkv,d,bs,t", [(8, 1, 256, 16, 1), (16, 16, 256, 16, 5), (4, 2, 128, 4, 7), (4, 1, 64, 16, 3),
+                                           (6, 2, 64, 32, 64)])
+def test_rope_append(cuda, dtype, hq, hkv, d, bs, t):
+    from ssd_b200.kernels.kv8_cache import gather_kv8, rope_append_kv8
+    from ssd_b200.models.gemma import rope_tables
+
+    torch, dts = _torch()
+    rng = np.random.default_rng(hq * d + t)
+    b = 3
+    lens, ql = np.array([t + 9, t + 30, t]), np.array([t, t, max(t - 1, 0)])
+    p = Pool(rng, b, bs, hkv, d, cols=-(-(t + 30) // bs))
+    old = _round(rng.standard_normal((b, 30, hkv, d)), "bf16")
+    p.append(lens - ql, old, old, np.minimum(lens - ql, 30), "bf16")
+    cos, sin = rope_tables(t + 40, d)
+    x = _round(rng.standard_normal((b, t, hq + 2 * hkv, d)), dtype)
+    i = lambda a: torch.tensor(np.asarray(a, np.int32), device="cuda")  # noqa: E731
+    q = rope_append_kv8(torch.tensor(x.reshape(b * t, -1)).to(dts[dtype]).cuda(), p.cache, 1, p.dev_tables, i(lens), hq,
+                        torch.tensor(cos, device="cuda"), torch.tensor(sin, device="cuda"), q_lens=i(ql))
+    got = q.float().cpu().numpy()
+    for r in range(b):
+        n = int(ql[r])
+        at = np.arange(lens[r] - n, lens[r])
+        c, s = cos[at].astype(np.float64)[:, None], sin[at].astype(np.float64)[:, None]
+        a, z = x[r, :n, :hq + hkv, :d // 2], x[r, :n, :hq + hkv, d // 2:]
+        y = np.concatenate([a * c - z * s, z * c + a * s], -1)
+        # two products and a sum in fp32, then the output's rounding
+        tol = 3 * 2.0 ** -24 * (np.abs(np.concatenate([a, z], -1)) + np.abs(np.concatenate([z, a], -1)))
+        assert (np.abs(got[r, :n] - y[:, :hq]) <= tol[:, :hq] + EPS[dtype] * np.abs(y[:, :hq])).all()
+        assert (got[r, n:] == 0).all()
+        o.append(p.vals, p.exps, p.tables[r], int(lens[r]), y[:, hq:], x[r, :n, hq + hkv:])
+        pos = np.arange(lens[r])
+        tab = p.dev_tables[r:r + 1].contiguous()
+        gk, gv = (g[0].float().cpu().numpy() for g in gather_kv8(p.cache, 1, tab, i(pos[None]), dtype=torch.float32))
+        rk, rv = o.rows_of(p.vals, p.exps, p.tables[r], pos)
+        np.testing.assert_array_equal(gv, rv)
+        # a K value whose fp32 rotation is off in its last bits may round to the next e4m3 value: one step, rarely
+        off = np.abs(gk - rk)
+        assert (off <= 2.0 ** -3 * np.abs(rk) + 2.0 ** -9 * 448 * np.exp2(p.exps[0, p.tables[r][pos // bs]])[..., None]).all()
+        assert (off > 0).mean() <= 1e-3
+
+
+CASES = [  # dtype, hq, hkv, d, bs, t, sequence lengths
+    ("bf16", 8, 1, 256, 16, 1, [1, 2, 15, 16, 17, 33, 127, 128, 129, 300]),
+    ("bf16", 16, 16, 256, 16, 5, [5, 6, 255, 256, 257, 1000]),
+    ("bf16", 16, 16, 64, 16, 7, [7, 100, 511, 513]),
+    ("bf16", 8, 2, 128, 16, 3, [3, 64, 65, 700]),
+    ("bf16", 8, 8, 64, 16, 1, [1, 31, 90]),
+    ("bf16", 8, 1, 256, 16, 2, [2, 40, 270]),        # 16 rows a KV head
+    ("bf16", 8, 1, 256, 16, 3, [3, 47, 200]),        # 24 rows
+    ("bf16", 8, 1, 256, 16, 40, [40, 41, 333]),      # prompt chunk: 320 rows
+    ("bf16", 4, 4, 128, 16, 65, [65, 128, 600]),
+    ("bf16", 16, 4, 64, 16, 150, [150, 407]),
+    ("bf16", 4, 2, 128, 4, 5, [5, 9, 130]),          # pages smaller than a tile
+    ("bf16", 4, 2, 64, 1, 4, [4, 21]),
+    ("bf16", 4, 2, 256, 7, 4, [4, 150]),             # pages that end inside a tile
+    ("bf16", 4, 2, 128, 24, 33, [33, 290]),
+    ("bf16", 4, 2, 64, 32, 6, [6, 95]),
+    ("bf16", 3, 1, 64, 64, 2, [2, 200]),
+    ("f32", 4, 1, 64, 16, 5, [5, 77, 200, 129]),
+    ("f32", 4, 2, 128, 4, 7, [7, 90]),
+    ("f32", 2, 2, 256, 16, 1, [1, 300]),
+]
+
+
+def _attention_inputs(case, seed, spread=2):
+    dtype, hq, hkv, d, bs, t, lens = case
+    rng = np.random.default_rng(seed)
+    b = len(lens)
+    p = Pool(rng, b, bs, hkv, d, cols=-(-max(lens) // bs))
+    n = max(lens)
+    k = rng.standard_normal((b, n, hkv, d)) * np.exp2(rng.integers(-spread, 1, (b, n, hkv, 1)))
+    v = rng.standard_normal((b, n, hkv, d)) * np.exp2(rng.integers(-4 * spread, 4 * spread, (b, n, hkv, 1)))
+    p.append(lens, k, v, lens, "bf16")
+    q = _round(rng.standard_normal((b, t, hq, d)), dtype)
+    ql = np.array([t if i % 3 != 1 else max(t - 2, 0) for i in range(b)])
+    return p, q, ql
+
+
+def _tolerance(case, q, p, lens, mass, size, ref):
+    """Error of the output, relative to what it sums up.  With A = sum_j w_j |V_j| and S the largest
+    scale * sum |q| |k| of the row:
+      scores: D products and sums in fp32, the 16-bit form of q (2^-25 of the row's largest, bf16 only) and
+              the exponential's own argument and result: ds <= (D + 8) 2^-24 S + 2^-21 + 2^-22 S, and 2^-25
+              D terms for q;  a weight's relative error is at most 2 ds, and the
+              normaliser's too, so 4 ds A in all;
+      weights as 16-bit operands (bf16 only): 2^-11 A, and below 2^-14 of the row's largest contribution an
+              absolute 2^-25 each: n 2^-25 448 of the largest w_j 2^c(j);
+      sums over n positions in fp32: (n + 64) 2^-24 A;
+      the output: half a step."""
+    dtype, hq, hkv, d, bs, t, _ = case
+    n = max(lens)
+    ds = ((d + 8) * 2.0 ** -24 + 2.0 ** -22) * size + 2.0 ** -21
+    tol = (4 * ds + (n + 64) * 2.0 ** -24) * mass + EPS[dtype] * np.abs(ref)
+    if dtype == "bf16":
+        big = np.abs(p.vals[~np.isnan(p.vals)]).max()
+        top = np.exp2(p.exps[1][p.exps[1] < 120].max().astype(np.float64)) if (p.exps[1] < 120).any() else 1.0
+        tol = tol + 2.0 ** -11 * mass + n * 2.0 ** -25 * 448 * np.minimum(top, mass.max(-1, keepdims=True) * 2)
+        tol = tol + 4 * d * 2.0 ** -25 * size / max(big, 1) * mass
+    return tol
+
+
+@pytest.mark.parametrize("case", CASES, ids=lambda c: "-".join(map(str, c[:6])))
+def test_attention_matches_the_oracle(cuda, case):
+    from ssd_b200.kernels.kv8_cache import paged_kv8_attention
+
+    torch, dts = _torch()
+    dtype, hq, hkv, d, bs, t, lens = case
+    p, q, ql = _attention_inputs(case, seed=hq * d + t + bs)
+    i = lambda a: torch.tensor(np.asarray(a, np.int32), device="cuda")  # noqa: E731
+    scale = 1 / math.sqrt(d)
+    got = paged_kv8_attention(torch.tensor(q).to(dts[dtype]).cuda(), p.cache, 1, p.dev_tables, i(lens), q_lens=i(ql))
+    ref, mass, size = o.attention(q, p.vals, p.exps, p.tables, lens, ql, scale)
+    got = got.float().cpu().numpy()
+    tol = _tolerance(case, q, p, lens, mass, size, ref)
+    bad = np.abs(got - ref) > tol
+    assert not bad.any(), (np.abs(got - ref) / np.maximum(tol, 1e-300)).max()
+    for r in range(len(lens)):
+        assert (got[r, ql[r]:] == 0).all()
+
+
+@pytest.mark.parametrize("hq,hkv,d,bs,t", [(8, 1, 256, 16, 1), (16, 16, 256, 16, 5), (4, 2, 64, 4, 6), (8, 1, 256, 16, 40)])
+def test_attention_without_positions(cuda, hq, hkv, d, bs, t):
+    """Lengths of zero, no new tokens, more new tokens than the sequence has: zero rows, nothing read."""
+    from ssd_b200.kernels.kv8_cache import paged_kv8_attention
+
+    torch, _ = _torch()
+    rng = np.random.default_rng(3)
+    p = Pool(rng, 4, bs, hkv, d, cols=-(-400 // bs))
+    lens = [0, 300, 2, 0]
+    k = _round(rng.standard_normal((4, 300, hkv, d)), "bf16")
+    p.append(lens, k, k, lens, "bf16")
+    p.dev_tables[0] = -1
+    i = lambda a: torch.tensor(np.asarray(a, np.int32), device="cuda")  # noqa: E731
+    q = _round(rng.standard_normal((4, t, hq, d)), "bf16")
+    ql = [t, 0, t, 0]
+    got = paged_kv8_attention(torch.tensor(q).bfloat16().cuda(), p.cache, 1, p.dev_tables, i(lens), q_lens=i(ql))
+    got = got.float().cpu().numpy()
+    assert (got[[0, 1, 3]] == 0).all()
+    ref, mass, _ = o.attention(q, p.vals, p.exps, p.tables, lens, ql, 1 / math.sqrt(d))
+    dead = max(0, t - 2)
+    assert (got[2, :dead] == 0).all()
+    assert (np.abs(got[2, dead:] - ref[2, dead:]) <= 2.0 ** -7 * mass[2, dead:]).all()  # 2^-8 out, 2^-11 weights, scores
+
+
+@pytest.mark.parametrize("dtype,hq,hkv,d,t", [("bf16", 4, 1, 256, 2), ("bf16", 8, 8, 64, 5), ("f32", 4, 1, 64, 3),
+                                              ("bf16", 8, 1, 128, 30)])
+def test_attention_masks_nan_of_later_tokens(cuda, dtype, hq, hkv, d, t):
+    """A new token with NaN in K and V reaches its own and later rows only, V's by dimension."""
+    from ssd_b200.kernels.kv8_cache import paged_kv8_attention
+
+    torch, dts = _torch()
+    rng = np.random.default_rng(8)
+    n = 130 + t
+    p = Pool(rng, 1, 16, hkv, d, cols=-(-n // 16))
+    k = _round(rng.standard_normal((1, n, hkv, d)), "bf16")
+    v = _round(rng.standard_normal((1, n, hkv, d)), "bf16")
+    v[0, n - 1, 0, 3] = np.nan          # the last token
+    v[0, n - 2, hkv - 1, 7] = np.inf    # the one before it, in the last head
+    p.append([n], k, v, [n], "bf16")
+    i = lambda a: torch.tensor(np.asarray(a, np.int32), device="cuda")  # noqa: E731
+    q = _round(rng.standard_normal((1, t, hq, d)), dtype)
+    got = paged_kv8_attention(torch.tensor(q).to(dts[dtype]).cuda(), p.cache, 1, p.dev_tables, i([n]))[0]
+    nan = got.isnan().cpu().numpy()
+    want = np.zeros_like(nan)
+    g = hq // hkv
+    want[t - 1, :g, 3] = True
+    want[t - 2:, (hkv - 1) * g:, 7] = True
+    np.testing.assert_array_equal(nan, want)
+    # K: a NaN score spoils the rows that see it, all of their dimensions
+    k[0, n - 1, 0, 0] = np.nan
+    p.append([n], k, np.nan_to_num(v, posinf=1.0), [n], "bf16")
+    got = paged_kv8_attention(torch.tensor(q).to(dts[dtype]).cuda(), p.cache, 1, p.dev_tables, i([n]))[0]
+    nan = got.isnan().cpu().numpy()
+    want = np.zeros_like(nan)
+    want[t - 1, :g] = True
+    np.testing.assert_array_equal(nan, want)
+
+
+def test_attention_of_pages_whose_scales_lie_far_apart(cuda):
+    """V pages at 2^-100 and 2^60, all-zero pages between: no overflow, small pages count where they are all there is."""
+    from ssd_b200.kernels.kv8_cache import paged_kv8_attention
+
+    torch, _ = _torch()
+    rng = np.random.default_rng(9)
+    p = Pool(rng, 3, 16, 1, 64, cols=20)
+    lens = [320, 320, 320]
+    k = _round(rng.standard_normal((3, 320, 1, 64)), "bf16")
+    v = rng.standard_normal((3, 320, 1, 64))
+    v[0] *= 2.0 ** -100
+    v[1, :160] *= 2.0 ** 60
+    v[2] = 0
+    p.append(lens, k, _round(v, "bf16"), lens, "bf16")
+    q = _round(rng.standard_normal((3, 2, 8, 64)), "bf16")
+    i = lambda a: torch.tensor(np.asarray(a, np.int32), device="cuda")  # noqa: E731
+    got = paged_kv8_attention(torch.tensor(q).bfloat16().cuda(), p.cache, 1, p.dev_tables, i(lens)).float().cpu().numpy()
+    ref, mass, size = o.attention(q, p.vals, p.exps, p.tables, lens, [2, 2, 2], 1 / 8)
+    assert (got[2] == 0).all()
+    # weights' 2^-11 and scores (64 + 16) 2^-24 * 4 S (S < 60) relative to the mass, the output's 2^-8
+    assert (np.abs(got - ref)[:2] <= 2.0 ** -8 * np.abs(ref[:2]) + 2.0 ** -10 * mass[:2]).all()
+
+
+@pytest.mark.parametrize("hq,hkv,d", [(16, 16, 256), (8, 1, 256), (8, 2, 128)])
+def test_attention_is_batch_invariant(cuda, hq, hkv, d):
+    """A query's bits do not depend on how many new tokens (up to the few-row kernel's rows) or sequences stand
+    beside it, nor on max_seq_len."""
+    from ssd_b200.kernels.kv8_cache import paged_kv8_attention
+
+    torch, _ = _torch()
+    rng = np.random.default_rng(12)
+    t = 5
+    p = Pool(rng, 2, 16, hkv, d, cols=64)
+    lens = [777, 400]
+    k = _round(rng.standard_normal((2, 777, hkv, d)), "bf16")
+    p.append(lens, k, 0.5 * k, lens, "bf16")
+    q = torch.tensor(_round(rng.standard_normal((2, t, hq, d)), "bf16")).bfloat16().cuda()
+    i = lambda a: torch.tensor(np.asarray(a, np.int32), device="cuda")  # noqa: E731
+    full = paged_kv8_attention(q, p.cache, 1, p.dev_tables, i(lens), max_seq_len=1024)
+    for j in range(t):
+        one = paged_kv8_attention(q[:1, j:j + 1].contiguous(), p.cache, 1, p.dev_tables[:1].contiguous(),
+                                  i([lens[0] - t + j + 1]), max_seq_len=800)
+        assert torch.equal(one[0, 0], full[0, j])
+
+
+def test_calls_on_two_streams_and_in_a_graph(cuda):
+    """Two streams at once, and a captured step (append, attention) replayed while eager calls run."""
+    from ssd_b200.kernels.kv8_cache import append_kv8, paged_kv8_attention
+
+    torch, _ = _torch()
+    rng = np.random.default_rng(4)
+    b, hq, hkv, d, n = 4, 8, 2, 128, 2000
+    p = Pool(rng, b, 16, hkv, d, cols=n // 16 + 1)
+    k = _round(rng.standard_normal((b, n, hkv, d)), "bf16")
+    p.append([n] * b, k, k, [n] * b, "bf16")
+    sl = torch.full((b,), n, dtype=torch.int32, device="cuda")
+    qs = [torch.randn((b, 3, hq, d), device="cuda").bfloat16() for _ in range(2)]
+    want = [paged_kv8_attention(x, p.cache, 1, p.dev_tables, sl) for x in qs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    outs = [[], []]
+    for _ in range(10):
+        for s, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                outs[s].append(paged_kv8_attention(qs[s], p.cache, 1, p.dev_tables, sl))
+    torch.cuda.synchronize()
+    for s in range(2):
+        assert all(torch.equal(x, want[s]) for x in outs[s])
+    kk = torch.randn((b, 1, hkv, d), device="cuda").bfloat16()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        append_kv8(p.cache, 1, p.dev_tables, sl, kk, kk)
+        cap = paged_kv8_attention(qs[0], p.cache, 1, p.dev_tables, sl)
+    kk.normal_()
+    graph.replay()
+    torch.cuda.synchronize()
+    got = cap.clone()
+    append_kv8(p.cache, 1, p.dev_tables, sl, kk, kk)
+    assert torch.equal(got, paged_kv8_attention(qs[0], p.cache, 1, p.dev_tables, sl))
+    # a larger eager call in between leaves the captured call's memory alone
+    big = paged_kv8_attention(torch.randn((b, 40, hq, d), device="cuda").bfloat16(), p.cache, 1, p.dev_tables, sl)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(cap, got) and big.isfinite().all()
+
+
+def test_strided_rows_and_refusals(cuda):
+    from ssd_b200.kernels.kv8_cache import KV8CacheState, append_kv8, gather_kv8, paged_kv8_attention
+
+    torch, _ = _torch()
+    cache = KV8CacheState.allocate(1, 8, 16, 2, 64)
+    tab = torch.arange(8, dtype=torch.int32, device="cuda").view(1, 8)
+    sl = torch.tensor([20], dtype=torch.int32, device="cuda")
+    qkv = torch.randn((1, 20, 8, 64), device="cuda").bfloat16()
+    append_kv8(cache, 0, tab, sl, qkv[:, :, 4:6], qkv[:, :, 6:8])  # views into wider rows
+    other = KV8CacheState.allocate(1, 8, 16, 2, 64)
+    append_kv8(other, 0, tab, sl, qkv[:, :, 4:6].contiguous(), qkv[:, :, 6:8].contiguous())
+    assert torch.equal(cache.pages.view(torch.uint8), other.pages.view(torch.uint8))
+    odd = torch.empty(1 * 1 * 4 * 64 + 1, device="cuda", dtype=torch.bfloat16)[1:].view(1, 1, 4, 64)
+    odd.copy_(qkv[:, 19:, :4])
+    assert torch.equal(paged_kv8_attention(odd, cache, 0, tab, sl),
+                       paged_kv8_attention(odd.clone(), cache, 0, tab, sl))
+    pos = torch.arange(20, dtype=torch.int32, device="cuda")[None]
+    k, _ = gather_kv8(cache, 0, tab, pos, dtype=torch.float32)
+    x = qkv[:, :, 4:6].float()
+    assert ((k - x).abs() <= 2.0 ** -4 * x.abs() + cache.scales.max() * 2.0 ** -10).all()  # one e4m3 rounding
+    q = qkv[:, 19:, :4].contiguous()
+    for bad in (lambda: append_kv8(cache, 0, tab, sl.long(), x, x),
+                lambda: append_kv8(cache, 0, tab[:, ::2], sl, x, x),
+                lambda: append_kv8(cache, 0, tab, sl, x[:, :, :1], x[:, :, :1]),
+                lambda: append_kv8(cache, 0, tab, sl, x.cpu(), x.cpu()),
+                lambda: append_kv8(cache, 0, tab, sl, x, x.bfloat16()),
+                lambda: append_kv8(KV8CacheState(cache.pages, cache.scales[:, :, :4], 16), 0, tab, sl, x, x),
+                lambda: append_kv8(KV8CacheState(cache.pages, cache.scales, 8), 0, tab, sl, x, x),
+                lambda: paged_kv8_attention(q[..., :32], cache, 0, tab, sl),
+                lambda: paged_kv8_attention(q, cache, 0, tab, sl.cpu()),
+                lambda: paged_kv8_attention(q, cache, 0, tab, sl, out=q.float())):
+        with pytest.raises(ValueError):
+            bad()
+    from ssd_b200._lib import SSDError
+
+    with pytest.raises(SSDError):
+        append_kv8(cache, 1, tab, sl, x, x)  # no such layer
+    with pytest.raises(SSDError):
+        paged_kv8_attention(q.half(), cache, 0, tab, sl)
+    with pytest.raises(SSDError):
+        paged_kv8_attention(q, cache, 0, tab, sl, max_seq_len=1000)  # more than the table holds
