@@ -12,6 +12,8 @@
 // workspace holds nothing between calls and may come uninitialised from any allocator.
 #include <float.h>
 
+#include <atomic>
+
 #include "kv8.cuh"
 
 namespace ssd {
@@ -26,7 +28,7 @@ struct Kv8Attn {
   const int32_t* seq_lens;
   const int32_t* q_lens;
   float scale;
-  int T, hq, G, row_groups, nsplit;
+  int T, hq, G, row_groups, nsplit, split;  // split: positions of one
   float* ws_o;          // [group][split][rows][D]
   float4* ws_ml;        // [group][split][rows]: maximum that o is relative to, that l is relative to, l
 };
@@ -36,7 +38,7 @@ __device__ __forceinline__ int splits_of(int seq, int split) { return max(1, (se
 
 // out = sum_s e^(m_s - M) o_s / sum_s e^(n_s - N) l_s * e^(M - N), M and N the largest m_s and n_s; one warp per
 // query row, lanes over the head dims.  LOG2: the maxima are in powers of two.
-template <typename T, int D, int R, int SPLIT, bool LOG2>
+template <typename T, int D, int R, bool LOG2>
 __global__ void __launch_bounds__(128) kv8_join_kernel(const Kv8Attn a, int64_t rows) {
   constexpr int DPL = D / 32;
   pdl_wait();
@@ -51,9 +53,9 @@ __global__ void __launch_bounds__(128) kv8_join_kernel(const Kv8Attn a, int64_t 
   const int gr = rg * R + r, t = gr / a.G, g = gr % a.G;
   if (t >= a.T) return;
   const int seq_full = a.seq_lens[b];
-  const int seq = min(min(seq_full, a.max_blocks * a.c.block_size), a.nsplit * SPLIT);
+  const int seq = min(min(seq_full, a.max_blocks * a.c.block_size), a.nsplit * a.split);
   const int ql = a.q_lens ? min(max(a.q_lens[b], 0), a.T) : a.T;
-  const int ns = splits_of(seq, SPLIT);
+  const int ns = splits_of(seq, a.split);
   auto ex = [](float v) { return LOG2 ? exp2f(v) : expf(v); };
   const float4* ml = a.ws_ml + grp * a.nsplit * R + r;
   float M = -INFINITY, N = -INFINITY;
@@ -92,10 +94,10 @@ __global__ void __launch_bounds__(128) kv8_join_kernel(const Kv8Attn a, int64_t 
   for (int i = 0; i < DPL; ++i) out[i * 32] = from_f<T>(o[i]);
 }
 
-template <typename T, int D, int R, int SPLIT, bool LOG2>
+template <typename T, int D, int R, bool LOG2>
 int launch_join(cudaStream_t st, const Kv8Attn& a, int B) {
   const int64_t rows = (int64_t)B * a.c.hkv * a.row_groups * R;
-  SSD_PDL((kv8_join_kernel<T, D, R, SPLIT, LOG2>), (unsigned)((rows + 3) / 4), 128, 0, st, a, rows);
+  SSD_PDL((kv8_join_kernel<T, D, R, LOG2>), (unsigned)((rows + 3) / 4), 128, 0, st, a, rows);
   return SSD_OK;
 }
 
@@ -222,22 +224,427 @@ __global__ void __launch_bounds__(kCcWarps * 32) kv8_attention_cc_kernel(const K
   }
 }
 
+
+// ------------------------------------------------------------------ few query rows (bf16): decode and verify
+// Bound by HBM: every K and V byte of the context is read once for up to 8 NT rows.  The transposed products
+//   S^T = K Q^T   and   O^T = V^T P^T   (m16n8k16, f16 operands, fp32 sums)
+// put the 16 positions of a tile and 16 head dims on the instruction's long side and the query rows on its
+// short one, so few rows waste little.  A warp takes whole tiles of 16 positions from global memory into
+// registers and needs no shared memory for them: the order of the summed-over index is free, so a lane's
+// operands are pieces of the 16 contiguous bytes it loads.
+//   K: lane (g, t) = (lane / 4, lane % 4) holds positions g and g + 8, dims 64 c + 16 t .. + 15; the word j of
+//      them is the A operand of step 4 c + j.  Q's registers follow the same order.
+//   V: positions 2t, 2t+1, 2t+8, 2t+9, dims 128 h + 16 g .. + 15 (D = 64: 8 g .. + 7); byte pairs of two
+//      positions become the A operand, m-tile i carrying dims 2i and 2i + 1 of each lane.
+//   P: the S^T accumulators, rounded to f16 pairs and transposed by movmatrix, are the B operand.
+// e4m3 converts to f16 exactly.  q is scaled per row by a power of two into f16's range, which keeps bf16's
+// eight bits (elements below 2^-14 of the row's largest lose the last ones).  V's page scales join the
+// weights' exponents: with M = max_j (s_j + c_j) (log2) every weight 2^(s_j + c_j - M) is at most 1 and
+// keeps f16's 11 bits relative to the largest contribution, whatever the pages' scales.
+// The next tile's K loads are in flight while this tile's V is used, and V's while S is computed.
+constexpr int kFewWarps = 4;
+
+__device__ __forceinline__ void mma_f16(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+  return r;
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+// Bytes of w that are e4m3 NaN (0x7f, 0xff), as 0x80 marks.
+__device__ __forceinline__ uint32_t nan_marks(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
+__device__ __forceinline__ uint32_t clear_nan(uint32_t w) { return w & ~((nan_marks(w) >> 7) * 0xffu); }
+
+template <int D, int NT>
+struct FewSmem {
+  static constexpr int PITCH = D + D / 8 + 4;  // floats of a row of the join: 16 dims then 2 of padding
+  static constexpr size_t os = sizeof(float) * kFewWarps * 8 * PITCH;
+  static constexpr size_t qs = NT > 1 ? sizeof(uint2) * NT * (D / 16) * 32 : 0;  // Q operands, in lane order
+  static size_t total(int split) { return os + qs + (size_t)split * 12; }
+};
+
+template <int D, int NT>
+__global__ void __launch_bounds__(kFewWarps * 32, 2) kv8_attention_few_kernel(const Kv8Attn a) {
+  constexpr int CK = D / 64;
+  constexpr int HV = D >= 128 ? D / 128 : 1;
+  constexpr int VW = D >= 128 ? 4 : 2;  // 32-bit words of V a lane takes per position
+  constexpr int MT = 2 * VW;            // m-tiles of one V half
+  constexpr int R = 8 * NT;
+  using S = FewSmem<D, NT>;
+  extern __shared__ __align__(16) unsigned char smem[];
+  float* os = reinterpret_cast<float*>(smem);
+  uint2* qsm = reinterpret_cast<uint2*>(smem + S::os);
+  int* row_s = reinterpret_cast<int*>(smem + S::os + S::qs);
+  float* ks_s = reinterpret_cast<float*>(row_s + a.split);
+  float* ve_s = ks_s + a.split;
+  __shared__ float4 ml_s[kFewWarps][R];
+  __shared__ int nan_seen;
+
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int g = lane >> 2, t4 = lane & 3;
+  const int split = blockIdx.x, b = blockIdx.z;
+  const int head = blockIdx.y / a.row_groups, rg = blockIdx.y % a.row_groups;
+  const int row0 = rg * R;
+  pdl_wait();
+  const int seq_full = ld_act(a.seq_lens + b);
+  const int ql = a.q_lens ? min(max(ld_act(a.q_lens + b), 0), a.T) : a.T;
+  const int seq = min(min(seq_full, a.max_blocks * a.c.block_size), a.nsplit * a.split);
+  const int base = split * a.split;
+  if (split > 0 && base >= seq) return;
+  const int kn = min(max(seq - base, 0), a.split);  // positions of this split that exist
+  const int total_rows = a.G * a.T;
+
+  // ---- where each position's rows lie, and its scales
+  {
+    const int32_t* table = a.tables + (int64_t)b * a.max_blocks;
+    for (int i = tid; i < ((kn + 15) & ~15); i += kFewWarps * 32) {
+      int row = -1;
+      float ks = 1.f, ve = 0.f;
+      if (i < kn) {
+        const int j = base + i, page = j / a.c.block_size;
+        const int blk = ld_act(table + page);
+        if ((unsigned)blk < (unsigned)a.c.num_blocks) {
+          row = blk * a.c.block_size + (j - page * a.c.block_size);
+          const float* sc = a.c.scales + a.c.scale_layer + (int64_t)blk * a.c.hkv + head;
+          ks = exp2i(scale_exponent(ld_act(sc)));
+          ve = (float)scale_exponent(ld_act(sc + a.c.scale_plane));
+        }
+      }
+      row_s[i] = row;
+      ks_s[i] = ks;
+      ve_s[i] = ve;
+    }
+    if (tid == 0) nan_seen = 0;
+  }
+
+  // ---- Q: rows 8 nt + g, scaled into f16; every warp holds all of them
+  uint2 qf[NT > 1 ? 1 : CK * 4];
+  float qscale[NT];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const int gr = row0 + 8 * nt + g, t = gr / a.G;
+    const bool real = gr < total_rows && t < ql;
+    const bf16* src = reinterpret_cast<const bf16*>(a.q) +
+                      (((int64_t)b * a.T + t) * a.hq + head * a.G + (gr - t * a.G)) * D + 16 * t4;
+    uint4 w[CK][2];
+    float amax = 0.f;
+#pragma unroll
+    for (int c = 0; c < CK; ++c) {
+      w[c][0] = w[c][1] = make_uint4(0, 0, 0, 0);
+      if (real) {
+        w[c][0] = ld_act_v4(src + 64 * c);
+        w[c][1] = ld_act_v4(src + 64 * c + 8);
+      }
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        float f[8];
+        unpack8(w[c][k], f);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) amax = fmaxf(amax, finite_abs(f[j]));
+      }
+    }
+    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+    const int e = min(max((int)(__float_as_uint(amax) >> 23) - 127, -118), 120);
+    const float inv = exp2i(-e);
+    qscale[nt] = exp2i(e) * a.scale * 1.4426950408889634f;
+#pragma unroll
+    for (int c = 0; c < CK; ++c)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        float f[8];
+        unpack8(w[c][k], f);
+        const uint2 lo = make_uint2(pack_f16(f[0] * inv, f[1] * inv), pack_f16(f[2] * inv, f[3] * inv));
+        const uint2 hi = make_uint2(pack_f16(f[4] * inv, f[5] * inv), pack_f16(f[6] * inv, f[7] * inv));
+        if constexpr (NT == 1) {
+          qf[4 * c + 2 * k] = lo;
+          qf[4 * c + 2 * k + 1] = hi;
+        } else if (warp == nt) {
+          qsm[(nt * CK * 4 + 4 * c + 2 * k) * 32 + lane] = lo;
+          qsm[(nt * CK * 4 + 4 * c + 2 * k + 1) * 32 + lane] = hi;
+        }
+      }
+  }
+  // this lane's columns: rows 8 nt + 2 t4 + {0, 1}
+  float qs[NT][2];
+  int pos[NT][2];
+  int kmin = 0x7fffffff;  // the last position that every real row of the group sees
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      qs[nt][e] = __shfl_sync(0xffffffffu, qscale[nt], (2 * t4 + e) * 4);
+      const int gr = row0 + 8 * nt + 2 * t4 + e, t = gr / a.G;
+      pos[nt][e] = (gr < total_rows && t < ql) ? seq_full - ql + t : -1;
+      if (pos[nt][e] >= 0) kmin = min(kmin, pos[nt][e]);
+    }
+  kmin = min(kmin, __shfl_xor_sync(0xffffffffu, kmin, 1));
+  kmin = min(kmin, __shfl_xor_sync(0xffffffffu, kmin, 2));
+  __syncthreads();
+
+  const uint8_t* kp = a.c.pages + a.c.layer + (int64_t)head * D + 16 * t4;
+  const uint8_t* vp = a.c.pages + a.c.plane + a.c.layer + (int64_t)head * D + (D >= 128 ? 16 : 8) * g;
+  const int64_t rs = (int64_t)a.c.hkv * D;
+  float M[NT][2], N[NT][2], l[NT][2], o[NT][HV * MT][4];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      M[nt][e] = N[nt][e] = -INFINITY;
+      l[nt][e] = 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < HV * MT; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[nt][i][e] = 0.f;
+  }
+  uint4 kr[CK][2];
+  auto load_k = [&](int i0) {
+    const uint8_t* p0 = kp + max(row_s[i0 + g], 0) * rs;
+    const uint8_t* p1 = kp + max(row_s[i0 + g + 8], 0) * rs;
+#pragma unroll
+    for (int c = 0; c < CK; ++c) {
+      kr[c][0] = ld_act_v4(p0 + 64 * c);
+      kr[c][1] = ld_act_v4(p1 + 64 * c);
+    }
+  };
+  int i0 = warp * 16;
+  if (i0 < kn) load_k(i0);
+  for (; i0 < kn; i0 += kFewWarps * 16) {
+    // ---- V of this tile
+    uint32_t vr[HV][4][VW];
+    int vrow[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      vrow[k] = row_s[i0 + 2 * t4 + (k & 1) + 8 * (k >> 1)];
+      const uint8_t* p = vp + max(vrow[k], 0) * rs;
+#pragma unroll
+      for (int h = 0; h < HV; ++h) {
+        if constexpr (VW == 4) {
+          const uint4 w = ld_act_v4(p + 128 * h);
+          vr[h][k][0] = w.x; vr[h][k][1] = w.y; vr[h][k][2] = w.z; vr[h][k][3] = w.w;
+        } else {
+          const uint2 w = __ldcg(reinterpret_cast<const uint2*>(p));
+          vr[h][k][0] = w.x; vr[h][k][1] = w.y;
+        }
+      }
+    }
+    // ---- S^T = K Q^T
+    float s[NT][4];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[nt][e] = 0.f;
+#pragma unroll
+    for (int c = 0; c < CK; ++c) {
+      const uint32_t w0[4] = {kr[c][0].x, kr[c][0].y, kr[c][0].z, kr[c][0].w};
+      const uint32_t w1[4] = {kr[c][1].x, kr[c][1].y, kr[c][1].z, kr[c][1].w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t a0 = f16x2_of(w0[j] & 0xffffu), a2 = f16x2_of(w0[j] >> 16);
+        const uint32_t a1 = f16x2_of(w1[j] & 0xffffu), a3 = f16x2_of(w1[j] >> 16);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          uint2 q;
+          if constexpr (NT == 1) q = qf[4 * c + j];
+          else q = qsm[(nt * CK * 4 + 4 * c + j) * 32 + lane];
+          mma_f16(s[nt], a0, a1, a2, a3, q.x, q.y);
+        }
+      }
+    }
+    // ---- next tile's K
+    if (i0 + kFewWarps * 16 < kn) load_k(i0 + kFewWarps * 16);
+    // ---- running maxima and weights
+    const int at0 = row_s[i0 + g] >= 0 ? base + i0 + g : 0x7fffffff;
+    const int at1 = row_s[i0 + g + 8] >= 0 ? base + i0 + g + 8 : 0x7fffffff;
+    const float k0 = ks_s[i0 + g], k1 = ks_s[i0 + g + 8], e0 = ve_s[i0 + g], e1 = ve_s[i0 + g + 8];
+    uint32_t pb[NT][2];
+    bool moved = false;
+    float f[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      float w[4];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const bool see0 = at0 <= pos[nt][e], see1 = at1 <= pos[nt][e];
+        const float s0 = s[nt][e] * (qs[nt][e] * k0), s1 = s[nt][2 + e] * (qs[nt][e] * k1);
+        // a NaN score counts as the lowest value here and spoils the sums below
+        float m = -INFINITY, n = -INFINITY;
+        if (see0) { n = fmaxf(s0, -1e38f); m = n + e0; }
+        if (see1) { const float x = fmaxf(s1, -1e38f); n = fmaxf(n, x); m = fmaxf(m, x + e1); }
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) {
+          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
+          n = fmaxf(n, __shfl_xor_sync(0xffffffffu, n, x));
+        }
+        m = fmaxf(m, M[nt][e]);
+        n = fmaxf(n, N[nt][e]);
+        moved |= m > M[nt][e];
+        f[nt][e] = m > M[nt][e] ? exp2f(M[nt][e] - m) : 1.f;
+        l[nt][e] *= n > N[nt][e] ? exp2f(N[nt][e] - n) : 1.f;
+        M[nt][e] = m;
+        N[nt][e] = n;
+        w[e] = see0 ? exp2f(s0 + e0 - m) : 0.f;
+        w[2 + e] = see1 ? exp2f(s1 + e1 - m) : 0.f;
+        if (see0) l[nt][e] += exp2f(s0 - n);
+        if (see1) l[nt][e] += exp2f(s1 - n);
+      }
+      pb[nt][0] = transpose8x8(pack_f16(w[0], w[1]));
+      pb[nt][1] = transpose8x8(pack_f16(w[2], w[3]));
+    }
+    if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int i = 0; i < HV * MT; ++i) {
+          o[nt][i][0] *= f[nt][0];
+          o[nt][i][1] *= f[nt][1];
+          o[nt][i][2] *= f[nt][0];
+          o[nt][i][3] *= f[nt][1];
+        }
+    }
+    // ---- V rows that are not there are zeros (their weights are, but their bytes may be NaN); NaN of
+    // positions that some row does not see are taken out here and put back by row below
+    const bool edge = base + i0 + 15 > kmin;
+    if (edge || __any_sync(0xffffffffu, (vrow[0] | vrow[1] | vrow[2] | vrow[3]) < 0)) {
+      uint32_t marks = 0;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const bool later = base + i0 + 2 * t4 + (k & 1) + 8 * (k >> 1) > kmin;
+#pragma unroll
+        for (int h = 0; h < HV; ++h)
+#pragma unroll
+          for (int x = 0; x < VW; ++x) {
+            uint32_t w = vrow[k] < 0 ? 0u : vr[h][k][x];
+            if (later) {
+              marks |= nan_marks(w);
+              w = clear_nan(w);
+            }
+            vr[h][k][x] = w;
+          }
+      }
+      if (marks) nan_seen = 1;
+    }
+    // ---- O^T += V^T P^T
+#pragma unroll
+    for (int h = 0; h < HV; ++h)
+#pragma unroll
+      for (int x = 0; x < VW; ++x)
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          const uint32_t sel = y ? 0x7362u : 0x5140u;
+          const uint32_t p0 = __byte_perm(vr[h][0][x], vr[h][1][x], sel);
+          const uint32_t p1 = __byte_perm(vr[h][2][x], vr[h][3][x], sel);
+          const uint32_t a0 = f16x2_of(p0 & 0xffffu), a1 = f16x2_of(p0 >> 16);
+          const uint32_t a2 = f16x2_of(p1 & 0xffffu), a3 = f16x2_of(p1 >> 16);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) mma_f16(o[nt][h * MT + 2 * x + y], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
+        }
+  }
+  pdl_trigger();
+
+  // ---- join the warps, in warp order
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      float x = l[nt][e];
+#pragma unroll
+      for (int m = 4; m < 32; m <<= 1) x += __shfl_xor_sync(0xffffffffu, x, m);
+      if (g == 0) ml_s[warp][8 * nt + 2 * t4 + e] = make_float4(M[nt][e], N[nt][e], x, 0.f);
+    }
+  __syncthreads();
+  const int64_t grp = ((int64_t)b * a.c.hkv + head) * a.row_groups + rg;
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    float f[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int r = 8 * nt + 2 * t4 + e;
+      float m = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < kFewWarps; ++w) m = fmaxf(m, ml_s[w][r].x);
+      f[e] = M[nt][e] == -INFINITY ? 0.f : exp2f(M[nt][e] - m);
+    }
+    float* ow = os + (warp * 8 + 2 * t4) * S::PITCH;
+#pragma unroll
+    for (int h = 0; h < HV; ++h)
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        const float* c = o[nt][h * MT + i];
+        const int d = (D >= 128 ? 128 * h + 16 * g : 8 * g) + 2 * i;
+        const int at = d + (d >> 4) * 2;
+        *reinterpret_cast<float2*>(ow + at) = make_float2(c[0] * f[0], c[2] * f[0]);
+        *reinterpret_cast<float2*>(ow + S::PITCH + at) = make_float2(c[1] * f[1], c[3] * f[1]);
+      }
+    __syncthreads();
+    for (int i = tid; i < 8 * D; i += kFewWarps * 32) {
+      const int r = i / D, d = i % D, at = d + (d >> 4) * 2;
+      const int gr = row0 + 8 * nt + r;
+      if (gr >= total_rows) continue;
+      float m = -INFINITY, n = -INFINITY, L = 0.f, O = 0.f;
+#pragma unroll
+      for (int w = 0; w < kFewWarps; ++w) {
+        m = fmaxf(m, ml_s[w][8 * nt + r].x);
+        n = fmaxf(n, ml_s[w][8 * nt + r].y);
+        O += os[(w * 8 + r) * S::PITCH + at];
+      }
+#pragma unroll
+      for (int w = 0; w < kFewWarps; ++w)
+        if (ml_s[w][8 * nt + r].y != -INFINITY) L += ml_s[w][8 * nt + r].z * exp2f(ml_s[w][8 * nt + r].y - n);
+      const int t = gr / a.G;
+      const int p = t < ql ? seq_full - ql + t : -1;
+      if (nan_seen) {  // rare: a position past kmin holds NaN in V
+        for (int j = max(kmin + 1, base); j <= min(p, base + kn - 1); ++j) {
+          const int row = row_s[j - base];
+          if (row >= 0 && (__ldcg(a.c.pages + a.c.plane + a.c.layer + row * rs + (int64_t)head * D + d) & 0x7f) == 0x7f)
+            O = __int_as_float(0x7fc00000);
+        }
+      }
+      if (a.nsplit == 1) {
+        reinterpret_cast<bf16*>(a.out)[(((int64_t)b * a.T + t) * a.hq + head * a.G + (gr - t * a.G)) * D + d] =
+            __float2bfloat16_rn(p >= 0 && L != 0.f ? O / L * exp2f(m - n) : 0.f);
+      } else {
+        a.ws_o[((grp * a.nsplit + split) * R + 8 * nt + r) * D + d] = O;
+        if (d == 0) a.ws_ml[(grp * a.nsplit + split) * R + 8 * nt + r] = make_float4(m, n, L, 0.f);
+      }
+    }
+    __syncthreads();
+  }
+}
+
 struct Kv8Layout {
+  bool cc;              // CUDA-core kernel (fp32)
+  int rows;             // query rows of a group
+  int split;            // positions of a split
   int row_groups, nsplit;
   size_t groups, off_o, off_ml, total;
 };
 
 inline size_t up256(size_t x) { return (x + 255) & ~size_t(255); }
 
-Kv8Layout kv8_layout(int B, int T, int hq, int hkv, int D, int max_seq_len) {
+Kv8Layout kv8_layout(bool cc, int B, int T, int hq, int hkv, int D, int max_seq_len) {
   Kv8Layout L;
-  L.row_groups = (int)(((int64_t)(hq / hkv) * T + kCcRows - 1) / kCcRows);
-  L.nsplit = (max_seq_len + kCcSplit - 1) / kCcSplit;
+  const int64_t total = (int64_t)(hq / hkv) * T;
+  L.cc = cc;
+  L.rows = cc ? kCcRows : total > 8 ? 16 : 8;
+  L.split = cc ? kCcSplit : 256;
+  L.row_groups = (int)((total + L.rows - 1) / L.rows);
+  L.nsplit = (max_seq_len + L.split - 1) / L.split;
   L.groups = (size_t)B * hkv * L.row_groups;
-  const size_t rows = L.groups * L.nsplit * kCcRows;
+  const size_t rows = L.nsplit == 1 ? 0 : L.groups * L.nsplit * L.rows;
   L.off_o = 0;
   L.off_ml = L.off_o + up256(sizeof(float) * rows * D);
-  L.total = L.off_ml + up256(sizeof(float4) * rows);
+  L.total = L.off_ml + up256(sizeof(float4) * rows) + 256;
   return L;
 }
 
@@ -245,7 +652,39 @@ template <typename T, int D>
 int launch_cc(cudaStream_t st, const Kv8Attn& a, int B) {
   const dim3 grid(a.nsplit, a.c.hkv * a.row_groups, B);
   SSD_PDL((kv8_attention_cc_kernel<T, D>), grid, kCcWarps * 32, 0, st, a);
-  return a.nsplit == 1 ? SSD_OK : launch_join<T, D, kCcRows, kCcSplit, false>(st, a, B);
+  return a.nsplit == 1 ? SSD_OK : launch_join<T, D, kCcRows, false>(st, a, B);
+}
+
+// A kernel's dynamic shared memory limit belongs to each device's context: raised once per device (`ready`: one
+// bit a device), always to the same size.
+template <typename K>
+bool allow_smem(std::atomic<uint64_t>& ready, K kern, int bytes) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return false;
+  if (ready.load(std::memory_order_acquire) >> dev & 1) return true;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) {
+    (void)cudaGetLastError();
+    return false;
+  }
+  ready.fetch_or(1ull << dev, std::memory_order_release);
+  return true;
+}
+
+template <int D, int NT>
+int launch_few(cudaStream_t st, const Kv8Attn& a, int B) {
+  const size_t smem = FewSmem<D, NT>::total(a.split);
+  const dim3 grid(a.nsplit, a.c.hkv * a.row_groups, B);
+  static_assert(FewSmem<D, NT>::os + FewSmem<D, NT>::qs + 256 * 12 + 2048 <= 227 * 1024);
+  auto kern = kv8_attention_few_kernel<D, NT>;
+  static std::atomic<uint64_t> ready{0};
+  if (!allow_smem(ready, kern, (int)smem)) return SSD_ERR_LAUNCH;
+  SSD_PDL(kern, grid, kFewWarps * 32, smem, st, a);
+  return a.nsplit == 1 ? SSD_OK : launch_join<bf16, D, 8 * NT, true>(st, a, B);
+}
+
+template <int D>
+int launch_bf16(cudaStream_t st, const Kv8Attn& a, const Kv8Layout& L, int B) {
+  return L.rows == 8 ? launch_few<D, 1>(st, a, B) : launch_few<D, 2>(st, a, B);
 }
 
 }  // namespace
@@ -258,7 +697,9 @@ extern "C" size_t ssd_kv8_attention_workspace_size(int B, int T, int num_heads, 
   if (B <= 0 || T <= 0 || num_kv_heads <= 0 || num_heads <= 0 || num_heads % num_kv_heads || head_dim <= 0 ||
       max_seq_len <= 0)
     return 0;
-  return kv8_layout(B, T, num_heads, num_kv_heads, head_dim, max_seq_len).total;
+  const size_t a = kv8_layout(true, B, T, num_heads, num_kv_heads, head_dim, max_seq_len).total;
+  const size_t b = kv8_layout(false, B, T, num_heads, num_kv_heads, head_dim, max_seq_len).total;
+  return a > b ? a : b;
 }
 
 extern "C" int ssd_kv8_attention(ssd_stream_t stream, const void* q, const void* pages, const float* scales,
@@ -274,7 +715,7 @@ extern "C" int ssd_kv8_attention(ssd_stream_t stream, const void* q, const void*
   if (!q || !out || (int64_t)max_blocks * block_size < max_seq_len) return SSD_ERR_INVALID;
   if (!kv8_aligned(q) || !kv8_aligned(out) || (int64_t)max_blocks * block_size > 0x7fffffff)
     return SSD_ERR_UNSUPPORTED;
-  const Kv8Layout L = kv8_layout(B, T, num_heads, num_kv_heads, head_dim, max_seq_len);
+  const Kv8Layout L = kv8_layout(dtype == SSD_DTYPE_F32, B, T, num_heads, num_kv_heads, head_dim, max_seq_len);
   if (B > 65535 || (int64_t)num_kv_heads * L.row_groups > 65535)
     return SSD_ERR_UNSUPPORTED;
   if (!workspace || workspace_bytes < L.total) return SSD_ERR_WORKSPACE;
@@ -294,13 +735,14 @@ extern "C" int ssd_kv8_attention(ssd_stream_t stream, const void* q, const void*
   a.G = num_heads / num_kv_heads;
   a.row_groups = L.row_groups;
   a.nsplit = L.nsplit;
+  a.split = L.split;
   a.ws_o = reinterpret_cast<float*>(w + L.off_o);
   a.ws_ml = reinterpret_cast<float4*>(w + L.off_ml);
   cudaStream_t st = (cudaStream_t)stream;
   if (dtype == SSD_DTYPE_BF16) {
-    if (head_dim == 256) return launch_cc<bf16, 256>(st, a, B);
-    if (head_dim == 128) return launch_cc<bf16, 128>(st, a, B);
-    return launch_cc<bf16, 64>(st, a, B);
+    if (head_dim == 256) return launch_bf16<256>(st, a, L, B);
+    if (head_dim == 128) return launch_bf16<128>(st, a, L, B);
+    return launch_bf16<64>(st, a, L, B);
   }
   if (head_dim == 256) return launch_cc<float, 256>(st, a, B);
   if (head_dim == 128) return launch_cc<float, 128>(st, a, B);
