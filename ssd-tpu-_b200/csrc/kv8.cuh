@@ -49,6 +49,12 @@ __device__ __forceinline__ uint32_t f16x2_of(uint32_t pair) {
   asm("{.reg .b16 p; cvt.u16.u32 p, %1; cvt.rn.f16x2.e4m3x2 %0, p;}" : "=r"(r) : "r"(pair));
   return r;
 }
+// The four e4m3 values of a word -> two f16 pairs (bytes 0, 1 and bytes 2, 3).
+__device__ __forceinline__ void f16x4_of(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  asm("{.reg .b16 a, b; mov.b32 {a, b}, %2; cvt.rn.f16x2.e4m3x2 %0, a; cvt.rn.f16x2.e4m3x2 %1, b;}"
+      : "=r"(lo), "=r"(hi)
+      : "r"(w));
+}
 __device__ __forceinline__ float2 e4m3_pair(uint32_t pair) {
   const uint32_t h = f16x2_of(pair & 0xffffu);
   return __half22float2(*reinterpret_cast<const __half2*>(&h));

@@ -13,6 +13,7 @@
 #include <float.h>
 
 #include <atomic>
+#include <cstdlib>
 
 #include "kv8.cuh"
 
@@ -229,19 +230,18 @@ __global__ void __launch_bounds__(kCcWarps * 32) kv8_attention_cc_kernel(const K
 // Bound by HBM: every K and V byte of the context is read once for up to 8 NT rows.  The transposed products
 //   S^T = K Q^T   and   O^T = V^T P^T   (m16n8k16, f16 operands, fp32 sums)
 // put the 16 positions of a tile and 16 head dims on the instruction's long side and the query rows on its
-// short one, so few rows waste little.  A warp takes whole tiles of 16 positions from global memory into
-// registers and needs no shared memory for them: the order of the summed-over index is free, so a lane's
-// operands are pieces of the 16 contiguous bytes it loads.
-//   K: lane (g, t) = (lane / 4, lane % 4) holds positions g and g + 8, dims 64 c + 16 t .. + 15; the word j of
-//      them is the A operand of step 4 c + j.  Q's registers follow the same order.
+// short one, so few rows waste little.  Each warp owns every fourth tile of 16 positions and a ring of tiles
+// in shared memory that only it fills (cp.async, zeros for rows that are not there) and reads, so the loop has
+// no barrier.  The order of the summed-over index is free, so a lane's operands are whole 16-byte pieces:
+//   K: lane (g, t) = (lane / 4, lane % 4) takes positions g and g + 8, dims 64 c + 16 t .. + 15; word j of a
+//      piece is the A operand of step 4 c + j.  Q's registers follow the same order.
 //   V: positions 2t, 2t+1, 2t+8, 2t+9, dims 128 h + 16 g .. + 15 (D = 64: 8 g .. + 7); byte pairs of two
 //      positions become the A operand, m-tile i carrying dims 2i and 2i + 1 of each lane.
 //   P: the S^T accumulators, rounded to f16 pairs and transposed by movmatrix, are the B operand.
 // e4m3 converts to f16 exactly.  q is scaled per row by a power of two into f16's range, which keeps bf16's
 // eight bits (elements below 2^-14 of the row's largest lose the last ones).  V's page scales join the
-// weights' exponents: with M = max_j (s_j + c_j) (log2) every weight 2^(s_j + c_j - M) is at most 1 and
+// weights' exponents: with M >= max_j (s_j + c_j) - 8 (log2) every weight 2^(s_j + c_j - M) is at most 2^8 and
 // keeps f16's 11 bits relative to the largest contribution, whatever the pages' scales.
-// The next tile's K loads are in flight while this tile's V is used, and V's while S is computed.
 constexpr int kFewWarps = 4;
 
 __device__ __forceinline__ void mma_f16(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -264,29 +264,49 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
 __device__ __forceinline__ uint32_t nan_marks(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
 __device__ __forceinline__ uint32_t clear_nan(uint32_t w) { return w & ~((nan_marks(w) >> 7) * 0xffu); }
 
-template <int D, int NT>
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ uint4 lds128(uint32_t p) {
+  uint4 r;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "r"(p));
+  return r;
+}
+
+template <int D, int NT, bool UNI>
 struct FewSmem {
+  static constexpr int STAGES = D == 256 ? 2 : 4;
+  static constexpr int TILE = 16 * D;          // bytes of a tile's K (or V) rows
   static constexpr int PITCH = D + D / 8 + 4;  // floats of a row of the join: 16 dims then 2 of padding
-  static constexpr size_t os = sizeof(float) * kFewWarps * 8 * PITCH;
-  static constexpr size_t qs = NT > 1 ? sizeof(uint2) * NT * (D / 16) * 32 : 0;  // Q operands, in lane order
-  static size_t total(int split) { return os + qs + (size_t)split * 12; }
+  static constexpr size_t ring = (size_t)kFewWarps * STAGES * 2 * TILE;
+  static_assert(sizeof(float) * kFewWarps * 8 * PITCH <= ring, "the join reuses the rings");
+  static constexpr size_t qs = sizeof(uint2) * NT * (D / 16) * 32;  // Q operands, in lane order
+  static size_t total(int split) { return ring + qs + (size_t)(UNI ? split / 16 : split) * 12; }
 };
 
-template <int D, int NT>
-__global__ void __launch_bounds__(kFewWarps * 32, 2) kv8_attention_few_kernel(const Kv8Attn a) {
+// UNI: block_size is a multiple of 16, so a tile lies in one page and has one pair of scales.
+template <int D, int NT, bool UNI>
+__global__ void __launch_bounds__(kFewWarps * 32, NT == 1 ? 3 : 2) kv8_attention_few_kernel(const Kv8Attn a) {
   constexpr int CK = D / 64;
   constexpr int HV = D >= 128 ? D / 128 : 1;
   constexpr int VW = D >= 128 ? 4 : 2;  // 32-bit words of V a lane takes per position
   constexpr int MT = 2 * VW;            // m-tiles of one V half
   constexpr int R = 8 * NT;
-  using S = FewSmem<D, NT>;
-  extern __shared__ __align__(16) unsigned char smem[];
+  constexpr int PCS = D / 16;           // 16-byte pieces of a row
+  using S = FewSmem<D, NT, UNI>;
+  extern __shared__ __align__(128) unsigned char smem[];
   float* os = reinterpret_cast<float*>(smem);
-  uint2* qsm = reinterpret_cast<uint2*>(smem + S::os);
-  int* row_s = reinterpret_cast<int*>(smem + S::os + S::qs);
-  float* ks_s = reinterpret_cast<float*>(row_s + a.split);
-  float* ve_s = ks_s + a.split;
-  __shared__ float4 ml_s[kFewWarps][R];
+  uint2* qsm = reinterpret_cast<uint2*>(smem + S::ring);
+  // per tile (UNI) or per position: row number in the layer (-1: none), K scale, exponent of V's scale
+  int* row_s = reinterpret_cast<int*>(smem + S::ring + S::qs);
+  const int nmeta = UNI ? a.split / 16 : a.split;
+  float* ks_s = reinterpret_cast<float*>(row_s + nmeta);
+  float* ve_s = ks_s + nmeta;
+  __shared__ float4 ml_s[kFewWarps][R], fin_s[R];
+  __shared__ float qscale_s[R];
   __shared__ int nan_seen;
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -306,11 +326,13 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2) kv8_attention_few_kernel(co
   // ---- where each position's rows lie, and its scales
   {
     const int32_t* table = a.tables + (int64_t)b * a.max_blocks;
-    for (int i = tid; i < ((kn + 15) & ~15); i += kFewWarps * 32) {
+    const int n = UNI ? (kn + 15) / 16 : (kn + 15) & ~15;
+    for (int i = tid; i < n; i += kFewWarps * 32) {
       int row = -1;
       float ks = 1.f, ve = 0.f;
-      if (i < kn) {
-        const int j = base + i, page = j / a.c.block_size;
+      const int j = base + (UNI ? 16 * i : i);
+      if (j < base + kn) {
+        const int page = j / a.c.block_size;
         const int blk = ld_act(table + page);
         if ((unsigned)blk < (unsigned)a.c.num_blocks) {
           row = blk * a.c.block_size + (j - page * a.c.block_size);
@@ -326,54 +348,37 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2) kv8_attention_few_kernel(co
     if (tid == 0) nan_seen = 0;
   }
 
-  // ---- Q: rows 8 nt + g, scaled into f16; every warp holds all of them
-  uint2 qf[NT > 1 ? 1 : CK * 4];
-  float qscale[NT];
+  // ---- Q, scaled into f16, in the order of the lanes' operands: a warp takes two rows of 8 (16 lanes a row)
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
-    const int gr = row0 + 8 * nt + g, t = gr / a.G;
+    const int r = 2 * warp + (lane >> 4), gr = row0 + 8 * nt + r, t = gr / a.G;
     const bool real = gr < total_rows && t < ql;
     const bf16* src = reinterpret_cast<const bf16*>(a.q) +
-                      (((int64_t)b * a.T + t) * a.hq + head * a.G + (gr - t * a.G)) * D + 16 * t4;
-    uint4 w[CK][2];
-    float amax = 0.f;
+                      (((int64_t)b * a.T + t) * a.hq + head * a.G + (gr - t * a.G)) * D + (lane & 15) * (D / 16);
+    float f[D / 16], amax = 0.f;
 #pragma unroll
-    for (int c = 0; c < CK; ++c) {
-      w[c][0] = w[c][1] = make_uint4(0, 0, 0, 0);
-      if (real) {
-        w[c][0] = ld_act_v4(src + 64 * c);
-        w[c][1] = ld_act_v4(src + 64 * c + 8);
-      }
+    for (int k = 0; k < D / 16; k += 4) {
+      uint2 w = make_uint2(0, 0);
+      if (real) w = __ldcg(reinterpret_cast<const uint2*>(src + k));
+      const float2 x = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w.x));
+      const float2 y = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w.y));
+      f[k] = x.x; f[k + 1] = x.y; f[k + 2] = y.x; f[k + 3] = y.y;
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        float f[8];
-        unpack8(w[c][k], f);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) amax = fmaxf(amax, finite_abs(f[j]));
-      }
+      for (int j = 0; j < 4; ++j) amax = fmaxf(amax, finite_abs(f[k + j]));
     }
-    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+#pragma unroll
+    for (int x = 1; x < 16; x <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, x));
     const int e = min(max((int)(__float_as_uint(amax) >> 23) - 127, -118), 120);
     const float inv = exp2i(-e);
-    qscale[nt] = exp2i(e) * a.scale * 1.4426950408889634f;
+    if ((lane & 15) == 0) qscale_s[8 * nt + r] = exp2i(e) * a.scale * 1.4426950408889634f;
 #pragma unroll
-    for (int c = 0; c < CK; ++c)
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        float f[8];
-        unpack8(w[c][k], f);
-        const uint2 lo = make_uint2(pack_f16(f[0] * inv, f[1] * inv), pack_f16(f[2] * inv, f[3] * inv));
-        const uint2 hi = make_uint2(pack_f16(f[4] * inv, f[5] * inv), pack_f16(f[6] * inv, f[7] * inv));
-        if constexpr (NT == 1) {
-          qf[4 * c + 2 * k] = lo;
-          qf[4 * c + 2 * k + 1] = hi;
-        } else if (warp == nt) {
-          qsm[(nt * CK * 4 + 4 * c + 2 * k) * 32 + lane] = lo;
-          qsm[(nt * CK * 4 + 4 * c + 2 * k + 1) * 32 + lane] = hi;
-        }
-      }
+    for (int k = 0; k < D / 16; k += 4) {
+      const int d = (lane & 15) * (D / 16) + k, c = d >> 6, tt = (d >> 4) & 3, j = (d >> 2) & 3;
+      qsm[(nt * CK * 4 + 4 * c + j) * 32 + r * 4 + tt] =
+          make_uint2(pack_f16(f[k] * inv, f[k + 1] * inv), pack_f16(f[k + 2] * inv, f[k + 3] * inv));
+    }
   }
+  __syncthreads();
   // this lane's columns: rows 8 nt + 2 t4 + {0, 1}
   float qs[NT][2];
   int pos[NT][2];
@@ -382,17 +387,19 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2) kv8_attention_few_kernel(co
   for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      qs[nt][e] = __shfl_sync(0xffffffffu, qscale[nt], (2 * t4 + e) * 4);
+      qs[nt][e] = qscale_s[8 * nt + 2 * t4 + e];
       const int gr = row0 + 8 * nt + 2 * t4 + e, t = gr / a.G;
       pos[nt][e] = (gr < total_rows && t < ql) ? seq_full - ql + t : -1;
       if (pos[nt][e] >= 0) kmin = min(kmin, pos[nt][e]);
     }
   kmin = min(kmin, __shfl_xor_sync(0xffffffffu, kmin, 1));
   kmin = min(kmin, __shfl_xor_sync(0xffffffffu, kmin, 2));
-  __syncthreads();
+  uint2 qf[NT == 1 ? CK * 4 : 1];
+  if constexpr (NT == 1) {
+#pragma unroll
+    for (int i = 0; i < CK * 4; ++i) qf[i] = qsm[i * 32 + lane];
+  }
 
-  const uint8_t* kp = a.c.pages + a.c.layer + (int64_t)head * D + 16 * t4;
-  const uint8_t* vp = a.c.pages + a.c.plane + a.c.layer + (int64_t)head * D + (D >= 128 ? 16 : 8) * g;
   const int64_t rs = (int64_t)a.c.hkv * D;
   float M[NT][2], N[NT][2], l[NT][2], o[NT][HV * MT][4];
 #pragma unroll
@@ -407,37 +414,39 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2) kv8_attention_few_kernel(co
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[nt][i][e] = 0.f;
   }
-  uint4 kr[CK][2];
-  auto load_k = [&](int i0) {
-    const uint8_t* p0 = kp + max(row_s[i0 + g], 0) * rs;
-    const uint8_t* p1 = kp + max(row_s[i0 + g + 8], 0) * rs;
+  // the ring: piece p of row r lies at p ^ 4 (r & 1) of K's rows and p ^ (r & 6) of V's, so that a quarter warp's
+  // 16-byte reads meet no bank twice (D = 64: a line holds two rows, V's 8-byte reads meet each bank twice)
+  auto k_piece = [](int r, int p) { return r * PCS + (D >= 128 ? p ^ ((r & 1) << 2) : p); };
+  auto v_piece = [](int r, int p) { return r * PCS + (D >= 128 ? p ^ (r & 6) : p ^ (r >> 1 & 3)); };
+  const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * (S::STAGES * 2 * S::TILE);
+  const uint8_t* kp = a.c.pages + a.c.layer + (int64_t)head * D + (lane % PCS) * 16;
+  const int tiles = (kn + 15) / 16;
+  const int mine = warp < tiles ? (tiles - warp + kFewWarps - 1) / kFewWarps : 0;
+  auto issue = [&](int k) {  // this warp's k-th tile, into stage k % STAGES
+    if (k < mine) {
+      const int i0 = (warp + k * kFewWarps) * 16;
+      const uint32_t st = ring + (k % S::STAGES) * (2 * S::TILE);
+      constexpr int RPI = 32 / PCS;  // rows an instruction covers
 #pragma unroll
-    for (int c = 0; c < CK; ++c) {
-      kr[c][0] = ld_act_v4(p0 + 64 * c);
-      kr[c][1] = ld_act_v4(p1 + 64 * c);
-    }
-  };
-  int i0 = warp * 16;
-  if (i0 < kn) load_k(i0);
-  for (; i0 < kn; i0 += kFewWarps * 16) {
-    // ---- V of this tile
-    uint32_t vr[HV][4][VW];
-    int vrow[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      vrow[k] = row_s[i0 + 2 * t4 + (k & 1) + 8 * (k >> 1)];
-      const uint8_t* p = vp + max(vrow[k], 0) * rs;
-#pragma unroll
-      for (int h = 0; h < HV; ++h) {
-        if constexpr (VW == 4) {
-          const uint4 w = ld_act_v4(p + 128 * h);
-          vr[h][k][0] = w.x; vr[h][k][1] = w.y; vr[h][k][2] = w.z; vr[h][k][3] = w.w;
-        } else {
-          const uint2 w = __ldcg(reinterpret_cast<const uint2*>(p));
-          vr[h][k][0] = w.x; vr[h][k][1] = w.y;
-        }
+      for (int x = 0; x < 16 / RPI; ++x) {
+        const int r = x * RPI + lane / PCS;
+        const int first = UNI ? row_s[i0 >> 4] : row_s[i0 + r];
+        const bool there = first >= 0 && (!UNI || i0 + r < kn);
+        const uint8_t* src = kp + (there ? first + (UNI ? r : 0) : 0) * rs;
+        cp_async16(st + k_piece(r, lane % PCS) * 16, src, there);
+        cp_async16(st + S::TILE + v_piece(r, lane % PCS) * 16, src + a.c.plane, there);
       }
     }
+    cp_async_commit();
+  };
+#pragma unroll
+  for (int k = 0; k < S::STAGES - 1; ++k) issue(k);
+  for (int k = 0; k < mine; ++k) {
+    cp_async_wait<S::STAGES - 2>();
+    __syncwarp();  // every lane's copies of tile k are there, and every lane is done with tile k - 1
+    issue(k + S::STAGES - 1);
+    const int i0 = (warp + k * kFewWarps) * 16;
+    const uint32_t st = ring + (k % S::STAGES) * (2 * S::TILE);
     // ---- S^T = K Q^T
     float s[NT][4];
 #pragma unroll
@@ -446,12 +455,14 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2) kv8_attention_few_kernel(co
       for (int e = 0; e < 4; ++e) s[nt][e] = 0.f;
 #pragma unroll
     for (int c = 0; c < CK; ++c) {
-      const uint32_t w0[4] = {kr[c][0].x, kr[c][0].y, kr[c][0].z, kr[c][0].w};
-      const uint32_t w1[4] = {kr[c][1].x, kr[c][1].y, kr[c][1].z, kr[c][1].w};
+      const uint4 p0 = lds128(st + k_piece(g, 4 * c + t4) * 16), p1 = lds128(st + k_piece(g + 8, 4 * c + t4) * 16);
+      const uint32_t w0[4] = {p0.x, p0.y, p0.z, p0.w};
+      const uint32_t w1[4] = {p1.x, p1.y, p1.z, p1.w};
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const uint32_t a0 = f16x2_of(w0[j] & 0xffffu), a2 = f16x2_of(w0[j] >> 16);
-        const uint32_t a1 = f16x2_of(w1[j] & 0xffffu), a3 = f16x2_of(w1[j] >> 16);
+        uint32_t a0, a1, a2, a3;
+        f16x4_of(w0[j], a0, a2);
+        f16x4_of(w1[j], a1, a3);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           uint2 q;
@@ -461,12 +472,12 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2) kv8_attention_few_kernel(co
         }
       }
     }
-    // ---- next tile's K
-    if (i0 + kFewWarps * 16 < kn) load_k(i0 + kFewWarps * 16);
     // ---- running maxima and weights
-    const int at0 = row_s[i0 + g] >= 0 ? base + i0 + g : 0x7fffffff;
-    const int at1 = row_s[i0 + g + 8] >= 0 ? base + i0 + g + 8 : 0x7fffffff;
-    const float k0 = ks_s[i0 + g], k1 = ks_s[i0 + g + 8], e0 = ve_s[i0 + g], e1 = ve_s[i0 + g + 8];
+    const int m0 = UNI ? i0 >> 4 : i0 + g, m1 = UNI ? m0 : m0 + 8;
+    // a position without a row lies behind every query
+    const int at0 = row_s[m0] >= 0 && (!UNI || i0 + g < kn) ? base + i0 + g : 0x7fffffff;
+    const int at1 = row_s[m1] >= 0 && (!UNI || i0 + g + 8 < kn) ? base + i0 + g + 8 : 0x7fffffff;
+    const float k0 = ks_s[m0], k1 = ks_s[m1], e0 = ve_s[m0], e1 = ve_s[m1];
     uint32_t pb[NT][2];
     bool moved = false;
     float f[NT][2];
@@ -478,25 +489,31 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2) kv8_attention_few_kernel(co
         const bool see0 = at0 <= pos[nt][e], see1 = at1 <= pos[nt][e];
         const float s0 = s[nt][e] * (qs[nt][e] * k0), s1 = s[nt][2 + e] * (qs[nt][e] * k1);
         // a NaN score counts as the lowest value here and spoils the sums below
-        float m = -INFINITY, n = -INFINITY;
-        if (see0) { n = fmaxf(s0, -1e38f); m = n + e0; }
-        if (see1) { const float x = fmaxf(s1, -1e38f); n = fmaxf(n, x); m = fmaxf(m, x + e1); }
+        float n = see0 ? fmaxf(s0, -1e38f) : -INFINITY, m = n + e0;
+        const float n1 = see1 ? fmaxf(s1, -1e38f) : -INFINITY;
+        if constexpr (!UNI) m = fmaxf(m, n1 + e1);
+        n = fmaxf(n, n1);
 #pragma unroll
         for (int x = 4; x < 32; x <<= 1) {
-          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
+          if constexpr (!UNI) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
           n = fmaxf(n, __shfl_xor_sync(0xffffffffu, n, x));
         }
-        m = fmaxf(m, M[nt][e]);
-        n = fmaxf(n, N[nt][e]);
-        moved |= m > M[nt][e];
-        f[nt][e] = m > M[nt][e] ? exp2f(M[nt][e] - m) : 1.f;
-        l[nt][e] *= n > N[nt][e] ? exp2f(N[nt][e] - n) : 1.f;
-        M[nt][e] = m;
-        N[nt][e] = n;
-        w[e] = see0 ? exp2f(s0 + e0 - m) : 0.f;
-        w[2 + e] = see1 ? exp2f(s1 + e1 - m) : 0.f;
-        if (see0) l[nt][e] += exp2f(s0 - n);
-        if (see1) l[nt][e] += exp2f(s1 - n);
+        if constexpr (UNI) m = n + e0;
+        // the reference moves only when a weight would pass 2^8 (f16 holds 2^15): most tiles rescale nothing
+        f[nt][e] = 1.f;
+        if (m > M[nt][e] + 8.f) {
+          f[nt][e] = exp2f(M[nt][e] - m);
+          M[nt][e] = m;
+          moved = true;
+        }
+        if (n > N[nt][e] + 8.f) {
+          l[nt][e] *= exp2f(N[nt][e] - n);
+          N[nt][e] = n;
+        }
+        w[e] = see0 ? exp2f(s0 + e0 - M[nt][e]) : 0.f;
+        w[2 + e] = see1 ? exp2f(s1 + e1 - M[nt][e]) : 0.f;
+        if (see0) l[nt][e] += exp2f(s0 - N[nt][e]);
+        if (see1) l[nt][e] += exp2f(s1 - N[nt][e]);
       }
       pb[nt][0] = transpose8x8(pack_f16(w[0], w[1]));
       pb[nt][1] = transpose8x8(pack_f16(w[2], w[3]));
@@ -512,24 +529,33 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2) kv8_attention_few_kernel(co
           o[nt][i][3] *= f[nt][1];
         }
     }
-    // ---- V rows that are not there are zeros (their weights are, but their bytes may be NaN); NaN of
-    // positions that some row does not see are taken out here and put back by row below
-    const bool edge = base + i0 + 15 > kmin;
-    if (edge || __any_sync(0xffffffffu, (vrow[0] | vrow[1] | vrow[2] | vrow[3]) < 0)) {
+    // ---- V; NaN of positions that some row does not see are taken out here and put back by row below
+    uint32_t vr[HV][4][VW];
+#pragma unroll
+    for (int h = 0; h < HV; ++h)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const int r = 2 * t4 + (x & 1) + 8 * (x >> 1);
+        if constexpr (VW == 4) {
+          const uint4 w = lds128(st + S::TILE + v_piece(r, 8 * h + g) * 16);
+          vr[h][x][0] = w.x; vr[h][x][1] = w.y; vr[h][x][2] = w.z; vr[h][x][3] = w.w;
+        } else {
+          asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];"
+                       : "=r"(vr[h][x][0]), "=r"(vr[h][x][1])
+                       : "r"(st + S::TILE + v_piece(r, g >> 1) * 16 + (g & 1) * 8));
+        }
+      }
+    if (base + i0 + 15 > kmin) {
       uint32_t marks = 0;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const bool later = base + i0 + 2 * t4 + (k & 1) + 8 * (k >> 1) > kmin;
+      for (int x = 0; x < 4; ++x) {
+        if (base + i0 + 2 * t4 + (x & 1) + 8 * (x >> 1) <= kmin) continue;
 #pragma unroll
         for (int h = 0; h < HV; ++h)
 #pragma unroll
-          for (int x = 0; x < VW; ++x) {
-            uint32_t w = vrow[k] < 0 ? 0u : vr[h][k][x];
-            if (later) {
-              marks |= nan_marks(w);
-              w = clear_nan(w);
-            }
-            vr[h][k][x] = w;
+          for (int y = 0; y < VW; ++y) {
+            marks |= nan_marks(vr[h][x][y]);
+            vr[h][x][y] = clear_nan(vr[h][x][y]);
           }
       }
       if (marks) nan_seen = 1;
@@ -542,10 +568,9 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2) kv8_attention_few_kernel(co
 #pragma unroll
         for (int y = 0; y < 2; ++y) {
           const uint32_t sel = y ? 0x7362u : 0x5140u;
-          const uint32_t p0 = __byte_perm(vr[h][0][x], vr[h][1][x], sel);
-          const uint32_t p1 = __byte_perm(vr[h][2][x], vr[h][3][x], sel);
-          const uint32_t a0 = f16x2_of(p0 & 0xffffu), a1 = f16x2_of(p0 >> 16);
-          const uint32_t a2 = f16x2_of(p1 & 0xffffu), a3 = f16x2_of(p1 >> 16);
+          uint32_t a0, a1, a2, a3;
+          f16x4_of(__byte_perm(vr[h][0][x], vr[h][1][x], sel), a0, a1);
+          f16x4_of(__byte_perm(vr[h][2][x], vr[h][3][x], sel), a2, a3);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) mma_f16(o[nt][h * MT + 2 * x + y], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
         }
@@ -563,6 +588,18 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2) kv8_attention_few_kernel(co
       if (g == 0) ml_s[warp][8 * nt + 2 * t4 + e] = make_float4(M[nt][e], N[nt][e], x, 0.f);
     }
   __syncthreads();
+  if (tid < R) {
+    float m = -INFINITY, n = -INFINITY, L = 0.f;
+#pragma unroll
+    for (int w = 0; w < kFewWarps; ++w) {
+      m = fmaxf(m, ml_s[w][tid].x);
+      n = fmaxf(n, ml_s[w][tid].y);
+    }
+#pragma unroll
+    for (int w = 0; w < kFewWarps; ++w)
+      if (ml_s[w][tid].y != -INFINITY) L += ml_s[w][tid].z * exp2f(ml_s[w][tid].y - n);
+    fin_s[tid] = make_float4(m, n, L, 0.f);
+  }
   const int64_t grp = ((int64_t)b * a.c.hkv + head) * a.row_groups + rg;
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
@@ -587,39 +624,44 @@ __global__ void __launch_bounds__(kFewWarps * 32, 2) kv8_attention_few_kernel(co
         *reinterpret_cast<float2*>(ow + S::PITCH + at) = make_float2(c[1] * f[1], c[3] * f[1]);
       }
     __syncthreads();
-    for (int i = tid; i < 8 * D; i += kFewWarps * 32) {
-      const int r = i / D, d = i % D, at = d + (d >> 4) * 2;
+    for (int i = tid; i < 4 * D; i += kFewWarps * 32) {
+      const int r = i / (D / 2), d = i % (D / 2) * 2, at = d + (d >> 4) * 2;
       const int gr = row0 + 8 * nt + r;
       if (gr >= total_rows) continue;
-      float m = -INFINITY, n = -INFINITY, L = 0.f, O = 0.f;
+      float2 O = make_float2(0.f, 0.f);
 #pragma unroll
       for (int w = 0; w < kFewWarps; ++w) {
-        m = fmaxf(m, ml_s[w][8 * nt + r].x);
-        n = fmaxf(n, ml_s[w][8 * nt + r].y);
-        O += os[(w * 8 + r) * S::PITCH + at];
+        const float2 x = *reinterpret_cast<const float2*>(os + (w * 8 + r) * S::PITCH + at);
+        O.x += x.x;
+        O.y += x.y;
       }
-#pragma unroll
-      for (int w = 0; w < kFewWarps; ++w)
-        if (ml_s[w][8 * nt + r].y != -INFINITY) L += ml_s[w][8 * nt + r].z * exp2f(ml_s[w][8 * nt + r].y - n);
       const int t = gr / a.G;
       const int p = t < ql ? seq_full - ql + t : -1;
       if (nan_seen) {  // rare: a position past kmin holds NaN in V
         for (int j = max(kmin + 1, base); j <= min(p, base + kn - 1); ++j) {
-          const int row = row_s[j - base];
-          if (row >= 0 && (__ldcg(a.c.pages + a.c.plane + a.c.layer + row * rs + (int64_t)head * D + d) & 0x7f) == 0x7f)
-            O = __int_as_float(0x7fc00000);
+          const int first = row_s[UNI ? (j - base) >> 4 : j - base];
+          if (first < 0) continue;
+          const int64_t row = first + (UNI ? (j - base) & 15 : 0);
+          const uint32_t v = __ldcg(reinterpret_cast<const uint16_t*>(a.c.pages + a.c.plane + a.c.layer + row * rs +
+                                                                      (int64_t)head * D + d));
+          if ((v & 0x7fu) == 0x7fu) O.x = __int_as_float(0x7fc00000);
+          if ((v & 0x7f00u) == 0x7f00u) O.y = __int_as_float(0x7fc00000);
         }
       }
       if (a.nsplit == 1) {
-        reinterpret_cast<bf16*>(a.out)[(((int64_t)b * a.T + t) * a.hq + head * a.G + (gr - t * a.G)) * D + d] =
-            __float2bfloat16_rn(p >= 0 && L != 0.f ? O / L * exp2f(m - n) : 0.f);
+        const float4 z = fin_s[8 * nt + r];
+        const float k = exp2f(z.x - z.y);
+        const bool ok = p >= 0 && z.z != 0.f;
+        *reinterpret_cast<__nv_bfloat162*>(reinterpret_cast<bf16*>(a.out) +
+                                           (((int64_t)b * a.T + t) * a.hq + head * a.G + (gr - t * a.G)) * D + d) =
+            __floats2bfloat162_rn(ok ? O.x / z.z * k : 0.f, ok ? O.y / z.z * k : 0.f);
       } else {
-        a.ws_o[((grp * a.nsplit + split) * R + 8 * nt + r) * D + d] = O;
-        if (d == 0) a.ws_ml[(grp * a.nsplit + split) * R + 8 * nt + r] = make_float4(m, n, L, 0.f);
+        *reinterpret_cast<float2*>(a.ws_o + ((grp * a.nsplit + split) * R + 8 * nt + r) * D + d) = O;
       }
     }
     __syncthreads();
   }
+  if (a.nsplit > 1 && tid < R) a.ws_ml[(grp * a.nsplit + split) * R + tid] = fin_s[tid];
 }
 
 struct Kv8Layout {
@@ -637,7 +679,7 @@ Kv8Layout kv8_layout(bool cc, int B, int T, int hq, int hkv, int D, int max_seq_
   const int64_t total = (int64_t)(hq / hkv) * T;
   L.cc = cc;
   L.rows = cc ? kCcRows : total > 8 ? 16 : 8;
-  L.split = cc ? kCcSplit : 256;
+  L.split = cc ? kCcSplit : getenv("KSPLIT") ? atoi(getenv("KSPLIT")) : 256;
   L.row_groups = (int)((total + L.rows - 1) / L.rows);
   L.nsplit = (max_seq_len + L.split - 1) / L.split;
   L.groups = (size_t)B * hkv * L.row_groups;
@@ -670,21 +712,21 @@ bool allow_smem(std::atomic<uint64_t>& ready, K kern, int bytes) {
   return true;
 }
 
-template <int D, int NT>
+template <int D, int NT, bool UNI>
 int launch_few(cudaStream_t st, const Kv8Attn& a, int B) {
-  const size_t smem = FewSmem<D, NT>::total(a.split);
+  const size_t smem = FewSmem<D, NT, UNI>::total(a.split);
   const dim3 grid(a.nsplit, a.c.hkv * a.row_groups, B);
-  static_assert(FewSmem<D, NT>::os + FewSmem<D, NT>::qs + 256 * 12 + 2048 <= 227 * 1024);
-  auto kern = kv8_attention_few_kernel<D, NT>;
+  auto kern = kv8_attention_few_kernel<D, NT, UNI>;
   static std::atomic<uint64_t> ready{0};
-  if (!allow_smem(ready, kern, (int)smem)) return SSD_ERR_LAUNCH;
+  if (!allow_smem(ready, kern, (int)FewSmem<D, NT, UNI>::total(2048))) return SSD_ERR_LAUNCH;
   SSD_PDL(kern, grid, kFewWarps * 32, smem, st, a);
   return a.nsplit == 1 ? SSD_OK : launch_join<bf16, D, 8 * NT, true>(st, a, B);
 }
 
 template <int D>
 int launch_bf16(cudaStream_t st, const Kv8Attn& a, const Kv8Layout& L, int B) {
-  return L.rows == 8 ? launch_few<D, 1>(st, a, B) : launch_few<D, 2>(st, a, B);
+  if (a.c.block_size % 16 == 0) return L.rows == 8 ? launch_few<D, 1, true>(st, a, B) : launch_few<D, 2, true>(st, a, B);
+  return L.rows == 8 ? launch_few<D, 1, false>(st, a, B) : launch_few<D, 2, false>(st, a, B);
 }
 
 }  // namespace
