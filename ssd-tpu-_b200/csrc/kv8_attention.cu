@@ -13,9 +13,9 @@
 #include <float.h>
 
 #include <atomic>
-#include <cstdlib>
 
 #include "kv8.cuh"
+#include "tcgen05.cuh"
 
 namespace ssd {
 namespace {
@@ -37,68 +37,90 @@ struct Kv8Attn {
 // Splits of a sequence that hold positions (at least one, which writes its zero rows).
 __device__ __forceinline__ int splits_of(int seq, int split) { return max(1, (seq + split - 1) / split); }
 
-// out = sum_s e^(m_s - M) o_s / sum_s e^(n_s - N) l_s * e^(M - N), M and N the largest m_s and n_s; one warp per
-// query row, lanes over the head dims.  LOG2: the maxima are in powers of two.
+// out = sum_s e^(m_s - M) o_s / sum_s e^(n_s - N) l_s * e^(M - N), M and N the largest m_s and n_s.  One CTA per
+// query row: its threads hold 4 dims of every SG-th split each and add the groups up in order, so that the
+// loads of many splits are in flight at once.  LOG2: the maxima are in powers of two.
+constexpr int kJoinThreads = 256;
+constexpr int kJoinChunk = 256;  // splits whose weights are held at a time
+
 template <typename T, int D, int R, bool LOG2>
-__global__ void __launch_bounds__(128) kv8_join_kernel(const Kv8Attn a, int64_t rows) {
-  constexpr int DPL = D / 32;
-  pdl_wait();
-  pdl_trigger();
-  const int lane = threadIdx.x & 31;
-  const int64_t x = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (x >= rows) return;
-  const int r = (int)(x % R);
-  const int64_t grp = x / R;
+__global__ void __launch_bounds__(kJoinThreads) kv8_join_kernel(const Kv8Attn a) {
+  constexpr int DQ = D / 4, SG = kJoinThreads / DQ;
+  __shared__ float w_s[kJoinChunk];
+  __shared__ float red[32];
+  __shared__ float4 part[SG][DQ];
+  const int tid = threadIdx.x;
+  const int r = blockIdx.x % R;
+  const int64_t grp = blockIdx.x / R;
   const int rg = (int)(grp % a.row_groups), head = (int)(grp / a.row_groups % a.c.hkv);
   const int b = (int)(grp / a.row_groups / a.c.hkv);
   const int gr = rg * R + r, t = gr / a.G, g = gr % a.G;
+  pdl_wait();
+  pdl_trigger();
   if (t >= a.T) return;
-  const int seq_full = a.seq_lens[b];
+  const int seq_full = ld_act(a.seq_lens + b);
   const int seq = min(min(seq_full, a.max_blocks * a.c.block_size), a.nsplit * a.split);
-  const int ql = a.q_lens ? min(max(a.q_lens[b], 0), a.T) : a.T;
+  const int ql = a.q_lens ? min(max(ld_act(a.q_lens + b), 0), a.T) : a.T;
   const int ns = splits_of(seq, a.split);
   auto ex = [](float v) { return LOG2 ? exp2f(v) : expf(v); };
   const float4* ml = a.ws_ml + grp * a.nsplit * R + r;
   float M = -INFINITY, N = -INFINITY;
-  for (int s = lane; s < ns; s += 32) {
+  for (int s = tid; s < ns; s += kJoinThreads) {
     const float4 v = __ldcg(ml + (int64_t)s * R);
     M = fmaxf(M, v.x);
     N = fmaxf(N, v.y);
   }
-  M = warp_max(M);
-  N = warp_max(N);
+  M = block_reduce(M, red, OpMax());
+  N = block_reduce(N, red, OpMax());
+  const int d4 = tid % DQ, sg = tid / DQ;
+  const float* po = a.ws_o + (grp * a.nsplit * R + r) * D + d4 * 4;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
   float L = 0.f;
-  for (int s = lane; s < ns; s += 32) {
-    const float4 v = __ldcg(ml + (int64_t)s * R);
-    if (v.y != -INFINITY) L += v.z * ex(v.y - N);
-  }
-  L = warp_sum(L);
-  float o[DPL];
-#pragma unroll
-  for (int i = 0; i < DPL; ++i) o[i] = 0.f;
-  const float* po = a.ws_o + (grp * a.nsplit * R + r) * D + lane;
-  if (t < ql && L != 0.f) {  // L is NaN, not 0, where a seen score is
+  for (int s0 = 0; s0 < ns; s0 += kJoinChunk) {
+    const int n = min(kJoinChunk, ns - s0);
+    if (tid < n) {
+      const float4 v = __ldcg(ml + (int64_t)(s0 + tid) * R);
+      if (v.y != -INFINITY) L += v.z * ex(v.y - N);
+      w_s[tid] = v.x == -INFINITY ? 0.f : ex(v.x - M);
+    }
+    __syncthreads();
 #pragma unroll 4
-    for (int s = 0; s < ns; ++s) {
-      const float m = __ldcg(ml + (int64_t)s * R).x;
-      if (m == -INFINITY) continue;
-      const float f = ex(m - M);
+    for (int s = sg; s < n; s += SG) {
+      const float f = w_s[s];
+      const float4 x = __ldcg(reinterpret_cast<const float4*>(po + (int64_t)(s0 + s) * R * D));
+      if (f != 0.f) {  // a split that the row does not see holds zeros, or NaN marks of other rows
+        o.x = fmaf(f, x.x, o.x);
+        o.y = fmaf(f, x.y, o.y);
+        o.z = fmaf(f, x.z, o.z);
+        o.w = fmaf(f, x.w, o.w);
+      }
+    }
+    __syncthreads();
+  }
+  part[sg][d4] = o;
+  L = block_reduce(L, red, OpSum());
+  const bool real = t < ql && L != 0.f;  // L is NaN, not 0, where a seen score is
+  if (tid < DQ) {
+    o = part[0][tid];
 #pragma unroll
-      for (int i = 0; i < DPL; ++i) o[i] = fmaf(f, __ldcg(po + (int64_t)s * R * D + i * 32), o[i]);
+    for (int x = 1; x < SG; ++x) {
+      const float4 p = part[x][tid];
+      o.x += p.x; o.y += p.y; o.z += p.z; o.w += p.w;
     }
     const float f = ex(M - N);
-#pragma unroll
-    for (int i = 0; i < DPL; ++i) o[i] = o[i] / L * f;
+    T* out = reinterpret_cast<T*>(a.out) + (((int64_t)b * a.T + t) * a.hq + head * a.G + g) * D + tid * 4;
+    out[0] = from_f<T>(real ? o.x / L * f : 0.f);
+    out[1] = from_f<T>(real ? o.y / L * f : 0.f);
+    out[2] = from_f<T>(real ? o.z / L * f : 0.f);
+    out[3] = from_f<T>(real ? o.w / L * f : 0.f);
   }
-  T* out = reinterpret_cast<T*>(a.out) + (((int64_t)b * a.T + t) * a.hq + head * a.G + g) * D + lane;
-#pragma unroll
-  for (int i = 0; i < DPL; ++i) out[i * 32] = from_f<T>(o[i]);
 }
 
 template <typename T, int D, int R, bool LOG2>
 int launch_join(cudaStream_t st, const Kv8Attn& a, int B) {
   const int64_t rows = (int64_t)B * a.c.hkv * a.row_groups * R;
-  SSD_PDL((kv8_join_kernel<T, D, R, LOG2>), (unsigned)((rows + 3) / 4), 128, 0, st, a, rows);
+  if (rows > 0x7fffffff) return SSD_ERR_UNSUPPORTED;
+  SSD_PDL((kv8_join_kernel<T, D, R, LOG2>), (unsigned)rows, kJoinThreads, 0, st, a);
   return SSD_OK;
 }
 
@@ -251,6 +273,11 @@ __device__ __forceinline__ void mma_f16(float* c, uint32_t a0, uint32_t a1, uint
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ float ex2(float x) {  // 2^x to 2^-22, zero below 2^-126
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   uint32_t r;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
@@ -284,7 +311,7 @@ struct FewSmem {
   static constexpr size_t ring = (size_t)kFewWarps * STAGES * 2 * TILE;
   static_assert(sizeof(float) * kFewWarps * 8 * PITCH <= ring, "the join reuses the rings");
   static constexpr size_t qs = sizeof(uint2) * NT * (D / 16) * 32;  // Q operands, in lane order
-  static size_t total(int split) { return ring + qs + (size_t)(UNI ? split / 16 : split) * 12; }
+  static size_t total(int split) { return ring + qs + (UNI ? 0 : (size_t)split * 12); }
 };
 
 // UNI: block_size is a multiple of 16, so a tile lies in one page and has one pair of scales.
@@ -300,11 +327,10 @@ __global__ void __launch_bounds__(kFewWarps * 32, NT == 1 ? 3 : 2) kv8_attention
   extern __shared__ __align__(128) unsigned char smem[];
   float* os = reinterpret_cast<float*>(smem);
   uint2* qsm = reinterpret_cast<uint2*>(smem + S::ring);
-  // per tile (UNI) or per position: row number in the layer (-1: none), K scale, exponent of V's scale
+  // !UNI, per position: row number in the layer (-1: none), K scale, exponent of V's scale
   int* row_s = reinterpret_cast<int*>(smem + S::ring + S::qs);
-  const int nmeta = UNI ? a.split / 16 : a.split;
-  float* ks_s = reinterpret_cast<float*>(row_s + nmeta);
-  float* ve_s = ks_s + nmeta;
+  float* ks_s = reinterpret_cast<float*>(row_s + a.split);
+  float* ve_s = ks_s + a.split;
   __shared__ float4 ml_s[kFewWarps][R], fin_s[R];
   __shared__ float qscale_s[R];
   __shared__ int nan_seen;
@@ -315,39 +341,80 @@ __global__ void __launch_bounds__(kFewWarps * 32, NT == 1 ? 3 : 2) kv8_attention
   const int head = blockIdx.y / a.row_groups, rg = blockIdx.y % a.row_groups;
   const int row0 = rg * R;
   pdl_wait();
+  // Block ids do not wait for the lengths: entries of this split that the table has.  UNI: lane k of a warp keeps
+  // row number (-1: none) and scales of the warp's k-th tile; otherwise shared memory holds them per position.
+  const int base = split * a.split;
+  const int32_t* table = a.tables + (int64_t)b * a.max_blocks;
+  const float* sc = a.c.scales + a.c.scale_layer + head;
+  int row_l = -1;
+  float ks_l = 1.f, ve_l = 0.f;
+  if constexpr (UNI) {
+    const int j = base + (warp + lane * kFewWarps) * 16, page = j / a.c.block_size;
+    if (lane * kFewWarps * 16 < a.split && page < a.max_blocks) {
+      const int blk = ld_act(table + page);
+      if ((unsigned)blk < (unsigned)a.c.num_blocks) {
+        row_l = blk * a.c.block_size + (j - page * a.c.block_size);
+        ks_l = ld_act(sc + (int64_t)blk * a.c.hkv);
+        ve_l = ld_act(sc + a.c.scale_plane + (int64_t)blk * a.c.hkv);
+      }
+    }
+  }
   const int seq_full = ld_act(a.seq_lens + b);
   const int ql = a.q_lens ? min(max(ld_act(a.q_lens + b), 0), a.T) : a.T;
   const int seq = min(min(seq_full, a.max_blocks * a.c.block_size), a.nsplit * a.split);
-  const int base = split * a.split;
   if (split > 0 && base >= seq) return;
   const int kn = min(max(seq - base, 0), a.split);  // positions of this split that exist
   const int total_rows = a.G * a.T;
-
-  // ---- where each position's rows lie, and its scales
-  {
-    const int32_t* table = a.tables + (int64_t)b * a.max_blocks;
-    const int n = UNI ? (kn + 15) / 16 : (kn + 15) & ~15;
-    for (int i = tid; i < n; i += kFewWarps * 32) {
+  if constexpr (!UNI) {
+    for (int i = tid; i < ((kn + 15) & ~15); i += kFewWarps * 32) {
       int row = -1;
       float ks = 1.f, ve = 0.f;
-      const int j = base + (UNI ? 16 * i : i);
-      if (j < base + kn) {
-        const int page = j / a.c.block_size;
+      if (i < kn) {
+        const int j = base + i, page = j / a.c.block_size;
         const int blk = ld_act(table + page);
         if ((unsigned)blk < (unsigned)a.c.num_blocks) {
           row = blk * a.c.block_size + (j - page * a.c.block_size);
-          const float* sc = a.c.scales + a.c.scale_layer + (int64_t)blk * a.c.hkv + head;
-          ks = exp2i(scale_exponent(ld_act(sc)));
-          ve = (float)scale_exponent(ld_act(sc + a.c.scale_plane));
+          ks = exp2i(scale_exponent(ld_act(sc + (int64_t)blk * a.c.hkv)));
+          ve = (float)scale_exponent(ld_act(sc + a.c.scale_plane + (int64_t)blk * a.c.hkv));
         }
       }
       row_s[i] = row;
       ks_s[i] = ks;
       ve_s[i] = ve;
     }
-    if (tid == 0) nan_seen = 0;
+    __syncthreads();
   }
+  if (tid == 0) nan_seen = 0;
 
+  const int64_t rs = (int64_t)a.c.hkv * D;
+  // the ring: piece p of row r lies at p ^ 4 (r & 1) of K's rows and p ^ (r & 6) of V's, so that a quarter warp's
+  // 16-byte reads meet no bank twice (D = 64: a line holds two rows, V's 8-byte reads meet each bank twice)
+  auto k_piece = [](int r, int p) { return r * PCS + (D >= 128 ? p ^ ((r & 1) << 2) : p); };
+  auto v_piece = [](int r, int p) { return r * PCS + (D >= 128 ? p ^ (r & 6) : p ^ (r >> 1 & 3)); };
+  const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * (S::STAGES * 2 * S::TILE);
+  const uint8_t* kp = a.c.pages + a.c.layer + (int64_t)head * D + (lane % PCS) * 16;
+  const int tiles = (kn + 15) / 16;
+  const int mine = warp < tiles ? (tiles - warp + kFewWarps - 1) / kFewWarps : 0;
+  auto issue = [&](int k) {  // this warp's k-th tile, into stage k % STAGES
+    const int first_l = UNI ? __shfl_sync(0xffffffffu, row_l, k & 31) : 0;
+    if (k < mine) {
+      const int i0 = (warp + k * kFewWarps) * 16;
+      const uint32_t st = ring + (k % S::STAGES) * (2 * S::TILE);
+      constexpr int RPI = 32 / PCS;  // rows an instruction covers
+#pragma unroll
+      for (int x = 0; x < 16 / RPI; ++x) {
+        const int r = x * RPI + lane / PCS;
+        const int first = UNI ? first_l : row_s[i0 + r];
+        const bool there = first >= 0 && (!UNI || i0 + r < kn);
+        const uint8_t* src = kp + (there ? first + (UNI ? r : 0) : 0) * rs;
+        cp_async16(st + k_piece(r, lane % PCS) * 16, src, there);
+        cp_async16(st + S::TILE + v_piece(r, lane % PCS) * 16, src + a.c.plane, there);
+      }
+    }
+    cp_async_commit();
+  };
+#pragma unroll
+  for (int k = 0; k < S::STAGES - 1; ++k) issue(k);
   // ---- Q, scaled into f16, in the order of the lanes' operands: a warp takes two rows of 8 (16 lanes a row)
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
@@ -400,7 +467,6 @@ __global__ void __launch_bounds__(kFewWarps * 32, NT == 1 ? 3 : 2) kv8_attention
     for (int i = 0; i < CK * 4; ++i) qf[i] = qsm[i * 32 + lane];
   }
 
-  const int64_t rs = (int64_t)a.c.hkv * D;
   float M[NT][2], N[NT][2], l[NT][2], o[NT][HV * MT][4];
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
@@ -414,33 +480,10 @@ __global__ void __launch_bounds__(kFewWarps * 32, NT == 1 ? 3 : 2) kv8_attention
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[nt][i][e] = 0.f;
   }
-  // the ring: piece p of row r lies at p ^ 4 (r & 1) of K's rows and p ^ (r & 6) of V's, so that a quarter warp's
-  // 16-byte reads meet no bank twice (D = 64: a line holds two rows, V's 8-byte reads meet each bank twice)
-  auto k_piece = [](int r, int p) { return r * PCS + (D >= 128 ? p ^ ((r & 1) << 2) : p); };
-  auto v_piece = [](int r, int p) { return r * PCS + (D >= 128 ? p ^ (r & 6) : p ^ (r >> 1 & 3)); };
-  const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * (S::STAGES * 2 * S::TILE);
-  const uint8_t* kp = a.c.pages + a.c.layer + (int64_t)head * D + (lane % PCS) * 16;
-  const int tiles = (kn + 15) / 16;
-  const int mine = warp < tiles ? (tiles - warp + kFewWarps - 1) / kFewWarps : 0;
-  auto issue = [&](int k) {  // this warp's k-th tile, into stage k % STAGES
-    if (k < mine) {
-      const int i0 = (warp + k * kFewWarps) * 16;
-      const uint32_t st = ring + (k % S::STAGES) * (2 * S::TILE);
-      constexpr int RPI = 32 / PCS;  // rows an instruction covers
-#pragma unroll
-      for (int x = 0; x < 16 / RPI; ++x) {
-        const int r = x * RPI + lane / PCS;
-        const int first = UNI ? row_s[i0 >> 4] : row_s[i0 + r];
-        const bool there = first >= 0 && (!UNI || i0 + r < kn);
-        const uint8_t* src = kp + (there ? first + (UNI ? r : 0) : 0) * rs;
-        cp_async16(st + k_piece(r, lane % PCS) * 16, src, there);
-        cp_async16(st + S::TILE + v_piece(r, lane % PCS) * 16, src + a.c.plane, there);
-      }
-    }
-    cp_async_commit();
-  };
-#pragma unroll
-  for (int k = 0; k < S::STAGES - 1; ++k) issue(k);
+  if constexpr (UNI) {
+    ks_l = exp2i(scale_exponent(ks_l));
+    ve_l = (float)scale_exponent(ve_l);
+  }
   for (int k = 0; k < mine; ++k) {
     cp_async_wait<S::STAGES - 2>();
     __syncwarp();  // every lane's copies of tile k are there, and every lane is done with tile k - 1
@@ -448,11 +491,11 @@ __global__ void __launch_bounds__(kFewWarps * 32, NT == 1 ? 3 : 2) kv8_attention
     const int i0 = (warp + k * kFewWarps) * 16;
     const uint32_t st = ring + (k % S::STAGES) * (2 * S::TILE);
     // ---- S^T = K Q^T
-    float s[NT][4];
+    float s[NT][4], s2[NT][4];  // two chains: an instruction does not wait for the one before it
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s[nt][e] = 0.f;
+      for (int e = 0; e < 4; ++e) s[nt][e] = s2[nt][e] = 0.f;
 #pragma unroll
     for (int c = 0; c < CK; ++c) {
       const uint4 p0 = lds128(st + k_piece(g, 4 * c + t4) * 16), p1 = lds128(st + k_piece(g + 8, 4 * c + t4) * 16);
@@ -468,16 +511,30 @@ __global__ void __launch_bounds__(kFewWarps * 32, NT == 1 ? 3 : 2) kv8_attention
           uint2 q;
           if constexpr (NT == 1) q = qf[4 * c + j];
           else q = qsm[(nt * CK * 4 + 4 * c + j) * 32 + lane];
-          mma_f16(s[nt], a0, a1, a2, a3, q.x, q.y);
+          mma_f16(j & 1 ? s2[nt] : s[nt], a0, a1, a2, a3, q.x, q.y);
         }
       }
     }
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[nt][e] += s2[nt][e];
     // ---- running maxima and weights
-    const int m0 = UNI ? i0 >> 4 : i0 + g, m1 = UNI ? m0 : m0 + 8;
     // a position without a row lies behind every query
-    const int at0 = row_s[m0] >= 0 && (!UNI || i0 + g < kn) ? base + i0 + g : 0x7fffffff;
-    const int at1 = row_s[m1] >= 0 && (!UNI || i0 + g + 8 < kn) ? base + i0 + g + 8 : 0x7fffffff;
-    const float k0 = ks_s[m0], k1 = ks_s[m1], e0 = ve_s[m0], e1 = ve_s[m1];
+    int at0 = base + i0 + g, at1 = at0 + 8;
+    float k0, k1, e0, e1;
+    if constexpr (UNI) {
+      const bool has = __shfl_sync(0xffffffffu, row_l, k) >= 0;
+      if (!has || i0 + g >= kn) at0 = 0x7fffffff;
+      if (!has || i0 + g + 8 >= kn) at1 = 0x7fffffff;
+      k0 = k1 = __shfl_sync(0xffffffffu, ks_l, k);
+      e0 = e1 = __shfl_sync(0xffffffffu, ve_l, k);
+    } else {
+      if (row_s[i0 + g] < 0) at0 = 0x7fffffff;
+      if (row_s[i0 + g + 8] < 0) at1 = 0x7fffffff;
+      k0 = ks_s[i0 + g], k1 = ks_s[i0 + g + 8];
+      e0 = ve_s[i0 + g], e1 = ve_s[i0 + g + 8];
+    }
     uint32_t pb[NT][2];
     bool moved = false;
     float f[NT][2];
@@ -502,18 +559,18 @@ __global__ void __launch_bounds__(kFewWarps * 32, NT == 1 ? 3 : 2) kv8_attention
         // the reference moves only when a weight would pass 2^8 (f16 holds 2^15): most tiles rescale nothing
         f[nt][e] = 1.f;
         if (m > M[nt][e] + 8.f) {
-          f[nt][e] = exp2f(M[nt][e] - m);
+          f[nt][e] = ex2(M[nt][e] - m);
           M[nt][e] = m;
           moved = true;
         }
         if (n > N[nt][e] + 8.f) {
-          l[nt][e] *= exp2f(N[nt][e] - n);
+          l[nt][e] *= ex2(N[nt][e] - n);
           N[nt][e] = n;
         }
-        w[e] = see0 ? exp2f(s0 + e0 - M[nt][e]) : 0.f;
-        w[2 + e] = see1 ? exp2f(s1 + e1 - M[nt][e]) : 0.f;
-        if (see0) l[nt][e] += exp2f(s0 - N[nt][e]);
-        if (see1) l[nt][e] += exp2f(s1 - N[nt][e]);
+        w[e] = see0 ? ex2(s0 + e0 - M[nt][e]) : 0.f;
+        w[2 + e] = see1 ? ex2(s1 + e1 - M[nt][e]) : 0.f;
+        if (see0) l[nt][e] += ex2(s0 - N[nt][e]);
+        if (see1) l[nt][e] += ex2(s1 - N[nt][e]);
       }
       pb[nt][0] = transpose8x8(pack_f16(w[0], w[1]));
       pb[nt][1] = transpose8x8(pack_f16(w[2], w[3]));
@@ -597,7 +654,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, NT == 1 ? 3 : 2) kv8_attention
     }
 #pragma unroll
     for (int w = 0; w < kFewWarps; ++w)
-      if (ml_s[w][tid].y != -INFINITY) L += ml_s[w][tid].z * exp2f(ml_s[w][tid].y - n);
+      if (ml_s[w][tid].y != -INFINITY) L += ml_s[w][tid].z * ex2(ml_s[w][tid].y - n);
     fin_s[tid] = make_float4(m, n, L, 0.f);
   }
   const int64_t grp = ((int64_t)b * a.c.hkv + head) * a.row_groups + rg;
@@ -610,7 +667,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, NT == 1 ? 3 : 2) kv8_attention
       float m = -INFINITY;
 #pragma unroll
       for (int w = 0; w < kFewWarps; ++w) m = fmaxf(m, ml_s[w][r].x);
-      f[e] = M[nt][e] == -INFINITY ? 0.f : exp2f(M[nt][e] - m);
+      f[e] = M[nt][e] == -INFINITY ? 0.f : ex2(M[nt][e] - m);
     }
     float* ow = os + (warp * 8 + 2 * t4) * S::PITCH;
 #pragma unroll
@@ -639,9 +696,9 @@ __global__ void __launch_bounds__(kFewWarps * 32, NT == 1 ? 3 : 2) kv8_attention
       const int p = t < ql ? seq_full - ql + t : -1;
       if (nan_seen) {  // rare: a position past kmin holds NaN in V
         for (int j = max(kmin + 1, base); j <= min(p, base + kn - 1); ++j) {
-          const int first = row_s[UNI ? (j - base) >> 4 : j - base];
-          if (first < 0) continue;
-          const int64_t row = first + (UNI ? (j - base) & 15 : 0);
+          const int blk = ld_act(table + j / a.c.block_size);
+          if ((unsigned)blk >= (unsigned)a.c.num_blocks) continue;
+          const int64_t row = (int64_t)blk * a.c.block_size + j % a.c.block_size;
           const uint32_t v = __ldcg(reinterpret_cast<const uint16_t*>(a.c.pages + a.c.plane + a.c.layer + row * rs +
                                                                       (int64_t)head * D + d));
           if ((v & 0x7fu) == 0x7fu) O.x = __int_as_float(0x7fc00000);
@@ -650,7 +707,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, NT == 1 ? 3 : 2) kv8_attention
       }
       if (a.nsplit == 1) {
         const float4 z = fin_s[8 * nt + r];
-        const float k = exp2f(z.x - z.y);
+        const float k = ex2(z.x - z.y);
         const bool ok = p >= 0 && z.z != 0.f;
         *reinterpret_cast<__nv_bfloat162*>(reinterpret_cast<bf16*>(a.out) +
                                            (((int64_t)b * a.T + t) * a.hq + head * a.G + (gr - t * a.G)) * D + d) =
@@ -664,6 +721,444 @@ __global__ void __launch_bounds__(kFewWarps * 32, NT == 1 ? 3 : 2) kv8_attention
   if (a.nsplit > 1 && tid < R) a.ws_ml[(grp * a.nsplit + split) * R + tid] = fin_s[tid];
 }
 
+
+// ------------------------------------------------------------------ many query rows (bf16): prompt chunks
+// A CTA takes 128 query rows of one KV head and a split of the positions, on the tensor cores (tcgen05, f16
+// operands, fp32 accumulators in TMEM): S = Q K^T for a tile of 64 positions (M = 128, N = 64), weights in f16
+// to shared memory, O += P V (N = D).  K and V become f16 on the way into shared memory, in one layout: rows
+// are positions, 64 dims to a 128-byte swizzled line.  That is K-major for K and, with V's dims as the long
+// side of its operand, MN-major for V, so nothing is transposed.
+//   warps 0-3   one query row a thread: scores out of TMEM, maxima, weights, rescaling of O (only when a row's
+//               reference has to move, see the few-row kernel), the result
+//   warps 4-11  pages to f16 tiles, the next tile's bytes in flight while this one is converted
+//   warp 12     issues the products: S of tile j + 1 goes before O of tile j, so the weights of one tile are
+//               made while the tensor cores work on the next
+// All waits are bounded: a CTA that gives up lets its copies and products end and writes NaN.
+namespace many {
+
+constexpr int ROWS = 128;    // query rows of a CTA: TMEM lanes
+constexpr int TILE = 64;     // positions of a tile
+constexpr int SOFT = 128;    // threads of the row warps
+constexpr int CONV = 256;    // threads of the converting warps
+constexpr int THREADS = SOFT + CONV + 32;
+constexpr int META = 4;      // tiles whose scales are kept: a tile's are read until its weights are done
+constexpr uint32_t kPolls = 1u << 24;
+
+template <int D>
+struct Cfg {
+  static constexpr uint32_t Q = ROWS * D * 2, KV = TILE * D * 2, P = ROWS * TILE * 2;
+  static constexpr uint32_t q = 0, k = Q, v = k + 2 * KV, p = v + 2 * KV, meta = p + P;
+  static constexpr uint32_t bars = meta + META * TILE * 8;
+  static constexpr size_t smem = 1024 + bars + 128;  // 14 barriers, TMEM address, two flags
+  static constexpr uint32_t tmem_cols = D == 256 ? 512 : 256, o_col = D == 256 ? 256 : 128;
+};
+
+__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile int* stop) {
+  for (uint32_t i = 0; i < kPolls; ++i) {
+    if (tc::mbar_try_wait(bar, parity)) return true;
+    if ((i & 255u) == 255u && *stop) return false;
+  }
+  *stop = 1;
+  return false;
+}
+
+// N fp32 columns of this warp's 32 TMEM lanes; the registers are valid once tmem_ready has seen them.
+__device__ __forceinline__ void tmem_load32(uint32_t addr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(addr));
+}
+__device__ __forceinline__ void tmem_ready(uint32_t* r) {  // ties the registers to the wait
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                 "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]),
+                 "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]),
+                 "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]),
+                 "+r"(r[30]), "+r"(r[31])::"memory");
+}
+__device__ __forceinline__ void tmem_store32(uint32_t addr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::"r"(r[0]),
+      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]),
+      "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]),
+      "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(addr)
+      : "memory");
+}
+
+// 16-byte piece `c` (of 64-dim lines) of row r of an operand whose lines of `rows` rows lie line after line.
+__device__ __forceinline__ uint32_t piece(uint32_t base, int rows, int r, int c) {
+  return base + (c >> 3) * (rows * 128) + (r >> 3) * 1024 + (r & 7) * 128 + (((c & 7) ^ (r & 7)) << 4);
+}
+__device__ __forceinline__ void sts128(uint32_t p, uint4 v) {
+  asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(p), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+
+// f16 operands, fp32 accumulator, M = 128; B's long side contiguous (MN-major) or not.
+template <int N, bool B_MN>
+__host__ __device__ constexpr uint32_t idesc() {
+  return (1u << 4) | ((B_MN ? 1u : 0u) << 16) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(ROWS >> 4) << 24);
+}
+// MN-major, 128-byte swizzle: 64 elements of the long side to a line, lines of the next 64 `TILE` rows further,
+// groups of 8 along the summed side 1024 bytes apart.
+__device__ __forceinline__ uint64_t mn_desc(uint32_t saddr) {
+  return (uint64_t)((saddr & 0x3FFFFu) >> 4) | ((uint64_t)((TILE * 128) >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+         ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+
+template <int D>
+__global__ void __launch_bounds__(THREADS, 1) kv8_attention_many_kernel(const Kv8Attn a) {
+  using C = Cfg<D>;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = tc::smem_u32(smem_raw), sm = (raw + 1023u) & ~1023u;
+  uint8_t* gen = smem_raw + (sm - raw);
+  float2* meta = reinterpret_cast<float2*>(gen + C::meta);  // [META][TILE]: K scale (< 0: no row), V exponent
+  auto bar = [&](int i) { return sm + C::bars + 8 * i; };
+  const uint32_t q_full = bar(0), p_full = bar(1), o_done = bar(2), drained = bar(13);
+  auto k_full = [&](int s) { return bar(3 + s); };
+  auto k_free = [&](int s) { return bar(5 + s); };
+  auto v_full = [&](int s) { return bar(7 + s); };
+  auto v_free = [&](int s) { return bar(9 + s); };
+  auto s_full = [&](int s) { return bar(11 + s); };
+  uint32_t* slot = reinterpret_cast<uint32_t*>(gen + C::bars + 112);
+  volatile int* stop = reinterpret_cast<volatile int*>(slot + 1);
+  volatile int* nan_seen = reinterpret_cast<volatile int*>(slot + 2);
+
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int split = blockIdx.x, b = blockIdx.z;
+  const int head = blockIdx.y / a.row_groups, rg = blockIdx.y % a.row_groups;
+  if (tid == 0) {
+    tc::mbar_init(q_full, SOFT);
+    tc::mbar_init(p_full, SOFT);
+    tc::mbar_init(o_done, 1);
+    tc::mbar_init(drained, 1);
+    for (int s = 0; s < 2; ++s) {
+      tc::mbar_init(k_full(s), CONV);
+      tc::mbar_init(k_free(s), 1);
+      tc::mbar_init(v_full(s), CONV);
+      tc::mbar_init(v_free(s), 1);
+      tc::mbar_init(s_full(s), 1);
+    }
+    *stop = 0;
+    *nan_seen = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  }
+  if (warp == THREADS / 32 - 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc::smem_u32(slot)),
+                 "r"(C::tmem_cols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  tc::tc_fence_after();
+  const uint32_t tmem = *slot;
+  pdl_wait();
+
+  const int seq_full = ld_act(a.seq_lens + b);
+  const int ql = a.q_lens ? min(max(ld_act(a.q_lens + b), 0), a.T) : a.T;
+  const int seq = min(min(seq_full, a.max_blocks * a.c.block_size), a.nsplit * a.split);
+  const int base = split * a.split;
+  const int row0 = rg * ROWS, rows = min(ROWS, a.G * a.T - row0);
+  const int n0 = seq_full - ql;
+  const int t0 = row0 / a.G, t1 = min((row0 + rows - 1) / a.G, ql - 1);  // the group's first and last real token
+  const int kmin = max(n0 + t0, 0);                                       // every row that sees anything sees 0..kmin
+  const int kn = t0 > t1 ? 0 : min(min(seq, base + a.split), n0 + t1 + 1) - base;
+  const int tiles = kn > 0 ? (kn + TILE - 1) / TILE : 0;
+  const int32_t* table = a.tables + (int64_t)b * a.max_blocks;
+
+  if (warp < SOFT / 32) {
+    // -------------------------------------------------------------- rows
+    const int r = tid, gr = row0 + r, t = gr / a.G, g = gr - t * a.G;
+    const bool real = r < rows && t < ql && n0 + t >= 0;
+    const int pos = real ? n0 + t : -1;
+    const int64_t at = (((int64_t)b * a.T + t) * a.hq + head * a.G + g) * D;
+    float qs = 0.f;
+    if (tiles > 0) {
+      const bf16* src = reinterpret_cast<const bf16*>(a.q) + (real ? at : 0);
+      float amax = 0.f;
+#pragma unroll 4
+      for (int i = 0; i < D / 8; ++i) {
+        float f[8];
+        unpack8(ld_act_v4(src + 8 * i), f);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) amax = fmaxf(amax, finite_abs(f[j]));
+      }
+      const int e = min(max((int)(__float_as_uint(amax) >> 23) - 127, -118), 120);
+      const float inv = real ? exp2i(-e) : 0.f;
+      qs = exp2i(e) * a.scale * 1.4426950408889634f;
+#pragma unroll 4
+      for (int i = 0; i < D / 8; ++i) {
+        float f[8];
+        unpack8(ld_act_v4(src + 8 * i), f);
+        uint4 w = make_uint4(pack_f16(f[0] * inv, f[1] * inv), pack_f16(f[2] * inv, f[3] * inv),
+                             pack_f16(f[4] * inv, f[5] * inv), pack_f16(f[6] * inv, f[7] * inv));
+        if (!real) w = make_uint4(0, 0, 0, 0);
+        sts128(piece(sm + C::q, ROWS, r, i), w);
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      tc::mbar_arrive(q_full);
+    }
+    const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
+    float M = -INFINITY, N = -INFINITY, l = 0.f;
+    bool ok = true;
+    for (int j = 0; ok && j < tiles; ++j) {
+      const float2* mt = meta + (j % META) * TILE;
+      ok = wait(s_full(j & 1), (j >> 1) & 1, stop);
+      if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+      tc::tc_fence_after();
+      uint32_t x[TILE];
+      tmem_load32(lanes + (j & 1) * TILE, x);
+      tmem_load32(lanes + (j & 1) * TILE + 32, x + 32);
+      tmem_ready(x);
+      tmem_ready(x + 32);
+      const int p0 = base + j * TILE;
+      float m = -INFINITY, n = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < TILE; ++i) {
+        const float2 kv = mt[i];
+        const bool see = kv.x >= 0.f && p0 + i <= pos;
+        const float s = __uint_as_float(x[i]) * (qs * kv.x);
+        x[i] = __float_as_uint(see ? s : -INFINITY);
+        if (see) {  // a NaN score counts as the lowest value here and spoils the sums below
+          const float y = fmaxf(s, -1e38f);
+          n = fmaxf(n, y);
+          m = fmaxf(m, y + kv.y);
+        }
+      }
+      float f = 1.f;
+      if (m > M + 8.f) {
+        f = ex2(M - m);
+        M = m;
+      }
+      if (n > N + 8.f) {
+        l *= ex2(N - n);
+        N = n;
+      }
+      // with nothing seen so far both references are -inf: every weight below is 2^-inf
+      const float Ms = M == -INFINITY ? 0.f : M, Ns = N == -INFINITY ? 0.f : N;
+      uint32_t w[TILE / 2];
+#pragma unroll
+      for (int i = 0; i < TILE; i += 2) {
+        const float s0 = __uint_as_float(x[i]), s1 = __uint_as_float(x[i + 1]);
+        w[i / 2] = pack_f16(ex2(s0 + mt[i].y - Ms), ex2(s1 + mt[i + 1].y - Ms));
+        l += ex2(s0 - Ns);
+        l += ex2(s1 - Ns);
+      }
+      if (j > 0) {  // O of the tile before: its weights' buffer is free and O may be rescaled
+        ok = wait(o_done, (j - 1) & 1, stop);
+        if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+        tc::tc_fence_after();
+        if (__any_sync(0xffffffffu, f != 1.f)) {
+#pragma unroll 1
+          for (int c = 0; c < D; c += 32) {
+            uint32_t y[32];
+            tmem_load32(lanes + C::o_col + c, y);
+            tmem_ready(y);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) y[i] = __float_as_uint(__uint_as_float(y[i]) * f);
+            tmem_store32(lanes + C::o_col + c, y);
+          }
+          asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < TILE / 8; ++i)
+        sts128(piece(sm + C::p, ROWS, r, i), make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]));
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      tc::tc_fence_before();
+      tc::mbar_arrive(p_full);
+    }
+    if (ok && tiles > 0) {
+      ok = wait(o_done, (tiles - 1) & 1, stop);
+      ok = __all_sync(0xffffffffu, ok);
+    }
+    tc::tc_fence_after();
+    if (!ok) l = __int_as_float(0x7fc00000);
+    const int64_t grp = ((int64_t)b * a.c.hkv + head) * a.row_groups + rg;
+    const int64_t po = (grp * a.nsplit + split) * ROWS + r;
+    const bool any = real && l != 0.f;  // l is NaN, not 0, where a seen score is
+    const float k = any ? ex2(M - N) : 0.f;
+    if (a.nsplit > 1) a.ws_ml[po] = make_float4(ok ? M : 0.f, ok ? N : 0.f, l, 0.f);
+    if (a.nsplit == 1 || tiles > 0) {
+#pragma unroll 1
+      for (int c = 0; c < D; c += 32) {
+        uint32_t y[32];
+        if (tiles > 0 && ok) {
+          tmem_load32(lanes + C::o_col + c, y);
+          tmem_ready(y);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) y[i] = 0;
+        }
+        if (*nan_seen && real) {  // rare: a position past kmin holds NaN in V
+          for (int j = max(kmin + 1, base); j <= min(pos, base + kn - 1); ++j) {
+            const int blk = ld_act(table + j / a.c.block_size);
+            if ((unsigned)blk >= (unsigned)a.c.num_blocks) continue;
+            const uint8_t* v = a.c.pages + a.c.plane + a.c.layer +
+                               (((int64_t)blk * a.c.block_size + j % a.c.block_size) * a.c.hkv + head) * D + c;
+            for (int i = 0; i < 32; ++i)
+              if ((__ldcg(v + i) & 0x7f) == 0x7f) {
+#pragma unroll
+                for (int z = 0; z < 32; ++z)
+                  if (z == i) y[z] = 0x7fc00000u;
+              }
+          }
+        }
+        if (a.nsplit > 1) {
+          float4* o = reinterpret_cast<float4*>(a.ws_o + po * D + c);
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            o[i] = make_float4(__uint_as_float(y[4 * i]), __uint_as_float(y[4 * i + 1]),
+                               __uint_as_float(y[4 * i + 2]), __uint_as_float(y[4 * i + 3]));
+        } else if (r < rows) {
+          bf16* o = reinterpret_cast<bf16*>(a.out) + at + c;
+          float z[8];
+#pragma unroll
+          for (int i = 0; i < 32; i += 8) {
+#pragma unroll
+            for (int h = 0; h < 8; ++h) z[h] = any ? __uint_as_float(y[i + h]) / l * k : 0.f;
+            uint4 u;
+            __nv_bfloat162* h2 = reinterpret_cast<__nv_bfloat162*>(&u);
+#pragma unroll
+            for (int h = 0; h < 4; ++h) h2[h] = __floats2bfloat162_rn(z[2 * h], z[2 * h + 1]);
+            *reinterpret_cast<uint4*>(o + i) = u;
+          }
+        }
+      }
+    }
+    tc::tc_fence_before();
+  } else if (warp < (SOFT + CONV) / 32) {
+    // -------------------------------------------------------------- pages to f16 tiles
+    // A warp takes 8 positions of a tile, 32 / PCS of them at a time, 16 dims a lane.
+    constexpr int PCS = D / 16, RPI = 32 / PCS, NI = 8 / RPI;
+    const int cw = warp - SOFT / 32, pc = lane % PCS, r0 = 8 * cw + lane / PCS;
+    const uint8_t* kp = a.c.pages + a.c.layer + (int64_t)head * D + pc * 16;
+    const float* sc = a.c.scales + a.c.scale_layer + head;
+    const int64_t rs = (int64_t)a.c.hkv * D;
+    uint4 kr[NI], vr[NI];
+    float2 sv[NI];
+    auto fetch = [&](int j) {
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+        const int p = j * TILE + r0 + i * RPI;
+        int blk = -1, off = 0;
+        if (p < kn) {
+          const int page = (base + p) / a.c.block_size;
+          blk = ld_act(table + page);
+          off = base + p - page * a.c.block_size;
+        }
+        kr[i] = vr[i] = make_uint4(0, 0, 0, 0);
+        sv[i] = make_float2(-1.f, 0.f);
+        if ((unsigned)blk < (unsigned)a.c.num_blocks) {
+          const uint8_t* s = kp + ((int64_t)blk * a.c.block_size + off) * rs;
+          kr[i] = ld_act_v4(s);
+          vr[i] = ld_act_v4(s + a.c.plane);
+          sv[i] = make_float2(ld_act(sc + (int64_t)blk * a.c.hkv), ld_act(sc + a.c.scale_plane + (int64_t)blk * a.c.hkv));
+        }
+      }
+    };
+    auto put = [&](uint32_t tile, int r, uint4 w) {
+      uint4 lo, hi;
+      f16x4_of(w.x, lo.x, lo.y);
+      f16x4_of(w.y, lo.z, lo.w);
+      f16x4_of(w.z, hi.x, hi.y);
+      f16x4_of(w.w, hi.z, hi.w);
+      // lanes of odd 64-dim lines write their halves in the other order: no bank twice in a quarter warp
+      const bool odd = (pc >> 2) & 1;
+      sts128(piece(tile, TILE, r, 2 * pc + odd), odd ? hi : lo);
+      sts128(piece(tile, TILE, r, 2 * pc + !odd), odd ? lo : hi);
+    };
+    if (tiles > 0) fetch(0);
+    bool ok = true;
+    for (int j = 0; ok && j < tiles; ++j) {
+      const int s = j & 1;
+      if (j >= 2) ok = wait(k_free(s), ((j >> 1) - 1) & 1, stop);
+      if (!ok) break;
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+        const int r = r0 + i * RPI;
+        if (pc == 0)
+          meta[(j % META) * TILE + r] =
+              sv[i].x < 0.f ? sv[i] : make_float2(exp2i(scale_exponent(sv[i].x)), (float)scale_exponent(sv[i].y));
+        put(sm + C::k + s * C::KV, r, kr[i]);
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      tc::mbar_arrive(k_full(s));
+      if (j >= 2) ok = wait(v_free(s), ((j >> 1) - 1) & 1, stop);
+      if (!ok) break;
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+        const int r = r0 + i * RPI;
+        if (base + j * TILE + r > kmin) {  // NaN of positions that some row does not see: put back by row above
+          if (nan_marks(vr[i].x) | nan_marks(vr[i].y) | nan_marks(vr[i].z) | nan_marks(vr[i].w)) *nan_seen = 1;
+          vr[i] = make_uint4(clear_nan(vr[i].x), clear_nan(vr[i].y), clear_nan(vr[i].z), clear_nan(vr[i].w));
+        }
+        put(sm + C::v + s * C::KV, r, vr[i]);
+      }
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      tc::mbar_arrive(v_full(s));
+      if (j + 1 < tiles) fetch(j + 1);
+    }
+    __syncwarp();
+  } else {
+    // -------------------------------------------------------------- products
+    if (lane == 0 && tiles > 0) {
+      auto scores = [&](int j) {
+        const int s = j & 1;
+        if (!wait(k_full(s), (j >> 1) & 1, stop)) return false;
+        tc::tc_fence_after();
+#pragma unroll
+        for (int d = 0; d < D / 64; ++d) {
+          const uint64_t qd = tc::sw128_desc(sm + C::q + d * (ROWS * 128));
+          const uint64_t kd = tc::sw128_desc(sm + C::k + s * C::KV + d * (TILE * 128));
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            tc::umma_bf16(tmem + s * TILE, qd + 2 * k, kd + 2 * k, idesc<TILE, false>(), d || k);
+        }
+        tc::umma_commit(k_free(s));
+        tc::umma_commit(s_full(s));
+        return true;
+      };
+      bool ok = wait(q_full, 0, stop) && scores(0);
+      for (int j = 0; ok && j < tiles; ++j) {
+        const int s = j & 1;
+        if (j + 1 < tiles) ok = scores(j + 1);
+        ok = ok && wait(p_full, j & 1, stop) && wait(v_full(s), (j >> 1) & 1, stop);
+        if (!ok) break;
+        tc::tc_fence_after();
+        const uint64_t pd = tc::sw128_desc(sm + C::p);
+        const uint64_t vd = mn_desc(sm + C::v + s * C::KV);
+#pragma unroll
+        for (int k = 0; k < TILE / 16; ++k)  // 16 positions: 32 bytes of P's line, two groups of 8 rows of V
+          tc::umma_bf16(tmem + C::o_col, pd + 2 * k, vd + (2048 >> 4) * k, idesc<D, true>(), j || k);
+        tc::umma_commit(v_free(s));
+        tc::umma_commit(o_done);
+      }
+      if (!ok) {  // let the products issued so far end before TMEM goes back
+        tc::umma_commit(drained);
+        for (uint32_t i = 0; i < kPolls && !tc::mbar_try_wait(drained, 0); ++i) {}
+      }
+    }
+    __syncwarp();
+  }
+  pdl_trigger();
+  __syncthreads();
+  if (warp == THREADS / 32 - 1) {
+    tc::tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::tmem_cols) : "memory");
+  }
+}
+
+}  // namespace many
+
 struct Kv8Layout {
   bool cc;              // CUDA-core kernel (fp32)
   int rows;             // query rows of a group
@@ -674,13 +1169,26 @@ struct Kv8Layout {
 
 inline size_t up256(size_t x) { return (x + 255) & ~size_t(255); }
 
+constexpr int kManyFrom = 16;  // query rows of a KV head above which a call goes to the many-row kernel
+
 Kv8Layout kv8_layout(bool cc, int B, int T, int hq, int hkv, int D, int max_seq_len) {
   Kv8Layout L;
   const int64_t total = (int64_t)(hq / hkv) * T;
   L.cc = cc;
-  L.rows = cc ? kCcRows : total > 8 ? 16 : 8;
-  L.split = cc ? kCcSplit : getenv("KSPLIT") ? atoi(getenv("KSPLIT")) : 256;
+  L.rows = cc ? kCcRows : total > kManyFrom ? many::ROWS : total > 8 ? 16 : 8;
+  // Few rows: 256 positions keep a short context's CTAs many (one sequence of 8192 positions, one KV head: 11.9 us
+  // against 18.7 us at 1024); where there is work for every SM either way, 1024 positions cost fewer prologues and
+  // partials (8 sequences, 16 heads, up to 4096 positions: 38.1 against 43.2 us).  The rule goes by the sequences,
+  // never by the rows, so a query's bits do not depend on how many new tokens stand beside it.
+  L.split = cc ? kCcSplit : (int64_t)B * hkv * ((max_seq_len + 255) / 256) >= 2048 ? 1024 : 256;
   L.row_groups = (int)((total + L.rows - 1) / L.rows);
+  if (L.rows == many::ROWS) {
+    const int64_t ctas = (int64_t)B * hkv * L.row_groups;
+    const int64_t want = (148 + ctas - 1) / ctas;  // splits that fill the SMs
+    int64_t sp = (max_seq_len + want - 1) / want;
+    sp = (sp + 63) / 64 * 64;
+    L.split = (int)(sp < 256 ? 256 : sp);
+  }
   L.nsplit = (max_seq_len + L.split - 1) / L.split;
   L.groups = (size_t)B * hkv * L.row_groups;
   const size_t rows = L.nsplit == 1 ? 0 : L.groups * L.nsplit * L.rows;
@@ -724,7 +1232,19 @@ int launch_few(cudaStream_t st, const Kv8Attn& a, int B) {
 }
 
 template <int D>
+int launch_many(cudaStream_t st, const Kv8Attn& a, int B) {
+  auto kern = many::kv8_attention_many_kernel<D>;
+  constexpr size_t smem = many::Cfg<D>::smem;
+  static_assert(smem <= 227 * 1024);
+  static std::atomic<uint64_t> ready{0};
+  if (!allow_smem(ready, kern, (int)smem)) return SSD_ERR_LAUNCH;
+  SSD_PDL(kern, dim3(a.nsplit, a.c.hkv * a.row_groups, B), many::THREADS, smem, st, a);
+  return a.nsplit == 1 ? SSD_OK : launch_join<bf16, D, many::ROWS, true>(st, a, B);
+}
+
+template <int D>
 int launch_bf16(cudaStream_t st, const Kv8Attn& a, const Kv8Layout& L, int B) {
+  if (L.rows == many::ROWS) return launch_many<D>(st, a, B);
   if (a.c.block_size % 16 == 0) return L.rows == 8 ? launch_few<D, 1, true>(st, a, B) : launch_few<D, 2, true>(st, a, B);
   return L.rows == 8 ? launch_few<D, 1, false>(st, a, B) : launch_few<D, 2, false>(st, a, B);
 }
