@@ -13,6 +13,7 @@
 #include <float.h>
 
 #include <atomic>
+#include <cstdlib>
 
 #include "kv8.cuh"
 #include "tcgen05.cuh"
@@ -728,17 +729,18 @@ __global__ void __launch_bounds__(kFewWarps * 32, NT == 1 ? 3 : 2) kv8_attention
 // to shared memory, O += P V (N = D).  K and V become f16 on the way into shared memory, in one layout: rows
 // are positions, 64 dims to a 128-byte swizzled line.  That is K-major for K and, with V's dims as the long
 // side of its operand, MN-major for V, so nothing is transposed.
-//   warps 0-3   one query row a thread: scores out of TMEM, maxima, weights, rescaling of O (only when a row's
-//               reference has to move, see the few-row kernel), the result
-//   warps 4-11  pages to f16 tiles, the next tile's bytes in flight while this one is converted
-//   warp 12     issues the products: S of tile j + 1 goes before O of tile j, so the weights of one tile are
+//   warps 0-7   two threads a query row, half a tile's positions each: scores out of TMEM, maxima (exchanged between
+//               the two), weights, rescaling of O (only when a row's reference has to move, see the few-row
+//               kernel), the result
+//   warps 8-15  pages to f16 tiles, the next tile's bytes in flight while this one is converted
+//   warp 16     issues the products: S of tile j + 1 goes before O of tile j, so the weights of one tile are
 //               made while the tensor cores work on the next
 // All waits are bounded: a CTA that gives up lets its copies and products end and writes NaN.
 namespace many {
 
 constexpr int ROWS = 128;    // query rows of a CTA: TMEM lanes
 constexpr int TILE = 64;     // positions of a tile
-constexpr int SOFT = 128;    // threads of the row warps
+constexpr int SOFT = 256;    // threads of the row warps: two a query row, 32 positions of a tile each
 constexpr int CONV = 256;    // threads of the converting warps
 constexpr int THREADS = SOFT + CONV + 32;
 constexpr int META = 4;      // tiles whose scales are kept: a tile's are read until its weights are done
@@ -747,11 +749,17 @@ constexpr uint32_t kPolls = 1u << 24;
 template <int D>
 struct Cfg {
   static constexpr uint32_t Q = ROWS * D * 2, KV = TILE * D * 2, P = ROWS * TILE * 2;
-  static constexpr uint32_t q = 0, k = Q, v = k + 2 * KV, p = v + 2 * KV, meta = p + P;
-  static constexpr uint32_t bars = meta + META * TILE * 8;
-  static constexpr size_t smem = 1024 + bars + 128;  // 14 barriers, TMEM address, two flags
-  static constexpr uint32_t tmem_cols = D == 256 ? 512 : 256, o_col = D == 256 ? 256 : 128;
+  static constexpr uint32_t q = 0, k = Q, v = k + 2 * KV, p = v + 2 * KV;
+  static constexpr uint32_t meta = p + 2 * P, qs = meta + META * TILE * 4, bars = qs + ROWS * 4;
+  static constexpr size_t smem = 1024 + bars + 192;  // 22 barriers, TMEM address, two flags
+  // TMEM columns: two tiles' scores, Q (two f16 to a column), O
+  static constexpr uint32_t q_col = 2 * TILE, o_col = q_col + D / 2, tmem_cols = D == 64 ? 256 : 512;
+  static_assert(o_col + D <= tmem_cols);
 };
+// A position's scale exponents in one word: K's + 256 in the upper half (0: the position has no row), V's + 256 below.
+__device__ __forceinline__ uint32_t pack_meta(int ke, int ve) { return (uint32_t)(ke + 256) << 16 | (uint32_t)(ve + 256); }
+__device__ __forceinline__ int meta_k(uint32_t m) { return (int)(m >> 16) - 256; }
+__device__ __forceinline__ float meta_v(uint32_t m) { return (float)((int)(m & 0xffffu) - 256); }
 
 __device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile int* stop) {
   for (uint32_t i = 0; i < kPolls; ++i) {
@@ -781,6 +789,13 @@ __device__ __forceinline__ void tmem_ready(uint32_t* r) {  // ties the registers
                  "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]),
                  "+r"(r[30]), "+r"(r[31])::"memory");
 }
+__device__ __forceinline__ void tmem_store16(uint32_t addr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::"r"(r[0]),
+      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(addr)
+      : "memory");
+}
 __device__ __forceinline__ void tmem_store32(uint32_t addr, const uint32_t* r) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
@@ -789,6 +804,16 @@ __device__ __forceinline__ void tmem_store32(uint32_t addr, const uint32_t* r) {
       "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]),
       "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]),
       "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(addr)
+      : "memory");
+}
+
+// D += A B with A in TMEM.
+__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b_desc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
 
@@ -812,21 +837,30 @@ __device__ __forceinline__ uint64_t mn_desc(uint32_t saddr) {
          ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
 }
 
-template <int D>
+// UNI: block_size is a multiple of 16.
+template <int D, bool UNI>
 __global__ void __launch_bounds__(THREADS, 1) kv8_attention_many_kernel(const Kv8Attn a) {
   using C = Cfg<D>;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = tc::smem_u32(smem_raw), sm = (raw + 1023u) & ~1023u;
   uint8_t* gen = smem_raw + (sm - raw);
-  float2* meta = reinterpret_cast<float2*>(gen + C::meta);  // [META][TILE]: K scale (< 0: no row), V exponent
+  uint32_t* meta = reinterpret_cast<uint32_t*>(gen + C::meta);  // [META][TILE], see pack_meta
+  float* qs_s = reinterpret_cast<float*>(gen + C::qs);
   auto bar = [&](int i) { return sm + C::bars + 8 * i; };
-  const uint32_t q_full = bar(0), p_full = bar(1), o_done = bar(2), drained = bar(13);
-  auto k_full = [&](int s) { return bar(3 + s); };
-  auto k_free = [&](int s) { return bar(5 + s); };
-  auto v_full = [&](int s) { return bar(7 + s); };
-  auto v_free = [&](int s) { return bar(9 + s); };
-  auto s_full = [&](int s) { return bar(11 + s); };
-  uint32_t* slot = reinterpret_cast<uint32_t*>(gen + C::bars + 112);
+  const uint32_t q_full = bar(0), o_done = bar(1), drained = bar(2);
+  auto p_full = [&](int s) { return bar(3 + s); };
+  auto p_free = [&](int s) { return bar(5 + s); };
+  auto k_full = [&](int s) { return bar(7 + s); };
+  auto k_free = [&](int s) { return bar(9 + s); };
+  auto v_full = [&](int s) { return bar(11 + s); };
+  auto v_free = [&](int s) { return bar(13 + s); };
+  auto s_full = [&](int s) { return bar(15 + s); };
+  const uint32_t q_tmem = bar(17);
+  auto pair = [&](int q) { return bar(18 + q); };
+  // [tile parity][half][row]: the threads' maxima, where Q was (every row thread has moved its part on before the
+  // first scores come; the result is staged there after the last product, hence after the last swap)
+  float2* pair_s = reinterpret_cast<float2*>(gen + C::q);
+  uint32_t* slot = reinterpret_cast<uint32_t*>(gen + C::bars + 176);
   volatile int* stop = reinterpret_cast<volatile int*>(slot + 1);
   volatile int* nan_seen = reinterpret_cast<volatile int*>(slot + 2);
 
@@ -834,11 +868,14 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_many_kernel(const Kv
   const int split = blockIdx.x, b = blockIdx.z;
   const int head = blockIdx.y / a.row_groups, rg = blockIdx.y % a.row_groups;
   if (tid == 0) {
-    tc::mbar_init(q_full, SOFT);
-    tc::mbar_init(p_full, SOFT);
+    tc::mbar_init(q_full, SOFT + CONV);
+    tc::mbar_init(q_tmem, SOFT);
     tc::mbar_init(o_done, 1);
     tc::mbar_init(drained, 1);
+    for (int q = 0; q < 4; ++q) tc::mbar_init(pair(q), 64);
     for (int s = 0; s < 2; ++s) {
+      tc::mbar_init(p_full(s), SOFT);
+      tc::mbar_init(p_free(s), 1);
       tc::mbar_init(k_full(s), CONV);
       tc::mbar_init(k_free(s), 1);
       tc::mbar_init(v_full(s), CONV);
@@ -874,66 +911,214 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_many_kernel(const Kv
   const int tiles = kn > 0 ? (kn + TILE - 1) / TILE : 0;
   const int32_t* table = a.tables + (int64_t)b * a.max_blocks;
 
+  // Q: raw rows into place (cp.async), then f16 under a power of two per row, in place; a lane converts the pieces
+  // it has copied.  By the row and the converting warps, STEP rows at a time.
+  auto load_q = [&]() {
+    constexpr int LPR = D / 8, RPW = 32 / LPR, STEP = (SOFT + CONV) / 32 * RPW;
+    static_assert(ROWS % STEP == 0);
+    const int first = warp * RPW + lane / LPR, pc = lane % LPR, dt = STEP / a.G, dg = STEP - dt * a.G;
+    int t = (row0 + first) / a.G, g = row0 + first - t * a.G;
+#pragma unroll 4
+    for (int r = first; r < ROWS; r += STEP) {
+      const bool there = r < rows && t < ql;
+      const bf16* src = reinterpret_cast<const bf16*>(a.q) +
+                        (there ? (((int64_t)b * a.T + t) * a.hq + head * a.G + g) * D + pc * 8 : 0);
+      cp_async16(piece(sm + C::q, ROWS, r, pc), src, there);
+      t += dt;
+      g += dg;
+      if (g >= a.G) {
+        g -= a.G;
+        ++t;
+      }
+    }
+    cp_async_commit();
+    cp_async_wait<0>();
+#pragma unroll 4
+    for (int r = first; r < ROWS; r += STEP) {  // STEP divides ROWS: every lane of a warp makes the same rounds
+      const uint32_t at = piece(sm + C::q, ROWS, r, pc);
+      const uint4 w = lds128(at);
+      // largest magnitude of the row, as bf16 bits (infinities and NaN end in NaN scores of the row)
+      const uint32_t v[4] = {w.x, w.y, w.z, w.w};
+      __nv_bfloat162 t2 = __float2bfloat162_rn(0.f);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) t2 = __hmax2(t2, __habs2(*reinterpret_cast<const __nv_bfloat162*>(&v[j])));
+      const uint32_t both = *reinterpret_cast<const uint32_t*>(&t2);
+      uint32_t top = max(both >> 16, both & 0xffffu);
+      if constexpr (LPR == 32) {
+        top = __reduce_max_sync(0xffffffffu, top);
+      } else {
+#pragma unroll
+        for (int x = 1; x < LPR; x <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, x));
+      }
+      const int e = min(max((int)(top >> 7) - 127, -118), 120);
+      const float inv = exp2i(-e);
+      uint32_t y[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        y[j] = pack_f16(__uint_as_float(v[j] << 16) * inv, __uint_as_float(v[j] & 0xffff0000u) * inv);
+      sts128(at, make_uint4(y[0], y[1], y[2], y[3]));
+      if (pc == 0) qs_s[r] = exp2i(e) * a.scale * 1.4426950408889634f;
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    tc::mbar_arrive(q_full);
+  };
+
+  // Converting warps: one takes 8 positions of a tile, RPI of them at a time, 16 dims a lane, eight lanes on four
+  // pieces of an even and an odd row (their 16-byte stores then meet no bank twice).  Block ids are read two tiles
+  // ahead, bytes one tile ahead, the first ones before Q.
+  constexpr int PCS = D / 16, RPI = 32 / PCS, NI = 8 / RPI, NB = UNI ? 1 : NI;
+  const int cw = warp - SOFT / 32;
+  const int rr = ((lane >> 2) & 1) | ((lane >> 3) / (PCS / 4)) << 1, pc = (lane & 3) | ((lane >> 3) % (PCS / 4)) << 2;
+  const uint8_t* kp = a.c.pages + a.c.layer + (int64_t)head * D + pc * 16;
+  const float* sc = a.c.scales + a.c.scale_layer + head;
+  const int64_t rs = (int64_t)a.c.hkv * D;
+  uint4 kb[NI], vb[NI];
+  float ks[NB], vs[NB];  // scales (ks < 0: no row); UNI: the eight positions lie in one page
+  int blk[NB], off[NB];  // of the tile to be fetched next
+  auto look = [&](int j) {
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+      const int p = j * TILE + 8 * cw + (UNI ? 0 : rr + i * RPI);
+      blk[i] = -1;
+      off[i] = 0;
+      if (p < kn) {
+        const int page = (base + p) / a.c.block_size;
+        blk[i] = ld_act(table + page);
+        off[i] = base + p - page * a.c.block_size;
+      }
+    }
+  };
+  // bytes of tile j's K (plane 0) or V rows into x, and the plane's scales
+  auto fetch = [&](int j, int64_t plane, int64_t scale_plane, uint4* x, float* xs) {
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+      xs[i] = (unsigned)blk[i] < (unsigned)a.c.num_blocks ? ld_act(sc + scale_plane + (int64_t)blk[i] * a.c.hkv) : -1.f;
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int n = UNI ? 0 : i;
+      x[i] = make_uint4(0, 0, 0, 0);
+      if ((unsigned)blk[n] < (unsigned)a.c.num_blocks && (!UNI || j * TILE + 8 * cw + rr + i * RPI < kn))
+        x[i] = ld_act_v4(kp + plane + ((int64_t)blk[n] * a.c.block_size + off[n] + (UNI ? rr + i * RPI : 0)) * rs);
+    }
+  };
+  if (tiles > 0 && warp < (SOFT + CONV) / 32) {
+    if (warp >= SOFT / 32) {
+      look(0);
+      fetch(0, 0, 0, kb, ks);
+      fetch(0, a.c.plane, a.c.scale_plane, vb, vs);
+      look(1);
+    }
+    load_q();
+  }
+
   if (warp < SOFT / 32) {
     // -------------------------------------------------------------- rows
-    const int r = tid, gr = row0 + r, t = gr / a.G, g = gr - t * a.G;
+    const int quad = warp & 3, half = warp >> 2;  // TMEM lanes 32 quad .., positions 32 half .. of a tile
+    const int r = quad * 32 + lane, gr = row0 + r, t = gr / a.G, g = gr - t * a.G;
     const bool real = r < rows && t < ql && n0 + t >= 0;
     const int pos = real ? n0 + t : -1;
     const int64_t at = (((int64_t)b * a.T + t) * a.hq + head * a.G + g) * D;
-    float qs = 0.f;
-    if (tiles > 0) {
-      const bf16* src = reinterpret_cast<const bf16*>(a.q) + (real ? at : 0);
-      float amax = 0.f;
-#pragma unroll 4
-      for (int i = 0; i < D / 8; ++i) {
-        float f[8];
-        unpack8(ld_act_v4(src + 8 * i), f);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) amax = fmaxf(amax, finite_abs(f[j]));
-      }
-      const int e = min(max((int)(__float_as_uint(amax) >> 23) - 127, -118), 120);
-      const float inv = real ? exp2i(-e) : 0.f;
-      qs = exp2i(e) * a.scale * 1.4426950408889634f;
-#pragma unroll 4
-      for (int i = 0; i < D / 8; ++i) {
-        float f[8];
-        unpack8(ld_act_v4(src + 8 * i), f);
-        uint4 w = make_uint4(pack_f16(f[0] * inv, f[1] * inv), pack_f16(f[2] * inv, f[3] * inv),
-                             pack_f16(f[4] * inv, f[5] * inv), pack_f16(f[6] * inv, f[7] * inv));
-        if (!real) w = make_uint4(0, 0, 0, 0);
-        sts128(piece(sm + C::q, ROWS, r, i), w);
-      }
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      tc::mbar_arrive(q_full);
-    }
-    const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
-    float M = -INFINITY, N = -INFINITY, l = 0.f;
+    const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16);
+    float qs = 1.f;
     bool ok = true;
-    for (int j = 0; ok && j < tiles; ++j) {
-      const float2* mt = meta + (j % META) * TILE;
-      ok = wait(s_full(j & 1), (j >> 1) & 1, stop);
-      if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-      tc::tc_fence_after();
-      uint32_t x[TILE];
-      tmem_load32(lanes + (j & 1) * TILE, x);
-      tmem_load32(lanes + (j & 1) * TILE + 32, x + 32);
-      tmem_ready(x);
-      tmem_ready(x + 32);
-      const int p0 = base + j * TILE;
-      float m = -INFINITY, n = -INFINITY;
+    if (tiles > 0) {
+      ok = __all_sync(0xffffffffu, wait(q_full, 0, stop));
+      // Q goes on to TMEM as the first operand: read from shared memory it would cost S more of that memory's
+      // bandwidth than K does
+#pragma unroll 1
+      for (int c = half * (D / 4); c < (half + 1) * (D / 4); c += 16) {
+        uint32_t y[16];
 #pragma unroll
-      for (int i = 0; i < TILE; ++i) {
-        const float2 kv = mt[i];
-        const bool see = kv.x >= 0.f && p0 + i <= pos;
-        const float s = __uint_as_float(x[i]) * (qs * kv.x);
-        x[i] = __float_as_uint(see ? s : -INFINITY);
-        if (see) {  // a NaN score counts as the lowest value here and spoils the sums below
-          const float y = fmaxf(s, -1e38f);
-          n = fmaxf(n, y);
-          m = fmaxf(m, y + kv.y);
+        for (int i = 0; i < 4; ++i) {
+          const uint4 z = lds128(piece(sm + C::q, ROWS, r, c / 4 + i));
+          y[4 * i] = z.x; y[4 * i + 1] = z.y; y[4 * i + 2] = z.z; y[4 * i + 3] = z.w;
+        }
+        tmem_store16(lanes + C::q_col + c, y);
+      }
+      asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+      tc::tc_fence_before();
+      tc::mbar_arrive(q_tmem);
+      qs = qs_s[r];
+      if (qs == 0.f) qs = 1e-38f;  // keeps the mask's infinity out of 0 * infinity; the scores stay below 2^-60
+    }
+    const float hidden = qs > 0.f ? -INFINITY : INFINITY;
+    // M: what the weights are relative to, N: what l is; -1e38 where nothing has been seen
+    float M = -1e38f, N = -1e38f, l = 0.f, vtop = -1000.f;
+    // The row's two threads swap a pair of numbers; false when the CTA gives up.  `k`: how many swaps went before.
+    auto swap = [&](float2* at2, int k, float& x, float& y) {
+      at2[((k & 1) * 2 + half) * ROWS + r] = make_float2(x, y);
+      tc::mbar_arrive(pair(quad));
+      if (!__all_sync(0xffffffffu, wait(pair(quad), k & 1, stop))) return false;
+      const float2 z = at2[((k & 1) * 2 + (half ^ 1)) * ROWS + r];
+      x = z.x;
+      y = z.y;
+      return true;
+    };
+#pragma unroll 1
+    for (int j = 0; ok && j < tiles; ++j) {
+      ok = __all_sync(0xffffffffu, wait(s_full(j & 1), (j >> 1) & 1, stop));
+      if (!ok) break;
+      tc::tc_fence_after();
+      const int p0 = base + j * TILE + 32 * half;  // this thread's 32 positions
+      const uint32_t* mt = meta + (j % META) * TILE + half * (UNI ? 4 : 32);
+      uint32_t x[32];
+      tmem_load32(lanes + (j & 1) * TILE + 32 * half, x);
+      float m = -1e38f, n = -1e38f, f = 1.f;
+      // a NaN score counts as the lowest value in the maxima and spoils the sums
+      float ca = 0.f, cb = 0.f, va = 0.f, vb2 = 0.f;
+      bool wide = false;
+      if constexpr (UNI) {
+        // two groups of 16 positions, one pair of scales each
+        uint32_t wa = mt[0], wb = mt[2];
+        const bool ina = wa >= 65536u, inb = wb >= 65536u;
+        if (!ina) wa = pack_meta(0, 0);
+        if (!inb) wb = pack_meta(0, 0);
+        ca = qs * exp2i(meta_k(wa));
+        cb = qs * exp2i(meta_k(wb));
+        va = meta_v(wa);
+        vb2 = meta_v(wb);
+        // Weights' sums can be carried over to l's reference unless a page's V scale is far below the largest so
+        // far (the weights could vanish); then l takes its own exponentials.
+        vtop = fmaxf(vtop, fmaxf(va, vb2));
+        wide = fminf(va, vb2) < vtop - 40.f;
+        tmem_ready(x);
+        if (p0 + 31 > kmin || p0 + 32 > base + kn || !ina || !inb) {  // hide what the row does not see
+          const int k = min(pos, base + kn - 1) - p0;
+          uint32_t keep = k >= 31 ? 0xffffffffu : k < 0 ? 0u : (2u << k) - 1;
+          if (!ina) keep &= 0xffff0000u;
+          if (!inb) keep &= 0x0000ffffu;
+#pragma unroll
+          for (int i = 0; i < 32; ++i)
+            if (!(keep >> i & 1)) x[i] = __float_as_uint(hidden);
+        }
+        float ya = -1e38f, yb = -1e38f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          ya = fmaxf(ya, __uint_as_float(x[i]) * ca);
+          yb = fmaxf(yb, __uint_as_float(x[16 + i]) * cb);
+        }
+        n = fmaxf(ya, yb);
+        m = fmaxf(ya + va, yb + vb2);
+      } else {
+        tmem_ready(x);
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          const uint32_t w = mt[i];
+          const bool see = w >= 65536u && p0 + i <= pos;
+          const float s = see ? __uint_as_float(x[i]) * (qs * exp2i(meta_k(w))) : -INFINITY;
+          x[i] = __float_as_uint(s);
+          if (see) {
+            const float y = fmaxf(s, -1e38f);
+            n = fmaxf(n, y);
+            m = fmaxf(m, y + meta_v(w));
+          }
         }
       }
-      float f = 1.f;
+      float mo = m, no = n;
+      ok = swap(pair_s, j, mo, no);
+      if (!ok) break;
+      m = fmaxf(m, mo);
+      n = fmaxf(n, no);
       if (m > M + 8.f) {
         f = ex2(M - m);
         M = m;
@@ -942,54 +1127,84 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_many_kernel(const Kv
         l *= ex2(N - n);
         N = n;
       }
-      // with nothing seen so far both references are -inf: every weight below is 2^-inf
-      const float Ms = M == -INFINITY ? 0.f : M, Ns = N == -INFINITY ? 0.f : N;
-      uint32_t w[TILE / 2];
+      uint32_t w[16];
+      if constexpr (UNI) {
+        if (wide) {
 #pragma unroll
-      for (int i = 0; i < TILE; i += 2) {
-        const float s0 = __uint_as_float(x[i]), s1 = __uint_as_float(x[i + 1]);
-        w[i / 2] = pack_f16(ex2(s0 + mt[i].y - Ms), ex2(s1 + mt[i + 1].y - Ms));
-        l += ex2(s0 - Ns);
-        l += ex2(s1 - Ns);
-      }
-      if (j > 0) {  // O of the tile before: its weights' buffer is free and O may be rescaled
-        ok = wait(o_done, (j - 1) & 1, stop);
-        if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-        tc::tc_fence_after();
-        if (__any_sync(0xffffffffu, f != 1.f)) {
-#pragma unroll 1
-          for (int c = 0; c < D; c += 32) {
-            uint32_t y[32];
-            tmem_load32(lanes + C::o_col + c, y);
-            tmem_ready(y);
+          for (int i = 0; i < 32; ++i) l += ex2(fmaf(__uint_as_float(x[i]), i < 16 ? ca : cb, -N));
+        }
+        const float oa = va - M, ob = vb2 - M;
+        float sa[2] = {0.f, 0.f}, sb[2] = {0.f, 0.f};
 #pragma unroll
-            for (int i = 0; i < 32; ++i) y[i] = __float_as_uint(__uint_as_float(y[i]) * f);
-            tmem_store32(lanes + C::o_col + c, y);
+        for (int i = 0; i < 16; i += 2) {
+          float e[4];
+#pragma unroll
+          for (int z = 0; z < 2; ++z) {
+            e[z] = ex2(fmaf(__uint_as_float(x[i + z]), ca, oa));
+            e[2 + z] = ex2(fmaf(__uint_as_float(x[16 + i + z]), cb, ob));
+            sa[z] += e[z];
+            sb[z] += e[2 + z];
           }
-          asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+          w[i / 2] = pack_f16(e[0], e[1]);
+          w[8 + i / 2] = pack_f16(e[2], e[3]);
+        }
+        if (!wide) {
+          l = fmaf(sa[0] + sa[1], ex2(-oa - N), l);
+          l = fmaf(sb[0] + sb[1], ex2(-ob - N), l);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) {
+          const float s0 = __uint_as_float(x[i]), s1 = __uint_as_float(x[i + 1]);
+          w[i / 2] = pack_f16(ex2(s0 + (meta_v(mt[i]) - M)), ex2(s1 + (meta_v(mt[i + 1]) - M)));
+          l += ex2(s0 - N) + ex2(s1 - N);
         }
       }
+      if (j >= 2) ok = __all_sync(0xffffffffu, wait(p_free(j & 1), ((j >> 1) - 1) & 1, stop));
+      if (!ok) break;
 #pragma unroll
-      for (int i = 0; i < TILE / 8; ++i)
-        sts128(piece(sm + C::p, ROWS, r, i), make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]));
+      for (int i = 0; i < 4; ++i)
+        sts128(piece(sm + C::p + (j & 1) * C::P, ROWS, r, 4 * half + i),
+               make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]));
+      if (j > 0 && __any_sync(0xffffffffu, f != 1.f)) {  // O, once the tile before has been added; half of it each
+        ok = __all_sync(0xffffffffu, wait(o_done, (j - 1) & 1, stop));
+        if (!ok) break;
+        tc::tc_fence_after();
+#pragma unroll 1
+        for (int c = half * (D / 2); c < (half + 1) * (D / 2); c += 32) {
+          uint32_t y[32];
+          tmem_load32(lanes + C::o_col + c, y);
+          tmem_ready(y);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) y[i] = __float_as_uint(__uint_as_float(y[i]) * f);
+          tmem_store32(lanes + C::o_col + c, y);
+        }
+        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+      }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       tc::tc_fence_before();
-      tc::mbar_arrive(p_full);
+      tc::mbar_arrive(p_full(j & 1));
     }
     if (ok && tiles > 0) {
-      ok = wait(o_done, (tiles - 1) & 1, stop);
-      ok = __all_sync(0xffffffffu, ok);
+      ok = __all_sync(0xffffffffu, wait(o_done, (tiles - 1) & 1, stop));
+      float lo = l, unused = 0.f;
+      ok = ok && swap(reinterpret_cast<float2*>(gen + C::p), tiles, lo, unused);
+      l += lo;
     }
     tc::tc_fence_after();
     if (!ok) l = __int_as_float(0x7fc00000);
     const int64_t grp = ((int64_t)b * a.c.hkv + head) * a.row_groups + rg;
     const int64_t po = (grp * a.nsplit + split) * ROWS + r;
     const bool any = real && l != 0.f;  // l is NaN, not 0, where a seen score is
-    const float k = any ? ex2(M - N) : 0.f;
-    if (a.nsplit > 1) a.ws_ml[po] = make_float4(ok ? M : 0.f, ok ? N : 0.f, l, 0.f);
+    if (a.nsplit > 1 && half == 0) a.ws_ml[po] = make_float4(M, N, l, 0.f);
     if (a.nsplit == 1 || tiles > 0) {
+      // O through the shared memory of Q and K (every product is done), so that rows leave in whole lines: a lane
+      // writes its half row in 16-byte pieces, piece c at c ^ (row % 8), the warp reads half row after half row
+      const float k = a.nsplit > 1 ? 1.f : any ? ex2(M - N) / l : 0.f;
+      const bool zero = a.nsplit == 1 && !any;  // O may be anything where a row sees nothing
+      const uint32_t mine = sm + r * (D * 4);
 #pragma unroll 1
-      for (int c = 0; c < D; c += 32) {
+      for (int c = half * (D / 2); c < (half + 1) * (D / 2); c += 32) {
         uint32_t y[32];
         if (tiles > 0 && ok) {
           tmem_load32(lanes + C::o_col + c, y);
@@ -998,38 +1213,51 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_many_kernel(const Kv
 #pragma unroll
           for (int i = 0; i < 32; ++i) y[i] = 0;
         }
-        if (*nan_seen && real) {  // rare: a position past kmin holds NaN in V
-          for (int j = max(kmin + 1, base); j <= min(pos, base + kn - 1); ++j) {
-            const int blk = ld_act(table + j / a.c.block_size);
-            if ((unsigned)blk >= (unsigned)a.c.num_blocks) continue;
-            const uint8_t* v = a.c.pages + a.c.plane + a.c.layer +
-                               (((int64_t)blk * a.c.block_size + j % a.c.block_size) * a.c.hkv + head) * D + c;
-            for (int i = 0; i < 32; ++i)
-              if ((__ldcg(v + i) & 0x7f) == 0x7f) {
 #pragma unroll
-                for (int z = 0; z < 32; ++z)
-                  if (z == i) y[z] = 0x7fc00000u;
-              }
-          }
+        for (int i = 0; i < 32; ++i) y[i] = zero ? 0u : __float_as_uint(__uint_as_float(y[i]) * k);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          sts128(mine + (((c / 4 + i) ^ (r & 7)) << 4), make_uint4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]));
+      }
+      __syncwarp();
+      constexpr int HD = D / 2;
+      if (a.nsplit > 1) {
+        float* o = a.ws_o + (po - lane) * D + half * HD;
+#pragma unroll 8
+        for (int i = lane; i < 32 * HD / 4; i += 32) {
+          const int rr = i / (HD / 4), c = half * (HD / 4) + i % (HD / 4);
+          const uint4 z = lds128(sm + (quad * 32 + rr) * (D * 4) + ((c ^ (rr & 7)) << 4));
+          *reinterpret_cast<uint4*>(o + rr * D + i % (HD / 4) * 4) = z;
         }
-        if (a.nsplit > 1) {
-          float4* o = reinterpret_cast<float4*>(a.ws_o + po * D + c);
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            o[i] = make_float4(__uint_as_float(y[4 * i]), __uint_as_float(y[4 * i + 1]),
-                               __uint_as_float(y[4 * i + 2]), __uint_as_float(y[4 * i + 3]));
-        } else if (r < rows) {
-          bf16* o = reinterpret_cast<bf16*>(a.out) + at + c;
-          float z[8];
-#pragma unroll
-          for (int i = 0; i < 32; i += 8) {
-#pragma unroll
-            for (int h = 0; h < 8; ++h) z[h] = any ? __uint_as_float(y[i + h]) / l * k : 0.f;
-            uint4 u;
-            __nv_bfloat162* h2 = reinterpret_cast<__nv_bfloat162*>(&u);
-#pragma unroll
-            for (int h = 0; h < 4; ++h) h2[h] = __floats2bfloat162_rn(z[2 * h], z[2 * h + 1]);
-            *reinterpret_cast<uint4*>(o + i) = u;
+      } else {
+#pragma unroll 4
+        for (int i = lane; i < 32 * HD / 8; i += 32) {
+          const int rr = i / (HD / 8), c = half * (HD / 8) + i % (HD / 8);
+          const uint32_t row = sm + (quad * 32 + rr) * (D * 4);
+          const uint4 z = lds128(row + (((2 * c) ^ (rr & 7)) << 4)), y = lds128(row + (((2 * c + 1) ^ (rr & 7)) << 4));
+          const int64_t to = __shfl_sync(0xffffffffu, at, rr);
+          uint4 u;
+          __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&u);
+          h[0] = __floats2bfloat162_rn(__uint_as_float(z.x), __uint_as_float(z.y));
+          h[1] = __floats2bfloat162_rn(__uint_as_float(z.z), __uint_as_float(z.w));
+          h[2] = __floats2bfloat162_rn(__uint_as_float(y.x), __uint_as_float(y.y));
+          h[3] = __floats2bfloat162_rn(__uint_as_float(y.z), __uint_as_float(y.w));
+          if (quad * 32 + rr < rows) *reinterpret_cast<uint4*>(reinterpret_cast<bf16*>(a.out) + to + c * 8) = u;
+        }
+      }
+      __syncwarp();
+      if (*nan_seen && real) {  // rare: a position past kmin holds NaN in V
+#pragma unroll 1
+        for (int j = max(kmin + 1, base); j <= min(pos, base + kn - 1); ++j) {
+          const int blk2 = ld_act(table + j / a.c.block_size);
+          if ((unsigned)blk2 >= (unsigned)a.c.num_blocks) continue;
+          const uint8_t* v = a.c.pages + a.c.plane + a.c.layer +
+                             (((int64_t)blk2 * a.c.block_size + j % a.c.block_size) * a.c.hkv + head) * D;
+#pragma unroll 1
+          for (int d = half * HD; d < (half + 1) * HD; ++d) {
+            if ((__ldcg(v + d) & 0x7f) != 0x7f) continue;
+            if (a.nsplit > 1) a.ws_o[po * D + d] = __int_as_float(0x7fc00000);
+            else reinterpret_cast<bf16*>(a.out)[at + d] = __ushort_as_bfloat16(0x7fc0);
           }
         }
       }
@@ -1037,113 +1265,108 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_many_kernel(const Kv
     tc::tc_fence_before();
   } else if (warp < (SOFT + CONV) / 32) {
     // -------------------------------------------------------------- pages to f16 tiles
-    // A warp takes 8 positions of a tile, 32 / PCS of them at a time, 16 dims a lane.
-    constexpr int PCS = D / 16, RPI = 32 / PCS, NI = 8 / RPI;
-    const int cw = warp - SOFT / 32, pc = lane % PCS, r0 = 8 * cw + lane / PCS;
-    const uint8_t* kp = a.c.pages + a.c.layer + (int64_t)head * D + pc * 16;
-    const float* sc = a.c.scales + a.c.scale_layer + head;
-    const int64_t rs = (int64_t)a.c.hkv * D;
-    uint4 kr[NI], vr[NI];
-    float2 sv[NI];
-    auto fetch = [&](int j) {
-#pragma unroll
-      for (int i = 0; i < NI; ++i) {
-        const int p = j * TILE + r0 + i * RPI;
-        int blk = -1, off = 0;
-        if (p < kn) {
-          const int page = (base + p) / a.c.block_size;
-          blk = ld_act(table + page);
-          off = base + p - page * a.c.block_size;
-        }
-        kr[i] = vr[i] = make_uint4(0, 0, 0, 0);
-        sv[i] = make_float2(-1.f, 0.f);
-        if ((unsigned)blk < (unsigned)a.c.num_blocks) {
-          const uint8_t* s = kp + ((int64_t)blk * a.c.block_size + off) * rs;
-          kr[i] = ld_act_v4(s);
-          vr[i] = ld_act_v4(s + a.c.plane);
-          sv[i] = make_float2(ld_act(sc + (int64_t)blk * a.c.hkv), ld_act(sc + a.c.scale_plane + (int64_t)blk * a.c.hkv));
-        }
-      }
-    };
-    auto put = [&](uint32_t tile, int r, uint4 w) {
+    // row rr + i RPI of the warp's eight: 128 bytes a row, pieces swizzled by it
+    const uint32_t to = (pc >> 2) * (TILE * 128) + cw * 1024 + rr * 128 + ((((2 * pc) & 7) ^ rr) << 4);
+    auto put = [&](uint32_t tile, int i, uint4 w) {
       uint4 lo, hi;
       f16x4_of(w.x, lo.x, lo.y);
       f16x4_of(w.y, lo.z, lo.w);
       f16x4_of(w.z, hi.x, hi.y);
       f16x4_of(w.w, hi.z, hi.w);
-      // lanes of odd 64-dim lines write their halves in the other order: no bank twice in a quarter warp
-      const bool odd = (pc >> 2) & 1;
-      sts128(piece(tile, TILE, r, 2 * pc + odd), odd ? hi : lo);
-      sts128(piece(tile, TILE, r, 2 * pc + !odd), odd ? lo : hi);
+      const uint32_t at = ((tile + to) ^ (i * RPI * 16)) + i * RPI * 128;
+      sts128(at, lo);
+      sts128(at ^ 16, hi);
     };
-    if (tiles > 0) fetch(0);
-    bool ok = true;
-    for (int j = 0; ok && j < tiles; ++j) {
+#pragma unroll 1
+    for (int j = 0; j < tiles; ++j) {
       const int s = j & 1;
-      if (j >= 2) ok = wait(k_free(s), ((j >> 1) - 1) & 1, stop);
-      if (!ok) break;
+      if (j >= 2 && !wait(k_free(s), ((j >> 1) - 1) & 1, stop)) break;
+      uint32_t* mt = meta + (j % META) * TILE;
+      if constexpr (UNI) {
+        if (lane == 0) mt[cw] = ks[0] < 0.f ? 0u : pack_meta(scale_exponent(ks[0]), scale_exponent(vs[0]));
+      }
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
-        const int r = r0 + i * RPI;
-        if (pc == 0)
-          meta[(j % META) * TILE + r] =
-              sv[i].x < 0.f ? sv[i] : make_float2(exp2i(scale_exponent(sv[i].x)), (float)scale_exponent(sv[i].y));
-        put(sm + C::k + s * C::KV, r, kr[i]);
+        if (!UNI && pc == 0)
+          mt[8 * cw + rr + i * RPI] =
+              ks[i % NB] < 0.f ? 0u : pack_meta(scale_exponent(ks[i % NB]), scale_exponent(vs[i % NB]));
+        put(sm + C::k + s * C::KV, i, kb[i]);
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       tc::mbar_arrive(k_full(s));
-      if (j >= 2) ok = wait(v_free(s), ((j >> 1) - 1) & 1, stop);
-      if (!ok) break;
+      fetch(j + 1, 0, 0, kb, ks);
+      if (j >= 2 && !wait(v_free(s), ((j >> 1) - 1) & 1, stop)) break;
+      if (base + j * TILE + 8 * cw + 7 > kmin) {  // NaN of positions that some row does not see: put back by row above
+        uint32_t marks = 0;
 #pragma unroll
-      for (int i = 0; i < NI; ++i) {
-        const int r = r0 + i * RPI;
-        if (base + j * TILE + r > kmin) {  // NaN of positions that some row does not see: put back by row above
-          if (nan_marks(vr[i].x) | nan_marks(vr[i].y) | nan_marks(vr[i].z) | nan_marks(vr[i].w)) *nan_seen = 1;
-          vr[i] = make_uint4(clear_nan(vr[i].x), clear_nan(vr[i].y), clear_nan(vr[i].z), clear_nan(vr[i].w));
+        for (int i = 0; i < NI; ++i)
+          if (base + j * TILE + 8 * cw + rr + i * RPI > kmin)
+            marks |= nan_marks(vb[i].x) | nan_marks(vb[i].y) | nan_marks(vb[i].z) | nan_marks(vb[i].w);
+        if (marks) {
+          *nan_seen = 1;
+#pragma unroll
+          for (int i = 0; i < NI; ++i)
+            if (base + j * TILE + 8 * cw + rr + i * RPI > kmin)
+              vb[i] = make_uint4(clear_nan(vb[i].x), clear_nan(vb[i].y), clear_nan(vb[i].z), clear_nan(vb[i].w));
         }
-        put(sm + C::v + s * C::KV, r, vr[i]);
       }
+#pragma unroll
+      for (int i = 0; i < NI; ++i) put(sm + C::v + s * C::KV, i, vb[i]);
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       tc::mbar_arrive(v_full(s));
-      if (j + 1 < tiles) fetch(j + 1);
+      fetch(j + 1, a.c.plane, a.c.scale_plane, vb, vs);
+      look(j + 2);
     }
     __syncwarp();
   } else {
     // -------------------------------------------------------------- products
-    if (lane == 0 && tiles > 0) {
+    // The whole warp walks the loop and one elected lane issues, so that addresses and descriptors stay in uniform
+    // registers: with the loop inside one lane's branch, every product waited for them to be moved there (2700
+    // instead of NNNN cycles a tile).
+    if (tiles > 0) {
+      uint32_t lead;
+      asm volatile("{.reg .pred p; elect.sync _|p, 0xffffffff; selp.u32 %0, 1, 0, p;}" : "=r"(lead));
+      auto ready = [&](uint32_t b, uint32_t parity) {
+        const bool ok = __all_sync(0xffffffffu, wait(b, parity, stop));
+        tc::tc_fence_after();
+        return ok;
+      };
       auto scores = [&](int j) {
         const int s = j & 1;
-        if (!wait(k_full(s), (j >> 1) & 1, stop)) return false;
-        tc::tc_fence_after();
+        if (!ready(k_full(s), (j >> 1) & 1)) return false;
+        const uint64_t kd = tc::sw128_desc(sm + C::k + s * C::KV);
+        if (lead) {
 #pragma unroll
-        for (int d = 0; d < D / 64; ++d) {
-          const uint64_t qd = tc::sw128_desc(sm + C::q + d * (ROWS * 128));
-          const uint64_t kd = tc::sw128_desc(sm + C::k + s * C::KV + d * (TILE * 128));
+          for (int d = 0; d < D / 64; ++d)
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            tc::umma_bf16(tmem + s * TILE, qd + 2 * k, kd + 2 * k, idesc<TILE, false>(), d || k);
+            for (int k = 0; k < 4; ++k)
+              umma_ts(tmem + s * TILE, tmem + C::q_col + d * 32 + 8 * k, kd + d * ((TILE * 128) >> 4) + 2 * k,
+                      idesc<TILE, false>(), d || k);
+          tc::umma_commit(k_free(s));
+          tc::umma_commit(s_full(s));
         }
-        tc::umma_commit(k_free(s));
-        tc::umma_commit(s_full(s));
         return true;
       };
-      bool ok = wait(q_full, 0, stop) && scores(0);
+      bool ok = ready(q_tmem, 0) && scores(0);
+#pragma unroll 1
       for (int j = 0; ok && j < tiles; ++j) {
         const int s = j & 1;
         if (j + 1 < tiles) ok = scores(j + 1);
-        ok = ok && wait(p_full, j & 1, stop) && wait(v_full(s), (j >> 1) & 1, stop);
+        ok = ok && ready(p_full(s), (j >> 1) & 1) && ready(v_full(s), (j >> 1) & 1);
         if (!ok) break;
-        tc::tc_fence_after();
-        const uint64_t pd = tc::sw128_desc(sm + C::p);
+        const uint64_t pd = tc::sw128_desc(sm + C::p + s * C::P);
         const uint64_t vd = mn_desc(sm + C::v + s * C::KV);
+        if (lead) {
 #pragma unroll
-        for (int k = 0; k < TILE / 16; ++k)  // 16 positions: 32 bytes of P's line, two groups of 8 rows of V
-          tc::umma_bf16(tmem + C::o_col, pd + 2 * k, vd + (2048 >> 4) * k, idesc<D, true>(), j || k);
-        tc::umma_commit(v_free(s));
-        tc::umma_commit(o_done);
+          for (int k = 0; k < TILE / 16; ++k)  // 16 positions: 32 bytes of P's line, two groups of 8 rows of V
+            tc::umma_bf16(tmem + C::o_col, pd + 2 * k, vd + (2048 >> 4) * k, idesc<D, true>(), j || k);
+          tc::umma_commit(v_free(s));
+          tc::umma_commit(p_free(s));
+          tc::umma_commit(o_done);
+        }
       }
       if (!ok) {  // let the products issued so far end before TMEM goes back
-        tc::umma_commit(drained);
+        if (lead) tc::umma_commit(drained);
         for (uint32_t i = 0; i < kPolls && !tc::mbar_try_wait(drained, 0); ++i) {}
       }
     }
@@ -1175,7 +1398,7 @@ Kv8Layout kv8_layout(bool cc, int B, int T, int hq, int hkv, int D, int max_seq_
   Kv8Layout L;
   const int64_t total = (int64_t)(hq / hkv) * T;
   L.cc = cc;
-  L.rows = cc ? kCcRows : total > kManyFrom ? many::ROWS : total > 8 ? 16 : 8;
+  L.rows = cc ? kCcRows : total > (getenv("KMANY") ? atoi(getenv("KMANY")) : 16) ? many::ROWS : total > 8 ? 16 : 8;
   // Few rows: 256 positions keep a short context's CTAs many (one sequence of 8192 positions, one KV head: 11.9 us
   // against 18.7 us at 1024); where there is work for every SM either way, 1024 positions cost fewer prologues and
   // partials (8 sequences, 16 heads, up to 4096 positions: 38.1 against 43.2 us).  The rule goes by the sequences,
@@ -1231,9 +1454,9 @@ int launch_few(cudaStream_t st, const Kv8Attn& a, int B) {
   return a.nsplit == 1 ? SSD_OK : launch_join<bf16, D, 8 * NT, true>(st, a, B);
 }
 
-template <int D>
+template <int D, bool UNI>
 int launch_many(cudaStream_t st, const Kv8Attn& a, int B) {
-  auto kern = many::kv8_attention_many_kernel<D>;
+  auto kern = many::kv8_attention_many_kernel<D, UNI>;
   constexpr size_t smem = many::Cfg<D>::smem;
   static_assert(smem <= 227 * 1024);
   static std::atomic<uint64_t> ready{0};
@@ -1244,7 +1467,7 @@ int launch_many(cudaStream_t st, const Kv8Attn& a, int B) {
 
 template <int D>
 int launch_bf16(cudaStream_t st, const Kv8Attn& a, const Kv8Layout& L, int B) {
-  if (L.rows == many::ROWS) return launch_many<D>(st, a, B);
+  if (L.rows == many::ROWS) return a.c.block_size % 16 == 0 ? launch_many<D, true>(st, a, B) : launch_many<D, false>(st, a, B);
   if (a.c.block_size % 16 == 0) return L.rows == 8 ? launch_few<D, 1, true>(st, a, B) : launch_few<D, 2, true>(st, a, B);
   return L.rows == 8 ? launch_few<D, 1, false>(st, a, B) : launch_few<D, 2, false>(st, a, B);
 }
