@@ -295,6 +295,9 @@ __device__ __forceinline__ uint32_t clear_nan(uint32_t w) { return w & ~((nan_ma
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool there) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
 }
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, bool there) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(there ? 4 : 0) : "memory");
+}
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
@@ -749,8 +752,14 @@ constexpr uint32_t kPolls = 1u << 24;
 template <int D>
 struct Cfg {
   static constexpr uint32_t Q = ROWS * D * 2, KV = TILE * D * 2, P = ROWS * TILE * 2;
-  static constexpr uint32_t q = 0, k = Q, v = k + 2 * KV, p = v + 2 * KV;
-  static constexpr uint32_t meta = p + 2 * P, qs = meta + META * TILE * 4, bars = qs + ROWS * 4;
+  static constexpr int RS = D == 256 ? 2 : 4;  // tiles of page bytes on their way
+  static constexpr uint32_t RAW = TILE * D;     // one plane of a tile, as stored
+  // Q passes through V's tiles on its way to TMEM; the result leaves through K's and V's
+  static_assert(Q <= 2 * KV && ROWS * D * 4 <= 4 * KV);
+  static constexpr uint32_t SC = TILE * 4;      // its scales: a position's (or, UNI, one of eight positions')
+  static constexpr uint32_t k = 0, v = 2 * KV, q = v, p = v + 2 * KV, raw = p + P, rsc = raw + RS * 2 * RAW;
+  static constexpr uint32_t pairs = rsc + RS * 2 * SC;
+  static constexpr uint32_t meta = pairs + 2 * 2 * ROWS * 8, qs = meta + META * TILE * 4, bars = qs + ROWS * 4;
   static constexpr size_t smem = 1024 + bars + 192;  // 22 barriers, TMEM address, two flags
   // TMEM columns: two tiles' scores, Q (two f16 to a column), O
   static constexpr uint32_t q_col = 2 * TILE, o_col = q_col + D / 2, tmem_cols = D == 64 ? 256 : 512;
@@ -768,6 +777,23 @@ __device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile int
   }
   *stop = 1;
   return false;
+}
+
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("{.reg .b64 x, y, z; mov.b64 x, {%2, %3}; mov.b64 y, {%4, %5}; mov.b64 z, {%6, %7};\n\t"
+      "fma.rn.f32x2 x, x, y, z; mov.b64 {%0, %1}, x;}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 r;
+  asm("{.reg .b64 x, y; mov.b64 x, {%2, %3}; mov.b64 y, {%4, %5}; add.rn.f32x2 x, x, y; mov.b64 {%0, %1}, x;}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
 }
 
 // N fp32 columns of this warp's 32 TMEM lanes; the registers are valid once tmem_ready has seen them.
@@ -847,19 +873,14 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_many_kernel(const Kv
   uint32_t* meta = reinterpret_cast<uint32_t*>(gen + C::meta);  // [META][TILE], see pack_meta
   float* qs_s = reinterpret_cast<float*>(gen + C::qs);
   auto bar = [&](int i) { return sm + C::bars + 8 * i; };
-  const uint32_t q_full = bar(0), o_done = bar(1), drained = bar(2);
-  auto p_full = [&](int s) { return bar(3 + s); };
-  auto p_free = [&](int s) { return bar(5 + s); };
+  const uint32_t q_full = bar(0), o_done = bar(1), drained = bar(2), p_full = bar(3), q_tmem = bar(4);
   auto k_full = [&](int s) { return bar(7 + s); };
   auto k_free = [&](int s) { return bar(9 + s); };
   auto v_full = [&](int s) { return bar(11 + s); };
   auto v_free = [&](int s) { return bar(13 + s); };
   auto s_full = [&](int s) { return bar(15 + s); };
-  const uint32_t q_tmem = bar(17);
   auto pair = [&](int q) { return bar(18 + q); };
-  // [tile parity][half][row]: the threads' maxima, where Q was (every row thread has moved its part on before the
-  // first scores come; the result is staged there after the last product, hence after the last swap)
-  float2* pair_s = reinterpret_cast<float2*>(gen + C::q);
+  float2* pair_s = reinterpret_cast<float2*>(gen + C::pairs);  // [tile parity][half][row]: the threads' maxima
   uint32_t* slot = reinterpret_cast<uint32_t*>(gen + C::bars + 176);
   volatile int* stop = reinterpret_cast<volatile int*>(slot + 1);
   volatile int* nan_seen = reinterpret_cast<volatile int*>(slot + 2);
@@ -870,12 +891,11 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_many_kernel(const Kv
   if (tid == 0) {
     tc::mbar_init(q_full, SOFT + CONV);
     tc::mbar_init(q_tmem, SOFT);
+    tc::mbar_init(p_full, SOFT);
     tc::mbar_init(o_done, 1);
     tc::mbar_init(drained, 1);
     for (int q = 0; q < 4; ++q) tc::mbar_init(pair(q), 64);
     for (int s = 0; s < 2; ++s) {
-      tc::mbar_init(p_full(s), SOFT);
-      tc::mbar_init(p_free(s), 1);
       tc::mbar_init(k_full(s), CONV);
       tc::mbar_init(k_free(s), 1);
       tc::mbar_init(v_full(s), CONV);
@@ -951,13 +971,13 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_many_kernel(const Kv
         for (int x = 1; x < LPR; x <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, x));
       }
       const int e = min(max((int)(top >> 7) - 127, -118), 120);
-      const float inv = exp2i(-e);
+      const float inv = copysignf(exp2i(-e), a.scale);  // the row's factor below is never negative
       uint32_t y[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j)
         y[j] = pack_f16(__uint_as_float(v[j] << 16) * inv, __uint_as_float(v[j] & 0xffff0000u) * inv);
       sts128(at, make_uint4(y[0], y[1], y[2], y[3]));
-      if (pc == 0) qs_s[r] = exp2i(e) * a.scale * 1.4426950408889634f;
+      if (pc == 0) qs_s[r] = exp2i(e) * fabsf(a.scale) * 1.4426950408889634f;
     }
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     tc::mbar_arrive(q_full);
@@ -972,41 +992,78 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_many_kernel(const Kv
   const uint8_t* kp = a.c.pages + a.c.layer + (int64_t)head * D + pc * 16;
   const float* sc = a.c.scales + a.c.scale_layer + head;
   const int64_t rs = (int64_t)a.c.hkv * D;
-  uint4 kb[NI], vb[NI];
-  float ks[NB], vs[NB];  // scales (ks < 0: no row); UNI: the eight positions lie in one page
+  constexpr int RS = C::RS;
   int blk[NB], off[NB];  // of the tile to be fetched next
+  const uint32_t raw8 = sm + C::raw + cw * (NI * 512) + lane * 16;  // this lane's pieces of a plane, 512 bytes apart
+  int ids = -1;          // UNI: lane x has the block id of the warp's positions in tile 32 k + x
   auto look = [&](int j) {
+    if constexpr (UNI) {
+      if ((j & 31) == 0) {
+        const int p = (j + lane) * TILE + 8 * cw;
+        ids = p < kn ? ld_act(table + (base + p) / a.c.block_size) : -1;
+      }
+      blk[0] = __shfl_sync(0xffffffffu, ids, j & 31);
+      if (j == 0) {
+        off[0] = (base + 8 * cw) % a.c.block_size;
+      } else {
+        off[0] += TILE % a.c.block_size;
+        if (off[0] >= a.c.block_size) off[0] -= a.c.block_size;
+      }
+    } else {
 #pragma unroll
-    for (int i = 0; i < NB; ++i) {
-      const int p = j * TILE + 8 * cw + (UNI ? 0 : rr + i * RPI);
-      blk[i] = -1;
-      off[i] = 0;
-      if (p < kn) {
-        const int page = (base + p) / a.c.block_size;
-        blk[i] = ld_act(table + page);
-        off[i] = base + p - page * a.c.block_size;
+      for (int i = 0; i < NB; ++i) {
+        const int p = j * TILE + 8 * cw + rr + i * RPI;
+        blk[i] = -1;
+        off[i] = 0;
+        if (p < kn) {
+          const int page = (base + p) / a.c.block_size;
+          blk[i] = ld_act(table + page);
+          off[i] = base + p - page * a.c.block_size;
+        }
       }
     }
   };
-  // bytes of tile j's K (plane 0) or V rows into x, and the plane's scales
-  auto fetch = [&](int j, int64_t plane, int64_t scale_plane, uint4* x, float* xs) {
+  // start the copies of tile j's K (plane 0) or V rows and scales into its stage (zeros where there is no row)
+  auto fetch = [&](int j, int plane) {
+    const uint32_t to = raw8 + (j % RS * 2 + plane) * C::RAW;
+    const uint32_t sto = sm + C::rsc + (j % RS * 2 + plane) * C::SC + cw * 32;
+    const float* from = sc + plane * a.c.scale_plane;
+    if (UNI ? lane == 0 : pc == 0) {
 #pragma unroll
-    for (int i = 0; i < NB; ++i)
-      xs[i] = (unsigned)blk[i] < (unsigned)a.c.num_blocks ? ld_act(sc + scale_plane + (int64_t)blk[i] * a.c.hkv) : -1.f;
-#pragma unroll
-    for (int i = 0; i < NI; ++i) {
-      const int n = UNI ? 0 : i;
-      x[i] = make_uint4(0, 0, 0, 0);
-      if ((unsigned)blk[n] < (unsigned)a.c.num_blocks && (!UNI || j * TILE + 8 * cw + rr + i * RPI < kn))
-        x[i] = ld_act_v4(kp + plane + ((int64_t)blk[n] * a.c.block_size + off[n] + (UNI ? rr + i * RPI : 0)) * rs);
+      for (int i = 0; i < NB; ++i) {
+        const bool there = (unsigned)blk[i] < (unsigned)a.c.num_blocks;
+        cp_async4(sto + (UNI ? 0 : rr + i * RPI) * 4, from + (there ? (int64_t)blk[i] * a.c.hkv : 0), there);
+      }
     }
+    if constexpr (UNI) {
+      const bool in = (unsigned)blk[0] < (unsigned)a.c.num_blocks;
+      const uint8_t* s = kp + plane * a.c.plane + (in ? ((int64_t)blk[0] * a.c.block_size + off[0] + rr) * rs : 0);
+      const int left = in ? kn - j * TILE - 8 * cw - rr : 0;  // row i of the lane is there where i RPI < left
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+        cp_async16(to + i * 512, s, i * RPI < left);
+        if (i * RPI + RPI < left) s += RPI * rs;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+        const int n = i % NB;
+        const bool there = (unsigned)blk[n] < (unsigned)a.c.num_blocks;
+        const int64_t row = there ? (int64_t)blk[n] * a.c.block_size + off[n] : 0;
+        cp_async16(to + i * 512, kp + plane * a.c.plane + row * rs, there);
+      }
+    }
+    cp_async_commit();
   };
   if (tiles > 0 && warp < (SOFT + CONV) / 32) {
     if (warp >= SOFT / 32) {
-      look(0);
-      fetch(0, 0, 0, kb, ks);
-      fetch(0, a.c.plane, a.c.scale_plane, vb, vs);
-      look(1);
+#pragma unroll
+      for (int j = 0; j < RS; ++j) {
+        look(j);
+        fetch(j, 0);
+        fetch(j, 1);
+      }
+      look(RS);
     }
     load_q();
   }
@@ -1041,7 +1098,6 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_many_kernel(const Kv
       qs = qs_s[r];
       if (qs == 0.f) qs = 1e-38f;  // keeps the mask's infinity out of 0 * infinity; the scores stay below 2^-60
     }
-    const float hidden = qs > 0.f ? -INFINITY : INFINITY;
     // M: what the weights are relative to, N: what l is; -1e38 where nothing has been seen
     float M = -1e38f, N = -1e38f, l = 0.f, vtop = -1000.f;
     // The row's two threads swap a pair of numbers; false when the CTA gives up.  `k`: how many swaps went before.
@@ -1089,14 +1145,16 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_many_kernel(const Kv
           if (!inb) keep &= 0x0000ffffu;
 #pragma unroll
           for (int i = 0; i < 32; ++i)
-            if (!(keep >> i & 1)) x[i] = __float_as_uint(hidden);
+            if (!(keep >> i & 1)) x[i] = 0xff800000u;
         }
-        float ya = -1e38f, yb = -1e38f;
+        float ya = -INFINITY, yb = -INFINITY;  // of the raw products: their factors are positive
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          ya = fmaxf(ya, __uint_as_float(x[i]) * ca);
-          yb = fmaxf(yb, __uint_as_float(x[16 + i]) * cb);
+        for (int i = 0; i < 16; i += 2) {
+          ya = fmaxf(ya, fmaxf(__uint_as_float(x[i]), __uint_as_float(x[i + 1])));
+          yb = fmaxf(yb, fmaxf(__uint_as_float(x[16 + i]), __uint_as_float(x[17 + i])));
         }
+        ya = fmaxf(ya * ca, -1e38f);
+        yb = fmaxf(yb * cb, -1e38f);
         n = fmaxf(ya, yb);
         m = fmaxf(ya + va, yb + vb2);
       } else {
@@ -1134,23 +1192,23 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_many_kernel(const Kv
           for (int i = 0; i < 32; ++i) l += ex2(fmaf(__uint_as_float(x[i]), i < 16 ? ca : cb, -N));
         }
         const float oa = va - M, ob = vb2 - M;
-        float sa[2] = {0.f, 0.f}, sb[2] = {0.f, 0.f};
+        float2 sa = make_float2(0.f, 0.f), sb = sa;
+        const float2 ca2 = make_float2(ca, ca), cb2 = make_float2(cb, cb);
+        const float2 oa2 = make_float2(oa, oa), ob2 = make_float2(ob, ob);
 #pragma unroll
         for (int i = 0; i < 16; i += 2) {
-          float e[4];
-#pragma unroll
-          for (int z = 0; z < 2; ++z) {
-            e[z] = ex2(fmaf(__uint_as_float(x[i + z]), ca, oa));
-            e[2 + z] = ex2(fmaf(__uint_as_float(x[16 + i + z]), cb, ob));
-            sa[z] += e[z];
-            sb[z] += e[2 + z];
-          }
-          w[i / 2] = pack_f16(e[0], e[1]);
-          w[8 + i / 2] = pack_f16(e[2], e[3]);
+          float2 e = fma2(make_float2(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), ca2, oa2);
+          float2 d = fma2(make_float2(__uint_as_float(x[16 + i]), __uint_as_float(x[17 + i])), cb2, ob2);
+          e = make_float2(ex2(e.x), ex2(e.y));
+          d = make_float2(ex2(d.x), ex2(d.y));
+          sa = add2(sa, e);
+          sb = add2(sb, d);
+          w[i / 2] = pack_f16(e.x, e.y);
+          w[8 + i / 2] = pack_f16(d.x, d.y);
         }
         if (!wide) {
-          l = fmaf(sa[0] + sa[1], ex2(-oa - N), l);
-          l = fmaf(sb[0] + sb[1], ex2(-ob - N), l);
+          l = fmaf(sa.x + sa.y, ex2(-oa - N), l);
+          l = fmaf(sb.x + sb.y, ex2(-ob - N), l);
         }
       } else {
 #pragma unroll
@@ -1160,16 +1218,16 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_many_kernel(const Kv
           l += ex2(s0 - N) + ex2(s1 - N);
         }
       }
-      if (j >= 2) ok = __all_sync(0xffffffffu, wait(p_free(j & 1), ((j >> 1) - 1) & 1, stop));
-      if (!ok) break;
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        sts128(piece(sm + C::p + (j & 1) * C::P, ROWS, r, 4 * half + i),
-               make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]));
-      if (j > 0 && __any_sync(0xffffffffu, f != 1.f)) {  // O, once the tile before has been added; half of it each
+      if (j > 0) {  // the tile before has been added: its weights may go, and O may be rescaled
         ok = __all_sync(0xffffffffu, wait(o_done, (j - 1) & 1, stop));
         if (!ok) break;
         tc::tc_fence_after();
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        sts128(piece(sm + C::p, ROWS, r, 4 * half + i),
+               make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]));
+      if (j > 0 && __any_sync(0xffffffffu, f != 1.f)) {  // half of O each
 #pragma unroll 1
         for (int c = half * (D / 2); c < (half + 1) * (D / 2); c += 32) {
           uint32_t y[32];
@@ -1183,13 +1241,13 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_many_kernel(const Kv
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       tc::tc_fence_before();
-      tc::mbar_arrive(p_full(j & 1));
+      tc::mbar_arrive(p_full);
     }
     if (ok && tiles > 0) {
-      ok = __all_sync(0xffffffffu, wait(o_done, (tiles - 1) & 1, stop));
       float lo = l, unused = 0.f;
-      ok = ok && swap(reinterpret_cast<float2*>(gen + C::p), tiles, lo, unused);
+      ok = swap(pair_s, tiles, lo, unused);
       l += lo;
+      ok = __all_sync(0xffffffffu, ok && wait(o_done, (tiles - 1) & 1, stop));
     }
     tc::tc_fence_after();
     if (!ok) l = __int_as_float(0x7fc00000);
@@ -1280,22 +1338,29 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_many_kernel(const Kv
 #pragma unroll 1
     for (int j = 0; j < tiles; ++j) {
       const int s = j & 1;
+      const uint32_t from = raw8 + (j % RS) * (2 * C::RAW);
       if (j >= 2 && !wait(k_free(s), ((j >> 1) - 1) & 1, stop)) break;
+      cp_async_wait<2 * RS - 2>();  // K and V of this tile; a lane reads what it has copied itself
       uint32_t* mt = meta + (j % META) * TILE;
-      if constexpr (UNI) {
-        if (lane == 0) mt[cw] = ks[0] < 0.f ? 0u : pack_meta(scale_exponent(ks[0]), scale_exponent(vs[0]));
+      const float* ksc = reinterpret_cast<const float*>(gen + C::rsc + (j % RS * 2) * C::SC + cw * 32);
+      if (UNI ? lane == 0 : pc == 0) {
+#pragma unroll
+        for (int i = 0; i < NB; ++i) {
+          const int r = UNI ? 0 : rr + i * RPI;
+          const float x = ksc[r], y = ksc[C::SC / 4 + r];
+          mt[UNI ? cw : 8 * cw + r] = x == 0.f ? 0u : pack_meta(scale_exponent(x), scale_exponent(y));
+        }
       }
 #pragma unroll
-      for (int i = 0; i < NI; ++i) {
-        if (!UNI && pc == 0)
-          mt[8 * cw + rr + i * RPI] =
-              ks[i % NB] < 0.f ? 0u : pack_meta(scale_exponent(ks[i % NB]), scale_exponent(vs[i % NB]));
-        put(sm + C::k + s * C::KV, i, kb[i]);
-      }
+      for (int i = 0; i < NI; ++i) put(sm + C::k + s * C::KV, i, lds128(from + i * 512));
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       tc::mbar_arrive(k_full(s));
-      fetch(j + 1, 0, 0, kb, ks);
+      fetch(j + RS, 0);
+      if (j == 0 && !wait(q_tmem, 0, stop)) break;  // V's tiles hold Q until then
       if (j >= 2 && !wait(v_free(s), ((j >> 1) - 1) & 1, stop)) break;
+      uint4 vb[NI];
+#pragma unroll
+      for (int i = 0; i < NI; ++i) vb[i] = lds128(from + C::RAW + i * 512);
       if (base + j * TILE + 8 * cw + 7 > kmin) {  // NaN of positions that some row does not see: put back by row above
         uint32_t marks = 0;
 #pragma unroll
@@ -1314,9 +1379,10 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_many_kernel(const Kv
       for (int i = 0; i < NI; ++i) put(sm + C::v + s * C::KV, i, vb[i]);
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       tc::mbar_arrive(v_full(s));
-      fetch(j + 1, a.c.plane, a.c.scale_plane, vb, vs);
-      look(j + 2);
+      fetch(j + RS, 1);
+      look(j + RS + 1);
     }
+    cp_async_wait<0>();
     __syncwarp();
   } else {
     // -------------------------------------------------------------- products
@@ -1352,16 +1418,15 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_many_kernel(const Kv
       for (int j = 0; ok && j < tiles; ++j) {
         const int s = j & 1;
         if (j + 1 < tiles) ok = scores(j + 1);
-        ok = ok && ready(p_full(s), (j >> 1) & 1) && ready(v_full(s), (j >> 1) & 1);
+        ok = ok && ready(p_full, j & 1) && ready(v_full(s), (j >> 1) & 1);
         if (!ok) break;
-        const uint64_t pd = tc::sw128_desc(sm + C::p + s * C::P);
+        const uint64_t pd = tc::sw128_desc(sm + C::p);
         const uint64_t vd = mn_desc(sm + C::v + s * C::KV);
         if (lead) {
 #pragma unroll
           for (int k = 0; k < TILE / 16; ++k)  // 16 positions: 32 bytes of P's line, two groups of 8 rows of V
             tc::umma_bf16(tmem + C::o_col, pd + 2 * k, vd + (2048 >> 4) * k, idesc<D, true>(), j || k);
           tc::umma_commit(v_free(s));
-          tc::umma_commit(p_free(s));
           tc::umma_commit(o_done);
         }
       }
