@@ -735,7 +735,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, NT == 1 ? 3 : 2) kv8_attention
 //   warps 0-7   two threads a query row, half a tile's positions each: scores out of TMEM, maxima (exchanged between
 //               the two), weights, rescaling of O (only when a row's reference has to move, see the few-row
 //               kernel), the result
-//   warps 8-15  pages to f16 tiles, the next tile's bytes in flight while this one is converted
+//   warps 8-15  pages to f16 tiles, four warps a tile in turn, the bytes of the next two tiles in flight
 //   warp 16     issues the products: S of tile j + 1 goes before O of tile j, so the weights of one tile are
 //               made while the tensor cores work on the next
 // All waits are bounded: a CTA that gives up lets its copies and products end and writes NaN.
@@ -751,15 +751,17 @@ constexpr uint32_t kPolls = 1u << 24;
 
 template <int D>
 struct Cfg {
-  static constexpr uint32_t Q = ROWS * D * 2, KV = TILE * D * 2, P = ROWS * TILE * 2;
-  static constexpr int RS = D == 256 ? 2 : 4;  // tiles of page bytes on their way
+  static constexpr uint32_t KV = TILE * D * 2, P = ROWS * TILE * 2;
   static constexpr uint32_t RAW = TILE * D;     // one plane of a tile, as stored
-  // Q passes through V's tiles on its way to TMEM; the result leaves through K's and V's
-  static_assert(Q <= 2 * KV && ROWS * D * 4 <= 4 * KV);
+  static constexpr uint32_t PITCH = D * 4 + 16;  // bytes of a row of the result, which leaves through K, V and P
+  static_assert(ROWS * PITCH <= 4 * KV + P);
+  // Q comes in through V and P, rows QPITCH bytes apart
+  static constexpr uint32_t QPITCH = D * 2 + 16;
+  static_assert(ROWS * QPITCH <= 2 * KV + P);
   static constexpr uint32_t SC = TILE * 4;      // its scales: a position's (or, UNI, one of eight positions')
-  static constexpr uint32_t k = 0, v = 2 * KV, q = v, p = v + 2 * KV, raw = p + P, rsc = raw + RS * 2 * RAW;
-  static constexpr uint32_t pairs = rsc + RS * 2 * SC;
-  static constexpr uint32_t meta = pairs + 2 * 2 * ROWS * 8, qs = meta + META * TILE * 4, bars = qs + ROWS * 4;
+  static constexpr uint32_t k = 0, v = 2 * KV, p = v + 2 * KV, raw = p + P, rsc = raw + 2 * 2 * RAW;
+  static constexpr uint32_t pairs = rsc + 2 * 2 * SC;
+  static constexpr uint32_t meta = pairs + 2 * 2 * ROWS * 8, bars = meta + META * TILE * 4;
   static constexpr size_t smem = 1024 + bars + 192;  // 22 barriers, TMEM address, two flags
   // TMEM columns: two tiles' scores, Q (two f16 to a column), O
   static constexpr uint32_t q_col = 2 * TILE, o_col = q_col + D / 2, tmem_cols = D == 64 ? 256 : 512;
@@ -871,9 +873,8 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_many_kernel(const Kv
   const uint32_t raw = tc::smem_u32(smem_raw), sm = (raw + 1023u) & ~1023u;
   uint8_t* gen = smem_raw + (sm - raw);
   uint32_t* meta = reinterpret_cast<uint32_t*>(gen + C::meta);  // [META][TILE], see pack_meta
-  float* qs_s = reinterpret_cast<float*>(gen + C::qs);
   auto bar = [&](int i) { return sm + C::bars + 8 * i; };
-  const uint32_t q_full = bar(0), o_done = bar(1), drained = bar(2), p_full = bar(3), q_tmem = bar(4);
+  const uint32_t q_in = bar(0), o_done = bar(1), drained = bar(2), p_full = bar(3), q_tmem = bar(4);
   auto k_full = [&](int s) { return bar(7 + s); };
   auto k_free = [&](int s) { return bar(9 + s); };
   auto v_full = [&](int s) { return bar(11 + s); };
@@ -889,16 +890,16 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_many_kernel(const Kv
   const int split = blockIdx.x, b = blockIdx.z;
   const int head = blockIdx.y / a.row_groups, rg = blockIdx.y % a.row_groups;
   if (tid == 0) {
-    tc::mbar_init(q_full, SOFT + CONV);
+    tc::mbar_init(q_in, ROWS);
     tc::mbar_init(q_tmem, SOFT);
     tc::mbar_init(p_full, SOFT);
     tc::mbar_init(o_done, 1);
     tc::mbar_init(drained, 1);
     for (int q = 0; q < 4; ++q) tc::mbar_init(pair(q), 64);
     for (int s = 0; s < 2; ++s) {
-      tc::mbar_init(k_full(s), CONV);
+      tc::mbar_init(k_full(s), CONV / 2);
       tc::mbar_init(k_free(s), 1);
-      tc::mbar_init(v_full(s), CONV);
+      tc::mbar_init(v_full(s), CONV / 2);
       tc::mbar_init(v_free(s), 1);
       tc::mbar_init(s_full(s), 1);
     }
@@ -931,143 +932,6 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_many_kernel(const Kv
   const int tiles = kn > 0 ? (kn + TILE - 1) / TILE : 0;
   const int32_t* table = a.tables + (int64_t)b * a.max_blocks;
 
-  // Q: raw rows into place (cp.async), then f16 under a power of two per row, in place; a lane converts the pieces
-  // it has copied.  By the row and the converting warps, STEP rows at a time.
-  auto load_q = [&]() {
-    constexpr int LPR = D / 8, RPW = 32 / LPR, STEP = (SOFT + CONV) / 32 * RPW;
-    static_assert(ROWS % STEP == 0);
-    const int first = warp * RPW + lane / LPR, pc = lane % LPR, dt = STEP / a.G, dg = STEP - dt * a.G;
-    int t = (row0 + first) / a.G, g = row0 + first - t * a.G;
-#pragma unroll 4
-    for (int r = first; r < ROWS; r += STEP) {
-      const bool there = r < rows && t < ql;
-      const bf16* src = reinterpret_cast<const bf16*>(a.q) +
-                        (there ? (((int64_t)b * a.T + t) * a.hq + head * a.G + g) * D + pc * 8 : 0);
-      cp_async16(piece(sm + C::q, ROWS, r, pc), src, there);
-      t += dt;
-      g += dg;
-      if (g >= a.G) {
-        g -= a.G;
-        ++t;
-      }
-    }
-    cp_async_commit();
-    cp_async_wait<0>();
-#pragma unroll 4
-    for (int r = first; r < ROWS; r += STEP) {  // STEP divides ROWS: every lane of a warp makes the same rounds
-      const uint32_t at = piece(sm + C::q, ROWS, r, pc);
-      const uint4 w = lds128(at);
-      // largest magnitude of the row, as bf16 bits (infinities and NaN end in NaN scores of the row)
-      const uint32_t v[4] = {w.x, w.y, w.z, w.w};
-      __nv_bfloat162 t2 = __float2bfloat162_rn(0.f);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) t2 = __hmax2(t2, __habs2(*reinterpret_cast<const __nv_bfloat162*>(&v[j])));
-      const uint32_t both = *reinterpret_cast<const uint32_t*>(&t2);
-      uint32_t top = max(both >> 16, both & 0xffffu);
-      if constexpr (LPR == 32) {
-        top = __reduce_max_sync(0xffffffffu, top);
-      } else {
-#pragma unroll
-        for (int x = 1; x < LPR; x <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, x));
-      }
-      const int e = min(max((int)(top >> 7) - 127, -118), 120);
-      const float inv = copysignf(exp2i(-e), a.scale);  // the row's factor below is never negative
-      uint32_t y[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        y[j] = pack_f16(__uint_as_float(v[j] << 16) * inv, __uint_as_float(v[j] & 0xffff0000u) * inv);
-      sts128(at, make_uint4(y[0], y[1], y[2], y[3]));
-      if (pc == 0) qs_s[r] = exp2i(e) * fabsf(a.scale) * 1.4426950408889634f;
-    }
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    tc::mbar_arrive(q_full);
-  };
-
-  // Converting warps: one takes 8 positions of a tile, RPI of them at a time, 16 dims a lane, eight lanes on four
-  // pieces of an even and an odd row (their 16-byte stores then meet no bank twice).  Block ids are read two tiles
-  // ahead, bytes one tile ahead, the first ones before Q.
-  constexpr int PCS = D / 16, RPI = 32 / PCS, NI = 8 / RPI, NB = UNI ? 1 : NI;
-  const int cw = warp - SOFT / 32;
-  const int rr = ((lane >> 2) & 1) | ((lane >> 3) / (PCS / 4)) << 1, pc = (lane & 3) | ((lane >> 3) % (PCS / 4)) << 2;
-  const uint8_t* kp = a.c.pages + a.c.layer + (int64_t)head * D + pc * 16;
-  const float* sc = a.c.scales + a.c.scale_layer + head;
-  const int64_t rs = (int64_t)a.c.hkv * D;
-  constexpr int RS = C::RS;
-  int blk[NB], off[NB];  // of the tile to be fetched next
-  const uint32_t raw8 = sm + C::raw + cw * (NI * 512) + lane * 16;  // this lane's pieces of a plane, 512 bytes apart
-  int ids = -1;          // UNI: lane x has the block id of the warp's positions in tile 32 k + x
-  auto look = [&](int j) {
-    if constexpr (UNI) {
-      if ((j & 31) == 0) {
-        const int p = (j + lane) * TILE + 8 * cw;
-        ids = p < kn ? ld_act(table + (base + p) / a.c.block_size) : -1;
-      }
-      blk[0] = __shfl_sync(0xffffffffu, ids, j & 31);
-      if (j == 0) {
-        off[0] = (base + 8 * cw) % a.c.block_size;
-      } else {
-        off[0] += TILE % a.c.block_size;
-        if (off[0] >= a.c.block_size) off[0] -= a.c.block_size;
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < NB; ++i) {
-        const int p = j * TILE + 8 * cw + rr + i * RPI;
-        blk[i] = -1;
-        off[i] = 0;
-        if (p < kn) {
-          const int page = (base + p) / a.c.block_size;
-          blk[i] = ld_act(table + page);
-          off[i] = base + p - page * a.c.block_size;
-        }
-      }
-    }
-  };
-  // start the copies of tile j's K (plane 0) or V rows and scales into its stage (zeros where there is no row)
-  auto fetch = [&](int j, int plane) {
-    const uint32_t to = raw8 + (j % RS * 2 + plane) * C::RAW;
-    const uint32_t sto = sm + C::rsc + (j % RS * 2 + plane) * C::SC + cw * 32;
-    const float* from = sc + plane * a.c.scale_plane;
-    if (UNI ? lane == 0 : pc == 0) {
-#pragma unroll
-      for (int i = 0; i < NB; ++i) {
-        const bool there = (unsigned)blk[i] < (unsigned)a.c.num_blocks;
-        cp_async4(sto + (UNI ? 0 : rr + i * RPI) * 4, from + (there ? (int64_t)blk[i] * a.c.hkv : 0), there);
-      }
-    }
-    if constexpr (UNI) {
-      const bool in = (unsigned)blk[0] < (unsigned)a.c.num_blocks;
-      const uint8_t* s = kp + plane * a.c.plane + (in ? ((int64_t)blk[0] * a.c.block_size + off[0] + rr) * rs : 0);
-      const int left = in ? kn - j * TILE - 8 * cw - rr : 0;  // row i of the lane is there where i RPI < left
-#pragma unroll
-      for (int i = 0; i < NI; ++i) {
-        cp_async16(to + i * 512, s, i * RPI < left);
-        if (i * RPI + RPI < left) s += RPI * rs;
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < NI; ++i) {
-        const int n = i % NB;
-        const bool there = (unsigned)blk[n] < (unsigned)a.c.num_blocks;
-        const int64_t row = there ? (int64_t)blk[n] * a.c.block_size + off[n] : 0;
-        cp_async16(to + i * 512, kp + plane * a.c.plane + row * rs, there);
-      }
-    }
-    cp_async_commit();
-  };
-  if (tiles > 0 && warp < (SOFT + CONV) / 32) {
-    if (warp >= SOFT / 32) {
-#pragma unroll
-      for (int j = 0; j < RS; ++j) {
-        look(j);
-        fetch(j, 0);
-        fetch(j, 1);
-      }
-      look(RS);
-    }
-    load_q();
-  }
-
   if (warp < SOFT / 32) {
     // -------------------------------------------------------------- rows
     const int quad = warp & 3, half = warp >> 2;  // TMEM lanes 32 quad .., positions 32 half .. of a tile
@@ -1076,30 +940,6 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_many_kernel(const Kv
     const int pos = real ? n0 + t : -1;
     const int64_t at = (((int64_t)b * a.T + t) * a.hq + head * a.G + g) * D;
     const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16);
-    float qs = 1.f;
-    bool ok = true;
-    if (tiles > 0) {
-      ok = __all_sync(0xffffffffu, wait(q_full, 0, stop));
-      // Q goes on to TMEM as the first operand: read from shared memory it would cost S more of that memory's
-      // bandwidth than K does
-#pragma unroll 1
-      for (int c = half * (D / 4); c < (half + 1) * (D / 4); c += 16) {
-        uint32_t y[16];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint4 z = lds128(piece(sm + C::q, ROWS, r, c / 4 + i));
-          y[4 * i] = z.x; y[4 * i + 1] = z.y; y[4 * i + 2] = z.z; y[4 * i + 3] = z.w;
-        }
-        tmem_store16(lanes + C::q_col + c, y);
-      }
-      asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-      tc::tc_fence_before();
-      tc::mbar_arrive(q_tmem);
-      qs = qs_s[r];
-      if (qs == 0.f) qs = 1e-38f;  // keeps the mask's infinity out of 0 * infinity; the scores stay below 2^-60
-    }
-    // M: what the weights are relative to, N: what l is; -1e38 where nothing has been seen
-    float M = -1e38f, N = -1e38f, l = 0.f, vtop = -1000.f;
     // The row's two threads swap a pair of numbers; false when the CTA gives up.  `k`: how many swaps went before.
     auto swap = [&](float2* at2, int k, float& x, float& y) {
       at2[((k & 1) * 2 + half) * ROWS + r] = make_float2(x, y);
@@ -1110,13 +950,68 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_many_kernel(const Kv
       y = z.y;
       return true;
     };
+    float qs = 1.f;
+    bool ok = true;
+    if (tiles > 0) {
+      // Q: rows to shared memory by bulk copies, then this thread's half of its row, in f16 under a power of two of
+      // the row, into TMEM as the first operand (from shared memory it would cost S more of that memory's bandwidth
+      // than K does)
+      constexpr int NQ = D / 16;
+      const uint32_t row = sm + C::v + r * C::QPITCH;
+      if (half == 0) {
+        if (real) {
+          tc::mbar_expect_tx(q_in, D * 2);
+          asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(row),
+                       "l"(reinterpret_cast<const bf16*>(a.q) + at), "r"(D * 2), "r"(q_in)
+                       : "memory");
+        } else {
+          tc::mbar_arrive(q_in);
+        }
+      }
+      ok = __all_sync(0xffffffffu, wait(q_in, 0, stop));
+      uint4 w[NQ];
+#pragma unroll
+      for (int i = 0; i < NQ; ++i) w[i] = real && ok ? lds128(row + half * D + 16 * i) : make_uint4(0, 0, 0, 0);
+      __nv_bfloat162 t2 = __float2bfloat162_rn(0.f);
+#pragma unroll
+      for (int i = 0; i < NQ; ++i) {
+        const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&w[i]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) t2 = __hmax2(t2, __habs2(h[j]));
+      }
+      // largest magnitude (infinities and NaN end in NaN scores of the row)
+      float top = fmaxf(__low2float(t2), __high2float(t2)), other = top, unused = 0.f;
+      ok = ok && swap(pair_s, 0, other, unused);
+      top = fmaxf(top, other);
+      const int e = min(max((int)(__float_as_uint(top) >> 23) - 127, -118), 120);
+      const float inv = copysignf(exp2i(-e), a.scale);  // the row's factor is never negative
+      qs = exp2i(e) * fabsf(a.scale) * 1.4426950408889634f;
+      if (qs == 0.f) qs = 1e-38f;  // keeps the mask's infinity out of 0 * infinity; the scores stay below 2^-60
+#pragma unroll
+      for (int c = 0; c < NQ; c += 4) {
+        uint32_t y[16];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t v[4] = {w[c + i].x, w[c + i].y, w[c + i].z, w[c + i].w};
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            y[4 * i + j] = pack_f16(__uint_as_float(v[j] << 16) * inv, __uint_as_float(v[j] & 0xffff0000u) * inv);
+        }
+        tmem_store16(lanes + C::q_col + half * (D / 4) + 4 * c, y);
+      }
+      asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+      tc::tc_fence_before();
+      if (ok) tc::mbar_arrive(q_tmem);
+    }
+    // M: what the weights are relative to, N: what l is; -1e38 where nothing has been seen
+    float M = -1e38f, N = -1e38f, l = 0.f, vtop = -1000.f;
 #pragma unroll 1
     for (int j = 0; ok && j < tiles; ++j) {
       ok = __all_sync(0xffffffffu, wait(s_full(j & 1), (j >> 1) & 1, stop));
       if (!ok) break;
       tc::tc_fence_after();
       const int p0 = base + j * TILE + 32 * half;  // this thread's 32 positions
-      const uint32_t* mt = meta + (j % META) * TILE + half * (UNI ? 4 : 32);
+      const uint32_t* mt = meta + (j % META) * TILE + half * (UNI ? 2 : 32);
       uint32_t x[32];
       tmem_load32(lanes + (j & 1) * TILE + 32 * half, x);
       float m = -1e38f, n = -1e38f, f = 1.f;
@@ -1125,7 +1020,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_many_kernel(const Kv
       bool wide = false;
       if constexpr (UNI) {
         // two groups of 16 positions, one pair of scales each
-        uint32_t wa = mt[0], wb = mt[2];
+        uint32_t wa = mt[0], wb = mt[1];
         const bool ina = wa >= 65536u, inb = wb >= 65536u;
         if (!ina) wa = pack_meta(0, 0);
         if (!inb) wb = pack_meta(0, 0);
@@ -1173,7 +1068,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_many_kernel(const Kv
         }
       }
       float mo = m, no = n;
-      ok = swap(pair_s, j, mo, no);
+      ok = swap(pair_s, j + 1, mo, no);
       if (!ok) break;
       m = fmaxf(m, mo);
       n = fmaxf(n, no);
@@ -1245,7 +1140,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_many_kernel(const Kv
     }
     if (ok && tiles > 0) {
       float lo = l, unused = 0.f;
-      ok = swap(pair_s, tiles, lo, unused);
+      ok = swap(pair_s, tiles + 1, lo, unused);
       l += lo;
       ok = __all_sync(0xffffffffu, ok && wait(o_done, (tiles - 1) & 1, stop));
     }
@@ -1256,54 +1151,50 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_many_kernel(const Kv
     const bool any = real && l != 0.f;  // l is NaN, not 0, where a seen score is
     if (a.nsplit > 1 && half == 0) a.ws_ml[po] = make_float4(M, N, l, 0.f);
     if (a.nsplit == 1 || tiles > 0) {
-      // O through the shared memory of Q and K (every product is done), so that rows leave in whole lines: a lane
-      // writes its half row in 16-byte pieces, piece c at c ^ (row % 8), the warp reads half row after half row
+      // O through the shared memory of K, V and P (every product is done): a thread puts its half row there and
+      // sends it off with one bulk copy
       const float k = a.nsplit > 1 ? 1.f : any ? ex2(M - N) / l : 0.f;
       const bool zero = a.nsplit == 1 && !any;  // O may be anything where a row sees nothing
-      const uint32_t mine = sm + r * (D * 4);
+      constexpr int HD = D / 2;
+      const uint32_t mine = sm + r * C::PITCH + half * (HD * 4);
 #pragma unroll 1
-      for (int c = half * (D / 2); c < (half + 1) * (D / 2); c += 32) {
+      for (int c = 0; c < HD; c += 32) {
         uint32_t y[32];
         if (tiles > 0 && ok) {
-          tmem_load32(lanes + C::o_col + c, y);
+          tmem_load32(lanes + C::o_col + half * HD + c, y);
           tmem_ready(y);
         } else {
 #pragma unroll
           for (int i = 0; i < 32; ++i) y[i] = 0;
         }
+        if (a.nsplit > 1) {
 #pragma unroll
-        for (int i = 0; i < 32; ++i) y[i] = zero ? 0u : __float_as_uint(__uint_as_float(y[i]) * k);
+          for (int i = 0; i < 8; ++i)
+            sts128(mine + c * 4 + 16 * i, make_uint4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]));
+        } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-          sts128(mine + (((c / 4 + i) ^ (r & 7)) << 4), make_uint4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]));
-      }
-      __syncwarp();
-      constexpr int HD = D / 2;
-      if (a.nsplit > 1) {
-        float* o = a.ws_o + (po - lane) * D + half * HD;
-#pragma unroll 8
-        for (int i = lane; i < 32 * HD / 4; i += 32) {
-          const int rr = i / (HD / 4), c = half * (HD / 4) + i % (HD / 4);
-          const uint4 z = lds128(sm + (quad * 32 + rr) * (D * 4) + ((c ^ (rr & 7)) << 4));
-          *reinterpret_cast<uint4*>(o + rr * D + i % (HD / 4) * 4) = z;
-        }
-      } else {
-#pragma unroll 4
-        for (int i = lane; i < 32 * HD / 8; i += 32) {
-          const int rr = i / (HD / 8), c = half * (HD / 8) + i % (HD / 8);
-          const uint32_t row = sm + (quad * 32 + rr) * (D * 4);
-          const uint4 z = lds128(row + (((2 * c) ^ (rr & 7)) << 4)), y = lds128(row + (((2 * c + 1) ^ (rr & 7)) << 4));
-          const int64_t to = __shfl_sync(0xffffffffu, at, rr);
-          uint4 u;
-          __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&u);
-          h[0] = __floats2bfloat162_rn(__uint_as_float(z.x), __uint_as_float(z.y));
-          h[1] = __floats2bfloat162_rn(__uint_as_float(z.z), __uint_as_float(z.w));
-          h[2] = __floats2bfloat162_rn(__uint_as_float(y.x), __uint_as_float(y.y));
-          h[3] = __floats2bfloat162_rn(__uint_as_float(y.z), __uint_as_float(y.w));
-          if (quad * 32 + rr < rows) *reinterpret_cast<uint4*>(reinterpret_cast<bf16*>(a.out) + to + c * 8) = u;
+          for (int i = 0; i < 32; i += 8) {
+            uint32_t z[4];
+#pragma unroll
+            for (int h = 0; h < 4; ++h) {
+              const __nv_bfloat162 v2 = __floats2bfloat162_rn(__uint_as_float(y[i + 2 * h]) * k,
+                                                              __uint_as_float(y[i + 2 * h + 1]) * k);
+              z[h] = zero ? 0u : *reinterpret_cast<const uint32_t*>(&v2);
+            }
+            sts128(mine + c * 2 + i * 2, make_uint4(z[0], z[1], z[2], z[3]));
+          }
         }
       }
-      __syncwarp();
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      if (a.nsplit > 1 || r < rows) {
+        const void* to = a.nsplit > 1 ? (const void*)(a.ws_o + po * D + half * HD)
+                                      : (const void*)(reinterpret_cast<bf16*>(a.out) + at + half * HD);
+        asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(to), "r"(mine),
+                     "r"(a.nsplit > 1 ? HD * 4 : HD * 2)
+                     : "memory");
+      }
+      asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+      asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");  // before shared memory goes, and before the NaN below
       if (*nan_seen && real) {  // rare: a position past kmin holds NaN in V
 #pragma unroll 1
         for (int j = max(kmin + 1, base); j <= min(pos, base + kn - 1); ++j) {
@@ -1323,64 +1214,143 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_many_kernel(const Kv
     tc::tc_fence_before();
   } else if (warp < (SOFT + CONV) / 32) {
     // -------------------------------------------------------------- pages to f16 tiles
-    // row rr + i RPI of the warp's eight: 128 bytes a row, pieces swizzled by it
-    const uint32_t to = (pc >> 2) * (TILE * 128) + cw * 1024 + rr * 128 + ((((2 * pc) & 7) ^ rr) << 4);
+    // Four warps take the even tiles, four the odd ones (a warp's waits and addresses cost as much as its rows), a
+    // warp 16 positions of a tile: RPI of them at a time, 16 dims a lane, eight lanes on four pieces of an even and
+    // an odd row (their 16-byte stores then meet no bank twice).  A lane converts the bytes that it has copied.
+    constexpr int PCS = D / 16, RPI = 32 / PCS, NI = 16 / RPI, NB = UNI ? 1 : NI;
+    const int set = (warp - SOFT / 32) >> 2, cw = warp & 3;
+    const int rr = ((lane >> 2) & 1) | ((lane >> 3) / (PCS / 4)) << 1, pc = (lane & 3) | ((lane >> 3) % (PCS / 4)) << 2;
+    const uint8_t* kp = a.c.pages + a.c.layer + (int64_t)head * D + pc * 16;
+    const float* sc = a.c.scales + a.c.scale_layer + head;
+    const int64_t rs = (int64_t)a.c.hkv * D;
+    int blk[NB], off[NB];  // of the tile to be fetched next
+    const uint32_t raw8 = sm + C::raw + set * 2 * C::RAW + cw * (NI * 512) + lane * 16;  // 512 bytes apart
+    const uint32_t scales = C::rsc + set * 2 * C::SC + cw * 64;
+    int ids = -1;          // UNI: lane x has the block id of the warp's positions in its tile 32 k + x
+    auto look = [&](int j) {
+      if constexpr (UNI) {
+        const int mine = j >> 1;
+        if ((mine & 31) == 0) {
+          // whatever the length says: a tile's rows are bounded where they are fetched
+          const int p = (j + 2 * lane) * TILE + 16 * cw, page = (base + p) / a.c.block_size;
+          ids = page < a.max_blocks && p < a.split ? ld_act(table + page) : -1;
+        }
+        blk[0] = __shfl_sync(0xffffffffu, ids, mine & 31);
+        if (mine == 0) {
+          off[0] = (base + j * TILE + 16 * cw) % a.c.block_size;
+        } else {
+          off[0] += 2 * TILE % a.c.block_size;
+          if (off[0] >= a.c.block_size) off[0] -= a.c.block_size;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < NB; ++i) {
+          const int p = j * TILE + 16 * cw + rr + i * RPI;
+          blk[i] = -1;
+          off[i] = 0;
+          if (p < kn) {
+            const int page = (base + p) / a.c.block_size;
+            blk[i] = ld_act(table + page);
+            off[i] = base + p - page * a.c.block_size;
+          }
+        }
+      }
+    };
+    // start the copies of tile j's K (plane 0) or V rows and scales (zeros where there is no row)
+    auto fetch = [&](int j, int plane) {
+      const uint32_t to = raw8 + plane * C::RAW;
+      const float* from = sc + plane * a.c.scale_plane;
+      if (UNI ? lane == 0 : pc == 0) {
+#pragma unroll
+        for (int i = 0; i < NB; ++i) {
+          const bool there = (unsigned)blk[i] < (unsigned)a.c.num_blocks;
+          cp_async4(sm + scales + plane * C::SC + (UNI ? 0 : rr + i * RPI) * 4, from + (there ? (int64_t)blk[i] * a.c.hkv : 0),
+                    there);
+        }
+      }
+      if constexpr (UNI) {
+        const bool in = (unsigned)blk[0] < (unsigned)a.c.num_blocks;
+        const uint8_t* s = kp + plane * a.c.plane + (in ? ((int64_t)blk[0] * a.c.block_size + off[0] + rr) * rs : 0);
+        const int left = in ? kn - j * TILE - 16 * cw - rr : 0;  // row i of the lane is there where i RPI < left
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+          cp_async16(to + i * 512, s, i * RPI < left);
+          if (i * RPI + RPI < left) s += RPI * rs;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+          const int n = i % NB;
+          const bool there = (unsigned)blk[n] < (unsigned)a.c.num_blocks;
+          const int64_t row = there ? (int64_t)blk[n] * a.c.block_size + off[n] : 0;
+          cp_async16(to + i * 512, kp + plane * a.c.plane + row * rs, there);
+        }
+      }
+      cp_async_commit();
+    };
+    if (set < tiles) {
+      look(set);
+      fetch(set, 0);
+      fetch(set, 1);
+      look(set + 2);
+    }
+    // row rr + i RPI of the warp's 16: 128 bytes a row, pieces swizzled by it
+    const uint32_t to = (pc >> 2) * (TILE * 128) + cw * 2048 + rr * 128 + ((((2 * pc) & 7) ^ rr) << 4);
     auto put = [&](uint32_t tile, int i, uint4 w) {
       uint4 lo, hi;
       f16x4_of(w.x, lo.x, lo.y);
       f16x4_of(w.y, lo.z, lo.w);
       f16x4_of(w.z, hi.x, hi.y);
       f16x4_of(w.w, hi.z, hi.w);
-      const uint32_t at = ((tile + to) ^ (i * RPI * 16)) + i * RPI * 128;
+      const uint32_t at = ((tile + to) ^ ((i * RPI & 7) * 16)) + i * RPI * 128;
       sts128(at, lo);
       sts128(at ^ 16, hi);
     };
+    const uint32_t kt = sm + C::k + set * C::KV, vt = sm + C::v + set * C::KV;
 #pragma unroll 1
-    for (int j = 0; j < tiles; ++j) {
-      const int s = j & 1;
-      const uint32_t from = raw8 + (j % RS) * (2 * C::RAW);
-      if (j >= 2 && !wait(k_free(s), ((j >> 1) - 1) & 1, stop)) break;
-      cp_async_wait<2 * RS - 2>();  // K and V of this tile; a lane reads what it has copied itself
+    for (int j = set; j < tiles; j += 2) {
+      if (j >= 2 && !wait(k_free(set), ((j >> 1) - 1) & 1, stop)) break;
+      cp_async_wait<0>();
       uint32_t* mt = meta + (j % META) * TILE;
-      const float* ksc = reinterpret_cast<const float*>(gen + C::rsc + (j % RS * 2) * C::SC + cw * 32);
       if (UNI ? lane == 0 : pc == 0) {
+        const float* x = reinterpret_cast<const float*>(gen + scales);
 #pragma unroll
         for (int i = 0; i < NB; ++i) {
           const int r = UNI ? 0 : rr + i * RPI;
-          const float x = ksc[r], y = ksc[C::SC / 4 + r];
-          mt[UNI ? cw : 8 * cw + r] = x == 0.f ? 0u : pack_meta(scale_exponent(x), scale_exponent(y));
+          mt[UNI ? cw : 16 * cw + r] = x[r] == 0.f ? 0u : pack_meta(scale_exponent(x[r]), scale_exponent(x[C::SC / 4 + r]));
         }
       }
 #pragma unroll
-      for (int i = 0; i < NI; ++i) put(sm + C::k + s * C::KV, i, lds128(from + i * 512));
+      for (int i = 0; i < NI; ++i) put(kt, i, lds128(raw8 + i * 512));
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      tc::mbar_arrive(k_full(s));
-      fetch(j + RS, 0);
-      if (j == 0 && !wait(q_tmem, 0, stop)) break;  // V's tiles hold Q until then
-      if (j >= 2 && !wait(v_free(s), ((j >> 1) - 1) & 1, stop)) break;
+      tc::mbar_arrive(k_full(set));
       uint4 vb[NI];
 #pragma unroll
-      for (int i = 0; i < NI; ++i) vb[i] = lds128(from + C::RAW + i * 512);
-      if (base + j * TILE + 8 * cw + 7 > kmin) {  // NaN of positions that some row does not see: put back by row above
+      for (int i = 0; i < NI; ++i) vb[i] = lds128(raw8 + C::RAW + i * 512);
+      __syncwarp();  // the scales have been read
+      fetch(j + 2, 0);
+      fetch(j + 2, 1);
+      look(j + 4);
+      if (j < 2 && !wait(q_tmem, 0, stop)) break;  // V's tiles hold Q until then
+      if (j >= 2 && !wait(v_free(set), ((j >> 1) - 1) & 1, stop)) break;
+      if (base + j * TILE + 16 * cw + 15 > kmin) {  // NaN of positions that some row does not see: put back by row above
         uint32_t marks = 0;
 #pragma unroll
         for (int i = 0; i < NI; ++i)
-          if (base + j * TILE + 8 * cw + rr + i * RPI > kmin)
+          if (base + j * TILE + 16 * cw + rr + i * RPI > kmin)
             marks |= nan_marks(vb[i].x) | nan_marks(vb[i].y) | nan_marks(vb[i].z) | nan_marks(vb[i].w);
         if (marks) {
           *nan_seen = 1;
 #pragma unroll
           for (int i = 0; i < NI; ++i)
-            if (base + j * TILE + 8 * cw + rr + i * RPI > kmin)
+            if (base + j * TILE + 16 * cw + rr + i * RPI > kmin)
               vb[i] = make_uint4(clear_nan(vb[i].x), clear_nan(vb[i].y), clear_nan(vb[i].z), clear_nan(vb[i].w));
         }
       }
 #pragma unroll
-      for (int i = 0; i < NI; ++i) put(sm + C::v + s * C::KV, i, vb[i]);
+      for (int i = 0; i < NI; ++i) put(vt, i, vb[i]);
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      tc::mbar_arrive(v_full(s));
-      fetch(j + RS, 1);
-      look(j + RS + 1);
+      tc::mbar_arrive(v_full(set));
     }
     cp_async_wait<0>();
     __syncwarp();
