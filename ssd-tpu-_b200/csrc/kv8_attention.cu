@@ -13,7 +13,6 @@
 #include <float.h>
 
 #include <atomic>
-#include <cstdlib>
 
 #include "kv8.cuh"
 #include "tcgen05.cuh"
@@ -117,11 +116,72 @@ __global__ void __launch_bounds__(kJoinThreads) kv8_join_kernel(const Kv8Attn a)
   }
 }
 
+// The same for few splits: one warp a row, 4 dims of a lane at a time.
+template <typename T, int D, int R, bool LOG2>
+__global__ void __launch_bounds__(128) kv8_join_few_kernel(const Kv8Attn a, int64_t rows) {
+  constexpr int DQ = D / 4, PL = DQ < 32 ? 1 : DQ / 32;  // float4 of a row, of a lane
+  const int lane = threadIdx.x & 31;
+  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+  const int r = (int)(row % R);
+  const int64_t grp = row / R;
+  const int rg = (int)(grp % a.row_groups), head = (int)(grp / a.row_groups % a.c.hkv);
+  const int b = (int)(grp / a.row_groups / a.c.hkv);
+  const int gr = rg * R + r, t = gr / a.G, g = gr % a.G;
+  pdl_wait();
+  pdl_trigger();
+  if (row >= rows || t >= a.T) return;
+  const int seq_full = ld_act(a.seq_lens + b);
+  const int ql = a.q_lens ? min(max(ld_act(a.q_lens + b), 0), a.T) : a.T;
+  const int ns = splits_of(min(min(seq_full, a.max_blocks * a.c.block_size), a.nsplit * a.split), a.split);
+  auto ex = [](float v) { return LOG2 ? exp2f(v) : expf(v); };
+  float4 v = make_float4(-INFINITY, -INFINITY, 0.f, 0.f);
+  if (lane < ns) v = __ldcg(a.ws_ml + (grp * a.nsplit + lane) * R + r);
+  const float M = warp_max(v.x), N = warp_max(v.y);
+  const float L = warp_sum(v.y == -INFINITY ? 0.f : v.z * ex(v.y - N));
+  const float w = v.x == -INFINITY ? 0.f : ex(v.x - M);
+  const float4* po = reinterpret_cast<const float4*>(a.ws_o) + (grp * a.nsplit * R + r) * DQ;
+  float4 o[PL];
+#pragma unroll
+  for (int i = 0; i < PL; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int s = 0; s < ns; ++s) {
+    const float f = __shfl_sync(0xffffffffu, w, s);
+#pragma unroll
+    for (int i = 0; i < PL; ++i) {
+      if (DQ < 32 && lane >= DQ) continue;
+      const float4 x = __ldcg(po + (int64_t)s * R * DQ + i * 32 + lane);
+      if (f != 0.f) {  // a split that the row does not see holds anything
+        o[i].x = fmaf(f, x.x, o[i].x);
+        o[i].y = fmaf(f, x.y, o[i].y);
+        o[i].z = fmaf(f, x.z, o[i].z);
+        o[i].w = fmaf(f, x.w, o[i].w);
+      }
+    }
+  }
+  const bool real = t < ql && L != 0.f;
+  const float k = ex(M - N);
+  T* out = reinterpret_cast<T*>(a.out) + (((int64_t)b * a.T + t) * a.hq + head * a.G + g) * D;
+#pragma unroll
+  for (int i = 0; i < PL; ++i) {
+    if (DQ < 32 && lane >= DQ) continue;
+    T y[4] = {from_f<T>(real ? o[i].x / L * k : 0.f), from_f<T>(real ? o[i].y / L * k : 0.f),
+              from_f<T>(real ? o[i].z / L * k : 0.f), from_f<T>(real ? o[i].w / L * k : 0.f)};
+    T* to = out + (i * 32 + lane) * 4;
+    if constexpr (sizeof(T) == 2)
+      *reinterpret_cast<uint2*>(to) = *reinterpret_cast<uint2*>(y);
+    else
+      *reinterpret_cast<uint4*>(to) = *reinterpret_cast<uint4*>(y);
+  }
+}
+
 template <typename T, int D, int R, bool LOG2>
 int launch_join(cudaStream_t st, const Kv8Attn& a, int B) {
   const int64_t rows = (int64_t)B * a.c.hkv * a.row_groups * R;
   if (rows > 0x7fffffff) return SSD_ERR_UNSUPPORTED;
-  SSD_PDL((kv8_join_kernel<T, D, R, LOG2>), (unsigned)rows, kJoinThreads, 0, st, a);
+  if (a.nsplit <= 16)
+    SSD_PDL((kv8_join_few_kernel<T, D, R, LOG2>), (unsigned)((rows + 3) / 4), 128, 0, st, a, rows);
+  else
+    SSD_PDL((kv8_join_kernel<T, D, R, LOG2>), (unsigned)rows, kJoinThreads, 0, st, a);
   return SSD_OK;
 }
 
@@ -1357,8 +1417,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_many_kernel(const Kv
   } else {
     // -------------------------------------------------------------- products
     // The whole warp walks the loop and one elected lane issues, so that addresses and descriptors stay in uniform
-    // registers: with the loop inside one lane's branch, every product waited for them to be moved there (2700
-    // instead of NNNN cycles a tile).
+    // registers: with the loop inside one lane's branch every product waited for them to be moved there.
     if (tiles > 0) {
       uint32_t lead;
       asm volatile("{.reg .pred p; elect.sync _|p, 0xffffffff; selp.u32 %0, 1, 0, p;}" : "=r"(lead));
@@ -1427,13 +1486,17 @@ struct Kv8Layout {
 
 inline size_t up256(size_t x) { return (x + 255) & ~size_t(255); }
 
-constexpr int kManyFrom = 16;  // query rows of a KV head above which a call goes to the many-row kernel
+// Which kernel: above 32 query rows of a KV head, and more than 8 new tokens, the many-row one (64 new tokens of one
+// sequence, one head a KV head, 2000 positions: 22 against 34 us; 24 tokens of eight: 102 against 90 us the other
+// way).  Up to 8 tokens always the few-row one, so that a verify step gives a query the bits that decoding it alone
+// does (40 rows, 32 sequences: 52 us, where the other kernel takes 37).
+constexpr int kManyRows = 32, kFewTokens = 8;
 
 Kv8Layout kv8_layout(bool cc, int B, int T, int hq, int hkv, int D, int max_seq_len) {
   Kv8Layout L;
   const int64_t total = (int64_t)(hq / hkv) * T;
   L.cc = cc;
-  L.rows = cc ? kCcRows : total > (getenv("KMANY") ? atoi(getenv("KMANY")) : 16) ? many::ROWS : total > 8 ? 16 : 8;
+  L.rows = cc ? kCcRows : total > kManyRows && T > kFewTokens ? many::ROWS : total > 8 ? 16 : 8;
   // Few rows: 256 positions keep a short context's CTAs many (one sequence of 8192 positions, one KV head: 11.9 us
   // against 18.7 us at 1024); where there is work for every SM either way, 1024 positions cost fewer prologues and
   // partials (8 sequences, 16 heads, up to 4096 positions: 38.1 against 43.2 us).  The rule goes by the sequences,
@@ -1441,11 +1504,12 @@ Kv8Layout kv8_layout(bool cc, int B, int T, int hq, int hkv, int D, int max_seq_
   L.split = cc ? kCcSplit : (int64_t)B * hkv * ((max_seq_len + 255) / 256) >= 2048 ? 1024 : 256;
   L.row_groups = (int)((total + L.rows - 1) / L.rows);
   if (L.rows == many::ROWS) {
+    // one CTA an SM: as many splits as one wave of them takes (four sequences of 8192 positions, 256 rows each: 42 us
+    // in 128 CTAs, 58 us in 160); a context of up to 512 positions stays whole (12.9 against 20.6 us at 300)
     const int64_t ctas = (int64_t)B * hkv * L.row_groups;
-    const int64_t want = (148 + ctas - 1) / ctas;  // splits that fill the SMs
-    int64_t sp = (max_seq_len + want - 1) / want;
-    sp = (sp + 63) / 64 * 64;
-    L.split = (int)(sp < 256 ? 256 : sp);
+    const int64_t n = ctas >= 148 || max_seq_len <= 512 ? 1 : 148 / ctas;
+    const int64_t sp = ((max_seq_len + n - 1) / n + 63) / 64 * 64;
+    L.split = (int)(sp < 128 ? 128 : sp);
   }
   L.nsplit = (max_seq_len + L.split - 1) / L.split;
   L.groups = (size_t)B * hkv * L.row_groups;
