@@ -325,7 +325,7 @@ int ssd_kv8_attention(ssd_stream_t stream, const void* q, const void* pages, con
  * same) pool, i < n, in each of `planes` planes (2 * num_layers): `page_bytes` per page and plane,
  * and, with scales_per_page > 0, that many fp32 scales (an 8-bit cache's Hkv).  A pool's plane is
  * its block count times page_bytes.  Pairs with an id out of range on either side (-1) are skipped.
- * count (device, may be NULL): number of pairs, at most n.  Within one pool no page may be both
+ * count (device, may be NULL): number of pairs, at most n (the ids past it are read, and may hold anything).  Within one pool no page may be both
  * copied from and copied to, nor copied to twice: the pairs move in no particular order.
  */
 int ssd_page_copy(ssd_stream_t stream, const void* src_pages, const float* src_scales, int src_blocks,
@@ -341,17 +341,17 @@ int ssd_page_copy(ssd_stream_t stream, const void* src_pages, const float* src_s
  *   move_src, move_dst [num_blocks / 2, at least 1], num_moves [1]  the moves, for ssd_page_copy
  *   ref_counts_out            the counts under the new ids
  *   free_list_out, free_top_out  num_blocks - U free blocks, handed out from U upwards
- * The *_out arrays may be the inputs themselves.  Pages and tables do not change: ssd_page_copy and
- * ssd_page_remap carry the plan out.
+ *   tables_out [B, max_blocks]   tables under the new ids: remap[tables[b][i]] for i < lens[b], else -1
+ *                                (B = 0: none); a second set for the draft's tables
+ * The *_out arrays may be the inputs themselves.  Pages do not change: ssd_page_copy with the moves
+ * carries the plan out, once for each cache of the pool.
  */
 int ssd_page_compact(ssd_stream_t stream, const int32_t* free_list, const int32_t* free_top,
                      const int32_t* ref_counts, int num_blocks, int32_t* free_list_out, int32_t* free_top_out,
                      int32_t* ref_counts_out, int32_t* remap, int32_t* move_src, int32_t* move_dst,
-                     int32_t* num_moves);
-
-/* tables_out[b][i] = remap[tables[b][i]] for i < lens[b], else -1; tables_out may be tables. */
-int ssd_page_remap(ssd_stream_t stream, const int32_t* tables, int32_t* tables_out, const int32_t* lens,
-                   int max_blocks, int B, const int32_t* remap, int num_blocks);
+                     int32_t* num_moves, const int32_t* tables, int32_t* tables_out, const int32_t* lens,
+                     int max_blocks, int B, const int32_t* draft_tables, int32_t* draft_tables_out,
+                     const int32_t* draft_lens, int draft_max_blocks, int draft_B);
 
 /* ------------------------------------------------------- K3: skinny projections */
 

@@ -71,7 +71,7 @@ __device__ __forceinline__ void rotate8(float* x1, float* x2, const float* c, co
   }
 }
 
-// Values of one item: 8 dims of V (or of K without rotation), or a rotation pair 8 + 8 of K.
+// Values of one item: dims d .. d + 7 and D/2 + d .. D/2 + d + 7 of a row, rotated where K is.
 template <typename T, int D>
 struct Rows {
   const AppendArgs& a;
@@ -79,19 +79,14 @@ struct Rows {
   int first;    // first new position in the page
   int head, plane;
   __device__ __forceinline__ bool rotated() const { return a.cos_t != nullptr && plane == 0; }
-  // item i of the page's rows: local row r, 16 dims as two groups of 8 (d0, d1)
+  // item i of the page's rows: local row r
   __device__ __forceinline__ void get(int i, int& r, int& d0, int& d1, float* x0, float* x1) const {
     constexpr int PER = D / 16;
     r = i / PER;
     const int c = i % PER;
     const T* base = reinterpret_cast<const T*>(plane ? a.v : a.k) + (m0 + r) * a.row + (int64_t)head * D;
-    if (rotated()) {
-      d0 = c * 8;
-      d1 = d0 + D / 2;
-    } else {
-      d0 = c * 16;
-      d1 = d0 + 8;
-    }
+    d0 = c * 8;  // two groups of 8 dims, half a row apart: a rotation pair, and whole sectors for a warp's loads
+    d1 = d0 + D / 2;
     load8<T>(base + d0, x0);
     load8<T>(base + d1, x1);
     if (rotated()) {
@@ -228,10 +223,7 @@ __global__ void __launch_bounds__(256) kv8_append_kernel(const AppendArgs a) {
     const int it = threadIdx.x + k * blockDim.x;
     if (it < items) {
       const int r = it / PER, c = it % PER;
-      if (src.rotated())
-        put(r, c * 8, c * 8 + D / 2, x[k]);
-      else
-        put(r, c * 16, c * 16 + 8, x[k]);
+      put(r, c * 8, c * 8 + D / 2, x[k]);
     }
   }
   for (int it = threadIdx.x + KEEP * blockDim.x; it < items; it += blockDim.x) {
@@ -276,17 +268,23 @@ int append_common(ssd_stream_t stream, AppendArgs a, int dtype, int B, int T, in
   return launch_append<float>(st, a, B, D);
 }
 
-// K and V rows of positions [B][N] (-1: zeros): one warp per position, lanes over 16-byte pieces of its
-// heads in both planes.  Bound: HBM (1 byte in, 2 or 4 out).
+// K and V rows of positions [B][N] (-1: zeros).  A row of one position is 2 Hkv D values; a warp takes up to
+// kGatherItems * 32 groups of 8 of them (8 bytes in, 16 or 32 out, neighbouring lanes on neighbouring groups), all
+// loads in flight at once.  Bound: HBM.
+constexpr int kGatherItems = 4;
+
 template <typename T, int D>
 __global__ void __launch_bounds__(256) kv8_gather_kernel(const Kv8Cache c, const int32_t* tables, int max_blocks,
-                                                         const int32_t* positions, int64_t rows, int N, T* k, T* v) {
+                                                         const int32_t* positions, int64_t rows, int N, int chunks,
+                                                         T* k, T* v) {
   pdl_wait();
   pdl_trigger();
-  constexpr int PER = D / 16;
+  constexpr int PER = D / 8;
   const int lane = threadIdx.x & 31;
-  const int64_t m = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (m >= rows) return;
+  const int64_t w = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (w >= rows * chunks) return;
+  const int64_t m = w / chunks;
+  const int first = (int)(w - m * chunks) * (kGatherItems * 32) + lane;
   const int b = (int)(m / N);
   const int pos = ld_act(positions + m);
   int blk = -1;
@@ -294,40 +292,52 @@ __global__ void __launch_bounds__(256) kv8_gather_kernel(const Kv8Cache c, const
     blk = ld_act(tables + (int64_t)b * max_blocks + pos / c.block_size);
   const bool ok = (unsigned)blk < (unsigned)c.num_blocks;
   const int items = c.hkv * PER;
-  const int64_t row = ok ? (int64_t)blk * c.block_size + pos % c.block_size : 0;
-  for (int i = lane; i < 2 * items; i += 32) {
-    const int plane = i >= items, j = plane ? i - items : i;
-    uint4 w = make_uint4(0, 0, 0, 0);
-    float s = 0.f;
-    if (ok) {
-      w = ld_act_v4(c.pages + plane * c.plane + c.layer + row * c.hkv * D + (int64_t)j * 16);
-      s = ld_act(c.scales + plane * c.scale_plane + c.scale_layer + (int64_t)blk * c.hkv + j / PER);
-    }
-    const uint32_t in[4] = {w.x, w.y, w.z, w.w};
-    float f[16];
+  const uint8_t* row = c.pages + c.layer + (ok ? (int64_t)blk * c.block_size + pos % c.block_size : 0) * c.hkv * D;
+  const float* sc = c.scales + c.scale_layer + (ok ? (int64_t)blk * c.hkv : 0);
+  uint2 x[kGatherItems];
+  float s[kGatherItems];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const float2 lo = e4m3_pair(in[q]), hi = e4m3_pair(in[q] >> 16);
-      f[4 * q] = lo.x * s; f[4 * q + 1] = lo.y * s; f[4 * q + 2] = hi.x * s; f[4 * q + 3] = hi.y * s;
+  for (int i = 0; i < kGatherItems; ++i) {
+    const int it = first + 32 * i;
+    const int plane = it >= items, j = plane ? it - items : it;
+    x[i] = make_uint2(0, 0);
+    s[i] = 0.f;
+    if (ok && it < 2 * items) {
+      x[i] = __ldcg(reinterpret_cast<const uint2*>(row + plane * c.plane + (int64_t)j * 8));
+      s[i] = ld_act(sc + plane * c.scale_plane + j / PER);
     }
-    T* o = (plane ? v : k) + m * c.hkv * D + (int64_t)j * 16;
-    store8(o, f);
-    store8(o + 8, f + 8);
+  }
+#pragma unroll
+  for (int i = 0; i < kGatherItems; ++i) {
+    const int it = first + 32 * i;
+    const int plane = it >= items, j = plane ? it - items : it;
+    if (it >= 2 * items) break;
+    const uint32_t in[2] = {x[i].x, x[i].y};
+    float f[8];
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      const float2 lo = e4m3_pair(in[q]), hi = e4m3_pair(in[q] >> 16);
+      f[4 * q] = lo.x * s[i]; f[4 * q + 1] = lo.y * s[i]; f[4 * q + 2] = hi.x * s[i]; f[4 * q + 3] = hi.y * s[i];
+    }
+    store8((plane ? v : k) + m * c.hkv * D + (int64_t)j * 8, f);
   }
 }
 
 template <typename T>
 int launch_gather(cudaStream_t st, const Kv8Cache& c, const int32_t* tables, int max_blocks, const int32_t* positions,
                   int64_t rows, int N, void* k, void* v, int D) {
-  const unsigned grid = (unsigned)((rows + 7) / 8);
+  const int chunks = (2 * c.hkv * (D / 8) + kGatherItems * 32 - 1) / (kGatherItems * 32);
+  const int64_t ctas = (rows * chunks + 7) / 8;
+  if (ctas > 0x7fffffff) return SSD_ERR_UNSUPPORTED;
+  const unsigned grid = (unsigned)ctas;
   T* ko = reinterpret_cast<T*>(k);
   T* vo = reinterpret_cast<T*>(v);
   if (D == 256)
-    SSD_PDL((kv8_gather_kernel<T, 256>), grid, 256, 0, st, c, tables, max_blocks, positions, rows, N, ko, vo);
+    SSD_PDL((kv8_gather_kernel<T, 256>), grid, 256, 0, st, c, tables, max_blocks, positions, rows, N, chunks, ko, vo);
   else if (D == 128)
-    SSD_PDL((kv8_gather_kernel<T, 128>), grid, 256, 0, st, c, tables, max_blocks, positions, rows, N, ko, vo);
+    SSD_PDL((kv8_gather_kernel<T, 128>), grid, 256, 0, st, c, tables, max_blocks, positions, rows, N, chunks, ko, vo);
   else
-    SSD_PDL((kv8_gather_kernel<T, 64>), grid, 256, 0, st, c, tables, max_blocks, positions, rows, N, ko, vo);
+    SSD_PDL((kv8_gather_kernel<T, 64>), grid, 256, 0, st, c, tables, max_blocks, positions, rows, N, chunks, ko, vo);
   return SSD_OK;
 }
 
@@ -402,7 +412,6 @@ extern "C" int ssd_kv8_gather(ssd_stream_t stream, const void* pages, const floa
   if (!positions || !k || !v) return SSD_ERR_INVALID;
   if (!kv8_aligned(k) || !kv8_aligned(v)) return SSD_ERR_UNSUPPORTED;
   const int64_t rows = (int64_t)B * N;
-  if ((rows + 7) / 8 > 0x7fffffff) return SSD_ERR_UNSUPPORTED;
   const Kv8Cache c = kv8_cache(const_cast<void*>(pages), const_cast<float*>(scales), num_layers, num_blocks,
                                block_size, num_kv_heads, head_dim, layer);
   cudaStream_t st = (cudaStream_t)stream;

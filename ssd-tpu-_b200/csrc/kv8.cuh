@@ -9,6 +9,8 @@
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>
 
+#include <atomic>
+
 #include "common.cuh"
 
 namespace ssd {
@@ -60,6 +62,10 @@ __device__ __forceinline__ float2 e4m3_pair(uint32_t pair) {
   return __half22float2(*reinterpret_cast<const __half2*>(&h));
 }
 
+// Bytes of w that are e4m3 NaN (0x7f, 0xff), as 0x80 marks.
+__device__ __forceinline__ uint32_t nan_marks(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
+__device__ __forceinline__ uint32_t clear_nan(uint32_t w) { return w & ~((nan_marks(w) >> 7) * 0xffu); }
+
 struct Kv8Cache {
   uint8_t* pages;
   float* scales;
@@ -98,6 +104,21 @@ inline int kv8_check(const void* pages, const float* scales, int num_layers, int
   if ((int64_t)num_blocks * block_size > 0x7fffffff) return SSD_ERR_UNSUPPORTED;  // row numbers are 32-bit
   if (!kv8_aligned(pages)) return SSD_ERR_UNSUPPORTED;
   return SSD_OK;
+}
+
+// A kernel's dynamic shared memory limit belongs to each device's context: raised once per device (`ready`: one
+// bit a device), always to the same size.
+template <typename K>
+bool allow_smem(std::atomic<uint64_t>& ready, K kern, int bytes) {
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return false;
+  if (ready.load(std::memory_order_acquire) >> dev & 1) return true;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) {
+    (void)cudaGetLastError();
+    return false;
+  }
+  ready.fetch_or(1ull << dev, std::memory_order_release);
+  return true;
 }
 
 }  // namespace ssd

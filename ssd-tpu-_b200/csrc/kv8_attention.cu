@@ -12,8 +12,6 @@
 // workspace holds nothing between calls and may come uninitialised from any allocator.
 #include <float.h>
 
-#include <atomic>
-
 #include "kv8.cuh"
 #include "tcgen05.cuh"
 
@@ -186,128 +184,163 @@ int launch_join(cudaStream_t st, const Kv8Attn& a, int B) {
 }
 
 // ------------------------------------------------------------------ CUDA-core kernel (fp32 models)
-// fp32 queries keep fp32 products: a warp walks its positions one by one with the running maximum and sum
-// of each row, lanes over the head dims.  Used for the fp32 (toy) models, whose forward takes at most 16 rows.
+// fp32 queries keep fp32 products.  A CTA takes 8 query rows and 128 positions: a thread scores one position
+// against all rows (Q broadcast from shared memory, no reduction across lanes), the rows' maxima and sums are
+// taken over the CTA, and for P V a thread holds 4 dims of all rows over every PG-th position.  Used by the fp32
+// (toy) models, whose forward takes at most 16 rows: bound by latency, not by bytes.
 constexpr int kCcRows = 8;
 constexpr int kCcSplit = 128;
-constexpr int kCcWarps = 4;
 
-template <int N>
-__device__ __forceinline__ void load_e4m3(const uint8_t* p, float* f) {
-  if constexpr (N == 8) {
-    const uint2 w = __ldcg(reinterpret_cast<const uint2*>(p));
-    const float2 a = e4m3_pair(w.x), b = e4m3_pair(w.x >> 16), c = e4m3_pair(w.y), d = e4m3_pair(w.y >> 16);
-    f[0] = a.x; f[1] = a.y; f[2] = b.x; f[3] = b.y; f[4] = c.x; f[5] = c.y; f[6] = d.x; f[7] = d.y;
-  } else if constexpr (N == 4) {
-    const uint32_t w = __ldcg(reinterpret_cast<const uint32_t*>(p));
-    const float2 a = e4m3_pair(w), b = e4m3_pair(w >> 16);
-    f[0] = a.x; f[1] = a.y; f[2] = b.x; f[3] = b.y;
-  } else {
-    const float2 a = e4m3_pair(__ldcg(reinterpret_cast<const uint16_t*>(p)));
-    f[0] = a.x; f[1] = a.y;
-  }
-}
-
-template <typename T, int D>
-__global__ void __launch_bounds__(kCcWarps * 32) kv8_attention_cc_kernel(const Kv8Attn a) {
-  constexpr int DPL = D / 32;
-  __shared__ float qs[kCcRows][D];
-  __shared__ float os[kCcWarps][kCcRows][D];
-  __shared__ float2 mls[kCcWarps][kCcRows];
+template <int D>
+__global__ void __launch_bounds__(kCcSplit) kv8_attention_cc_kernel(const Kv8Attn a) {
+  constexpr int DG = D / 4, PG = kCcSplit / DG;
+  __shared__ float4 q_s[D][2];                 // dim d of rows 0-3 and 4-7
+  __shared__ float4 p_s[kCcSplit][2];          // weights of position j
+  __shared__ float o_s[PG][kCcRows][D];
+  __shared__ float red[2][4][kCcRows];
   __shared__ int pos_s[kCcRows];
-  pdl_wait();
-  pdl_trigger();
+  __shared__ int64_t v_s[kCcSplit];            // byte offset of a position's V row (-1: none)
+  __shared__ float vs_s[kCcSplit];
   const int split = blockIdx.x, b = blockIdx.z;
   const int head = blockIdx.y / a.row_groups, rg = blockIdx.y % a.row_groups;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int seq_full = a.seq_lens[b];
+  pdl_wait();
+  pdl_trigger();
+  const int j = split * kCcSplit + tid;        // this thread's position
+  const int page = j / a.c.block_size;
+  int blk = -1;                                // read whatever the length says, so as not to wait for it
+  if (page < a.max_blocks) blk = ld_act(a.tables + (int64_t)b * a.max_blocks + page);
+  const int seq_full = ld_act(a.seq_lens + b);
+  const int ql = a.q_lens ? min(max(ld_act(a.q_lens + b), 0), a.T) : a.T;
   // positions beyond the table or the split count are never read (a seq_len larger than the caller's bound)
   const int seq = min(min(seq_full, a.max_blocks * a.c.block_size), a.nsplit * kCcSplit);
-  const int ql = a.q_lens ? min(max(a.q_lens[b], 0), a.T) : a.T;
   const int row0 = rg * kCcRows;
   const int nrows = min(kCcRows, a.G * a.T - row0);
-  const int ns = splits_of(seq, kCcSplit);
-  if (split >= ns) return;
+  if (split >= splits_of(seq, kCcSplit)) return;
+  for (int i = tid; i < kCcRows * D; i += kCcSplit) {
+    const int r = i / D, d = i % D;
+    const int gr = row0 + r, t = gr / a.G, g = gr % a.G;
+    reinterpret_cast<float*>(q_s[d])[r] =
+        r < nrows ? ld_act(reinterpret_cast<const float*>(a.q) + (((int64_t)b * a.T + t) * a.hq + head * a.G + g) * D + d)
+                  : 0.f;
+  }
   if (tid < kCcRows) {
     const int t = (row0 + tid) / a.G;
     pos_s[tid] = (tid < nrows && t < ql) ? seq_full - ql + t : -1;
   }
-  for (int i = tid; i < kCcRows * D; i += blockDim.x) {
-    const int r = i / D, d = i % D;
-    const int gr = row0 + r, t = gr / a.G, g = gr % a.G;
-    qs[r][d] = r < nrows ? to_f(ld_act(reinterpret_cast<const T*>(a.q) +
-                                       (((int64_t)b * a.T + t) * a.hq + head * a.G + g) * D + d)) : 0.f;
+  const bool there = j < seq && (unsigned)blk < (unsigned)a.c.num_blocks;
+  float s[kCcRows];
+#pragma unroll
+  for (int r = 0; r < kCcRows; ++r) s[r] = 0.f;
+  uint4 w[D / 16];
+  float ks = 0.f, vs = 0.f;
+  int64_t off = -1;
+  if (there) {
+    off = a.c.layer + (((int64_t)blk * a.c.block_size + j % a.c.block_size) * a.c.hkv + head) * D;
+    const float* sc = a.c.scales + a.c.scale_layer + (int64_t)blk * a.c.hkv + head;
+    ks = ld_act(sc);
+    vs = ld_act(sc + a.c.scale_plane);
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) w[i] = ld_act_v4(a.c.pages + off + 16 * i);
   }
+  v_s[tid] = there ? off + a.c.plane : -1;
+  vs_s[tid] = vs;
   __syncthreads();
-  float m[kCcRows], l[kCcRows], o[kCcRows][DPL];
+  if (there) {
 #pragma unroll
-  for (int r = 0; r < kCcRows; ++r) {
-    m[r] = -INFINITY;
-    l[r] = 0.f;
+    for (int i = 0; i < D / 16; ++i) {
+      const uint32_t in[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
 #pragma unroll
-    for (int i = 0; i < DPL; ++i) o[r][i] = 0.f;
-  }
-  const int k1 = min(seq, (split + 1) * kCcSplit);
-  const int32_t* table = a.tables + (int64_t)b * a.max_blocks;
-  for (int j = split * kCcSplit + warp; j < k1; j += kCcWarps) {
-    const int blk = ld_act(table + j / a.c.block_size);
-    if ((unsigned)blk >= (unsigned)a.c.num_blocks) continue;
-    const int64_t off = a.c.layer + (((int64_t)blk * a.c.block_size + j % a.c.block_size) * a.c.hkv + head) * D;
-    const int64_t so = a.c.scale_layer + (int64_t)blk * a.c.hkv + head;
-    const float ks = ld_act(a.c.scales + so), vs = ld_act(a.c.scales + a.c.scale_plane + so);
-    float k[DPL], v[DPL];
-    load_e4m3<DPL>(a.c.pages + off + lane * DPL, k);
-    load_e4m3<DPL>(a.c.pages + a.c.plane + off + lane * DPL, v);
+      for (int x = 0; x < 8; ++x) {
+        const float2 k = e4m3_pair(in[x >> 1] >> (x & 1 ? 16 : 0));
 #pragma unroll
-    for (int i = 0; i < DPL; ++i) v[i] *= vs;
-#pragma unroll
-    for (int r = 0; r < kCcRows; ++r) {
-      if (pos_s[r] < j) continue;  // the same for every lane
-      float s = 0.f;
-#pragma unroll
-      for (int i = 0; i < DPL; ++i) s = fmaf(qs[r][lane * DPL + i], k[i], s);
-      s = warp_sum(s) * ks * a.scale;
-      const float mn = fmaxf(m[r], fmaxf(s, -FLT_MAX));  // finite once a position is seen, a NaN score included
-      const float f = m[r] == -INFINITY ? 0.f : expf(m[r] - mn), p = expf(s - mn);
-      l[r] = l[r] * f + p;
-#pragma unroll
-      for (int i = 0; i < DPL; ++i) o[r][i] = fmaf(p, v[i], o[r][i] * f);
-      m[r] = mn;
+        for (int y = 0; y < 2; ++y) {
+          const float kd = y ? k.y : k.x;
+          const float4 qa = q_s[16 * i + 2 * x + y][0], qb = q_s[16 * i + 2 * x + y][1];
+          s[0] = fmaf(qa.x, kd, s[0]); s[1] = fmaf(qa.y, kd, s[1]); s[2] = fmaf(qa.z, kd, s[2]); s[3] = fmaf(qa.w, kd, s[3]);
+          s[4] = fmaf(qb.x, kd, s[4]); s[5] = fmaf(qb.y, kd, s[5]); s[6] = fmaf(qb.z, kd, s[6]); s[7] = fmaf(qb.w, kd, s[7]);
+        }
+      }
     }
   }
+  float m[kCcRows];
 #pragma unroll
   for (int r = 0; r < kCcRows; ++r) {
-    if (lane == 0) mls[warp][r] = make_float2(m[r], l[r]);
-#pragma unroll
-    for (int i = 0; i < DPL; ++i) os[warp][r][lane * DPL + i] = o[r][i];
+    s[r] = there && j <= pos_s[r] ? s[r] * ks * a.scale : -INFINITY;
+    // finite once a position is seen, a NaN score included: it spoils the sums below
+    const float x = warp_max(there && j <= pos_s[r] ? fmaxf(s[r], -FLT_MAX) : -INFINITY);
+    if (lane == 0) red[0][warp][r] = x;
   }
   __syncthreads();
-  // join the warps in warp order
+  float p[kCcRows];
+#pragma unroll
+  for (int r = 0; r < kCcRows; ++r) {
+    m[r] = fmaxf(fmaxf(red[0][0][r], red[0][1][r]), fmaxf(red[0][2][r], red[0][3][r]));
+    p[r] = there && j <= pos_s[r] ? expf(s[r] - m[r]) : 0.f;
+    const float x = warp_sum(p[r]);
+    if (lane == 0) red[1][warp][r] = x;
+  }
+  p_s[tid][0] = make_float4(p[0], p[1], p[2], p[3]);
+  p_s[tid][1] = make_float4(p[4], p[5], p[6], p[7]);
+  __syncthreads();
+  {
+    const int dg = tid % DG, pg = tid / DG;
+    float o[kCcRows][4];
+#pragma unroll
+    for (int r = 0; r < kCcRows; ++r)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[r][i] = 0.f;
+    const int n = min(kCcSplit, seq - split * kCcSplit);
+#pragma unroll 8
+    for (int i = pg; i < n; i += PG) {
+      const int64_t vo = v_s[i];
+      if (vo < 0) continue;
+      uint32_t v4 = __ldcg(reinterpret_cast<const uint32_t*>(a.c.pages + vo + 4 * dg));
+      if (nan_marks(v4)) {  // rare: NaN reaches the rows that see the position, no others
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+          if ((v4 >> (8 * x) & 0x7fu) == 0x7fu)
+#pragma unroll
+            for (int r = 0; r < kCcRows; ++r)
+              if (split * kCcSplit + i <= pos_s[r]) o[r][x] = __int_as_float(0x7fc00000);
+        v4 = clear_nan(v4);
+      }
+      const float2 lo = e4m3_pair(v4), hi = e4m3_pair(v4 >> 16);
+      const float f = vs_s[i];
+      const float v[4] = {lo.x * f, lo.y * f, hi.x * f, hi.y * f};
+      const float4 pa = p_s[i][0], pb = p_s[i][1];
+      const float pr[8] = {pa.x, pa.y, pa.z, pa.w, pb.x, pb.y, pb.z, pb.w};
+#pragma unroll
+      for (int r = 0; r < kCcRows; ++r)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) o[r][x] = fmaf(pr[r], v[x], o[r][x]);
+    }
+#pragma unroll
+    for (int r = 0; r < kCcRows; ++r)
+      *reinterpret_cast<float4*>(&o_s[pg][r][4 * dg]) = make_float4(o[r][0], o[r][1], o[r][2], o[r][3]);
+  }
+  __syncthreads();
   const int64_t grp = ((int64_t)b * a.c.hkv + head) * a.row_groups + rg;
-  T* out = reinterpret_cast<T*>(a.out);
-  auto out_at = [&](int r, int d) -> T& {
-    const int gr = row0 + r, t = gr / a.G, g = gr % a.G;
-    return out[(((int64_t)b * a.T + t) * a.hq + head * a.G + g) * D + d];
-  };
-  for (int i = tid; i < nrows * D; i += blockDim.x) {
+  for (int i = tid; i < nrows * D; i += kCcSplit) {
     const int r = i / D, d = i % D;
-    float M = -INFINITY;
-    for (int w = 0; w < kCcWarps; ++w) M = fmaxf(M, mls[w][r].x);
-    float O = 0.f, L = 0.f;
-    for (int w = 0; w < kCcWarps; ++w) {
-      const float f = mls[w][r].x == -INFINITY ? 0.f : expf(mls[w][r].x - M);
-      L += mls[w][r].y * f;
-      if (f != 0.f) O += os[w][r][d] * f;
-    }
+    float O = 0.f;
+#pragma unroll
+    for (int x = 0; x < PG; ++x) O += o_s[x][r][d];
+    const float L = (red[1][0][r] + red[1][1][r]) + (red[1][2][r] + red[1][3][r]);
+    const int64_t at = (grp * a.nsplit + split) * kCcRows + r;
     if (a.nsplit == 1) {
-      out_at(r, d) = from_f<T>(pos_s[r] >= 0 && L != 0.f ? O / L : 0.f);
+      const int gr = row0 + r, t = gr / a.G, g = gr % a.G;
+      reinterpret_cast<float*>(a.out)[(((int64_t)b * a.T + t) * a.hq + head * a.G + g) * D + d] =
+          pos_s[r] >= 0 && L != 0.f ? O / L : 0.f;
     } else {
-      a.ws_o[((grp * a.nsplit + split) * kCcRows + r) * D + d] = O;
-      if (d == 0) a.ws_ml[(grp * a.nsplit + split) * kCcRows + r] = make_float4(M, M, L, 0.f);
+      a.ws_o[at * D + d] = O;
+      if (d == 0) {
+        const float M = fmaxf(fmaxf(red[0][0][r], red[0][1][r]), fmaxf(red[0][2][r], red[0][3][r]));
+        a.ws_ml[at] = make_float4(M, M, L, 0.f);
+      }
     }
   }
 }
-
 
 // ------------------------------------------------------------------ few query rows (bf16): decode and verify
 // Bound by HBM: every K and V byte of the context is read once for up to 8 NT rows.  The transposed products
@@ -348,9 +381,6 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
-// Bytes of w that are e4m3 NaN (0x7f, 0xff), as 0x80 marks.
-__device__ __forceinline__ uint32_t nan_marks(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
-__device__ __forceinline__ uint32_t clear_nan(uint32_t w) { return w & ~((nan_marks(w) >> 7) * 0xffu); }
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool there) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
@@ -1520,26 +1550,11 @@ Kv8Layout kv8_layout(bool cc, int B, int T, int hq, int hkv, int D, int max_seq_
   return L;
 }
 
-template <typename T, int D>
+template <int D>
 int launch_cc(cudaStream_t st, const Kv8Attn& a, int B) {
   const dim3 grid(a.nsplit, a.c.hkv * a.row_groups, B);
-  SSD_PDL((kv8_attention_cc_kernel<T, D>), grid, kCcWarps * 32, 0, st, a);
-  return a.nsplit == 1 ? SSD_OK : launch_join<T, D, kCcRows, false>(st, a, B);
-}
-
-// A kernel's dynamic shared memory limit belongs to each device's context: raised once per device (`ready`: one
-// bit a device), always to the same size.
-template <typename K>
-bool allow_smem(std::atomic<uint64_t>& ready, K kern, int bytes) {
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return false;
-  if (ready.load(std::memory_order_acquire) >> dev & 1) return true;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) {
-    (void)cudaGetLastError();
-    return false;
-  }
-  ready.fetch_or(1ull << dev, std::memory_order_release);
-  return true;
+  SSD_PDL(kv8_attention_cc_kernel<D>, grid, kCcSplit, 0, st, a);
+  return a.nsplit == 1 ? SSD_OK : launch_join<float, D, kCcRows, false>(st, a, B);
 }
 
 template <int D, int NT, bool UNI>
@@ -1628,7 +1643,7 @@ extern "C" int ssd_kv8_attention(ssd_stream_t stream, const void* q, const void*
     if (head_dim == 128) return launch_bf16<128>(st, a, L, B);
     return launch_bf16<64>(st, a, L, B);
   }
-  if (head_dim == 256) return launch_cc<float, 256>(st, a, B);
-  if (head_dim == 128) return launch_cc<float, 128>(st, a, B);
-  return launch_cc<float, 64>(st, a, B);
+  if (head_dim == 256) return launch_cc<256>(st, a, B);
+  if (head_dim == 128) return launch_cc<128>(st, a, B);
+  return launch_cc<64>(st, a, B);
 }

@@ -3,7 +3,7 @@
 //
 // A page is a run of `page_bytes` at a fixed stride in each of `planes` arrays (K and V of every layer), so
 // the copies know nothing of the element type; an 8-bit cache's scales are a second, small set of runs.
-#include "common.cuh"
+#include "kv8.cuh"
 
 namespace ssd {
 namespace {
@@ -25,33 +25,50 @@ struct CopyArgs {
   const int32_t* count;          // pairs on the device, or NULL (= n)
   int n, planes;
   int src_blocks, dst_blocks;
-  int parts;                     // CTAs a page of one plane is cut into
+  int parts;                     // CTAs a pair is cut into
 };
 
-// One CTA per (pair, plane, part).  Pairs with an id out of range on either side (-1) are skipped.
+// One CTA per (pair, part): a part is kCopyItems vectors a thread out of the pair's pages in all planes, their loads
+// in flight together (a page of one plane may be small: 8 KB pages, one plane a CTA, reached 3.0 TB/s).  Pairs
+// with an id out of range on either side (-1) are skipped.  Bound: HBM.
+constexpr int kCopyItems = 8;
+
 template <typename V>
 __global__ void __launch_bounds__(kCopyThreads) page_copy_kernel(const CopyArgs a) {
   pdl_wait();
   pdl_trigger();
-  const int n = a.count ? min(ld_act(a.count), a.n) : a.n;
-  const int64_t work = (int64_t)n * a.planes * a.parts;
-  for (int64_t w = blockIdx.x; w < work; w += gridDim.x) {
-    const int part = (int)(w % a.parts);
-    const int64_t pp = w / a.parts;
-    const int plane = (int)(pp % a.planes), i = (int)(pp / a.planes);
-    const int s = ld_act(a.src_ids + i * a.src_step), d = ld_act(a.dst_ids + i * a.dst_step);
-    if ((unsigned)s >= (unsigned)a.src_blocks || (unsigned)d >= (unsigned)a.dst_blocks) continue;
-    const V* from = reinterpret_cast<const V*>(a.data.src + plane * a.data.src_plane + s * a.data.bytes);
-    V* to = reinterpret_cast<V*>(a.data.dst + plane * a.data.dst_plane + d * a.data.bytes);
-    if (from == to) continue;
-    const int64_t items = a.data.bytes / (int64_t)sizeof(V);
-    const int64_t per = (items + a.parts - 1) / a.parts;
-    const int64_t end = min(items, (part + 1) * per);
-    for (int64_t k = part * per + threadIdx.x; k < end; k += kCopyThreads) to[k] = __ldcg(from + k);
-    if (part == 0 && a.scales.bytes) {
-      const float* fs = reinterpret_cast<const float*>(a.scales.src + plane * a.scales.src_plane + s * a.scales.bytes);
-      float* ts = reinterpret_cast<float*>(a.scales.dst + plane * a.scales.dst_plane + d * a.scales.bytes);
-      for (int k = threadIdx.x; k < a.scales.bytes / 4; k += kCopyThreads) ts[k] = __ldcg(fs + k);
+  const int i = (int)(blockIdx.x / a.parts), part = (int)(blockIdx.x % a.parts);
+  // ids past the count are read too (they are there) so that the two loads do not wait for each other
+  const int s = ld_act(a.src_ids + i * a.src_step), d = ld_act(a.dst_ids + i * a.dst_step);
+  if (a.count && i >= ld_act(a.count)) return;
+  if ((unsigned)s >= (unsigned)a.src_blocks || (unsigned)d >= (unsigned)a.dst_blocks) return;
+  const int64_t items = a.data.bytes / (int64_t)sizeof(V), total = items * a.planes;
+  const char* from = a.data.src + s * a.data.bytes;
+  char* to = a.data.dst + d * a.data.bytes;
+  if (from == to && a.data.src == a.data.dst) return;
+  const int64_t k0 = (int64_t)part * (kCopyItems * kCopyThreads) + threadIdx.x;
+  V x[kCopyItems];
+  int64_t at[kCopyItems];
+#pragma unroll
+  for (int q = 0; q < kCopyItems; ++q) {
+    const int64_t k = k0 + q * kCopyThreads;
+    at[q] = -1;
+    if (k < total) {
+      const int plane = total <= 0xffffffffll ? (int)((uint32_t)k / (uint32_t)items) : (int)(k / items);
+      const int64_t off = (k - plane * items) * (int64_t)sizeof(V);
+      x[q] = __ldcg(reinterpret_cast<const V*>(from + plane * a.data.src_plane + off));
+      at[q] = plane * a.data.dst_plane + off;
+    }
+  }
+#pragma unroll
+  for (int q = 0; q < kCopyItems; ++q)
+    if (at[q] >= 0) *reinterpret_cast<V*>(to + at[q]) = x[q];
+  if (part == 0 && a.scales.bytes) {
+    const int per = (int)(a.scales.bytes / 4);
+    for (int k = threadIdx.x; k < per * a.planes; k += kCopyThreads) {
+      const int plane = k / per, h = k - plane * per;
+      reinterpret_cast<float*>(a.scales.dst + plane * a.scales.dst_plane + d * a.scales.bytes)[h] =
+          __ldcg(reinterpret_cast<const float*>(a.scales.src + plane * a.scales.src_plane + s * a.scales.bytes) + h);
     }
   }
 }
@@ -59,14 +76,25 @@ __global__ void __launch_bounds__(kCopyThreads) page_copy_kernel(const CopyArgs 
 // ---------------------------------------------------------------------------------------- compaction
 // U = blocks not on the free list.  The k-th of them at U or above (ascending) moves to the k-th free block
 // below U: the fewest moves there can be, and no block is both read and written.  One CTA: the pool's state
-// is a few integers per block; each thread owns a run of blocks, ranks come from one block-wide scan.
+// is a few integers per block; each thread owns a run of blocks, ranks come from block-wide scans, and what is
+// free or used is kept in shared memory (a byte a block; pools past kFlagCap in the remap array itself).  The
+// same CTA then rewrites the tables.
 constexpr int kPlanThreads = 1024;
+constexpr int kFlagCap = 160 * 1024;
+
+struct TableArgs {
+  const int32_t* in;
+  int32_t* out;
+  const int32_t* lens;
+  int rows, max_blocks;
+};
 
 struct CompactArgs {
   const int32_t *free_list, *free_top, *ref_counts;
   int32_t *free_list_out, *free_top_out, *ref_counts_out;
   int32_t *remap, *src, *dst, *moves;  // [num_blocks], [num_blocks / 2], [num_blocks / 2], [1]
   int num_blocks;
+  TableArgs tables[2];                 // tables that this kernel rewrites (rows = 0: none)
 };
 
 __device__ __forceinline__ int2 block_scan2(int2 v, int2* tmp, int2* total) {
@@ -95,44 +123,64 @@ __device__ __forceinline__ int2 block_scan2(int2 v, int2* tmp, int2* total) {
   return make_int2(base.x + x.x - v.x, base.y + x.y - v.y);  // exclusive
 }
 
+// out[b][i] = remap[in[b][i]] for i < lens[b], -1 behind (ids out of range become -1).
+__device__ __forceinline__ void remap_entry(const TableArgs& t, int64_t e, const int32_t* remap, int num_blocks) {
+  const int b = (int)(e / t.max_blocks), i = (int)(e % t.max_blocks);
+  const int blk = i < ld_act(t.lens + b) ? ld_act(t.in + e) : -1;
+  t.out[e] = (unsigned)blk < (unsigned)num_blocks ? ld_act(remap + blk) : -1;
+}
+
+template <bool SMEM>
 __global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(const CompactArgs a) {
+  extern __shared__ uint8_t used_s[];
   __shared__ int2 tmp[32];
   pdl_wait();
   const int nb = a.num_blocks, tid = threadIdx.x;
+  auto is_used = [&](int i) { return SMEM ? used_s[i] != 0 : a.remap[i] >= 0; };
+  for (int i = tid; i < nb; i += kPlanThreads) {
+    if (SMEM) used_s[i] = 1;
+    else a.remap[i] = i;
+  }
   const int top = min(max(ld_act(a.free_top), 0), nb);
-  for (int i = tid; i < nb; i += kPlanThreads) a.remap[i] = i;
   __syncthreads();
-  for (int i = tid; i < top; i += kPlanThreads) {
-    const int f = ld_act(a.free_list + i);
-    if ((unsigned)f < (unsigned)nb) a.remap[f] = -1;
+  for (int i = tid; i < nb; i += kPlanThreads) {
+    const int f = ld_act(a.free_list + i);  // entries past the top are read and dropped
+    if (i < top && (unsigned)f < (unsigned)nb) {
+      if (SMEM) used_s[f] = 0;
+      else a.remap[f] = -1;
+    }
   }
   __syncthreads();
   const int per = (nb + kPlanThreads - 1) / kPlanThreads;
   const int i0 = min(nb, tid * per), i1 = min(nb, i0 + per);
   int used = 0;
-  for (int i = i0; i < i1; ++i) used += a.remap[i] >= 0;
+  for (int i = i0; i < i1; ++i) used += is_used(i);
   int2 total;
   block_scan2(make_int2(used, 0), tmp, &total);
   const int U = total.x;
   // free blocks below U, used blocks at or above it
   int2 mine = make_int2(0, 0);
   for (int i = i0; i < i1; ++i) {
-    const bool u = a.remap[i] >= 0;
+    const bool u = is_used(i);
     mine.x += !u && i < U;
     mine.y += u && i >= U;
   }
   int2 at = block_scan2(mine, tmp, &total);
   for (int i = i0; i < i1; ++i) {
-    const bool u = a.remap[i] >= 0;
+    const bool u = is_used(i);
     if (!u && i < U) a.dst[at.x++] = i;
     if (u && i >= U) a.src[at.y++] = i;
   }
-  __syncthreads();
-  const int n = total.y;  // == total.x: both count U minus the used blocks below U
-  for (int i = tid; i < nb; i += kPlanThreads)
+  for (int i = tid; i < nb; i += kPlanThreads) {
+    if (SMEM) a.remap[i] = is_used(i) ? i : -1;
     a.free_list_out[i] = i < nb - U ? nb - 1 - i : -1;  // pops hand out U, U + 1, ...
-  if (a.ref_counts_out != a.ref_counts)
-    for (int i = tid; i < nb; i += kPlanThreads) a.ref_counts_out[i] = ld_act(a.ref_counts + i);
+    if (a.ref_counts_out != a.ref_counts) a.ref_counts_out[i] = ld_act(a.ref_counts + i);
+  }
+  const int n = total.y;  // == total.x: both count U minus the used blocks below U
+  if (tid == 0) {
+    *a.moves = n;
+    *a.free_top_out = nb - U;
+  }
   __syncthreads();
   for (int k = tid; k < n; k += kPlanThreads) {
     const int s = a.src[k], d = a.dst[k];
@@ -140,32 +188,29 @@ __global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(const Compac
     a.ref_counts_out[d] = ld_act(a.ref_counts + s);
     a.ref_counts_out[s] = 0;
   }
-  if (tid == 0) {
-    *a.moves = n;
-    *a.free_top_out = nb - U;
-  }
   pdl_trigger();
+  __syncthreads();
+  for (int x = 0; x < 2; ++x) {
+    const int64_t entries = (int64_t)a.tables[x].rows * a.tables[x].max_blocks;
+    for (int64_t e = tid; e < entries; e += kPlanThreads) remap_entry(a.tables[x], e, a.remap, nb);
+  }
 }
 
-// out[b][i] = remap[in[b][i]] for i < lens[b], -1 behind (ids out of range become -1).
-__global__ void table_remap_kernel(const int32_t* in, int32_t* out, const int32_t* lens, int64_t entries,
-                                   int max_blocks, const int32_t* remap, int num_blocks) {
+__global__ void table_remap_kernel(const TableArgs t, const int32_t* remap, int num_blocks) {
   pdl_wait();
   pdl_trigger();
-  for (int64_t e = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; e < entries; e += (int64_t)gridDim.x * blockDim.x) {
-    const int b = (int)(e / max_blocks), i = (int)(e % max_blocks);
-    const int blk = i < ld_act(lens + b) ? ld_act(in + e) : -1;
-    out[e] = (unsigned)blk < (unsigned)num_blocks ? ld_act(remap + blk) : -1;
-  }
+  const int64_t entries = (int64_t)t.rows * t.max_blocks;
+  for (int64_t e = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; e < entries; e += (int64_t)gridDim.x * blockDim.x)
+    remap_entry(t, e, remap, num_blocks);
 }
 
 template <typename V>
 int launch_copy(cudaStream_t st, CopyArgs a) {
-  const int64_t items = a.data.bytes / (int64_t)sizeof(V);
-  // a CTA moves up to 16 vectors a thread; small pages take one CTA
-  a.parts = (int)((items + kCopyThreads * 16 - 1) / (kCopyThreads * 16));
-  const int64_t work = (int64_t)a.n * a.planes * a.parts;
-  SSD_PDL(page_copy_kernel<V>, (unsigned)(work < (1 << 20) ? work : (1 << 20)), kCopyThreads, 0, st, a);
+  const int64_t items = a.data.bytes / (int64_t)sizeof(V) * a.planes;
+  const int64_t parts = (items + kCopyThreads * kCopyItems - 1) / (kCopyThreads * kCopyItems);
+  if (parts * a.n > 0x7fffffff) return SSD_ERR_UNSUPPORTED;
+  a.parts = (int)parts;
+  SSD_PDL(page_copy_kernel<V>, (unsigned)(parts * a.n), kCopyThreads, 0, st, a);
   return SSD_OK;
 }
 
@@ -218,24 +263,38 @@ extern "C" int ssd_page_copy(ssd_stream_t stream, const void* src_pages, const f
 extern "C" int ssd_page_compact(ssd_stream_t stream, const int32_t* free_list, const int32_t* free_top,
                                 const int32_t* ref_counts, int num_blocks, int32_t* free_list_out,
                                 int32_t* free_top_out, int32_t* ref_counts_out, int32_t* remap, int32_t* move_src,
-                                int32_t* move_dst, int32_t* num_moves) {
+                                int32_t* move_dst, int32_t* num_moves, const int32_t* tables, int32_t* tables_out,
+                                const int32_t* lens, int max_blocks, int B, const int32_t* draft_tables,
+                                int32_t* draft_tables_out, const int32_t* draft_lens, int draft_max_blocks,
+                                int draft_B) {
   if (num_blocks <= 0 || !free_list || !free_top || !ref_counts || !free_list_out || !free_top_out ||
-      !ref_counts_out || !remap || !move_src || !move_dst || !num_moves)
+      !ref_counts_out || !remap || !move_src || !move_dst || !num_moves || B < 0 || draft_B < 0)
     return SSD_ERR_INVALID;
-  const CompactArgs a{free_list, free_top, ref_counts, free_list_out, free_top_out, ref_counts_out,
-                      remap, move_src, move_dst, num_moves, num_blocks};
-  SSD_PDL(compact_plan_kernel, 1, kPlanThreads, 0, (cudaStream_t)stream, a);
-  return SSD_OK;
-}
-
-extern "C" int ssd_page_remap(ssd_stream_t stream, const int32_t* tables, int32_t* tables_out, const int32_t* lens,
-                              int max_blocks, int B, const int32_t* remap, int num_blocks) {
-  if (B < 0 || max_blocks <= 0 || num_blocks <= 0) return SSD_ERR_INVALID;
-  if (B == 0) return SSD_OK;
-  if (!tables || !tables_out || !lens || !remap) return SSD_ERR_INVALID;
-  const int64_t entries = (int64_t)B * max_blocks;
-  const int64_t ctas = (entries + 255) / 256;
-  SSD_PDL(table_remap_kernel, (unsigned)(ctas < 1184 ? ctas : 1184), 256, 0, (cudaStream_t)stream, tables, tables_out,
-          lens, entries, max_blocks, remap, num_blocks);
+  if (B > 0 && (!tables || !tables_out || !lens || max_blocks <= 0)) return SSD_ERR_INVALID;
+  if (draft_B > 0 && (!draft_tables || !draft_tables_out || !draft_lens || draft_max_blocks <= 0))
+    return SSD_ERR_INVALID;
+  cudaStream_t st = (cudaStream_t)stream;
+  CompactArgs a{free_list, free_top, ref_counts, free_list_out, free_top_out, ref_counts_out,
+                remap, move_src, move_dst, num_moves, num_blocks, {}};
+  const TableArgs t[2] = {{tables, tables_out, lens, B, max_blocks},
+                          {draft_tables, draft_tables_out, draft_lens, draft_B, draft_max_blocks}};
+  // up to 16 entries a thread in the plan's own CTA; larger tables get a launch of their own
+  bool own[2];
+  for (int x = 0; x < 2; ++x) {
+    own[x] = (int64_t)t[x].rows * t[x].max_blocks > 16 * kPlanThreads;
+    if (!own[x]) a.tables[x] = t[x];
+  }
+  if (num_blocks <= kFlagCap) {
+    static std::atomic<uint64_t> ready{0};
+    if (num_blocks > 40 * 1024 && !allow_smem(ready, compact_plan_kernel<true>, kFlagCap)) return SSD_ERR_LAUNCH;
+    SSD_PDL(compact_plan_kernel<true>, 1, kPlanThreads, num_blocks, st, a);
+  } else {
+    SSD_PDL(compact_plan_kernel<false>, 1, kPlanThreads, 0, st, a);
+  }
+  for (int x = 0; x < 2; ++x) {
+    if (!own[x]) continue;
+    const int64_t ctas = ((int64_t)t[x].rows * t[x].max_blocks + 255) / 256;
+    SSD_PDL(table_remap_kernel, (unsigned)(ctas < 1184 ? ctas : 1184), 256, 0, st, t[x], remap, num_blocks);
+  }
   return SSD_OK;
 }

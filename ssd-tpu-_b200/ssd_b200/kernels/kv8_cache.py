@@ -16,21 +16,32 @@ the cache's device and keeps nothing of its arguments.
 
 from __future__ import annotations
 
-import contextlib
-from dataclasses import dataclass
+from dataclasses import dataclass, field
 
 import torch
 
-from .._lib import check, dtype_code, lib, ptr
+from .._lib import check, dtype_code, lib
 
 
-@dataclass
+@dataclass(frozen=True)
 class KV8CacheState:
     """Paged e4m3 cache and its scales, [2, L, num_blocks, block_size, Hkv, D] and [2, L, num_blocks, Hkv]."""
 
     pages: torch.Tensor
     scales: torch.Tensor
     block_size: int
+    # (device index, -1 on the CPU; pages, scales: pointers; layers, blocks, block size, KV heads, head dim)
+    dims: tuple = field(init=False, repr=False, compare=False)
+
+    def __post_init__(self) -> None:
+        p, s = self.pages, self.scales
+        if (p.dtype != torch.float8_e4m3fn or s.dtype != torch.float32 or p.dim() != 6 or not p.is_contiguous()
+                or not s.is_contiguous() or s.device != p.device):
+            raise ValueError("an 8-bit cache is contiguous e4m3 pages [2, L, NB, BS, Hkv, D] and fp32 scales on one GPU")
+        two, nl, nb, bs, hkv, hd = p.shape
+        if two != 2 or bs != self.block_size or s.shape != (2, nl, nb, hkv):
+            raise ValueError(f"scales {tuple(s.shape)} and block_size {self.block_size} do not fit pages {tuple(p.shape)}")
+        object.__setattr__(self, "dims", (p.get_device(), p.data_ptr(), s.data_ptr(), nl, nb, bs, hkv, hd))
 
     @classmethod
     def allocate(cls, num_layers: int, num_blocks: int, block_size: int, num_kv_heads: int, head_dim: int,
@@ -49,45 +60,44 @@ class KV8CacheState:
         return self.pages.shape[1]
 
 
-_NO_GUARD = contextlib.nullcontext()
+def launch(name: str, dev: int, *args) -> None:
+    """Call a C entry point on the current stream of GPU ``dev``; raise for its status."""
+    if dev < 0:
+        raise ValueError(f"{name}: the tensors must be on a GPU")
+    fn = getattr(lib(), name)
+    if dev == torch.cuda.current_device():
+        rc = fn(torch.cuda.current_stream(dev).cuda_stream, *args)
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(torch.cuda.current_stream(dev).cuda_stream, *args)
+    if rc:
+        check(rc, name)
 
 
-def on_device(dev: torch.device):
-    """A context with ``dev`` current (nothing to do when it already is, the usual case)."""
-    return _NO_GUARD if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
-
-
-def _stream(dev: torch.device) -> int:
-    return torch.cuda.current_stream(dev).cuda_stream
-
-
-def _cache_dims(cache: KV8CacheState):
-    p, s = cache.pages, cache.scales
-    if (p.dtype != torch.float8_e4m3fn or s.dtype != torch.float32 or p.dim() != 6 or not p.is_contiguous()
-            or not s.is_contiguous() or not p.is_cuda or s.device != p.device):
-        raise ValueError("an 8-bit cache is contiguous e4m3 pages [2, L, NB, BS, Hkv, D] and fp32 scales on one GPU")
-    two, nl, nb, bs, hkv, hd = p.shape
-    if two != 2 or bs != cache.block_size or s.shape != (2, nl, nb, hkv):
-        raise ValueError(f"scales {tuple(s.shape)} and block_size {cache.block_size} do not fit pages {tuple(p.shape)}")
-    return nl, nb, bs, hkv, hd
-
-
-def _ints(t: torch.Tensor | None, shape: tuple, what: str, dev: torch.device) -> int | None:
-    """Pointer of an int32 device array of the shape (-1: any size)."""
+def ints(t: torch.Tensor | None, shape: tuple, what: str, dev: int) -> int | None:
+    """Pointer of a contiguous int32 array of the shape on GPU ``dev`` (None for None)."""
     if t is None:
         return None
-    if (t.dtype != torch.int32 or t.device != dev or t.dim() != len(shape)
-            or any(n >= 0 and n != m for n, m in zip(shape, t.shape)) or not t.is_contiguous()):
-        raise ValueError(f"{what} must be a contiguous int32 tensor {list(shape)} on {dev}, got "
+    if t.dtype is not torch.int32 or t.get_device() != dev or t.shape != shape or not t.is_contiguous():
+        raise ValueError(f"{what} must be a contiguous int32 tensor {list(shape)} on cuda:{dev}, got "
                          f"{t.dtype} {list(t.shape)} on {t.device}")
     return t.data_ptr()
 
 
-def _rows(t: torch.Tensor, what: str, dev: torch.device) -> torch.Tensor:
-    if t.device != dev:
-        raise ValueError(f"{what} is on {t.device}, the cache on {dev}")
-    t = t.contiguous()
+def _rows(t: torch.Tensor, what: str, dev: int) -> torch.Tensor:
+    if t.get_device() != dev:
+        raise ValueError(f"{what} is on {t.device}, the cache on cuda:{dev}")
+    if not t.is_contiguous():
+        return t.contiguous()
     return t.clone() if t.data_ptr() & 15 else t  # the kernels move 16 bytes at a time
+
+
+def _tables(t: torch.Tensor, b: int, dev: int) -> tuple[int, int]:
+    """(pointer, columns) of block tables [b, max_blocks]."""
+    if t.dim() != 2:
+        raise ValueError(f"block_tables must be [{b}, max_blocks], got {list(t.shape)}")
+    m = t.shape[1]
+    return ints(t, (b, m), "block_tables", dev), m
 
 
 def append_kv8(cache: KV8CacheState, layer: int, block_tables: torch.Tensor, seq_lens: torch.Tensor,
@@ -96,19 +106,18 @@ def append_kv8(cache: KV8CacheState, layer: int, block_tables: torch.Tensor, seq
 
     Token t < q_lens[b] (None: T) of row b goes to position seq_lens[b] - q_lens[b] + t; ``seq_lens``
     counts the new tokens, as for ``paged_kv8_attention``.  A page whose first row is among the new
-    ones starts over; in any other page the earlier rows keep their values.
+    ones starts over; in any other page the earlier rows keep their values.  A page that is written
+    belongs to one sequence (fork a shared one first, ``PageManager.fork_rows``).
     """
-    nl, nb, bs, hkv, hd = _cache_dims(cache)
-    dev = cache.pages.device
-    if k.dim() != 4 or k.shape[2:] != (hkv, hd) or v.shape != k.shape or v.dtype != k.dtype:
+    dev, pages, scales, nl, nb, bs, hkv, hd = cache.dims
+    if k.dim() != 4 or k.shape[2] != hkv or k.shape[3] != hd or v.shape != k.shape or v.dtype != k.dtype:
         raise ValueError(f"k and v must be [B, T, {hkv}, {hd}] of one dtype, got {list(k.shape)} and {list(v.shape)}")
-    b, t = k.shape[:2]
+    b, t = k.shape[0], k.shape[1]
     k, v = _rows(k, "k", dev), _rows(v, "v", dev)
-    with on_device(dev):
-        check(lib().ssd_kv8_append(_stream(dev), ptr(cache.pages), ptr(cache.scales), nl, nb, bs, hkv, hd, layer,
-                                   _ints(block_tables, (b, -1), "block_tables", dev), block_tables.shape[1],
-                                   _ints(seq_lens, (b,), "seq_lens", dev), _ints(q_lens, (b,), "q_lens", dev),
-                                   ptr(k), ptr(v), dtype_code(k.dtype), b, t), "ssd_kv8_append")
+    tab, cols = _tables(block_tables, b, dev)
+    launch("ssd_kv8_append", dev, pages, scales, nl, nb, bs, hkv, hd, layer, tab, cols,
+           ints(seq_lens, (b,), "seq_lens", dev), ints(q_lens, (b,), "q_lens", dev), k.data_ptr(), v.data_ptr(),
+           dtype_code(k.dtype), b, t)
     return cache
 
 
@@ -117,45 +126,42 @@ def rope_append_kv8(qkv: torch.Tensor, cache: KV8CacheState, layer: int, block_t
                     q_lens: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """RoPE on the q and k parts of qkv [B*T, (Hq+2Hkv)*D], k and v appended to the cache
     (``ssd_kv8_rope_append``); returns the rotated q [B, T, Hq, D] (zeros for t >= q_lens[b])."""
-    nl, nb, bs, hkv, hd = _cache_dims(cache)
-    dev = cache.pages.device
+    dev, pages, scales, nl, nb, bs, hkv, hd = cache.dims
     b = block_tables.shape[0]
-    if qkv.dim() != 2 or qkv.shape[1] != (num_heads + 2 * hkv) * hd or (b == 0) != (qkv.shape[0] == 0) or (
-            b and qkv.shape[0] % b):
-        raise ValueError(f"qkv must be [B*T, {(num_heads + 2 * hkv) * hd}] for {b} sequences, got {list(qkv.shape)}")
+    width = (num_heads + 2 * hkv) * hd
+    if qkv.dim() != 2 or qkv.shape[1] != width or (qkv.shape[0] % b if b else qkv.shape[0]):
+        raise ValueError(f"qkv must be [B*T, {width}] for {b} sequences, got {list(qkv.shape)}")
     t = qkv.shape[0] // b if b else 0
+    max_pos = rope_cos.shape[0]
     for tab, name in ((rope_cos, "rope_cos"), (rope_sin, "rope_sin")):
-        if (tab.dtype != torch.float32 or tab.device != dev or tab.shape != (rope_cos.shape[0], hd // 2)
+        if (tab.dtype is not torch.float32 or tab.get_device() != dev or tab.shape != (max_pos, hd // 2)
                 or not tab.is_contiguous()):
-            raise ValueError(f"{name} must be a contiguous fp32 tensor [positions, {hd // 2}] on {dev}")
+            raise ValueError(f"{name} must be a contiguous fp32 tensor [positions, {hd // 2}] on cuda:{dev}")
     qkv = _rows(qkv, "qkv", dev)
     if out is None:
-        out = torch.empty((b, t, num_heads, hd), dtype=qkv.dtype, device=dev)
-    elif (out.shape != (b, t, num_heads, hd) or out.dtype != qkv.dtype or out.device != dev
+        out = torch.empty((b, t, num_heads, hd), dtype=qkv.dtype, device=qkv.device)
+    elif (out.shape != (b, t, num_heads, hd) or out.dtype != qkv.dtype or out.get_device() != dev
           or not out.is_contiguous()):
-        raise ValueError(f"out must be a contiguous {qkv.dtype} tensor [{b}, {t}, {num_heads}, {hd}] on {dev}")
-    with on_device(dev):
-        check(lib().ssd_kv8_rope_append(_stream(dev), ptr(qkv), ptr(out), ptr(cache.pages), ptr(cache.scales),
-                                        dtype_code(qkv.dtype), nl, nb, bs, num_heads, hkv, hd, layer,
-                                        _ints(block_tables, (b, -1), "block_tables", dev), block_tables.shape[1],
-                                        _ints(seq_lens, (b,), "seq_lens", dev), _ints(q_lens, (b,), "q_lens", dev),
-                                        ptr(rope_cos), ptr(rope_sin), rope_cos.shape[0], b, t), "ssd_kv8_rope_append")
+        raise ValueError(f"out must be a contiguous {qkv.dtype} tensor [{b}, {t}, {num_heads}, {hd}] on cuda:{dev}")
+    tab, cols = _tables(block_tables, b, dev)
+    launch("ssd_kv8_rope_append", dev, qkv.data_ptr(), out.data_ptr(), pages, scales, dtype_code(qkv.dtype), nl, nb,
+           bs, num_heads, hkv, hd, layer, tab, cols, ints(seq_lens, (b,), "seq_lens", dev),
+           ints(q_lens, (b,), "q_lens", dev), rope_cos.data_ptr(), rope_sin.data_ptr(), max_pos, b, t)
     return out
 
 
 def gather_kv8(cache: KV8CacheState, layer: int, block_tables: torch.Tensor, positions: torch.Tensor,
                dtype=torch.bfloat16) -> tuple[torch.Tensor, torch.Tensor]:
     """K and V rows [B, N, Hkv, D] of positions [B, N] (-1: zeros), as the values the cache holds (``ssd_kv8_gather``)."""
-    nl, nb, bs, hkv, hd = _cache_dims(cache)
-    dev = cache.pages.device
+    dev, pages, scales, nl, nb, bs, hkv, hd = cache.dims
+    if positions.dim() != 2:
+        raise ValueError(f"positions must be [B, N], got {list(positions.shape)}")
     b, n = positions.shape
-    k = torch.empty((b, n, hkv, hd), dtype=dtype, device=dev)
-    v = torch.empty((b, n, hkv, hd), dtype=dtype, device=dev)
-    with on_device(dev):
-        check(lib().ssd_kv8_gather(_stream(dev), ptr(cache.pages), ptr(cache.scales), nl, nb, bs, hkv, hd, layer,
-                                   _ints(block_tables, (b, -1), "block_tables", dev), block_tables.shape[1],
-                                   _ints(positions, (b, n), "positions", dev), ptr(k), ptr(v), dtype_code(dtype), b,
-                                   n), "ssd_kv8_gather")
+    kv = torch.empty((2, b, n, hkv, hd), dtype=dtype, device=cache.pages.device)
+    k, v = kv.unbind(0)
+    tab, cols = _tables(block_tables, b, dev)
+    launch("ssd_kv8_gather", dev, pages, scales, nl, nb, bs, hkv, hd, layer, tab, cols,
+           ints(positions, (b, n), "positions", dev), k.data_ptr(), v.data_ptr(), dtype_code(dtype), b, n)
     return k, v
 
 
@@ -166,30 +172,24 @@ def paged_kv8_attention(q: torch.Tensor, cache: KV8CacheState, layer: int, block
 
     Arguments as ``paged_verify_attention``: seq_lens [B] counts cached tokens INCLUDING the new
     ones; new token t of sequence b sits at position seq_lens[b] - q_lens[b] + t.  Rows past
-    q_lens[b] come back as zeros.
+    q_lens[b] come back as zeros.  For T up to 8 a query's bits do not depend on how many new tokens
+    stand beside it.
     """
-    nl, nb, bs, hkv, hd = _cache_dims(cache)
-    dev = cache.pages.device
+    dev, pages, scales, nl, nb, bs, hkv, hd = cache.dims
     if q.dim() != 4 or q.shape[3] != hd:
         raise ValueError(f"q must be [B, T, Hq, {hd}], got {list(q.shape)}")
     b, t, hq, _ = q.shape
-    if max_seq_len is None:
-        max_seq_len = block_tables.shape[1] * bs
-    if scale is None:
-        scale = 1.0 / float(hd) ** 0.5
     q = _rows(q, "q", dev)
+    tab, cols = _tables(block_tables, b, dev)
+    max_seq_len = cols * bs if max_seq_len is None else int(max_seq_len)
     if out is None:
         out = torch.empty_like(q)
-    elif out.shape != q.shape or out.dtype != q.dtype or out.device != dev or not out.is_contiguous():
-        raise ValueError(f"out must be a contiguous {q.dtype} tensor {list(q.shape)} on {dev}")
-    with on_device(dev):
-        # a workspace of its own for every call: calls on other streams or in captured graphs share nothing
-        ws = torch.empty(lib().ssd_kv8_attention_workspace_size(b, t, hq, hkv, hd, int(max_seq_len)),
-                         dtype=torch.uint8, device=dev)
-        check(lib().ssd_kv8_attention(_stream(dev), ptr(q), ptr(cache.pages), ptr(cache.scales), dtype_code(q.dtype),
-                                      nl, nb, bs, hkv, hd, layer, _ints(block_tables, (b, -1), "block_tables", dev),
-                                      block_tables.shape[1], _ints(seq_lens, (b,), "seq_lens", dev),
-                                      _ints(q_lens, (b,), "q_lens", dev), ptr(out), float(scale), b, t, hq,
-                                      int(max_seq_len), ptr(ws), ws.numel()), "ssd_kv8_attention")
+    elif out.shape != q.shape or out.dtype != q.dtype or out.get_device() != dev or not out.is_contiguous():
+        raise ValueError(f"out must be a contiguous {q.dtype} tensor {list(q.shape)} on cuda:{dev}")
+    # a workspace of its own for every call: calls on other streams or in captured graphs share nothing
+    ws = torch.empty(lib().ssd_kv8_attention_workspace_size(b, t, hq, hkv, hd, max_seq_len), dtype=torch.uint8,
+                     device=q.device)
+    launch("ssd_kv8_attention", dev, q.data_ptr(), pages, scales, dtype_code(q.dtype), nl, nb, bs, hkv, hd, layer, tab,
+           cols, ints(seq_lens, (b,), "seq_lens", dev), ints(q_lens, (b,), "q_lens", dev), out.data_ptr(),
+           hd ** -0.5 if scale is None else float(scale), b, t, hq, max_seq_len, ws.data_ptr(), ws.numel())
     return out
-

@@ -10,31 +10,31 @@ from dataclasses import dataclass
 
 import torch
 
-from .._lib import check, lib, ptr
-from .kv8_cache import _ints, _stream, on_device
+from .kv8_cache import ints, launch
 
 
-def _pool(cache):
-    """(pages, scales or None, bytes of a page in one plane, scales of a page, planes)."""
+def _pool(cache) -> tuple:
+    """(device, pages, scales or None: pointers, blocks, planes, bytes of a page in one plane, scales of a page, rest)."""
     p = cache.pages
+    shape = p.shape
+    if len(shape) != 6 or not p.is_contiguous():
+        raise ValueError("a cache's pages are a contiguous tensor [2, L, NB, BS, Hkv, D]")
     s = getattr(cache, "scales", None)
-    if p.dim() != 6 or not p.is_contiguous() or not p.is_cuda:
-        raise ValueError("a cache's pages are a contiguous CUDA tensor [2, L, NB, BS, Hkv, D]")
-    if s is not None and (s.dtype != torch.float32 or s.shape != (*p.shape[:3], p.shape[4]) or s.device != p.device
+    if s is not None and (s.dtype is not torch.float32 or s.shape != (*shape[:3], shape[4]) or s.device != p.device
                           or not s.is_contiguous()):
-        raise ValueError(f"scales do not fit pages {tuple(p.shape)}")
-    return p, s, p.shape[3] * p.shape[4] * p.shape[5] * p.element_size(), 0 if s is None else p.shape[4]
+        raise ValueError(f"scales do not fit pages {tuple(shape)}")
+    return (p.get_device(), p.data_ptr(), None if s is None else s.data_ptr(), shape[2], 2 * shape[1],
+            shape[3] * shape[4] * shape[5] * p.element_size(), 0 if s is None else shape[4],
+            (p.dtype, shape[3], shape[4], shape[5]))
 
 
-def _copy(cache, dst_cache, src: int, src_step: int, dst: int, dst_step: int, n: int, count: int | None) -> None:
-    p, s, nbytes, nscales = _pool(cache)
-    dp, ds, dbytes, dscales = _pool(dst_cache)
-    if (dp.dtype != p.dtype or dp.shape[:2] != p.shape[:2] or dp.shape[3:] != p.shape[3:] or dscales != nscales
-            or dp.device != p.device):
-        raise ValueError(f"pages {tuple(dp.shape)} {dp.dtype} cannot take copies of pages {tuple(p.shape)} {p.dtype}")
-    check(lib().ssd_page_copy(_stream(p.device), ptr(p), ptr(s), p.shape[2], ptr(dp), ptr(ds), dp.shape[2],
-                              2 * p.shape[1], nbytes, nscales, src, src_step, dst, dst_step, n, count),
-          "ssd_page_copy")
+def _copy(src: tuple, dst: tuple, src_ids: int, src_step: int, dst_ids: int, dst_step: int, n: int,
+          count: int | None) -> None:
+    if dst is not src and (dst[0] != src[0] or dst[4:] != src[4:]):
+        raise ValueError("the caches' devices, layers or page shapes differ")
+    dev, p, s, nb, planes, nbytes, nscales, _ = src
+    launch("ssd_page_copy", dev, p, s, nb, dst[1], dst[2], dst[3], planes, nbytes, nscales, src_ids, src_step, dst_ids,
+           dst_step, n, count)
 
 
 def copy_pages(cache, src: torch.Tensor, dst: torch.Tensor, dst_cache=None):
@@ -45,13 +45,14 @@ def copy_pages(cache, src: torch.Tensor, dst: torch.Tensor, dst_cache=None):
     the same page shape to copy into.  Within one cache a page may not be both source and
     destination, nor a destination twice.  Returns the cache written to.
     """
-    dev = cache.pages.device
+    pool = _pool(cache)
+    n = src.shape[0] if src.dim() == 1 else -1
     for t, name in ((src, "src"), (dst, "dst")):
-        if t.dtype != torch.int32 or t.dim() != 1 or t.device != dev or t.shape != src.shape:
-            raise ValueError(f"{name} must be an int32 tensor [n] on {dev}")
+        if t.dtype is not torch.int32 or t.get_device() != pool[0] or t.shape != (n,):
+            raise ValueError(f"{name} must be an int32 tensor [n] on cuda:{pool[0]}, got {t.dtype} {list(t.shape)} on {t.device}")
     out = cache if dst_cache is None else dst_cache
-    with on_device(dev):
-        _copy(cache, out, src.data_ptr(), src.stride(0), dst.data_ptr(), dst.stride(0), src.shape[0], None)
+    _copy(pool, pool if out is cache else _pool(out), src.data_ptr(), src.stride(0), dst.data_ptr(), dst.stride(0), n,
+          None)
     return out
 
 
@@ -77,37 +78,39 @@ def compact_pages(cache, tables: torch.Tensor, lens: torch.Tensor, ref_counts: t
     ``free_list`` [num_blocks] and ``free_top`` [1] (the arrays of ``PageManager``) come back as new
     tensors, or are changed too with ``inplace``.  Every block that is not on the free list counts as
     in use.  The fewest pages move: the k-th used block at U or above to the k-th free one below U.
-    ``ssd_page_compact``, ``ssd_page_remap`` and ``ssd_page_copy``.
+    ``ssd_page_compact`` and ``ssd_page_copy``.
     """
-    caches = list(cache) if isinstance(cache, (list, tuple)) else [cache]
-    if not caches:
+    pools = [_pool(c) for c in cache] if isinstance(cache, (list, tuple)) else [_pool(cache)]
+    if not pools:
         raise ValueError("compact_pages wants a cache")
-    dev = caches[0].pages.device
-    nb = caches[0].pages.shape[2]
-    for c in caches:
-        if c.pages.shape[2] != nb or c.pages.device != dev:
-            raise ValueError("the caches of one pool have the same blocks and device")
+    dev, nb = pools[0][0], pools[0][3]
+    if any(p[0] != dev or p[3] != nb for p in pools):
+        raise ValueError("the caches of one pool have the same blocks and device")
     if (draft_tables is None) != (draft_lens is None):
         raise ValueError("draft_tables and draft_lens go together")
-    fl, ft = _ints(free_list, (nb,), "free_list", dev), _ints(free_top, (1,), "free_top", dev)
-    rc = _ints(ref_counts, (nb,), "ref_counts", dev)
-    pairs = [(tables, lens, "tables")] + ([] if draft_tables is None else [(draft_tables, draft_lens, "draft_tables")])
-    for t, n, name in pairs:
-        _ints(t, (n.shape[0], -1), name, dev)
-        _ints(n, (t.shape[0],), "lens of " + name, dev)
+    if tables.dim() != 2 or (draft_tables is not None and draft_tables.dim() != 2):
+        raise ValueError("tables are [rows, max_blocks]")
     half = max(1, nb // 2)
-    buf = torch.empty(nb + 2 * half + 1, dtype=torch.int32, device=dev)
-    remap, src, dst, count = buf[:nb], buf[nb:nb + half], buf[nb + half:nb + 2 * half], buf[nb + 2 * half:]
-    new = (lambda t: t) if inplace else torch.empty_like
-    free_list_out, free_top_out, ref_out = new(free_list), new(free_top), new(ref_counts)
-    outs = [new(t) for t, _, _ in pairs]
-    with on_device(dev):
-        st = _stream(dev)
-        check(lib().ssd_page_compact(st, fl, ft, rc, nb, ptr(free_list_out), ptr(free_top_out), ptr(ref_out),
-                                     ptr(remap), ptr(src), ptr(dst), ptr(count)), "ssd_page_compact")
-        for (t, n, _), o in zip(pairs, outs):
-            check(lib().ssd_page_remap(st, ptr(t), ptr(o), ptr(n), t.shape[1], t.shape[0], ptr(remap), nb),
-                  "ssd_page_remap")
-        for c in caches:
-            _copy(c, c, ptr(src), 1, ptr(dst), 1, nb // 2, ptr(count))
-    return Compaction(outs[0], ref_out, free_list_out, free_top_out, remap, outs[1] if len(outs) > 1 else None)
+    remap = torch.empty(nb, dtype=torch.int32, device=tables.device)
+    plan = torch.empty(2 * half + 1, dtype=torch.int32, device=tables.device)  # the moves' sources, targets, number
+    src = plan.data_ptr()
+    dst, count = src + 4 * half, src + 8 * half
+    if inplace:
+        out = Compaction(tables, ref_counts, free_list, free_top, remap, draft_tables)
+    else:
+        new = torch.empty_like
+        out = Compaction(new(tables), new(ref_counts), new(free_list), new(free_top), remap,
+                         None if draft_tables is None else new(draft_tables))
+    drafts = (None, None, None, 0, 0)
+    if draft_tables is not None:
+        rows, cols = draft_tables.shape
+        drafts = (ints(draft_tables, (rows, cols), "draft_tables", dev), out.draft_tables.data_ptr(),
+                  ints(draft_lens, (rows,), "draft_lens", dev), cols, rows)
+    rows, cols = tables.shape
+    launch("ssd_page_compact", dev, ints(free_list, (nb,), "free_list", dev), ints(free_top, (1,), "free_top", dev),
+           ints(ref_counts, (nb,), "ref_counts", dev), nb, out.free_list.data_ptr(), out.free_top.data_ptr(),
+           out.ref_counts.data_ptr(), remap.data_ptr(), src, dst, count, ints(tables, (rows, cols), "tables", dev),
+           out.tables.data_ptr(), ints(lens, (rows,), "lens", dev), cols, rows, *drafts)
+    for p in pools:
+        _copy(p, p, src, 1, dst, 1, nb // 2, count)
+    return out

@@ -93,10 +93,14 @@ def test_c_abi_refusals():
                 dict(did=None), dict(st=-1), dict(n=-1)):
         assert copy(**bad) == 1, bad
     assert copy(nbytes=(1 << 31) + 16) == 4
-    assert so.ssd_page_compact(None, P, P, P, 0, P, P, P, P, P, P, P) == 1
-    assert so.ssd_page_compact(None, P, P, P, 8, P, P, P, P, P, P, None) == 1
-    assert so.ssd_page_remap(None, P, P, P, 4, 0, P, 8) == 0
-    assert so.ssd_page_remap(None, P, None, P, 4, 1, P, 8) == 1
+
+    def compact(nb=8, out=P, tab=P, tab_out=P, lens=P, mb=4, rows=1, draft=None, drows=0):
+        return so.ssd_page_compact(None, P, P, P, nb, out, P, P, P, P, P, P, tab, tab_out, lens, mb, rows, draft, P, P,
+                                   4, drows)
+
+    for bad in (dict(nb=0), dict(out=None), dict(tab=None), dict(tab_out=None), dict(lens=None), dict(mb=0),
+                dict(rows=-1), dict(drows=1), dict(drows=-1)):
+        assert compact(**bad) == 1, bad
 
 
 def test_python_refusals():
