@@ -7,25 +7,47 @@
 // A page whose first row is among the new ones starts over: what it held counts for nothing.  Rows behind
 // the last new one keep their bytes.
 //
-// One CTA per (sequence, touched page, KV head, plane): the page's scale has one owner, no atomics, and the
-// result does not depend on scheduling.  The rows stay in registers between the maximum and the rounding, so
-// each input byte is read once; old rows are read only when the scale grows.  Bound: HBM bytes for prompts,
-// launch latency for single tokens.
+// One warp per (sequence, touched page, KV head, plane): the page's scale has one owner, no atomics, no barrier, and
+// the result does not depend on scheduling.  The rows stay in registers, as they came, between the maximum and the
+// rounding, all their loads in flight at once (8 KB a warp for a page of 16 rows of 256 in bf16); old rows are read
+// only when the scale grows.  Bound: HBM bytes for prompts, launch latency for single tokens.
+#include <type_traits>
+
 #include "kv8.cuh"
 
 namespace ssd {
 namespace {
 
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, float* f);
-template <>
-__device__ __forceinline__ void load8<bf16>(const bf16* p, float* f) { unpack8(ld_act_v4(p), f); }
-template <>
-__device__ __forceinline__ void load8<float>(const float* p, float* f) {
-  const uint4 a = ld_act_v4(p), b = ld_act_v4(p + 4);
-  f[0] = __uint_as_float(a.x); f[1] = __uint_as_float(a.y); f[2] = __uint_as_float(a.z); f[3] = __uint_as_float(a.w);
-  f[4] = __uint_as_float(b.x); f[5] = __uint_as_float(b.y); f[6] = __uint_as_float(b.z); f[7] = __uint_as_float(b.w);
-}
+// 8 values as they came, and as fp32.
+template <typename T> struct Raw8;
+template <> struct Raw8<bf16> {
+  uint4 a;
+  __device__ __forceinline__ void load(const bf16* p) { a = ld_act_v4(p); }
+  __device__ __forceinline__ void get(float* f) const { unpack8(a, f); }
+  __device__ __forceinline__ float largest() const {  // magnitude, NaN not counted
+    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&a);
+    const __nv_bfloat162 m = __hmax2(__hmax2(__habs2(h[0]), __habs2(h[1])), __hmax2(__habs2(h[2]), __habs2(h[3])));
+    return fmaxf(__low2float(m), __high2float(m));
+  }
+};
+template <> struct Raw8<float> {
+  uint4 a, b;
+  __device__ __forceinline__ void load(const float* p) {
+    a = ld_act_v4(p);
+    b = ld_act_v4(p + 4);
+  }
+  __device__ __forceinline__ void get(float* f) const {
+    f[0] = __uint_as_float(a.x); f[1] = __uint_as_float(a.y); f[2] = __uint_as_float(a.z); f[3] = __uint_as_float(a.w);
+    f[4] = __uint_as_float(b.x); f[5] = __uint_as_float(b.y); f[6] = __uint_as_float(b.z); f[7] = __uint_as_float(b.w);
+  }
+  __device__ __forceinline__ float largest() const {
+    float f[8], m = 0.f;
+    get(f);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(f[i]));
+    return m;
+  }
+};
 __device__ __forceinline__ void store8(bf16* p, const float* f) {
   uint4 u;
   __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&u);
@@ -47,7 +69,7 @@ struct AppendArgs {
   const void* k;        // row m, head h at k + m * row + h * D
   const void* v;
   int64_t row;          // elements between token rows
-  int T, pages_per_seq, kv_ctas;
+  int T, pages_per_seq, units, kv_ctas;
   // rotary embedding (nullptr cos: none)
   const void* q;
   void* q_out;          // [B*T, hq, D]
@@ -71,27 +93,26 @@ __device__ __forceinline__ void rotate8(float* x1, float* x2, const float* c, co
   }
 }
 
-// Values of one item: dims d .. d + 7 and D/2 + d .. D/2 + d + 7 of a row, rotated where K is.
+// An item: dims d .. d + 7 and D/2 + d .. D/2 + d + 7 of a row, so a rotation pair where K is rotated.
 template <typename T, int D>
 struct Rows {
   const AppendArgs& a;
-  int64_t m0;   // token row of position `first`
-  int first;    // first new position in the page
-  int head, plane;
-  __device__ __forceinline__ bool rotated() const { return a.cos_t != nullptr && plane == 0; }
-  // item i of the page's rows: local row r
-  __device__ __forceinline__ void get(int i, int& r, int& d0, int& d1, float* x0, float* x1) const {
-    constexpr int PER = D / 16;
-    r = i / PER;
-    const int c = i % PER;
-    const T* base = reinterpret_cast<const T*>(plane ? a.v : a.k) + (m0 + r) * a.row + (int64_t)head * D;
-    d0 = c * 8;  // two groups of 8 dims, half a row apart: a rotation pair, and whole sectors for a warp's loads
-    d1 = d0 + D / 2;
-    load8<T>(base + d0, x0);
-    load8<T>(base + d1, x1);
-    if (rotated()) {
-      const int p = min(first + r, a.rope_max_pos - 1);
-      rotate8(x0, x1, a.cos_t + (int64_t)p * (D / 2) + d0, a.sin_t + (int64_t)p * (D / 2) + d0);
+  const T* base;  // head's values in the token row of position `first`
+  int first;      // first new position in the page
+  bool rotated;
+  struct Item { Raw8<T> lo, hi; };
+  __device__ __forceinline__ void load(int i, Item& x) const {
+    const T* p = base + (i / (D / 16)) * a.row + (i % (D / 16)) * 8;
+    x.lo.load(p);
+    x.hi.load(p + D / 2);
+  }
+  __device__ __forceinline__ void get(int i, const Item& x, float* f) const {  // 16 values
+    x.lo.get(f);
+    x.hi.get(f + 8);
+    if (rotated) {
+      const int p = min(first + i / (D / 16), a.rope_max_pos - 1);
+      const int64_t at = (int64_t)p * (D / 2) + (i % (D / 16)) * 8;
+      rotate8(f, f + 8, a.cos_t + at, a.sin_t + at);
     }
   }
 };
@@ -114,8 +135,11 @@ __device__ __forceinline__ void rope_q_cta(const AppendArgs& a, int cta) {
     const int h = i / PER, d = (i % PER) * 8;
     float x0[8], x1[8];
     if (real) {
-      load8<T>(src + h * D + d, x0);
-      load8<T>(src + h * D + d + D / 2, x1);
+      Raw8<T> lo, hi;
+      lo.load(src + h * D + d);
+      hi.load(src + h * D + d + D / 2);
+      lo.get(x0);
+      hi.get(x1);
       rotate8(x0, x1, a.cos_t + (int64_t)p * (D / 2) + d, a.sin_t + (int64_t)p * (D / 2) + d);
     } else {
 #pragma unroll
@@ -126,26 +150,28 @@ __device__ __forceinline__ void rope_q_cta(const AppendArgs& a, int cta) {
   }
 }
 
-// KEEP: items (of 16 values) a thread holds in registers between the two passes; rows of a page beyond
-// KEEP * blockDim.x items are read a second time (through L2).
+// KEEP: items a lane holds between the two passes; a page's items beyond KEEP * 32 are read a second time (L2).
+constexpr int kAppendWarps = 4;
+
 template <typename T, int D, int KEEP>
-__global__ void __launch_bounds__(256) kv8_append_kernel(const AppendArgs a) {
-  __shared__ float red[32];
+__global__ void __launch_bounds__(kAppendWarps * 32, 4) kv8_append_kernel(const AppendArgs a) {
   pdl_wait();
   pdl_trigger();
   if ((int)blockIdx.x >= a.kv_ctas) {
     rope_q_cta<T, D>(a, blockIdx.x - a.kv_ctas);
     return;
   }
-  int u = blockIdx.x;
+  const int lane = threadIdx.x & 31;
+  int u = blockIdx.x * kAppendWarps + (threadIdx.x >> 5);
+  if (u >= a.units) return;
   const int plane = u & 1;
   u >>= 1;
   const int head = u % a.c.hkv;
   u /= a.c.hkv;
   const int i = u % a.pages_per_seq, b = u / a.pages_per_seq;
   const int bs = a.c.block_size;
-  const int seq = a.seq_lens[b];
-  const int ql = a.q_lens ? min(max(a.q_lens[b], 0), a.T) : a.T;
+  const int seq = ld_act(a.seq_lens + b);
+  const int ql = a.q_lens ? min(max(ld_act(a.q_lens + b), 0), a.T) : a.T;
   const int n0 = seq - ql;
   const int start = max(n0, 0);
   const int page = start / bs + i;
@@ -155,117 +181,121 @@ __global__ void __launch_bounds__(256) kv8_append_kernel(const AppendArgs a) {
   const int rows = (int)min((int64_t)seq, p0 + bs) - first;
   if (rows <= 0) return;
   const int blk = ld_act(a.tables + (int64_t)b * a.max_blocks + page);
-  if ((unsigned)blk >= (unsigned)a.c.num_blocks) return;
 
   constexpr int PER = D / 16;
-  const Rows<T, D> src{a, (int64_t)b * a.T + (first - n0), first, head, plane};
+  const Rows<T, D> src{a, reinterpret_cast<const T*>(plane ? a.v : a.k) + ((int64_t)b * a.T + (first - n0)) * a.row +
+                              (int64_t)head * D, first, a.cos_t != nullptr && plane == 0};
   const int items = rows * PER;
-  float x[KEEP][16];
-  float amax = 0.f;
+  typename Rows<T, D>::Item x[KEEP];
 #pragma unroll
-  for (int k = 0; k < KEEP; ++k) {
-    const int it = threadIdx.x + k * blockDim.x;
-    if (it < items) {
-      int r, d0, d1;
-      src.get(it, r, d0, d1, x[k], x[k] + 8);
-#pragma unroll
-      for (int j = 0; j < 16; ++j) amax = fmaxf(amax, finite_abs(x[k][j]));
-    }
-  }
-  for (int it = threadIdx.x + KEEP * blockDim.x; it < items; it += blockDim.x) {
-    int r, d0, d1;
-    float y[16];
-    src.get(it, r, d0, d1, y, y + 8);
-#pragma unroll
-    for (int j = 0; j < 16; ++j) amax = fmaxf(amax, finite_abs(y[j]));
-  }
-  amax = block_reduce(amax, red, OpMax());
-
+  for (int k = 0; k < KEEP; ++k)
+    if (lane + 32 * k < items) src.load(lane + 32 * k, x[k]);
+  if ((unsigned)blk >= (unsigned)a.c.num_blocks) return;
   float* scale = a.c.scales + plane * a.c.scale_plane + a.c.scale_layer + (int64_t)blk * a.c.hkv + head;
   uint8_t* base = a.c.pages + plane * a.c.plane + a.c.layer + ((int64_t)blk * bs * a.c.hkv + head) * D;
   const int64_t rstride = (int64_t)a.c.hkv * D;
   const int r0 = first - (int)p0;  // first new row of the page
-  int e = kv8_exponent(amax);
-  if (r0 > 0) {
-    const int eo = scale_exponent(ld_act(scale));
-    if (e > eo) {
-      // the earlier rows move to the larger scale; exp2i's range holds the difference down to 2^-126, below
-      // which every value rounds to zero anyway
-      const float f = exp2i(max(eo - e, -126));
-      for (int it = threadIdx.x; it < r0 * PER; it += blockDim.x) {
-        uint4* p = reinterpret_cast<uint4*>(base + (it / PER) * rstride + (it % PER) * 16);
-        const uint4 w = ld_act_v4(p);
-        const uint32_t in[4] = {w.x, w.y, w.z, w.w};
-        uint32_t out[4];
+  const int eo = r0 > 0 ? scale_exponent(ld_act(scale)) : kKv8MinExp;
+
+  auto each = [&](auto&& use) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float2 lo = e4m3_pair(in[j]), hi = e4m3_pair(in[j] >> 16);
-          const float v[4] = {lo.x, lo.y, hi.x, hi.y};
-          out[j] = e4m3x4(v, f);
-        }
-        *p = make_uint4(out[0], out[1], out[2], out[3]);
-      }
-    } else {
-      e = eo;
+    for (int k = 0; k < KEEP; ++k)
+      if (lane + 32 * k < items) use(lane + 32 * k, x[k]);
+    for (int it = lane + 32 * KEEP; it < items; it += 32) {
+      typename Rows<T, D>::Item y;
+      src.load(it, y);
+      use(it, y);
     }
-  }
-  // every thread of the CTA has read the old scale only if r0 > 0; the barrier keeps the new one behind those reads
-  __syncthreads();
-  if (threadIdx.x == 0) *scale = exp2i(e);
-  const float inv = exp2i(-e);
-  auto put = [&](int r, int d0, int d1, const float* y) {
-    uint8_t* p = base + (r0 + r) * rstride;
-    *reinterpret_cast<uint2*>(p + d0) = make_uint2(e4m3x4(y, inv), e4m3x4(y + 4, inv));
-    *reinterpret_cast<uint2*>(p + d1) = make_uint2(e4m3x4(y + 8, inv), e4m3x4(y + 12, inv));
   };
+  float amax = 0.f;
+  if (src.rotated) {
+    each([&](int it, const typename Rows<T, D>::Item& y) {
+      float f[16];
+      src.get(it, y, f);
 #pragma unroll
-  for (int k = 0; k < KEEP; ++k) {
-    const int it = threadIdx.x + k * blockDim.x;
-    if (it < items) {
-      const int r = it / PER, c = it % PER;
-      put(r, c * 8, c * 8 + D / 2, x[k]);
+      for (int j = 0; j < 16; ++j) amax = fmaxf(amax, fabsf(f[j]));
+    });
+  } else {
+    each([&](int, const typename Rows<T, D>::Item& y) { amax = fmaxf(amax, fmaxf(y.lo.largest(), y.hi.largest())); });
+  }
+  amax = warp_max(amax);
+  const bool inf = amax > 3.402823466e38f;
+  if (inf) {  // rare: the scale goes by the finite values
+    amax = 0.f;
+    each([&](int it, const typename Rows<T, D>::Item& y) {
+      float f[16];
+      src.get(it, y, f);
+#pragma unroll
+      for (int j = 0; j < 16; ++j) amax = fmaxf(amax, finite_abs(f[j]));
+    });
+    amax = warp_max(amax);
+  }
+  int e = kv8_exponent(amax);
+  if (r0 > 0 && e > eo) {
+    // the earlier rows move to the larger scale; exp2i's range holds the difference down to 2^-126, below
+    // which every value rounds to zero anyway
+    const float f = exp2i(max(eo - e, -126));
+    for (int it = lane; it < r0 * PER; it += 32) {
+      uint4* p = reinterpret_cast<uint4*>(base + (it / PER) * rstride + (it % PER) * 16);
+      const uint4 w = ld_act_v4(p);
+      const uint32_t in[4] = {w.x, w.y, w.z, w.w};
+      uint32_t out[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 lo = e4m3_pair(in[j]), hi = e4m3_pair(in[j] >> 16);
+        const float v[4] = {lo.x, lo.y, hi.x, hi.y};
+        out[j] = e4m3x4(v, f);
+      }
+      *p = make_uint4(out[0], out[1], out[2], out[3]);
     }
   }
-  for (int it = threadIdx.x + KEEP * blockDim.x; it < items; it += blockDim.x) {
-    int r, d0, d1;
-    float y[16];
-    src.get(it, r, d0, d1, y, y + 8);
-    put(r, d0, d1, y);
-  }
+  e = max(e, eo);
+  __syncwarp();  // every lane has read the old scale
+  if (lane == 0) *scale = exp2i(e);
+  const float inv = exp2i(-e);
+  auto put = [&](int it, const typename Rows<T, D>::Item& y, auto may_inf) {
+    constexpr bool INF = decltype(may_inf)::value;
+    float f[16];
+    src.get(it, y, f);
+    uint8_t* p = base + (r0 + it / PER) * rstride + (it % PER) * 8;
+    *reinterpret_cast<uint2*>(p) = make_uint2(e4m3x4<INF>(f, inv), e4m3x4<INF>(f + 4, inv));
+    *reinterpret_cast<uint2*>(p + D / 2) = make_uint2(e4m3x4<INF>(f + 8, inv), e4m3x4<INF>(f + 12, inv));
+  };
+  if (!inf)
+    each([&](int it, const typename Rows<T, D>::Item& y) { put(it, y, std::false_type()); });
+  else
+    each([&](int it, const typename Rows<T, D>::Item& y) { put(it, y, std::true_type()); });
 }
 
 template <typename T, int D>
-int launch_append_d(cudaStream_t st, const AppendArgs& a, int B) {
-  constexpr int KEEP = 2;
-  // two items (32 values) a thread, the block size a power of two between one warp and 256 threads
-  const int64_t items = (int64_t)a.c.block_size * (D / 16);
-  int threads = 32;
-  while (threads < 256 && (int64_t)threads * KEEP < items) threads *= 2;
+int launch_append_d(cudaStream_t st, const AppendArgs& a) {
+  constexpr int KEEP = sizeof(T) == 2 ? 8 : 4;
   const int64_t q_ctas = a.cos_t ? (int64_t)a.total_rows : 0;
   if (a.kv_ctas + q_ctas > 0x7fffffff) return SSD_ERR_UNSUPPORTED;
-  SSD_PDL((kv8_append_kernel<T, D, KEEP>), (unsigned)(a.kv_ctas + q_ctas), threads, 0, st, a);
+  SSD_PDL((kv8_append_kernel<T, D, KEEP>), (unsigned)(a.kv_ctas + q_ctas), kAppendWarps * 32, 0, st, a);
   return SSD_OK;
 }
 
 template <typename T>
-int launch_append(cudaStream_t st, const AppendArgs& a, int B, int D) {
-  if (D == 256) return launch_append_d<T, 256>(st, a, B);
-  if (D == 128) return launch_append_d<T, 128>(st, a, B);
-  return launch_append_d<T, 64>(st, a, B);
+int launch_append(cudaStream_t st, const AppendArgs& a, int D) {
+  if (D == 256) return launch_append_d<T, 256>(st, a);
+  if (D == 128) return launch_append_d<T, 128>(st, a);
+  return launch_append_d<T, 64>(st, a);
 }
 
 int append_common(ssd_stream_t stream, AppendArgs a, int dtype, int B, int T, int D) {
   const int bs = a.c.block_size;
   const int64_t pages = ((int64_t)T + bs - 2) / bs + 1;  // pages that T consecutive rows can touch
-  const int64_t ctas = (int64_t)B * pages * a.c.hkv * 2;
-  if (ctas > 0x7fffffff || (int64_t)B * T > 0x7fffffff) return SSD_ERR_UNSUPPORTED;
+  const int64_t units = (int64_t)B * pages * a.c.hkv * 2;
+  if (units > 0x7fffffff - kAppendWarps || (int64_t)B * T > 0x7fffffff) return SSD_ERR_UNSUPPORTED;
   a.T = T;
   a.total_rows = B * T;
   a.pages_per_seq = (int)pages;
-  a.kv_ctas = (int)ctas;
+  a.units = (int)units;
+  a.kv_ctas = (int)((units + kAppendWarps - 1) / kAppendWarps);
   cudaStream_t st = (cudaStream_t)stream;
-  if (dtype == SSD_DTYPE_BF16) return launch_append<bf16>(st, a, B, D);
-  return launch_append<float>(st, a, B, D);
+  if (dtype == SSD_DTYPE_BF16) return launch_append<bf16>(st, a, D);
+  return launch_append<float>(st, a, D);
 }
 
 // K and V rows of positions [B][N] (-1: zeros).  A row of one position is 2 Hkv D values; a warp takes up to

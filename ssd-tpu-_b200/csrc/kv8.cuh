@@ -35,15 +35,20 @@ __device__ __forceinline__ float finite_abs(float x) {
   return a <= 3.402823466e38f ? a : 0.f;
 }
 
-// Two fp32 values (already divided by the scale) to e4m3, nearest even; non-finite values become NaN.
+// Two fp32 values (already divided by the scale, hence within 448 unless infinite) to e4m3, nearest even.  NaN stays
+// NaN; so do infinities where INF says that there may be some (the conversion alone would make them 448).
+template <bool INF = false>
 __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
   uint32_t r = __nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
-  if (!(fabsf(lo) <= 3.402823466e38f)) r = (r & 0xff00u) | 0x7fu;
-  if (!(fabsf(hi) <= 3.402823466e38f)) r = (r & 0x00ffu) | 0x7f00u;
+  if (INF) {
+    if (!(fabsf(lo) <= 3.402823466e38f)) r = (r & 0xff00u) | 0x7fu;
+    if (!(fabsf(hi) <= 3.402823466e38f)) r = (r & 0x00ffu) | 0x7f00u;
+  }
   return r;
 }
+template <bool INF = false>
 __device__ __forceinline__ uint32_t e4m3x4(const float* f, float inv) {
-  return e4m3x2(f[0] * inv, f[1] * inv) | (e4m3x2(f[2] * inv, f[3] * inv) << 16);
+  return e4m3x2<INF>(f[0] * inv, f[1] * inv) | (e4m3x2<INF>(f[2] * inv, f[3] * inv) << 16);
 }
 // e4m3 pair (low 16 bits) -> f16 pair, exact.
 __device__ __forceinline__ uint32_t f16x2_of(uint32_t pair) {
