@@ -509,7 +509,7 @@ typedef struct {
   const int32_t* tokens;           /* [B, T] */
   const int32_t* seq_lens_before;  /* [B] tokens already cached */
   const int32_t* q_lens;           /* [B] valid new tokens, or NULL (= T) */
-  void* kv_pages;                  /* [2, L, num_blocks, block_size, Hkv, D] */
+  void* kv_pages;                  /* [2, L, num_blocks, block_size, Hkv, D] (see kv_scales) */
   int num_blocks, block_size;
   const int32_t* block_tables;     /* [B, max_blocks] */
   int max_blocks;
@@ -531,6 +531,10 @@ typedef struct {
    * run as ssd_linear_allreduce and the LM head as ssd_linear_allgather, so
    * `logits` must lie in comm's heap, at the same offset on every rank. */
   const ssd_comm* comm;
+  /* 8-bit cache (NULL: kv_pages is in the weights' dtype).  When set, kv_pages holds e4m3 and
+   * kv_scales its scales [2, L, num_blocks, Hkv]: K and V enter by ssd_kv8_rope_append and the
+   * attention is ssd_kv8_attention.  Not with qk_pairs weights. */
+  float* kv_scales;
 } ssd_gemma_batch;
 
 size_t ssd_gemma_scratch_size(const ssd_gemma_weights* w, int B, int T, int max_seq_len);

@@ -143,6 +143,8 @@ size_t linear_ws_any(int M, int N, int K, int dtype) {
   return linear_cc_workspace(M, N, K, dtype == SSD_DTYPE_BF16 ? 2 : 4);
 }
 
+constexpr size_t kKv8WsOffset = kCounterBytes + 256;  // counters and error word of the paged attention
+
 Scratch carve(const ssd_gemma_weights* w, int B, int T, int max_seq_len, char* base) {
   Scratch s{};
   const size_t es = w->dtype == SSD_DTYPE_BF16 ? 2 : 4;
@@ -170,7 +172,9 @@ Scratch carve(const ssd_gemma_weights* w, int B, int T, int max_seq_len, char* b
   upd(B, w->vocab, d);
   s.lin_ws_bytes = lw;
   s.lin_ws = take(lw);
-  s.attn_ws_bytes = ssd_paged_attention_workspace_size(B, T, hq, hkv, D, max_seq_len);
+  // one workspace for either cache; the 8-bit one's part lies behind the ticket counters, which it must not touch
+  const size_t kv8 = ssd_kv8_attention_workspace_size(B, T, hq, hkv, D, max_seq_len);
+  s.attn_ws_bytes = std::max(ssd_paged_attention_workspace_size(B, T, hq, hkv, D, max_seq_len), kKv8WsOffset + kv8);
   s.attn_ws = take(s.attn_ws_bytes);
   s.total = off;
   return s;
@@ -208,7 +212,7 @@ extern "C" const char* ssd_status_string(int status) {
   }
 }
 
-extern "C" int ssd_abi_version(void) { return (1 << 16) | 1; }
+extern "C" int ssd_abi_version(void) { return (1 << 16) | 2; }
 
 extern "C" int ssd_linear_max_m(void) { return max_m(); }
 
@@ -310,6 +314,7 @@ extern "C" int ssd_gemma_forward(ssd_stream_t stream, const ssd_gemma_weights* w
   if ((int64_t)bt->max_blocks * bt->block_size < bt->max_seq_len) return SSD_ERR_INVALID;
   if (bt->max_seq_len > w->rope_max_pos) return SSD_ERR_INVALID;
   if (w->tp_world > 1 && !bt->comm) return SSD_ERR_INVALID;
+  if (bt->kv_scales && w->qk_pairs) return SSD_ERR_INVALID;
   if (bt->comm) {
     const ssd_comm* c = bt->comm;
     if (c->world != std::max(w->tp_world, 1) || c->rank != w->tp_rank || w->dtype != SSD_DTYPE_BF16 ||
@@ -404,10 +409,21 @@ extern "C" int ssd_gemma_forward(ssd_stream_t stream, const ssd_gemma_weights* w
       }));
     } else {
       SSD_TRY(proj(0, s.x, w->w_qkv[l], s.qkv, SSD_EPI_STORE, M, (hq + 2 * hkv) * D, d, 1));
-      SSD_TRY(ssd_rope_kv_write(stream, s.qkv, s.q, bt->kv_pages, dt, L, bt->num_blocks, bt->block_size, hq, hkv, D,
+      if (bt->kv_scales)
+        SSD_TRY(ssd_kv8_rope_append(stream, s.qkv, s.q, bt->kv_pages, bt->kv_scales, dt, L, bt->num_blocks,
+                                    bt->block_size, hq, hkv, D, l, bt->block_tables, bt->max_blocks, s.seq_after,
+                                    s.qlen, w->rope_cos, w->rope_sin, w->rope_max_pos, B, T));
+      else
+        SSD_TRY(ssd_rope_kv_write(stream, s.qkv, s.q, bt->kv_pages, dt, L, bt->num_blocks, bt->block_size, hq, hkv, D,
                                 l, bt->block_tables, bt->max_blocks, s.pos, w->rope_cos, w->rope_sin,
                                 w->rope_max_pos, B, T));
     }
+    if (bt->kv_scales)
+      SSD_TRY(ssd_kv8_attention(stream, s.q, bt->kv_pages, bt->kv_scales, dt, L, bt->num_blocks, bt->block_size, hkv, D,
+                                l, bt->block_tables, bt->max_blocks, s.seq_after, s.qlen, s.attn, scale, B, T, hq,
+                                bt->max_seq_len, reinterpret_cast<char*>(s.attn_ws) + kKv8WsOffset,
+                                s.attn_ws_bytes - kKv8WsOffset));
+    else
     // early = 1: the kernel before it (RoPE + K/V write, or the QKV projection that
     // does them) writes only q and the new rows
     SSD_TRY(paged_verify_attention_impl(stream, s.q, bt->kv_pages, dt, L, bt->num_blocks, bt->block_size, hkv, D, l,

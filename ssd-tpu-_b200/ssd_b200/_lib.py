@@ -118,6 +118,7 @@ class GemmaBatchC(C.Structure):
         ("prof_events", C.POINTER(_p)), ("prof_capacity", _i), ("prof_count", C.POINTER(_i)),
         ("prof_kind", C.POINTER(_i)),
         ("comm", C.POINTER(CommC)),
+        ("kv_scales", _p),
     ]
 
 

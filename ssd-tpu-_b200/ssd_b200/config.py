@@ -43,6 +43,8 @@ class SSDConfig:
     # target tensor parallelism over GPUs 0..tensor_parallel_size-1 (one process, one thread per GPU);
     # in sd and ar modes the draft is sharded over the same GPUs, in ssd mode it runs on draft_device
     tensor_parallel_size: int = field(default_factory=lambda: int(os.getenv("SSD_TP_SIZE", "1")))
+    # "auto": caches in the weights' dtype; "fp8": 8-bit caches with a scale per page and KV head
+    kv_cache_dtype: str = field(default_factory=lambda: os.getenv("SSD_KV_CACHE_DTYPE", "auto"))
     tpu_role: str = field(default_factory=lambda: os.getenv("SSD_TPU_ROLE", "both").lower())
     mesh_allocation: object | None = None
     instance_context_ratio: float = 0.3

@@ -35,6 +35,8 @@ import torch
 
 from .. import _lib
 from .._lib import GemmaBatchC, GemmaWeightsC, check, dtype_code, lib, ptr, stream_ptr
+from ..kernels.kv8_cache import KV8CacheState
+from ..kernels.kv_cache import KVCacheState
 
 
 @dataclass(frozen=True)
@@ -260,8 +262,29 @@ class GemmaWeights:
         return self.shape.num_params() * es
 
 
+KV_CACHE_DTYPES = ("auto", "fp8")
+
+
+def allocate_kv_cache(weights: GemmaWeights, num_blocks: int, block_size: int, kv_cache_dtype: str = "auto"):
+    """A paged cache for the model: ``"auto"`` in the weights' dtype (``KVCacheState``), ``"fp8"`` in 8 bits
+    (``KV8CacheState``: half the bytes of bf16)."""
+    s = weights.shape
+    if kv_cache_dtype == "fp8":
+        if weights.qk_pairs:
+            raise ValueError("an fp8 cache needs the canonical q/k row order (no pair_qk_rows)")
+        return KV8CacheState.allocate(s.num_layers, num_blocks, block_size, s.num_kv_heads, s.head_dim,
+                                      device=weights.device)
+    if kv_cache_dtype != "auto":
+        raise ValueError(f"kv_cache_dtype must be one of {KV_CACHE_DTYPES}, got {kv_cache_dtype!r}")
+    return KVCacheState.allocate(s.num_layers, num_blocks, block_size, s.num_kv_heads, s.head_dim,
+                                 dtype=weights.dtype, device=weights.device)
+
+
 class GemmaRunner:
     """One ``ssd_gemma_forward`` per call; scratch sized for (max_batch, max_tokens).
+
+    ``forward`` takes the cache as its pages tensor or as the cache object; a ``KV8CacheState`` has to
+    come as the object (its scales go with it).
 
     With ``comm`` (a ``runtime.tensor_parallel.TPComm``) the weights are one
     rank's shard and the logits buffers passed to ``forward`` must come from
@@ -288,15 +311,20 @@ class GemmaRunner:
             self._scratch[key] = buf
         return buf
 
-    def forward(self, tokens: torch.Tensor, seq_lens_before: torch.Tensor, pages: torch.Tensor,
+    def forward(self, tokens: torch.Tensor, seq_lens_before: torch.Tensor, pages,
                 block_tables: torch.Tensor, logits: torch.Tensor | None, q_lens: torch.Tensor | None = None,
                 last_only: bool = False, stream=None, prof: "ProjectionTimer | None" = None) -> torch.Tensor:
         b, t = tokens.shape
         sc = self.scratch(b, t)
+        scales = None
+        if not isinstance(pages, torch.Tensor):
+            scales, pages = getattr(pages, "scales", None), pages.pages
+        if scales is None and pages.dtype == torch.float8_e4m3fn:
+            raise ValueError("an fp8 cache is passed as the KV8CacheState: its pages mean nothing without the scales")
         bt = GemmaBatchC()
         bt.B, bt.T = b, t
         bt.tokens, bt.seq_lens_before, bt.q_lens = ptr(tokens), ptr(seq_lens_before), ptr(q_lens)
-        bt.kv_pages = ptr(pages)
+        bt.kv_pages, bt.kv_scales = ptr(pages), ptr(scales)
         bt.num_blocks, bt.block_size = pages.shape[2], pages.shape[3]
         bt.block_tables, bt.max_blocks = ptr(block_tables), block_tables.shape[1]
         bt.max_seq_len = self.max_seq_len

@@ -26,18 +26,19 @@ from typing import Callable
 import torch
 
 from ..algorithm.verify import argmax_rows
+from ..kernels.kv8_cache import KV8CacheState
 from ..kernels.kv_cache import KVCacheState
 from ..kernels.ops import max_tokens_per_forward
 from ..runtime.page_manager import PageManager
 from .base import DecodeResult, PrefillResult, VerifyResultModel
-from .gemma import GemmaRunner, GemmaWeights
+from .gemma import GemmaRunner, GemmaWeights, allocate_kv_cache
 
 
 class GemmaAdapter:
     def __init__(self, model_path: GemmaWeights | str | None = None, vocab_size: int | None = None,
                  share_key: str | None = None, mesh=None, devices=None, role: str = "target", *,
                  max_model_len: int = 4096, block_size: int = 16, max_tokens: int = 64, name: str | None = None,
-                 max_branches: int = 0, comm=None) -> None:
+                 max_branches: int = 0, comm=None, kv_cache_dtype: str = "auto") -> None:
         """Positional arguments in the reference's order (gemma_adapter.py:28-36).
 
         ``model_path``: a ``GemmaWeights`` already on the device, or a model path.  A path names a
@@ -49,7 +50,9 @@ class GemmaAdapter:
 
         ``comm`` (a ``runtime.tensor_parallel.TPComm``): the weights are one rank's shard and
         every rank of the group makes the same calls; logits land in the group's symmetric heap
-        (the LM head all-gathers into it) and are returned as copies."""
+        (the LM head all-gathers into it) and are returned as copies.
+
+        ``kv_cache_dtype``: ``"fp8"`` holds the cache in 8 bits (``models.gemma.allocate_kv_cache``)."""
         if isinstance(model_path, GemmaWeights):
             weights = model_path
         else:
@@ -74,8 +77,7 @@ class GemmaAdapter:
         self.comm = comm
         self.runner = GemmaRunner(weights, 1 + self.max_branches, max(self.chunk, max_tokens), max_model_len,
                                   comm=comm)
-        self.cache = KVCacheState.allocate(s.num_layers, self.num_blocks, block_size, s.num_kv_heads, s.head_dim,
-                                           dtype=weights.dtype, device=self.dev)
+        self.cache = allocate_kv_cache(weights, self.num_blocks, block_size, kv_cache_dtype)
         self.pm = PageManager(block_size, self.num_blocks, max_seqs=1 + self.max_branches,
                               max_blocks_per_seq=per_seq, device=self.dev)
         self.cached: list[int] = []   # tokens whose K/V rows are valid in the cache
@@ -118,7 +120,7 @@ class GemmaAdapter:
             last = c0 + self.chunk >= len(tokens)
             t = torch.tensor([part], dtype=torch.int32, device=self.dev)
             lg = logits if last else None
-            self.runner.forward(t, self._i32(n0 + c0), self.cache.pages, self.pm.tables, lg, last_only=last_only)
+            self.runner.forward(t, self._i32(n0 + c0), self.cache, self.pm.tables, lg, last_only=last_only)
             out = lg
         self.cached.extend(int(x) for x in tokens)
         return out
@@ -127,7 +129,7 @@ class GemmaAdapter:
         """Forget the cached tokens and release their pages (gemma_adapter.py:74-75)."""
         self._truncate(0)
 
-    def allocate_kv(self) -> KVCacheState:
+    def allocate_kv(self) -> KVCacheState | KV8CacheState:
         self.reset_cache()
         return self.cache
 
@@ -154,7 +156,7 @@ class GemmaAdapter:
         n0 = len(self.cached)
         self.pm.allocate_rows(0, 1, self._i32(n0), self._i32(len(toks)), None)
         self.runner.forward(torch.tensor([toks], dtype=torch.int32, device=self.dev), self._i32(n0),
-                            self.cache.pages, self.pm.tables, lg, last_only=False)
+                            self.cache, self.pm.tables, lg, last_only=False)
         self.pending = toks
         return VerifyResultModel(logits=lg if self.comm is None else lg.clone(), kv_cache=self.cache)
 
@@ -230,13 +232,13 @@ class GemmaAdapter:
         toks = self._d_tok
         lg = self._lg1
         pos0 = 4 + rows - 1
-        self.runner.forward(d[pos0:pos0 + f].view(1, f), d[2:3], self.cache.pages, self.pm.tables, lg,
+        self.runner.forward(d[pos0:pos0 + f].view(1, f), d[2:3], self.cache, self.pm.tables, lg,
                             last_only=True)
         logits[0].copy_(lg[0])
         if k > 0:
             argmax_rows(lg, toks[0:1])
         for i in range(1, rows):
-            self.runner.forward(toks[i - 1:i].view(1, 1), d[4 + i - 1:4 + i], self.cache.pages, self.pm.tables, lg,
+            self.runner.forward(toks[i - 1:i].view(1, 1), d[4 + i - 1:4 + i], self.cache, self.pm.tables, lg,
                                 last_only=True)
             logits[i].copy_(lg[0])
             if i < k:
@@ -301,14 +303,14 @@ class GemmaAdapter:
             lg = self._logits(n)
             nxt = torch.empty((k, n), dtype=torch.int32, device=self.dev)
             tables = self.pm.tables[1:1 + n]
-            self.runner.forward(toks, base, self.cache.pages, tables, lg, q_lens=qlen, last_only=True)
+            self.runner.forward(toks, base, self.cache, tables, lg, q_lens=qlen, last_only=True)
             argmax_rows(lg, nxt[0])
             stopped = False
             for i in range(1, k):
                 if stop is not None and self._wait_or_stop(stop):
                     stopped = True
                     break
-                self.runner.forward(nxt[i - 1].view(n, 1), base + qlen + (i - 1), self.cache.pages, tables, lg,
+                self.runner.forward(nxt[i - 1].view(n, 1), base + qlen + (i - 1), self.cache, tables, lg,
                                     last_only=True)
                 argmax_rows(lg, nxt[i])
             self.pm.free_rows(1, n)

@@ -33,22 +33,20 @@ import torch
 
 from .._lib import check, lib, ptr, stream_ptr
 from ..algorithm.verify import argmax_rows, sample_rows, top_p_mask_, verify_sample
-from ..kernels.kv_cache import KVCacheState
+from ..kernels.kv8_cache import KV8CacheState
 from ..kernels.ops import max_tokens_per_forward
-from ..models.gemma import GemmaRunner, GemmaWeights
+from ..models.gemma import GemmaRunner, GemmaWeights, allocate_kv_cache
 from ..workspace import workspace
 from .page_manager import PageManager
 
 
 class _BatchModel:
     def __init__(self, weights: GemmaWeights, batch: int, max_seq_len: int, block_size: int, tokens: int,
-                 comm=None, num_blocks: int | None = None):
-        s = weights.shape
+                 comm=None, num_blocks: int | None = None, kv_cache_dtype: str = "auto"):
         self.w = weights
         self.max_blocks = (max_seq_len + block_size - 1) // block_size + 1
         self.num_blocks = num_blocks or batch * self.max_blocks + 2
-        self.cache = KVCacheState.allocate(s.num_layers, self.num_blocks, block_size, s.num_kv_heads, s.head_dim,
-                                           dtype=weights.dtype, device=weights.device)
+        self.cache = allocate_kv_cache(weights, self.num_blocks, block_size, kv_cache_dtype)
         self.pm = PageManager(block_size, self.num_blocks, max_seqs=batch, max_blocks_per_seq=self.max_blocks,
                               device=weights.device)
         self.runner = GemmaRunner(weights, batch, tokens, max_seq_len, comm=comm)
@@ -59,7 +57,7 @@ class _BatchModel:
 class BatchedSpeculativeDecoder:
     def __init__(self, target: GemmaWeights, draft: GemmaWeights, batch: int, k: int = 4, max_seq_len: int = 1024,
                  block_size: int = 16, temperature: float = 0.0, sampler_x: float = 0.5, seed: int = 0, comm=None,
-                 num_blocks: int | None = None, top_p: float = 1.0):
+                 num_blocks: int | None = None, top_p: float = 1.0, kv_cache_dtype: str = "auto"):
         B = self.B = int(batch)
         self.k = k
         self.temperature = float(temperature)
@@ -74,8 +72,8 @@ class BatchedSpeculativeDecoder:
             raise ValueError("target and draft must share the vocabulary")
         if B * (k + 1) > max_tokens_per_forward(target.dtype):
             raise ValueError(f"B*(k+1) = {B * (k + 1)} exceeds one forward ({max_tokens_per_forward(target.dtype)})")
-        self.t = _BatchModel(target, B, max_seq_len, block_size, max(k + 1, 64), comm, num_blocks)
-        self.d = _BatchModel(draft, B, max_seq_len, block_size, 64, comm, num_blocks)
+        self.t = _BatchModel(target, B, max_seq_len, block_size, max(k + 1, 64), comm, num_blocks, kv_cache_dtype)
+        self.d = _BatchModel(draft, B, max_seq_len, block_size, 64, comm, num_blocks, kv_cache_dtype)
         dev = self.dev
         buf = comm.alloc if comm is not None else (lambda shape, dtype: torch.empty(shape, dtype=dtype, device=dev))
         self.vt = torch.zeros((B, k + 1), dtype=torch.int32, device=dev)      # [recovery, drafts...]
@@ -118,7 +116,7 @@ class BatchedSpeculativeDecoder:
         for c0 in range(0, n, m.chunk):
             c1 = min(n, c0 + m.chunk)
             lg = self.logits_d[b:b + 1] if (c1 == n and want_logits) else None
-            m.runner.forward(p[:, c0:c1].contiguous(), self._i32([c0]), m.cache.pages, m.pm.tables[b:b + 1], lg,
+            m.runner.forward(p[:, c0:c1].contiguous(), self._i32([c0]), m.cache, m.pm.tables[b:b + 1], lg,
                              last_only=True)
         m.n[b] = n
 
@@ -164,6 +162,13 @@ class BatchedSpeculativeDecoder:
             m.pm.allocate_rows(0, self.B, self._i32(np.zeros(self.B)), self._i32(contexts), None)
             m.n[:] = np.asarray(contexts, np.int64)
             c = m.cache.pages
+            if isinstance(m.cache, KV8CacheState):  # the same under scales of 1
+                g = torch.Generator(device=self.dev)
+                g.manual_seed(int(rng.integers(1, 2**62)))
+                m.cache.scales.fill_(1.0)
+                for layer in c.flatten(0, 1):
+                    layer.copy_(torch.randn(layer.shape, generator=g, device=self.dev))
+                continue
             check(lib().ssd_normal_fill(stream_ptr(), ptr(c), 0 if c.dtype == torch.bfloat16 else 1, c.numel(),
                                         1.0, int(rng.integers(1, 2**62))), "ssd_normal_fill")
         for b, n in enumerate(contexts):
@@ -211,10 +216,10 @@ class BatchedSpeculativeDecoder:
         d.pm.allocate_rows(0, B, ds[5], ds[6], None)
         for i in range(k):
             if i == 0:
-                d.runner.forward(self.feed[:, :two].contiguous() if two == 1 else self.feed, ds[5], d.cache.pages,
+                d.runner.forward(self.feed[:, :two].contiguous() if two == 1 else self.feed, ds[5], d.cache,
                                  d.pm.tables, self.logits_d, q_lens=ds[7], last_only=True)
             else:
-                d.runner.forward(self.dtok[i - 1].view(B, 1), ds[11 + i], d.cache.pages, d.pm.tables, self.logits_d,
+                d.runner.forward(self.dtok[i - 1].view(B, 1), ds[11 + i], d.cache, d.pm.tables, self.logits_d,
                                  last_only=True)
             if self.sampling:
                 if self.top_p < 1.0:
@@ -229,7 +234,7 @@ class BatchedSpeculativeDecoder:
         st = torch.cuda.current_stream()
         self.ev[0].record(st)
         t.pm.allocate_rows(0, B, ds[10], ds[11], None)
-        t.runner.forward(self.vt, ds[10], t.cache.pages, t.pm.tables, self.logits_t, last_only=False)
+        t.runner.forward(self.vt, ds[10], t.cache, t.pm.tables, self.logits_t, last_only=False)
         if self.sampling and self.top_p < 1.0:
             top_p_mask_(self.logits_t.view(B * (k + 1), self.V), self.temperature, self.top_p)
         if self.sampling:

@@ -41,7 +41,7 @@ from .._lib import SSD_MAX_TP
 from ..algorithm.async_protocol import DraftCommand, DraftRequest
 from ..config import DecodeMode, SSDConfig
 from ..kernels.ops import max_tokens_per_forward
-from ..models.gemma import PRESETS
+from ..models.gemma import KV_CACHE_DTYPES, PRESETS
 from ..models.gemma_adapter import GemmaAdapter
 from ..models.model_loader import default_preset, load_weights
 from ..sampling_params import SamplingParams
@@ -63,6 +63,8 @@ class LLMEngine:
         ngpu = torch.cuda.device_count()
         if not 1 <= T <= min(ngpu, SSD_MAX_TP):
             raise ValueError(f"tensor_parallel_size {T} needs 1..{min(ngpu, SSD_MAX_TP)} GPUs (this host has {ngpu})")
+        if config.kv_cache_dtype not in KV_CACHE_DTYPES:
+            raise ValueError(f"kv_cache_dtype must be one of {KV_CACHE_DTYPES}, got {config.kv_cache_dtype!r}")
         self.tp = T
         mode = config.mode
         self.async_draft = mode in (DecodeMode.SSD, DecodeMode.INSTANCE)
@@ -79,6 +81,7 @@ class LLMEngine:
         self.target_preset = tpath if tpath in PRESETS else default_preset("target", use_toy)
         cfg = {"target_model_path": tpath, "draft_model_path": dpath, "use_toy_model": use_toy,
                "seed": config.seed, "draft_seed": self._draft_seed, "max_model_len": config.max_model_len,
+               "kv_cache_dtype": config.kv_cache_dtype,
                "local_draft": mode != DecodeMode.AR and not self.async_draft, "target_adapter": self.async_draft}
         self.ranks = LocalRank(cfg, 0) if T == 1 else RankGroup(list(range(T)), cfg)
         self.vocab_size = PRESETS[self.target_preset].vocab
@@ -89,7 +92,8 @@ class LLMEngine:
             dw = load_weights(dpath, use_toy=use_toy, seed=self._draft_seed, role="draft", device=self.draft_device)
             with torch.cuda.device(self.draft_device):
                 self.draft = GemmaAdapter(dw, max_model_len=config.max_model_len, name="draft",
-                                          max_branches=max(1, config.mq_len))
+                                          max_branches=max(1, config.mq_len),
+                                          kv_cache_dtype=config.kv_cache_dtype)
                 self.draft_worker = DraftWorker(config, self.draft)
                 self.draft_worker.start()
 

@@ -22,6 +22,8 @@ from __future__ import annotations
 import torch
 
 from .._lib import check, lib, ptr, stream_ptr
+from ..kernels.kv8_cache import KV8CacheState
+from ..kernels.page_moves import compact_pages, copy_pages
 from .sequence import Sequence
 
 
@@ -143,11 +145,12 @@ class PageManager:
 
     def fork_rows(self, src_row: int, dst_row0: int, n: int, num_tokens: int, cache=None) -> torch.Tensor:
         """Rows dst_row0.. (empty) take src_row's first num_tokens tokens: full blocks shared,
-        the partial block copied (K/V rows too when ``cache`` -- a ``KVCacheState`` -- is given).
-        Returns ok [n] uint8 (device)."""
+        the partial block copied (K/V rows too when ``cache`` -- a ``KVCacheState`` or a
+        ``KV8CacheState`` -- is given).  Returns ok [n] uint8 (device)."""
         ok = torch.zeros(max(n, 1), dtype=torch.uint8, device=self.device)
         kv, dt, nl, hkv, hd = None, 0, 0, 0, 0
-        if cache is not None:
+        kv8 = isinstance(cache, KV8CacheState)
+        if cache is not None and not kv8:
             p = cache.pages
             kv = ptr(p)
             dt = 0 if p.dtype == torch.bfloat16 else 1
@@ -156,7 +159,20 @@ class PageManager:
                                   ptr(self.free_list), ptr(self.free_top), ptr(self.ref_counts_dev), self.num_blocks,
                                   src_row, dst_row0, n, int(num_tokens), self.block_size, ptr(ok), kv, dt, nl, hkv,
                                   hd), "ssd_page_fork")
+        full = int(num_tokens) // self.block_size
+        if kv8 and n > 0 and int(num_tokens) % self.block_size and full < self.max_blocks:
+            # the partial page and its scales; a row that got no block has -1 there
+            copy_pages(cache, self.tables[src_row, full:full + 1].expand(n), self.tables[dst_row0:dst_row0 + n, full])
         return ok[:n]
+
+    def compact(self, cache) -> torch.Tensor:
+        """Move the blocks in use to the front of the pool (``page_moves.compact_pages``): tables, counts
+        and free list follow in place, so captured graphs that read them stay valid.  ``cache``: the
+        cache, or every cache that uses this manager's blocks.  Returns the blocks' new ids
+        [num_blocks] (-1: free) for references held elsewhere; ``Sequence.block_table`` lists follow
+        with the sequence's next host call.  Nothing synchronises."""
+        return compact_pages(cache, self.tables, self.lens, self.ref_counts_dev, self.free_list, self.free_top,
+                             self.draft_tables, self.draft_lens, inplace=True).remap
 
     def free_rows(self, row0: int, n: int) -> None:
         """Release rows row0 .. row0+n-1 (their blocks' ref counts drop; freed blocks return)."""

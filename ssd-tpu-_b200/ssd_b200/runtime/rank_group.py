@@ -38,6 +38,7 @@ class RankState:
 
         self.cfg = cfg
         self.rank, self.world = rank, world
+        self.kv_cache_dtype = cfg.get("kv_cache_dtype", "auto")
         self.dev = torch.device("cuda", device_index)
         torch.cuda.set_device(self.dev)
         use_toy = cfg["use_toy_model"]
@@ -88,15 +89,15 @@ class RankState:
     def ar_generate(self, prompt: list[int], max_new: int, max_len: int, block_size: int) -> list[int]:
         from .speculative import GreedyDecoder
 
-        return GreedyDecoder(self.target_w, max_seq_len=max_len, block_size=block_size,
-                             comm=self.comm).generate(prompt, max_new)
+        return GreedyDecoder(self.target_w, max_seq_len=max_len, block_size=block_size, comm=self.comm,
+                             kv_cache_dtype=self.kv_cache_dtype).generate(prompt, max_new)
 
     # ------------------------------------------------------------ sd, one sequence (graph-replayed step)
     def sd_start(self, prompt: list[int], k: int, max_len: int, block_size: int) -> int:
         from .speculative import SpeculativeDecoder
 
         self.dec = SpeculativeDecoder(self.target_w, self.draft_w, k=k, max_seq_len=max_len, block_size=block_size,
-                                      comm=self.comm)
+                                      comm=self.comm, kv_cache_dtype=self.kv_cache_dtype)
         return self.dec.start(prompt)
 
     def sd_step(self) -> tuple[list[int], float, int]:
@@ -110,7 +111,8 @@ class RankState:
 
         self.dec = BatchedSpeculativeDecoder(self.target_w, self.draft_w, batch=batch, k=k, max_seq_len=max_len,
                                              block_size=block_size, temperature=temperature, top_p=top_p,
-                                             sampler_x=sampler_x, seed=seed, comm=self.comm)
+                                             sampler_x=sampler_x, seed=seed, comm=self.comm,
+                                             kv_cache_dtype=self.kv_cache_dtype)
 
     def batch_admit(self, placed: list[tuple[int, list[int]]]) -> list[int]:
         return [self.dec.admit(slot, prompt) for slot, prompt in placed]
@@ -128,7 +130,7 @@ class RankState:
             from ..models.gemma_adapter import GemmaAdapter
 
             self.target = GemmaAdapter(self.target_w, max_model_len=self.cfg["max_model_len"], name="target",
-                                       comm=self.comm)
+                                       comm=self.comm, kv_cache_dtype=self.kv_cache_dtype)
         return self.target
 
     def target_prefill(self, prompt: list[int]) -> int:

@@ -31,20 +31,18 @@ import torch
 
 from ..algorithm.verify import argmax_rows
 from .._lib import check, lib, ptr, stream_ptr
-from ..kernels.kv_cache import KVCacheState
 from ..kernels.ops import max_tokens_per_forward
-from ..models.gemma import GemmaRunner, GemmaWeights
+from ..models.gemma import GemmaRunner, GemmaWeights, allocate_kv_cache
 from ..workspace import workspace
 from .page_manager import PageManager
 
 
 class _Model:
-    def __init__(self, weights: GemmaWeights, max_seq_len: int, block_size: int, k: int, comm=None):
-        s = weights.shape
+    def __init__(self, weights: GemmaWeights, max_seq_len: int, block_size: int, k: int, comm=None,
+                 kv_cache_dtype: str = "auto"):
         self.w = weights
         self.num_blocks = (max_seq_len + block_size - 1) // block_size + 2
-        self.cache = KVCacheState.allocate(s.num_layers, self.num_blocks, block_size, s.num_kv_heads, s.head_dim,
-                                           dtype=weights.dtype, device=weights.device)
+        self.cache = allocate_kv_cache(weights, self.num_blocks, block_size, kv_cache_dtype)
         self.pm = PageManager(block_size, self.num_blocks, max_seqs=1, device=weights.device)
         self.runner = GemmaRunner(weights, 1, max(k + 1, max_tokens_per_forward(weights.dtype)), max_seq_len,
                                   comm=comm)
@@ -54,15 +52,16 @@ class _Model:
 
 class SpeculativeDecoder:
     def __init__(self, target: GemmaWeights, draft: GemmaWeights, k: int = 4, max_seq_len: int = 1024,
-                 block_size: int = 16, use_graphs: bool = True, timer=None, comm=None):
+                 block_size: int = 16, use_graphs: bool = True, timer=None, comm=None, kv_cache_dtype: str = "auto"):
         """``comm``: tensor-parallel group (``runtime.tensor_parallel.TPComm``); the
-        weights are then this rank's shards and every rank runs the same steps."""
+        weights are then this rank's shards and every rank runs the same steps.
+        ``kv_cache_dtype``: see ``models.gemma.allocate_kv_cache``."""
         self.k = k
         self.dev = target.device
         self.max_seq_len = max_seq_len
         self.comm = comm
-        self.t = _Model(target, max_seq_len, block_size, k, comm)
-        self.d = _Model(draft, max_seq_len, block_size, k, comm)
+        self.t = _Model(target, max_seq_len, block_size, k, comm, kv_cache_dtype)
+        self.d = _Model(draft, max_seq_len, block_size, k, comm, kv_cache_dtype)
         V = target.shape.vocab
         if draft.shape.vocab != V:
             raise ValueError("target and draft must share the vocabulary")
@@ -114,7 +113,7 @@ class SpeculativeDecoder:
             c1 = min(n, c0 + chunk)
             lg = self.logits_d if (c1 == n and want_logits) else None
             slb = torch.tensor([c0], dtype=torch.int32, device=dev)
-            m.runner.forward(prompt[:, c0:c1].contiguous(), slb, m.cache.pages, m.pm.tables, lg, last_only=True)
+            m.runner.forward(prompt[:, c0:c1].contiguous(), slb, m.cache, m.pm.tables, lg, last_only=True)
             out = lg
         m.n = n
         return out
@@ -167,17 +166,17 @@ class SpeculativeDecoder:
         self.vt[0, 0:1].copy_(self.d_scal[10:11])
         # draft: k greedy forwards, tokens written into vt[0, 1..k]
         d.pm.allocate_rows(0, 1, self._scal(0), self._scal(1), None)
-        d.runner.forward(self.d_scal[2:2 + nf].view(1, nf), self._scal(16), d.cache.pages, d.pm.tables,
+        d.runner.forward(self.d_scal[2:2 + nf].view(1, nf), self._scal(16), d.cache, d.pm.tables,
                          self.logits_d, last_only=True)
         argmax_rows(self.logits_d, self.vt[0, 1:2])
         for i in range(1, k):
-            d.runner.forward(self.vt[:, i:i + 1], self._scal(16 + i), d.cache.pages, d.pm.tables, self.logits_d,
+            d.runner.forward(self.vt[:, i:i + 1], self._scal(16 + i), d.cache, d.pm.tables, self.logits_d,
                              last_only=True)
             argmax_rows(self.logits_d, self.vt[0, i + 1:i + 2])
         # verify: target forward over k+1 tokens + fused greedy acceptance
         self.ev_verify[0].record(st)
         t.pm.allocate_rows(0, 1, self._scal(4), self._scal(5), None)
-        t.runner.forward(self.vt, self._scal(4), t.cache.pages, t.pm.tables, self.logits_t, last_only=False,
+        t.runner.forward(self.vt, self._scal(4), t.cache, t.pm.tables, self.logits_t, last_only=False,
                          prof=prof)
         check(lib().ssd_verify_greedy(stream_ptr(), ptr(self.logits_t), ptr(self.vt), ptr(self.acc_rec[0:1]),
                                       ptr(self.acc_rec[1:2]), ptr(self.mask), None, ptr(self.ws_greedy),
@@ -243,8 +242,9 @@ class SpeculativeDecoder:
 class GreedyDecoder:
     """Target-only greedy decode (the AR loop of engine.py:162-211) on the same kernels."""
 
-    def __init__(self, target: GemmaWeights, max_seq_len: int = 1024, block_size: int = 16, comm=None):
-        self.t = _Model(target, max_seq_len, block_size, 1, comm)
+    def __init__(self, target: GemmaWeights, max_seq_len: int = 1024, block_size: int = 16, comm=None,
+                 kv_cache_dtype: str = "auto"):
+        self.t = _Model(target, max_seq_len, block_size, 1, comm, kv_cache_dtype)
         self.dev = target.device
         V = target.shape.vocab
         self.lg = comm.alloc((1, V), torch.float32) if comm is not None else torch.empty(
@@ -260,7 +260,7 @@ class GreedyDecoder:
         for c0 in range(0, n, chunk):
             c1 = min(n, c0 + chunk)
             slb = torch.tensor([c0], dtype=torch.int32, device=dev)
-            t.runner.forward(p[:, c0:c1].contiguous(), slb, t.cache.pages, t.pm.tables, lg if c1 == n else None,
+            t.runner.forward(p[:, c0:c1].contiguous(), slb, t.cache, t.pm.tables, lg if c1 == n else None,
                              last_only=True)
         t.n = n
         tok = torch.empty((1, 1), dtype=torch.int32, device=dev)
@@ -273,7 +273,7 @@ class GreedyDecoder:
         while len(out) < max_new:
             nn = torch.tensor([t.n], dtype=torch.int32, device=dev)
             t.pm.allocate_rows(0, 1, nn, one, None)
-            t.runner.forward(tok, nn, t.cache.pages, t.pm.tables, lg, last_only=True)
+            t.runner.forward(tok, nn, t.cache, t.pm.tables, lg, last_only=True)
             argmax_rows(lg, tok[0])
             host.copy_(tok[0], non_blocking=True)
             torch.cuda.current_stream().synchronize()
