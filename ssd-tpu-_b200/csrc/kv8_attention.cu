@@ -1528,15 +1528,19 @@ Kv8Layout kv8_layout(bool cc, int B, int T, int hq, int hkv, int D, int max_seq_
   L.cc = cc;
   L.rows = cc ? kCcRows : total > kManyRows && T > kFewTokens ? many::ROWS : total > 8 ? 16 : 8;
   // Few rows: 256 positions keep a short context's CTAs many (one sequence of 8192 positions, one KV head: 11.9 us
-  // against 18.7 us at 1024); where there is work for every SM either way, 1024 positions cost fewer prologues and
-  // partials (8 sequences, 16 heads, up to 4096 positions: 38.1 against 43.2 us).  The rule goes by the sequences,
-  // never by the rows, so a query's bits do not depend on how many new tokens stand beside it.
-  L.split = cc ? kCcSplit : (int64_t)B * hkv * ((max_seq_len + 255) / 256) >= 2048 ? 1024 : 256;
+  // against 18.7 us at 1024); where there is work for every SM either way, longer splits cost fewer prologues and
+  // partials (8 sequences, 16 heads, 512 to 4096 positions: 34.5 us at 832, 38.1 at 1024, 43.2 at 256), up to 1024,
+  // which leaves many sequences enough CTAs to balance.  Three CTAs an SM, half as many again since not every
+  // sequence is as long as the bound.  The rule goes by the sequences, never by the rows, so a query's bits do not
+  // depend on how many new tokens stand beside it.
+  const int64_t groups = (int64_t)B * hkv, n = groups >= 666 ? 1 : 666 / groups;
+  const int64_t even = ((max_seq_len + n - 1) / n + 63) / 64 * 64;
+  L.split = cc ? kCcSplit : (int)(even < 256 ? 256 : even > 1024 ? 1024 : even);
   L.row_groups = (int)((total + L.rows - 1) / L.rows);
   if (L.rows == many::ROWS) {
     // one CTA an SM: as many splits as one wave of them takes (four sequences of 8192 positions, 256 rows each: 42 us
     // in 128 CTAs, 58 us in 160); a context of up to 512 positions stays whole (12.9 against 20.6 us at 300)
-    const int64_t ctas = (int64_t)B * hkv * L.row_groups;
+    const int64_t ctas = groups * L.row_groups;
     const int64_t n = ctas >= 148 || max_seq_len <= 512 ? 1 : 148 / ctas;
     const int64_t sp = ((max_seq_len + n - 1) / n + 63) / 64 * 64;
     L.split = (int)(sp < 128 ? 128 : sp);

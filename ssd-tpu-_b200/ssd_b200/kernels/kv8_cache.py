@@ -60,16 +60,21 @@ class KV8CacheState:
         return self.pages.shape[1]
 
 
+# the current stream's handle without the Stream object around it (a microsecond of each call)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda dev: torch.cuda.current_stream(dev).cuda_stream)
+
+
 def launch(name: str, dev: int, *args) -> None:
     """Call a C entry point on the current stream of GPU ``dev``; raise for its status."""
     if dev < 0:
         raise ValueError(f"{name}: the tensors must be on a GPU")
     fn = getattr(lib(), name)
     if dev == torch.cuda.current_device():
-        rc = fn(torch.cuda.current_stream(dev).cuda_stream, *args)
+        rc = fn(_raw_stream(dev), *args)
     else:
         with torch.cuda.device(dev):
-            rc = fn(torch.cuda.current_stream(dev).cuda_stream, *args)
+            rc = fn(_raw_stream(dev), *args)
     if rc:
         check(rc, name)
 
