@@ -385,9 +385,6 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool there) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
 }
-__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, bool there) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(there ? 4 : 0) : "memory");
-}
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
@@ -842,15 +839,12 @@ constexpr uint32_t kPolls = 1u << 24;
 template <int D>
 struct Cfg {
   static constexpr uint32_t KV = TILE * D * 2, P = ROWS * TILE * 2;
-  static constexpr uint32_t RAW = TILE * D;     // one plane of a tile, as stored
   static constexpr uint32_t PITCH = D * 4 + 16;  // bytes of a row of the result, which leaves through K, V and P
   static_assert(ROWS * PITCH <= 4 * KV + P);
   // Q comes in through V and P, rows QPITCH bytes apart
   static constexpr uint32_t QPITCH = D * 2 + 16;
   static_assert(ROWS * QPITCH <= 2 * KV + P);
-  static constexpr uint32_t SC = TILE * 4;      // its scales: a position's (or, UNI, one of eight positions')
-  static constexpr uint32_t k = 0, v = 2 * KV, p = v + 2 * KV, raw = p + P, rsc = raw + 2 * 2 * RAW;
-  static constexpr uint32_t pairs = rsc + 2 * 2 * SC;
+  static constexpr uint32_t k = 0, v = 2 * KV, p = v + 2 * KV, pairs = p + P;
   static constexpr uint32_t meta = pairs + 2 * 2 * ROWS * 8, bars = meta + META * TILE * 4;
   static constexpr size_t smem = 1024 + bars + 192;  // 22 barriers, TMEM address, two flags
   // TMEM columns: two tiles' scores, Q (two f16 to a column), O
@@ -1306,16 +1300,17 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_many_kernel(const Kv
     // -------------------------------------------------------------- pages to f16 tiles
     // Four warps take the even tiles, four the odd ones (a warp's waits and addresses cost as much as its rows), a
     // warp 16 positions of a tile: RPI of them at a time, 16 dims a lane, eight lanes on four pieces of an even and
-    // an odd row (their 16-byte stores then meet no bank twice).  A lane converts the bytes that it has copied.
+    // an odd row (their 16-byte stores then meet no bank twice).  The bytes come through registers: shared memory's
+    // bandwidth is what a tile takes most of.
     constexpr int PCS = D / 16, RPI = 32 / PCS, NI = 16 / RPI, NB = UNI ? 1 : NI;
     const int set = (warp - SOFT / 32) >> 2, cw = warp & 3;
     const int rr = ((lane >> 2) & 1) | ((lane >> 3) / (PCS / 4)) << 1, pc = (lane & 3) | ((lane >> 3) % (PCS / 4)) << 2;
     const uint8_t* kp = a.c.pages + a.c.layer + (int64_t)head * D + pc * 16;
     const float* sc = a.c.scales + a.c.scale_layer + head;
     const int64_t rs = (int64_t)a.c.hkv * D;
-    int blk[NB], off[NB];  // of the tile to be fetched next
-    const uint32_t raw8 = sm + C::raw + set * 2 * C::RAW + cw * (NI * 512) + lane * 16;  // 512 bytes apart
-    const uint32_t scales = C::rsc + set * 2 * C::SC + cw * 64;
+    int blk[NB], off[NB];        // of the tile to be fetched next
+    uint4 kb[NI], vb[NI];        // this tile's bytes, then the next one's as soon as they are converted: they have two
+    float ks[NB], vs[NB];        // tiles' time to arrive; and the scales (0: no row)
     int ids = -1;          // UNI: lane x has the block id of the warp's positions in its tile 32 k + x
     auto look = [&](int j) {
       if constexpr (UNI) {
@@ -1346,42 +1341,36 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_many_kernel(const Kv
         }
       }
     };
-    // start the copies of tile j's K (plane 0) or V rows and scales (zeros where there is no row)
-    auto fetch = [&](int j, int plane) {
-      const uint32_t to = raw8 + plane * C::RAW;
+    // load tile j's K (plane 0) or V rows and scales (zeros where there is no row)
+    auto fetch = [&](int j, int plane, uint4* x, float* xs) {
       const float* from = sc + plane * a.c.scale_plane;
-      if (UNI ? lane == 0 : pc == 0) {
 #pragma unroll
-        for (int i = 0; i < NB; ++i) {
-          const bool there = (unsigned)blk[i] < (unsigned)a.c.num_blocks;
-          cp_async4(sm + scales + plane * C::SC + (UNI ? 0 : rr + i * RPI) * 4, from + (there ? (int64_t)blk[i] * a.c.hkv : 0),
-                    there);
-        }
-      }
+      for (int i = 0; i < NB; ++i)
+        xs[i] = (unsigned)blk[i] < (unsigned)a.c.num_blocks ? ld_act(from + (int64_t)blk[i] * a.c.hkv) : 0.f;
       if constexpr (UNI) {
         const bool in = (unsigned)blk[0] < (unsigned)a.c.num_blocks;
         const uint8_t* s = kp + plane * a.c.plane + (in ? ((int64_t)blk[0] * a.c.block_size + off[0] + rr) * rs : 0);
         const int left = in ? kn - j * TILE - 16 * cw - rr : 0;  // row i of the lane is there where i RPI < left
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
-          cp_async16(to + i * 512, s, i * RPI < left);
-          if (i * RPI + RPI < left) s += RPI * rs;
+          x[i] = make_uint4(0, 0, 0, 0);
+          if (i * RPI < left) x[i] = ld_act_v4(s);
+          s += RPI * rs;
         }
       } else {
 #pragma unroll
         for (int i = 0; i < NI; ++i) {
           const int n = i % NB;
-          const bool there = (unsigned)blk[n] < (unsigned)a.c.num_blocks;
-          const int64_t row = there ? (int64_t)blk[n] * a.c.block_size + off[n] : 0;
-          cp_async16(to + i * 512, kp + plane * a.c.plane + row * rs, there);
+          x[i] = make_uint4(0, 0, 0, 0);
+          if ((unsigned)blk[n] < (unsigned)a.c.num_blocks)
+            x[i] = ld_act_v4(kp + plane * a.c.plane + ((int64_t)blk[n] * a.c.block_size + off[n]) * rs);
         }
       }
-      cp_async_commit();
     };
     if (set < tiles) {
       look(set);
-      fetch(set, 0);
-      fetch(set, 1);
+      fetch(set, 0, kb, ks);
+      fetch(set, 1, vb, vs);
       look(set + 2);
     }
     // row rr + i RPI of the warp's 16: 128 bytes a row, pieces swizzled by it
@@ -1400,27 +1389,17 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_many_kernel(const Kv
 #pragma unroll 1
     for (int j = set; j < tiles; j += 2) {
       if (j >= 2 && !wait(k_free(set), ((j >> 1) - 1) & 1, stop)) break;
-      cp_async_wait<0>();
       uint32_t* mt = meta + (j % META) * TILE;
       if (UNI ? lane == 0 : pc == 0) {
-        const float* x = reinterpret_cast<const float*>(gen + scales);
 #pragma unroll
-        for (int i = 0; i < NB; ++i) {
-          const int r = UNI ? 0 : rr + i * RPI;
-          mt[UNI ? cw : 16 * cw + r] = x[r] == 0.f ? 0u : pack_meta(scale_exponent(x[r]), scale_exponent(x[C::SC / 4 + r]));
-        }
+        for (int i = 0; i < NB; ++i)
+          mt[UNI ? cw : 16 * cw + rr + i * RPI] = ks[i] == 0.f ? 0u : pack_meta(scale_exponent(ks[i]), scale_exponent(vs[i]));
       }
 #pragma unroll
-      for (int i = 0; i < NI; ++i) put(kt, i, lds128(raw8 + i * 512));
+      for (int i = 0; i < NI; ++i) put(kt, i, kb[i]);
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       tc::mbar_arrive(k_full(set));
-      uint4 vb[NI];
-#pragma unroll
-      for (int i = 0; i < NI; ++i) vb[i] = lds128(raw8 + C::RAW + i * 512);
-      __syncwarp();  // the scales have been read
-      fetch(j + 2, 0);
-      fetch(j + 2, 1);
-      look(j + 4);
+      fetch(j + 2, 0, kb, ks);
       if (j < 2 && !wait(q_tmem, 0, stop)) break;  // V's tiles hold Q until then
       if (j >= 2 && !wait(v_free(set), ((j >> 1) - 1) & 1, stop)) break;
       if (base + j * TILE + 16 * cw + 15 > kmin) {  // NaN of positions that some row does not see: put back by row above
@@ -1441,8 +1420,9 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_many_kernel(const Kv
       for (int i = 0; i < NI; ++i) put(vt, i, vb[i]);
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       tc::mbar_arrive(v_full(set));
+      fetch(j + 2, 1, vb, vs);
+      look(j + 4);
     }
-    cp_async_wait<0>();
     __syncwarp();
   } else {
     // -------------------------------------------------------------- products
