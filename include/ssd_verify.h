@@ -266,7 +266,7 @@ int ssd_paged_verify_attention(ssd_stream_t stream, const void* q, const void* p
  *   scales [2, num_layers, num_blocks, Hkv] fp32, powers of two: an element is its e4m3 value times
  *          the scale of its plane, layer, page and KV head
  * head_dim is 64, 128 or 256; pages, k, v, q, qkv and the outputs are 16-byte aligned
- * (else SSD_ERR_UNSUPPORTED).  num_blocks * block_size < 2^31.
+ * (else SSD_ERR_UNSUPPORTED).  num_blocks * block_size < 2^31, block_size <= 2^20.
  * A page's scale is the smallest power of two (at least 2^-118) under which its largest finite
  * magnitude stays within e4m3's 448.  Rounding is to nearest even; infinities and NaN are stored as
  * NaN and do not count for the scale.
@@ -311,7 +311,9 @@ size_t ssd_kv8_attention_workspace_size(int B, int T, int num_heads, int num_kv_
 /*
  * ssd_paged_verify_attention over an 8-bit cache: same rows, positions, lengths and zero rows.
  * q and out [B, T, Hq, D] in `dtype`; scores, softmax statistics and sums in fp32.  What a row does
- * not see (positions past its own, rows behind seq_lens) does not reach it, NaN included.
+ * not see (positions past its own, rows behind seq_lens) does not reach it, NaN included; a row of q
+ * that holds an infinity or NaN comes out as NaN.  max_seq_len <= 2^30.  The workspace is 16-byte
+ * aligned, needs no initial content and keeps none.
  */
 int ssd_kv8_attention(ssd_stream_t stream, const void* q, const void* pages, const float* scales, int dtype,
                       int num_layers, int num_blocks, int block_size, int num_kv_heads, int head_dim, int layer,
@@ -325,8 +327,9 @@ int ssd_kv8_attention(ssd_stream_t stream, const void* q, const void* pages, con
  * same) pool, i < n, in each of `planes` planes (2 * num_layers): `page_bytes` per page and plane,
  * and, with scales_per_page > 0, that many fp32 scales (an 8-bit cache's Hkv).  A pool's plane is
  * its block count times page_bytes.  Pairs with an id out of range on either side (-1) are skipped.
- * count (device, may be NULL): number of pairs, at most n (the ids past it are read, and may hold anything).  Within one pool no page may be both
- * copied from and copied to, nor copied to twice: the pairs move in no particular order.
+ * count (device, may be NULL): number of pairs, at most n (the ids past it are read, and may hold
+ * anything).  Within one pool no page may be both copied from and copied to, nor copied to twice: the
+ * pairs move in no particular order.
  */
 int ssd_page_copy(ssd_stream_t stream, const void* src_pages, const float* src_scales, int src_blocks,
                   void* dst_pages, float* dst_scales, int dst_blocks, int planes, size_t page_bytes,

@@ -124,8 +124,8 @@ __device__ __forceinline__ void rope_q_cta(const AppendArgs& a, int cta) {
   const int items = a.hq * PER;
   const int64_t m = cta;
   const int b = (int)(m / a.T), t = (int)(m % a.T);
-  const int seq = a.seq_lens[b];
-  const int ql = a.q_lens ? min(max(a.q_lens[b], 0), a.T) : a.T;
+  const int seq = ld_act(a.seq_lens + b);
+  const int ql = a.q_lens ? min(max(ld_act(a.q_lens + b), 0), a.T) : a.T;
   const int pos = seq - ql + t;
   const bool real = t < ql && pos >= 0;
   const int p = real ? min(pos, a.rope_max_pos - 1) : 0;

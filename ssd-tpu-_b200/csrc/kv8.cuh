@@ -106,7 +106,8 @@ inline int kv8_check(const void* pages, const float* scales, int num_layers, int
       layer >= num_layers)
     return SSD_ERR_INVALID;
   if (D != 64 && D != 128 && D != 256) return SSD_ERR_UNSUPPORTED;
-  if ((int64_t)num_blocks * block_size > 0x7fffffff) return SSD_ERR_UNSUPPORTED;  // row numbers are 32-bit
+  // row numbers, and the pieces of a page's rows, are 32-bit
+  if ((int64_t)num_blocks * block_size > 0x7fffffff || block_size > 1 << 20) return SSD_ERR_UNSUPPORTED;
   if (!kv8_aligned(pages)) return SSD_ERR_UNSUPPORTED;
   return SSD_OK;
 }

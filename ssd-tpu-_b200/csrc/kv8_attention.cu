@@ -38,6 +38,14 @@ __device__ __forceinline__ int splits_of(int seq, int split) { return max(1, (se
 // out = sum_s e^(m_s - M) o_s / sum_s e^(n_s - N) l_s * e^(M - N), M and N the largest m_s and n_s.  One CTA per
 // query row: its threads hold 4 dims of every SG-th split each and add the groups up in order, so that the
 // loads of many splits are in flight at once.  LOG2: the maxima are in powers of two.
+// The weight of a split in the join; -1 where the row saw none of it, so that what it left (zeros, or NaN of other
+// rows' positions) is passed over.  A seen split counts however small its weight: its NaN has to come through.
+template <bool LOG2>
+__device__ __forceinline__ float split_weight(float m, float M) {
+  if (m <= (LOG2 ? -1e38f : -INFINITY)) return -1.f;
+  return LOG2 ? exp2f(m - M) : expf(m - M);
+}
+
 constexpr int kJoinThreads = 256;
 constexpr int kJoinChunk = 256;  // splits whose weights are held at a time
 
@@ -79,14 +87,14 @@ __global__ void __launch_bounds__(kJoinThreads) kv8_join_kernel(const Kv8Attn a)
     if (tid < n) {
       const float4 v = __ldcg(ml + (int64_t)(s0 + tid) * R);
       if (v.y != -INFINITY) L += v.z * ex(v.y - N);
-      w_s[tid] = v.x == -INFINITY ? 0.f : ex(v.x - M);
+      w_s[tid] = split_weight<LOG2>(v.x, M);
     }
     __syncthreads();
 #pragma unroll 4
     for (int s = sg; s < n; s += SG) {
       const float f = w_s[s];
       const float4 x = __ldcg(reinterpret_cast<const float4*>(po + (int64_t)(s0 + s) * R * D));
-      if (f != 0.f) {  // a split that the row does not see holds zeros, or NaN marks of other rows
+      if (f >= 0.f) {
         o.x = fmaf(f, x.x, o.x);
         o.y = fmaf(f, x.y, o.y);
         o.z = fmaf(f, x.z, o.z);
@@ -136,7 +144,7 @@ __global__ void __launch_bounds__(128) kv8_join_few_kernel(const Kv8Attn a, int6
   if (lane < ns) v = __ldcg(a.ws_ml + (grp * a.nsplit + lane) * R + r);
   const float M = warp_max(v.x), N = warp_max(v.y);
   const float L = warp_sum(v.y == -INFINITY ? 0.f : v.z * ex(v.y - N));
-  const float w = v.x == -INFINITY ? 0.f : ex(v.x - M);
+  const float w = split_weight<LOG2>(v.x, M);
   const float4* po = reinterpret_cast<const float4*>(a.ws_o) + (grp * a.nsplit * R + r) * DQ;
   float4 o[PL];
 #pragma unroll
@@ -148,7 +156,7 @@ __global__ void __launch_bounds__(128) kv8_join_few_kernel(const Kv8Attn a, int6
     for (int i = 0; i < PL; ++i) {
       if (DQ < 32 && lane >= DQ) continue;
       const float4 x = __ldcg(po + (int64_t)s * R * DQ + i * 32 + lane);
-      if (f != 0.f) {  // a split that the row does not see holds anything
+      if (f >= 0.f) {
         o[i].x = fmaf(f, x.x, o[i].x);
         o[i].y = fmaf(f, x.y, o[i].y);
         o[i].z = fmaf(f, x.z, o[i].z);
@@ -220,9 +228,10 @@ __global__ void __launch_bounds__(kCcSplit) kv8_attention_cc_kernel(const Kv8Att
   for (int i = tid; i < kCcRows * D; i += kCcSplit) {
     const int r = i / D, d = i % D;
     const int gr = row0 + r, t = gr / a.G, g = gr % a.G;
-    reinterpret_cast<float*>(q_s[d])[r] =
-        r < nrows ? ld_act(reinterpret_cast<const float*>(a.q) + (((int64_t)b * a.T + t) * a.hq + head * a.G + g) * D + d)
-                  : 0.f;
+    float x = 0.f;
+    if (r < nrows) x = ld_act(reinterpret_cast<const float*>(a.q) + (((int64_t)b * a.T + t) * a.hq + head * a.G + g) * D + d);
+    if (fabsf(x) == INFINITY) x = __int_as_float(0x7fc00000);  // the row's scores hold NaN or an infinity less itself
+    reinterpret_cast<float*>(q_s[d])[r] = x;
   }
   if (tid < kCcRows) {
     const int t = (row0 + tid) / a.G;
@@ -522,13 +531,15 @@ __global__ void __launch_bounds__(kFewWarps * 32, NT == 1 ? 3 : 2) kv8_attention
       const float2 y = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w.y));
       f[k] = x.x; f[k + 1] = x.y; f[k + 2] = y.x; f[k + 3] = y.y;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) amax = fmaxf(amax, finite_abs(f[k + j]));
+      for (int j = 0; j < 4; ++j) amax = fmaxf(amax, fabsf(f[k + j]));  // NaN reaches the scores by itself
     }
 #pragma unroll
     for (int x = 1; x < 16; x <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, x));
     const int e = min(max((int)(__float_as_uint(amax) >> 23) - 127, -118), 120);
     const float inv = exp2i(-e);
-    if ((lane & 15) == 0) qscale_s[8 * nt + r] = exp2i(e) * a.scale * 1.4426950408889634f;
+    // an infinity in q leaves no finite score, or one less itself: NaN
+    if ((lane & 15) == 0)
+      qscale_s[8 * nt + r] = amax == INFINITY ? __int_as_float(0x7fc00000) : exp2i(e) * a.scale * 1.4426950408889634f;
 #pragma unroll
     for (int k = 0; k < D / 16; k += 4) {
       const int d = (lane & 15) * (D / 16) + k, c = d >> 6, tt = (d >> 4) & 3, j = (d >> 2) & 3;
@@ -1063,13 +1074,14 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_many_kernel(const Kv
 #pragma unroll
         for (int j = 0; j < 4; ++j) t2 = __hmax2(t2, __habs2(h[j]));
       }
-      // largest magnitude (infinities and NaN end in NaN scores of the row)
+      // largest magnitude, NaN aside (it reaches the scores by itself)
       float top = fmaxf(__low2float(t2), __high2float(t2)), other = top, unused = 0.f;
       ok = ok && swap(pair_s, 0, other, unused);
       top = fmaxf(top, other);
       const int e = min(max((int)(__float_as_uint(top) >> 23) - 127, -118), 120);
       const float inv = copysignf(exp2i(-e), a.scale);  // the row's factor is never negative
       qs = exp2i(e) * fabsf(a.scale) * 1.4426950408889634f;
+      if (top == INFINITY) qs = __int_as_float(0x7fc00000);  // such a row has no finite score, or one less itself
       if (qs == 0.f) qs = 1e-38f;  // keeps the mask's infinity out of 0 * infinity; the scores stay below 2^-60
 #pragma unroll
       for (int c = 0; c < NQ; c += 4) {
@@ -1490,7 +1502,8 @@ struct Kv8Layout {
   bool cc;              // CUDA-core kernel (fp32)
   int rows;             // query rows of a group
   int split;            // positions of a split
-  int row_groups, nsplit;
+  int64_t row_groups;
+  int nsplit;
   size_t groups, off_o, off_ml, total;
 };
 
@@ -1501,6 +1514,9 @@ inline size_t up256(size_t x) { return (x + 255) & ~size_t(255); }
 // way).  Up to 8 tokens always the few-row one, so that a verify step gives a query the bits that decoding it alone
 // does (40 rows, 32 sequences: 52 us, where the other kernel takes 37).
 constexpr int kManyRows = 32, kFewTokens = 8;
+constexpr int kMaxFewSplit = 1024;  // positions of a split of the few-row kernel, at most
+
+constexpr int kMaxSeqLen = 1 << 30;  // so that a position behind the last split's end is still an int
 
 Kv8Layout kv8_layout(bool cc, int B, int T, int hq, int hkv, int D, int max_seq_len) {
   Kv8Layout L;
@@ -1515,8 +1531,8 @@ Kv8Layout kv8_layout(bool cc, int B, int T, int hq, int hkv, int D, int max_seq_
   // depend on how many new tokens stand beside it.
   const int64_t groups = (int64_t)B * hkv, n = groups >= 666 ? 1 : 666 / groups;
   const int64_t even = ((max_seq_len + n - 1) / n + 63) / 64 * 64;
-  L.split = cc ? kCcSplit : (int)(even < 256 ? 256 : even > 1024 ? 1024 : even);
-  L.row_groups = (int)((total + L.rows - 1) / L.rows);
+  L.split = cc ? kCcSplit : (int)(even < 256 ? 256 : even > kMaxFewSplit ? kMaxFewSplit : even);
+  L.row_groups = (total + L.rows - 1) / L.rows;
   if (L.rows == many::ROWS) {
     // one CTA an SM: as many splits as one wave of them takes (four sequences of 8192 positions, 256 rows each: 42 us
     // in 128 CTAs, 58 us in 160); a context of up to 512 positions stays whole (12.9 against 20.6 us at 300)
@@ -1547,7 +1563,7 @@ int launch_few(cudaStream_t st, const Kv8Attn& a, int B) {
   const dim3 grid(a.nsplit, a.c.hkv * a.row_groups, B);
   auto kern = kv8_attention_few_kernel<D, NT, UNI>;
   static std::atomic<uint64_t> ready{0};
-  if (!allow_smem(ready, kern, (int)FewSmem<D, NT, UNI>::total(2048))) return SSD_ERR_LAUNCH;
+  if (!allow_smem(ready, kern, (int)FewSmem<D, NT, UNI>::total(kMaxFewSplit))) return SSD_ERR_LAUNCH;
   SSD_PDL(kern, grid, kFewWarps * 32, smem, st, a);
   return a.nsplit == 1 ? SSD_OK : launch_join<bf16, D, 8 * NT, true>(st, a, B);
 }
@@ -1578,7 +1594,7 @@ using namespace ssd;
 extern "C" size_t ssd_kv8_attention_workspace_size(int B, int T, int num_heads, int num_kv_heads, int head_dim,
                                                    int max_seq_len) {
   if (B <= 0 || T <= 0 || num_kv_heads <= 0 || num_heads <= 0 || num_heads % num_kv_heads || head_dim <= 0 ||
-      max_seq_len <= 0)
+      max_seq_len <= 0 || max_seq_len > kMaxSeqLen)
     return 0;
   const size_t a = kv8_layout(true, B, T, num_heads, num_kv_heads, head_dim, max_seq_len).total;
   const size_t b = kv8_layout(false, B, T, num_heads, num_kv_heads, head_dim, max_seq_len).total;
@@ -1596,10 +1612,11 @@ extern "C" int ssd_kv8_attention(ssd_stream_t stream, const void* q, const void*
     return SSD_ERR_INVALID;
   if (B == 0 || T == 0) return SSD_OK;
   if (!q || !out || (int64_t)max_blocks * block_size < max_seq_len) return SSD_ERR_INVALID;
-  if (!kv8_aligned(q) || !kv8_aligned(out) || (int64_t)max_blocks * block_size > 0x7fffffff)
+  if (!kv8_aligned(q) || !kv8_aligned(out) || !kv8_aligned(workspace) ||
+      (int64_t)max_blocks * block_size > 0x7fffffff || max_seq_len > kMaxSeqLen)
     return SSD_ERR_UNSUPPORTED;
   const Kv8Layout L = kv8_layout(dtype == SSD_DTYPE_F32, B, T, num_heads, num_kv_heads, head_dim, max_seq_len);
-  if (B > 65535 || (int64_t)num_kv_heads * L.row_groups > 65535)
+  if (B > 65535 || L.row_groups > 65535 || num_kv_heads * L.row_groups > 65535)
     return SSD_ERR_UNSUPPORTED;
   if (!workspace || workspace_bytes < L.total) return SSD_ERR_WORKSPACE;
   char* w = reinterpret_cast<char*>(workspace);
@@ -1616,7 +1633,7 @@ extern "C" int ssd_kv8_attention(ssd_stream_t stream, const void* q, const void*
   a.T = T;
   a.hq = num_heads;
   a.G = num_heads / num_kv_heads;
-  a.row_groups = L.row_groups;
+  a.row_groups = (int)L.row_groups;
   a.nsplit = L.nsplit;
   a.split = L.split;
   a.ws_o = reinterpret_cast<float*>(w + L.off_o);

@@ -30,7 +30,7 @@ class KV8CacheState:
     pages: torch.Tensor
     scales: torch.Tensor
     block_size: int
-    # (device index, -1 on the CPU; pages, scales: pointers; layers, blocks, block size, KV heads, head dim)
+    # layers, blocks, block size, KV heads, head dim
     dims: tuple = field(init=False, repr=False, compare=False)
 
     def __post_init__(self) -> None:
@@ -41,7 +41,7 @@ class KV8CacheState:
         two, nl, nb, bs, hkv, hd = p.shape
         if two != 2 or bs != self.block_size or s.shape != (2, nl, nb, hkv):
             raise ValueError(f"scales {tuple(s.shape)} and block_size {self.block_size} do not fit pages {tuple(p.shape)}")
-        object.__setattr__(self, "dims", (p.get_device(), p.data_ptr(), s.data_ptr(), nl, nb, bs, hkv, hd))
+        object.__setattr__(self, "dims", (nl, nb, bs, hkv, hd))
 
     @classmethod
     def allocate(cls, num_layers: int, num_blocks: int, block_size: int, num_kv_heads: int, head_dim: int,
@@ -89,6 +89,12 @@ def ints(t: torch.Tensor | None, shape: tuple, what: str, dev: int) -> int | Non
     return t.data_ptr()
 
 
+def _cache(cache: KV8CacheState) -> tuple:
+    """(device index, pages and scales: pointers, layers, blocks, block size, KV heads, head dim)."""
+    p = cache.pages
+    return (p.get_device(), p.data_ptr(), cache.scales.data_ptr(), *cache.dims)
+
+
 def _rows(t: torch.Tensor, what: str, dev: int) -> torch.Tensor:
     if t.get_device() != dev:
         raise ValueError(f"{what} is on {t.device}, the cache on cuda:{dev}")
@@ -114,7 +120,7 @@ def append_kv8(cache: KV8CacheState, layer: int, block_tables: torch.Tensor, seq
     ones starts over; in any other page the earlier rows keep their values.  A page that is written
     belongs to one sequence (fork a shared one first, ``PageManager.fork_rows``).
     """
-    dev, pages, scales, nl, nb, bs, hkv, hd = cache.dims
+    dev, pages, scales, nl, nb, bs, hkv, hd = _cache(cache)
     if k.dim() != 4 or k.shape[2] != hkv or k.shape[3] != hd or v.shape != k.shape or v.dtype != k.dtype:
         raise ValueError(f"k and v must be [B, T, {hkv}, {hd}] of one dtype, got {list(k.shape)} and {list(v.shape)}")
     b, t = k.shape[0], k.shape[1]
@@ -131,7 +137,7 @@ def rope_append_kv8(qkv: torch.Tensor, cache: KV8CacheState, layer: int, block_t
                     q_lens: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """RoPE on the q and k parts of qkv [B*T, (Hq+2Hkv)*D], k and v appended to the cache
     (``ssd_kv8_rope_append``); returns the rotated q [B, T, Hq, D] (zeros for t >= q_lens[b])."""
-    dev, pages, scales, nl, nb, bs, hkv, hd = cache.dims
+    dev, pages, scales, nl, nb, bs, hkv, hd = _cache(cache)
     b = block_tables.shape[0]
     width = (num_heads + 2 * hkv) * hd
     if qkv.dim() != 2 or qkv.shape[1] != width or (qkv.shape[0] % b if b else qkv.shape[0]):
@@ -158,7 +164,7 @@ def rope_append_kv8(qkv: torch.Tensor, cache: KV8CacheState, layer: int, block_t
 def gather_kv8(cache: KV8CacheState, layer: int, block_tables: torch.Tensor, positions: torch.Tensor,
                dtype=torch.bfloat16) -> tuple[torch.Tensor, torch.Tensor]:
     """K and V rows [B, N, Hkv, D] of positions [B, N] (-1: zeros), as the values the cache holds (``ssd_kv8_gather``)."""
-    dev, pages, scales, nl, nb, bs, hkv, hd = cache.dims
+    dev, pages, scales, nl, nb, bs, hkv, hd = _cache(cache)
     if positions.dim() != 2:
         raise ValueError(f"positions must be [B, N], got {list(positions.shape)}")
     b, n = positions.shape
@@ -180,7 +186,7 @@ def paged_kv8_attention(q: torch.Tensor, cache: KV8CacheState, layer: int, block
     q_lens[b] come back as zeros.  For T up to 8 a query's bits do not depend on how many new tokens
     stand beside it.
     """
-    dev, pages, scales, nl, nb, bs, hkv, hd = cache.dims
+    dev, pages, scales, nl, nb, bs, hkv, hd = _cache(cache)
     if q.dim() != 4 or q.shape[3] != hd:
         raise ValueError(f"q must be [B, T, Hq, {hd}], got {list(q.shape)}")
     b, t, hq, _ = q.shape

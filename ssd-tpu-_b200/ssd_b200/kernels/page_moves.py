@@ -90,6 +90,8 @@ def compact_pages(cache, tables: torch.Tensor, lens: torch.Tensor, ref_counts: t
         raise ValueError("draft_tables and draft_lens go together")
     if tables.dim() != 2 or (draft_tables is not None and draft_tables.dim() != 2):
         raise ValueError("tables are [rows, max_blocks]")
+    if inplace and draft_tables is not None and draft_tables.data_ptr() == tables.data_ptr() and tables.numel():
+        raise ValueError("tables and draft_tables are the same memory: in place, they would be mapped twice")
     half = max(1, nb // 2)
     remap = torch.empty(nb, dtype=torch.int32, device=tables.device)
     plan = torch.empty(2 * half + 1, dtype=torch.int32, device=tables.device)  # the moves' sources, targets, number

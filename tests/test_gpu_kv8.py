@@ -437,3 +437,97 @@ def test_strided_rows_and_refusals(cuda):
         paged_kv8_attention(q.half(), cache, 0, tab, sl)
     with pytest.raises(SSDError):
         paged_kv8_attention(q, cache, 0, tab, sl, max_seq_len=1000)  # more than the table holds
+
+
+@pytest.mark.parametrize("dtype,hq,hkv,d,t", [("bf16", 8, 2, 256, 1), ("bf16", 16, 2, 64, 3), ("bf16", 8, 2, 128, 30),
+                                              ("f32", 8, 2, 64, 3)])
+@pytest.mark.parametrize("n", [40, 2000])
+def test_attention_of_non_finite_queries(cuda, dtype, hq, hkv, d, t, n):
+    """An infinity or NaN in a row of q: that row is NaN (it has no finite score, or an infinite one less itself), also
+    where every score is minus infinity; the rows beside it do not notice."""
+    from ssd_b200.kernels.kv8_cache import paged_kv8_attention
+
+    torch, dts = _torch()
+    rng = np.random.default_rng(n + d)
+    p = Pool(rng, 1, 16, hkv, d, cols=n // 16 + 1)
+    k = _round(rng.standard_normal((1, n, hkv, d)), "bf16")
+    k[..., 0] = 1.0  # an infinity in dim 0 gives every score its sign
+    p.append([n], k, k, [n], "bf16")
+    i = lambda a: torch.tensor(np.asarray(a, np.int32), device="cuda")  # noqa: E731
+    q = torch.tensor(_round(rng.standard_normal((1, t, hq, d)), dtype)).to(dts[dtype]).cuda()
+    want = paged_kv8_attention(q, p.cache, 1, p.dev_tables, i([n]))
+    bad = q.clone()
+    rows = [(0, 0, 0, float("inf")), (0, 2, 0, float("-inf")), (t - 1, hq - 1, 5, float("nan")),
+            (t - 1, hq // 2, d - 1, float("inf"))]
+    dead = torch.zeros(want.shape, dtype=torch.bool, device="cuda")
+    for tt, h, dim, x in rows:
+        bad[0, tt, h, dim] = x
+        dead[0, tt, h] = True
+    got = paged_kv8_attention(bad, p.cache, 1, p.dev_tables, i([n]))
+    assert torch.equal(got.isnan(), dead)
+    assert torch.equal(got[~dead], want[~dead])
+
+
+@pytest.mark.parametrize("dtype,hq,hkv,d,t", [("bf16", 8, 1, 256, 1), ("bf16", 4, 2, 64, 3), ("bf16", 8, 1, 128, 30),
+                                              ("f32", 4, 1, 64, 3)])
+def test_nan_at_a_position_of_vanishing_weight(cuda, dtype, hq, hkv, d, t):
+    """NaN in V reaches every row that sees it, though its weight is e^-1000 and lies in another part of the context."""
+    from ssd_b200.kernels.kv8_cache import paged_kv8_attention
+
+    torch, dts = _torch()
+    rng = np.random.default_rng(2)
+    n = 6000
+    p = Pool(rng, 1, 16, hkv, d, cols=n // 16)
+    k = np.zeros((1, n, hkv, d))
+    k[0, 5000, :, 0] = 100.0
+    v = _round(rng.standard_normal((1, n, hkv, d)), "bf16")
+    v[0, 17, :, 3] = np.nan
+    p.append([n], k, v, [n], "bf16")
+    q = torch.zeros((1, t, hq, d), dtype=dts[dtype], device="cuda")
+    q[..., 0] = 10.0
+    i = lambda a: torch.tensor(np.asarray(a, np.int32), device="cuda")  # noqa: E731
+    got = paged_kv8_attention(q, p.cache, 1, p.dev_tables, i([n]), scale=1.0)
+    nan = got.isnan()
+    assert nan[..., 3].all() and int(nan.sum()) == t * hq
+    val = torch.tensor(p.vals[1, p.tables[0, 5000 // 16], 5000 % 16]).cuda()
+    scale = np.exp2(p.exps[1, p.tables[0, 5000 // 16]].astype(np.float64))
+    want = (val * torch.tensor(scale).cuda()[:, None]).repeat_interleave(hq // hkv, 0)
+    keep = torch.arange(d, device="cuda") != 3
+    assert torch.equal(got[0, :, :, keep].double(), want[None, :, keep].to(dts[dtype]).double().expand(t, -1, -1))
+
+
+def test_cache_past_32_bit_offsets(cuda):
+    """Planes of more than 4 GB: the highest pages hold and give what low pages of a small cache do, bit for bit."""
+    from ssd_b200.kernels.kv8_cache import KV8CacheState, append_kv8, gather_kv8, paged_kv8_attention, rope_append_kv8
+    from ssd_b200.kernels.page_moves import copy_pages
+
+    torch, dts = _torch()
+    hkv, d, n, nb = 16, 256, 400, 66_000  # 64 KB a page and plane
+    cols = -(-n // 16)
+    small = KV8CacheState.allocate(1, cols, 16, hkv, d)
+    big = KV8CacheState.allocate(1, nb, 16, hkv, d)
+    assert big.pages[0].numel() > 2 ** 32
+    lo = torch.arange(cols, dtype=torch.int32, device="cuda").view(1, -1)
+    hi = (nb - 1 - lo).contiguous()
+    sl = torch.tensor([n], dtype=torch.int32, device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(1)
+    rnd = lambda *s: torch.randn(s, generator=g, device="cuda")  # noqa: E731
+    k, v = rnd(1, n, hkv, d).bfloat16(), rnd(1, n, hkv, d).bfloat16()
+    qkv, cos = rnd(4, 3 * hkv * d).bfloat16(), rnd(512, d // 2)
+    at = torch.arange(n, dtype=torch.int32, device="cuda").view(1, -1)
+    outs = []
+    for c, tab in ((small, lo), (big, hi)):
+        append_kv8(c, 0, tab, sl, k, v)
+        outs.append([rope_append_kv8(qkv, c, 0, tab, sl, hkv, cos, cos), *gather_kv8(c, 0, tab, at)])
+        for t, dt in ((1, "bf16"), (5, "bf16"), (100, "bf16"), (3, "f32")):
+            g2 = torch.Generator(device="cuda").manual_seed(t)
+            q = torch.randn((1, t, hkv, d), generator=g2, device="cuda").to(dts[dt])
+            outs[-1].append(paged_kv8_attention(q, c, 0, tab, sl, max_seq_len=n))
+    for a, b in zip(*outs):
+        assert torch.equal(a, b)
+    ids = hi[0, :5]
+    copy_pages(big, ids, torch.arange(5, dtype=torch.int32, device="cuda") + 65_700)
+    copy_pages(big, ids, torch.arange(5, dtype=torch.int32, device="cuda"))
+    for first in (0, 65_700):
+        assert torch.equal(big.pages[:, 0, first:first + 5].view(torch.uint8), small.pages[:, 0, :5].view(torch.uint8))
+        assert torch.equal(big.scales[:, 0, first:first + 5], small.scales[:, 0, :5])

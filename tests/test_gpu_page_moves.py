@@ -138,3 +138,47 @@ def test_compact_pages(cuda, kind, nb, used, inplace):
         assert r.tables is args[0] and r.free_top is args[4]
     else:
         assert all(torch.equal(a, k) for a, k in zip(args, kept))
+
+
+@pytest.mark.parametrize("nb,rows,cols", [(50_000, 64, 600), (200_000, 3, 20_000)])
+def test_compact_large_pools(cuda, nb, rows, cols):
+    """Pools whose flags take more than the default shared memory, or more than there is; tables that get a launch of
+    their own, the draft's among them."""
+    import torch
+
+    from ssd_b200.kernels.page_moves import compact_pages
+
+    rng = np.random.default_rng(nb)
+    c = _cache("kv8", 1, nb, 1, 1, 64, 3)
+    perm = rng.permutation(nb)
+    used = nb // 2 + 17
+    tables = rng.permutation(perm[:used])[rng.integers(0, used, (rows, cols))].astype(np.int32)
+    draft = perm[rng.integers(0, used, (2, cols))].astype(np.int32)
+    lens, dlens = rng.integers(0, cols + 1, rows).astype(np.int32), np.array([cols, 5], np.int32)
+    ref = rng.integers(0, 4, nb).astype(np.int32)
+    free = np.full(nb, -1, np.int32)
+    free[:nb - used] = perm[used:]
+    ref[perm[used:]] = 0
+    u, src, dst, remap, nref, ntab, fl = _plain_compact(nb, perm[used:], ref, tables, lens)
+    dtab = np.where(np.arange(cols)[None] < dlens[:, None], remap[draft], -1)
+    t = lambda a: torch.tensor(np.asarray(a, np.int32), device="cuda")  # noqa: E731
+    want = _bytes(c)
+    for w in want:
+        w[:, :, dst] = w[:, :, src]
+    r = compact_pages(c, t(tables), t(lens), t(ref), t(free), t([nb - used]), t(draft), t(dlens))
+    assert all(torch.equal(a, w) for a, w in zip(_bytes(c), want))
+    for got, exp in ((r.remap, remap), (r.ref_counts, nref), (r.tables, ntab), (r.draft_tables, dtab),
+                     (r.free_list, fl), (r.free_top, np.array([nb - u]))):
+        np.testing.assert_array_equal(got.cpu().numpy(), exp)
+
+
+def test_compact_refuses_one_table_for_both(cuda):
+    import torch
+
+    from ssd_b200.kernels.page_moves import compact_pages
+
+    c = _cache("bf16", 1, 8, 16, 1, 64, 1)
+    z = lambda *s: torch.zeros(s, dtype=torch.int32, device="cuda")  # noqa: E731
+    tab, lens = z(2, 4), z(2)
+    with pytest.raises(ValueError):
+        compact_pages(c, tab, lens, z(8), z(8), z(1), tab, lens, inplace=True)

@@ -119,3 +119,21 @@ def test_python_refusals():
         copy_pages(cache, torch.zeros(1, dtype=torch.int64), torch.zeros(1, dtype=torch.int32))
     with pytest.raises(ValueError):
         compact_pages([], tab, lens, lens, lens, lens)
+
+
+def test_sizes_past_the_kernels_integers_are_refused():
+    """Limits that keep 32-bit positions, rows and pieces in range: 4 (unsupported), before anything is launched."""
+    from ssd_b200._lib import lib
+
+    so, P, big = lib(), 4096, 1 << 30
+
+    def attn(nb=8, bs=16, hkv=2, b=1, t=1, hq=4, mb=4, mx=64, ws=P):
+        return so.ssd_kv8_attention(None, P, P, P, 0, 1, nb, bs, hkv, 64, 0, P, mb, P, None, P, 0.1, b, t, hq, mx, ws,
+                                    1 << 62)
+
+    assert attn(t=big, hq=1 << 20, hkv=1) == 4          # more row groups than a grid has
+    assert attn(mb=(1 << 31) - 1, bs=1, mx=big + 1) == 4
+    assert attn(ws=P + 8) == 4
+    assert attn(nb=1, bs=(1 << 20) + 1) == 4
+    assert so.ssd_kv8_attention_workspace_size(1, 1, 4, 2, 64, big + 1) == 0
+    assert so.ssd_kv8_append(None, P, P, 1, 1, (1 << 20) + 1, 2, 64, 0, P, 4, P, None, P, P, 0, 1, 1) == 4
