@@ -12,6 +12,8 @@
 // workspace holds nothing between calls and may come uninitialised from any allocator.
 #include <float.h>
 
+#include <algorithm>
+
 #include "kv8.cuh"
 #include "tcgen05.cuh"
 
@@ -27,13 +29,29 @@ struct Kv8Attn {
   const int32_t* seq_lens;
   const int32_t* q_lens;
   float scale;
-  int T, hq, G, row_groups, nsplit, split;  // split: positions of one
+  int B, T, hq, G, row_groups, nsplit, split;  // split: positions of one
   float* ws_o;          // [group][split][rows][D]
   float4* ws_ml;        // [group][split][rows]: maximum that o is relative to, that l is relative to, l
+  // With a plan (many rows), the splits go by the sequences' own lengths: nsplit of them for all sequences together,
+  // partials [head][row group][split][rows], and plan[b] says which are sequence b's: the first, and how many.
+  int2* plan;
 };
+
+constexpr int kMaxSeqLen = 1 << 30;  // so that a position behind the last split's end is still an int
 
 // Splits of a sequence that hold positions (at least one, which writes its zero rows).
 __device__ __forceinline__ int splits_of(int seq, int split) { return max(1, (seq + split - 1) / split); }
+
+// A row group's partials: how many, and the index of the first.
+__device__ __forceinline__ int partials_of(const Kv8Attn& a, int b, int head, int rg, int64_t grp, int64_t& first) {
+  if (a.plan) {
+    const int2 p = __ldcg(a.plan + b);
+    first = (int64_t)(head * a.row_groups + rg) * a.nsplit + p.x;
+    return p.y;
+  }
+  first = grp * a.nsplit;
+  return splits_of(min(min(ld_act(a.seq_lens + b), a.max_blocks * a.c.block_size), a.nsplit * a.split), a.split);
+}
 
 // out = sum_s e^(m_s - M) o_s / sum_s e^(n_s - N) l_s * e^(M - N), M and N the largest m_s and n_s.  One CTA per
 // query row: its threads hold 4 dims of every SG-th split each and add the groups up in order, so that the
@@ -64,12 +82,11 @@ __global__ void __launch_bounds__(kJoinThreads) kv8_join_kernel(const Kv8Attn a)
   pdl_wait();
   pdl_trigger();
   if (t >= a.T) return;
-  const int seq_full = ld_act(a.seq_lens + b);
-  const int seq = min(min(seq_full, a.max_blocks * a.c.block_size), a.nsplit * a.split);
   const int ql = a.q_lens ? min(max(ld_act(a.q_lens + b), 0), a.T) : a.T;
-  const int ns = splits_of(seq, a.split);
+  int64_t s0;
+  const int ns = partials_of(a, b, head, rg, grp, s0);
   auto ex = [](float v) { return LOG2 ? exp2f(v) : expf(v); };
-  const float4* ml = a.ws_ml + grp * a.nsplit * R + r;
+  const float4* ml = a.ws_ml + s0 * R + r;
   float M = -INFINITY, N = -INFINITY;
   for (int s = tid; s < ns; s += kJoinThreads) {
     const float4 v = __ldcg(ml + (int64_t)s * R);
@@ -79,13 +96,13 @@ __global__ void __launch_bounds__(kJoinThreads) kv8_join_kernel(const Kv8Attn a)
   M = block_reduce(M, red, OpMax());
   N = block_reduce(N, red, OpMax());
   const int d4 = tid % DQ, sg = tid / DQ;
-  const float* po = a.ws_o + (grp * a.nsplit * R + r) * D + d4 * 4;
+  const float* po = a.ws_o + (s0 * R + r) * D + d4 * 4;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
   float L = 0.f;
-  for (int s0 = 0; s0 < ns; s0 += kJoinChunk) {
-    const int n = min(kJoinChunk, ns - s0);
+  for (int c0 = 0; c0 < ns; c0 += kJoinChunk) {
+    const int n = min(kJoinChunk, ns - c0);
     if (tid < n) {
-      const float4 v = __ldcg(ml + (int64_t)(s0 + tid) * R);
+      const float4 v = __ldcg(ml + (int64_t)(c0 + tid) * R);
       if (v.y != -INFINITY) L += v.z * ex(v.y - N);
       w_s[tid] = split_weight<LOG2>(v.x, M);
     }
@@ -93,7 +110,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv8_join_kernel(const Kv8Attn a)
 #pragma unroll 4
     for (int s = sg; s < n; s += SG) {
       const float f = w_s[s];
-      const float4 x = __ldcg(reinterpret_cast<const float4*>(po + (int64_t)(s0 + s) * R * D));
+      const float4 x = __ldcg(reinterpret_cast<const float4*>(po + (int64_t)(c0 + s) * R * D));
       if (f >= 0.f) {
         o.x = fmaf(f, x.x, o.x);
         o.y = fmaf(f, x.y, o.y);
@@ -122,7 +139,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv8_join_kernel(const Kv8Attn a)
   }
 }
 
-// The same for few splits: one warp a row, 4 dims of a lane at a time.
+// The same for few splits: one warp a row, 4 dims of a lane at a time, the weights of 32 splits in its lanes.
 template <typename T, int D, int R, bool LOG2>
 __global__ void __launch_bounds__(128) kv8_join_few_kernel(const Kv8Attn a, int64_t rows) {
   constexpr int DQ = D / 4, PL = DQ < 32 ? 1 : DQ / 32;  // float4 of a row, of a lane
@@ -136,34 +153,51 @@ __global__ void __launch_bounds__(128) kv8_join_few_kernel(const Kv8Attn a, int6
   pdl_wait();
   pdl_trigger();
   if (row >= rows || t >= a.T) return;
-  const int seq_full = ld_act(a.seq_lens + b);
   const int ql = a.q_lens ? min(max(ld_act(a.q_lens + b), 0), a.T) : a.T;
-  const int ns = splits_of(min(min(seq_full, a.max_blocks * a.c.block_size), a.nsplit * a.split), a.split);
+  int64_t s0;
+  const int ns = partials_of(a, b, head, rg, grp, s0);
   auto ex = [](float v) { return LOG2 ? exp2f(v) : expf(v); };
-  float4 v = make_float4(-INFINITY, -INFINITY, 0.f, 0.f);
-  if (lane < ns) v = __ldcg(a.ws_ml + (grp * a.nsplit + lane) * R + r);
-  const float M = warp_max(v.x), N = warp_max(v.y);
-  const float L = warp_sum(v.y == -INFINITY ? 0.f : v.z * ex(v.y - N));
-  const float w = split_weight<LOG2>(v.x, M);
-  const float4* po = reinterpret_cast<const float4*>(a.ws_o) + (grp * a.nsplit * R + r) * DQ;
+  const float4* ml = a.ws_ml + s0 * R + r;
+  float M = -INFINITY, N = -INFINITY;
+  float4 v;
+  for (int c0 = 0; c0 < ns; c0 += 32) {
+    v = make_float4(-INFINITY, -INFINITY, 0.f, 0.f);
+    if (c0 + lane < ns) v = __ldcg(ml + (int64_t)(c0 + lane) * R);
+    M = fmaxf(M, v.x);
+    N = fmaxf(N, v.y);
+  }
+  M = warp_max(M);
+  N = warp_max(N);
+  float L = 0.f;
+  const float4* po = reinterpret_cast<const float4*>(a.ws_o) + (s0 * R + r) * DQ;
   float4 o[PL];
 #pragma unroll
   for (int i = 0; i < PL; ++i) o[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int c0 = 0; c0 < ns; c0 += 32) {
+    if (ns > 32) {  // else they are still there
+      v = make_float4(-INFINITY, -INFINITY, 0.f, 0.f);
+      if (c0 + lane < ns) v = __ldcg(ml + (int64_t)(c0 + lane) * R);
+    }
+    L += v.y == -INFINITY ? 0.f : v.z * ex(v.y - N);
+    const float w = split_weight<LOG2>(v.x, M);
+    const int n = min(32, ns - c0);
 #pragma unroll 4
-  for (int s = 0; s < ns; ++s) {
-    const float f = __shfl_sync(0xffffffffu, w, s);
+    for (int s = 0; s < n; ++s) {
+      const float f = __shfl_sync(0xffffffffu, w, s);
 #pragma unroll
-    for (int i = 0; i < PL; ++i) {
-      if (DQ < 32 && lane >= DQ) continue;
-      const float4 x = __ldcg(po + (int64_t)s * R * DQ + i * 32 + lane);
-      if (f >= 0.f) {
-        o[i].x = fmaf(f, x.x, o[i].x);
-        o[i].y = fmaf(f, x.y, o[i].y);
-        o[i].z = fmaf(f, x.z, o[i].z);
-        o[i].w = fmaf(f, x.w, o[i].w);
+      for (int i = 0; i < PL; ++i) {
+        if (DQ < 32 && lane >= DQ) continue;
+        const float4 x = __ldcg(po + (int64_t)(c0 + s) * R * DQ + i * 32 + lane);
+        if (f >= 0.f) {
+          o[i].x = fmaf(f, x.x, o[i].x);
+          o[i].y = fmaf(f, x.y, o[i].y);
+          o[i].z = fmaf(f, x.z, o[i].z);
+          o[i].w = fmaf(f, x.w, o[i].w);
+        }
       }
     }
   }
+  L = warp_sum(L);
   const bool real = t < ql && L != 0.f;
   const float k = ex(M - N);
   T* out = reinterpret_cast<T*>(a.out) + (((int64_t)b * a.T + t) * a.hq + head * a.G + g) * D;
@@ -184,7 +218,7 @@ template <typename T, int D, int R, bool LOG2>
 int launch_join(cudaStream_t st, const Kv8Attn& a, int B) {
   const int64_t rows = (int64_t)B * a.c.hkv * a.row_groups * R;
   if (rows > 0x7fffffff) return SSD_ERR_UNSUPPORTED;
-  if (a.nsplit <= 16)
+  if ((a.plan ? a.nsplit / B : a.nsplit) <= 16)
     SSD_PDL((kv8_join_few_kernel<T, D, R, LOG2>), (unsigned)((rows + 3) / 4), 128, 0, st, a, rows);
   else
     SSD_PDL((kv8_join_kernel<T, D, R, LOG2>), (unsigned)rows, kJoinThreads, 0, st, a);
@@ -844,6 +878,7 @@ constexpr int TILE = 64;     // positions of a tile
 constexpr int SOFT = 256;    // threads of the row warps: two a query row, 32 positions of a tile each
 constexpr int CONV = 256;    // threads of the converting warps
 constexpr int THREADS = SOFT + CONV + 32;
+constexpr int kMinTiles = 2; // of a split
 constexpr int META = 4;      // tiles whose scales are kept: a tile's are read until its weights are done
 constexpr uint32_t kPolls = 1u << 24;
 
@@ -960,6 +995,71 @@ __device__ __forceinline__ uint64_t mn_desc(uint32_t saddr) {
          ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
 }
 
+// Which part of which sequence split `slot` is, where the splits go by the sequences' lengths: the shortest split of
+// whole tiles with which all sequences together make no more than nsplit, found by bisection.  Every warp works it out
+// for itself; lane x holds sequences x, x + 32, ..
+struct Part {
+  int b, split, span;  // sequence (-1: none), number in it, positions of a split
+  int seq, ql;         // its lengths
+};
+constexpr int kPlanRegs = 3;          // 148 splits at most, two of them at least for each sequence
+
+__device__ __forceinline__ Part find_part(const Kv8Attn& a, int slot, bool publish) {
+  const int lane = threadIdx.x & 31;
+  int seq[kPlanRegs], ql[kPlanRegs];
+#pragma unroll
+  for (int k = 0; k < kPlanRegs; ++k) {
+    seq[k] = lane + 32 * k < a.B ? ld_act(a.seq_lens + lane + 32 * k) : 0;
+    ql[k] = lane + 32 * k < a.B && a.q_lens ? ld_act(a.q_lens + lane + 32 * k) : a.T;
+  }
+  uint32_t t[kPlanRegs], total = 0;
+#pragma unroll
+  for (int k = 0; k < kPlanRegs; ++k) {
+    const int n = max(min(seq[k], min(a.max_blocks * a.c.block_size, kMaxSeqLen)), 0);
+    t[k] = (uint32_t)(n / TILE + (n % TILE != 0));
+    total += t[k];
+  }
+  total = __reduce_add_sync(0xffffffffu, total);
+  auto parts = [&](int k, uint32_t span) {
+    return lane + 32 * k < a.B ? max(1u, (t[k] + span - 1) / span) : 0u;
+  };
+  const uint32_t N = (uint32_t)a.nsplit, extra = N - (uint32_t)a.B;
+  uint32_t lo = max((uint32_t)kMinTiles, (total + N - 1) / N), hi = max(lo, (total + extra - 1) / extra);
+  while (lo < hi) {
+    const uint32_t mid = (lo + hi) / 2;
+    uint32_t n = 0;
+#pragma unroll
+    for (int k = 0; k < kPlanRegs; ++k) n += parts(k, mid);
+    if (__reduce_add_sync(0xffffffffu, n) <= N) hi = mid;
+    else lo = mid + 1;
+  }
+  Part p{-1, 0, (int)(lo * TILE), 0, 0};
+  uint32_t before = 0;
+#pragma unroll
+  for (int k = 0; k < kPlanRegs; ++k) {
+    if (32 * k >= a.B) break;
+    const uint32_t mine = parts(k, lo);
+    uint32_t x = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    const int first = (int)(before + x - mine);
+    if (publish && mine) a.plan[lane + 32 * k] = make_int2(first, (int)mine);
+    const uint32_t hit = __ballot_sync(0xffffffffu, slot >= first && slot < first + (int)mine);
+    if (hit) {
+      const int from = __ffs(hit) - 1;
+      p.b = from + 32 * k;
+      p.split = slot - __shfl_sync(0xffffffffu, first, from);
+      p.seq = __shfl_sync(0xffffffffu, seq[k], from);
+      p.ql = __shfl_sync(0xffffffffu, ql[k], from);
+    }
+    before += __shfl_sync(0xffffffffu, x, 31);
+  }
+  return p;
+}
+
 // UNI: block_size is a multiple of 16.
 template <int D, bool UNI>
 __global__ void __launch_bounds__(THREADS, 1) kv8_attention_many_kernel(const Kv8Attn a) {
@@ -982,7 +1082,6 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_many_kernel(const Kv
   volatile int* nan_seen = reinterpret_cast<volatile int*>(slot + 2);
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int split = blockIdx.x, b = blockIdx.z;
   const int head = blockIdx.y / a.row_groups, rg = blockIdx.y % a.row_groups;
   if (tid == 0) {
     tc::mbar_init(q_in, ROWS);
@@ -1015,15 +1114,22 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_many_kernel(const Kv
   const uint32_t tmem = *slot;
   pdl_wait();
 
-  const int seq_full = ld_act(a.seq_lens + b);
-  const int ql = a.q_lens ? min(max(ld_act(a.q_lens + b), 0), a.T) : a.T;
-  const int seq = min(min(seq_full, a.max_blocks * a.c.block_size), a.nsplit * a.split);
-  const int base = split * a.split;
+  Part part;
+  if (a.plan) {
+    part = find_part(a, blockIdx.x, blockIdx.x == 0 && blockIdx.y == 0 && warp == 0);
+  } else {
+    const int z = blockIdx.z;
+    part = Part{z, 0, a.split, ld_act(a.seq_lens + z), a.q_lens ? ld_act(a.q_lens + z) : a.T};
+  }
+  const bool idle = part.b < 0;  // fewer splits than there may be
+  const int b = idle ? 0 : part.b, span = part.span, seq_full = part.seq, ql = min(max(part.ql, 0), a.T);
+  const int seq = min(min(seq_full, a.max_blocks * a.c.block_size), a.plan ? kMaxSeqLen : span);
+  const int base = part.split * span;
   const int row0 = rg * ROWS, rows = min(ROWS, a.G * a.T - row0);
   const int n0 = seq_full - ql;
   const int t0 = row0 / a.G, t1 = min((row0 + rows - 1) / a.G, ql - 1);  // the group's first and last real token
   const int kmin = max(n0 + t0, 0);                                       // every row that sees anything sees 0..kmin
-  const int kn = t0 > t1 ? 0 : min(min(seq, base + a.split), n0 + t1 + 1) - base;
+  const int kn = idle || t0 > t1 ? 0 : min(min(seq, base + span), n0 + t1 + 1) - base;
   const int tiles = kn > 0 ? (kn + TILE - 1) / TILE : 0;
   const int32_t* table = a.tables + (int64_t)b * a.max_blocks;
 
@@ -1242,15 +1348,15 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_many_kernel(const Kv
     }
     tc::tc_fence_after();
     if (!ok) l = __int_as_float(0x7fc00000);
-    const int64_t grp = ((int64_t)b * a.c.hkv + head) * a.row_groups + rg;
-    const int64_t po = (grp * a.nsplit + split) * ROWS + r;
+    const bool partial = a.plan != nullptr;
+    const int64_t po = ((int64_t)blockIdx.y * a.nsplit + blockIdx.x) * ROWS + r;
     const bool any = real && l != 0.f;  // l is NaN, not 0, where a seen score is
-    if (a.nsplit > 1 && half == 0) a.ws_ml[po] = make_float4(M, N, l, 0.f);
-    if (a.nsplit == 1 || tiles > 0) {
+    if (partial && !idle && half == 0) a.ws_ml[po] = make_float4(M, N, l, 0.f);
+    if (!partial || tiles > 0) {
       // O through the shared memory of K, V and P (every product is done): a thread puts its half row there and
       // sends it off with one bulk copy
-      const float k = a.nsplit > 1 ? 1.f : any ? ex2(M - N) / l : 0.f;
-      const bool zero = a.nsplit == 1 && !any;  // O may be anything where a row sees nothing
+      const float k = partial ? 1.f : any ? ex2(M - N) / l : 0.f;
+      const bool zero = !partial && !any;  // O may be anything where a row sees nothing
       constexpr int HD = D / 2;
       const uint32_t mine = sm + r * C::PITCH + half * (HD * 4);
 #pragma unroll 1
@@ -1263,7 +1369,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_many_kernel(const Kv
 #pragma unroll
           for (int i = 0; i < 32; ++i) y[i] = 0;
         }
-        if (a.nsplit > 1) {
+        if (partial) {
 #pragma unroll
           for (int i = 0; i < 8; ++i)
             sts128(mine + c * 4 + 16 * i, make_uint4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]));
@@ -1282,11 +1388,11 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_many_kernel(const Kv
         }
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      if (a.nsplit > 1 || r < rows) {
-        const void* to = a.nsplit > 1 ? (const void*)(a.ws_o + po * D + half * HD)
+      if (partial || r < rows) {
+        const void* to = partial ? (const void*)(a.ws_o + po * D + half * HD)
                                       : (const void*)(reinterpret_cast<bf16*>(a.out) + at + half * HD);
         asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(to), "r"(mine),
-                     "r"(a.nsplit > 1 ? HD * 4 : HD * 2)
+                     "r"(partial ? HD * 4 : HD * 2)
                      : "memory");
       }
       asm volatile("cp.async.bulk.commit_group;" ::: "memory");
@@ -1301,7 +1407,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_many_kernel(const Kv
 #pragma unroll 1
           for (int d = half * HD; d < (half + 1) * HD; ++d) {
             if ((__ldcg(v + d) & 0x7f) != 0x7f) continue;
-            if (a.nsplit > 1) a.ws_o[po * D + d] = __int_as_float(0x7fc00000);
+            if (partial) a.ws_o[po * D + d] = __int_as_float(0x7fc00000);
             else reinterpret_cast<bf16*>(a.out)[at + d] = __ushort_as_bfloat16(0x7fc0);
           }
         }
@@ -1330,7 +1436,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_many_kernel(const Kv
         if ((mine & 31) == 0) {
           // whatever the length says: a tile's rows are bounded where they are fetched
           const int p = (j + 2 * lane) * TILE + 16 * cw, page = (base + p) / a.c.block_size;
-          ids = page < a.max_blocks && p < a.split ? ld_act(table + page) : -1;
+          ids = page < a.max_blocks && p < span ? ld_act(table + page) : -1;
         }
         blk[0] = __shfl_sync(0xffffffffu, ids, mine & 31);
         if (mine == 0) {
@@ -1504,7 +1610,9 @@ struct Kv8Layout {
   int split;            // positions of a split
   int64_t row_groups;
   int nsplit;
-  size_t groups, off_o, off_ml, total;
+  bool planned;         // the splits go by the sequences' lengths
+  size_t partials;      // rows of them
+  size_t off_ml, off_plan, total;
 };
 
 inline size_t up256(size_t x) { return (x + 255) & ~size_t(255); }
@@ -1516,10 +1624,8 @@ inline size_t up256(size_t x) { return (x + 255) & ~size_t(255); }
 constexpr int kManyRows = 32, kFewTokens = 8;
 constexpr int kMaxFewSplit = 1024;  // positions of a split of the few-row kernel, at most
 
-constexpr int kMaxSeqLen = 1 << 30;  // so that a position behind the last split's end is still an int
-
 Kv8Layout kv8_layout(bool cc, int B, int T, int hq, int hkv, int D, int max_seq_len) {
-  Kv8Layout L;
+  Kv8Layout L{};
   const int64_t total = (int64_t)(hq / hkv) * T;
   L.cc = cc;
   L.rows = cc ? kCcRows : total > kManyRows && T > kFewTokens ? many::ROWS : total > 8 ? 16 : 8;
@@ -1534,19 +1640,22 @@ Kv8Layout kv8_layout(bool cc, int B, int T, int hq, int hkv, int D, int max_seq_
   L.split = cc ? kCcSplit : (int)(even < 256 ? 256 : even > kMaxFewSplit ? kMaxFewSplit : even);
   L.row_groups = (total + L.rows - 1) / L.rows;
   if (L.rows == many::ROWS) {
-    // one CTA an SM: as many splits as one wave of them takes (four sequences of 8192 positions, 256 rows each: 42 us
-    // in 128 CTAs, 58 us in 160); a context of up to 512 positions stays whole (12.9 against 20.6 us at 300)
-    const int64_t ctas = groups * L.row_groups;
-    const int64_t n = ctas >= 148 || max_seq_len <= 512 ? 1 : 148 / ctas;
-    const int64_t sp = ((max_seq_len + n - 1) / n + 63) / 64 * 64;
-    L.split = (int)(sp < 128 ? 128 : sp);
+    // One CTA an SM: as many splits, over all sequences, as one wave of them takes (four sequences of 8192 positions,
+    // 256 rows each: 42 us in 128 CTAs, 58 us in 160), where that is two a sequence or more; a context of up to 512
+    // positions stays whole (12.9 against 20.6 us at 300).
+    const int64_t most = B * (((int64_t)max_seq_len - 1) / (many::kMinTiles * many::TILE) + 1);
+    const int64_t n = std::min(148 / (hkv * L.row_groups), most);
+    L.planned = n >= (int64_t)2 * B && max_seq_len > 512;
+    L.nsplit = L.planned ? (int)n : 1;
+    L.split = (max_seq_len + many::TILE - 1) / many::TILE * many::TILE;
+    L.partials = L.planned ? (size_t)(hkv * L.row_groups * n * L.rows) : 0;
+  } else {
+    L.nsplit = (max_seq_len + L.split - 1) / L.split;
+    L.partials = L.nsplit == 1 ? 0 : (size_t)(groups * L.row_groups) * L.nsplit * L.rows;
   }
-  L.nsplit = (max_seq_len + L.split - 1) / L.split;
-  L.groups = (size_t)B * hkv * L.row_groups;
-  const size_t rows = L.nsplit == 1 ? 0 : L.groups * L.nsplit * L.rows;
-  L.off_o = 0;
-  L.off_ml = L.off_o + up256(sizeof(float) * rows * D);
-  L.total = L.off_ml + up256(sizeof(float4) * rows) + 256;
+  L.off_ml = up256(sizeof(float) * L.partials * D);
+  L.off_plan = L.off_ml + up256(sizeof(float4) * L.partials);
+  L.total = L.off_plan + up256(L.planned ? sizeof(int2) * B : 1);
   return L;
 }
 
@@ -1575,8 +1684,8 @@ int launch_many(cudaStream_t st, const Kv8Attn& a, int B) {
   static_assert(smem <= 227 * 1024);
   static std::atomic<uint64_t> ready{0};
   if (!allow_smem(ready, kern, (int)smem)) return SSD_ERR_LAUNCH;
-  SSD_PDL(kern, dim3(a.nsplit, a.c.hkv * a.row_groups, B), many::THREADS, smem, st, a);
-  return a.nsplit == 1 ? SSD_OK : launch_join<bf16, D, many::ROWS, true>(st, a, B);
+  SSD_PDL(kern, dim3(a.nsplit, a.c.hkv * a.row_groups, a.plan ? 1 : B), many::THREADS, smem, st, a);
+  return !a.plan ? SSD_OK : launch_join<bf16, D, many::ROWS, true>(st, a, B);
 }
 
 template <int D>
@@ -1630,14 +1739,16 @@ extern "C" int ssd_kv8_attention(ssd_stream_t stream, const void* q, const void*
   a.seq_lens = seq_lens;
   a.q_lens = q_lens;
   a.scale = scale;
+  a.B = B;
   a.T = T;
   a.hq = num_heads;
   a.G = num_heads / num_kv_heads;
   a.row_groups = (int)L.row_groups;
   a.nsplit = L.nsplit;
   a.split = L.split;
-  a.ws_o = reinterpret_cast<float*>(w + L.off_o);
+  a.ws_o = reinterpret_cast<float*>(w);
   a.ws_ml = reinterpret_cast<float4*>(w + L.off_ml);
+  a.plan = L.planned ? reinterpret_cast<int2*>(w + L.off_plan) : nullptr;
   cudaStream_t st = (cudaStream_t)stream;
   if (dtype == SSD_DTYPE_BF16) {
     if (head_dim == 256) return launch_bf16<256>(st, a, L, B);

@@ -531,3 +531,34 @@ def test_cache_past_32_bit_offsets(cuda):
     for first in (0, 65_700):
         assert torch.equal(big.pages[:, 0, first:first + 5].view(torch.uint8), small.pages[:, 0, :5].view(torch.uint8))
         assert torch.equal(big.scales[:, 0, first:first + 5], small.scales[:, 0, :5])
+
+
+@pytest.mark.parametrize("case", [
+    ("bf16", 4, 1, 64, 16, 9, [9 + 17 * i % 700 for i in range(70)]),       # three registers of lengths
+    ("bf16", 8, 1, 64, 16, 12, [0, 12, 4000] + [15 + i for i in range(17)]),  # one sequence takes most of the splits
+    ("bf16", 4, 2, 128, 16, 40, [0, 40, 1000, 41, 333]),
+    ("bf16", 8, 1, 128, 4, 20, [20, 900, 0]),                               # pages smaller than a tile
+    ("bf16", 2, 2, 256, 16, 33, [33, 700]),
+], ids=lambda c: f"{len(c[6])}x{c[5]}-{c[3]}")
+def test_many_rows_over_ragged_batches(cuda, case):
+    """Splits that go by the sequences' own lengths: empty, short and long ones beside each other; a bound that is
+    far above every length gives the same, and so does a second run."""
+    from ssd_b200.kernels.kv8_cache import paged_kv8_attention
+
+    torch, dts = _torch()
+    dtype, hq, hkv, d, bs, t, lens = case
+    p, q, ql = _attention_inputs(case, seed=len(lens) + t)
+    ql = np.minimum(ql, lens)
+    i = lambda a: torch.tensor(np.asarray(a, np.int32), device="cuda")  # noqa: E731
+    args = (torch.tensor(q).to(dts[dtype]).cuda(), p.cache, 1, p.dev_tables, i(lens))
+    got = paged_kv8_attention(*args, q_lens=i(ql))
+    assert torch.equal(got, paged_kv8_attention(*args, q_lens=i(ql)))
+    ref, mass, size = o.attention(q, p.vals, p.exps, p.tables, lens, ql, 1 / math.sqrt(d))
+    tol = _tolerance(case, q, p, lens, mass, size, ref)
+    err = np.abs(got.float().cpu().numpy() - ref)
+    assert (err <= tol).all(), (err / np.maximum(tol, 1e-300)).max()
+    for r in range(len(lens)):
+        assert (got[r, ql[r]:] == 0).all()
+    wide = torch.cat([p.dev_tables, torch.full_like(p.dev_tables, -1)], 1)
+    far = paged_kv8_attention(*args[:3], wide, args[4], q_lens=i(ql)).float().cpu().numpy()
+    assert (np.abs(far - ref) <= tol).all()
