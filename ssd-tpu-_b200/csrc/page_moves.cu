@@ -29,8 +29,9 @@ struct CopyArgs {
 };
 
 // One CTA per (pair, part): a part is kCopyItems vectors a thread out of the pair's pages in all planes, their loads
-// in flight together (a page of one plane may be small: 8 KB pages, one plane a CTA, reached 3.0 TB/s).  Pairs
-// with an id out of range on either side (-1) are skipped.  Bound: HBM.
+// in flight together (a page of one plane may be small: 8 KB pages, one plane a CTA, reached 3.0 TB/s; so 5.6).
+// Pairs with an id out of range on either side (-1) are skipped.  Bound: HBM (1100 pages of 36 planes of 32 KB: 2.6 GB
+// in 394 us, 6.6 TB/s).
 constexpr int kCopyItems = 8;
 
 template <typename V>
@@ -78,7 +79,8 @@ __global__ void __launch_bounds__(kCopyThreads) page_copy_kernel(const CopyArgs 
 // below U: the fewest moves there can be, and no block is both read and written.  One CTA: the pool's state
 // is a few integers per block; each thread owns a run of blocks, ranks come from block-wide scans, and what is
 // free or used is kept in shared memory (a byte a block; pools past kFlagCap in the remap array itself).  The
-// same CTA then rewrites the tables.
+// same CTA then rewrites the tables.  Bound by latency: 7 us with the copies of a pool of 256 blocks, some 10 us of
+// the 91 that 3000 blocks of 18 layers take (438 MB moved).
 constexpr int kPlanThreads = 1024;
 constexpr int kFlagCap = 160 * 1024;
 
