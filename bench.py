@@ -70,6 +70,8 @@ def parse():
                     help="batched mode: top-p nucleus of the draft and target distributions (1 = off)")
     ap.add_argument("--ctx-min", type=int, default=1024)
     ap.add_argument("--ctx-max", type=int, default=8192)
+    ap.add_argument("--kv-cache-dtype", choices=["auto", "fp8"], default="auto",
+                    help="--batch: caches in the weights' dtype, or in 8 bits")
     ap.add_argument("--mode", choices=["sd", "ssd"], default="sd",
                     help="ssd: the async ssd engine through LLM.generate in ONE process -- target "
                          "tensor-parallel over GPUs 0..--tp-1, draft and its worker on GPU --tp; prints "
@@ -736,7 +738,7 @@ def run_batched(args):
     blocks = sum((c + grow + 15) // 16 + 1 for c in ctx) + 2
     dec = BatchedSpeculativeDecoder(target, draft, batch=B, k=k, max_seq_len=max_seq,
                                     temperature=args.temperature, top_p=args.top_p, seed=7, comm=comm,
-                                    num_blocks=blocks)
+                                    num_blocks=blocks, kv_cache_dtype=args.kv_cache_dtype)
     dec.start_synthetic(ctx, np.random.default_rng(1))
     for _ in range(args.warmup):
         dec.step()
@@ -771,8 +773,9 @@ def run_batched(args):
     mean_ctx = ctx_sum / args.steps / B
     w_t = lt.layer_weight_bytes() * lt.num_layers + (st_.vocab // world) * st_.d_model * 2
     w_d = ld.layer_weight_bytes() * ld.num_layers + (sd_.vocab // world) * sd_.d_model * 2
-    kv_t = B * mean_ctx * lt.kv_bytes_per_token()
-    kv_d = B * mean_ctx * ld.kv_bytes_per_token()
+    kv_part = 0.5 if args.kv_cache_dtype == "fp8" else 1.0  # of the bf16 cache's bytes
+    kv_t = B * mean_ctx * lt.kv_bytes_per_token() * kv_part
+    kv_d = B * mean_ctx * ld.kv_bytes_per_token() * kv_part
     step_bytes = w_t + kv_t + k * (w_d + kv_d)
     step_s = ms / 1000.0 / args.steps
     # FLOPs per step on this rank: 2 per weight element per token row (verify: B*(k+1) rows,
@@ -796,7 +799,8 @@ def run_batched(args):
             "data": "synthetic (random-init weights; contexts stood in by seeded N(0,1) K/V)",
             "config": {"workload": f"batched serving B={B}, k={k}, T={args.temperature}, ctx U[{args.ctx_min}, "
                                    f"{args.ctx_max}]", "parallelism": f"tp{world}",
-                       "top_p": args.top_p if args.temperature > 0 and args.top_p < 1 else None},
+                       "top_p": args.top_p if args.temperature > 0 and args.top_p < 1 else None,
+                       "kv_cache_dtype": args.kv_cache_dtype},
             "tokens_per_step": tokens / args.steps, "accept_rate": accepted / (args.steps * B * k),
             "verify_ms": statistics.mean(verify_ms),
             "step_bytes_per_rank": step_bytes, "step_hbm_gbs": step_bytes / step_s / 1e9,
