@@ -302,8 +302,8 @@ int append_common(ssd_stream_t stream, AppendArgs a, int dtype, int B, int T, in
 
 // K and V rows of positions [B][N] (-1: zeros).  A row of one position is 2 Hkv D values; a warp takes up to
 // kGatherItems * 32 groups of 8 of them (8 bytes in, 16 or 32 out, neighbouring lanes on neighbouring groups), all
-// loads in flight at once.  Bound: HBM (the 6000 rows above: 147 MB in 28 us, 5.2 TB/s).
-constexpr int kGatherItems = 4;
+// loads in flight at once (4, 8, 16 groups a lane: 28, 25.5, 29 us).  Bound: HBM (the 6000 rows above: 147 MB, 5.8 TB/s).
+constexpr int kGatherItems = 8;
 
 template <typename T, int D>
 __global__ void __launch_bounds__(256) kv8_gather_kernel(const Kv8Cache c, const int32_t* tables, int max_blocks,

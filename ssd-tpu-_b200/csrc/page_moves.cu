@@ -8,7 +8,7 @@
 namespace ssd {
 namespace {
 
-constexpr int kCopyThreads = 256;
+constexpr int kCopyThreads = 128;
 
 struct PageRuns {
   const char* src;
@@ -25,20 +25,20 @@ struct CopyArgs {
   const int32_t* count;          // pairs on the device, or NULL (= n)
   int n, planes;
   int src_blocks, dst_blocks;
-  int parts;                     // CTAs a pair is cut into
 };
 
-// One CTA per (pair, part): a part is kCopyItems vectors a thread out of the pair's pages in all planes, their loads
-// in flight together (a page of one plane may be small: 8 KB pages, one plane a CTA, reached 3.0 TB/s; so 5.6).
-// Pairs with an id out of range on either side (-1) are skipped.  Bound: HBM (1100 pages of 36 planes of 32 KB: 2.6 GB
-// in 394 us, 6.6 TB/s).
+// One CTA per (part, pair): a part is kCopyItems vectors a thread out of the pair's pages in all planes, their loads
+// in flight together.  Neighbouring CTAs take the same part of neighbouring pairs, so that what is in flight lies close
+// together in one plane (742 moves of 36 planes of 8 KB: 85 us where the parts of a pair were neighbours 91, and 80
+// with 128 threads for 256; one plane a CTA reached half of that).  Pairs with an id out of range on either side (-1)
+// are skipped.  Bound: HBM (1100 pages of 36 planes of 32 KB: 2.6 GB in 387 us, 6.7 TB/s).
 constexpr int kCopyItems = 8;
 
 template <typename V>
 __global__ void __launch_bounds__(kCopyThreads) page_copy_kernel(const CopyArgs a) {
   pdl_wait();
   pdl_trigger();
-  const int i = (int)(blockIdx.x / a.parts), part = (int)(blockIdx.x % a.parts);
+  const int i = (int)(blockIdx.x % a.n), part = (int)(blockIdx.x / a.n);
   // ids past the count are read too (they are there) so that the two loads do not wait for each other
   const int s = ld_act(a.src_ids + i * a.src_step), d = ld_act(a.dst_ids + i * a.dst_step);
   if (a.count && i >= ld_act(a.count)) return;
@@ -80,7 +80,7 @@ __global__ void __launch_bounds__(kCopyThreads) page_copy_kernel(const CopyArgs 
 // is a few integers per block; each thread owns a run of blocks, ranks come from block-wide scans, and what is
 // free or used is kept in shared memory (a byte a block; pools past kFlagCap in the remap array itself).  The
 // same CTA then rewrites the tables.  Bound by latency: 7 us with the copies of a pool of 256 blocks, some 10 us of
-// the 91 that 3000 blocks of 18 layers take (438 MB moved).
+// the 80 that 3000 blocks of 18 layers take (438 MB moved).
 constexpr int kPlanThreads = 1024;
 constexpr int kFlagCap = 160 * 1024;
 
@@ -207,11 +207,10 @@ __global__ void table_remap_kernel(const TableArgs t, const int32_t* remap, int 
 }
 
 template <typename V>
-int launch_copy(cudaStream_t st, CopyArgs a) {
+int launch_copy(cudaStream_t st, const CopyArgs& a) {
   const int64_t items = a.data.bytes / (int64_t)sizeof(V) * a.planes;
   const int64_t parts = (items + kCopyThreads * kCopyItems - 1) / (kCopyThreads * kCopyItems);
   if (parts * a.n > 0x7fffffff) return SSD_ERR_UNSUPPORTED;
-  a.parts = (int)parts;
   SSD_PDL(page_copy_kernel<V>, (unsigned)(parts * a.n), kCopyThreads, 0, st, a);
   return SSD_OK;
 }
