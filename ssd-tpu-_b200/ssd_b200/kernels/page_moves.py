@@ -12,6 +12,8 @@ import torch
 
 from .kv8_cache import ints, launch
 
+_MAX_PAGE = 1 << 31  # bytes of a page in one plane (``ssd_page_copy``)
+
 
 def _pool(cache) -> tuple:
     """(device, pages, scales or None: pointers, blocks, planes, bytes of a page in one plane, scales of a page, rest)."""
@@ -86,6 +88,8 @@ def compact_pages(cache, tables: torch.Tensor, lens: torch.Tensor, ref_counts: t
     dev, nb = pools[0][0], pools[0][3]
     if any(p[0] != dev or p[3] != nb for p in pools):
         raise ValueError("the caches of one pool have the same blocks and device")
+    if any(p[5] > _MAX_PAGE for p in pools):  # before the tables change: the copies would be refused
+        raise ValueError(f"a page of one plane may hold {_MAX_PAGE} bytes at most")
     if (draft_tables is None) != (draft_lens is None):
         raise ValueError("draft_tables and draft_lens go together")
     if tables.dim() != 2 or (draft_tables is not None and draft_tables.dim() != 2):

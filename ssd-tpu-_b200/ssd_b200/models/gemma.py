@@ -319,6 +319,10 @@ class GemmaRunner:
         scales = None
         if not isinstance(pages, torch.Tensor):
             scales, pages = getattr(pages, "scales", None), pages.pages
+            sh = self.w.shape
+            if (pages.shape[1], *pages.shape[4:]) != (sh.num_layers, sh.num_kv_heads, sh.head_dim):
+                raise ValueError(f"a cache {list(pages.shape)} is not this model's: {sh.num_layers} layers, "
+                                 f"{sh.num_kv_heads} KV heads of {sh.head_dim}")
         if scales is None and pages.dtype == torch.float8_e4m3fn:
             raise ValueError("an fp8 cache is passed as the KV8CacheState: its pages mean nothing without the scales")
         bt = GemmaBatchC()

@@ -562,3 +562,24 @@ def test_many_rows_over_ragged_batches(cuda, case):
     wide = torch.cat([p.dev_tables, torch.full_like(p.dev_tables, -1)], 1)
     far = paged_kv8_attention(*args[:3], wide, args[4], q_lens=i(ql)).float().cpu().numpy()
     assert (np.abs(far - ref) <= tol).all()
+
+
+@pytest.mark.parametrize("case", [
+    ("bf16", 8, 2, 64, 48, 3, [3, 700, 1300]),     # pages of three groups of 16
+    ("bf16", 8, 2, 64, 48, 30, [30, 700, 1300]),
+    ("bf16", 4, 1, 128, 512, 2, [2, 513, 1500]),   # pages longer than a tile, and than a split
+    ("bf16", 4, 1, 128, 512, 40, [40, 513, 1500]),
+    ("f32", 4, 1, 64, 512, 3, [3, 513, 700]),
+], ids=lambda c: f"{c[0]}-{c[4]}-{c[5]}")
+def test_page_sizes_beside_the_tiles(cuda, case):
+    from ssd_b200.kernels.kv8_cache import paged_kv8_attention
+
+    torch, dts = _torch()
+    dtype, hq, hkv, d, bs, t, lens = case
+    p, q, ql = _attention_inputs(case, seed=bs + t)
+    p.check()
+    i = lambda a: torch.tensor(np.asarray(a, np.int32), device="cuda")  # noqa: E731
+    got = paged_kv8_attention(torch.tensor(q).to(dts[dtype]).cuda(), p.cache, 1, p.dev_tables, i(lens), q_lens=i(ql))
+    ref, mass, size = o.attention(q, p.vals, p.exps, p.tables, lens, ql, 1 / math.sqrt(d))
+    err, tol = np.abs(got.float().cpu().numpy() - ref), _tolerance(case, q, p, lens, mass, size, ref)
+    assert (err <= tol).all(), (err / np.maximum(tol, 1e-300)).max()

@@ -255,3 +255,21 @@ def test_adapter_branches_on_an_8_bit_cache(cuda):
     assert [len(o) for o in out] == [4, 4, 4] and all(0 <= t < 1024 for o in out for t in o)
     spec, logits = ad.draft_speculate([3, 1, 4, 1, 5], 3)
     assert len(spec) == 3 and logits.shape == (3, 1024)
+
+
+def test_forward_refuses_another_models_cache(cuda):
+    import torch
+
+    from ssd_b200.kernels.kv8_cache import KV8CacheState
+    from ssd_b200.kernels.kv_cache import KVCacheState
+    from ssd_b200.models.gemma import GemmaRunner, GemmaShape
+
+    s = GemmaShape(2, 256, 8, 2, 64, 1024, 2048)
+    run = GemmaRunner(_model(torch.bfloat16, s), 1, 4, 64)
+    table, tok = _i32([[0, 1, 2, 3]]), _i32([[1, 2]])
+    good = KV8CacheState.allocate(2, 4, 16, 2, 64)
+    run.forward(tok, _i32([0]), good, table, None)
+    for bad in (KV8CacheState.allocate(1, 4, 16, 2, 64), KV8CacheState.allocate(2, 4, 16, 1, 64),
+                KV8CacheState.allocate(2, 4, 16, 2, 128), KVCacheState.allocate(1, 4, 16, 2, 64), good.pages):
+        with pytest.raises(ValueError):
+            run.forward(tok, _i32([0]), bad, table, None)

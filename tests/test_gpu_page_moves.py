@@ -182,3 +182,57 @@ def test_compact_refuses_one_table_for_both(cuda):
     tab, lens = z(2, 4), z(2)
     with pytest.raises(ValueError):
         compact_pages(c, tab, lens, z(8), z(8), z(1), tab, lens, inplace=True)
+
+
+def test_moves_in_a_graph_and_on_another_stream(cuda):
+    """A captured copy and compaction, replayed on fresh contents; the same on a side stream."""
+    import torch
+
+    from ssd_b200.kernels.page_moves import compact_pages, copy_pages
+
+    nb, rows, cols = 60, 3, 12
+    t = lambda a: torch.tensor(np.asarray(a, np.int32), device="cuda")  # noqa: E731
+
+    def state(seed):
+        r = np.random.default_rng(seed)
+        perm = r.permutation(nb)
+        tables, lens = np.full((rows, cols), -1, np.int32), np.full(rows, 8, np.int32)
+        tables[:, :8] = perm[:24].reshape(rows, 8)
+        ref = np.zeros(nb, np.int32)
+        ref[perm[:24]] = 1
+        free = np.full(nb, -1, np.int32)
+        free[:nb - 24] = perm[24:]
+        return perm, tables, lens, ref, free
+
+    c = _cache("kv8", 2, nb, 16, 2, 64, 5)
+    fill = [_cache("kv8", 2, nb, 16, 2, 64, 6 + i) for i in range(2)]
+    src, dst = t([3, 5, 3]), t([10, 11, -1])
+    args = [t(x) for x in state(0)[1:]] + [t([nb - 24])]
+    compact_pages(c, *args)  # loads the kernels
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        copy_pages(c, src, dst)
+        r = compact_pages(c, *args)
+    side = torch.cuda.Stream()
+    for seed in (1, 2):
+        perm, *new = state(seed)
+        for a, x in zip(args, new):
+            a.copy_(t(x))
+        for x, y in ((c.pages.view(torch.uint8), fill[seed - 1].pages.view(torch.uint8)), (c.scales, fill[seed - 1].scales)):
+            x.copy_(y)
+        want = _bytes(c)
+        u, s, d, remap, nref, ntab, fl = _plain_compact(nb, perm[24:], new[2], new[0], new[1])
+        for w in want:
+            w[:, :, 10], w[:, :, 11] = w[:, :, 3].clone(), w[:, :, 5].clone()
+            w[:, :, d] = w[:, :, s]
+        torch.cuda.synchronize()
+        if seed == 1:
+            graph.replay()
+        else:
+            with torch.cuda.stream(side):
+                copy_pages(c, src, dst)
+                r = compact_pages(c, *args)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, w) for a, w in zip(_bytes(c), want))
+        assert r.tables.tolist() == ntab.tolist() and r.free_list.tolist() == fl.tolist()
+        assert r.remap.tolist() == remap.tolist() and r.ref_counts.tolist() == nref.tolist()
