@@ -60,9 +60,12 @@ class KV8CacheState:
         return self.pages.shape[1]
 
 
-# the current stream's handle without the Stream object around it (a microsecond of each call)
+# the current stream's handle without the Stream object around it, and the current device without the module's lazy
+# initialisation (a tensor on a GPU has seen to that): a microsecond of each call
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda dev: torch.cuda.current_stream(dev).cuda_stream)
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+_int32 = torch.int32
 
 
 def launch(name: str, dev: int, *args) -> None:
@@ -70,7 +73,7 @@ def launch(name: str, dev: int, *args) -> None:
     if dev < 0:
         raise ValueError(f"{name}: the tensors must be on a GPU")
     fn = getattr(lib(), name)
-    if dev == torch.cuda.current_device():
+    if dev == _current_device():
         rc = fn(_raw_stream(dev), *args)
     else:
         with torch.cuda.device(dev):
@@ -83,10 +86,10 @@ def ints(t: torch.Tensor | None, shape: tuple, what: str, dev: int) -> int | Non
     """Pointer of a contiguous int32 array of the shape on GPU ``dev`` (None for None)."""
     if t is None:
         return None
-    if t.dtype is not torch.int32 or t.get_device() != dev or t.shape != shape or not t.is_contiguous():
-        raise ValueError(f"{what} must be a contiguous int32 tensor {list(shape)} on cuda:{dev}, got "
-                         f"{t.dtype} {list(t.shape)} on {t.device}")
-    return t.data_ptr()
+    if t.dtype is _int32 and t.shape == shape and t.get_device() == dev and t.is_contiguous():
+        return t.data_ptr()
+    raise ValueError(f"{what} must be a contiguous int32 tensor {list(shape)} on cuda:{dev}, got "
+                     f"{t.dtype} {list(t.shape)} on {t.device}")
 
 
 def _cache(cache: KV8CacheState) -> tuple:
@@ -95,19 +98,25 @@ def _cache(cache: KV8CacheState) -> tuple:
     return (p.get_device(), p.data_ptr(), cache.scales.data_ptr(), *cache.dims)
 
 
-def _rows(t: torch.Tensor, what: str, dev: int) -> torch.Tensor:
+def _rows(t: torch.Tensor, what: str, dev: int) -> tuple[torch.Tensor, int]:
+    """The rows as the kernels read them (contiguous, 16 bytes at a time), and their pointer."""
     if t.get_device() != dev:
         raise ValueError(f"{what} is on {t.device}, the cache on cuda:{dev}")
     if not t.is_contiguous():
-        return t.contiguous()
-    return t.clone() if t.data_ptr() & 15 else t  # the kernels move 16 bytes at a time
+        t = t.contiguous()
+    at = t.data_ptr()
+    if at & 15:
+        t = t.clone()
+        at = t.data_ptr()
+    return t, at
 
 
 def _tables(t: torch.Tensor, b: int, dev: int) -> tuple[int, int]:
     """(pointer, columns) of block tables [b, max_blocks]."""
-    if t.dim() != 2:
-        raise ValueError(f"block_tables must be [{b}, max_blocks], got {list(t.shape)}")
-    m = t.shape[1]
+    shape = t.shape
+    if len(shape) != 2:
+        raise ValueError(f"block_tables must be [{b}, max_blocks], got {list(shape)}")
+    m = shape[1]
     return ints(t, (b, m), "block_tables", dev), m
 
 
@@ -121,13 +130,15 @@ def append_kv8(cache: KV8CacheState, layer: int, block_tables: torch.Tensor, seq
     belongs to one sequence (fork a shared one first, ``PageManager.fork_rows``).
     """
     dev, pages, scales, nl, nb, bs, hkv, hd = _cache(cache)
-    if k.dim() != 4 or k.shape[2] != hkv or k.shape[3] != hd or v.shape != k.shape or v.dtype != k.dtype:
-        raise ValueError(f"k and v must be [B, T, {hkv}, {hd}] of one dtype, got {list(k.shape)} and {list(v.shape)}")
-    b, t = k.shape[0], k.shape[1]
-    k, v = _rows(k, "k", dev), _rows(v, "v", dev)
+    shape = k.shape
+    if len(shape) != 4 or shape[2] != hkv or shape[3] != hd or v.shape != shape or v.dtype != k.dtype:
+        raise ValueError(f"k and v must be [B, T, {hkv}, {hd}] of one dtype, got {list(shape)} and {list(v.shape)}")
+    b, t = shape[0], shape[1]
+    k, k_at = _rows(k, "k", dev)
+    v, v_at = _rows(v, "v", dev)
     tab, cols = _tables(block_tables, b, dev)
     launch("ssd_kv8_append", dev, pages, scales, nl, nb, bs, hkv, hd, layer, tab, cols,
-           ints(seq_lens, (b,), "seq_lens", dev), ints(q_lens, (b,), "q_lens", dev), k.data_ptr(), v.data_ptr(),
+           ints(seq_lens, (b,), "seq_lens", dev), ints(q_lens, (b,), "q_lens", dev), k_at, v_at,
            dtype_code(k.dtype), b, t)
     return cache
 
@@ -148,14 +159,14 @@ def rope_append_kv8(qkv: torch.Tensor, cache: KV8CacheState, layer: int, block_t
         if (tab.dtype is not torch.float32 or tab.get_device() != dev or tab.shape != (max_pos, hd // 2)
                 or not tab.is_contiguous()):
             raise ValueError(f"{name} must be a contiguous fp32 tensor [positions, {hd // 2}] on cuda:{dev}")
-    qkv = _rows(qkv, "qkv", dev)
+    qkv, at = _rows(qkv, "qkv", dev)
     if out is None:
-        out = torch.empty((b, t, num_heads, hd), dtype=qkv.dtype, device=qkv.device)
+        out = qkv.new_empty((b, t, num_heads, hd))
     elif (out.shape != (b, t, num_heads, hd) or out.dtype != qkv.dtype or out.get_device() != dev
           or not out.is_contiguous()):
         raise ValueError(f"out must be a contiguous {qkv.dtype} tensor [{b}, {t}, {num_heads}, {hd}] on cuda:{dev}")
     tab, cols = _tables(block_tables, b, dev)
-    launch("ssd_kv8_rope_append", dev, qkv.data_ptr(), out.data_ptr(), pages, scales, dtype_code(qkv.dtype), nl, nb,
+    launch("ssd_kv8_rope_append", dev, at, out.data_ptr(), pages, scales, dtype_code(qkv.dtype), nl, nb,
            bs, num_heads, hkv, hd, layer, tab, cols, ints(seq_lens, (b,), "seq_lens", dev),
            ints(q_lens, (b,), "q_lens", dev), rope_cos.data_ptr(), rope_sin.data_ptr(), max_pos, b, t)
     return out
@@ -168,8 +179,7 @@ def gather_kv8(cache: KV8CacheState, layer: int, block_tables: torch.Tensor, pos
     if positions.dim() != 2:
         raise ValueError(f"positions must be [B, N], got {list(positions.shape)}")
     b, n = positions.shape
-    kv = torch.empty((2, b, n, hkv, hd), dtype=dtype, device=cache.pages.device)
-    k, v = kv.unbind(0)
+    k, v = cache.scales.new_empty((2, b, n, hkv, hd), dtype=dtype).unbind(0)
     tab, cols = _tables(block_tables, b, dev)
     launch("ssd_kv8_gather", dev, pages, scales, nl, nb, bs, hkv, hd, layer, tab, cols,
            ints(positions, (b, n), "positions", dev), k.data_ptr(), v.data_ptr(), dtype_code(dtype), b, n)
@@ -187,10 +197,11 @@ def paged_kv8_attention(q: torch.Tensor, cache: KV8CacheState, layer: int, block
     stand beside it.
     """
     dev, pages, scales, nl, nb, bs, hkv, hd = _cache(cache)
-    if q.dim() != 4 or q.shape[3] != hd:
-        raise ValueError(f"q must be [B, T, Hq, {hd}], got {list(q.shape)}")
-    b, t, hq, _ = q.shape
-    q = _rows(q, "q", dev)
+    shape = q.shape
+    if len(shape) != 4 or shape[3] != hd:
+        raise ValueError(f"q must be [B, T, Hq, {hd}], got {list(shape)}")
+    b, t, hq, _ = shape
+    q, at = _rows(q, "q", dev)
     tab, cols = _tables(block_tables, b, dev)
     max_seq_len = cols * bs if max_seq_len is None else int(max_seq_len)
     if out is None:
@@ -198,9 +209,9 @@ def paged_kv8_attention(q: torch.Tensor, cache: KV8CacheState, layer: int, block
     elif out.shape != q.shape or out.dtype != q.dtype or out.get_device() != dev or not out.is_contiguous():
         raise ValueError(f"out must be a contiguous {q.dtype} tensor {list(q.shape)} on cuda:{dev}")
     # a workspace of its own for every call: calls on other streams or in captured graphs share nothing
-    ws = torch.empty(lib().ssd_kv8_attention_workspace_size(b, t, hq, hkv, hd, max_seq_len), dtype=torch.uint8,
-                     device=q.device)
-    launch("ssd_kv8_attention", dev, q.data_ptr(), pages, scales, dtype_code(q.dtype), nl, nb, bs, hkv, hd, layer, tab,
+    need = lib().ssd_kv8_attention_workspace_size(b, t, hq, hkv, hd, max_seq_len)
+    ws = q.new_empty((need,), dtype=torch.uint8)
+    launch("ssd_kv8_attention", dev, at, pages, scales, dtype_code(q.dtype), nl, nb, bs, hkv, hd, layer, tab,
            cols, ints(seq_lens, (b,), "seq_lens", dev), ints(q_lens, (b,), "q_lens", dev), out.data_ptr(),
-           hd ** -0.5 if scale is None else float(scale), b, t, hq, max_seq_len, ws.data_ptr(), ws.numel())
+           hd ** -0.5 if scale is None else float(scale), b, t, hq, max_seq_len, ws.data_ptr(), need)
     return out

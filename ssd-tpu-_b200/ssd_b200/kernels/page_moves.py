@@ -10,7 +10,7 @@ from dataclasses import dataclass
 
 import torch
 
-from .kv8_cache import ints, launch
+from .kv8_cache import KV8CacheState, ints, launch
 
 _MAX_PAGE = 1 << 31  # bytes of a page in one plane (``ssd_page_copy``)
 
@@ -19,15 +19,14 @@ def _pool(cache) -> tuple:
     """(device, pages, scales or None: pointers, blocks, planes, bytes of a page in one plane, scales of a page, rest)."""
     p = cache.pages
     shape = p.shape
-    if len(shape) != 6 or not p.is_contiguous():
+    if len(shape) != 6 or shape[0] != 2 or not p.is_contiguous():
         raise ValueError("a cache's pages are a contiguous tensor [2, L, NB, BS, Hkv, D]")
-    s = getattr(cache, "scales", None)
-    if s is not None and (s.dtype is not torch.float32 or s.shape != (*shape[:3], shape[4]) or s.device != p.device
-                          or not s.is_contiguous()):
-        raise ValueError(f"scales do not fit pages {tuple(shape)}")
-    return (p.get_device(), p.data_ptr(), None if s is None else s.data_ptr(), shape[2], 2 * shape[1],
-            shape[3] * shape[4] * shape[5] * p.element_size(), 0 if s is None else shape[4],
-            (p.dtype, shape[3], shape[4], shape[5]))
+    _, nl, nb, bs, hkv, hd = shape
+    kv8 = isinstance(cache, KV8CacheState)  # its scales fit: it has looked
+    if not kv8 and p.dtype is torch.float8_e4m3fn:
+        raise ValueError("8-bit pages move as a KV8CacheState: they mean nothing without the scales")
+    return (p.get_device(), p.data_ptr(), cache.scales.data_ptr() if kv8 else None, nb, 2 * nl,
+            bs * hkv * hd * p.element_size(), hkv if kv8 else 0, (p.dtype, bs, hkv, hd))
 
 
 def _copy(src: tuple, dst: tuple, src_ids: int, src_step: int, dst_ids: int, dst_step: int, n: int,
@@ -92,14 +91,16 @@ def compact_pages(cache, tables: torch.Tensor, lens: torch.Tensor, ref_counts: t
         raise ValueError(f"a page of one plane may hold {_MAX_PAGE} bytes at most")
     if (draft_tables is None) != (draft_lens is None):
         raise ValueError("draft_tables and draft_lens go together")
+    if free_list.dtype is not torch.int32:
+        raise ValueError(f"free_list must be int32, got {free_list.dtype}")
     if tables.dim() != 2 or (draft_tables is not None and draft_tables.dim() != 2):
         raise ValueError("tables are [rows, max_blocks]")
     if inplace and draft_tables is not None and draft_tables.data_ptr() == tables.data_ptr() and tables.numel():
         raise ValueError("tables and draft_tables are the same memory: in place, they would be mapped twice")
     half = max(1, nb // 2)
-    remap = torch.empty(nb, dtype=torch.int32, device=tables.device)
-    plan = torch.empty(2 * half + 1, dtype=torch.int32, device=tables.device)  # the moves' sources, targets, number
-    src = plan.data_ptr()
+    work = free_list.new_empty((nb + 2 * half + 1,))  # new ids; the moves' sources, targets, number
+    remap = work[:nb]
+    src = work.data_ptr() + 4 * nb
     dst, count = src + 4 * half, src + 8 * half
     if inplace:
         out = Compaction(tables, ref_counts, free_list, free_top, remap, draft_tables)

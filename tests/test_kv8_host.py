@@ -137,3 +137,15 @@ def test_sizes_past_the_kernels_integers_are_refused():
     assert attn(nb=1, bs=(1 << 20) + 1) == 4
     assert so.ssd_kv8_attention_workspace_size(1, 1, 4, 2, 64, big + 1) == 0
     assert so.ssd_kv8_append(None, P, P, 1, 1, (1 << 20) + 1, 2, 64, 0, P, 4, P, None, P, P, 0, 1, 1) == 4
+
+
+def test_pages_in_8_bits_do_not_move_without_their_scales():
+    from types import SimpleNamespace
+
+    from ssd_b200.kernels.kv8_cache import KV8CacheState
+    from ssd_b200.kernels.page_moves import copy_pages
+
+    cache = KV8CacheState.allocate(1, 4, 16, 2, 64, device="cpu")
+    ids = torch.zeros(1, dtype=torch.int32)
+    with pytest.raises(ValueError, match="scales"):
+        copy_pages(SimpleNamespace(pages=cache.pages, block_size=16), ids, ids)
