@@ -230,21 +230,23 @@ int launch_join(cudaStream_t st, const Kv8Attn& a, int B) {
 }
 
 // ------------------------------------------------------------------ CUDA-core kernel (fp32 models)
-// fp32 queries keep fp32 products.  A CTA takes 8 query rows and 128 positions: a thread scores one position
+// fp32 queries keep fp32 products.  A CTA takes 8 query rows and 256 positions: a thread scores one position
 // against all rows (Q broadcast from shared memory, no reduction across lanes), the rows' maxima and sums are
 // taken over the CTA, and for P V a thread holds 4 dims of all rows over every PG-th position.  Used by the fp32
 // (toy) models, whose forward takes at most 16 rows: bound by latency, not by bytes (two sequences of 77 and 200
-// positions, 20 rows of 64 dims: 13.9 us with the join).
+// positions, 20 rows of 64 dims: 10.3 us; with 128 positions a CTA, hence a join, 13.9).
 constexpr int kCcRows = 8;
-constexpr int kCcSplit = 128;
+constexpr int kCcSplit = 256;
+constexpr int kCcWarps = kCcSplit / 32;
 
 template <int D>
 __global__ void __launch_bounds__(kCcSplit) kv8_attention_cc_kernel(const Kv8Attn a) {
   constexpr int DG = D / 4, PG = kCcSplit / DG;
-  __shared__ float4 q_s[D][2];                 // dim d of rows 0-3 and 4-7
   __shared__ float4 p_s[kCcSplit][2];          // weights of position j
-  __shared__ float o_s[PG][kCcRows][D];
-  __shared__ float red[2][4][kCcRows];
+  __shared__ __align__(16) float o_s[PG][kCcRows][D];
+  __shared__ float red[2][kCcWarps][kCcRows];
+  static_assert(sizeof(o_s) >= sizeof(float4) * 2 * D);
+  float4(*q_s)[2] = reinterpret_cast<float4(*)[2]>(o_s);  // dim d of rows 0-3 and 4-7, until the scores are done
   __shared__ int pos_s[kCcRows];
   __shared__ int64_t v_s[kCcSplit];            // byte offset of a position's V row (-1: none)
   __shared__ float vs_s[kCcSplit];
@@ -323,7 +325,9 @@ __global__ void __launch_bounds__(kCcSplit) kv8_attention_cc_kernel(const Kv8Att
   float p[kCcRows];
 #pragma unroll
   for (int r = 0; r < kCcRows; ++r) {
-    m[r] = fmaxf(fmaxf(red[0][0][r], red[0][1][r]), fmaxf(red[0][2][r], red[0][3][r]));
+    m[r] = red[0][0][r];
+#pragma unroll
+    for (int w = 1; w < kCcWarps; ++w) m[r] = fmaxf(m[r], red[0][w][r]);
     p[r] = there && j <= pos_s[r] ? expf(s[r] - m[r]) : 0.f;
     const float x = warp_sum(p[r]);
     if (lane == 0) red[1][warp][r] = x;
@@ -374,7 +378,12 @@ __global__ void __launch_bounds__(kCcSplit) kv8_attention_cc_kernel(const Kv8Att
     float O = 0.f;
 #pragma unroll
     for (int x = 0; x < PG; ++x) O += o_s[x][r][d];
-    const float L = (red[1][0][r] + red[1][1][r]) + (red[1][2][r] + red[1][3][r]);
+    float L = 0.f, M = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kCcWarps; ++w) {
+      L += red[1][w][r];
+      M = fmaxf(M, red[0][w][r]);
+    }
     const int64_t at = (grp * a.nsplit + split) * kCcRows + r;
     if (a.nsplit == 1) {
       const int gr = row0 + r, t = gr / a.G, g = gr % a.G;
@@ -382,10 +391,7 @@ __global__ void __launch_bounds__(kCcSplit) kv8_attention_cc_kernel(const Kv8Att
           pos_s[r] >= 0 && L != 0.f ? O / L : 0.f;
     } else {
       a.ws_o[at * D + d] = O;
-      if (d == 0) {
-        const float M = fmaxf(fmaxf(red[0][0][r], red[0][1][r]), fmaxf(red[0][2][r], red[0][3][r]));
-        a.ws_ml[at] = make_float4(M, M, L, 0.f);
-      }
+      if (d == 0) a.ws_ml[at] = make_float4(M, M, L, 0.f);
     }
   }
 }
