@@ -312,7 +312,9 @@ size_t ssd_kv8_attention_workspace_size(int B, int T, int num_heads, int num_kv_
  * ssd_paged_verify_attention over an 8-bit cache: same rows, positions, lengths and zero rows.
  * q and out [B, T, Hq, D] in `dtype`; scores, softmax statistics and sums in fp32.  What a row does
  * not see (positions past its own, rows behind seq_lens) does not reach it, NaN included; a row of q
- * that holds an infinity or NaN comes out as NaN.  max_seq_len <= 2^30.  The workspace is 16-byte
+ * that holds an infinity or NaN comes out as NaN.  For T <= 8 a query's bits do not depend on the
+ * tokens beside it; they may on B and max_seq_len, by which the context is split (above 8 tokens, on
+ * the sequences' lengths).  max_seq_len <= 2^30.  The workspace is 16-byte
  * aligned, needs no initial content and keeps none.
  */
 int ssd_kv8_attention(ssd_stream_t stream, const void* q, const void* pages, const float* scales, int dtype,

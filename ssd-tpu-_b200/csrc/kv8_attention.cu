@@ -1651,11 +1651,14 @@ Kv8Layout kv8_layout(bool cc, int B, int T, int hq, int hkv, int D, int max_seq_
   // against 18.7 us at 1024); where there is work for every SM either way, longer splits cost fewer prologues and
   // partials (8 sequences, 16 heads, 512 to 4096 positions: 34.5 us at 832, 38.1 at 1024, 43.2 at 256), up to 1024,
   // which leaves many sequences enough CTAs to balance.  Three CTAs an SM, half as many again since not every
-  // sequence is as long as the bound.  The rule goes by the sequences, never by the rows, so a query's bits do not
-  // depend on how many new tokens stand beside it.
+  // sequence is as long as the bound.  A bound of 512 stays in one split, which needs no join (one sequence of 500
+  // positions, 8 heads of 64: 5.9 against 7.2 us; four of 16 heads of 256: 10.5 against 13.8), but where 8 or more
+  // query heads share a KV head and a verify step has several row groups (16.1 against 13.3).  The rule goes by the
+  // sequences and the model, never by the new tokens, so a query's bits do not depend on how many stand beside it.
   const int64_t groups = (int64_t)B * hkv, n = groups >= 666 ? 1 : 666 / groups;
   const int64_t even = ((max_seq_len + n - 1) / n + 63) / 64 * 64;
-  L.split = cc ? kCcSplit : (int)(even < 256 ? 256 : even > kMaxFewSplit ? kMaxFewSplit : even);
+  const int least = max_seq_len <= 512 && hq / hkv < 8 ? 512 : 256;
+  L.split = cc ? kCcSplit : (int)(even < least ? least : even > kMaxFewSplit ? kMaxFewSplit : even);
   L.row_groups = (total + L.rows - 1) / L.rows;
   if (L.rows == many::ROWS) {
     // One CTA an SM: as many splits, over all sequences, as one wave of them takes (four sequences of 8192 positions,

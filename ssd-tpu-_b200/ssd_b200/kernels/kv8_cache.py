@@ -194,7 +194,8 @@ def paged_kv8_attention(q: torch.Tensor, cache: KV8CacheState, layer: int, block
     Arguments as ``paged_verify_attention``: seq_lens [B] counts cached tokens INCLUDING the new
     ones; new token t of sequence b sits at position seq_lens[b] - q_lens[b] + t.  Rows past
     q_lens[b] come back as zeros.  For T up to 8 a query's bits do not depend on how many new tokens
-    stand beside it.
+    stand beside it; they may differ between batch sizes and values of ``max_seq_len``, by which the
+    context is split.
     """
     dev, pages, scales, nl, nb, bs, hkv, hd = _cache(cache)
     shape = q.shape
