@@ -315,7 +315,8 @@ size_t ssd_kv8_attention_workspace_size(int B, int T, int num_heads, int num_kv_
  * that holds an infinity or NaN comes out as NaN.  For T <= 8 a query's bits do not depend on the
  * tokens beside it; they may on B and max_seq_len, by which the context is split (above 8 tokens, on
  * the sequences' lengths).  max_seq_len <= 2^30.  The workspace is 16-byte
- * aligned, needs no initial content and keeps none.
+ * aligned, needs no initial content and keeps none; its size is 0, and it may be NULL, where no context
+ * is split.
  */
 int ssd_kv8_attention(ssd_stream_t stream, const void* q, const void* pages, const float* scales, int dtype,
                       int num_layers, int num_blocks, int block_size, int num_kv_heads, int head_dim, int layer,

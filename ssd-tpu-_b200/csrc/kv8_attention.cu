@@ -1677,7 +1677,7 @@ Kv8Layout kv8_layout(bool cc, int B, int T, int hq, int hkv, int D, int max_seq_
   }
   L.off_ml = up256(sizeof(float) * L.partials * D);
   L.off_plan = L.off_ml + up256(sizeof(float4) * L.partials);
-  L.total = L.off_plan + up256(L.planned ? sizeof(int2) * B : 1);
+  L.total = L.partials ? L.off_plan + up256(sizeof(int2) * B) : 0;
   return L;
 }
 
@@ -1743,13 +1743,14 @@ extern "C" int ssd_kv8_attention(ssd_stream_t stream, const void* q, const void*
     return SSD_ERR_INVALID;
   if (B == 0 || T == 0) return SSD_OK;
   if (!q || !out || (int64_t)max_blocks * block_size < max_seq_len) return SSD_ERR_INVALID;
-  if (!kv8_aligned(q) || !kv8_aligned(out) || !kv8_aligned(workspace) ||
+  if (!kv8_aligned(q) || !kv8_aligned(out) ||
       (int64_t)max_blocks * block_size > 0x7fffffff || max_seq_len > kMaxSeqLen)
     return SSD_ERR_UNSUPPORTED;
   const Kv8Layout L = kv8_layout(dtype == SSD_DTYPE_F32, B, T, num_heads, num_kv_heads, head_dim, max_seq_len);
   if (B > 65535 || L.row_groups > 65535 || num_kv_heads * L.row_groups > 65535)
     return SSD_ERR_UNSUPPORTED;
-  if (!workspace || workspace_bytes < L.total) return SSD_ERR_WORKSPACE;
+  if (L.total && (!workspace || workspace_bytes < L.total)) return SSD_ERR_WORKSPACE;
+  if (L.total && !kv8_aligned(workspace)) return SSD_ERR_UNSUPPORTED;
   char* w = reinterpret_cast<char*>(workspace);
   Kv8Attn a{};
   a.c = kv8_cache(const_cast<void*>(pages), const_cast<float*>(scales), num_layers, num_blocks, block_size,

@@ -17,6 +17,7 @@ the cache's device and keeps nothing of its arguments.
 from __future__ import annotations
 
 from dataclasses import dataclass, field
+from functools import lru_cache
 
 import torch
 
@@ -35,10 +36,11 @@ class KV8CacheState:
 
     def __post_init__(self) -> None:
         p, s = self.pages, self.scales
-        if (p.dtype != torch.float8_e4m3fn or s.dtype != torch.float32 or p.dim() != 6 or not p.is_contiguous()
-                or not s.is_contiguous() or s.device != p.device):
+        shape = p.shape
+        if (p.dtype is not torch.float8_e4m3fn or s.dtype is not torch.float32 or len(shape) != 6
+                or not p.is_contiguous() or not s.is_contiguous() or s.get_device() != p.get_device()):
             raise ValueError("an 8-bit cache is contiguous e4m3 pages [2, L, NB, BS, Hkv, D] and fp32 scales on one GPU")
-        two, nl, nb, bs, hkv, hd = p.shape
+        two, nl, nb, bs, hkv, hd = shape
         if two != 2 or bs != self.block_size or s.shape != (2, nl, nb, hkv):
             raise ValueError(f"scales {tuple(s.shape)} and block_size {self.block_size} do not fit pages {tuple(p.shape)}")
         object.__setattr__(self, "dims", (nl, nb, bs, hkv, hd))
@@ -186,6 +188,11 @@ def gather_kv8(cache: KV8CacheState, layer: int, block_tables: torch.Tensor, pos
     return k, v
 
 
+@lru_cache(maxsize=1024)  # a function of these sizes alone
+def _workspace_size(b: int, t: int, hq: int, hkv: int, hd: int, max_seq_len: int) -> int:
+    return lib().ssd_kv8_attention_workspace_size(b, t, hq, hkv, hd, max_seq_len)
+
+
 def paged_kv8_attention(q: torch.Tensor, cache: KV8CacheState, layer: int, block_tables: torch.Tensor,
                         seq_lens: torch.Tensor, q_lens: torch.Tensor | None = None, scale: float | None = None,
                         max_seq_len: int | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
@@ -210,9 +217,9 @@ def paged_kv8_attention(q: torch.Tensor, cache: KV8CacheState, layer: int, block
     elif out.shape != q.shape or out.dtype != q.dtype or out.get_device() != dev or not out.is_contiguous():
         raise ValueError(f"out must be a contiguous {q.dtype} tensor {list(q.shape)} on cuda:{dev}")
     # a workspace of its own for every call: calls on other streams or in captured graphs share nothing
-    need = lib().ssd_kv8_attention_workspace_size(b, t, hq, hkv, hd, max_seq_len)
-    ws = q.new_empty((need,), dtype=torch.uint8)
+    need = _workspace_size(b, t, hq, hkv, hd, max_seq_len)
+    ws = q.new_empty((need,), dtype=torch.uint8) if need else None
     launch("ssd_kv8_attention", dev, at, pages, scales, dtype_code(q.dtype), nl, nb, bs, hkv, hd, layer, tab,
            cols, ints(seq_lens, (b,), "seq_lens", dev), ints(q_lens, (b,), "q_lens", dev), out.data_ptr(),
-           hd ** -0.5 if scale is None else float(scale), b, t, hq, max_seq_len, ws.data_ptr(), need)
+           hd ** -0.5 if scale is None else float(scale), b, t, hq, max_seq_len, None if ws is None else ws.data_ptr(), need)
     return out

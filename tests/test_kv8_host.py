@@ -72,8 +72,8 @@ def test_c_abi_refusals():
     assert gather(pos=None) == gather(k=None) == gather(dt=7) == gather(n=-1) == 1
     assert gather(d=48) == gather(k=P + 2) == 4
 
-    def attn(q=P, out=P, hq=4, hkv=2, d=64, sl=P, b=1, t=1, mx=64, ws=P, nbytes=1 << 40, dt=0):
-        return so.ssd_kv8_attention(None, q, P, P, dt, 2, 8, 16, hkv, d, 0, P, 4, sl, None, out, 0.1, b, t, hq, mx, ws,
+    def attn(q=P, out=P, hq=4, hkv=2, d=64, sl=P, b=1, t=1, mx=64, ws=P, nbytes=1 << 40, dt=0, mb=4):
+        return so.ssd_kv8_attention(None, q, P, P, dt, 2, 8, 16, hkv, d, 0, P, mb, sl, None, out, 0.1, b, t, hq, mx, ws,
                                     nbytes)
 
     assert attn(b=0) == 0
@@ -81,9 +81,10 @@ def test_c_abi_refusals():
                 dict(t=-1)):
         assert attn(**bad) == 1, bad
     assert attn(d=80) == attn(q=P + 2) == attn(b=70000) == 4
-    assert attn(ws=None) == attn(nbytes=0) == 5
-    assert so.ssd_kv8_attention_workspace_size(1, 5, 4, 3, 64, 64) == 0
-    assert so.ssd_kv8_attention_workspace_size(1, 5, 4, 2, 64, 64) > 0
+    assert attn(mb=63, mx=1000, ws=None) == attn(mb=63, mx=1000, nbytes=0) == 5  # split contexts
+    assert so.ssd_kv8_attention_workspace_size(1, 5, 4, 3, 64, 1000) == 0
+    assert so.ssd_kv8_attention_workspace_size(1, 5, 4, 2, 64, 1000) > 0
+    assert so.ssd_kv8_attention_workspace_size(1, 5, 4, 2, 64, 64) == 0  # one split: nothing to join
 
     def copy(src=P, ss=None, dst=P, ds=None, planes=4, nbytes=64, sc=0, sid=P, st=1, did=P, n=1):
         return so.ssd_page_copy(None, src, ss, 8, dst, ds, 8, planes, nbytes, sc, sid, st, did, 1, n, None)
@@ -133,7 +134,7 @@ def test_sizes_past_the_kernels_integers_are_refused():
 
     assert attn(t=big, hq=1 << 20, hkv=1) == 4          # more row groups than a grid has
     assert attn(mb=(1 << 31) - 1, bs=1, mx=big + 1) == 4
-    assert attn(ws=P + 8) == 4
+    assert attn(mb=63, mx=1000, ws=P + 8) == 4
     assert attn(nb=1, bs=(1 << 20) + 1) == 4
     assert so.ssd_kv8_attention_workspace_size(1, 1, 4, 2, 64, big + 1) == 0
     assert so.ssd_kv8_append(None, P, P, 1, 1, (1 << 20) + 1, 2, 64, 0, P, 4, P, None, P, P, 0, 1, 1) == 4
