@@ -548,14 +548,26 @@ __global__ void __launch_bounds__(kFewWarps * 32, NT == 1 ? 3 : 2) kv8_attention
       const int i0 = (warp + k * kFewWarps) * 16;
       const uint32_t st = ring + (k % S::STAGES) * (2 * S::TILE);
       constexpr int RPI = 32 / PCS;  // rows an instruction covers
+      if constexpr (UNI) {
+        // one product a tile: its rows lie rs apart, and past the sequence's end they are in the page all the same
+        const uint8_t* src = kp + (int64_t)(max(first_l, 0) + lane / PCS) * rs;
+        const int left = first_l < 0 ? 0 : kn - i0 - lane / PCS;  // row x RPI of the lane is there where it is below
 #pragma unroll
-      for (int x = 0; x < 16 / RPI; ++x) {
-        const int r = x * RPI + lane / PCS;
-        const int first = UNI ? first_l : row_s[i0 + r];
-        const bool there = first >= 0 && (!UNI || i0 + r < kn);
-        const uint8_t* src = kp + (there ? first + (UNI ? r : 0) : 0) * rs;
-        cp_async16(st + k_piece(r, lane % PCS) * 16, src, there);
-        cp_async16(st + S::TILE + v_piece(r, lane % PCS) * 16, src + a.c.plane, there);
+        for (int x = 0; x < 16 / RPI; ++x) {
+          const int r = x * RPI + lane / PCS;
+          cp_async16(st + k_piece(r, lane % PCS) * 16, src, x * RPI < left);
+          cp_async16(st + S::TILE + v_piece(r, lane % PCS) * 16, src + a.c.plane, x * RPI < left);
+          src += RPI * rs;
+        }
+      } else {
+#pragma unroll
+        for (int x = 0; x < 16 / RPI; ++x) {
+          const int r = x * RPI + lane / PCS;
+          const int first = row_s[i0 + r];
+          const uint8_t* src = kp + max(first, 0) * rs;
+          cp_async16(st + k_piece(r, lane % PCS) * 16, src, first >= 0);
+          cp_async16(st + S::TILE + v_piece(r, lane % PCS) * 16, src + a.c.plane, first >= 0);
+        }
       }
     }
     cp_async_commit();
