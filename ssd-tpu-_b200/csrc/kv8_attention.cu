@@ -6,8 +6,9 @@
 //   s_j = scale * 2^a(j) * (q_r . k_j),   out_r = sum_j e^(s_j - M) 2^c(j) v_j / sum_j e^(s_j - M).
 // Rows past q_lens[b] and rows that see no position are zeros.
 //
-// A CTA owns one KV head of one sequence, a fixed slice of its positions (a split) and a group of query rows
-// (G query heads times the new tokens), so a query's result does not depend on how many rows stand beside it.
+// A CTA owns one KV head of one sequence, a slice of its positions (a split) and a group of query rows (G query heads
+// times the new tokens).  Up to kFewTokens new tokens the slices are fixed, so a query's result does not depend on how
+// many tokens stand beside it.
 // Splits leave unnormalised partials, which a second kernel joins in split order.  It needs no counters, so a
 // workspace holds nothing between calls and may come uninitialised from any allocator.  Times below are of both
 // kernels, from replayed graphs, on a GPU that copies 6.5 TB/s.
