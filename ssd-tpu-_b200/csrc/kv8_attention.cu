@@ -413,9 +413,12 @@ __global__ void __launch_bounds__(kCcSplit) kv8_attention_cc_kernel(const Kv8Att
 //   P: the S^T accumulators, rounded to f16 pairs and transposed by movmatrix, are the B operand.
 // e4m3 converts to f16 exactly.  q is scaled per row by a power of two into f16's range, which keeps bf16's
 // eight bits (elements below 2^-14 of the row's largest lose the last ones).  V's page scales join the
-// weights' exponents: with M >= max_j (s_j + c_j) - 8 (log2) every weight 2^(s_j + c_j - M) is at most 2^8 and
-// keeps f16's 11 bits relative to the largest contribution, whatever the pages' scales.
+// weights' exponents: the reference M is put kBelow = 7 (log2) below the largest s_j + c_j seen, and moves when one
+// passes it by kSpan = 15, so a weight 2^(s_j + c_j - M) is at most 2^15 (f16 holds nearly 2^16) and the largest is at
+// least 2^7: weights keep f16's 11 bits down to 2^-21 of the largest and are off by 2^-32 of it below, whatever the
+// pages' scales.
 constexpr int kFewWarps = 4;
+constexpr float kBelow = 7.f, kSpan = 15.f;
 
 __device__ __forceinline__ void mma_f16(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                         uint32_t b1) {
@@ -718,9 +721,10 @@ __global__ void __launch_bounds__(kFewWarps * 32, NT == 1 ? 3 : 2) kv8_attention
           n = fmaxf(n, __shfl_xor_sync(0xffffffffu, n, x));
         }
         if constexpr (UNI) m = n + e0;
-        // the reference moves only when a weight would pass 2^8 (f16 holds 2^15): most tiles rescale nothing
+        // most tiles move no reference and rescale nothing
         f[nt][e] = 1.f;
-        if (m > M[nt][e] + 8.f) {
+        if (m > M[nt][e] + kSpan) {
+          m -= kBelow;
           f[nt][e] = ex2(M[nt][e] - m);
           M[nt][e] = m;
           moved = true;
@@ -1304,7 +1308,8 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_many_kernel(const Kv
       if (!ok) break;
       m = fmaxf(m, mo);
       n = fmaxf(n, no);
-      if (m > M + 8.f) {
+      if (m > M + kSpan) {
+        m -= kBelow;
         f = ex2(M - m);
         M = m;
       }

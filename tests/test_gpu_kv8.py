@@ -583,3 +583,33 @@ def test_page_sizes_beside_the_tiles(cuda, case):
     ref, mass, size = o.attention(q, p.vals, p.exps, p.tables, lens, ql, 1 / math.sqrt(d))
     err, tol = np.abs(got.float().cpu().numpy() - ref), _tolerance(case, q, p, lens, mass, size, ref)
     assert (err <= tol).all(), (err / np.maximum(tol, 1e-300)).max()
+
+
+@pytest.mark.parametrize("hq,hkv,d,t", [(8, 1, 256, 3), (8, 1, 256, 40), (4, 2, 64, 3), (4, 2, 64, 40)])
+def test_small_weights_on_large_values(cuda, hq, hkv, d, t):
+    """The position that takes nearly all of the softmax holds V values far below its page's scale, so that positions
+    of weight 2^-20 count as much: their weights must not be rounded to a few bits.
+
+    Scores are exact products (one dimension), so ds is the exponential's own: at most 4 roundings of arguments below
+    32, and 2^-22, ds <= 2^-16.  Weights: 2^-11 relative, and 2^-32 of the largest below 2^-21 of it.  n sums in fp32."""
+    from ssd_b200.kernels.kv8_cache import paged_kv8_attention
+
+    torch, _ = _torch()
+    rng = np.random.default_rng(d + t)
+    n = 64 + t
+    p = Pool(rng, 1, 16, hkv, d, cols=-(-n // 16))
+    k = np.zeros((1, n, hkv, d))
+    k[..., 0] = np.exp2(rng.integers(-6, -2, (1, n, hkv)))  # scores 16 * that, small
+    k[0, 5, :, 0] = 1.0
+    v = rng.uniform(-448, 448, (1, n, hkv, d))
+    v[0, ::16, :, 0] = 448                                  # every page's scale is 1
+    v[0, 5] = rng.integers(-7, 8, (hkv, d)) * 2.0 ** -9
+    p.append([n], k, v, [n], "bf16")
+    q = np.zeros((1, t, hq, d))
+    q[..., 0] = 16.0
+    i = lambda a: torch.tensor(np.asarray(a, np.int32), device="cuda")  # noqa: E731
+    got = paged_kv8_attention(torch.tensor(q).bfloat16().cuda(), p.cache, 1, p.dev_tables, i([n]), scale=1.0)
+    ref, mass, _ = o.attention(q, p.vals, p.exps, p.tables, [n], [t], 1.0)
+    tol = EPS["bf16"] * np.abs(ref) + (2.0 ** -11 + 4 * 2.0 ** -16 + n * 2.0 ** -24) * mass + n * 2.0 ** -32 * 448
+    err = np.abs(got.float().cpu().numpy() - ref)
+    assert (err <= tol).all(), (err / tol).max()
