@@ -411,8 +411,8 @@ __global__ void __launch_bounds__(kCcSplit) kv8_attention_cc_kernel(const Kv8Att
 //   V: positions 2t, 2t+1, 2t+8, 2t+9, dims 128 h + 16 g .. + 15 (D = 64: 8 g .. + 7); byte pairs of two
 //      positions become the A operand, m-tile i carrying dims 2i and 2i + 1 of each lane.
 //   P: the S^T accumulators, rounded to f16 pairs and transposed by movmatrix, are the B operand.
-// e4m3 converts to f16 exactly.  q is scaled per row by a power of two into f16's range, which keeps bf16's
-// eight bits (elements below 2^-14 of the row's largest lose the last ones).  V's page scales join the
+// e4m3 converts to f16 exactly.  q is scaled per row by a power of two, its largest into [2^14, 2^15), which keeps
+// bf16's eight bits (elements below 2^-28 of the row's largest lose the last ones).  V's page scales join the
 // weights' exponents: the reference M is put kBelow = 7 (log2) below the largest s_j + c_j seen, and moves when one
 // passes it by kSpan = 15, so a weight 2^(s_j + c_j - M) is at most 2^15 (f16 holds nearly 2^16) and the largest is at
 // least 2^7: weights keep f16's 11 bits down to 2^-21 of the largest and are off by 2^-32 of it below, whatever the
@@ -598,7 +598,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, NT == 1 ? 3 : 2) kv8_attention
     }
 #pragma unroll
     for (int x = 1; x < 16; x <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, x));
-    const int e = min(max((int)(__float_as_uint(amax) >> 23) - 127, -118), 120);
+    const int e = min(max((int)(__float_as_uint(amax) >> 23) - 127 - 14, -118), 120);
     const float inv = exp2i(-e);
     // an infinity in q leaves no finite score, or one less itself: NaN
     if ((lane & 15) == 0)
@@ -1218,11 +1218,10 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_many_kernel(const Kv
       float top = fmaxf(__low2float(t2), __high2float(t2)), other = top, unused = 0.f;
       ok = ok && swap(pair_s, 0, other, unused);
       top = fmaxf(top, other);
-      const int e = min(max((int)(__float_as_uint(top) >> 23) - 127, -118), 120);
+      const int e = min(max((int)(__float_as_uint(top) >> 23) - 127 - 14, -118), 120);
       const float inv = copysignf(exp2i(-e), a.scale);  // the row's factor is never negative
       qs = exp2i(e) * fabsf(a.scale) * 1.4426950408889634f;
       if (top == INFINITY) qs = __int_as_float(0x7fc00000);  // such a row has no finite score, or one less itself
-      if (qs == 0.f) qs = 1e-38f;  // keeps the mask's infinity out of 0 * infinity; the scores stay below 2^-60
 #pragma unroll
       for (int c = 0; c < NQ; c += 4) {
         uint32_t y[16];
@@ -1262,6 +1261,9 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_many_kernel(const Kv
         if (!inb) wb = pack_meta(0, 0);
         ca = qs * exp2i(meta_k(wa));
         cb = qs * exp2i(meta_k(wb));
+        // keeps the mask's infinity out of 0 * infinity (the scores stay below 2^-90): all-zero pages, zero rows
+        if (ca == 0.f) ca = 1e-38f;
+        if (cb == 0.f) cb = 1e-38f;
         va = meta_v(wa);
         vb2 = meta_v(wb);
         // Weights' sums can be carried over to l's reference unless a page's V scale is far below the largest so

@@ -613,3 +613,53 @@ def test_small_weights_on_large_values(cuda, hq, hkv, d, t):
     tol = EPS["bf16"] * np.abs(ref) + (2.0 ** -11 + 4 * 2.0 ** -16 + n * 2.0 ** -24) * mass + n * 2.0 ** -32 * 448
     err = np.abs(got.float().cpu().numpy() - ref)
     assert (err <= tol).all(), (err / tol).max()
+
+
+@pytest.mark.parametrize("dtype,hq,hkv,d,bs,t", [("bf16", 8, 1, 256, 16, 3), ("bf16", 8, 1, 256, 16, 40),
+                                                 ("bf16", 4, 2, 64, 4, 40), ("f32", 4, 2, 64, 16, 3)])
+@pytest.mark.parametrize("qmag", [0.0, 2.0 ** -100, 2.0 ** -30, 1.0])
+def test_zero_keys_and_small_queries(cuda, dtype, hq, hkv, d, bs, t, qmag):
+    """Pages whose K is zero carry the smallest scale; with it, rows of q of any size, zero included, weigh every
+    position they see alike."""
+    from ssd_b200.kernels.kv8_cache import paged_kv8_attention
+
+    torch, dts = _torch()
+    rng = np.random.default_rng(t)
+    n = 130 + t  # ends inside a page and a tile
+    p = Pool(rng, 1, bs, hkv, d, cols=-(-n // bs))
+    v = _round(rng.standard_normal((1, n, hkv, d)), "bf16")
+    p.append([n], np.zeros((1, n, hkv, d)), v, [n], "bf16")
+    q = _round(qmag * rng.standard_normal((1, t, hq, d)), dtype)
+    i = lambda a: torch.tensor(np.asarray(a, np.int32), device="cuda")  # noqa: E731
+    got = paged_kv8_attention(torch.tensor(q).to(dts[dtype]).cuda(), p.cache, 1, p.dev_tables, i([n]))
+    ref, mass, _ = o.attention(q, p.vals, p.exps, p.tables, [n], [t], 1 / math.sqrt(d))
+    # equal weights: exact but for V's page exponents, 2^-11; n sums in fp32, the output's rounding
+    tol = EPS[dtype] * np.abs(ref) + (2.0 ** -11 + 2 * n * 2.0 ** -24) * mass
+    assert (np.abs(got.float().cpu().numpy() - ref) <= tol).all()
+
+
+@pytest.mark.parametrize("hq,hkv,d,t", [(4, 2, 64, 3), (4, 2, 64, 40), (8, 1, 256, 2), (8, 1, 256, 12)])
+def test_small_elements_beside_a_large_one_in_q(cuda, hq, hkv, d, t):
+    """One element of q lies 2^18 above the others, on a dimension where K is zero: the others decide, with all of
+    their bits."""
+    from ssd_b200.kernels.kv8_cache import paged_kv8_attention
+
+    torch, _ = _torch()
+    rng = np.random.default_rng(d * t)
+    n = 100 + t
+    p = Pool(rng, 1, 16, hkv, d, cols=-(-n // 16))
+    k, v = 16 * rng.standard_normal((1, n, hkv, d)), rng.standard_normal((1, n, hkv, d))
+    k[..., 0] = 0
+    p.append([n], k, v, [n], "bf16")
+    q = 2.0 ** -5 * rng.standard_normal((1, t, hq, d))
+    q[..., 0] = 8192
+    q = _round(q, "bf16")
+    i = lambda a: torch.tensor(np.asarray(a, np.int32), device="cuda")  # noqa: E731
+    scale = 8 / d ** 0.5
+    got = paged_kv8_attention(torch.tensor(q).bfloat16().cuda(), p.cache, 1, p.dev_tables, i([n]), scale=scale)
+    ref, mass, size = o.attention(q, p.vals, p.exps, p.tables, [n], [t], scale)
+    # scores: products exact in f16, d sums in fp32, the exponential; weights' 2^-11 and n sums; the output's half step
+    ds = ((d + 8) * 2.0 ** -24 + 2.0 ** -22) * size + 2.0 ** -21
+    tol = EPS["bf16"] * np.abs(ref) + (4 * ds + 2.0 ** -11 + n * 2.0 ** -24) * mass
+    err = np.abs(got.float().cpu().numpy() - ref)
+    assert (err <= tol).all(), (err / tol).max()
