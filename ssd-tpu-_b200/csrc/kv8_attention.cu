@@ -1239,7 +1239,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_many_kernel(const Kv
       if (ok) tc::mbar_arrive(q_tmem);
     }
     // M: what the weights are relative to, N: what l is; -1e38 where nothing has been seen
-    float M = -1e38f, N = -1e38f, l = 0.f, vtop = -1000.f;
+    float M = -1e38f, N = -1e38f, l = 0.f;
 #pragma unroll 1
     for (int j = 0; ok && j < tiles; ++j) {
       ok = __all_sync(0xffffffffu, wait(s_full(j & 1), (j >> 1) & 1, stop));
@@ -1252,7 +1252,6 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_many_kernel(const Kv
       float m = -1e38f, n = -1e38f, f = 1.f;
       // a NaN score counts as the lowest value in the maxima and spoils the sums
       float ca = 0.f, cb = 0.f, va = 0.f, vb2 = 0.f;
-      bool wide = false;
       if constexpr (UNI) {
         // two groups of 16 positions, one pair of scales each
         uint32_t wa = mt[0], wb = mt[1];
@@ -1266,10 +1265,6 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_many_kernel(const Kv
         if (cb == 0.f) cb = 1e-38f;
         va = meta_v(wa);
         vb2 = meta_v(wb);
-        // Weights' sums can be carried over to l's reference unless a page's V scale is far below the largest so
-        // far (the weights could vanish); then l takes its own exponentials.
-        vtop = fmaxf(vtop, fmaxf(va, vb2));
-        wide = fminf(va, vb2) < vtop - 40.f;
         tmem_ready(x);
         if (p0 + 31 > kmin || p0 + 32 > base + kn || !ina || !inb) {  // hide what the row does not see
           const int k = min(pos, base + kn - 1) - p0;
@@ -1321,6 +1316,11 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_many_kernel(const Kv
       }
       uint32_t w[16];
       if constexpr (UNI) {
+        // Weights are 2^(s + v - M), l's terms 2^(s - N): a group's sum of weights is carried over by 2^(M - v - N).
+        // Not where v lies more than 40 below M - N (a page of small V beside one of large V, whichever of the row's two
+        // threads has it): there weights vanish below 2^-126 that count in l, 2^-86 of its largest and up, and the
+        // factor may overflow.  Then l takes its own exponentials.
+        const bool wide = fminf(va, vb2) < M - N - 40.f;
         if (wide) {
 #pragma unroll
           for (int i = 0; i < 32; ++i) l += ex2(fmaf(__uint_as_float(x[i]), i < 16 ? ca : cb, -N));

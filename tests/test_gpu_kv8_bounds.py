@@ -1,0 +1,64 @@
+"""GPU: attention over the 8-bit cache against 64 bits, at the bounds that its arithmetic states."""
+
+from __future__ import annotations
+
+import math
+
+import numpy as np
+import pytest
+
+import kv8_reference as ref
+from test_gpu_kv8 import Pool, _round, _torch
+
+pytestmark = pytest.mark.gpu
+
+
+def _i(a):
+    import torch
+
+    return torch.tensor(np.asarray(a, np.int32), device="cuda")
+
+
+def _run(p, q, lens, ql, dtype="bf16", **kw):
+    """(output on the host, its tensor) for the numpy queries."""
+    from ssd_b200.kernels.kv8_cache import paged_kv8_attention
+
+    torch, dts = _torch()
+    out = paged_kv8_attention(torch.tensor(q).to(dts[dtype]).cuda(), p.cache, 1, p.dev_tables, _i(lens), q_lens=_i(ql),
+                              **kw)
+    return out.float().cpu().numpy(), out
+
+
+def _near(got, r, p, dtype="bf16"):
+    tol = ref.bound(r, p.exps, dtype)
+    off = np.abs(got - r["out"])
+    assert (off <= tol).all(), f"{np.nanmax(off / np.maximum(tol, 1e-300)):.3g} times the bound, {np.isnan(off).sum()} NaN"
+
+
+@pytest.mark.parametrize("hq,hkv,d,t", [(8, 1, 256, 40), (4, 4, 128, 40), (16, 4, 64, 33), (8, 2, 128, 5), (4, 1, 256, 1)])
+@pytest.mark.parametrize("kind", ["zeros, large", "large, zeros", "one large page", "tiny, large", "large, tiny"])
+@pytest.mark.parametrize("big", [18, 24, 30, 100])
+def test_v_scales_far_apart_within_a_tile(cuda, hq, hkv, d, t, kind, big):
+    """Runs of 32 positions whose V is all zero, or tiny, beside runs of |V| near 2^big: every position counts in
+    the normaliser, at 512 positions (one split) and at 1100."""
+    rng = np.random.default_rng(big)
+    lens = [512, 1100, 470]
+    ql = [t, t, max(t - 1, 1)]
+    p = Pool(rng, 3, 16, hkv, d, cols=70)
+    k = _round(rng.standard_normal((3, 1100, hkv, d)), "bf16")
+    v = rng.standard_normal((3, 1100, hkv, d))
+    run = np.arange(1100) // 32 % 2
+    first, second = {"zeros, large": (0, 2.0 ** big), "large, zeros": (2.0 ** big, 0), "tiny, large": (2.0 ** -90, 2.0 ** big),
+                     "large, tiny": (2.0 ** big, 2.0 ** -90), "one large page": (0, 0)}[kind]
+    v *= np.where(run == 0, first, second)[None, :, None, None]
+    if kind == "one large page":
+        v[:, 208:224] = 2.0 ** big * rng.standard_normal((3, 16, hkv, d))
+    p.append(lens, k, _round(v, "bf16"), lens, "bf16")
+    q = _round(rng.standard_normal((3, t, hq, d)), "bf16")
+    scale = 1 / math.sqrt(d)
+    r = ref.attention(q, p.vals, p.exps, p.tables, lens, ql, scale)
+    _near(_run(p, q, lens, ql)[0], r, p)
+    few = dict(lens=[512, 500, 470], cols=32)  # a bound of 512: one split
+    p.dev_tables = p.dev_tables[:, :few["cols"]].contiguous()
+    r = ref.attention(q, p.vals, p.exps, p.tables, few["lens"], ql, scale)
+    _near(_run(p, q, few["lens"], ql)[0], r, p)
