@@ -324,6 +324,17 @@ int ssd_kv8_attention(ssd_stream_t stream, const void* q, const void* pages, con
                       void* out, float scale, int B, int T, int num_heads, int max_seq_len, void* workspace,
                       size_t workspace_bytes);
 
+/*
+ * Above 8 tokens and 32 rows a KV head, bf16, the kernel's warps wait for one another inside a CTA, each wait
+ * for a bounded number of polls.  A CTA whose wait runs out ends with NaN in the rows that it has not finished;
+ * the call itself has long returned SSD_OK.  ssd_kv8_attention_status waits for `stream` and returns
+ * SSD_ERR_TIMEOUT if that has happened on the current device since it last said so, else SSD_OK.  Not for
+ * captured streams.  ssd_kv8_attention_set_polls sets the polls of each wait for later calls of this process
+ * (-1: the default, 2^24, some seconds).
+ */
+int ssd_kv8_attention_status(ssd_stream_t stream);
+int ssd_kv8_attention_set_polls(int polls);
+
 /* ---------------------------------------------------------------- page moves */
 /*
  * Copy page src_ids[i * src_step] of one pool to page dst_ids[i * dst_step] of another (or the

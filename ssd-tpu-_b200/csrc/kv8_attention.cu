@@ -37,6 +37,7 @@ struct Kv8Attn {
   // With a plan (many rows), the splits go by the sequences' own lengths: nsplit of them for all sequences together,
   // partials [head][row group][split][rows], and plan[b] says which are sequence b's: the first, and how many.
   int2* plan;
+  uint32_t polls;       // of a device-side wait before the CTA gives up
 };
 
 constexpr int kMaxSeqLen = 1 << 30;  // so that a position behind the last split's end is still an int
@@ -904,7 +905,10 @@ __global__ void __launch_bounds__(kFewWarps * 32, NT == 1 ? 3 : 2) kv8_attention
 // its 8 row warps, which 17 warps and two stages do not hide (issue slots 36 % busy, tensor cores 21 %).  Four
 // sequences of 1000 to 8192 positions, 512 rows each: 27 us, 304 TFLOP/s.  Two groups of row warps that take tiles in
 // turn came out no faster (their two P tiles cost as much shared memory as a third stage would).
-// All waits are bounded: a CTA that gives up lets its copies and products end and writes NaN.
+// All waits are bounded, and a warp's lanes give up together.  A CTA that gives up raises `gave_up`, lets its copies and
+// products end, frees its TMEM and writes NaN to the rows that it has not finished, straight to global memory: warps
+// that have not noticed may still be writing tiles where results are staged.  (A row that is finished has waited for
+// the last product, hence for every tile.)
 namespace many {
 
 constexpr int ROWS = 128;    // query rows of a CTA: TMEM lanes
@@ -915,6 +919,7 @@ constexpr int THREADS = SOFT + CONV + 32;
 constexpr int kMinTiles = 2; // of a split
 constexpr int META = 4;      // tiles whose scales are kept: a tile's are read until its weights are done
 constexpr uint32_t kPolls = 1u << 24;
+__device__ uint32_t gave_up;  // 1 once a CTA's wait ran out (ssd_kv8_attention_status)
 
 template <int D>
 struct Cfg {
@@ -936,13 +941,15 @@ __device__ __forceinline__ uint32_t pack_meta(int ke, int ve) { return (uint32_t
 __device__ __forceinline__ int meta_k(uint32_t m) { return (int)(m >> 16) - 256; }
 __device__ __forceinline__ float meta_v(uint32_t m) { return (float)((int)(m & 0xffffu) - 256); }
 
-__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile int* stop) {
-  for (uint32_t i = 0; i < kPolls; ++i) {
-    if (tc::mbar_try_wait(bar, parity)) return true;
-    if ((i & 255u) == 255u && *stop) return false;
+// For whole warps: true in every lane, or false in every lane (some lanes' waits may have ended: nothing goes by that).
+__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile int* stop, uint32_t polls) {
+  bool ok = false;
+  for (uint32_t i = 0; i < polls; ++i) {
+    ok = tc::mbar_try_wait(bar, parity);
+    if (ok || ((i & 255u) == 255u && *stop)) break;
   }
-  *stop = 1;
-  return false;
+  if (!ok) *stop = 1;
+  return __all_sync(0xffffffffu, ok);
 }
 
 // Two fp32 operations in one instruction.
@@ -1114,6 +1121,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_many_kernel(const Kv
   uint32_t* slot = reinterpret_cast<uint32_t*>(gen + C::bars + 176);
   volatile int* stop = reinterpret_cast<volatile int*>(slot + 1);
   volatile int* nan_seen = reinterpret_cast<volatile int*>(slot + 2);
+  auto held = [&](uint32_t b, uint32_t parity) { return wait(b, parity, stop, a.polls); };
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int head = blockIdx.y / a.row_groups, rg = blockIdx.y % a.row_groups;
@@ -1179,7 +1187,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_many_kernel(const Kv
     auto swap = [&](float2* at2, int k, float& x, float& y) {
       at2[((k & 1) * 2 + half) * ROWS + r] = make_float2(x, y);
       tc::mbar_arrive(pair(quad));
-      if (!__all_sync(0xffffffffu, wait(pair(quad), k & 1, stop))) return false;
+      if (!held(pair(quad), k & 1)) return false;
       const float2 z = at2[((k & 1) * 2 + (half ^ 1)) * ROWS + r];
       x = z.x;
       y = z.y;
@@ -1203,7 +1211,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_many_kernel(const Kv
           tc::mbar_arrive(q_in);
         }
       }
-      ok = __all_sync(0xffffffffu, wait(q_in, 0, stop));
+      ok = held(q_in, 0);
       uint4 w[NQ];
 #pragma unroll
       for (int i = 0; i < NQ; ++i) w[i] = real && ok ? lds128(row + half * D + 16 * i) : make_uint4(0, 0, 0, 0);
@@ -1242,7 +1250,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_many_kernel(const Kv
     float M = -1e38f, N = -1e38f, l = 0.f;
 #pragma unroll 1
     for (int j = 0; ok && j < tiles; ++j) {
-      ok = __all_sync(0xffffffffu, wait(s_full(j & 1), (j >> 1) & 1, stop));
+      ok = held(s_full(j & 1), (j >> 1) & 1);
       if (!ok) break;
       tc::tc_fence_after();
       const int p0 = base + j * TILE + 32 * half;  // this thread's 32 positions
@@ -1353,7 +1361,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_many_kernel(const Kv
         }
       }
       if (j > 0) {  // the tile before has been added: its weights may go, and O may be rescaled
-        ok = __all_sync(0xffffffffu, wait(o_done, (j - 1) & 1, stop));
+        ok = held(o_done, (j - 1) & 1);
         if (!ok) break;
         tc::tc_fence_after();
       }
@@ -1381,15 +1389,24 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_many_kernel(const Kv
       float lo = l, unused = 0.f;
       ok = swap(pair_s, tiles + 1, lo, unused);
       l += lo;
-      ok = __all_sync(0xffffffffu, ok && wait(o_done, (tiles - 1) & 1, stop));
+      ok = ok && held(o_done, (tiles - 1) & 1);
     }
     tc::tc_fence_after();
-    if (!ok) l = __int_as_float(0x7fc00000);
     const bool partial = a.plan != nullptr;
     const int64_t po = ((int64_t)blockIdx.y * a.nsplit + blockIdx.x) * ROWS + r;
     const bool any = real && l != 0.f;  // l is NaN, not 0, where a seen score is
-    if (partial && !idle && half == 0) a.ws_ml[po] = make_float4(M, N, l, 0.f);
-    if (!partial || tiles > 0) {
+    const float nan = __int_as_float(0x7fc00000);
+    if (partial && !idle && half == 0) a.ws_ml[po] = make_float4(M, N, ok ? l : nan, 0.f);
+    if (!ok) {
+      if (lane == 0) atomicExch(&gave_up, 1u);
+      // Q's copies land before shared memory goes
+      for (uint32_t i = 0; i < kPolls && !tc::mbar_try_wait(q_in, 0); ++i) {}
+#pragma unroll 1
+      for (int d = half * (D / 2); d < (half + 1) * (D / 2); ++d) {
+        if (partial) a.ws_o[po * D + d] = nan;
+        else if (r < rows) reinterpret_cast<bf16*>(a.out)[at + d] = __float2bfloat16_rn(real ? nan : 0.f);
+      }
+    } else if (!partial || tiles > 0) {
       // O through the shared memory of K, V and P (every product is done): a thread puts its half row there and
       // sends it off with one bulk copy
       const float k = partial ? 1.f : any ? ex2(M - N) / l : 0.f;
@@ -1399,7 +1416,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_many_kernel(const Kv
 #pragma unroll 1
       for (int c = 0; c < HD; c += 32) {
         uint32_t y[32];
-        if (tiles > 0 && ok) {
+        if (tiles > 0) {
           tmem_load32(lanes + C::o_col + half * HD + c, y);
           tmem_ready(y);
         } else {
@@ -1543,7 +1560,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_many_kernel(const Kv
     const uint32_t kt = sm + C::k + set * C::KV, vt = sm + C::v + set * C::KV;
 #pragma unroll 1
     for (int j = set; j < tiles; j += 2) {
-      if (j >= 2 && !wait(k_free(set), ((j >> 1) - 1) & 1, stop)) break;
+      if (j >= 2 && !held(k_free(set), ((j >> 1) - 1) & 1)) break;
       uint32_t* mt = meta + (j % META) * TILE;
       if (UNI ? lane == 0 : pc == 0) {
 #pragma unroll
@@ -1555,8 +1572,8 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_many_kernel(const Kv
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       tc::mbar_arrive(k_full(set));
       fetch(j + 2, 0, kb, ks);
-      if (j < 2 && !wait(q_tmem, 0, stop)) break;  // V's tiles hold Q until then
-      if (j >= 2 && !wait(v_free(set), ((j >> 1) - 1) & 1, stop)) break;
+      if (j < 2 && !held(q_tmem, 0)) break;  // V's tiles hold Q until then
+      if (j >= 2 && !held(v_free(set), ((j >> 1) - 1) & 1)) break;
       if (base + j * TILE + 16 * cw + 15 > kmin) {  // NaN of positions that some row does not see: put back by row above
         uint32_t marks = 0;
 #pragma unroll
@@ -1587,7 +1604,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_many_kernel(const Kv
       uint32_t lead;
       asm volatile("{.reg .pred p; elect.sync _|p, 0xffffffff; selp.u32 %0, 1, 0, p;}" : "=r"(lead));
       auto ready = [&](uint32_t b, uint32_t parity) {
-        const bool ok = __all_sync(0xffffffffu, wait(b, parity, stop));
+        const bool ok = held(b, parity);
         tc::tc_fence_after();
         return ok;
       };
@@ -1640,6 +1657,8 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_many_kernel(const Kv
 }
 
 }  // namespace many
+
+std::atomic<uint32_t> wait_polls{many::kPolls};
 
 struct Kv8Layout {
   bool cc;              // CUDA-core kernel (fp32)
@@ -1789,6 +1808,7 @@ extern "C" int ssd_kv8_attention(ssd_stream_t stream, const void* q, const void*
   a.row_groups = (int)L.row_groups;
   a.nsplit = L.nsplit;
   a.split = L.split;
+  a.polls = wait_polls.load(std::memory_order_relaxed);
   a.ws_o = reinterpret_cast<float*>(w);
   a.ws_ml = reinterpret_cast<float4*>(w + L.off_ml);
   a.plan = L.planned ? reinterpret_cast<int2*>(w + L.off_plan) : nullptr;
@@ -1801,4 +1821,28 @@ extern "C" int ssd_kv8_attention(ssd_stream_t stream, const void* q, const void*
   if (head_dim == 256) return launch_cc<256>(st, a, B);
   if (head_dim == 128) return launch_cc<128>(st, a, B);
   return launch_cc<64>(st, a, B);
+}
+
+extern "C" int ssd_kv8_attention_status(ssd_stream_t stream) {
+  cudaStream_t st = (cudaStream_t)stream;
+  uint32_t gave_up = 0;
+  bool ok = cudaMemcpyFromSymbolAsync(&gave_up, many::gave_up, sizeof(gave_up), 0, cudaMemcpyDeviceToHost, st) ==
+                cudaSuccess &&
+            cudaStreamSynchronize(st) == cudaSuccess;
+  if (ok && gave_up) {
+    const uint32_t none = 0;
+    ok = cudaMemcpyToSymbolAsync(many::gave_up, &none, sizeof(none), 0, cudaMemcpyHostToDevice, st) == cudaSuccess &&
+         cudaStreamSynchronize(st) == cudaSuccess;
+  }
+  if (!ok) {
+    (void)cudaGetLastError();
+    return SSD_ERR_LAUNCH;
+  }
+  return gave_up ? SSD_ERR_TIMEOUT : SSD_OK;
+}
+
+extern "C" int ssd_kv8_attention_set_polls(int polls) {
+  if (polls < -1) return SSD_ERR_INVALID;
+  wait_polls.store(polls < 0 ? many::kPolls : (uint32_t)polls, std::memory_order_relaxed);
+  return SSD_OK;
 }

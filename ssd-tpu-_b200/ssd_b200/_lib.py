@@ -57,6 +57,8 @@ SIGNATURES = {
     "ssd_kv8_attention_workspace_size": (_sz, [_i, _i, _i, _i, _i, _i]),
     "ssd_kv8_attention": (_i, [_p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _i, _p, _i, _p, _p, _p, _f, _i, _i, _i, _i,
                                _p, _sz]),
+    "ssd_kv8_attention_status": (_i, [_p]),
+    "ssd_kv8_attention_set_polls": (_i, [_i]),
     "ssd_page_copy": (_i, [_p, _p, _p, _i, _p, _p, _i, _i, _sz, _i, _p, _i64, _p, _i64, _i, _p]),
     "ssd_page_compact": (_i, [_p, _p, _p, _p, _i, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i, _i, _p, _p, _p, _i,
                               _i]),

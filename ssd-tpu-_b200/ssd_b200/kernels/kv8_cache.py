@@ -223,3 +223,10 @@ def paged_kv8_attention(q: torch.Tensor, cache: KV8CacheState, layer: int, block
            cols, ints(seq_lens, (b,), "seq_lens", dev), ints(q_lens, (b,), "q_lens", dev), out.data_ptr(),
            hd ** -0.5 if scale is None else float(scale), b, t, hq, max_seq_len, None if ws is None else ws.data_ptr(), need)
     return out
+
+
+def check_kv8_attention(device=None) -> None:
+    """Wait for the current stream of the GPU (None: the current one) and raise if a ``paged_kv8_attention`` there gave
+    up a device-side wait since the last check (``ssd_kv8_attention_status``); its unfinished rows are NaN."""
+    dev = torch.device("cuda" if device is None else device)
+    launch("ssd_kv8_attention_status", _current_device() if dev.index is None else dev.index)

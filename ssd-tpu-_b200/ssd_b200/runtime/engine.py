@@ -40,6 +40,7 @@ import torch
 from .._lib import SSD_MAX_TP
 from ..algorithm.async_protocol import DraftCommand, DraftRequest
 from ..config import DecodeMode, SSDConfig
+from ..kernels.kv8_cache import check_kv8_attention
 from ..kernels.ops import max_tokens_per_forward
 from ..models.gemma import KV_CACHE_DTYPES, PRESETS
 from ..models.gemma_adapter import GemmaAdapter
@@ -131,8 +132,11 @@ class LLMEngine:
         finally:
             status = self.ranks.call("end")
         if any(status):
-            # a collective whose peer never arrived ends with a timeout status instead of hanging
-            raise RuntimeError(f"tensor-parallel collective timed out (rank statuses {status})")
+            # a collective whose peer never arrived, or another device-side wait, ends with a timeout status
+            # instead of hanging
+            raise RuntimeError(f"a collective or another device-side wait timed out (rank statuses {status})")
+        if self.draft is not None and self.config.kv_cache_dtype == "fp8":
+            check_kv8_attention(self.draft_device)
         return [s.completion_token_ids for s in seqs], collector.finish()
 
     def generate_stream(self, prompt: list[int], sampling: SamplingParams,

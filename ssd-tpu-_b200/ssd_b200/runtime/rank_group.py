@@ -28,6 +28,8 @@ import traceback
 
 import torch
 
+from .._lib import lib, stream_ptr
+
 
 class RankState:
     """One rank's share of the engine (weights, comm, decoders); its methods are the commands."""
@@ -75,7 +77,8 @@ class RankState:
         self._mark = self.comm.mark() if self.comm is not None else None
 
     def end(self) -> int:
-        """End of a generate call: drop its decoders, free their heap buffers; the collective status."""
+        """End of a generate call: drop its decoders, free their heap buffers; the status of the device-side waits (the
+        collectives', and the 8-bit cache attention's)."""
         torch.cuda.current_stream().synchronize()
         self.dec = None
         status = 0
@@ -83,6 +86,8 @@ class RankState:
             status = self.comm.status()
             if self._mark is not None:
                 self.comm.release(self._mark)
+        if self.kv_cache_dtype == "fp8":
+            status = lib().ssd_kv8_attention_status(stream_ptr()) or status
         return status
 
     # ------------------------------------------------------------ ar

@@ -62,3 +62,35 @@ def test_v_scales_far_apart_within_a_tile(cuda, hq, hkv, d, t, kind, big):
     p.dev_tables = p.dev_tables[:, :few["cols"]].contiguous()
     r = ref.attention(q, p.vals, p.exps, p.tables, few["lens"], ql, scale)
     _near(_run(p, q, few["lens"], ql)[0], r, p)
+
+
+@pytest.mark.parametrize("hq,hkv,d,lens", [(8, 1, 256, [500, 300]), (8, 1, 256, [3000, 100]), (16, 4, 64, [512, 12]),
+                                           (4, 2, 128, [1500, 700])])
+def test_a_wait_that_runs_out_is_reported(cuda, hq, hkv, d, lens):
+    """No polls allowed: every CTA gives up at its first wait.  Rows are NaN (those past q_lens zeros), the status says so
+    once, and the next call is right."""
+    from ssd_b200._lib import SSDError, lib
+    from ssd_b200.kernels.kv8_cache import check_kv8_attention
+
+    rng = np.random.default_rng(1)
+    t, ql = 40, [40, 33]
+    lens = [max(n, t) for n in lens]
+    p = Pool(rng, 2, 16, hkv, d, cols=-(-max(lens) // 16))
+    k = _round(rng.standard_normal((2, max(lens), hkv, d)), "bf16")
+    p.append(lens, k, k, lens, "bf16")
+    q = _round(rng.standard_normal((2, t, hq, d)), "bf16")
+    check_kv8_attention()
+    assert lib().ssd_kv8_attention_set_polls(-2) == 1
+    try:
+        assert lib().ssd_kv8_attention_set_polls(0) == 0
+        got = _run(p, q, lens, ql)[0]
+    finally:
+        assert lib().ssd_kv8_attention_set_polls(-1) == 0
+    with pytest.raises(SSDError, match="timed out"):
+        check_kv8_attention()
+    check_kv8_attention("cuda")
+    for b in range(2):
+        assert np.isnan(got[b, :ql[b]]).all() and (got[b, ql[b]:] == 0).all()
+    r = ref.attention(q, p.vals, p.exps, p.tables, lens, ql, 1 / math.sqrt(d))
+    _near(_run(p, q, lens, ql)[0], r, p)
+    check_kv8_attention()
