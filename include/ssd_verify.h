@@ -263,8 +263,9 @@ int ssd_paged_verify_attention(ssd_stream_t stream, const void* q, const void* p
  * A paged cache that holds K and V in 8 bits (no counterpart in the reference, whose cache is
  * bf16/fp32, jax_ssd/kernels/kv_cache.py:13): half the bytes of bf16 to store and to read.
  *   pages  [2, num_layers, num_blocks, block_size, Hkv, D] e4m3
- *   scales [2, num_layers, num_blocks, Hkv] fp32, powers of two: an element is its e4m3 value times
- *          the scale of its plane, layer, page and KV head
+ *   scales [2, num_layers, num_blocks, Hkv] fp32, powers of two 2^-118 .. 2^120: an element is its e4m3
+ *          value times the scale of its plane, layer, page and KV head.  Any other stored value counts
+ *          as the power of two at its exponent field, within those limits
  * head_dim is 64, 128 or 256; pages, k, v, q, qkv and the outputs are 16-byte aligned
  * (else SSD_ERR_UNSUPPORTED).  num_blocks * block_size < 2^31, block_size <= 2^20.
  * A page's scale is the smallest power of two (at least 2^-118) under which its largest finite

@@ -345,11 +345,13 @@ __global__ void __launch_bounds__(256) kv8_gather_kernel(const Kv8Cache c, const
     const int plane = it >= items, j = plane ? it - items : it;
     if (it >= 2 * items) break;
     const uint32_t in[2] = {x[i].x, x[i].y};
+    asm volatile("" : "+f"(s[i]));  // keeps what follows behind the loads: interleaved with them it costs 3.5 us of 25.5
+    const float by = stored_scale(s[i]);
     float f[8];
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
       const float2 lo = e4m3_pair(in[q]), hi = e4m3_pair(in[q] >> 16);
-      f[4 * q] = lo.x * s[i]; f[4 * q + 1] = lo.y * s[i]; f[4 * q + 2] = hi.x * s[i]; f[4 * q + 3] = hi.y * s[i];
+      f[4 * q] = lo.x * by; f[4 * q + 1] = lo.y * by; f[4 * q + 2] = hi.x * by; f[4 * q + 3] = hi.y * by;
     }
     store8((plane ? v : k) + m * c.hkv * D + (int64_t)j * 8, f);
   }

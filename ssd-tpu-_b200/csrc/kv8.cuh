@@ -24,9 +24,13 @@ __device__ __forceinline__ int kv8_exponent(float amax) {
   return max(e, kKv8MinExp);
 }
 __device__ __forceinline__ float exp2i(int e) { return __int_as_float((e + 127) << 23); }  // -126 <= e <= 127
-// Exponent of a stored scale.  A page that nothing was appended to may hold anything there: clamped.
+// Exponent of a stored scale.  A page that nothing was appended to may hold anything there: clamped, and every kernel
+// takes a scale by this exponent, so that a page reads the same whichever is chosen.
 __device__ __forceinline__ int scale_exponent(float s) {
   return min(max((int)((__float_as_uint(s) >> 23) & 0xffu) - 127, kKv8MinExp), 120);
+}
+__device__ __forceinline__ float stored_scale(float s) {  // exp2i(scale_exponent(s)) in three instructions
+  return fminf(fmaxf(__uint_as_float(__float_as_uint(s) & 0x7f800000u), 3.009265538e-36f), 1.329227996e36f);
 }
 
 // |x| where x is finite, else 0 (the scale goes by the finite values; the others are stored as NaN).

@@ -290,8 +290,8 @@ __global__ void __launch_bounds__(kCcSplit) kv8_attention_cc_kernel(const Kv8Att
   if (there) {
     off = a.c.layer + (((int64_t)blk * a.c.block_size + j % a.c.block_size) * a.c.hkv + head) * D;
     const float* sc = a.c.scales + a.c.scale_layer + (int64_t)blk * a.c.hkv + head;
-    ks = ld_act(sc);
-    vs = ld_act(sc + a.c.scale_plane);
+    ks = stored_scale(ld_act(sc));
+    vs = stored_scale(ld_act(sc + a.c.scale_plane));
 #pragma unroll
     for (int i = 0; i < D / 16; ++i) w[i] = ld_act_v4(a.c.pages + off + 16 * i);
   }
@@ -526,7 +526,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, NT == 1 ? 3 : 2) kv8_attention
         const int blk = ld_act(table + page);
         if ((unsigned)blk < (unsigned)a.c.num_blocks) {
           row = blk * a.c.block_size + (j - page * a.c.block_size);
-          ks = exp2i(scale_exponent(ld_act(sc + (int64_t)blk * a.c.hkv)));
+          ks = stored_scale(ld_act(sc + (int64_t)blk * a.c.hkv));
           ve = (float)scale_exponent(ld_act(sc + a.c.scale_plane + (int64_t)blk * a.c.hkv));
         }
       }
@@ -647,7 +647,7 @@ __global__ void __launch_bounds__(kFewWarps * 32, NT == 1 ? 3 : 2) kv8_attention
       for (int e = 0; e < 4; ++e) o[nt][i][e] = 0.f;
   }
   if constexpr (UNI) {
-    ks_l = exp2i(scale_exponent(ks_l));
+    ks_l = stored_scale(ks_l);
     ve_l = (float)scale_exponent(ve_l);
   }
   for (int k = 0; k < mine; ++k) {
@@ -1482,7 +1482,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_many_kernel(const Kv
     const int64_t rs = (int64_t)a.c.hkv * D;
     int blk[NB], off[NB];        // of the tile to be fetched next
     uint4 kb[NI], vb[NI];        // this tile's bytes, then the next one's as soon as they are converted: they have two
-    float ks[NB], vs[NB];        // tiles' time to arrive; and the scales (0: no row)
+    float ks[NB], vs[NB];        // tiles' time to arrive; and the scales (-1: no row)
     int ids = -1;          // UNI: lane x has the block id of the warp's positions in its tile 32 k + x
     auto look = [&](int j) {
       if constexpr (UNI) {
@@ -1518,7 +1518,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_many_kernel(const Kv
       const float* from = sc + plane * a.c.scale_plane;
 #pragma unroll
       for (int i = 0; i < NB; ++i)
-        xs[i] = (unsigned)blk[i] < (unsigned)a.c.num_blocks ? ld_act(from + (int64_t)blk[i] * a.c.hkv) : 0.f;
+        xs[i] = (unsigned)blk[i] < (unsigned)a.c.num_blocks ? fabsf(ld_act(from + (int64_t)blk[i] * a.c.hkv)) : -1.f;
       if constexpr (UNI) {
         const bool in = (unsigned)blk[0] < (unsigned)a.c.num_blocks;
         const uint8_t* s = kp + plane * a.c.plane + (in ? ((int64_t)blk[0] * a.c.block_size + off[0] + rr) * rs : 0);
@@ -1565,7 +1565,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_many_kernel(const Kv
       if (UNI ? lane == 0 : pc == 0) {
 #pragma unroll
         for (int i = 0; i < NB; ++i)
-          mt[UNI ? cw : 16 * cw + rr + i * RPI] = ks[i] == 0.f ? 0u : pack_meta(scale_exponent(ks[i]), scale_exponent(vs[i]));
+          mt[UNI ? cw : 16 * cw + rr + i * RPI] = ks[i] < 0.f ? 0u : pack_meta(scale_exponent(ks[i]), scale_exponent(vs[i]));
       }
 #pragma unroll
       for (int i = 0; i < NI; ++i) put(kt, i, kb[i]);

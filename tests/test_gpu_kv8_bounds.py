@@ -94,3 +94,31 @@ def test_a_wait_that_runs_out_is_reported(cuda, hq, hkv, d, lens):
     r = ref.attention(q, p.vals, p.exps, p.tables, lens, ql, 1 / math.sqrt(d))
     _near(_run(p, q, lens, ql)[0], r, p)
     check_kv8_attention()
+
+
+@pytest.mark.parametrize("dtype,hq,hkv,d,bs,t", [("bf16", 8, 1, 64, 16, 2), ("bf16", 8, 1, 64, 16, 40), ("bf16", 4, 2, 128, 4, 3),
+                                                 ("bf16", 8, 2, 128, 4, 33), ("f32", 4, 1, 64, 16, 5)])
+def test_scales_count_by_their_exponent_everywhere(cuda, dtype, hq, hkv, d, bs, t):
+    """A stored scale that append would not have written -- zero, subnormal, negative, no power of two -- is the power of
+    two at its exponent, 2^-118 at least, for every kernel that reads it; a scale of zero is no missing page."""
+    from ssd_b200.kernels.kv8_cache import gather_kv8
+
+    torch, _ = _torch()
+    rng = np.random.default_rng(31)
+    lens, ql = [200, 90], [t, t - 1]
+    p = Pool(rng, 2, bs, hkv, d, cols=-(-200 // bs))
+    k = _round(rng.standard_normal((2, 200, hkv, d)), "bf16")
+    p.append(lens, k, _round(rng.standard_normal((2, 200, hkv, d)), "bf16"), lens, "bf16")
+    for col, (stored, e) in enumerate([(0.0, -118), (1e-42, -118), (-2.0 ** -8, -8), (3 * 2.0 ** -8, -7)]):
+        for plane in range(2):
+            blk = p.tables[0, 2 * col + plane]
+            p.cache.scales[plane, 1, blk] = stored
+            p.exps[plane, blk] = e
+    q = _round(rng.standard_normal((2, t, hq, d)), dtype)
+    r = ref.attention(q, p.vals, p.exps, p.tables, lens, ql, 1 / math.sqrt(d))
+    _near(_run(p, q, lens, ql, dtype)[0], r, p, dtype)
+    pos = np.arange(200)
+    gk, gv = gather_kv8(p.cache, 1, p.dev_tables[:1].contiguous(), _i(pos[None]), dtype=torch.float32)
+    rk, rv = ref.o.rows_of(p.vals, p.exps, p.tables[0], pos)
+    np.testing.assert_array_equal(gk[0].cpu().numpy(), rk)
+    np.testing.assert_array_equal(gv[0].cpu().numpy(), rv)
