@@ -1227,9 +1227,10 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_many_kernel(const Kv
       ok = ok && swap(pair_s, 0, other, unused);
       top = fmaxf(top, other);
       const int e = min(max((int)(__float_as_uint(top) >> 23) - 127 - 14, -118), 120);
-      const float inv = copysignf(exp2i(-e), a.scale);  // the row's factor is never negative
+      // The row's factor is never negative.  A row with an infinity has no finite score, or one less itself: NaN, put
+      // into Q so that only positions that it sees bring it in.
+      const float inv = top == INFINITY ? __int_as_float(0x7fc00000) : copysignf(exp2i(-e), a.scale);
       qs = exp2i(e) * fabsf(a.scale) * 1.4426950408889634f;
-      if (top == INFINITY) qs = __int_as_float(0x7fc00000);  // such a row has no finite score, or one less itself
 #pragma unroll
       for (int c = 0; c < NQ; c += 4) {
         uint32_t y[16];

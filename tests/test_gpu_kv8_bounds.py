@@ -122,3 +122,30 @@ def test_scales_count_by_their_exponent_everywhere(cuda, dtype, hq, hkv, d, bs, 
     rk, rv = ref.o.rows_of(p.vals, p.exps, p.tables[0], pos)
     np.testing.assert_array_equal(gk[0].cpu().numpy(), rk)
     np.testing.assert_array_equal(gv[0].cpu().numpy(), rv)
+
+
+@pytest.mark.parametrize("dtype,t,bs", [("bf16", 2, 16), ("bf16", 40, 16), ("bf16", 40, 4), ("f32", 5, 16)])
+def test_infinite_queries_that_see_nothing(cuda, dtype, t, bs):
+    """A row of q with an infinity is NaN where it sees a position, zeros where every page it could see is missing."""
+    rng = np.random.default_rng(17)
+    lens = [300, 300, 90]
+    p = Pool(rng, 3, bs, 1, 64, cols=-(-300 // bs))
+    k = _round(rng.standard_normal((3, 300, 1, 64)), "bf16")
+    p.append(lens, k, k, lens, "bf16")
+    p.tables[0] = -1
+    p.tables[2, 1:] = 10 ** 6  # one page left
+    import torch
+
+    p.dev_tables = torch.tensor(p.tables, device="cuda")
+    q = _round(rng.standard_normal((3, t, 8, 64)), dtype)
+    q[:, 0, 3, 5] = np.inf
+    q[:, t - 1, 4] = -np.inf
+    got = _run(p, q, lens, [t] * 3, dtype)[0]
+    assert (got[0] == 0).all()
+    for b in (1, 2):
+        assert np.isnan(got[b, 0, 3]).all() and np.isnan(got[b, t - 1, 4]).all()
+    finite = np.isfinite(q).all(-1)
+    q[~finite] = 0
+    r = ref.attention(q, p.vals, p.exps, p.tables, lens, [t] * 3, 1 / 8)
+    off, tol = np.abs(got - r["out"])[finite], ref.bound(r, p.exps, dtype)[finite]
+    assert (off <= tol).all()
