@@ -306,6 +306,10 @@ int ssd_kv8_gather(ssd_stream_t stream, const void* pages, const float* scales, 
                    int block_size, int num_kv_heads, int head_dim, int layer, const int32_t* block_tables,
                    int max_blocks, const int32_t* positions, void* k, void* v, int dtype, int B, int N);
 
+/* Bytes that ssd_kv8_attention wants for q of `dtype`; without the type, enough for either (fp32's partials can
+ * be gigabytes where bf16 needs none: prompts of thousands of rows). */
+size_t ssd_kv8_attention_workspace_size_for(int dtype, int B, int T, int num_heads, int num_kv_heads, int head_dim,
+                                            int max_seq_len);
 size_t ssd_kv8_attention_workspace_size(int B, int T, int num_heads, int num_kv_heads, int head_dim,
                                         int max_seq_len);
 

@@ -1762,14 +1762,19 @@ int launch_bf16(cudaStream_t st, const Kv8Attn& a, const Kv8Layout& L, int B) {
 
 using namespace ssd;
 
+extern "C" size_t ssd_kv8_attention_workspace_size_for(int dtype, int B, int T, int num_heads, int num_kv_heads,
+                                                       int head_dim, int max_seq_len) {
+  if (B <= 0 || T <= 0 || num_kv_heads <= 0 || num_heads <= 0 || num_heads % num_kv_heads || head_dim <= 0 ||
+      max_seq_len <= 0 || max_seq_len > kMaxSeqLen || (dtype != SSD_DTYPE_BF16 && dtype != SSD_DTYPE_F32))
+    return 0;
+  return kv8_layout(dtype == SSD_DTYPE_F32, B, T, num_heads, num_kv_heads, head_dim, max_seq_len).total;
+}
+
 extern "C" size_t ssd_kv8_attention_workspace_size(int B, int T, int num_heads, int num_kv_heads, int head_dim,
                                                    int max_seq_len) {
-  if (B <= 0 || T <= 0 || num_kv_heads <= 0 || num_heads <= 0 || num_heads % num_kv_heads || head_dim <= 0 ||
-      max_seq_len <= 0 || max_seq_len > kMaxSeqLen)
-    return 0;
-  const size_t a = kv8_layout(true, B, T, num_heads, num_kv_heads, head_dim, max_seq_len).total;
-  const size_t b = kv8_layout(false, B, T, num_heads, num_kv_heads, head_dim, max_seq_len).total;
-  return a > b ? a : b;
+  return std::max(
+      ssd_kv8_attention_workspace_size_for(SSD_DTYPE_F32, B, T, num_heads, num_kv_heads, head_dim, max_seq_len),
+      ssd_kv8_attention_workspace_size_for(SSD_DTYPE_BF16, B, T, num_heads, num_kv_heads, head_dim, max_seq_len));
 }
 
 extern "C" int ssd_kv8_attention(ssd_stream_t stream, const void* q, const void* pages, const float* scales,

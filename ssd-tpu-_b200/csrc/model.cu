@@ -173,7 +173,7 @@ Scratch carve(const ssd_gemma_weights* w, int B, int T, int max_seq_len, char* b
   s.lin_ws_bytes = lw;
   s.lin_ws = take(lw);
   // one workspace for either cache; the 8-bit one's part lies behind the ticket counters, which it must not touch
-  const size_t kv8 = ssd_kv8_attention_workspace_size(B, T, hq, hkv, D, max_seq_len);
+  const size_t kv8 = ssd_kv8_attention_workspace_size_for(w->dtype, B, T, hq, hkv, D, max_seq_len);
   s.attn_ws_bytes = std::max(ssd_paged_attention_workspace_size(B, T, hq, hkv, D, max_seq_len), kKv8WsOffset + kv8);
   s.attn_ws = take(s.attn_ws_bytes);
   s.total = off;

@@ -54,6 +54,7 @@ SIGNATURES = {
     "ssd_kv8_rope_append": (_i, [_p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _i, _i, _p, _i, _p, _p, _p, _p, _i,
                                  _i, _i]),
     "ssd_kv8_gather": (_i, [_p, _p, _p, _i, _i, _i, _i, _i, _i, _p, _i, _p, _p, _p, _i, _i, _i]),
+    "ssd_kv8_attention_workspace_size_for": (_sz, [_i, _i, _i, _i, _i, _i, _i]),
     "ssd_kv8_attention_workspace_size": (_sz, [_i, _i, _i, _i, _i, _i]),
     "ssd_kv8_attention": (_i, [_p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _i, _p, _i, _p, _p, _p, _f, _i, _i, _i, _i,
                                _p, _sz]),

@@ -189,8 +189,8 @@ def gather_kv8(cache: KV8CacheState, layer: int, block_tables: torch.Tensor, pos
 
 
 @lru_cache(maxsize=1024)  # a function of these sizes alone
-def _workspace_size(b: int, t: int, hq: int, hkv: int, hd: int, max_seq_len: int) -> int:
-    return lib().ssd_kv8_attention_workspace_size(b, t, hq, hkv, hd, max_seq_len)
+def _workspace_size(dtype: int, b: int, t: int, hq: int, hkv: int, hd: int, max_seq_len: int) -> int:
+    return lib().ssd_kv8_attention_workspace_size_for(dtype, b, t, hq, hkv, hd, max_seq_len)
 
 
 def paged_kv8_attention(q: torch.Tensor, cache: KV8CacheState, layer: int, block_tables: torch.Tensor,
@@ -217,9 +217,10 @@ def paged_kv8_attention(q: torch.Tensor, cache: KV8CacheState, layer: int, block
     elif out.shape != q.shape or out.dtype != q.dtype or out.get_device() != dev or not out.is_contiguous():
         raise ValueError(f"out must be a contiguous {q.dtype} tensor {list(q.shape)} on cuda:{dev}")
     # a workspace of its own for every call: calls on other streams or in captured graphs share nothing
-    need = _workspace_size(b, t, hq, hkv, hd, max_seq_len)
+    dtype = dtype_code(q.dtype)
+    need = _workspace_size(dtype, b, t, hq, hkv, hd, max_seq_len)
     ws = q.new_empty((need,), dtype=torch.uint8) if need else None
-    launch("ssd_kv8_attention", dev, at, pages, scales, dtype_code(q.dtype), nl, nb, bs, hkv, hd, layer, tab,
+    launch("ssd_kv8_attention", dev, at, pages, scales, dtype, nl, nb, bs, hkv, hd, layer, tab,
            cols, ints(seq_lens, (b,), "seq_lens", dev), ints(q_lens, (b,), "q_lens", dev), out.data_ptr(),
            hd ** -0.5 if scale is None else float(scale), b, t, hq, max_seq_len, None if ws is None else ws.data_ptr(), need)
     return out

@@ -149,3 +149,21 @@ def test_infinite_queries_that_see_nothing(cuda, dtype, t, bs):
     r = ref.attention(q, p.vals, p.exps, p.tables, lens, [t] * 3, 1 / 8)
     off, tol = np.abs(got - r["out"])[finite], ref.bound(r, p.exps, dtype)[finite]
     assert (off <= tol).all()
+
+
+def test_long_prompts_allocate_their_output_alone(cuda):
+    """600 rows of 16 heads against 8192 positions: unsplit, so a call's memory is its output."""
+    from ssd_b200.kernels.kv8_cache import KV8CacheState, append_kv8, paged_kv8_attention
+
+    torch, _ = _torch()
+    t, cols = 600, 512
+    cache = KV8CacheState.allocate(1, cols, 16, 16, 64)
+    table = torch.arange(cols, dtype=torch.int32, device="cuda")[None]
+    q = torch.randn((1, t, 16, 64), device="cuda").bfloat16()
+    append_kv8(cache, 0, table, _i([t]), q, q)
+    paged_kv8_attention(q, cache, 0, table, _i([t]))
+    n = _i([t])
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    paged_kv8_attention(q, cache, 0, table, n)
+    assert torch.cuda.max_memory_allocated() - before <= q.numel() * 2 + (1 << 21)  # one block of the allocator beside it

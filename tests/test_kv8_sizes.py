@@ -1,0 +1,17 @@
+"""CPU: what calls over the 8-bit cache ask for."""
+
+from __future__ import annotations
+
+
+def test_workspace_goes_by_the_type():
+    """Prompts of thousands of bf16 rows are not split and need no workspace, whatever fp32 would take."""
+    from ssd_b200._lib import SSD_DTYPE_BF16, SSD_DTYPE_F32, lib
+
+    so = lib()
+    size, either = so.ssd_kv8_attention_workspace_size_for, so.ssd_kv8_attention_workspace_size
+    for shape in ((4, 2048, 16, 16, 256, 8192), (1, 1500, 16, 16, 256, 8192)):
+        assert size(SSD_DTYPE_BF16, *shape) == 0
+        assert size(SSD_DTYPE_F32, *shape) > 1 << 29
+    for shape in ((1, 5, 4, 2, 64, 1000), (8, 5, 16, 16, 256, 4096), (4, 64, 8, 1, 256, 8192), (1, 1, 8, 1, 256, 137)):
+        assert either(*shape) == max(size(d, *shape) for d in (SSD_DTYPE_BF16, SSD_DTYPE_F32))
+    assert size(2, 1, 5, 4, 2, 64, 1000) == size(0, 1, 5, 4, 3, 64, 1000) == size(0, 1, 5, 4, 2, 64, (1 << 30) + 1) == 0
