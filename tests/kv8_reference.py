@@ -66,3 +66,24 @@ def bound(r: dict, exps, dtype: str) -> np.ndarray:
     if dtype == "bf16":
         tol = tol + 2.0 ** -11 * A + n * 2.0 ** -32 * 448 * r["top"] + D * 2.0 ** -39 * S * A
     return tol + {"bf16": 2.0 ** -8, "f32": 2.0 ** -24}[dtype] * np.abs(r["out"])
+
+
+def sparse_pool(rng, nb: int, bs: int, hkv: int, d: int) -> tuple[np.ndarray, np.ndarray]:
+    """One layer, vals [2, nb, bs, hkv, d] and exps [2, nb, hkv]: normal K, and V rows with one positive element, its
+    dimension spread evenly over the rows.  An output is then a sum over every d-th position or so, without
+    cancellation: one that is lost or counted twice moves it by about d / n of itself."""
+    vals = np.zeros((2, nb, bs, hkv, d))
+    exps = rng.integers(-8, -4, (2, nb, hkv))
+    vals[0] = o.e4m3_round(np.clip(rng.standard_normal((nb, bs, hkv, d)) * np.exp2(-exps[0].astype(float))[:, None, :, None],
+                                   -448, 448))
+    dim = rng.permuted(np.tile(np.arange(nb * bs) % d, (hkv, 1)), axis=1).T.reshape(nb, bs, hkv)
+    mag = o.e4m3_round(rng.uniform(0.6, 1, dim.shape) * np.exp2(-exps[1].astype(float))[:, None])
+    np.put_along_axis(vals[1], dim[..., None], mag[..., None], axis=-1)
+    return vals, exps
+
+
+def e4m3_bytes(vals: np.ndarray) -> np.ndarray:
+    """The bytes of e4m3 numbers."""
+    table = o.e4m3_values()[:127]
+    b = np.searchsorted(table, np.abs(vals)).astype(np.uint8)
+    return b | np.where(np.signbit(vals), 128, 0).astype(np.uint8)

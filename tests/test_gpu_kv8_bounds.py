@@ -8,7 +8,7 @@ import numpy as np
 import pytest
 
 import kv8_reference as ref
-from test_gpu_kv8 import Pool, _round, _torch
+from test_gpu_kv8 import CASES, Pool, _attention_inputs, _round, _torch
 
 pytestmark = pytest.mark.gpu
 
@@ -167,3 +167,84 @@ def test_long_prompts_allocate_their_output_alone(cuda):
     before = torch.cuda.memory_allocated()
     paged_kv8_attention(q, cache, 0, table, n)
     assert torch.cuda.max_memory_allocated() - before <= q.numel() * 2 + (1 << 21)  # one block of the allocator beside it
+
+
+def _sparse(seed, b, nb, cols, bs, hkv, d):
+    """A pool as ``Pool`` has it, from ``ref.sparse_pool``; sequences share pages (they are only read)."""
+    from types import SimpleNamespace
+
+    from ssd_b200.kernels.kv8_cache import KV8CacheState
+
+    torch, _ = _torch()
+    rng = np.random.default_rng(seed)
+    vals, exps = ref.sparse_pool(rng, nb, bs, hkv, d)
+    cache = KV8CacheState.allocate(2, nb, bs, hkv, d)
+    cache.pages.view(torch.uint8)[:, 0].fill_(0x7F)
+    cache.pages.view(torch.uint8)[:, 1] = torch.tensor(ref.e4m3_bytes(vals)).cuda()
+    cache.scales[:, 1] = torch.tensor(np.exp2(exps.astype(np.float32))).cuda()
+    tables = np.stack([rng.permutation(nb)[np.arange(cols) % nb] for _ in range(b)]).astype(np.int32)
+    return SimpleNamespace(cache=cache, vals=vals, exps=exps, tables=tables, dev_tables=torch.tensor(tables).cuda()), rng
+
+
+LONG = [  # dtype, hq, hkv, d, bs, t, longest, sequences: split of the bound at 666 CTAs
+    ("bf16", 16, 16, 64, 16, 1, 4096, 8),     # 832
+    ("bf16", 16, 16, 64, 16, 5, 4096, 8),
+    ("bf16", 16, 16, 64, 4, 5, 4096, 8),      # 832, a row and scales a position
+    ("bf16", 16, 16, 128, 16, 5, 2500, 8),    # 512
+    ("bf16", 8, 8, 256, 16, 3, 3000, 6),      # 256
+    ("bf16", 4, 4, 256, 16, 2, 3333, 20),     # 448
+    ("bf16", 8, 1, 64, 16, 8, 4096, 170),     # 1024, 64 rows a KV head
+    ("bf16", 8, 1, 64, 1, 2, 4000, 170),
+    ("bf16", 16, 2, 128, 24, 7, 4000, 90),    # 1024, pages of 24
+    ("bf16", 8, 1, 256, 16, 64, 8192, 4),     # prompt chunks: by the lengths
+    ("bf16", 8, 1, 128, 4, 33, 5000, 3),
+    ("bf16", 16, 4, 64, 16, 200, 6000, 2),
+    ("f32", 4, 1, 64, 16, 5, 3000, 5),
+    ("f32", 2, 2, 256, 4, 3, 1500, 3),
+]
+
+
+@pytest.mark.parametrize("case", LONG, ids=lambda c: "-".join(map(str, c)))
+def test_long_contexts_at_their_bounds(cuda, case):
+    """Contexts of many splits, of every length the rule gives; a position lost or counted twice would show.  A few
+    heads and sequences are compared, the longest and the shortest among them."""
+    dtype, hq, hkv, d, bs, t, top, b = case
+    p, rng = _sparse(b * t, b, -(-top // bs), -(-top // bs), bs, hkv, d)
+    lens = rng.integers(t, top + 1, b)
+    lens[0], lens[1], lens[b - 1] = top, t, top - 1
+    ql = np.where(np.arange(b) % 4 == 2, max(t - 1, 1), t)
+    q = _round(0.25 * rng.standard_normal((b, t, hq, d)), dtype)  # weights alike: each position counts
+    got, _ = _run(p, q, lens, ql, dtype)
+    some = sorted({0, 1, min(2, b - 1), b - 1})
+    heads = sorted({0, hq // 2, hq - 1})
+    r = ref.attention(q[some], p.vals, p.exps, p.tables[some], lens[some], ql[some], 1 / math.sqrt(d), heads=heads)
+    tol = ref.bound(r, p.exps, dtype)
+    off = np.abs(got[some] - r["out"])[:, :, heads]
+    assert (off <= tol[:, :, heads]).all(), (off / np.maximum(tol[:, :, heads], 1e-300)).max()
+    assert all((got[i, ql[i]:] == 0).all() for i in range(b))
+
+
+@pytest.mark.parametrize("hq,hkv,d,bs,t,top,b", [(16, 16, 64, 16, 5, 4096, 8), (16, 16, 64, 4, 5, 4096, 8),
+                                                 (8, 1, 256, 16, 8, 8192, 3), (8, 1, 64, 16, 8, 4096, 170),
+                                                 (16, 4, 128, 16, 6, 3000, 16)])
+def test_bits_do_not_depend_on_the_tokens_beside(cuda, hq, hkv, d, bs, t, top, b):
+    """At a given batch and bound, a verify step gives each token the bits that decoding it alone does, whatever the split
+    (832, 832, 256, 1024 and 320 positions here)."""
+    torch, _ = _torch()
+    p, rng = _sparse(t, b, -(-top // bs), -(-top // bs), bs, hkv, d)
+    lens = rng.integers(t, top + 1, b)
+    lens[0], lens[1] = top, t
+    q = _round(rng.standard_normal((b, t, hq, d)), "bf16")
+    _, full = _run(p, q, lens, [t] * b)
+    for j in range(t):
+        _, one = _run(p, q[:, j:j + 1], lens - t + j + 1, [1] * b)
+        assert torch.equal(one[:, 0], full[:, j]), j
+
+
+@pytest.mark.parametrize("case", CASES, ids=lambda c: "-".join(map(str, c[:6])))
+def test_attention_at_its_bounds(cuda, case):
+    """The shapes of the oracle's test, at the bounds of the present arithmetic."""
+    dtype, hq, hkv, d, bs, t, lens = case
+    p, q, ql = _attention_inputs(case, seed=hq * d + t + bs)
+    r = ref.attention(q, p.vals, p.exps, p.tables, lens, ql, 1 / math.sqrt(d))
+    _near(_run(p, q, lens, ql, dtype)[0], r, p, dtype)
