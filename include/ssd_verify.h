@@ -271,7 +271,8 @@ int ssd_paged_verify_attention(ssd_stream_t stream, const void* q, const void* p
  * A page's scale is the smallest power of two (at least 2^-118) under which its largest finite
  * magnitude stays within e4m3's 448.  Rounding is to nearest even; infinities and NaN are stored as
  * NaN and do not count for the scale.
- * B = 0 or T = 0 is allowed and does nothing.
+ * B = 0 or T = 0 is allowed and does nothing; with B = 0 the per-sequence arrays, the rows and the
+ * outputs may be NULL, with T = 0 the rows and outputs.
  */
 
 /*

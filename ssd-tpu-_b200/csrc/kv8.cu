@@ -385,11 +385,9 @@ extern "C" int ssd_kv8_append(ssd_stream_t stream, void* pages, float* scales, i
                               int max_blocks, const int32_t* seq_lens, const int32_t* q_lens, const void* k,
                               const void* v, int dtype, int B, int T) {
   if (int rc = kv8_check(pages, scales, num_layers, num_blocks, block_size, num_kv_heads, head_dim, layer)) return rc;
-  if (B < 0 || T < 0 || max_blocks <= 0 || !block_tables || !seq_lens ||
-      (dtype != SSD_DTYPE_BF16 && dtype != SSD_DTYPE_F32))
-    return SSD_ERR_INVALID;
-  if (B == 0 || T == 0) return SSD_OK;
-  if (!k || !v) return SSD_ERR_INVALID;
+  if (B < 0 || T < 0 || max_blocks <= 0 || (dtype != SSD_DTYPE_BF16 && dtype != SSD_DTYPE_F32)) return SSD_ERR_INVALID;
+  if (B == 0 || (T == 0 && block_tables && seq_lens)) return SSD_OK;  // arrays of nothing may have no address
+  if (!block_tables || !seq_lens || !k || !v) return SSD_ERR_INVALID;
   if (!kv8_aligned(k) || !kv8_aligned(v)) return SSD_ERR_UNSUPPORTED;
   AppendArgs a{};
   a.c = kv8_cache(pages, scales, num_layers, num_blocks, block_size, num_kv_heads, head_dim, layer);
@@ -409,11 +407,11 @@ extern "C" int ssd_kv8_rope_append(ssd_stream_t stream, const void* qkv, void* q
                                    int max_blocks, const int32_t* seq_lens, const int32_t* q_lens,
                                    const float* rope_cos, const float* rope_sin, int rope_max_pos, int B, int T) {
   if (int rc = kv8_check(pages, scales, num_layers, num_blocks, block_size, num_kv_heads, head_dim, layer)) return rc;
-  if (B < 0 || T < 0 || max_blocks <= 0 || num_heads <= 0 || rope_max_pos <= 0 || !block_tables || !seq_lens ||
-      !rope_cos || !rope_sin || (dtype != SSD_DTYPE_BF16 && dtype != SSD_DTYPE_F32))
+  if (B < 0 || T < 0 || max_blocks <= 0 || num_heads <= 0 || rope_max_pos <= 0 || !rope_cos || !rope_sin ||
+      (dtype != SSD_DTYPE_BF16 && dtype != SSD_DTYPE_F32))
     return SSD_ERR_INVALID;
-  if (B == 0 || T == 0) return SSD_OK;
-  if (!qkv || !q_out) return SSD_ERR_INVALID;
+  if (B == 0 || (T == 0 && block_tables && seq_lens)) return SSD_OK;
+  if (!block_tables || !seq_lens || !qkv || !q_out) return SSD_ERR_INVALID;
   if (!kv8_aligned(qkv) || !kv8_aligned(q_out) || !kv8_aligned(rope_cos) || !kv8_aligned(rope_sin))
     return SSD_ERR_UNSUPPORTED;
   const size_t es = dtype == SSD_DTYPE_BF16 ? 2 : 4;
@@ -440,10 +438,9 @@ extern "C" int ssd_kv8_gather(ssd_stream_t stream, const void* pages, const floa
                               const int32_t* block_tables, int max_blocks, const int32_t* positions, void* k, void* v,
                               int dtype, int B, int N) {
   if (int rc = kv8_check(pages, scales, num_layers, num_blocks, block_size, num_kv_heads, head_dim, layer)) return rc;
-  if (B < 0 || N < 0 || max_blocks <= 0 || !block_tables || (dtype != SSD_DTYPE_BF16 && dtype != SSD_DTYPE_F32))
-    return SSD_ERR_INVALID;
-  if (B == 0 || N == 0) return SSD_OK;
-  if (!positions || !k || !v) return SSD_ERR_INVALID;
+  if (B < 0 || N < 0 || max_blocks <= 0 || (dtype != SSD_DTYPE_BF16 && dtype != SSD_DTYPE_F32)) return SSD_ERR_INVALID;
+  if (B == 0 || (N == 0 && block_tables)) return SSD_OK;
+  if (!block_tables || !positions || !k || !v) return SSD_ERR_INVALID;
   if (!kv8_aligned(k) || !kv8_aligned(v)) return SSD_ERR_UNSUPPORTED;
   const int64_t rows = (int64_t)B * N;
   const Kv8Cache c = kv8_cache(const_cast<void*>(pages), const_cast<float*>(scales), num_layers, num_blocks,

@@ -1784,10 +1784,10 @@ extern "C" int ssd_kv8_attention(ssd_stream_t stream, const void* q, const void*
                                  int num_heads, int max_seq_len, void* workspace, size_t workspace_bytes) {
   if (int rc = kv8_check(pages, scales, num_layers, num_blocks, block_size, num_kv_heads, head_dim, layer)) return rc;
   if (B < 0 || T < 0 || num_heads <= 0 || num_heads % num_kv_heads || max_blocks <= 0 || max_seq_len <= 0 ||
-      !block_tables || !seq_lens || (dtype != SSD_DTYPE_BF16 && dtype != SSD_DTYPE_F32))
+      (dtype != SSD_DTYPE_BF16 && dtype != SSD_DTYPE_F32))
     return SSD_ERR_INVALID;
-  if (B == 0 || T == 0) return SSD_OK;
-  if (!q || !out || (int64_t)max_blocks * block_size < max_seq_len) return SSD_ERR_INVALID;
+  if (B == 0 || (T == 0 && block_tables && seq_lens)) return SSD_OK;  // arrays of nothing may have no address
+  if (!block_tables || !seq_lens || !q || !out || (int64_t)max_blocks * block_size < max_seq_len) return SSD_ERR_INVALID;
   if (!kv8_aligned(q) || !kv8_aligned(out) ||
       (int64_t)max_blocks * block_size > 0x7fffffff || max_seq_len > kMaxSeqLen)
     return SSD_ERR_UNSUPPORTED;

@@ -248,3 +248,23 @@ def test_attention_at_its_bounds(cuda, case):
     p, q, ql = _attention_inputs(case, seed=hq * d + t + bs)
     r = ref.attention(q, p.vals, p.exps, p.tables, lens, ql, 1 / math.sqrt(d))
     _near(_run(p, q, lens, ql, dtype)[0], r, p, dtype)
+
+
+@pytest.mark.parametrize("b,t", [(0, 3), (0, 0), (2, 0)])
+def test_calls_on_nothing(cuda, b, t):
+    from ssd_b200.kernels.kv8_cache import KV8CacheState, append_kv8, gather_kv8, paged_kv8_attention, rope_append_kv8
+
+    torch, _ = _torch()
+    cache = KV8CacheState.allocate(1, 4, 16, 2, 64)
+    table, lens = torch.zeros((b, 3), dtype=torch.int32, device="cuda"), torch.zeros(b, dtype=torch.int32, device="cuda")
+    x = torch.zeros((b, t, 2, 64), device="cuda").bfloat16()
+    before = cache.pages.view(torch.uint8).clone()
+    append_kv8(cache, 0, table, lens, x, x)
+    cos = torch.ones((8, 32), device="cuda")
+    qkv = torch.zeros((b * t, 8 * 64), device="cuda").bfloat16()
+    assert rope_append_kv8(qkv, cache, 0, table, lens, 4, cos, cos).shape == (b, t, 4, 64)
+    at = torch.zeros((b, t), dtype=torch.int32, device="cuda")
+    assert gather_kv8(cache, 0, table, at)[0].shape == (b, t, 2, 64)
+    q = torch.zeros((b, t, 4, 64), device="cuda").bfloat16()
+    assert paged_kv8_attention(q, cache, 0, table, lens).shape == q.shape
+    assert torch.equal(cache.pages.view(torch.uint8), before)

@@ -15,3 +15,20 @@ def test_workspace_goes_by_the_type():
     for shape in ((1, 5, 4, 2, 64, 1000), (8, 5, 16, 16, 256, 4096), (4, 64, 8, 1, 256, 8192), (1, 1, 8, 1, 256, 137)):
         assert either(*shape) == max(size(d, *shape) for d in (SSD_DTYPE_BF16, SSD_DTYPE_F32))
     assert size(2, 1, 5, 4, 2, 64, 1000) == size(0, 1, 5, 4, 3, 64, 1000) == size(0, 1, 5, 4, 2, 64, (1 << 30) + 1) == 0
+
+
+def test_batches_of_nothing_have_no_addresses():
+    """An empty tensor's pointer is NULL: B = 0 and T = 0 do nothing all the same."""
+    from ssd_b200._lib import lib
+
+    so, P = lib(), 4096
+    for b, t, table, rows in ((0, 3, None, None), (0, 0, None, None), (2, 0, P, None)):
+        assert so.ssd_kv8_append(None, P, P, 2, 8, 16, 2, 64, 0, table, 4, table, None, rows, rows, 0, b, t) == 0
+        assert so.ssd_kv8_rope_append(None, rows, rows, P, P, 0, 2, 8, 16, 4, 2, 64, 0, table, 4, table, None, P, P, 64, b,
+                                      t) == 0
+        assert so.ssd_kv8_gather(None, P, P, 2, 8, 16, 2, 64, 0, table, 4, rows, rows, rows, 0, b, t) == 0
+        assert so.ssd_kv8_attention(None, rows, P, P, 0, 2, 8, 16, 2, 64, 0, table, 4, table, None, rows, 0.1, b, t, 4, 64,
+                                    None, 0) == 0
+    # with sequences, their arrays have to be there
+    assert so.ssd_kv8_append(None, P, P, 2, 8, 16, 2, 64, 0, None, 4, P, None, None, None, 0, 2, 0) == 1
+    assert so.ssd_kv8_attention(None, P, P, P, 0, 2, 8, 16, 2, 64, 0, P, 4, None, None, P, 0.1, 1, 1, 4, 64, None, 0) == 1
