@@ -366,7 +366,8 @@ int ssd_page_copy(ssd_stream_t stream, const void* src_pages, const float* src_s
  *   free_list_out, free_top_out  num_blocks - U free blocks, handed out from U upwards
  *   tables_out [B, max_blocks]   tables under the new ids: remap[tables[b][i]] for i < lens[b], else -1
  *                                (B = 0: none); a second set for the draft's tables
- * The *_out arrays may be the inputs themselves.  Pages do not change: ssd_page_copy with the moves
+ * The *_out arrays may be the inputs themselves; the two table sets may then share no entry, which would be
+ * mapped twice.  Pages do not change: ssd_page_copy with the moves
  * carries the plan out, once for each cache of the pool.
  */
 int ssd_page_compact(ssd_stream_t stream, const int32_t* free_list, const int32_t* free_top,

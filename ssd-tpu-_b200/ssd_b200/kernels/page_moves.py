@@ -57,6 +57,12 @@ def copy_pages(cache, src: torch.Tensor, dst: torch.Tensor, dst_cache=None):
     return out
 
 
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two contiguous tensors share memory."""
+    (a0, a1), (b0, b1) = ((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in (a, b))
+    return max(a0, b0) < min(a1, b1)
+
+
 @dataclass
 class Compaction:
     """State of a pool after ``compact_pages``: what the arguments became, and the blocks' new ids."""
@@ -95,8 +101,8 @@ def compact_pages(cache, tables: torch.Tensor, lens: torch.Tensor, ref_counts: t
         raise ValueError(f"free_list must be int32, got {free_list.dtype}")
     if tables.dim() != 2 or (draft_tables is not None and draft_tables.dim() != 2):
         raise ValueError("tables are [rows, max_blocks]")
-    if inplace and draft_tables is not None and draft_tables.data_ptr() == tables.data_ptr() and tables.numel():
-        raise ValueError("tables and draft_tables are the same memory: in place, they would be mapped twice")
+    if inplace and draft_tables is not None and _overlap(tables, draft_tables):
+        raise ValueError("tables and draft_tables share memory: in place, entries would be mapped twice")
     half = max(1, nb // 2)
     work = free_list.new_empty((nb + 2 * half + 1,))  # new ids; the moves' sources, targets, number
     remap = work[:nb]

@@ -262,7 +262,8 @@ def test_calls_on_nothing(cuda, b, t):
     append_kv8(cache, 0, table, lens, x, x)
     cos = torch.ones((8, 32), device="cuda")
     qkv = torch.zeros((b * t, 8 * 64), device="cuda").bfloat16()
-    assert rope_append_kv8(qkv, cache, 0, table, lens, 4, cos, cos).shape == (b, t, 4, 64)
+    # tokens a sequence are told from the rows: none without sequences
+    assert rope_append_kv8(qkv, cache, 0, table, lens, 4, cos, cos).shape == (b, t if b else 0, 4, 64)
     at = torch.zeros((b, t), dtype=torch.int32, device="cuda")
     assert gather_kv8(cache, 0, table, at)[0].shape == (b, t, 2, 64)
     q = torch.zeros((b, t, 4, 64), device="cuda").bfloat16()

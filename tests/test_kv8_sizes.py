@@ -32,3 +32,19 @@ def test_batches_of_nothing_have_no_addresses():
     # with sequences, their arrays have to be there
     assert so.ssd_kv8_append(None, P, P, 2, 8, 16, 2, 64, 0, None, 4, P, None, None, None, 0, 2, 0) == 1
     assert so.ssd_kv8_attention(None, P, P, P, 0, 2, 8, 16, 2, 64, 0, P, 4, None, None, P, 0.1, 1, 1, 4, 64, None, 0) == 1
+
+
+def test_compaction_in_place_refuses_tables_that_share_entries():
+    """Also where only some rows are the same memory; views side by side are fine (and refused for want of a GPU)."""
+    import pytest
+    import torch
+
+    from ssd_b200.kernels.kv8_cache import KV8CacheState
+    from ssd_b200.kernels.page_moves import compact_pages
+
+    cache = KV8CacheState.allocate(1, 8, 16, 1, 64, device="cpu")
+    z = lambda *s: torch.zeros(s, dtype=torch.int32)  # noqa: E731
+    base = z(6, 4)
+    for a, b, why in ((base[:3], base[2:], "share"), (base[1:5], base[2:3], "share"), (base[:3], base[3:], "on a GPU")):
+        with pytest.raises(ValueError, match=why):
+            compact_pages(cache, a, z(a.shape[0]), z(8), z(8), z(1), b, z(b.shape[0]), inplace=True)
