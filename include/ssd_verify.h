@@ -280,8 +280,12 @@ int ssd_paged_verify_attention(ssd_stream_t stream, const void* q, const void* p
  * seq_lens[b] - q_lens[b] + t, seq_lens counting the new tokens -- the positions
  * ssd_kv8_attention gives them.  k, v [B, T, Hkv, D] in `dtype`.
  * A page whose first row is among the new ones starts over.  In any other page the rows before
- * the new ones keep their values: where a new row needs a larger scale they are rewritten under
- * it (exactly, but for values below 2^-14 of the page's largest).  Rows behind the last new one
+ * the new ones keep their values: where a new row needs a larger scale 2^e they are rewritten under
+ * it, exactly but for values below 2^-6 2^e (e4m3's subnormals, up to 2^-13.8 of that row's largest),
+ * which round once more to multiples of 2^-9 2^e.  A scale never shrinks before its page starts over:
+ * rows that are appended and then rejected (the next call's positions begin before them) leave it as
+ * large as they needed it, for the rows before and behind them.  In all a value x of a page is off by at
+ * most 2^-4 |x| + 2^-9 2^e, e the page's exponent.  Rows behind the last new one
  * keep their bytes.  A page written by the call belongs to one sequence; positions below 0, past
  * max_blocks pages, or whose table entry is no block are skipped.
  */
@@ -292,7 +296,7 @@ int ssd_kv8_append(ssd_stream_t stream, void* pages, float* scales, int num_laye
 
 /*
  * The same from a QKV projection's rows, qkv [B*T, (Hq+2Hkv)*D], with RoPE as ssd_rope_kv_write
- * applies it: rotated q to q_out [B*T, Hq, D] (zeros for t >= q_lens[b]), rotated k and v into the
+ * applies it: rotated q to q_out [B*T, Hq, D] (zeros for t >= q_lens[b]), k (rotated) and v into the
  * pages with one rounding.  rope_cos, rope_sin [rope_max_pos, D/2] fp32.
  */
 int ssd_kv8_rope_append(ssd_stream_t stream, const void* qkv, void* q_out, void* pages, float* scales, int dtype,

@@ -3,8 +3,8 @@
 // pages  [2][L][NB][BS][Hkv][D] e4m3, scales [2][L][NB][Hkv] fp32: element = byte value * scale of its
 // (plane, layer, page, head).  Every scale is a power of two, so dividing by it is exact, an e4m3 value
 // keeps its four significant bits whatever the scale, and a page whose scale has to grow is rewritten
-// without rounding again (but for values that fall among e4m3's subnormals, below 2^-14.8 of the page's
-// largest).
+// without rounding again, but for values that fall among e4m3's subnormals: below 2^-6 of the scale, hence at most
+// 2^-13.8 of the largest value that the page has held.
 #pragma once
 #include <cuda_fp16.h>
 #include <cuda_fp8.h>

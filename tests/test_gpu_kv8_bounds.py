@@ -269,3 +269,41 @@ def test_calls_on_nothing(cuda, b, t):
     q = torch.zeros((b, t, 4, 64), device="cuda").bfloat16()
     assert paged_kv8_attention(q, cache, 0, table, lens).shape == q.shape
     assert torch.equal(cache.pages.view(torch.uint8), before)
+
+
+@pytest.mark.parametrize("dtype,bs,hkv,d", [("bf16", 16, 2, 64), ("f32", 16, 1, 256), ("bf16", 7, 2, 128)])
+@pytest.mark.parametrize("outlier", [2.0 ** 6, 2.0 ** 12, 2.0 ** 30])
+def test_rows_beside_a_rejected_one(cuda, dtype, bs, hkv, d, outlier):
+    """A draft row far larger than the others is appended, rejected (the length goes back) and other rows follow.  The
+    page keeps the scale that it needed until its first row is appended again: its rows, earlier and later, are off by
+    their own rounding, 2^-4 of a value at most, and by less than 2^-9 2^e in all (each growth to an exponent e_i
+    rounds at most half a step 2^-10 2^e_i more, the e_i rise to e).  The pages beside it are not touched."""
+    from ssd_b200.kernels.kv8_cache import gather_kv8
+
+    torch, _ = _torch()
+    rng = np.random.default_rng(41)
+    p = Pool(rng, 2, bs, hkv, d, cols=-(-48 // bs))
+    x = _round(rng.standard_normal((2, 48, hkv, d)), dtype)
+    n = 2 * bs + 3  # the accepted length, inside the third page
+    p.append([n, n], x[:, :n], x[:, :n], [n, n], dtype)
+    top = np.abs(x).max()
+    for step in (1.0, 4.0, outlier):  # the scale grows more than once
+        draft = x[:, n:n + 2].copy()
+        draft[:, 1] = _round(step * draft[:, 1], dtype)
+        top = max(top, np.abs(draft).max())
+        p.append([n + 2, n + 2], draft, draft, [2, 2], dtype)
+        p.check()
+    p.append([n + 4, n + 4], x[:, n:n + 4], x[:, n:n + 4], [4, 4], dtype)  # rejected: other rows in its place
+    p.check()
+    e = np.ceil(np.log2(top / 448))
+    pos = np.arange(n + 4)
+    got = gather_kv8(p.cache, 1, p.dev_tables, _i(np.tile(pos, (2, 1))), dtype=torch.float32)
+    hurt = pos // bs == n // bs
+    for g in got:
+        off = np.abs(g.double().cpu().numpy() - x[:, pos])
+        assert (off <= 2.0 ** -4 * np.abs(x[:, pos]) + 2.0 ** -9 * 2.0 ** e).all()
+        own = np.ceil(np.log2(np.abs(x).max() / 448))
+        assert (off <= 2.0 ** -4 * np.abs(x[:, pos]) + 2.0 ** -9 * 2.0 ** own)[:, ~hurt].all()
+    q = _round(rng.standard_normal((2, 3, 2 * hkv, d)), dtype)
+    r = ref.attention(q, p.vals, p.exps, p.tables, [n + 4] * 2, [3, 3], 1 / math.sqrt(d))
+    _near(_run(p, q, [n + 4] * 2, [3, 3], dtype)[0], r, p, dtype)
