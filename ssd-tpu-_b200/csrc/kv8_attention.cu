@@ -919,6 +919,10 @@ constexpr int THREADS = SOFT + CONV + 32;
 constexpr int kMinTiles = 2; // of a split
 constexpr int META = 4;      // tiles whose scales are kept: a tile's are read until its weights are done
 constexpr uint32_t kPolls = 1u << 24;
+// Stands in a scale's place for a position without a row: a NaN of no computation.  No flag of its own and no change of
+// sign, since the scales are not touched before their tile is converted (touching them where they are fetched costs the
+// loads' latency: 41 -> 46 us for 4 sequences of 500 to 4000 positions, 16 heads of 256, 64 rows each).
+constexpr uint32_t kNoRow = 0xffc0a5e1u;
 __device__ uint32_t gave_up;  // 1 once a CTA's wait ran out (ssd_kv8_attention_status)
 
 template <int D>
@@ -1483,7 +1487,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_many_kernel(const Kv
     const int64_t rs = (int64_t)a.c.hkv * D;
     int blk[NB], off[NB];        // of the tile to be fetched next
     uint4 kb[NI], vb[NI];        // this tile's bytes, then the next one's as soon as they are converted: they have two
-    float ks[NB], vs[NB];        // tiles' time to arrive; and the scales (-1: no row)
+    uint32_t ks[NB], vs[NB];     // tiles' time to arrive; and the bits of the scales (kNoRow: no row)
     int ids = -1;          // UNI: lane x has the block id of the warp's positions in its tile 32 k + x
     auto look = [&](int j) {
       if constexpr (UNI) {
@@ -1515,11 +1519,11 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_many_kernel(const Kv
       }
     };
     // load tile j's K (plane 0) or V rows and scales (zeros where there is no row)
-    auto fetch = [&](int j, int plane, uint4* x, float* xs) {
-      const float* from = sc + plane * a.c.scale_plane;
+    auto fetch = [&](int j, int plane, uint4* x, uint32_t* xs) {
+      const uint32_t* from = reinterpret_cast<const uint32_t*>(sc + plane * a.c.scale_plane);
 #pragma unroll
       for (int i = 0; i < NB; ++i)
-        xs[i] = (unsigned)blk[i] < (unsigned)a.c.num_blocks ? fabsf(ld_act(from + (int64_t)blk[i] * a.c.hkv)) : -1.f;
+        xs[i] = (unsigned)blk[i] < (unsigned)a.c.num_blocks ? ld_act(from + (int64_t)blk[i] * a.c.hkv) : kNoRow;
       if constexpr (UNI) {
         const bool in = (unsigned)blk[0] < (unsigned)a.c.num_blocks;
         const uint8_t* s = kp + plane * a.c.plane + (in ? ((int64_t)blk[0] * a.c.block_size + off[0] + rr) * rs : 0);
@@ -1566,7 +1570,8 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_many_kernel(const Kv
       if (UNI ? lane == 0 : pc == 0) {
 #pragma unroll
         for (int i = 0; i < NB; ++i)
-          mt[UNI ? cw : 16 * cw + rr + i * RPI] = ks[i] < 0.f ? 0u : pack_meta(scale_exponent(ks[i]), scale_exponent(vs[i]));
+          mt[UNI ? cw : 16 * cw + rr + i * RPI] =
+              ks[i] == kNoRow ? 0u : pack_meta(scale_exponent(__uint_as_float(ks[i])), scale_exponent(__uint_as_float(vs[i])));
       }
 #pragma unroll
       for (int i = 0; i < NI; ++i) put(kt, i, kb[i]);
