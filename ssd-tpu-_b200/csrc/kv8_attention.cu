@@ -56,7 +56,8 @@ __device__ __forceinline__ int partials_of(const Kv8Attn& a, int b, int head, in
   return splits_of(min(min(ld_act(a.seq_lens + b), a.max_blocks * a.c.block_size), a.nsplit * a.split), a.split);
 }
 
-// out = sum_s e^(m_s - M) o_s / sum_s e^(n_s - N) l_s * e^(M - N), M and N the largest m_s and n_s.  One CTA per
+// out = sum_s e^(m_s - M) o_s / sum_s e^(n_s - N) l_s * e^(M - N), M and N the largest m_s and n_s.  The last factor is
+// applied as its square root, twice: M - N, about V's exponent less 7 to 15, may lie below fp32's.  One CTA per
 // query row: its threads hold 4 dims of every SG-th split each and add the groups up in order, so that the
 // loads of many splits are in flight at once.  LOG2: the maxima are in powers of two.  Bound by latency: two dependent
 // reads, 2 to 3 us of a call.
@@ -134,12 +135,12 @@ __global__ void __launch_bounds__(kJoinThreads) kv8_join_kernel(const Kv8Attn a)
       const float4 p = part[x][tid];
       o.x += p.x; o.y += p.y; o.z += p.z; o.w += p.w;
     }
-    const float f = ex(M - N);
+    const float f = ex(0.5f * (M - N));
     T* out = reinterpret_cast<T*>(a.out) + (((int64_t)b * a.T + t) * a.hq + head * a.G + g) * D + tid * 4;
-    out[0] = from_f<T>(real ? o.x / L * f : 0.f);
-    out[1] = from_f<T>(real ? o.y / L * f : 0.f);
-    out[2] = from_f<T>(real ? o.z / L * f : 0.f);
-    out[3] = from_f<T>(real ? o.w / L * f : 0.f);
+    out[0] = from_f<T>(real ? o.x / L * f * f : 0.f);
+    out[1] = from_f<T>(real ? o.y / L * f * f : 0.f);
+    out[2] = from_f<T>(real ? o.z / L * f * f : 0.f);
+    out[3] = from_f<T>(real ? o.w / L * f * f : 0.f);
   }
 }
 
@@ -205,13 +206,13 @@ __global__ void __launch_bounds__(128) kv8_join_few_kernel(const Kv8Attn a, int6
   }
   L = warp_sum(L);
   const bool real = t < ql && L != 0.f;
-  const float k = ex(M - N);
+  const float k = ex(0.5f * (M - N));
   T* out = reinterpret_cast<T*>(a.out) + (((int64_t)b * a.T + t) * a.hq + head * a.G + g) * D;
 #pragma unroll
   for (int i = 0; i < PL; ++i) {
     if (DQ < 32 && lane >= DQ) continue;
-    T y[4] = {from_f<T>(real ? o[i].x / L * k : 0.f), from_f<T>(real ? o[i].y / L * k : 0.f),
-              from_f<T>(real ? o[i].z / L * k : 0.f), from_f<T>(real ? o[i].w / L * k : 0.f)};
+    T y[4] = {from_f<T>(real ? o[i].x / L * k * k : 0.f), from_f<T>(real ? o[i].y / L * k * k : 0.f),
+              from_f<T>(real ? o[i].z / L * k * k : 0.f), from_f<T>(real ? o[i].w / L * k * k : 0.f)};
     T* to = out + (i * 32 + lane) * 4;
     if constexpr (sizeof(T) == 2)
       *reinterpret_cast<uint2*>(to) = *reinterpret_cast<uint2*>(y);
@@ -874,11 +875,11 @@ __global__ void __launch_bounds__(kFewWarps * 32, NT == 1 ? 3 : 2) kv8_attention
       }
       if (a.nsplit == 1) {
         const float4 z = fin_s[8 * nt + r];
-        const float k = ex2(z.x - z.y);
+        const float k = ex2(0.5f * (z.x - z.y));  // twice, as in the join
         const bool ok = p >= 0 && z.z != 0.f;
         *reinterpret_cast<__nv_bfloat162*>(reinterpret_cast<bf16*>(a.out) +
                                            (((int64_t)b * a.T + t) * a.hq + head * a.G + (gr - t * a.G)) * D + d) =
-            __floats2bfloat162_rn(ok ? O.x / z.z * k : 0.f, ok ? O.y / z.z * k : 0.f);
+            __floats2bfloat162_rn(ok ? O.x / z.z * k * k : 0.f, ok ? O.y / z.z * k * k : 0.f);
       } else {
         *reinterpret_cast<float2*>(a.ws_o + ((grp * a.nsplit + split) * R + 8 * nt + r) * D + d) = O;
       }
@@ -1414,7 +1415,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_many_kernel(const Kv
     } else if (!partial || tiles > 0) {
       // O through the shared memory of K, V and P (every product is done): a thread puts its half row there and
       // sends it off with one bulk copy
-      const float k = partial ? 1.f : any ? ex2(M - N) / l : 0.f;
+      const float kk = partial ? 1.f : any ? ex2(0.5f * (M - N)) : 0.f, k = partial ? 1.f : any ? kk / l : 0.f;
       const bool zero = !partial && !any;  // O may be anything where a row sees nothing
       constexpr int HD = D / 2;
       const uint32_t mine = sm + r * C::PITCH + half * (HD * 4);
@@ -1438,8 +1439,8 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_many_kernel(const Kv
             uint32_t z[4];
 #pragma unroll
             for (int h = 0; h < 4; ++h) {
-              const __nv_bfloat162 v2 = __floats2bfloat162_rn(__uint_as_float(y[i + 2 * h]) * k,
-                                                              __uint_as_float(y[i + 2 * h + 1]) * k);
+              const __nv_bfloat162 v2 = __floats2bfloat162_rn(__uint_as_float(y[i + 2 * h]) * k * kk,
+                                                              __uint_as_float(y[i + 2 * h + 1]) * k * kk);
               z[h] = zero ? 0u : *reinterpret_cast<const uint32_t*>(&v2);
             }
             sts128(mine + c * 2 + i * 2, make_uint4(z[0], z[1], z[2], z[3]));

@@ -307,3 +307,19 @@ def test_rows_beside_a_rejected_one(cuda, dtype, bs, hkv, d, outlier):
     q = _round(rng.standard_normal((2, 3, 2 * hkv, d)), dtype)
     r = ref.attention(q, p.vals, p.exps, p.tables, [n + 4] * 2, [3, 3], 1 / math.sqrt(d))
     _near(_run(p, q, [n + 4] * 2, [3, 3], dtype)[0], r, p, dtype)
+
+
+@pytest.mark.parametrize("hq,hkv,d,bs,t", [(8, 1, 256, 16, 3), (16, 4, 64, 16, 40), (4, 2, 128, 4, 2), (4, 2, 128, 4, 40)])
+@pytest.mark.parametrize("lens", [[450, 300], [2500, 1100]])
+def test_v_near_the_smallest_scale(cuda, hq, hkv, d, bs, t, lens):
+    """V of 2^-112 to 2^-100, page by page, under scores that spread over tens of powers of two: outputs are that small, and
+    right (bf16 and fp32 hold numbers down to 2^-126)."""
+    rng = np.random.default_rng(77)
+    p = Pool(rng, 2, bs, hkv, d, cols=-(-max(lens) // bs))
+    n = max(lens)
+    mag = np.exp2(-rng.integers(100, 113, (2, -(-n // 16), hkv)).astype(float)).repeat(16, 1)[:, :n, :, None]
+    k = _round(rng.standard_normal((2, n, hkv, d)), "bf16")
+    p.append(lens, k, _round(mag * rng.standard_normal((2, n, hkv, d)), "bf16"), lens, "bf16")
+    q = _round(4 * rng.standard_normal((2, t, hq, d)), "bf16")
+    r = ref.attention(q, p.vals, p.exps, p.tables, lens, [t] * 2, 1 / math.sqrt(d))
+    _near(_run(p, q, lens, [t] * 2)[0], r, p)
