@@ -323,3 +323,39 @@ def test_v_near_the_smallest_scale(cuda, hq, hkv, d, bs, t, lens):
     q = _round(4 * rng.standard_normal((2, t, hq, d)), "bf16")
     r = ref.attention(q, p.vals, p.exps, p.tables, lens, [t] * 2, 1 / math.sqrt(d))
     _near(_run(p, q, lens, [t] * 2)[0], r, p)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("hq,hkv,d,bs,t,lens", [(16, 16, 256, 16, 256, [256, 300]), (8, 1, 256, 16, 200, [1999]),
+                                                (6, 2, 64, 7, 33, [33, 40, 90]), (4, 4, 128, 100, 130, [131, 700]),
+                                                (3, 1, 64, 1, 5, [5, 4, 0, 77])])
+def test_rope_append_is_rotation_then_append(cuda, dtype, hq, hkv, d, bs, t, lens):
+    """Byte for byte what append_kv8 makes of the rotated rows in fp32 (products and sums rounded one by one), a whole
+    forward's rows among them; q is that rotation, rounded once."""
+    from ssd_b200.kernels.kv8_cache import KV8CacheState, append_kv8, rope_append_kv8
+
+    torch, dts = _torch()
+    g = torch.Generator(device="cuda").manual_seed(t + d)
+    b, cols = len(lens), -(-max(lens) // bs)
+    ql = [t if i % 2 == 0 else max(t - 3, 0) for i in range(b)]
+    perm = torch.randperm(b * cols, generator=g, device="cuda")
+    table = perm.to(torch.int32).view(b, cols)
+    caches = [KV8CacheState.allocate(1, b * cols, bs, hkv, d) for _ in range(2)]
+    old = torch.randn((b, max(lens), hkv, d), generator=g, device="cuda") * 0.3
+    before = [max(n - m, 0) for n, m in zip(lens, ql)]
+    for c in caches:
+        append_kv8(c, 0, table, _i(before), old, old, q_lens=_i(before))
+    qkv = torch.randn((b * t, (hq + 2 * hkv) * d), generator=g, device="cuda").to(dts[dtype])
+    ang = torch.arange(max(lens) + 1, device="cuda")[:, None] * torch.exp(-torch.arange(d // 2, device="cuda") / 9)[None]
+    cos, sin = ang.cos(), ang.sin()
+    q = rope_append_kv8(qkv, caches[0], 0, table, _i(lens), hq, cos, sin, q_lens=_i(ql))
+    x = qkv.float().view(b, t, hq + 2 * hkv, d)
+    pos = (torch.tensor(lens, device="cuda") - torch.tensor(ql, device="cuda"))[:, None] + torch.arange(t, device="cuda")
+    real = (torch.arange(t, device="cuda")[None] < torch.tensor(ql, device="cuda")[:, None]) & (pos >= 0)
+    cc, ss = (a[pos.clamp(0, max(lens))][:, :, None] for a in (cos, sin))
+    lo, hi = x[:, :, :hq + hkv, :d // 2], x[:, :, :hq + hkv, d // 2:]
+    y = torch.cat([lo * cc - hi * ss, hi * cc + lo * ss], -1)
+    append_kv8(caches[1], 0, table, _i(lens), y[:, :, hq:], x[:, :, hq + hkv:], q_lens=_i(ql))
+    assert torch.equal(caches[0].pages.view(torch.uint8), caches[1].pages.view(torch.uint8))
+    assert torch.equal(caches[0].scales, caches[1].scales)
+    assert torch.equal(q, (y[:, :, :hq] * real[:, :, None, None]).to(dts[dtype]))

@@ -65,3 +65,32 @@ def test_decoders_with_group_of_one(comm, cuda):
 def _batched(dec, prompts):
     first = [dec.admit(i, p) for i, p in enumerate(prompts)]
     return first, [dec.step() for _ in range(4)]
+
+
+def test_a_rank_reports_waits_that_ran_out(cuda):
+    """The status that ends a generate call holds the 8-bit attention's, once."""
+    from ssd_b200._lib import lib
+    from ssd_b200.kernels.kv8_cache import KV8CacheState, append_kv8, paged_kv8_attention
+    from ssd_b200.runtime.rank_group import LocalRank
+
+    rank = LocalRank({"target_model_path": None, "draft_model_path": None, "use_toy_model": True, "seed": 0,
+                      "draft_seed": 1, "max_model_len": 64, "kv_cache_dtype": "fp8", "local_draft": False,
+                      "target_adapter": False}, 0)
+    try:
+        cache = KV8CacheState.allocate(1, 4, 16, 1, 64)
+        table = torch.arange(4, dtype=torch.int32, device=cuda)[None]
+        n = torch.full((1,), 40, dtype=torch.int32, device=cuda)
+        q = torch.randn((1, 40, 2, 64), device=cuda).bfloat16()
+        append_kv8(cache, 0, table, n, q[:, :, :1], q[:, :, :1])
+        rank.call("begin")
+        lib().ssd_kv8_attention_set_polls(0)
+        try:
+            paged_kv8_attention(q, cache, 0, table, n)
+        finally:
+            lib().ssd_kv8_attention_set_polls(-1)
+        assert rank.call("end") == [3]
+        rank.call("begin")
+        assert paged_kv8_attention(q, cache, 0, table, n).isfinite().all()
+        assert rank.call("end") == [0]
+    finally:
+        rank.close()
