@@ -10,8 +10,8 @@
 // One warp per (sequence, touched page, KV head, plane): the page's scale has one owner, no atomics, no barrier, and
 // the result does not depend on scheduling.  The rows stay in registers, as they came, between the maximum and the
 // rounding, all their loads in flight at once (8 KB a warp for a page of 16 rows of 256 in bf16); old rows are read
-// only when the scale grows.  Bound: HBM for prompts (4 sequences, 6000 rows of 16 heads of 256 in bf16: 147 MB in
-// 26.7 us, 5.5 TB/s; with the rows converted to fp32 before the maximum, 57 us), launch latency for single tokens
+// only when the scale grows.  Bound: HBM for prompts (4 sequences, 5500 rows of 16 heads of 256 in bf16: 135 MB in
+// 25.0 us, 5.4 TB/s; with the rows converted to fp32 before the maximum, 57 us), launch latency for single tokens
 // (2 to 4 us).
 #include <type_traits>
 
@@ -121,7 +121,7 @@ struct Rows {
 
 template <typename T, int D>
 __device__ __forceinline__ void rope_q_cta(const AppendArgs& a, int cta) {
-  // one warp per token row and CTA-strided heads: items of 16 dims
+  // one CTA a token row, its threads over the heads: items of 16 dims
   constexpr int PER = D / 16;
   const int items = a.hq * PER;
   const int64_t m = cta;
@@ -302,7 +302,8 @@ int append_common(ssd_stream_t stream, AppendArgs a, int dtype, int B, int T, in
 
 // K and V rows of positions [B][N] (-1: zeros).  A row of one position is 2 Hkv D values; a warp takes up to
 // kGatherItems * 32 groups of 8 of them (8 bytes in, 16 or 32 out, neighbouring lanes on neighbouring groups), all
-// loads in flight at once (4, 8, 16 groups a lane: 28, 25.5, 29 us).  Bound: HBM (the 6000 rows above: 147 MB, 5.8 TB/s).
+// loads in flight at once (4 or 16 groups a lane: 10 to 14 % slower).  Bound: HBM (the rows above with their pages' earlier
+// ones, 5533 of 6128 positions: 146 MB in 27.2 us, 5.4 TB/s).
 constexpr int kGatherItems = 8;
 
 template <typename T, int D>
@@ -345,7 +346,7 @@ __global__ void __launch_bounds__(256) kv8_gather_kernel(const Kv8Cache c, const
     const int plane = it >= items, j = plane ? it - items : it;
     if (it >= 2 * items) break;
     const uint32_t in[2] = {x[i].x, x[i].y};
-    asm volatile("" : "+f"(s[i]));  // keeps what follows behind the loads: interleaved with them it costs 3.5 us of 25.5
+    asm volatile("" : "+f"(s[i]));  // keeps what follows behind the loads: interleaved with them it costs 3.5 us more than 27
     const float by = stored_scale(s[i]);
     float f[8];
 #pragma unroll

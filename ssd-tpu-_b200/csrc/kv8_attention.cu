@@ -401,7 +401,7 @@ __global__ void __launch_bounds__(kCcSplit) kv8_attention_cc_kernel(const Kv8Att
 
 // ------------------------------------------------------------------ few query rows (bf16): decode and verify
 // Bound by HBM: every K and V byte of the context is read once for up to 8 NT rows (32 sequences of 2000 to 8192
-// positions, 16 heads of 256, 7 new tokens: 1.34 GB in 222 us, 6.0 TB/s; 8 sequences of 512 to 4096, 5 new tokens:
+// positions, 16 heads of 256, 5 or 7 new tokens: 1.34 GB in 222 us, 6.0 TB/s; 8 sequences of 512 to 4096, 4 or 5:
 // 152 MB in 34.7 us, 4.4 TB/s, where the CTAs of the longest sequences end last).  The transposed products
 //   S^T = K Q^T   and   O^T = V^T P^T   (m16n8k16, f16 operands, fp32 sums)
 // put the 16 positions of a tile and 16 head dims on the instruction's long side and the query rows on its
@@ -903,8 +903,8 @@ __global__ void __launch_bounds__(kFewWarps * 32, NT == 1 ? 3 : 2) kv8_attention
 //   warp 16     issues the products: S of tile j + 1 goes before O of tile j, so the weights of one tile are
 //               made while the tensor cores work on the next
 // A tile takes 2300 cycles, its products alone 1080: bound by the latency of the chain scores - maxima - weights of
-// its 8 row warps, which 17 warps and two stages do not hide (issue slots 36 % busy, tensor cores 21 %).  Four
-// sequences of 1000 to 8192 positions, 512 rows each: 27 us, 304 TFLOP/s.  Two groups of row warps that take tiles in
+// its 8 row warps, which 17 warps and two stages do not hide (issue slots 40 % busy, tensor cores 23 %).  Four
+// sequences of 1000 to 8192 positions, 512 rows each (one 344): 27 us, 307 TFLOP/s.  Two groups of row warps that take tiles in
 // turn came out no faster (their two P tiles cost as much shared memory as a third stage would).
 // All waits are bounded, and a warp's lanes give up together.  A CTA that gives up raises `gave_up`, lets its copies and
 // products end, frees its TMEM and writes NaN to the rows that it has not finished, straight to global memory: warps

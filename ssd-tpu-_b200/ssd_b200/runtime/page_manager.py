@@ -168,9 +168,11 @@ class PageManager:
     def compact(self, cache) -> torch.Tensor:
         """Move the blocks in use to the front of the pool (``page_moves.compact_pages``): tables, counts
         and free list follow in place, so captured graphs that read them stay valid.  ``cache``: the
-        cache, or every cache that uses this manager's blocks.  Returns the blocks' new ids
-        [num_blocks] (-1: free) for references held elsewhere; ``Sequence.block_table`` lists follow
-        with the sequence's next host call.  Nothing synchronises."""
+        cache, or every cache that uses this manager's blocks.  For a pool that is to shrink (its used
+        blocks copied into a smaller cache, ``copy_pages``) or whose used range is wanted in one piece;
+        attention gains nothing from it.  Returns the blocks' new ids [num_blocks] (-1: free) for
+        references held elsewhere; the ``block_table`` of a ``Sequence`` that has a slot here follows with
+        the sequence's next host call.  Nothing synchronises."""
         return compact_pages(cache, self.tables, self.lens, self.ref_counts_dev, self.free_list, self.free_top,
                              self.draft_tables, self.draft_lens, inplace=True).remap
 
