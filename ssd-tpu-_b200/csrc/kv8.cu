@@ -346,7 +346,7 @@ __global__ void __launch_bounds__(256) kv8_gather_kernel(const Kv8Cache c, const
     const int plane = it >= items, j = plane ? it - items : it;
     if (it >= 2 * items) break;
     const uint32_t in[2] = {x[i].x, x[i].y};
-    asm volatile("" : "+f"(s[i]));  // keeps what follows behind the loads: interleaved with them it costs 3.5 us more than 27
+    asm volatile("" : "+f"(s[i]));  // keeps the next line behind all loads: among them it costs 3.5 us more than 27
     const float by = stored_scale(s[i]);
     float f[8];
 #pragma unroll

@@ -904,8 +904,8 @@ __global__ void __launch_bounds__(kFewWarps * 32, NT == 1 ? 3 : 2) kv8_attention
 //               made while the tensor cores work on the next
 // A tile takes 2300 cycles, its products alone 1080: bound by the latency of the chain scores - maxima - weights of
 // its 8 row warps, which 17 warps and two stages do not hide (issue slots 40 % busy, tensor cores 23 %).  Four
-// sequences of 1000 to 8192 positions, 512 rows each (one 344): 27 us, 307 TFLOP/s.  Two groups of row warps that take tiles in
-// turn came out no faster (their two P tiles cost as much shared memory as a third stage would).
+// sequences of 1000 to 8192 positions, 512 rows each (one 344): 27 us, 307 TFLOP/s.  Two groups of row warps that take
+// tiles in turn came out no faster (their two P tiles cost as much shared memory as a third stage would).
 // All waits are bounded, and a warp's lanes give up together.  A CTA that gives up raises `gave_up`, lets its copies and
 // products end, frees its TMEM and writes NaN to the rows that it has not finished, straight to global memory: warps
 // that have not noticed may still be writing tiles where results are staged.  (A row that is finished has waited for
@@ -1572,7 +1572,8 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_many_kernel(const Kv
 #pragma unroll
         for (int i = 0; i < NB; ++i)
           mt[UNI ? cw : 16 * cw + rr + i * RPI] =
-              ks[i] == kNoRow ? 0u : pack_meta(scale_exponent(__uint_as_float(ks[i])), scale_exponent(__uint_as_float(vs[i])));
+              ks[i] == kNoRow ? 0u
+                              : pack_meta(scale_exponent(__uint_as_float(ks[i])), scale_exponent(__uint_as_float(vs[i])));
       }
 #pragma unroll
       for (int i = 0; i < NI; ++i) put(kt, i, kb[i]);

@@ -3,9 +3,10 @@
 Layout: ``pages[2, num_layers, num_blocks, block_size, num_kv_heads, head_dim]`` e4m3 (as
 ``kv_cache.KVCacheState``, plane 0 = K, plane 1 = V) and ``scales[2, num_layers, num_blocks,
 num_kv_heads]`` fp32: an element is its e4m3 value times the scale of its page and KV head.  Scales
-are powers of two, 2^-118 to 2^120 (any other value counts as the one at its exponent), so a page whose scale 2^e grows as rows are appended is rewritten without a second
-rounding (values below 2^-6 2^e aside).  A scale keeps to the largest row its page has held since its first
-row was appended, a rejected draft's included: a value x is off by at most 2^-4 |x| + 2^-9 2^e.
+are powers of two, 2^-118 to 2^120 (any other value counts as the one at its exponent), so a page whose
+scale 2^e grows as rows are appended is rewritten without a second rounding (values below 2^-6 2^e
+aside).  A scale keeps to the largest row its page has held since its first row was appended, a rejected
+draft's included: a value x is off by at most 2^-4 |x| + 2^-9 2^e.
 
 Rows enter by ``append_kv8`` / ``rope_append_kv8`` at the end of each sequence, in the order of its
 positions: a block's scale follows what has been appended to it, so there is no write at arbitrary
