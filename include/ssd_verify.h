@@ -258,6 +258,30 @@ int ssd_paged_verify_attention(ssd_stream_t stream, const void* q, const void* p
                                float scale, int B, int T, int num_heads, int max_seq_len,
                                void* workspace, size_t workspace_bytes);
 
+/*
+ * The same over rows that share prefixes (no counterpart in the reference, which decodes one sequence at a
+ * time): beams, branches or samples of one prompt after ssd_page_fork, or a batch under one system prompt.
+ *   group_starts [num_groups + 1] ascending, 0 .. B: rows group_starts[g] .. group_starts[g+1]-1 form group g
+ *   prefix_lens  [num_groups] leading positions in which a group's rows agree (0: none; any number, a partial
+ *                page that every row holds a copy of included).  They are read through the table of the group's
+ *                first row, once for as many of its rows as fit a tile
+ * Rows, positions, lengths and zero rows as in ssd_paged_verify_attention, whatever the groups: a row sees the
+ * positions up to its own.  What it does not see does not reach it, infinities and NaN included; positions
+ * whose table entry is no block hold nothing.  Statistics and sums in fp32.  A row's bits depend on the rows
+ * beside it and on the lengths, by which the positions are split.  max_seq_len (at most 2^30) bounds seq_lens;
+ * B and num_groups are at most 1024, head_dim is 64, 128 or 256, q, pages, out and the workspace are 16-byte
+ * aligned (else SSD_ERR_UNSUPPORTED).  B = 0 or T = 0 does nothing.  The workspace needs no initial content and
+ * keeps none.
+ */
+size_t ssd_shared_prefix_attention_workspace_size(int dtype, int B, int T, int num_heads, int num_kv_heads,
+                                                  int head_dim, int block_size, int num_groups, int max_seq_len);
+int ssd_shared_prefix_attention(ssd_stream_t stream, const void* q, const void* pages, int dtype, int num_layers,
+                                int num_blocks, int block_size, int num_kv_heads, int head_dim, int layer,
+                                const int32_t* block_tables, int max_blocks, const int32_t* seq_lens,
+                                const int32_t* q_lens, const int32_t* group_starts, const int32_t* prefix_lens,
+                                int num_groups, void* out, float scale, int B, int T, int num_heads, int max_seq_len,
+                                void* workspace, size_t workspace_bytes);
+
 /* ------------------------------------------------------- 8-bit paged KV cache */
 /*
  * A paged cache that holds K and V in 8 bits (no counterpart in the reference, whose cache is
@@ -380,6 +404,51 @@ int ssd_page_compact(ssd_stream_t stream, const int32_t* free_list, const int32_
                      int32_t* num_moves, const int32_t* tables, int32_t* tables_out, const int32_t* lens,
                      int max_blocks, int B, const int32_t* draft_tables, int32_t* draft_tables_out,
                      const int32_t* draft_lens, int draft_max_blocks, int draft_B);
+
+/* ---------------------------------------------------------------- beam search */
+/*
+ * One step's selection for G requests of W beams (no counterpart in the reference, which decodes greedily).
+ *   logits   fp32, row g*W + w at ld * (g*W + w)
+ *   scores   [G, W] sum of log-probabilities of each beam; -inf: the beam offers nothing (before the first
+ *            step all but one beam of a request)
+ *   lengths  [G, W] tokens that each beam has generated, or NULL (0)
+ *   finished [G, W] or NULL: beams that have ended (needs eos >= 0)
+ * A live beam offers every token v at s = score + x[v] - log sum e^x, ranked by s / (length + 1)^length_penalty;
+ * a finished one offers itself, unchanged, as token eos, ranked by score / max(length, 1)^length_penalty.  The W
+ * best come out in order of rank, compared in 64 bits (within a beam in the order of its logits), ties to the
+ * lowest w * V + v.  Logits of -inf are never taken; a beam whose logits hold NaN or +inf, or nothing but -inf,
+ * offers nothing.  Places that nothing is left for: score -inf, parent and token -1, length 0, finished.
+ *   out_scores, out_parents (0 .. W-1), out_tokens [G, W]; out_lengths, out_finished [G, W] or NULL.  The
+ *   outputs may not be the inputs.  eos is -1 (none) or below V; W <= 32, G*W <= 65535 (else
+ *   SSD_ERR_UNSUPPORTED).  The workspace (16-byte aligned) needs no initial content and keeps none.
+ */
+size_t ssd_beam_select_workspace_size(int G, int W, int V);
+int ssd_beam_select(ssd_stream_t stream, const float* logits, int64_t ld, const float* scores, const int32_t* lengths,
+                    const uint8_t* finished, int eos, float length_penalty, float* out_scores, int32_t* out_parents,
+                    int32_t* out_tokens, int32_t* out_lengths, uint8_t* out_finished, void* workspace,
+                    size_t workspace_bytes, int G, int W, int V);
+
+/*
+ * Row g*W + i (i < W) becomes what row g*W + parents[g*W + i] was, in place, for the first num_tokens[row] tokens
+ * of the old rows (blocks past them are let go).  Whole blocks are shared (ref counts follow; every block in the
+ * tables has its count).  A parent's partial last block stays with the lowest-numbered of its children; every
+ * other child gets a block from the free-list top, in row order, and an entry of the copy list: copy_src,
+ * copy_dst, copy_rows [G*W] (-1, -1, 0 where there is nothing to copy), for ssd_page_copy_rows.  A partial block
+ * belongs to one row.  Blocks that no row refers to any more are pushed on the free list before, in ascending
+ * order.  A row whose parent is out of range (-1) is emptied; one that cannot get its block is emptied with
+ * ok = 0 (ok [G*W] may be NULL).  G*W <= 1024 (else SSD_ERR_UNSUPPORTED).
+ */
+int ssd_page_reorder(ssd_stream_t stream, int32_t* block_tables, int32_t* table_lens, int max_blocks,
+                     int32_t* free_list, int32_t* free_top, int32_t* ref_counts, int num_blocks,
+                     const int32_t* parents, const int32_t* num_tokens, int block_size, uint8_t* ok,
+                     int32_t* copy_src, int32_t* copy_dst, int32_t* copy_rows, int G, int W);
+
+/* Copy the first rows[i] rows (of row_bytes each) of page src_ids[i] to page dst_ids[i], i < n, in each of `planes`
+ * planes, and the page's scales where it has some (see ssd_page_copy).  Pairs with an id out of range are skipped;
+ * no page may be both copied from and copied to, nor copied to twice. */
+int ssd_page_copy_rows(ssd_stream_t stream, void* pages, float* scales, int num_blocks, int block_size, int planes,
+                       size_t row_bytes, int scales_per_page, const int32_t* src_ids, const int32_t* dst_ids,
+                       const int32_t* rows, int n);
 
 /* ------------------------------------------------------- K3: skinny projections */
 

@@ -63,6 +63,13 @@ SIGNATURES = {
     "ssd_page_copy": (_i, [_p, _p, _p, _i, _p, _p, _i, _i, _sz, _i, _p, _i64, _p, _i64, _i, _p]),
     "ssd_page_compact": (_i, [_p, _p, _p, _p, _i, _p, _p, _p, _p, _p, _p, _p, _p, _p, _p, _i, _i, _p, _p, _p, _i,
                               _i]),
+    "ssd_shared_prefix_attention_workspace_size": (_sz, [_i, _i, _i, _i, _i, _i, _i, _i, _i]),
+    "ssd_shared_prefix_attention": (_i, [_p, _p, _p, _i, _i, _i, _i, _i, _i, _i, _p, _i, _p, _p, _p, _p, _i, _p, _f,
+                                         _i, _i, _i, _i, _p, _sz]),
+    "ssd_beam_select_workspace_size": (_sz, [_i, _i, _i]),
+    "ssd_beam_select": (_i, [_p, _p, _i64, _p, _p, _p, _i, _f, _p, _p, _p, _p, _p, _p, _sz, _i, _i, _i]),
+    "ssd_page_reorder": (_i, [_p, _p, _p, _i, _p, _p, _p, _i, _p, _p, _i, _p, _p, _p, _p, _i, _i]),
+    "ssd_page_copy_rows": (_i, [_p, _p, _p, _i, _i, _i, _sz, _i, _p, _p, _p, _i]),
     "ssd_linear_workspace_size": (_sz, [_i, _i, _i]),
     "ssd_linear_max_m": (_i, []),
     "ssd_linear": (_i, [_p, _p, _p, _i, _p, _i, _i, _i, _i, _p, _sz]),

@@ -127,3 +127,42 @@ def compact_pages(cache, tables: torch.Tensor, lens: torch.Tensor, ref_counts: t
     for p in pools:
         _copy(p, p, src, 1, dst, 1, nb // 2, count)
     return out
+
+
+def reorder_pages(cache, tables: torch.Tensor, lens: torch.Tensor, ref_counts: torch.Tensor, free_list: torch.Tensor,
+                  free_top: torch.Tensor, parents: torch.Tensor, num_tokens: torch.Tensor) -> torch.Tensor:
+    """Rows follow their parents (beam search): row g*W + i becomes what row g*W + parents[g, i] was, in place.
+
+    ``tables`` [G*W, max_blocks] with ``lens``, ``ref_counts``, ``free_list`` and ``free_top`` are the arrays of
+    ``PageManager``; ``parents`` int32 [G, W] (-1: the row is emptied), ``num_tokens`` int32 [G*W] the tokens that each
+    old row holds.  Whole blocks are shared, a partial last block stays with the lowest of its parent's children and is
+    copied for the others, in ``cache`` (one cache, or a sequence of caches that share the pool's block ids); blocks
+    that no row holds any more return to the free list.  Returns ok uint8 [G*W]: 0 where no block was left for a
+    copy and the row is empty.  Nothing synchronises.  ``ssd_page_reorder`` and ``ssd_page_copy_rows``.
+    """
+    pools = [_pool(c) for c in cache] if isinstance(cache, (list, tuple)) else [_pool(cache)]
+    if not pools:
+        raise ValueError("reorder_pages wants a cache")
+    dev, nb = pools[0][0], pools[0][3]
+    bs = pools[0][7][1]
+    if any(p[0] != dev or p[3] != nb or p[7][1] != bs for p in pools):
+        raise ValueError("the caches of one pool have the same blocks, block size and device")
+    if any(p[5] > _MAX_PAGE for p in pools):  # before the tables change: the copies would be refused
+        raise ValueError(f"a page of one plane may hold {_MAX_PAGE} bytes at most")
+    if parents.dim() != 2 or tables.dim() != 2:
+        raise ValueError(f"parents are [G, W] and tables [G*W, max_blocks], got {list(parents.shape)} and {list(tables.shape)}")
+    g, w = parents.shape
+    n, cols = tables.shape
+    if n != g * w:
+        raise ValueError(f"{list(parents.shape)} parents do not fit {n} rows")
+    work = parents.new_empty((3, max(n, 1)))  # the copies: sources, targets, rows
+    ok = parents.new_empty((n,), dtype=torch.uint8)
+    src, step = work.data_ptr(), 4 * max(n, 1)
+    launch("ssd_page_reorder", dev, ints(tables, (n, cols), "tables", dev), ints(lens, (n,), "lens", dev), cols,
+           ints(free_list, (nb,), "free_list", dev), ints(free_top, (1,), "free_top", dev),
+           ints(ref_counts, (nb,), "ref_counts", dev), nb, ints(parents, (g, w), "parents", dev),
+           ints(num_tokens, (n,), "num_tokens", dev), bs, ok.data_ptr(), src, src + step, src + 2 * step, g, w)
+    for _, pages, scales, _, planes, nbytes, nscales, _ in pools:
+        launch("ssd_page_copy_rows", dev, pages, scales, nb, bs, planes, nbytes // bs, nscales, src, src + step,
+               src + 2 * step, n)
+    return ok
