@@ -282,6 +282,17 @@ int ssd_shared_prefix_attention(ssd_stream_t stream, const void* q, const void* 
                                 int num_groups, void* out, float scale, int B, int T, int num_heads, int max_seq_len,
                                 void* workspace, size_t workspace_bytes);
 
+/*
+ * bf16 over pages of whole runs of 16 rows: the kernel's warps wait for one another inside a CTA, each wait for a
+ * bounded number of polls.  A CTA whose wait runs out leaves NaN in the rows that it has not finished; the call
+ * itself has long returned SSD_OK.  ssd_shared_prefix_attention_status waits for `stream` and returns
+ * SSD_ERR_TIMEOUT if that has happened on the current device since it last said so, else SSD_OK.  Not for captured
+ * streams.  ssd_shared_prefix_attention_set_polls sets the polls of each wait for later calls of this process (-1:
+ * the default, 2^24, some seconds).
+ */
+int ssd_shared_prefix_attention_status(ssd_stream_t stream);
+int ssd_shared_prefix_attention_set_polls(int polls);
+
 /* ------------------------------------------------------- 8-bit paged KV cache */
 /*
  * A paged cache that holds K and V in 8 bits (no counterpart in the reference, whose cache is

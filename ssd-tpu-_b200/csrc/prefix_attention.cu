@@ -15,6 +15,8 @@
 #include <algorithm>
 
 #include "kv8.cuh"
+#include "linear.cuh"
+#include "tcgen05.cuh"
 
 namespace ssd {
 namespace {
@@ -35,6 +37,8 @@ struct PrefixAttn {
   int R;                 // query rows of a sequence and KV head: G * T
   int spt, tps;          // sequences of a row tile (R <= its rows), else tiles of a sequence
   int tiles;             // bound on the row tiles of all groups
+  int num_layers, layer_no;
+  uint32_t polls;        // of each device-side wait
   int nsplit;            // parts of a tile's list (CUDA-core kernel)
   float* ws_o;           // [part][row][D] unnormalised sums
   float2* ws_ml;         // [part][row] what they are relative to, sum of weights
@@ -322,6 +326,694 @@ __global__ void __launch_bounds__(kChunkC) prefix_attention_cc_kernel(const Pref
   }
 }
 
+// ------------------------------------------------------------------ tensor-core kernel (bf16, pages of 16 k rows)
+// Persistent CTAs, one an SM, share out the positions of all row tiles and KV heads in equal runs of 16 (units), so
+// a CTA works through one or more segments: a run of units of one tile and head.  128 query rows (TMEM lanes) a tile:
+//   S = Q K^T   for TILE positions (M = 128, N = TILE), Q from TMEM, K as it lies in the pages (K-major)
+//   O += P V    (N = D), P in bf16 from the TMEM columns of its own S, V as it lies in the pages (MN-major)
+// A unit is 16 rows of one page, so a tile of positions mixes pages of any kind, the prefix's and tails of different
+// sequences; which rows see which of its positions is said by 16 bytes a unit.  Rows that see nothing of a unit put
+// zero weights on it: that wastes products, of which there are enough, and saves bytes, of which there are not.
+//   warps 0-7   two threads a query row, half a tile's positions each: scores out of TMEM, maxima (exchanged between
+//               the two), weights, rescaling of O (only when a row's reference has to move), the result
+//   warp 8      walks the tables and fetches units by TMA into a ring of stages, K and V in turn
+//   warp 9      issues the products: S of tile j + 1 goes before O of tile j, so the weights of one tile are made
+//               while the tensor cores work on the next
+// A product with weight zero still spreads infinities and NaN of V over rows that do not see them.  Then a row's O is
+// not finite although its sum of weights is, and the row is worked out again by itself, from the pages.
+// All waits are bounded, and a warp's lanes give up together.  A CTA that gives up raises `gave_up`, lets its copies and
+// products end, frees its TMEM and leaves NaN in the rows that it has not finished.
+namespace tile {
+
+constexpr int ROWS = 128;              // query rows of a CTA: TMEM lanes
+constexpr int SOFT = 256;              // threads of the row warps
+constexpr int THREADS = SOFT + 64;
+constexpr int META = 8;                // tiles whose units are described: more than there are between fetch and use
+constexpr int kMaxTiles = 1024;
+constexpr int kMinUnits = 8;           // of a CTA: shorter runs cost more in prologues and joins than they save
+constexpr float kSpan = 8.f;           // weights are at most 2^8
+constexpr uint32_t kPolls = 1u << 24;
+__device__ uint32_t gave_up;           // 1 once a CTA's wait ran out
+
+template <int D>
+struct Cfg {
+  static constexpr int TILE = D == 256 ? 64 : 128, UNITS = TILE / 16, STAGES = 6;
+  static constexpr uint32_t KV = TILE * D * 2;  // bytes of a stage: one tile's K or V
+  static constexpr uint32_t ring = STAGES * KV;
+  static constexpr uint32_t pref = ring;                              // int [kMaxTiles + 1]: units before each tile
+  static constexpr uint32_t info = pref + 4 * (kMaxTiles + 4);        // int2 [kMaxTiles]
+  static constexpr uint32_t cum = info + 8 * kMaxTiles;               // int [ROWS + 4]: units before a sequence's tail
+  static constexpr uint32_t meta = cum + 4 * (ROWS + 4);              // int4 [META][UNITS]
+  static constexpr uint32_t pairs = meta + 16 * META * UNITS;         // float [2][2][ROWS]: the threads' maxima
+  static constexpr uint32_t bars = pairs + 4 * 4 * ROWS;
+  static constexpr uint32_t misc = bars + 8 * (2 * STAGES + META + 12);
+  static constexpr size_t smem = 1024 + misc + 32;
+  // TMEM columns: two tiles' scores (then weights), Q (two bf16 to a column), O
+  static constexpr uint32_t q_col = 2 * TILE, o_col = q_col + D / 2, tmem_cols = 512;
+  static_assert(o_col + D <= tmem_cols);
+  static_assert(smem <= 227 * 1024);
+  // planning, in the ring's place: group starts, their first tiles
+  static_assert(ring >= 8 * (kMaxRowsB + 1));
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+// For whole warps: true in every lane, or false in every lane.
+__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile int* stop, uint32_t polls) {
+  bool ok = false;
+  for (uint32_t i = 0; i < polls; ++i) {
+    ok = tc::mbar_try_wait(bar, parity);
+    if (ok || ((i & 255u) == 255u && *stop)) break;
+  }
+  if (!ok) *stop = 1;
+  return __all_sync(0xffffffffu, ok);
+}
+// bf16 operands, fp32 accumulator, M = 128; B's long side contiguous (MN-major) or not.
+template <int N, bool B_MN>
+__host__ __device__ constexpr uint32_t idesc() {
+  return (1u << 4) | (1u << 7) | (1u << 10) | ((B_MN ? 1u : 0u) << 16) | ((uint32_t)(N >> 3) << 17) |
+         ((uint32_t)(ROWS >> 4) << 24);
+}
+__device__ __forceinline__ void tma_rows(uint32_t dst, const CUtensorMap* map, uint32_t bar, int chunk, int head,
+                                         int row) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::
+          "r"(dst), "l"(map), "r"(bar), "r"(0), "r"(chunk), "r"(head), "r"(row)
+      : "memory");
+}
+
+// A run of units of one tile and head.
+struct Segment {
+  int tile, head, lo, hi;   // units [lo, hi) of the tile's list
+  int slot;                 // of partials; -1: the whole list, straight to the output
+  RowTile rows;
+};
+// The CTA's run of all units, segment by segment.  `pref`: units before each tile (one head).
+struct Walk {
+  int64_t pos, end;
+  int tile;
+  __device__ Walk(const PrefixAttn& a, const int* pref, int tiles, int ctas) : tile(0) {
+    const int64_t all = (int64_t)pref[tiles] * a.hkv;
+    pos = all * blockIdx.x / ctas;
+    end = (int)blockIdx.x < ctas ? all * (blockIdx.x + 1) / ctas : pos;
+    int n = tiles;
+    while (n > 1) {  // the last tile that starts at or before pos
+      const int half = n / 2;
+      if ((int64_t)pref[tile + half] * a.hkv <= pos) tile += half, n -= half;
+      else n = half;
+    }
+  }
+  __device__ bool next(const PrefixAttn& a, const int* pref, const int2* info, Segment& s) {
+    if (pos >= end) return false;
+    while ((int64_t)pref[tile + 1] * a.hkv <= pos) ++tile;
+    const int units = pref[tile + 1] - pref[tile];
+    const int64_t off = pos - (int64_t)pref[tile] * a.hkv;
+    s.tile = tile;
+    s.head = (int)(off / units);
+    s.lo = (int)(off - (int64_t)s.head * units);
+    s.hi = (int)min((int64_t)units, s.lo + (end - pos));
+    s.slot = s.lo == 0 && s.hi == units ? -1 : s.lo > 0 ? 2 * (int)blockIdx.x : 2 * (int)blockIdx.x + 1;
+    pos += s.hi - s.lo;
+    const int2 t = info[tile];
+    s.rows.seq0 = t.x & 0xffff;
+    s.rows.nseq = a.tps > 1 ? 1 : t.x >> 16;
+    s.rows.part = a.tps > 1 ? t.x >> 16 : 0;
+    s.rows.group = t.y & 0xffff;
+    s.rows.first = t.y >> 16;
+    return true;
+  }
+};
+
+// Units of the prefix and of a sequence's tail (which begins with the unit that holds position P, if that is a part).
+__device__ __forceinline__ int prefix_units(int P) { return (P + 15) / 16; }
+__device__ __forceinline__ int tail_units(const PrefixAttn& a, int b, int P) {
+  if (new_tokens(a, b) <= 0) return 0;
+  const int seq = min(ld_act(a.seq_lens + b), a.cap);
+  return seq > P ? (seq + 15) / 16 - P / 16 : 0;
+}
+
+// Row r of the segment once more, alone: dims [d0, d0 + D / 2) of sum_j w_j v_j over the positions that it sees, weights
+// as the tensor cores had them.  For whole warps.
+template <int D>
+__device__ __noinline__ void row_again(const PrefixAttn& a, const Segment& sg, int seq, int pos, int64_t at, float c,
+                                       float M, int d0, float k, float* to_f32, bf16* to_bf16) {
+  constexpr int PL = D / 32, HL = D / 64;
+  const int lane = threadIdx.x & 31;
+  const bf16* pages = reinterpret_cast<const bf16*>(a.pages) + a.layer;
+  const int P = prefix_of(a, sg.rows.group);
+  float q[PL], o[HL];
+#pragma unroll
+  for (int i = 0; i < PL; ++i) {
+    q[i] = to_f(ld_act(reinterpret_cast<const bf16*>(a.q) + at + lane + 32 * i));
+    if (a.scale < 0.f) q[i] = -q[i];
+  }
+#pragma unroll
+  for (int i = 0; i < HL; ++i) o[i] = 0.f;
+  int before = prefix_units(P);  // units before the sequence's tail
+  for (int i = 0; i < seq; ++i) before += tail_units(a, sg.rows.seq0 + i, P);
+  const int own = tail_units(a, sg.rows.seq0 + seq, P);
+  const int end = min(min(ld_act(a.seq_lens + sg.rows.seq0 + seq), a.cap), pos + 1);
+  for (int pass = 0; pass < 2; ++pass) {
+    const int first = pass ? before : 0, n = pass ? own : prefix_units(P);
+    const int row = pass ? sg.rows.seq0 + seq : sg.rows.first;
+    for (int u = max(sg.lo, first); u < min(sg.hi, first + n); ++u) {
+      const int p0 = 16 * (u - first + (pass ? P / 16 : 0));
+      for (int j = max(p0, pass ? P : 0); j < min(p0 + 16, pass ? end : min(P, pos + 1)); ++j) {
+        const int blk = ld_act(a.tables + (int64_t)row * a.max_blocks + j / a.block_size);
+        if ((unsigned)blk >= (unsigned)a.num_blocks) continue;
+        const bf16* kr = pages + (((int64_t)blk * a.block_size + j % a.block_size) * a.hkv + sg.head) * D;
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < PL; ++i) s = fmaf(q[i], to_f(ld_act(kr + lane + 32 * i)), s);
+        const float w = round_bf16(ex2(fmaf(warp_sum(s), c, -M)));
+#pragma unroll
+        for (int i = 0; i < HL; ++i) o[i] = fmaf(w, to_f(ld_act(kr + a.plane + d0 + lane + 32 * i)), o[i]);
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < HL; ++i) {
+    if (to_f32) to_f32[d0 + lane + 32 * i] = o[i];
+    else to_bf16[d0 + lane + 32 * i] = __float2bfloat16_rn(o[i] * k);
+  }
+}
+
+template <int D>
+__global__ void __launch_bounds__(THREADS, 1)
+prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const PrefixAttn a) {
+  using C = Cfg<D>;
+  constexpr int TILE = C::TILE, UNITS = C::UNITS, HALF = TILE / 2;
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = tc::smem_u32(smem_raw), sm = (raw + 1023u) & ~1023u;
+  uint8_t* gen = smem_raw + (sm - raw);
+  int* pref = reinterpret_cast<int*>(gen + C::pref);
+  int2* info = reinterpret_cast<int2*>(gen + C::info);
+  int* cum = reinterpret_cast<int*>(gen + C::cum);
+  int4* meta = reinterpret_cast<int4*>(gen + C::meta);
+  float* pair_s = reinterpret_cast<float*>(gen + C::pairs);
+  auto bar = [&](int i) { return sm + C::bars + 8 * i; };
+  auto full = [&](int s) { return bar(s); };
+  auto freed = [&](int s) { return bar(C::STAGES + s); };
+  auto meta_full = [&](int s) { return bar(2 * C::STAGES + s); };
+  constexpr int B0 = 2 * C::STAGES + META;
+  auto s_full = [&](int s) { return bar(B0 + s); };
+  auto p_full = [&](int s) { return bar(B0 + 2 + s); };
+  const uint32_t o_done = bar(B0 + 4), q_tmem = bar(B0 + 5), drained = bar(B0 + 6);
+  auto pair = [&](int q) { return bar(B0 + 8 + q); };
+  uint32_t* slot = reinterpret_cast<uint32_t*>(gen + C::misc);
+  volatile int* stop = reinterpret_cast<volatile int*>(slot + 1);
+  auto held = [&](uint32_t b, uint32_t parity) { return wait(b, parity, stop, a.polls); };
+
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (tid == 0) {
+    for (int s = 0; s < C::STAGES; ++s) {
+      tc::mbar_init(full(s), 1);
+      tc::mbar_init(freed(s), 1);
+    }
+    for (int s = 0; s < META; ++s) tc::mbar_init(meta_full(s), 1);
+    for (int s = 0; s < 2; ++s) {
+      tc::mbar_init(s_full(s), 1);
+      tc::mbar_init(p_full(s), SOFT / 32);
+    }
+    tc::mbar_init(o_done, 1);
+    tc::mbar_init(q_tmem, SOFT / 32);
+    tc::mbar_init(drained, 1);
+    for (int q = 0; q < 4; ++q) tc::mbar_init(pair(q), 2);
+    *stop = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&map) : "memory");
+  }
+  if (warp == THREADS / 32 - 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc::smem_u32(slot)),
+                 "r"(C::tmem_cols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  pdl_wait();
+  pdl_trigger();
+
+  // ---------------------------------------------------------------- the tiles and their units
+  {
+    int* g_start = reinterpret_cast<int*>(gen);           // [groups + 1]
+    int* g_tile = reinterpret_cast<int*>(gen) + kMaxRowsB + 1;
+    for (int i = tid; i < a.tiles; i += THREADS) {
+      pref[1 + i] = 0;
+      info[i] = make_int2(0, 0);
+    }
+    for (int g = tid; g <= a.groups; g += THREADS) g_start[g] = clamped(ld_act(a.starts + g), a.B);
+    __syncthreads();
+    if (warp == 0) {
+      int before = 0;
+      for (int g0 = 0; g0 < a.groups; g0 += 32) {
+        const int g = g0 + lane, n = g < a.groups ? group_tiles(a, g_start[g + 1] - g_start[g]) : 0;
+        int incl = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int y = __shfl_up_sync(0xffffffffu, incl, o);
+          if (lane >= o) incl += y;
+        }
+        if (g < a.groups) g_tile[g] = before + incl - n;
+        before += __shfl_sync(0xffffffffu, incl, 31);
+      }
+    }
+    __syncthreads();
+    for (int b = tid; b < a.B; b += THREADS) {
+      int g = 0, n = a.groups;
+      while (n > 1) {  // the last group that starts at or before b
+        const int half = n / 2;
+        if (g_start[g + half] <= b) g += half, n -= half;
+        else n = half;
+      }
+      const int s = g_start[g], e = g_start[g + 1];
+      if (b < s || b >= e) continue;  // starts that are not ascending from 0 to B
+      const int P = prefix_of(a, g), tail = tail_units(a, b, P), k = b - s;
+      const int t0 = g_tile[g] + (a.tps > 1 ? k * a.tps : k / a.spt);
+      const bool lead = a.tps > 1 || k % a.spt == 0;
+      for (int p = 0; p < a.tps; ++p) {
+        if (t0 + p >= a.tiles) break;
+        atomicAdd(&pref[1 + t0 + p], tail + (lead ? prefix_units(P) : 0));
+        if (lead) info[t0 + p] = make_int2(b | (a.tps > 1 ? p : min(a.spt, e - b)) << 16, g | s << 16);
+      }
+      if (blockIdx.x == 0) a.place[b] = make_int2(t0, a.tps > 1 ? 0 : k % a.spt);
+    }
+    __syncthreads();
+    if (warp == 0) {
+      int before = 0;
+      if (lane == 0) pref[0] = 0;
+      for (int t0 = 0; t0 < a.tiles; t0 += 32) {
+        const int t = t0 + lane, n = t < a.tiles ? pref[1 + t] : 0;
+        int incl = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int y = __shfl_up_sync(0xffffffffu, incl, o);
+          if (lane >= o) incl += y;
+        }
+        if (t < a.tiles) {
+          pref[1 + t] = before + incl;
+          if (n == 0 && blockIdx.x == 0)  // rows that see nothing: the join writes their zeros
+            for (int h = 0; h < a.hkv; ++h) a.plan[t * a.hkv + h] = make_int2(0, 0);
+        }
+        before += __shfl_sync(0xffffffffu, incl, 31);
+      }
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the ring was written by threads
+  }
+  tc::tc_fence_before();
+  __syncthreads();
+  tc::tc_fence_after();
+  const uint32_t tmem = *slot;
+  const int64_t all = (int64_t)pref[a.tiles] * a.hkv;
+  const int ctas = (int)max((int64_t)1, min((int64_t)gridDim.x, (all + kMinUnits - 1) / kMinUnits));
+  Walk walk(a, pref, a.tiles, ctas);
+  Segment sg;
+  const float c = fmaxf(fabsf(a.scale) * 1.4426950408889634f, 1e-38f);  // not 0: keeps the mask's infinity an infinity
+  int jg = 0;  // tiles before this segment
+
+  if (warp < SOFT / 32) {
+    // -------------------------------------------------------------- rows
+    const int quad = warp & 3, half = warp >> 2;  // TMEM lanes 32 quad .., positions HALF half .. of a tile
+    const int r = quad * 32 + lane;
+    const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16);
+    int swaps = 0;
+    bool ok = true;
+    // the row's two threads swap a number; false when the CTA gives up
+    auto swap = [&](float& x) {
+      float* at = pair_s + (swaps & 1) * 2 * ROWS;
+      at[half * ROWS + r] = x;
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(pair(quad));
+      if (!held(pair(quad), swaps & 1)) return false;
+      x = at[(half ^ 1) * ROWS + r];
+      ++swaps;
+      return true;
+    };
+    for (int seg = 0; walk.next(a, pref, info, sg); ++seg) {
+      const int tiles = (sg.hi - sg.lo + UNITS - 1) / UNITS;
+      const RowAt w = row_at<D>(a, sg.rows, sg.head, r, ROWS);
+      if (sg.lo == 0 && tid == 0) {  // where the tile's parts are
+        const int units = pref[sg.tile + 1] - pref[sg.tile];
+        const int64_t last = (int64_t)pref[sg.tile] * a.hkv + (int64_t)(sg.head + 1) * units - 1;
+        const int c1 = (int)(((last + 1) * ctas - 1) / all);
+        a.plan[sg.tile * a.hkv + sg.head] = make_int2(2 * (int)blockIdx.x + 1, c1 - (int)blockIdx.x + 1);
+      }
+      const bool real = w.pos >= 0;
+      const bool busy = __any_sync(0xffffffffu, real);
+      if (ok) {
+        // this thread's half of its row of Q into TMEM
+        constexpr int NQ = D / 16;  // 16-byte pieces
+        uint4 x[NQ];
+#pragma unroll
+        for (int i = 0; i < NQ; ++i)
+          x[i] = real ? ld_act_v4(reinterpret_cast<const bf16*>(a.q) + w.at + half * (D / 2) + 8 * i)
+                      : make_uint4(0, 0, 0, 0);
+        const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
+#pragma unroll
+        for (int i = 0; i < NQ; i += 4) {
+          uint32_t y[16];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            y[4 * k] = x[i + k].x ^ flip;
+            y[4 * k + 1] = x[i + k].y ^ flip;
+            y[4 * k + 2] = x[i + k].z ^ flip;
+            y[4 * k + 3] = x[i + k].w ^ flip;
+          }
+          tc::tmem_store16(lanes + C::q_col + half * (D / 4) + 4 * i, y);
+        }
+        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+        tc::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(q_tmem);
+      }
+      // M: what the weights are relative to; -1e38 where nothing has been seen
+      float M = -1e38f, l = 0.f;
+#pragma unroll 1
+      for (int j = 0; ok && j < tiles; ++j) {
+        const int jt = jg + j, buf = jt & 1;
+        ok = held(s_full(buf), (jt >> 1) & 1) && held(meta_full(jt % META), (jt / META) & 1);
+        if (!ok) break;
+        tc::tc_fence_after();
+        if (busy) {
+          uint32_t x[HALF];
+#pragma unroll
+          for (int i = 0; i < HALF; i += 32) tc::tmem_load32(lanes + buf * TILE + half * HALF + i, x + i);
+          // which of this thread's positions its row sees
+          uint32_t see[HALF / 32];
+          const int4* mt = meta + (jt % META) * UNITS + half * (UNITS / 2);
+          bool all_seen = true, none = true;
+#pragma unroll
+          for (int u = 0; u < UNITS / 2; ++u) {
+            const int4 m = mt[u];  // first position, positions from, to, whose (-1: every row's)
+            const int to = min(min(m.z, w.pos + 1) - m.x, 16), from = max(m.y - m.x, 0);
+            uint32_t bits = to > from ? (0xffffu >> (16 - to)) & (0xffffu << from) : 0u;
+            if (m.w >= 0 && m.w != w.seq) bits = 0;
+            if (u & 1) see[u >> 1] |= bits << 16;
+            else see[u >> 1] = bits;
+          }
+#pragma unroll
+          for (int i = 0; i < HALF / 32; ++i) {
+            all_seen &= see[i] == 0xffffffffu;
+            none &= see[i] == 0;
+          }
+          all_seen = __all_sync(0xffffffffu, all_seen);
+          none = __all_sync(0xffffffffu, none);
+#pragma unroll
+          for (int i = 0; i < HALF; i += 32) tc::tmem_ready(x + i);
+          float m = -INFINITY;
+          if (!none) {
+            if (!all_seen) {
+#pragma unroll
+              for (int i = 0; i < HALF; ++i)
+                if (!(see[i / 32] >> (i % 32) & 1)) x[i] = 0xff800000u;
+            }
+            float m2 = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < HALF; i += 4) {
+              m = fmaxf(m, fmaxf(__uint_as_float(x[i]), __uint_as_float(x[i + 1])));
+              m2 = fmaxf(m2, fmaxf(__uint_as_float(x[i + 2]), __uint_as_float(x[i + 3])));
+            }
+            m = fmaxf(m, m2);
+          }
+          m = fmaxf(m * c, -1e38f);  // a NaN score counts as the lowest value here and spoils the sums
+          float mo = m, f = 1.f;
+          ok = swap(mo);
+          if (!ok) break;
+          m = fmaxf(m, mo);
+          if (m > M + kSpan) {
+            f = ex2(M - m);
+            M = m;
+            l *= f;
+          }
+          uint32_t p[HALF / 2];
+          if (none) {
+#pragma unroll
+            for (int i = 0; i < HALF / 2; ++i) p[i] = 0;
+          } else {
+            float2 s0 = make_float2(0.f, 0.f), s1 = s0;
+            const float2 c2 = make_float2(c, c), o2 = make_float2(-M, -M);
+#pragma unroll
+            for (int i = 0; i < HALF; i += 4) {
+              float2 e = tc::fma2(make_float2(__uint_as_float(x[i]), __uint_as_float(x[i + 1])), c2, o2);
+              float2 d = tc::fma2(make_float2(__uint_as_float(x[i + 2]), __uint_as_float(x[i + 3])), c2, o2);
+              e = make_float2(ex2(e.x), ex2(e.y));
+              d = make_float2(ex2(d.x), ex2(d.y));
+              s0 = tc::add2(s0, e);
+              s1 = tc::add2(s1, d);
+              p[i / 2] = pack_bf16(e.x, e.y);
+              p[i / 2 + 1] = pack_bf16(d.x, d.y);
+            }
+            l += (s0.x + s0.y) + (s1.x + s1.y);
+          }
+          if constexpr (HALF == 32) tc::tmem_store16(lanes + buf * TILE + half * (HALF / 2), p);
+          else tc::tmem_store32(lanes + buf * TILE + half * (HALF / 2), p);
+          if (j > 0 && __any_sync(0xffffffffu, f != 1.f)) {  // half of O each, once the tile before has been added
+            ok = held(o_done, (jt - 1) & 1);
+            if (!ok) break;
+            tc::tc_fence_after();
+#pragma unroll 1
+            for (int i = half * (D / 2); i < (half + 1) * (D / 2); i += 32) {
+              uint32_t y[32];
+              tc::tmem_load32(lanes + C::o_col + i, y);
+              tc::tmem_ready(y);
+#pragma unroll
+              for (int k = 0; k < 32; ++k) y[k] = __float_as_uint(__uint_as_float(y[k]) * f);
+              tc::tmem_store32(lanes + C::o_col + i, y);
+            }
+          }
+          asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+        }
+        tc::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(p_full(buf));
+      }
+      if (ok && busy) {
+        float lo = l;
+        ok = swap(lo);
+        l += lo;
+      }
+      ok = ok && held(o_done, (jg + tiles - 1) & 1);
+      tc::tc_fence_after();
+      jg += tiles;
+      const float nan = __int_as_float(0x7fc00000);
+      const bool direct = sg.slot < 0;
+      const int64_t po = (int64_t)max(sg.slot, 0) * ROWS + r;
+      if (!direct && half == 0) a.ws_ml[po] = make_float2(M, !real ? 0.f : ok ? l : nan);
+      bf16* out = reinterpret_cast<bf16*>(a.out) + w.at;
+      if (!ok) {
+        if (lane == 0) atomicExch(&gave_up, 1u);
+        if (direct && w.at >= 0)
+#pragma unroll 1
+          for (int d = half * (D / 2); d < (half + 1) * (D / 2); ++d) out[d] = __float2bfloat16_rn(real ? nan : 0.f);
+        continue;
+      }
+      const bool any = real && l != 0.f;  // l is NaN, not 0, where a seen score is
+      const float k = any ? 1.f / l : 0.f;
+      bool odd = false;
+#pragma unroll 1
+      for (int d = half * (D / 2); d < (half + 1) * (D / 2); d += 32) {
+        uint32_t y[32];
+        if (busy) {
+          tc::tmem_load32(lanes + C::o_col + d, y);
+          tc::tmem_ready(y);
+        }
+        float t = 0.f;
+        if (any) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) t += fabsf(__uint_as_float(y[i]));
+          odd |= !(t <= FLT_MAX);
+        }
+        if (direct) {
+          if (w.at >= 0) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 8) {
+              uint32_t z[4];
+#pragma unroll
+              for (int h = 0; h < 4; ++h)
+                z[h] = any ? pack_bf16(__uint_as_float(y[i + 2 * h]) * k, __uint_as_float(y[i + 2 * h + 1]) * k) : 0u;
+              *reinterpret_cast<uint4*>(out + d + i) = make_uint4(z[0], z[1], z[2], z[3]);
+            }
+          }
+        } else if (any) {
+          float* to = a.ws_o + po * D + d;
+#pragma unroll
+          for (int i = 0; i < 32; i += 4)
+            *reinterpret_cast<uint4*>(to + i) = make_uint4(y[i], y[i + 1], y[i + 2], y[i + 3]);
+        }
+      }
+      // rows that V's infinities or NaN have reached: seen ones come out as they are, others are taken out
+      for (uint32_t left = __ballot_sync(0xffffffffu, odd && l == l); left; left &= left - 1) {
+        const int from = __ffs(left) - 1;
+        const int64_t at = __shfl_sync(0xffffffffu, w.at, from), pr = __shfl_sync(0xffffffffu, po, from);
+        row_again<D>(a, sg, __shfl_sync(0xffffffffu, w.seq, from), __shfl_sync(0xffffffffu, w.pos, from), at, c,
+                     __shfl_sync(0xffffffffu, M, from), half * (D / 2), __shfl_sync(0xffffffffu, k, from),
+                     direct ? nullptr : a.ws_o + pr * D, direct ? reinterpret_cast<bf16*>(a.out) + at : nullptr);
+      }
+      tc::tc_fence_before();
+    }
+  } else if (warp == SOFT / 32) {
+    // -------------------------------------------------------------- pages
+    const int64_t rows_plane = (int64_t)a.num_layers * a.num_blocks * a.block_size;
+    const int64_t row_layer = (int64_t)a.layer_no * a.num_blocks * a.block_size;
+    int n = 0;        // stages filled
+    bool ok = true;
+    for (int seg = 0; ok && walk.next(a, pref, info, sg); ++seg) {
+      const int tiles = (sg.hi - sg.lo + UNITS - 1) / UNITS;
+      const int P = prefix_of(a, sg.rows.group), pu = prefix_units(P);
+      int before = pu;
+      for (int i0 = 0; i0 < sg.rows.nseq; i0 += 32) {
+        const int i = i0 + lane, t = i < sg.rows.nseq ? tail_units(a, sg.rows.seq0 + i, P) : 0;
+        int incl = t;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int y = __shfl_up_sync(0xffffffffu, incl, o);
+          if (lane >= o) incl += y;
+        }
+        if (i < sg.rows.nseq) cum[i] = before + incl - t;
+        before += __shfl_sync(0xffffffffu, incl, 31);
+      }
+      __syncwarp();
+      // units of a batch of tiles, a lane each: where their rows are, and who sees them
+      constexpr int BATCH = 32 / UNITS;
+      int vrow[2] = {0, 0};  // rows of this lane's unit, of this batch and of the one before
+      auto look = [&](int j0) {
+        const int u = sg.lo + j0 * UNITS + lane;
+        int4 m = make_int4(0, 0, 0, -1);
+        int row = 0;
+        if (u < sg.hi) {
+          int owner = -1, from = sg.rows.first, p0 = 16 * u, lo = 0, hi = P;
+          if (u >= pu) {
+            owner = 0;
+            for (int step = sg.rows.nseq; step > 1;) {  // the last sequence whose tail starts at or before u
+              const int hf = step / 2;
+              if (cum[owner + hf] <= u) owner += hf, step -= hf;
+              else step = hf;
+            }
+            from = sg.rows.seq0 + owner;
+            p0 = 16 * (P / 16 + u - cum[owner]);
+            lo = P;
+            hi = min(ld_act(a.seq_lens + from), a.cap);
+          }
+          const int blk = ld_act(a.tables + (int64_t)from * a.max_blocks + p0 / a.block_size);
+          if ((unsigned)blk < (unsigned)a.num_blocks) {
+            m = make_int4(p0, lo, hi, owner);
+            row = blk * a.block_size + p0 % a.block_size;
+          }
+        }
+        // units that are not there fetch the batch's first rows: finite values as a rule, and no bytes of DRAM
+        const int first = __shfl_sync(0xffffffffu, row, 0);
+        if (m.z == 0) row = first;
+        vrow[1] = vrow[0];
+        vrow[0] = row;
+        return m;
+      };
+      int4 m = look(0);
+      auto fetch = [&](int row_of_lane, int in_batch, int64_t base, int plane) {
+        const int s = n % C::STAGES;
+        if (n >= C::STAGES && !held(freed(s), (n / C::STAGES - 1) & 1)) return false;
+        if (lane == 0) tc::mbar_expect_tx(full(s), C::KV);
+        __syncwarp();
+        constexpr int CH = D / 64;
+        const int u = lane / CH, ch = lane % CH;
+        const int row = __shfl_sync(0xffffffffu, row_of_lane, (in_batch * UNITS + u) & 31);
+        if (u < UNITS)
+          tma_rows(sm + s * C::KV + ch * (TILE * 128) + u * 2048, &map, full(s), ch, sg.head,
+                   (int)(plane * rows_plane + base) + row);
+        ++n;
+        return true;
+      };
+      for (int j = 0; ok && j <= tiles; ++j) {
+        if (j < tiles) {
+          if (j > 0 && j % BATCH == 0) m = look(j);
+          const int jt = jg + j;
+          if (lane / UNITS == j % BATCH) meta[(jt % META) * UNITS + lane % UNITS] = m;
+          __syncwarp();
+          if (lane == 0) tc::mbar_arrive(meta_full(jt % META));
+          ok = fetch(vrow[0], j % BATCH, row_layer, 0);
+        }
+        if (ok && j > 0) ok = fetch(j < tiles && j % BATCH == 0 ? vrow[1] : vrow[0], (j - 1) % BATCH, row_layer, 1);
+      }
+      jg += tiles;
+    }
+    if (!ok) {  // copies in flight land before shared memory goes
+      for (int i = max(0, n - C::STAGES); i < n; ++i)
+        for (uint32_t p = 0; p < kPolls && !tc::mbar_try_wait(full(i % C::STAGES), (i / C::STAGES) & 1); ++p) {}
+    }
+    __syncwarp();
+  } else {
+    // -------------------------------------------------------------- products
+    // The whole warp walks the loop and one elected lane issues, so that addresses and descriptors stay in uniform
+    // registers.
+    uint32_t lead;
+    asm volatile("{.reg .pred p; elect.sync _|p, 0xffffffff; selp.u32 %0, 1, 0, p;}" : "=r"(lead));
+    int n = 0;
+    bool ok = true;
+    auto ready = [&](uint32_t b, uint32_t parity) {
+      const bool yes = held(b, parity);
+      tc::tc_fence_after();
+      return yes;
+    };
+    auto scores = [&](int jt) {
+      const int s = n % C::STAGES;
+      if (!ready(full(s), (n / C::STAGES) & 1)) return false;
+      const uint64_t kd = tc::sw128_desc(sm + s * C::KV);
+      if (lead) {
+#pragma unroll
+        for (int d = 0; d < D / 64; ++d)
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            tc::umma_ts(tmem + (jt & 1) * TILE, tmem + C::q_col + d * 32 + 8 * k, kd + d * ((TILE * 128) >> 4) + 2 * k,
+                        idesc<TILE, false>(), d || k);
+        tc::umma_commit(freed(s));
+        tc::umma_commit(s_full(jt & 1));
+      }
+      ++n;
+      return true;
+    };
+    for (int seg = 0; ok && walk.next(a, pref, info, sg); ++seg) {
+      const int tiles = (sg.hi - sg.lo + UNITS - 1) / UNITS;
+      ok = ready(q_tmem, seg & 1) && scores(jg);
+#pragma unroll 1
+      for (int j = 0; ok && j < tiles; ++j) {
+        const int jt = jg + j;
+        if (j + 1 < tiles) ok = scores(jt + 1);
+        const int s = n % C::STAGES;
+        ok = ok && ready(p_full(jt & 1), (jt >> 1) & 1) && ready(full(s), (n / C::STAGES) & 1);
+        if (!ok) break;
+        const uint64_t vd = tc::mn128_desc<TILE>(sm + s * C::KV);
+        if (lead) {
+#pragma unroll
+          for (int k = 0; k < TILE / 16; ++k)  // 16 positions: 8 columns of P, two groups of 8 rows of V
+            tc::umma_ts(tmem + C::o_col, tmem + (jt & 1) * TILE + 8 * k, vd + (2048 >> 4) * k, idesc<D, true>(),
+                        j || k);
+          tc::umma_commit(freed(s));
+          tc::umma_commit(o_done);
+        }
+        ++n;
+      }
+      jg += tiles;
+    }
+    if (!ok) {  // let the products issued so far end before TMEM goes back
+      if (lead) tc::umma_commit(drained);
+      for (uint32_t i = 0; i < kPolls && !tc::mbar_try_wait(drained, 0); ++i) {}
+    }
+    __syncwarp();
+  }
+  __syncthreads();
+  if (warp == THREADS / 32 - 1) {
+    tc::tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::tmem_cols) : "memory");
+  }
+}
+
+}  // namespace tile
+
 // ------------------------------------------------------------------ join
 // out = sum_i w_i o_i / sum_i w_i l_i over a row's parts, w_i = e^(m_i - M).  A warp a query row; bound by latency.
 template <typename T, int D, int ROWS, bool TC>
@@ -388,30 +1080,66 @@ __global__ void __launch_bounds__(128) prefix_join_kernel(const PrefixAttn a) {
 // ------------------------------------------------------------------ host
 inline size_t up256(size_t x) { return (x + 255) & ~size_t(255); }
 
+std::atomic<uint32_t> wait_polls{tile::kPolls};
+constexpr int kSms = 148;
+
 struct PrefixLayout {
+  bool tc;               // tensor-core kernel
   int rows;              // of a row tile
+  int ctas;
   int R, spt, tps, tiles, nsplit;
   size_t parts;          // rows of partials
   size_t off_ml, off_plan, off_place, total;
 };
 
-PrefixLayout prefix_layout(int B, int T, int hq, int hkv, int D, int groups, int max_seq_len) {
+PrefixLayout prefix_layout(int dtype, int B, int T, int hq, int hkv, int D, int block_size, int groups,
+                           int max_seq_len) {
   PrefixLayout L{};
-  L.rows = kRowsC;
   L.R = hq / hkv * T;
-  L.spt = std::max(1, L.rows / L.R);
-  L.tps = L.R > L.rows ? (L.R + L.rows - 1) / L.rows : 1;
-  // every group starts a tile of its own
-  L.tiles = L.tps > 1 ? B * L.tps : (int)std::min<int64_t>(B, (int64_t)B / L.spt + groups);
-  const int64_t ctas = (int64_t)L.tiles * hkv;
-  const int64_t chunks = ((int64_t)max_seq_len + kChunkC - 1) / kChunkC;
-  L.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>({kMaxSplitC, chunks, 592 / ctas}));
-  L.parts = L.nsplit == 1 ? 0 : (size_t)ctas * L.nsplit * L.rows;
+  auto tiles_of = [&](int rows) {
+    L.rows = rows;
+    L.spt = std::max(1, rows / L.R);
+    L.tps = L.R > rows ? (L.R + rows - 1) / rows : 1;
+    // every group starts a tile of its own
+    const int64_t n = L.tps > 1 ? (int64_t)B * L.tps : std::min<int64_t>(B, (int64_t)B / L.spt + groups);
+    L.tiles = (int)std::min<int64_t>(n, 0x7fffffff);
+  };
+  if (dtype == SSD_DTYPE_BF16 && block_size % 16 == 0) {
+    tiles_of(tile::ROWS);
+    L.tc = L.tiles <= tile::kMaxTiles;
+  }
+  if (L.tc) {
+    const int64_t units = ((int64_t)max_seq_len + 15) / 16 * ((int64_t)L.tiles + B) * hkv;
+    L.ctas = (int)std::min<int64_t>(kSms, (units + tile::kMinUnits - 1) / tile::kMinUnits);
+    L.nsplit = 0;
+    L.parts = (size_t)2 * L.ctas * L.rows;
+  } else {
+    tiles_of(kRowsC);
+    const int64_t ctas = (int64_t)L.tiles * hkv;
+    const int64_t chunks = ((int64_t)max_seq_len + kChunkC - 1) / kChunkC;
+    L.nsplit = (int)std::max<int64_t>(1, std::min<int64_t>({kMaxSplitC, chunks, 592 / ctas}));
+    L.parts = L.nsplit == 1 ? 0 : (size_t)ctas * L.nsplit * L.rows;
+  }
   L.off_ml = up256(sizeof(float) * L.parts * D);
   L.off_plan = L.off_ml + up256(sizeof(float2) * L.parts);
-  L.off_place = L.off_plan + up256(sizeof(int2) * (size_t)ctas);
+  L.off_place = L.off_plan + up256(sizeof(int2) * (size_t)L.tiles * hkv);
   L.total = L.off_place + up256(sizeof(int2) * B);
   return L;
+}
+
+template <int D>
+int launch_tc(cudaStream_t st, const PrefixAttn& a, int ctas) {
+  CUtensorMap map;
+  if (!make_kv_row_map(&map, a.pages, (int64_t)2 * a.num_layers * a.num_blocks * a.block_size, a.hkv, D))
+    return SSD_ERR_LAUNCH;
+  auto kern = tile::prefix_attention_tc_kernel<D>;
+  constexpr size_t smem = tile::Cfg<D>::smem;
+  static std::atomic<uint64_t> ready{0};
+  if (!allow_smem(ready, kern, (int)smem)) return SSD_ERR_LAUNCH;
+  SSD_PDL(kern, ctas, tile::THREADS, smem, st, map, a);
+  const int64_t rows = (int64_t)a.B * a.T * a.hq;
+  SSD_PDL((prefix_join_kernel<bf16, D, tile::ROWS, true>), (unsigned)((rows + 3) / 4), 128, 0, st, a);
+  return SSD_OK;
 }
 
 template <typename T, int D>
@@ -444,7 +1172,7 @@ extern "C" size_t ssd_shared_prefix_attention_workspace_size(int dtype, int B, i
   if (!sizes_ok(B, T, num_heads, num_kv_heads, head_dim, num_groups, max_seq_len) || block_size <= 0 ||
       (dtype != SSD_DTYPE_BF16 && dtype != SSD_DTYPE_F32))
     return 0;
-  return prefix_layout(B, T, num_heads, num_kv_heads, head_dim, num_groups, max_seq_len).total;
+  return prefix_layout(dtype, B, T, num_heads, num_kv_heads, head_dim, block_size, num_groups, max_seq_len).total;
 }
 
 extern "C" int ssd_shared_prefix_attention(ssd_stream_t stream, const void* q, const void* pages, int dtype,
@@ -464,10 +1192,11 @@ extern "C" int ssd_shared_prefix_attention(ssd_stream_t stream, const void* q, c
     return SSD_ERR_INVALID;
   if ((head_dim != 64 && head_dim != 128 && head_dim != 256) || B > kMaxRowsB || num_groups > kMaxRowsB ||
       !sizes_ok(B, T, num_heads, num_kv_heads, head_dim, num_groups, max_seq_len) || !kv8_aligned(q) ||
-      !kv8_aligned(out) || !kv8_aligned(pages) || (int64_t)num_blocks * block_size > 0x7fffffff ||
+      !kv8_aligned(out) || !kv8_aligned(pages) || (int64_t)2 * num_layers * num_blocks * block_size > 0x7fffffff ||
       num_kv_heads > 65535)
     return SSD_ERR_UNSUPPORTED;
-  const PrefixLayout L = prefix_layout(B, T, num_heads, num_kv_heads, head_dim, num_groups, max_seq_len);
+  const PrefixLayout L =
+      prefix_layout(dtype, B, T, num_heads, num_kv_heads, head_dim, block_size, num_groups, max_seq_len);
   if (L.tiles > 65535) return SSD_ERR_UNSUPPORTED;
   if (!workspace || workspace_bytes < L.total) return SSD_ERR_WORKSPACE;
   if (!kv8_aligned(workspace)) return SSD_ERR_UNSUPPORTED;
@@ -500,10 +1229,41 @@ extern "C" int ssd_shared_prefix_attention(ssd_stream_t stream, const void* q, c
   a.tps = L.tps;
   a.tiles = L.tiles;
   a.nsplit = L.nsplit;
+  a.num_layers = num_layers;
+  a.layer_no = layer;
+  a.polls = wait_polls.load(std::memory_order_relaxed);
   a.ws_o = reinterpret_cast<float*>(w);
   a.ws_ml = reinterpret_cast<float2*>(w + L.off_ml);
   a.plan = reinterpret_cast<int2*>(w + L.off_plan);
   a.place = reinterpret_cast<int2*>(w + L.off_place);
   cudaStream_t st = (cudaStream_t)stream;
+  if (L.tc)
+    return head_dim == 256   ? launch_tc<256>(st, a, L.ctas)
+           : head_dim == 128 ? launch_tc<128>(st, a, L.ctas)
+                             : launch_tc<64>(st, a, L.ctas);
   return dtype == SSD_DTYPE_BF16 ? launch_cc<bf16>(st, a, head_dim) : launch_cc<float>(st, a, head_dim);
+}
+
+extern "C" int ssd_shared_prefix_attention_status(ssd_stream_t stream) {
+  cudaStream_t st = (cudaStream_t)stream;
+  uint32_t gave_up = 0;
+  bool ok = cudaMemcpyFromSymbolAsync(&gave_up, tile::gave_up, sizeof(gave_up), 0, cudaMemcpyDeviceToHost, st) ==
+                cudaSuccess &&
+            cudaStreamSynchronize(st) == cudaSuccess;
+  if (ok && gave_up) {
+    const uint32_t none = 0;
+    ok = cudaMemcpyToSymbolAsync(tile::gave_up, &none, sizeof(none), 0, cudaMemcpyHostToDevice, st) == cudaSuccess &&
+         cudaStreamSynchronize(st) == cudaSuccess;
+  }
+  if (!ok) {
+    (void)cudaGetLastError();
+    return SSD_ERR_LAUNCH;
+  }
+  return gave_up ? SSD_ERR_TIMEOUT : SSD_OK;
+}
+
+extern "C" int ssd_shared_prefix_attention_set_polls(int polls) {
+  if (polls < -1) return SSD_ERR_INVALID;
+  wait_polls.store(polls < 0 ? tile::kPolls : (uint32_t)polls, std::memory_order_relaxed);
+  return SSD_OK;
 }

@@ -66,6 +66,8 @@ SIGNATURES = {
     "ssd_shared_prefix_attention_workspace_size": (_sz, [_i, _i, _i, _i, _i, _i, _i, _i, _i]),
     "ssd_shared_prefix_attention": (_i, [_p, _p, _p, _i, _i, _i, _i, _i, _i, _i, _p, _i, _p, _p, _p, _p, _i, _p, _f,
                                          _i, _i, _i, _i, _p, _sz]),
+    "ssd_shared_prefix_attention_status": (_i, [_p]),
+    "ssd_shared_prefix_attention_set_polls": (_i, [_i]),
     "ssd_beam_select_workspace_size": (_sz, [_i, _i, _i]),
     "ssd_beam_select": (_i, [_p, _p, _i64, _p, _p, _p, _i, _f, _p, _p, _p, _p, _p, _p, _sz, _i, _i, _i]),
     "ssd_page_reorder": (_i, [_p, _p, _p, _i, _p, _p, _p, _i, _p, _p, _i, _p, _p, _p, _p, _i, _i]),
