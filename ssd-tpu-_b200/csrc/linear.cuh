@@ -62,7 +62,7 @@ bool linear_tc_supported(int M, int N, int K);
 // TMA map over a bf16 KV cache plane stack [plane_pages][block_size][hkv][D]: box = one
 // page of one head, 64 dims wide (128-byte swizzle); D % 64 == 0.
 bool make_kv_page_map(CUtensorMap* m, const void* pages, int plane_pages, int block_size, int hkv, int D);
-bool make_kv_row_map(CUtensorMap* m, const void* pages, int64_t rows, int hkv, int D);
+bool make_kv_row_map(CUtensorMap* m, const void* base, int64_t rows, int heads, int D, int box_heads, int box_rows);
 
 // ssd_paged_verify_attention with `early`: nonzero when the previous kernel in
 // the stream writes only q and this step's new K/V rows (the decoder forward),

@@ -1178,15 +1178,15 @@ bool make_kv_page_map(CUtensorMap* m, const void* pages, int plane_pages, int bl
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-bool make_kv_row_map(CUtensorMap* m, const void* pages, int64_t rows, int hkv, int D) {
-  // the same pages as rows [rows][hkv][D] in 4-D (d % 64, d / 64, head, row): one box = 16 rows x 64 dims of one head
+bool make_kv_row_map(CUtensorMap* m, const void* base, int64_t rows, int heads, int D, int box_heads, int box_rows) {
+  // bf16 rows [rows][heads][D] in 4-D (d % 64, d / 64, head, row): one box = box_rows x box_heads x 64 dims
   tc::EncodeFn fn = tc::encode_fn();
   if (!fn || D % 64 || rows > 0x7fffffff) return false;
-  cuuint64_t dims[4] = {64, (cuuint64_t)(D / 64), (cuuint64_t)hkv, (cuuint64_t)rows};
-  cuuint64_t strides[3] = {128, (cuuint64_t)D * 2, (cuuint64_t)hkv * D * 2};
-  cuuint32_t box[4] = {64, 1, 1, 16};
+  cuuint64_t dims[4] = {64, (cuuint64_t)(D / 64), (cuuint64_t)heads, (cuuint64_t)rows};
+  cuuint64_t strides[3] = {128, (cuuint64_t)D * 2, (cuuint64_t)heads * D * 2};
+  cuuint32_t box[4] = {64, 1, (cuuint32_t)box_heads, (cuuint32_t)box_rows};
   cuuint32_t estr[4] = {1, 1, 1, 1};
-  return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(pages), dims, strides, box, estr,
+  return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, box, estr,
             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }

@@ -35,10 +35,12 @@ struct PrefixAttn {
   int B, T, hq, hkv, G, groups, num_blocks, block_size, max_blocks;
   int cap;               // positions of a sequence that may be read
   int R;                 // query rows of a sequence and KV head: G * T
+  int tile_rows;         // query rows of a row tile
   int spt, tps;          // sequences of a row tile (R <= its rows), else tiles of a sequence
   int tiles;             // bound on the row tiles of all groups
   int num_layers, layer_no;
   uint32_t polls;        // of each device-side wait
+  int q_box;             // query rows that a fetch of Q brings in
   int nsplit;            // parts of a tile's list (CUDA-core kernel)
   float* ws_o;           // [part][row][D] unnormalised sums
   float2* ws_ml;         // [part][row] what they are relative to, sum of weights
@@ -109,7 +111,8 @@ struct RowAt {
   int64_t at;            // element offset of the row
 };
 template <int D>
-__device__ __forceinline__ RowAt row_at(const PrefixAttn& a, const RowTile& tl, int head, int r, int rows) {
+__device__ __forceinline__ RowAt row_at(const PrefixAttn& a, const RowTile& tl, int head, int r, int rows,
+                                        const int* seq_s = nullptr, const int* ql_s = nullptr) {
   RowAt w;
   const int gr = tl.part * rows + r;
   w.seq = a.tps > 1 ? 0 : gr / a.R;
@@ -118,10 +121,10 @@ __device__ __forceinline__ RowAt row_at(const PrefixAttn& a, const RowTile& tl, 
   w.b = tl.seq0 + w.seq;
   w.pos = -1;
   w.at = -1;
-  if (tl.group >= 0 && w.seq < tl.nseq && in < a.R) {
+  if (tl.group >= 0 && r < rows && w.seq < tl.nseq && in < a.R) {
     w.at = (((int64_t)w.b * a.T + w.t) * a.hq + head * a.G + (in - w.t * a.G)) * D;
-    const int ql = new_tokens(a, w.b);
-    if (w.t < ql) w.pos = max(ld_act(a.seq_lens + w.b) - ql + w.t, -1);
+    const int ql = ql_s ? ql_s[w.b] : new_tokens(a, w.b);
+    if (w.t < ql) w.pos = max((seq_s ? seq_s[w.b] : ld_act(a.seq_lens + w.b)) - ql + w.t, -1);
   }
   return w;
 }
@@ -349,7 +352,7 @@ constexpr int ROWS = 128;              // query rows of a CTA: TMEM lanes
 constexpr int SOFT = 256;              // threads of the row warps
 constexpr int THREADS = SOFT + 64;
 constexpr int META = 8;                // tiles whose units are described: more than there are between fetch and use
-constexpr int kMaxTiles = 1024;
+constexpr int kMaxTiles = 512;         // also sequences and groups: their numbers are kept in shared memory
 constexpr int kMinUnits = 8;           // of a CTA: shorter runs cost more in prologues and joins than they save
 constexpr float kSpan = 8.f;           // weights are at most 2^8
 constexpr uint32_t kPolls = 1u << 24;
@@ -358,11 +361,16 @@ __device__ uint32_t gave_up;           // 1 once a CTA's wait ran out
 template <int D>
 struct Cfg {
   static constexpr int TILE = D == 256 ? 64 : 128, UNITS = TILE / 16, STAGES = 6;
+  static constexpr int QST = ROWS / TILE;       // stages that Q takes on its way in
   static constexpr uint32_t KV = TILE * D * 2;  // bytes of a stage: one tile's K or V
   static constexpr uint32_t ring = STAGES * KV;
-  static constexpr uint32_t pref = ring;                              // int [kMaxTiles + 1]: units before each tile
+  static constexpr uint32_t stage = ring;                             // float [SOFT][16]: results on their way out
+  static constexpr uint32_t pref = stage + 64 * SOFT;                 // int [kMaxTiles + 1]: units before each tile
   static constexpr uint32_t info = pref + 4 * (kMaxTiles + 4);        // int2 [kMaxTiles]
-  static constexpr uint32_t cum = info + 8 * kMaxTiles;               // int [ROWS + 4]: units before a sequence's tail
+  static constexpr uint32_t seq = info + 8 * kMaxTiles;               // int [kMaxTiles]: lengths,
+  static constexpr uint32_t ql = seq + 4 * kMaxTiles;                 // new tokens of the sequences,
+  static constexpr uint32_t pre = ql + 4 * kMaxTiles;                 // prefixes of the groups
+  static constexpr uint32_t cum = pre + 4 * kMaxTiles;                // int [ROWS + 4]: units before a sequence's tail
   static constexpr uint32_t meta = cum + 4 * (ROWS + 4);              // int4 [META][UNITS]
   static constexpr uint32_t pairs = meta + 16 * META * UNITS;         // float [2][2][ROWS]: the threads' maxima
   static constexpr uint32_t bars = pairs + 4 * 4 * ROWS;
@@ -373,13 +381,21 @@ struct Cfg {
   static_assert(o_col + D <= tmem_cols);
   static_assert(smem <= 227 * 1024);
   // planning, in the ring's place: group starts, their first tiles
-  static_assert(ring >= 8 * (kMaxRowsB + 1));
+  static_assert(ring >= 8 * (kMaxTiles + 1));
 };
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+__device__ __forceinline__ uint4 lds128(uint32_t p) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(p) : "memory");
+  return v;
+}
+__device__ __forceinline__ void sts128(uint32_t p, uint4 v) {
+  asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(p), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   uint32_t r;
@@ -454,10 +470,9 @@ struct Walk {
 
 // Units of the prefix and of a sequence's tail (which begins with the unit that holds position P, if that is a part).
 __device__ __forceinline__ int prefix_units(int P) { return (P + 15) / 16; }
-__device__ __forceinline__ int tail_units(const PrefixAttn& a, int b, int P) {
-  if (new_tokens(a, b) <= 0) return 0;
-  const int seq = min(ld_act(a.seq_lens + b), a.cap);
-  return seq > P ? (seq + 15) / 16 - P / 16 : 0;
+__device__ __forceinline__ int tail_units(const PrefixAttn& a, int seq, int ql, int P) {
+  const int n = min(seq, a.cap);
+  return ql > 0 && n > P ? (n + 15) / 16 - P / 16 : 0;
 }
 
 // Row r of the segment once more, alone: dims [d0, d0 + D / 2) of sum_j w_j v_j over the positions that it sees, weights
@@ -478,8 +493,9 @@ __device__ __noinline__ void row_again(const PrefixAttn& a, const Segment& sg, i
 #pragma unroll
   for (int i = 0; i < HL; ++i) o[i] = 0.f;
   int before = prefix_units(P);  // units before the sequence's tail
-  for (int i = 0; i < seq; ++i) before += tail_units(a, sg.rows.seq0 + i, P);
-  const int own = tail_units(a, sg.rows.seq0 + seq, P);
+  auto units = [&](int b) { return tail_units(a, ld_act(a.seq_lens + b), new_tokens(a, b), P); };
+  for (int i = 0; i < seq; ++i) before += units(sg.rows.seq0 + i);
+  const int own = units(sg.rows.seq0 + seq);
   const int end = min(min(ld_act(a.seq_lens + sg.rows.seq0 + seq), a.cap), pos + 1);
   for (int pass = 0; pass < 2; ++pass) {
     const int first = pass ? before : 0, n = pass ? own : prefix_units(P);
@@ -508,7 +524,8 @@ __device__ __noinline__ void row_again(const PrefixAttn& a, const Segment& sg, i
 
 template <int D>
 __global__ void __launch_bounds__(THREADS, 1)
-prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const PrefixAttn a) {
+prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ CUtensorMap qmap,
+                           const PrefixAttn a) {
   using C = Cfg<D>;
   constexpr int TILE = C::TILE, UNITS = C::UNITS, HALF = TILE / 2;
   extern __shared__ uint8_t smem_raw[];
@@ -516,6 +533,9 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const Prefix
   uint8_t* gen = smem_raw + (sm - raw);
   int* pref = reinterpret_cast<int*>(gen + C::pref);
   int2* info = reinterpret_cast<int2*>(gen + C::info);
+  int* seq_s = reinterpret_cast<int*>(gen + C::seq);
+  int* ql_s = reinterpret_cast<int*>(gen + C::ql);
+  int* pre_s = reinterpret_cast<int*>(gen + C::pre);
   int* cum = reinterpret_cast<int*>(gen + C::cum);
   int4* meta = reinterpret_cast<int4*>(gen + C::meta);
   float* pair_s = reinterpret_cast<float*>(gen + C::pairs);
@@ -563,12 +583,19 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const Prefix
   // ---------------------------------------------------------------- the tiles and their units
   {
     int* g_start = reinterpret_cast<int*>(gen);           // [groups + 1]
-    int* g_tile = reinterpret_cast<int*>(gen) + kMaxRowsB + 1;
+    int* g_tile = reinterpret_cast<int*>(gen) + kMaxTiles + 1;
     for (int i = tid; i < a.tiles; i += THREADS) {
       pref[1 + i] = 0;
       info[i] = make_int2(0, 0);
     }
-    for (int g = tid; g <= a.groups; g += THREADS) g_start[g] = clamped(ld_act(a.starts + g), a.B);
+    for (int b = tid; b < a.B; b += THREADS) {
+      seq_s[b] = ld_act(a.seq_lens + b);
+      ql_s[b] = new_tokens(a, b);
+    }
+    for (int g = tid; g <= a.groups; g += THREADS) {
+      g_start[g] = clamped(ld_act(a.starts + g), a.B);
+      if (g < a.groups) pre_s[g] = prefix_of(a, g);
+    }
     __syncthreads();
     if (warp == 0) {
       int before = 0;
@@ -594,7 +621,7 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const Prefix
       }
       const int s = g_start[g], e = g_start[g + 1];
       if (b < s || b >= e) continue;  // starts that are not ascending from 0 to B
-      const int P = prefix_of(a, g), tail = tail_units(a, b, P), k = b - s;
+      const int P = pre_s[g], tail = tail_units(a, seq_s[b], ql_s[b], P), k = b - s;
       const int t0 = g_tile[g] + (a.tps > 1 ? k * a.tps : k / a.spt);
       const bool lead = a.tps > 1 || k % a.spt == 0;
       for (int p = 0; p < a.tps; ++p) {
@@ -642,7 +669,7 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const Prefix
     const int quad = warp & 3, half = warp >> 2;  // TMEM lanes 32 quad .., positions HALF half .. of a tile
     const int r = quad * 32 + lane;
     const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16);
-    int swaps = 0;
+    int swaps = 0, n = 0;  // n: stages filled before
     bool ok = true;
     // the row's two threads swap a number; false when the CTA gives up
     auto swap = [&](float& x) {
@@ -657,7 +684,7 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const Prefix
     };
     for (int seg = 0; walk.next(a, pref, info, sg); ++seg) {
       const int tiles = (sg.hi - sg.lo + UNITS - 1) / UNITS;
-      const RowAt w = row_at<D>(a, sg.rows, sg.head, r, ROWS);
+      const RowAt w = row_at<D>(a, sg.rows, sg.head, r, a.tile_rows, seq_s, ql_s);
       if (sg.lo == 0 && tid == 0) {  // where the tile's parts are
         const int units = pref[sg.tile + 1] - pref[sg.tile];
         const int64_t last = (int64_t)pref[sg.tile] * a.hkv + (int64_t)(sg.head + 1) * units - 1;
@@ -666,32 +693,34 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const Prefix
       }
       const bool real = w.pos >= 0;
       const bool busy = __any_sync(0xffffffffu, real);
-      if (ok) {
-        // this thread's half of its row of Q into TMEM
-        constexpr int NQ = D / 16;  // 16-byte pieces
-        uint4 x[NQ];
+      // this thread's half of its row of Q out of the ring into TMEM (rows that are not there may hold anything)
 #pragma unroll
-        for (int i = 0; i < NQ; ++i)
-          x[i] = real ? ld_act_v4(reinterpret_cast<const bf16*>(a.q) + w.at + half * (D / 2) + 8 * i)
-                      : make_uint4(0, 0, 0, 0);
+      for (int h = 0; h < C::QST; ++h) ok = ok && held(full((n + h) % C::STAGES), ((n + h) / C::STAGES) & 1);
+      if (ok) {
+        constexpr int CH = D / 64;  // lines of 64 dims; ROWS of them a chunk, CH / QST chunks a stage
         const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
 #pragma unroll
-        for (int i = 0; i < NQ; i += 4) {
+        for (int i = 0; i < D / 32; i += 2) {  // 32 dims at a time: 4 pieces of 16 bytes
+          const int dim = half * (D / 2) + 16 * i;
+          const int ch = dim / 64, st = (n + ch / (CH / C::QST)) % C::STAGES;
+          const uint32_t line = sm + st * C::KV + (ch % (CH / C::QST)) * (ROWS * 128) + r * 128;
           uint32_t y[16];
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            y[4 * k] = x[i + k].x ^ flip;
-            y[4 * k + 1] = x[i + k].y ^ flip;
-            y[4 * k + 2] = x[i + k].z ^ flip;
-            y[4 * k + 3] = x[i + k].w ^ flip;
+            const uint4 v = lds128(line + ((((dim % 64) / 8 + k) ^ (r & 7)) << 4));
+            y[4 * k] = v.x ^ flip;
+            y[4 * k + 1] = v.y ^ flip;
+            y[4 * k + 2] = v.z ^ flip;
+            y[4 * k + 3] = v.w ^ flip;
           }
-          tc::tmem_store16(lanes + C::q_col + half * (D / 4) + 4 * i, y);
+          tc::tmem_store16(lanes + C::q_col + dim / 2, y);
         }
         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
         tc::tc_fence_before();
         __syncwarp();
         if (lane == 0) tc::mbar_arrive(q_tmem);
       }
+      n += C::QST + 2 * tiles;
       // M: what the weights are relative to; -1e38 where nothing has been seen
       float M = -1e38f, l = 0.f;
 #pragma unroll 1
@@ -747,7 +776,8 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const Prefix
           if (!ok) break;
           m = fmaxf(m, mo);
           if (m > M + kSpan) {
-            f = ex2(M - m);
+            // (a row that has seen nothing has zeros in O, or what it is worked out again for: nothing to rescale)
+            if (M > -1e38f) f = ex2(M - m);
             M = m;
             l *= f;
           }
@@ -815,6 +845,7 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const Prefix
       }
       const bool any = real && l != 0.f;  // l is NaN, not 0, where a seen score is
       const float k = any ? 1.f / l : 0.f;
+      const uint32_t seen = __ballot_sync(0xffffffffu, any);
       bool odd = false;
 #pragma unroll 1
       for (int d = half * (D / 2); d < (half + 1) * (D / 2); d += 32) {
@@ -840,11 +871,25 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const Prefix
               *reinterpret_cast<uint4*>(out + d + i) = make_uint4(z[0], z[1], z[2], z[3]);
             }
           }
-        } else if (any) {
-          float* to = a.ws_o + po * D + d;
+        } else if (busy) {
+          // 16 floats a row through shared memory, so that a store covers 8 rows of 64 bytes, not 32 of 16
+          const uint32_t box = sm + C::stage + warp * 2048;
+          float* to = a.ws_o + (po - lane) * D + d;
 #pragma unroll
-          for (int i = 0; i < 32; i += 4)
-            *reinterpret_cast<uint4*>(to + i) = make_uint4(y[i], y[i + 1], y[i + 2], y[i + 3]);
+          for (int h = 0; h < 32; h += 16) {
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              sts128(box + lane * 64 + ((i ^ (lane >> 1 & 3)) << 4),
+                     make_uint4(y[h + 4 * i], y[h + 4 * i + 1], y[h + 4 * i + 2], y[h + 4 * i + 3]));
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int row = 8 * i + (lane >> 2);
+              const uint4 v = lds128(box + row * 64 + (((lane & 3) ^ (row >> 1 & 3)) << 4));
+              if (seen >> row & 1) *reinterpret_cast<uint4*>(to + row * D + h + 4 * (lane & 3)) = v;
+            }
+          }
         }
       }
       // rows that V's infinities or NaN have reached: seen ones come out as they are, others are taken out
@@ -861,14 +906,17 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const Prefix
     // -------------------------------------------------------------- pages
     const int64_t rows_plane = (int64_t)a.num_layers * a.num_blocks * a.block_size;
     const int64_t row_layer = (int64_t)a.layer_no * a.num_blocks * a.block_size;
+    uint32_t lead;    // one lane issues: operands of the copies then stay in uniform registers
+    asm volatile("{.reg .pred p; elect.sync _|p, 0xffffffff; selp.u32 %0, 1, 0, p;}" : "=r"(lead));
     int n = 0;        // stages filled
     bool ok = true;
     for (int seg = 0; ok && walk.next(a, pref, info, sg); ++seg) {
       const int tiles = (sg.hi - sg.lo + UNITS - 1) / UNITS;
-      const int P = prefix_of(a, sg.rows.group), pu = prefix_units(P);
+      const int P = pre_s[sg.rows.group], pu = prefix_units(P);
       int before = pu;
       for (int i0 = 0; i0 < sg.rows.nseq; i0 += 32) {
-        const int i = i0 + lane, t = i < sg.rows.nseq ? tail_units(a, sg.rows.seq0 + i, P) : 0;
+        const int i = i0 + lane, b = sg.rows.seq0 + i;
+        const int t = i < sg.rows.nseq ? tail_units(a, seq_s[b], ql_s[b], P) : 0;
         int incl = t;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -879,58 +927,87 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const Prefix
         before += __shfl_sync(0xffffffffu, incl, 31);
       }
       __syncwarp();
-      // units of a batch of tiles, a lane each: where their rows are, and who sees them
+      // units of a batch of tiles, a lane each: where their rows are, and who sees them.  The table is read a batch ahead.
       constexpr int BATCH = 32 / UNITS;
-      int vrow[2] = {0, 0};  // rows of this lane's unit, of this batch and of the one before
+      int4 next_m;
+      int next_blk;
       auto look = [&](int j0) {
         const int u = sg.lo + j0 * UNITS + lane;
-        int4 m = make_int4(0, 0, 0, -1);
-        int row = 0;
+        next_m = make_int4(0, 0, 0, -1);
+        next_blk = -1;
         if (u < sg.hi) {
-          int owner = -1, from = sg.rows.first, p0 = 16 * u, lo = 0, hi = P;
+          int from = sg.rows.first;
+          next_m = make_int4(16 * u, 0, P, -1);
           if (u >= pu) {
-            owner = 0;
+            int owner = 0;
             for (int step = sg.rows.nseq; step > 1;) {  // the last sequence whose tail starts at or before u
               const int hf = step / 2;
               if (cum[owner + hf] <= u) owner += hf, step -= hf;
               else step = hf;
             }
             from = sg.rows.seq0 + owner;
-            p0 = 16 * (P / 16 + u - cum[owner]);
-            lo = P;
-            hi = min(ld_act(a.seq_lens + from), a.cap);
+            next_m = make_int4(16 * (P / 16 + u - cum[owner]), P, min(seq_s[from], a.cap), owner);
           }
-          const int blk = ld_act(a.tables + (int64_t)from * a.max_blocks + p0 / a.block_size);
-          if ((unsigned)blk < (unsigned)a.num_blocks) {
-            m = make_int4(p0, lo, hi, owner);
-            row = blk * a.block_size + p0 % a.block_size;
-          }
+          next_blk = ld_act(a.tables + (int64_t)from * a.max_blocks + next_m.x / a.block_size);
         }
+      };
+      int4 m;
+      int vrow[2] = {0, 0};  // rows of this lane's unit, of this batch and of the one before
+      auto advance = [&] {
+        const bool there = (unsigned)next_blk < (unsigned)a.num_blocks;
+        m = there ? next_m : make_int4(0, 0, 0, -1);
+        int row = there ? next_blk * a.block_size + next_m.x % a.block_size : 0;
         // units that are not there fetch the batch's first rows: finite values as a rule, and no bytes of DRAM
         const int first = __shfl_sync(0xffffffffu, row, 0);
-        if (m.z == 0) row = first;
+        if (!there) row = first;
         vrow[1] = vrow[0];
         vrow[0] = row;
-        return m;
       };
-      int4 m = look(0);
+      look(0);
+      // Q: rows of all of the tile's tokens and heads, a box of 64 dims at a time
+#pragma unroll
+      for (int h = 0; h < C::QST; ++h) {
+        const int s = n % C::STAGES;
+        if (n >= C::STAGES && !held(freed(s), (n / C::STAGES - 1) & 1)) {
+          ok = false;
+          break;
+        }
+        if (lead) {
+          constexpr int CS = D / 64 / C::QST;
+          tc::mbar_expect_tx(full(s), CS * a.q_box * 128);
+#pragma unroll
+          for (int ch = 0; ch < CS; ++ch)
+            tma_rows(sm + s * C::KV + ch * (ROWS * 128), &qmap, full(s), h * CS + ch, sg.head * a.G,
+                     sg.rows.seq0 * a.T + sg.rows.part * (a.tile_rows / a.G));
+        }
+        __syncwarp();
+        ++n;
+      }
       auto fetch = [&](int row_of_lane, int in_batch, int64_t base, int plane) {
         const int s = n % C::STAGES;
         if (n >= C::STAGES && !held(freed(s), (n / C::STAGES - 1) & 1)) return false;
-        if (lane == 0) tc::mbar_expect_tx(full(s), C::KV);
+        int rows[UNITS];
+#pragma unroll
+        for (int u = 0; u < UNITS; ++u)
+          rows[u] = (int)(plane * rows_plane + base) + __shfl_sync(0xffffffffu, row_of_lane, (in_batch * UNITS + u) & 31);
+        if (lead) {
+          tc::mbar_expect_tx(full(s), C::KV);
+#pragma unroll
+          for (int u = 0; u < UNITS; ++u)
+#pragma unroll
+            for (int ch = 0; ch < D / 64; ++ch)
+              tma_rows(sm + s * C::KV + ch * (TILE * 128) + u * 2048, &map, full(s), ch, sg.head, rows[u]);
+        }
         __syncwarp();
-        constexpr int CH = D / 64;
-        const int u = lane / CH, ch = lane % CH;
-        const int row = __shfl_sync(0xffffffffu, row_of_lane, (in_batch * UNITS + u) & 31);
-        if (u < UNITS)
-          tma_rows(sm + s * C::KV + ch * (TILE * 128) + u * 2048, &map, full(s), ch, sg.head,
-                   (int)(plane * rows_plane + base) + row);
         ++n;
         return true;
       };
       for (int j = 0; ok && j <= tiles; ++j) {
         if (j < tiles) {
-          if (j > 0 && j % BATCH == 0) m = look(j);
+          if (j % BATCH == 0) {
+            advance();
+            look(j + BATCH);
+          }
           const int jt = jg + j;
           if (lane / UNITS == j % BATCH) meta[(jt % META) * UNITS + lane % UNITS] = m;
           __syncwarp();
@@ -978,7 +1055,12 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const Prefix
     };
     for (int seg = 0; ok && walk.next(a, pref, info, sg); ++seg) {
       const int tiles = (sg.hi - sg.lo + UNITS - 1) / UNITS;
-      ok = ready(q_tmem, seg & 1) && scores(jg);
+      ok = ready(q_tmem, seg & 1);
+      if (!ok) break;
+#pragma unroll
+      for (int h = 0; h < C::QST; ++h, ++n)
+        if (lead) tc::mbar_arrive(freed(n % C::STAGES));  // Q has left the ring
+      ok = scores(jg);
 #pragma unroll 1
       for (int j = 0; ok && j < tiles; ++j) {
         const int jt = jg + j;
@@ -1027,8 +1109,8 @@ __global__ void __launch_bounds__(128) prefix_join_kernel(const PrefixAttn a) {
   const int in = t * a.G + h % a.G;  // among the sequence's rows of this KV head
   pdl_wait();
   const int2 pl = __ldcg(a.place + b);
-  const int tile = pl.x + (a.tps > 1 ? in / ROWS : 0);
-  const int r = a.tps > 1 ? in % ROWS : pl.y * a.R + in;
+  const int tile = pl.x + (a.tps > 1 ? in / a.tile_rows : 0);
+  const int r = a.tps > 1 ? in % a.tile_rows : pl.y * a.R + in;
   if ((unsigned)tile >= (unsigned)a.tiles || (unsigned)r >= (unsigned)ROWS) return;
   const int2 plan = __ldcg(a.plan + (int64_t)tile * a.hkv + head);
   if (plan.y == 1) return;
@@ -1085,7 +1167,8 @@ constexpr int kSms = 148;
 
 struct PrefixLayout {
   bool tc;               // tensor-core kernel
-  int rows;              // of a row tile
+  int rows;              // of a row tile's partials
+  int tile_rows;
   int ctas;
   int R, spt, tps, tiles, nsplit;
   size_t parts;          // rows of partials
@@ -1101,14 +1184,17 @@ PrefixLayout prefix_layout(int dtype, int B, int T, int hq, int hkv, int D, int 
     L.spt = std::max(1, rows / L.R);
     L.tps = L.R > rows ? (L.R + rows - 1) / rows : 1;
     // every group starts a tile of its own
+    L.tile_rows = rows;
     const int64_t n = L.tps > 1 ? (int64_t)B * L.tps : std::min<int64_t>(B, (int64_t)B / L.spt + groups);
     L.tiles = (int)std::min<int64_t>(n, 0x7fffffff);
   };
-  if (dtype == SSD_DTYPE_BF16 && block_size % 16 == 0) {
-    tiles_of(tile::ROWS);
-    L.tc = L.tiles <= tile::kMaxTiles;
+  const int G = hq / hkv;
+  if (dtype == SSD_DTYPE_BF16 && block_size % 16 == 0 && G <= tile::ROWS) {
+    tiles_of(tile::ROWS / G * G);  // whole tokens
+    L.tc = L.tiles <= tile::kMaxTiles && B <= tile::kMaxTiles && groups <= tile::kMaxTiles;
   }
   if (L.tc) {
+    L.rows = tile::ROWS;
     const int64_t units = ((int64_t)max_seq_len + 15) / 16 * ((int64_t)L.tiles + B) * hkv;
     L.ctas = (int)std::min<int64_t>(kSms, (units + tile::kMinUnits - 1) / tile::kMinUnits);
     L.nsplit = 0;
@@ -1129,14 +1215,15 @@ PrefixLayout prefix_layout(int dtype, int B, int T, int hq, int hkv, int D, int 
 
 template <int D>
 int launch_tc(cudaStream_t st, const PrefixAttn& a, int ctas) {
-  CUtensorMap map;
-  if (!make_kv_row_map(&map, a.pages, (int64_t)2 * a.num_layers * a.num_blocks * a.block_size, a.hkv, D))
+  CUtensorMap map, qmap;
+  if (!make_kv_row_map(&map, a.pages, (int64_t)2 * a.num_layers * a.num_blocks * a.block_size, a.hkv, D, 1, 16) ||
+      !make_kv_row_map(&qmap, a.q, (int64_t)a.B * a.T, a.hq, D, a.G, tile::ROWS / a.G))
     return SSD_ERR_LAUNCH;
   auto kern = tile::prefix_attention_tc_kernel<D>;
   constexpr size_t smem = tile::Cfg<D>::smem;
   static std::atomic<uint64_t> ready{0};
   if (!allow_smem(ready, kern, (int)smem)) return SSD_ERR_LAUNCH;
-  SSD_PDL(kern, ctas, tile::THREADS, smem, st, map, a);
+  SSD_PDL(kern, ctas, tile::THREADS, smem, st, map, qmap, a);
   const int64_t rows = (int64_t)a.B * a.T * a.hq;
   SSD_PDL((prefix_join_kernel<bf16, D, tile::ROWS, true>), (unsigned)((rows + 3) / 4), 128, 0, st, a);
   return SSD_OK;
@@ -1225,6 +1312,8 @@ extern "C" int ssd_shared_prefix_attention(ssd_stream_t stream, const void* q, c
   a.max_blocks = max_blocks;
   a.cap = max_seq_len;
   a.R = L.R;
+  a.tile_rows = L.tile_rows;
+  a.q_box = tile::ROWS / a.G * a.G;
   a.spt = L.spt;
   a.tps = L.tps;
   a.tiles = L.tiles;
