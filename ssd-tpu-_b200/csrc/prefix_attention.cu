@@ -44,8 +44,10 @@ struct PrefixAttn {
   int nsplit;            // parts of a tile's list (CUDA-core kernel)
   float* ws_o;           // [part][row][D] unnormalised sums
   float2* ws_ml;         // [part][row] what they are relative to, sum of weights
-  int2* plan;            // [tile][head]: first part, parts (0: the tile sees nothing; 1: written by the kernel itself)
-  int2* place;           // [sequence]: its (first) tile, its number in that tile
+  // [sequence, or tile where a sequence has several][head]: first part, parts (1: the kernel has
+  // written the rows itself), step from part to part, the sequence's first row
+  int4* parts;
+  bool whole;            // lists are not cut
 };
 
 struct RowTile {
@@ -188,7 +190,6 @@ __global__ void __launch_bounds__(kChunkC) prefix_attention_cc_kernel(const Pref
     if (lane == 0) cum[0] = P;
     if (lane < kRowsC) cum[1 + lane] = P + incl;
   }
-  if (split == 0 && tid < tl.nseq && head == 0) a.place[tl.seq0 + tid] = make_int2(tile - tl.part, tid);
   __syncthreads();
   for (int i = tid; i < kRowsC * D; i += kChunkC) {
     const int r = i / D, d = i % D;
@@ -199,7 +200,9 @@ __global__ void __launch_bounds__(kChunkC) prefix_attention_cc_kernel(const Pref
   const int chunks = (len + kChunkC - 1) / kChunkC;
   const int per = max(1, (chunks + a.nsplit - 1) / a.nsplit);
   const int parts = max(1, (chunks + per - 1) / per);
-  if (a.plan && split == 0 && tid == 0) a.plan[tile * a.hkv + head] = make_int2(0, parts);
+  if (a.nsplit > 1 && split == 0 && tid < tl.nseq)
+    a.parts[(int64_t)(a.tps > 1 ? tile : tl.seq0 + tid) * a.hkv + head] =
+        make_int4((tile * a.hkv + head) * a.nsplit, parts, 1, a.tps > 1 ? 0 : tid * a.R);
   if (split >= parts) return;
   const int lo = split * per * kChunkC, hi = min(len, lo + per * kChunkC);
   const KV* pages = reinterpret_cast<const KV*>(a.pages) + a.layer;
@@ -353,7 +356,9 @@ constexpr int SOFT = 256;              // threads of the row warps
 constexpr int THREADS = SOFT + 64;
 constexpr int META = 8;                // tiles whose units are described: more than there are between fetch and use
 constexpr int kMaxTiles = 512;         // also sequences and groups: their numbers are kept in shared memory
-constexpr int kMinUnits = 8;           // of a CTA: shorter runs cost more in prologues and joins than they save
+constexpr int kMinUnits = 8;           // of a run: shorter ones cost more in prologues and joins than they save
+constexpr int kWhole = 64;             // lists of at most so many units are not cut
+constexpr int kMaxTeam = 8;            // CTAs that walk a group's lists side by side
 constexpr float kSpan = 8.f;           // weights are at most 2^8
 constexpr uint32_t kPolls = 1u << 24;
 __device__ uint32_t gave_up;           // 1 once a CTA's wait ran out
@@ -365,8 +370,9 @@ struct Cfg {
   static constexpr uint32_t KV = TILE * D * 2;  // bytes of a stage: one tile's K or V
   static constexpr uint32_t ring = STAGES * KV;
   static constexpr uint32_t stage = ring;                             // float [SOFT][16]: results on their way out
-  static constexpr uint32_t pref = stage + 64 * SOFT;                 // int [kMaxTiles + 1]: units before each tile
-  static constexpr uint32_t info = pref + 4 * (kMaxTiles + 4);        // int2 [kMaxTiles]
+  static constexpr uint32_t pref = stage + 64 * SOFT;                 // int [kMaxTiles + 1], see Walk
+  static constexpr uint32_t units = pref + 4 * (kMaxTiles + 4);       // int [kMaxTiles]: units of each tile
+  static constexpr uint32_t info = units + 4 * kMaxTiles;             // int2 [kMaxTiles]
   static constexpr uint32_t seq = info + 8 * kMaxTiles;               // int [kMaxTiles]: lengths,
   static constexpr uint32_t ql = seq + 4 * kMaxTiles;                 // new tokens of the sequences,
   static constexpr uint32_t pre = ql + 4 * kMaxTiles;                 // prefixes of the groups
@@ -430,41 +436,75 @@ __device__ __forceinline__ void tma_rows(uint32_t dst, const CUtensorMap* map, u
 struct Segment {
   int tile, head, lo, hi;   // units [lo, hi) of the tile's list
   int slot;                 // of partials; -1: the whole list, straight to the output
+  int parts;                // with lo = 0: of the list
   RowTile rows;
 };
-// The CTA's run of all units, segment by segment.  `pref`: units before each tile (one head).
+// How the units are shared out.  They stand in a row: tile after tile, in each the KV heads, in each the tile's list;
+// every CTA takes a run of them.  Where all groups have the same few (nm) tiles, nm CTAs work as a team: the lists of a
+// group's tiles are walked side by side, one CTA a tile, so that the prefix that they all read is fetched from DRAM
+// once and found in L2 after that.  Where a list is short whatever the lengths (`whole`), runs end with lists: nothing
+// is joined.
+struct Shares {
+  int nm;           // CTAs of a team (1: no teams)
+  int runs;         // runs that the units are cut into
+  int64_t all;      // units, over all heads (of the longest list of each group, where there are teams)
+  bool whole;
+};
 struct Walk {
   int64_t pos, end;
-  int tile;
-  __device__ Walk(const PrefixAttn& a, const int* pref, int tiles, int ctas) : tile(0) {
-    const int64_t all = (int64_t)pref[tiles] * a.hkv;
-    pos = all * blockIdx.x / ctas;
-    end = (int)blockIdx.x < ctas ? all * (blockIdx.x + 1) / ctas : pos;
-    int n = tiles;
-    while (n > 1) {  // the last tile that starts at or before pos
+  int at;           // tile (group, where there are teams) that pos is in
+  __device__ Walk(const PrefixAttn& a, const Shares& sh, const int* pref, int n) : at(0) {
+    const int run = (int)blockIdx.x / sh.nm;
+    pos = end = 0;
+    if (run >= sh.runs) return;
+    if (sh.whole) {
+      const int64_t lists = (int64_t)n * a.hkv, l0 = lists * run / sh.runs, l1 = lists * (run + 1) / sh.runs;
+      auto start = [&](int64_t l) {
+        const int t = (int)(l / a.hkv);
+        return t >= n ? sh.all : (int64_t)pref[t] * a.hkv + (l - (int64_t)t * a.hkv) * (pref[t + 1] - pref[t]);
+      };
+      pos = start(l0);
+      end = start(l1);
+    } else {
+      pos = sh.all * run / sh.runs;
+      end = sh.all * (run + 1) / sh.runs;
+    }
+    while (n > 1) {  // the last one that starts at or before pos
       const int half = n / 2;
-      if ((int64_t)pref[tile + half] * a.hkv <= pos) tile += half, n -= half;
+      if ((int64_t)pref[at + half] * a.hkv <= pos) at += half, n -= half;
       else n = half;
     }
   }
-  __device__ bool next(const PrefixAttn& a, const int* pref, const int2* info, Segment& s) {
-    if (pos >= end) return false;
-    while ((int64_t)pref[tile + 1] * a.hkv <= pos) ++tile;
-    const int units = pref[tile + 1] - pref[tile];
-    const int64_t off = pos - (int64_t)pref[tile] * a.hkv;
-    s.tile = tile;
-    s.head = (int)(off / units);
-    s.lo = (int)(off - (int64_t)s.head * units);
-    s.hi = (int)min((int64_t)units, s.lo + (end - pos));
-    s.slot = s.lo == 0 && s.hi == units ? -1 : s.lo > 0 ? 2 * (int)blockIdx.x : 2 * (int)blockIdx.x + 1;
-    pos += s.hi - s.lo;
-    const int2 t = info[tile];
-    s.rows.seq0 = t.x & 0xffff;
-    s.rows.nseq = a.tps > 1 ? 1 : t.x >> 16;
-    s.rows.part = a.tps > 1 ? t.x >> 16 : 0;
-    s.rows.group = t.y & 0xffff;
-    s.rows.first = t.y >> 16;
-    return true;
+  __device__ bool next(const PrefixAttn& a, const Shares& sh, const int* pref, const int* units_s, const int2* info,
+                       Segment& s) {
+    while (pos < end) {
+      while ((int64_t)pref[at + 1] * a.hkv <= pos) ++at;
+      const int list = pref[at + 1] - pref[at];
+      const int off = (int)(pos - (int64_t)pref[at] * a.hkv);
+      s.head = off / list;
+      s.lo = off - s.head * list;
+      s.hi = (int)min((int64_t)list, s.lo + (end - pos));
+      pos += s.hi - s.lo;
+      s.tile = at * sh.nm + (int)blockIdx.x % sh.nm;
+      const int units = units_s[s.tile];
+      s.hi = min(s.hi, units);
+      if (s.lo >= s.hi) continue;
+      const bool all = s.lo == 0 && s.hi == units;
+      s.slot = all ? -1 : s.lo > 0 ? 2 * (int)blockIdx.x : 2 * (int)blockIdx.x + 1;
+      s.parts = 1;
+      if (s.lo == 0 && !all) {
+        const int64_t last = (int64_t)pref[at] * a.hkv + (int64_t)s.head * list + units - 1;
+        s.parts = (int)(((last + 1) * sh.runs - 1) / sh.all) - (int)blockIdx.x / sh.nm + 1;
+      }
+      const int2 t = info[s.tile];
+      s.rows.seq0 = t.x & 0xffff;
+      s.rows.nseq = a.tps > 1 ? 1 : t.x >> 16;
+      s.rows.part = a.tps > 1 ? t.x >> 16 : 0;
+      s.rows.group = t.y & 0xffff;
+      s.rows.first = t.y >> 16;
+      return true;
+    }
+    return false;
   }
 };
 
@@ -522,6 +562,15 @@ __device__ __noinline__ void row_again(const PrefixAttn& a, const Segment& sg, i
   }
 }
 
+// Where the join finds the parts of a tile's list: for each of its sequences (from `i`, every `by`-th) the first part,
+// their number, the step from part to part, and the sequence's first row.
+__device__ __forceinline__ void put_parts(const PrefixAttn& a, int2 info, int tile, int head, int first, int parts,
+                                          int step, int i, int by) {
+  const int seq0 = info.x & 0xffff, n = a.tps > 1 ? 1 : info.x >> 16;
+  for (; i < n; i += by)
+    a.parts[(int64_t)(a.tps > 1 ? tile : seq0 + i) * a.hkv + head] = make_int4(first, parts, step, a.tps > 1 ? 0 : i * a.R);
+}
+
 template <int D>
 __global__ void __launch_bounds__(THREADS, 1)
 prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ CUtensorMap qmap,
@@ -532,6 +581,7 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid
   const uint32_t raw = tc::smem_u32(smem_raw), sm = (raw + 1023u) & ~1023u;
   uint8_t* gen = smem_raw + (sm - raw);
   int* pref = reinterpret_cast<int*>(gen + C::pref);
+  int* units_s = reinterpret_cast<int*>(gen + C::units);
   int2* info = reinterpret_cast<int2*>(gen + C::info);
   int* seq_s = reinterpret_cast<int*>(gen + C::seq);
   int* ql_s = reinterpret_cast<int*>(gen + C::ql);
@@ -585,8 +635,8 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid
     int* g_start = reinterpret_cast<int*>(gen);           // [groups + 1]
     int* g_tile = reinterpret_cast<int*>(gen) + kMaxTiles + 1;
     for (int i = tid; i < a.tiles; i += THREADS) {
-      pref[1 + i] = 0;
       info[i] = make_int2(0, 0);
+      units_s[i] = 0;
     }
     for (int b = tid; b < a.B; b += THREADS) {
       seq_s[b] = ld_act(a.seq_lens + b);
@@ -598,9 +648,11 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid
     }
     __syncthreads();
     if (warp == 0) {
-      int before = 0;
+      int before = 0, nm = -1;  // nm: tiles of every group; 0: not the same for all
       for (int g0 = 0; g0 < a.groups; g0 += 32) {
         const int g = g0 + lane, n = g < a.groups ? group_tiles(a, g_start[g + 1] - g_start[g]) : 0;
+        if (nm < 0) nm = __shfl_sync(0xffffffffu, n, 0);
+        if (__any_sync(0xffffffffu, g < a.groups && n != nm)) nm = 0;
         int incl = n;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -610,6 +662,7 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid
         if (g < a.groups) g_tile[g] = before + incl - n;
         before += __shfl_sync(0xffffffffu, incl, 31);
       }
+      if (lane == 0) pref[0] = nm > 1 && nm <= kMaxTeam && nm * 4 <= (int)gridDim.x && !a.whole ? nm : 1;
     }
     __syncthreads();
     for (int b = tid; b < a.B; b += THREADS) {
@@ -626,30 +679,42 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid
       const bool lead = a.tps > 1 || k % a.spt == 0;
       for (int p = 0; p < a.tps; ++p) {
         if (t0 + p >= a.tiles) break;
-        atomicAdd(&pref[1 + t0 + p], tail + (lead ? prefix_units(P) : 0));
+        atomicAdd(&units_s[t0 + p], tail + (lead ? prefix_units(P) : 0));
         if (lead) info[t0 + p] = make_int2(b | (a.tps > 1 ? p : min(a.spt, e - b)) << 16, g | s << 16);
       }
-      if (blockIdx.x == 0) a.place[b] = make_int2(t0, a.tps > 1 ? 0 : k % a.spt);
     }
     __syncthreads();
     if (warp == 0) {
+      const int nm = pref[0], lists = nm > 1 ? a.groups : a.tiles;
       int before = 0;
-      if (lane == 0) pref[0] = 0;
-      for (int t0 = 0; t0 < a.tiles; t0 += 32) {
-        const int t = t0 + lane, n = t < a.tiles ? pref[1 + t] : 0;
+      __syncwarp();
+      for (int t0 = 0; t0 < lists; t0 += 32) {
+        const int t = t0 + lane;
+        int n = 0;
+        if (t < lists)
+          for (int i = 0; i < nm; ++i) n = max(n, units_s[t * nm + i]);
         int incl = n;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
           const int y = __shfl_up_sync(0xffffffffu, incl, o);
           if (lane >= o) incl += y;
         }
-        if (t < a.tiles) {
-          pref[1 + t] = before + incl;
-          if (n == 0 && blockIdx.x == 0)  // rows that see nothing: the join writes their zeros
-            for (int h = 0; h < a.hkv; ++h) a.plan[t * a.hkv + h] = make_int2(0, 0);
-        }
+        if (t < lists) pref[1 + t] = before + incl;
         before += __shfl_sync(0xffffffffu, incl, 31);
       }
+      if (lane == 0) {
+        pref[0] = 0;
+        slot[3] = nm;
+      }
+    }
+    for (int t = blockIdx.x; t < a.tiles; t += gridDim.x) {  // rows that see nothing
+      if (units_s[t] != 0) continue;
+      const int2 in = info[t];
+      const int seq0 = in.x & 0xffff, n = a.tps > 1 ? (in.x >> 16 ? 0 : 1) : in.x >> 16;
+      const int64_t row = (int64_t)a.T * a.hq * D / 8;
+      for (int64_t i = tid; i < n * row; i += THREADS)
+        reinterpret_cast<uint4*>(a.out)[seq0 * row + i] = make_uint4(0, 0, 0, 0);
+      for (int h = tid; h < a.hkv; h += THREADS) put_parts(a, in, t, h, 0, 1, 0, 0, 1);
     }
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the ring was written by threads
   }
@@ -657,9 +722,14 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid
   __syncthreads();
   tc::tc_fence_after();
   const uint32_t tmem = *slot;
-  const int64_t all = (int64_t)pref[a.tiles] * a.hkv;
-  const int ctas = (int)max((int64_t)1, min((int64_t)gridDim.x, (all + kMinUnits - 1) / kMinUnits));
-  Walk walk(a, pref, a.tiles, ctas);
+  Shares sh;
+  sh.nm = slot[3];
+  const int lists = sh.nm > 1 ? a.groups : a.tiles;
+  sh.all = (int64_t)pref[lists] * a.hkv;
+  sh.whole = a.whole;
+  sh.runs = (int)max((int64_t)1, min((int64_t)((int)gridDim.x / sh.nm), sh.whole ? (int64_t)lists * a.hkv
+                                                                                   : (sh.all + kMinUnits - 1) / kMinUnits));
+  Walk walk(a, sh, pref, lists);
   Segment sg;
   const float c = fmaxf(fabsf(a.scale) * 1.4426950408889634f, 1e-38f);  // not 0: keeps the mask's infinity an infinity
   int jg = 0;  // tiles before this segment
@@ -682,15 +752,11 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid
       ++swaps;
       return true;
     };
-    for (int seg = 0; walk.next(a, pref, info, sg); ++seg) {
+    for (int seg = 0; walk.next(a, sh, pref, units_s, info, sg); ++seg) {
       const int tiles = (sg.hi - sg.lo + UNITS - 1) / UNITS;
       const RowAt w = row_at<D>(a, sg.rows, sg.head, r, a.tile_rows, seq_s, ql_s);
-      if (sg.lo == 0 && tid == 0) {  // where the tile's parts are
-        const int units = pref[sg.tile + 1] - pref[sg.tile];
-        const int64_t last = (int64_t)pref[sg.tile] * a.hkv + (int64_t)(sg.head + 1) * units - 1;
-        const int c1 = (int)(((last + 1) * ctas - 1) / all);
-        a.plan[sg.tile * a.hkv + sg.head] = make_int2(2 * (int)blockIdx.x + 1, c1 - (int)blockIdx.x + 1);
-      }
+      if (sg.lo == 0 && warp == 0)
+        put_parts(a, info[sg.tile], sg.tile, sg.head, 2 * (int)blockIdx.x + 1, sg.parts, 2 * sh.nm, lane, 32);
       const bool real = w.pos >= 0;
       const bool busy = __any_sync(0xffffffffu, real);
       // this thread's half of its row of Q out of the ring into TMEM (rows that are not there may hold anything)
@@ -845,53 +911,69 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid
       }
       const bool any = real && l != 0.f;  // l is NaN, not 0, where a seen score is
       const float k = any ? 1.f / l : 0.f;
-      const uint32_t seen = __ballot_sync(0xffffffffu, any);
-      bool odd = false;
-#pragma unroll 1
-      for (int d = half * (D / 2); d < (half + 1) * (D / 2); d += 32) {
+      // A warp's 32 rows by 64 bytes go through shared memory, so that a store covers 8 rows of 64 bytes, not 32 of 16.
+      const uint32_t seen = __ballot_sync(0xffffffffu, any), exist = __ballot_sync(0xffffffffu, w.at >= 0);
+      const uint32_t box = sm + C::stage + warp * 2048, mine = box + lane * 64;
+      const int q4 = lane & 3;
+      int64_t at4[4];  // of the rows that this lane stores a quarter of
+      uint32_t put4 = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int row = 8 * i + (lane >> 2);
+        at4[i] = direct ? __shfl_sync(0xffffffffu, w.at, row) : (po - lane + row) * D;
+        put4 |= ((direct ? exist : seen) >> row & 1u) << i;
+      }
+      auto send = [&](const uint32_t* y, char* base, int size, int d) {  // 16 words of each row, dims d ..
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          sts128(mine + ((i ^ (lane >> 1 & 3)) << 4), make_uint4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]));
+        __syncwarp();
+        uint4 v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int row = 8 * i + (lane >> 2);
+          v[i] = lds128(box + row * 64 + ((q4 ^ (row >> 1 & 3)) << 4));
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (put4 >> i & 1) *reinterpret_cast<uint4*>(base + (at4[i] + d) * size + 16 * q4) = v[i];
+      };
+      float odd0 = 0.f, odd1 = 0.f;  // NaN once an element is not finite
+      if (busy || (direct && exist)) {
         uint32_t y[32];
-        if (busy) {
-          tc::tmem_load32(lanes + C::o_col + d, y);
-          tc::tmem_ready(y);
-        }
-        float t = 0.f;
-        if (any) {
+        const int d0 = half * (D / 2);
+        if (busy) tc::tmem_load32(lanes + C::o_col + d0, y);
+#pragma unroll 1
+        for (int d = d0; d < d0 + D / 2; d += 32) {
+          uint32_t z[32];
+          if (busy) {
+            tc::tmem_ready(y);
 #pragma unroll
-          for (int i = 0; i < 32; ++i) t += fabsf(__uint_as_float(y[i]));
-          odd |= !(t <= FLT_MAX);
-        }
-        if (direct) {
-          if (w.at >= 0) {
+            for (int i = 0; i < 32; ++i) z[i] = y[i];
+            if (d + 32 < d0 + D / 2) tc::tmem_load32(lanes + C::o_col + d + 32, y);
+          } else {
 #pragma unroll
-            for (int i = 0; i < 32; i += 8) {
-              uint32_t z[4];
-#pragma unroll
-              for (int h = 0; h < 4; ++h)
-                z[h] = any ? pack_bf16(__uint_as_float(y[i + 2 * h]) * k, __uint_as_float(y[i + 2 * h + 1]) * k) : 0u;
-              *reinterpret_cast<uint4*>(out + d + i) = make_uint4(z[0], z[1], z[2], z[3]);
-            }
+            for (int i = 0; i < 32; ++i) z[i] = 0;
           }
-        } else if (busy) {
-          // 16 floats a row through shared memory, so that a store covers 8 rows of 64 bytes, not 32 of 16
-          const uint32_t box = sm + C::stage + warp * 2048;
-          float* to = a.ws_o + (po - lane) * D + d;
 #pragma unroll
-          for (int h = 0; h < 32; h += 16) {
-            __syncwarp();
+          for (int i = 0; i < 32; i += 2) {
+            odd0 = fmaf(__uint_as_float(z[i]), 0.f, odd0);
+            odd1 = fmaf(__uint_as_float(z[i + 1]), 0.f, odd1);
+          }
+          if (direct) {
+            uint32_t p[16];
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-              sts128(box + lane * 64 + ((i ^ (lane >> 1 & 3)) << 4),
-                     make_uint4(y[h + 4 * i], y[h + 4 * i + 1], y[h + 4 * i + 2], y[h + 4 * i + 3]));
-            __syncwarp();
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int row = 8 * i + (lane >> 2);
-              const uint4 v = lds128(box + row * 64 + (((lane & 3) ^ (row >> 1 & 3)) << 4));
-              if (seen >> row & 1) *reinterpret_cast<uint4*>(to + row * D + h + 4 * (lane & 3)) = v;
-            }
+            for (int i = 0; i < 16; ++i)
+              p[i] = any ? pack_bf16(__uint_as_float(z[2 * i]) * k, __uint_as_float(z[2 * i + 1]) * k) : 0u;
+            send(p, reinterpret_cast<char*>(a.out), 2, d);
+          } else {
+            send(z, reinterpret_cast<char*>(a.ws_o), 4, d);
+            send(z + 16, reinterpret_cast<char*>(a.ws_o), 4, d + 16);
           }
         }
       }
+      const bool odd = any && odd0 + odd1 != 0.f;
       // rows that V's infinities or NaN have reached: seen ones come out as they are, others are taken out
       for (uint32_t left = __ballot_sync(0xffffffffu, odd && l == l); left; left &= left - 1) {
         const int from = __ffs(left) - 1;
@@ -910,7 +992,7 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid
     asm volatile("{.reg .pred p; elect.sync _|p, 0xffffffff; selp.u32 %0, 1, 0, p;}" : "=r"(lead));
     int n = 0;        // stages filled
     bool ok = true;
-    for (int seg = 0; ok && walk.next(a, pref, info, sg); ++seg) {
+    for (int seg = 0; ok && walk.next(a, sh, pref, units_s, info, sg); ++seg) {
       const int tiles = (sg.hi - sg.lo + UNITS - 1) / UNITS;
       const int P = pre_s[sg.rows.group], pu = prefix_units(P);
       int before = pu;
@@ -1053,7 +1135,7 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid
       ++n;
       return true;
     };
-    for (int seg = 0; ok && walk.next(a, pref, info, sg); ++seg) {
+    for (int seg = 0; ok && walk.next(a, sh, pref, units_s, info, sg); ++seg) {
       const int tiles = (sg.hi - sg.lo + UNITS - 1) / UNITS;
       ok = ready(q_tmem, seg & 1);
       if (!ok) break;
@@ -1097,56 +1179,90 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid
 }  // namespace tile
 
 // ------------------------------------------------------------------ join
-// out = sum_i w_i o_i / sum_i w_i l_i over a row's parts, w_i = e^(m_i - M).  A warp a query row; bound by latency.
-template <typename T, int D, int ROWS, bool TC>
-__global__ void __launch_bounds__(128) prefix_join_kernel(const PrefixAttn a) {
-  constexpr int PL = D / 32;
-  const int lane = threadIdx.x & 31;
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (row >= (int64_t)a.B * a.T * a.hq) return;
+// out = sum_i w_i o_i / sum_i w_i l_i over a row's parts, w_i = e^(m_i - M).  Four warps a query row, each every fourth
+// part, a lane D / 32 dims.  Bound by latency: where the parts are, their statistics and sums at once, the
+// exchange between the warps.
+constexpr int kJoinWarps = 4, kJoinParts = 256;
+
+template <typename T, int D, int ROWS, bool LOG2>
+__global__ void __launch_bounds__(32 * kJoinWarps) prefix_join_kernel(const PrefixAttn a) {
+  constexpr int PL = D / 32, AHEAD = 4;
+  __shared__ float2 ml_s[kJoinParts];
+  __shared__ __align__(16) float o_s[kJoinWarps - 1][D];
+  __shared__ float sum_s[kJoinWarps];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t row = blockIdx.x;
   const int h = (int)(row % a.hq), t = (int)(row / a.hq % a.T), b = (int)(row / a.hq / a.T);
   const int head = h / a.G;
   const int in = t * a.G + h % a.G;  // among the sequence's rows of this KV head
   pdl_wait();
-  const int2 pl = __ldcg(a.place + b);
-  const int tile = pl.x + (a.tps > 1 ? in / a.tile_rows : 0);
-  const int r = a.tps > 1 ? in % a.tile_rows : pl.y * a.R + in;
-  if ((unsigned)tile >= (unsigned)a.tiles || (unsigned)r >= (unsigned)ROWS) return;
-  const int2 plan = __ldcg(a.plan + (int64_t)tile * a.hkv + head);
-  if (plan.y == 1) return;
-  auto part = [&](int i) -> int64_t {
-    if constexpr (TC) return i == 0 ? plan.x : (plan.x & ~1) + 2 * i;
-    else return (int64_t)(tile * a.hkv + head) * a.nsplit + i;
-  };
-  float M = -INFINITY, L = 0.f;
-  for (int i = lane; i < plan.y; i += 32) M = fmaxf(M, __ldcg(a.ws_ml + part(i) * ROWS + r).x);
-  M = warp_max(M);
-  float o[PL];
+  const int4 at = __ldcg(a.parts + (int64_t)(a.tps > 1 ? b * a.tps + in / a.tile_rows : b) * a.hkv + head);
+  const int r = a.tps > 1 ? in % a.tile_rows : at.w + in;
+  if (at.y == 1 || (unsigned)at.y > (unsigned)kJoinParts || (unsigned)r >= (unsigned)ROWS) return;
+  auto part = [&](int i) { return (int64_t)(i == 0 ? at.x : (LOG2 ? at.x & ~1 : at.x) + i * at.z) * ROWS + r; };
+  float v[AHEAD][PL];
 #pragma unroll
-  for (int x = 0; x < PL; ++x) o[x] = 0.f;
-  for (int i0 = 0; i0 < plan.y; i0 += 32) {
-    float w = 0.f;
-    if (i0 + lane < plan.y) {
-      const float2 ml = __ldcg(a.ws_ml + part(i0 + lane) * ROWS + r);
-      // a part that the row sees nothing of has no weight and is passed over, whatever it left
-      w = ml.y == 0.f ? -1.f : TC ? exp2f(ml.x - M) : expf(ml.x - M);
-      if (ml.y != 0.f) L = fmaf(w, ml.y, L);
-    }
-    const int n = min(32, plan.y - i0);
-#pragma unroll 4
-    for (int i = 0; i < n; ++i) {
-      const float wi = __shfl_sync(0xffffffffu, w, i);
-      if (wi < 0.f) continue;
-      const float* p = a.ws_o + (part(i0 + i) * ROWS + r) * D + lane * 2;
+  for (int k = 0; k < AHEAD; ++k) {  // the first parts' sums before anything is known of their weights
+    const int i = warp + k * kJoinWarps;
+    if (i < at.y)
 #pragma unroll
       for (int x = 0; x < PL; x += 2) {
-        const float2 v = __ldcg(reinterpret_cast<const float2*>(p + x * 32));
-        o[x] = fmaf(wi, v.x, o[x]);
-        o[x + 1] = fmaf(wi, v.y, o[x + 1]);
+        const float2 y = __ldcg(reinterpret_cast<const float2*>(a.ws_o + part(i) * D + lane * 2 + x * 32));
+        v[k][x] = y.x;
+        v[k][x + 1] = y.y;
       }
+  }
+  float M = -INFINITY;
+  for (int i = threadIdx.x; i < at.y; i += 32 * kJoinWarps) ml_s[i] = __ldcg(a.ws_ml + part(i));
+  __syncthreads();
+  for (int i = lane; i < at.y; i += 32) M = fmaxf(M, ml_s[i].x);
+  M = warp_max(M);
+  float o[PL], L = 0.f;
+#pragma unroll
+  for (int x = 0; x < PL; ++x) o[x] = 0.f;
+  for (int i0 = warp; i0 < at.y; i0 += AHEAD * kJoinWarps) {
+    if (i0 != warp)
+#pragma unroll
+      for (int k = 0; k < AHEAD; ++k) {
+        const int i = i0 + k * kJoinWarps;
+        if (i < at.y)
+#pragma unroll
+          for (int x = 0; x < PL; x += 2) {
+            const float2 y = __ldcg(reinterpret_cast<const float2*>(a.ws_o + part(i) * D + lane * 2 + x * 32));
+            v[k][x] = y.x;
+            v[k][x + 1] = y.y;
+          }
+      }
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {
+      const int i = i0 + k * kJoinWarps;
+      if (i >= at.y) break;
+      const float2 ml = ml_s[i];
+      if (ml.y == 0.f) continue;  // a part that the row sees nothing of is passed over, whatever it left
+      const float w = LOG2 ? exp2f(ml.x - M) : expf(ml.x - M);
+      L = fmaf(w, ml.y, L);
+#pragma unroll
+      for (int x = 0; x < PL; ++x) o[x] = fmaf(w, v[k][x], o[x]);
     }
   }
-  L = warp_sum(L);
+  if (warp > 0) {
+#pragma unroll
+    for (int x = 0; x < PL; x += 2)
+      *reinterpret_cast<float2*>(&o_s[warp - 1][lane * 2 + x * 32]) = make_float2(o[x], o[x + 1]);
+    if (lane == 0) sum_s[warp] = L;
+  }
+  __syncthreads();
+  if (warp > 0) return;
+#pragma unroll
+  for (int k = 1; k < kJoinWarps; ++k) {
+    L += sum_s[k];
+#pragma unroll
+    for (int x = 0; x < PL; x += 2) {
+      const float2 y = *reinterpret_cast<const float2*>(&o_s[k - 1][lane * 2 + x * 32]);
+      o[x] += y.x;
+      o[x + 1] += y.y;
+    }
+  }
   const float k = L != 0.f ? 1.f / L : 0.f;
   T* out = reinterpret_cast<T*>(a.out) + row * D + lane * 2;
 #pragma unroll
@@ -1172,7 +1288,8 @@ struct PrefixLayout {
   int ctas;
   int R, spt, tps, tiles, nsplit;
   size_t parts;          // rows of partials
-  size_t off_ml, off_plan, off_place, total;
+  bool whole;            // no list is long enough to be cut
+  size_t off_ml, off_parts, total;
 };
 
 PrefixLayout prefix_layout(int dtype, int B, int T, int hq, int hkv, int D, int block_size, int groups,
@@ -1193,12 +1310,16 @@ PrefixLayout prefix_layout(int dtype, int B, int T, int hq, int hkv, int D, int 
     tiles_of(tile::ROWS / G * G);  // whole tokens
     L.tc = L.tiles <= tile::kMaxTiles && B <= tile::kMaxTiles && groups <= tile::kMaxTiles;
   }
+  const int64_t units = ((int64_t)max_seq_len + 15) / 16;  // of a sequence
   if (L.tc) {
     L.rows = tile::ROWS;
-    const int64_t units = ((int64_t)max_seq_len + 15) / 16 * ((int64_t)L.tiles + B) * hkv;
-    L.ctas = (int)std::min<int64_t>(kSms, (units + tile::kMinUnits - 1) / tile::kMinUnits);
+    // a list is longest where nothing is shared
+    L.whole = units * std::min(L.spt, B) <= tile::kWhole;
+    const int64_t most = L.whole ? (int64_t)L.tiles * hkv
+                                 : (units * (L.tiles + B) * hkv + tile::kMinUnits - 1) / tile::kMinUnits;
+    L.ctas = (int)std::min<int64_t>(kSms, most);
     L.nsplit = 0;
-    L.parts = (size_t)2 * L.ctas * L.rows;
+    L.parts = L.whole ? 0 : (size_t)2 * L.ctas * L.rows;
   } else {
     tiles_of(kRowsC);
     const int64_t ctas = (int64_t)L.tiles * hkv;
@@ -1207,9 +1328,8 @@ PrefixLayout prefix_layout(int dtype, int B, int T, int hq, int hkv, int D, int 
     L.parts = L.nsplit == 1 ? 0 : (size_t)ctas * L.nsplit * L.rows;
   }
   L.off_ml = up256(sizeof(float) * L.parts * D);
-  L.off_plan = L.off_ml + up256(sizeof(float2) * L.parts);
-  L.off_place = L.off_plan + up256(sizeof(int2) * (size_t)L.tiles * hkv);
-  L.total = L.off_place + up256(sizeof(int2) * B);
+  L.off_parts = L.off_ml + up256(sizeof(float2) * L.parts);
+  L.total = L.off_parts + up256(sizeof(int4) * (size_t)(L.tps > 1 ? L.tiles : B) * hkv);
   return L;
 }
 
@@ -1225,7 +1345,8 @@ int launch_tc(cudaStream_t st, const PrefixAttn& a, int ctas) {
   if (!allow_smem(ready, kern, (int)smem)) return SSD_ERR_LAUNCH;
   SSD_PDL(kern, ctas, tile::THREADS, smem, st, map, qmap, a);
   const int64_t rows = (int64_t)a.B * a.T * a.hq;
-  SSD_PDL((prefix_join_kernel<bf16, D, tile::ROWS, true>), (unsigned)((rows + 3) / 4), 128, 0, st, a);
+  if (a.whole) return SSD_OK;
+  SSD_PDL((prefix_join_kernel<bf16, D, tile::ROWS, true>), (unsigned)rows, 32 * kJoinWarps, 0, st, a);
   return SSD_OK;
 }
 
@@ -1234,7 +1355,7 @@ int launch_cc(cudaStream_t st, const PrefixAttn& a) {
   SSD_PDL((prefix_attention_cc_kernel<T, D>), dim3(a.nsplit, a.hkv, a.tiles), kChunkC, 0, st, a);
   if (a.nsplit == 1) return SSD_OK;
   const int64_t rows = (int64_t)a.B * a.T * a.hq;
-  SSD_PDL((prefix_join_kernel<T, D, kRowsC, false>), (unsigned)((rows + 3) / 4), 128, 0, st, a);
+  SSD_PDL((prefix_join_kernel<T, D, kRowsC, false>), (unsigned)rows, 32 * kJoinWarps, 0, st, a);
   return SSD_OK;
 }
 
@@ -1323,8 +1444,8 @@ extern "C" int ssd_shared_prefix_attention(ssd_stream_t stream, const void* q, c
   a.polls = wait_polls.load(std::memory_order_relaxed);
   a.ws_o = reinterpret_cast<float*>(w);
   a.ws_ml = reinterpret_cast<float2*>(w + L.off_ml);
-  a.plan = reinterpret_cast<int2*>(w + L.off_plan);
-  a.place = reinterpret_cast<int2*>(w + L.off_place);
+  a.parts = reinterpret_cast<int4*>(w + L.off_parts);
+  a.whole = L.whole;
   cudaStream_t st = (cudaStream_t)stream;
   if (L.tc)
     return head_dim == 256   ? launch_tc<256>(st, a, L.ctas)
