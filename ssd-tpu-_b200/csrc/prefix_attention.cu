@@ -114,7 +114,7 @@ struct RowAt {
 };
 template <int D>
 __device__ __forceinline__ RowAt row_at(const PrefixAttn& a, const RowTile& tl, int head, int r, int rows,
-                                        const int* seq_s = nullptr, const int* ql_s = nullptr) {
+                                        const int* seq_s = nullptr, const uint16_t* ql_s = nullptr) {
   RowAt w;
   const int gr = tl.part * rows + r;
   w.seq = a.tps > 1 ? 0 : gr / a.R;
@@ -335,55 +335,66 @@ __global__ void __launch_bounds__(kChunkC) prefix_attention_cc_kernel(const Pref
 // ------------------------------------------------------------------ tensor-core kernel (bf16, pages of 16 k rows)
 // Persistent CTAs, one an SM, share out the positions of all row tiles and KV heads in equal runs of 16 (units), so
 // a CTA works through one or more segments: a run of units of one tile and head.  128 query rows (TMEM lanes) a tile:
-//   S = Q K^T   for TILE positions (M = 128, N = TILE), Q from TMEM, K as it lies in the pages (K-major)
-//   O += P V    (N = D), P in bf16 from the TMEM columns of its own S, V as it lies in the pages (MN-major)
+//   S = Q K^T   for 64 positions (M = 128, N = 64), Q from TMEM, K as it lies in the pages (K-major)
+//   O += P V    (N = D), P in bf16 from TMEM, V as it lies in the pages (MN-major)
 // A unit is 16 rows of one page, so a tile of positions mixes pages of any kind, the prefix's and tails of different
 // sequences; which rows see which of its positions is said by 16 bytes a unit.  Rows that see nothing of a unit put
 // zero weights on it: that wastes products, of which there are enough, and saves bytes, of which there are not.
-//   warps 0-7   two threads a query row, half a tile's positions each: scores out of TMEM, maxima (exchanged between
-//               the two), weights, rescaling of O (only when a row's reference has to move), the result
-//   warp 8      walks the tables and fetches units by TMA into a ring of stages, K and V in turn
-//   warp 9      issues the products: S of tile j + 1 goes before O of tile j, so the weights of one tile are made
-//               while the tensor cores work on the next
+//   warps 0-15  two sets of eight that take tiles of positions in turn, in each two threads a query row with half a
+//               tile's positions each: scores out of TMEM, maxima (exchanged between the two), weights, rescaling of
+//               O (only when a row's reference has to move).  Set 0 also writes results, set 1 brings Q into TMEM.
+//   warp 16     walks the tables and fetches Q and units by TMA into a ring of stages
+//   warp 17     issues the products S: S has one place in TMEM, free again as soon as the scores have been read
+//   warp 18     issues the products with V: the weights have two places, so the tensor cores run while both sets are
+//               at work.  (Two warps: a product's issue and each wait take long enough to hold up the other's.)
+// The sets share a row's reference M through shared memory: tile j decides on it once tile j - 1 has (`decided`), which
+// is early in a tile's work; the weights themselves overlap.
 // A product with weight zero still spreads infinities and NaN of V over rows that do not see them.  Then a row's O is
 // not finite although its sum of weights is, and the row is worked out again by itself, from the pages.
 // All waits are bounded, and a warp's lanes give up together.  A CTA that gives up raises `gave_up`, lets its copies and
-// products end, frees its TMEM and leaves NaN in the rows that it has not finished.
+// products end, frees its TMEM and leaves NaN in the rows that it has not finished.  (A wait for a phase of a barrier is
+// only begun when the phase before is known to be over: parities tell no more apart.)
 namespace tile {
 
 constexpr int ROWS = 128;              // query rows of a CTA: TMEM lanes
-constexpr int SOFT = 256;              // threads of the row warps
-constexpr int THREADS = SOFT + 64;
-constexpr int META = 8;                // tiles whose units are described: more than there are between fetch and use
-constexpr int kMaxTiles = 512;         // also sequences and groups: their numbers are kept in shared memory
+constexpr int TILE = 64;               // positions of a tile
+constexpr int UNITS = TILE / 16;
+constexpr int HALF = TILE / 2;         // positions of a thread
+constexpr int SET = 256;               // threads of a set of row warps
+constexpr int SETW = SET / 32;
+constexpr int THREADS = 2 * SET + 96;
+constexpr int META = 16;               // tiles whose units are described: more than there are between fetch and use
+constexpr int kMaxTiles = 256;         // also sequences and groups: their numbers are kept in shared memory
 constexpr int kMinUnits = 8;           // of a run: shorter ones cost more in prologues and joins than they save
+constexpr int kStart = 24;             // units that the start of a list is worth
 constexpr int kWhole = 64;             // lists of at most so many units are not cut
 constexpr int kMaxTeam = 8;            // CTAs that walk a group's lists side by side
 constexpr float kSpan = 8.f;           // weights are at most 2^8
+constexpr float kNothing = -1e38f;     // M of a row that has seen nothing
 constexpr uint32_t kPolls = 1u << 24;
 __device__ uint32_t gave_up;           // 1 once a CTA's wait ran out
 
 template <int D>
 struct Cfg {
-  static constexpr int TILE = D == 256 ? 64 : 128, UNITS = TILE / 16, STAGES = 6;
-  static constexpr int QST = ROWS / TILE;       // stages that Q takes on its way in
-  static constexpr uint32_t KV = TILE * D * 2;  // bytes of a stage: one tile's K or V
+  static constexpr int STAGES = D == 256 ? 6 : D == 128 ? 12 : 16;
+  static constexpr uint32_t KV = TILE * D * 2;  // bytes of a stage: one tile's K or V; Q takes two
   static constexpr uint32_t ring = STAGES * KV;
-  static constexpr uint32_t stage = ring;                             // float [SOFT][16]: results on their way out
-  static constexpr uint32_t pref = stage + 64 * SOFT;                 // int [kMaxTiles + 1], see Walk
+  static constexpr uint32_t pref = ring;                              // int [kMaxTiles + 1], see Walk
   static constexpr uint32_t units = pref + 4 * (kMaxTiles + 4);       // int [kMaxTiles]: units of each tile
   static constexpr uint32_t info = units + 4 * kMaxTiles;             // int2 [kMaxTiles]
   static constexpr uint32_t seq = info + 8 * kMaxTiles;               // int [kMaxTiles]: lengths,
-  static constexpr uint32_t ql = seq + 4 * kMaxTiles;                 // new tokens of the sequences,
-  static constexpr uint32_t pre = ql + 4 * kMaxTiles;                 // prefixes of the groups
+  static constexpr uint32_t ql = seq + 4 * kMaxTiles;                 // uint16: new tokens of the sequences,
+  static constexpr uint32_t pre = ql + 2 * kMaxTiles;                 // prefixes of the groups
   static constexpr uint32_t cum = pre + 4 * kMaxTiles;                // int [ROWS + 4]: units before a sequence's tail
   static constexpr uint32_t meta = cum + 4 * (ROWS + 4);              // int4 [META][UNITS]
-  static constexpr uint32_t pairs = meta + 16 * META * UNITS;         // float [2][2][ROWS]: the threads' maxima
-  static constexpr uint32_t bars = pairs + 4 * 4 * ROWS;
-  static constexpr uint32_t misc = bars + 8 * (2 * STAGES + META + 12);
+  static constexpr uint32_t pairs = meta + 16 * META * UNITS;         // float [set][turn][half][ROWS]: maxima
+  static constexpr uint32_t refs = pairs + 4 * 8 * ROWS;              // float [tile parity][ROWS]: M
+  static constexpr uint32_t sums = refs + 4 * 2 * ROWS;               // float [segment parity][set, half][ROWS]
+  static constexpr uint32_t bars = sums + 4 * 8 * ROWS;
+  static constexpr uint32_t misc = bars + 8 * (2 * STAGES + 32);
   static constexpr size_t smem = 1024 + misc + 32;
-  // TMEM columns: two tiles' scores (then weights), Q (two bf16 to a column), O
-  static constexpr uint32_t q_col = 2 * TILE, o_col = q_col + D / 2, tmem_cols = 512;
+  // TMEM columns: scores, two tiles' weights (two bf16 to a column), Q (likewise), O
+  static constexpr uint32_t p_col = TILE, q_col = 2 * TILE, o_col = q_col + D / 2, tmem_cols = D == 64 ? 256 : 512;
   static_assert(o_col + D <= tmem_cols);
   static_assert(smem <= 227 * 1024);
   // planning, in the ring's place: group starts, their first tiles
@@ -395,13 +406,19 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// 16 TMEM lanes by 16 fp32 columns: lane L holds columns 2 (L % 4), + 1 of row L / 4 and of row L / 4 + 8, then the same 8
+// columns further on.
+__device__ __forceinline__ void tmem_load_16x16(uint32_t addr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];\n\ttcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+      : "r"(addr)
+      : "memory");
+}
 __device__ __forceinline__ uint4 lds128(uint32_t p) {
   uint4 v;
   asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(p) : "memory");
   return v;
-}
-__device__ __forceinline__ void sts128(uint32_t p, uint4 v) {
-  asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(p), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   uint32_t r;
@@ -413,6 +430,18 @@ __device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile int
   bool ok = false;
   for (uint32_t i = 0; i < polls; ++i) {
     ok = tc::mbar_try_wait(bar, parity);
+    if (ok || ((i & 255u) == 255u && *stop)) break;
+  }
+  if (!ok) *stop = 1;
+  return __all_sync(0xffffffffu, ok);
+}
+// Three waits at once: as a rule all are over.
+__device__ __forceinline__ bool wait3(uint32_t b0, uint32_t p0, uint32_t b1, uint32_t p1, uint32_t b2, uint32_t p2,
+                                      volatile int* stop, uint32_t polls) {
+  bool ok = false;
+  for (uint32_t i = 0; i < polls; ++i) {
+    const bool x = tc::mbar_try_wait(b0, p0), y = tc::mbar_try_wait(b1, p1), z = tc::mbar_try_wait(b2, p2);
+    ok = x && y && z;
     if (ok || ((i & 255u) == 255u && *stop)) break;
   }
   if (!ok) *stop = 1;
@@ -440,61 +469,66 @@ struct Segment {
   RowTile rows;
 };
 // How the units are shared out.  They stand in a row: tile after tile, in each the KV heads, in each the tile's list;
-// every CTA takes a run of them.  Where all groups have the same few (nm) tiles, nm CTAs work as a team: the lists of a
-// group's tiles are walked side by side, one CTA a tile, so that the prefix that they all read is fetched from DRAM
-// once and found in L2 after that.  Where a list is short whatever the lengths (`whole`), runs end with lists: nothing
-// is joined.
+// every CTA takes a run of them.  A list counts kStart units more than it has, about what a CTA loses where it goes on to
+// another list (results out, Q in).  Where all groups have the same few (nm) tiles, nm CTAs work as a team: the lists
+// of a group's tiles are walked side by side, one CTA a tile, so that the prefix that they all read is fetched from
+// DRAM once and found in L2 after that.  Where a list is short whatever the lengths (`whole`), runs end with lists:
+// nothing is joined.
 struct Shares {
   int nm;           // CTAs of a team (1: no teams)
   int runs;         // runs that the units are cut into
-  int64_t all;      // units, over all heads (of the longest list of each group, where there are teams)
+  int all;          // units, over all heads (of the longest list of each group, where there are teams)
   bool whole;
+  __device__ int start(int run) const {  // all * run / runs, without an overflow
+    const int q = all / runs;
+    return run * q + run * (all - q * runs) / runs;
+  }
 };
 struct Walk {
-  int64_t pos, end;
+  int pos, end;
   int at;           // tile (group, where there are teams) that pos is in
   __device__ Walk(const PrefixAttn& a, const Shares& sh, const int* pref, int n) : at(0) {
     const int run = (int)blockIdx.x / sh.nm;
     pos = end = 0;
     if (run >= sh.runs) return;
     if (sh.whole) {
-      const int64_t lists = (int64_t)n * a.hkv, l0 = lists * run / sh.runs, l1 = lists * (run + 1) / sh.runs;
-      auto start = [&](int64_t l) {
-        const int t = (int)(l / a.hkv);
-        return t >= n ? sh.all : (int64_t)pref[t] * a.hkv + (l - (int64_t)t * a.hkv) * (pref[t + 1] - pref[t]);
+      const int lists = n * a.hkv, l0 = lists * run / sh.runs, l1 = lists * (run + 1) / sh.runs;
+      auto start = [&](int l) {
+        const int t = l / a.hkv;
+        return t >= n ? sh.all : pref[t] * a.hkv + (l - t * a.hkv) * (pref[t + 1] - pref[t]);
       };
       pos = start(l0);
       end = start(l1);
     } else {
-      pos = sh.all * run / sh.runs;
-      end = sh.all * (run + 1) / sh.runs;
+      pos = sh.start(run);
+      end = sh.start(run + 1);
     }
     while (n > 1) {  // the last one that starts at or before pos
       const int half = n / 2;
-      if ((int64_t)pref[at + half] * a.hkv <= pos) at += half, n -= half;
+      if (pref[at + half] * a.hkv <= pos) at += half, n -= half;
       else n = half;
     }
   }
   __device__ bool next(const PrefixAttn& a, const Shares& sh, const int* pref, const int* units_s, const int2* info,
                        Segment& s) {
     while (pos < end) {
-      while ((int64_t)pref[at + 1] * a.hkv <= pos) ++at;
-      const int list = pref[at + 1] - pref[at];
-      const int off = (int)(pos - (int64_t)pref[at] * a.hkv);
-      s.head = off / list;
-      s.lo = off - s.head * list;
-      s.hi = (int)min((int64_t)list, s.lo + (end - pos));
-      pos += s.hi - s.lo;
+      while (pref[at + 1] * a.hkv <= pos) ++at;
+      const int list = pref[at + 1] - pref[at], first = pref[at] * a.hkv;
+      s.head = (pos - first) / list;
+      const int base = first + s.head * list + kStart;  // of the list's first unit
       s.tile = at * sh.nm + (int)blockIdx.x % sh.nm;
       const int units = units_s[s.tile];
-      s.hi = min(s.hi, units);
+      s.lo = max(pos - base, 0);
+      s.hi = min(min(base - kStart + list, end) - base, units);
+      pos = min(base - kStart + list, end);
       if (s.lo >= s.hi) continue;
       const bool all = s.lo == 0 && s.hi == units;
       s.slot = all ? -1 : s.lo > 0 ? 2 * (int)blockIdx.x : 2 * (int)blockIdx.x + 1;
       s.parts = 1;
       if (s.lo == 0 && !all) {
-        const int64_t last = (int64_t)pref[at] * a.hkv + (int64_t)s.head * list + units - 1;
-        s.parts = (int)(((last + 1) * sh.runs - 1) / sh.all) - (int)blockIdx.x / sh.nm + 1;
+        int run = (int)blockIdx.x / sh.nm;
+        while (sh.start(run + 1) < base + units) ++run;  // the run that the last unit is in
+        s.parts = run - (int)blockIdx.x / sh.nm + 1;
       }
       const int2 t = info[s.tile];
       s.rows.seq0 = t.x & 0xffff;
@@ -515,12 +549,12 @@ __device__ __forceinline__ int tail_units(const PrefixAttn& a, int seq, int ql, 
   return ql > 0 && n > P ? (n + 15) / 16 - P / 16 : 0;
 }
 
-// Row r of the segment once more, alone: dims [d0, d0 + D / 2) of sum_j w_j v_j over the positions that it sees, weights
+// Row r of the segment once more, alone: dims [d0, d0 + D / 4) of sum_j w_j v_j over the positions that it sees, weights
 // as the tensor cores had them.  For whole warps.
 template <int D>
 __device__ __noinline__ void row_again(const PrefixAttn& a, const Segment& sg, int seq, int pos, int64_t at, float c,
                                        float M, int d0, float k, float* to_f32, bf16* to_bf16) {
-  constexpr int PL = D / 32, HL = D / 64;
+  constexpr int PL = D / 32, HL = D >= 128 ? D / 128 : 1;  // (of 64 dims every second lane's sums are not used)
   const int lane = threadIdx.x & 31;
   const bf16* pages = reinterpret_cast<const bf16*>(a.pages) + a.layer;
   const int P = prefix_of(a, sg.rows.group);
@@ -551,12 +585,13 @@ __device__ __noinline__ void row_again(const PrefixAttn& a, const Segment& sg, i
         for (int i = 0; i < PL; ++i) s = fmaf(q[i], to_f(ld_act(kr + lane + 32 * i)), s);
         const float w = round_bf16(ex2(fmaf(warp_sum(s), c, -M)));
 #pragma unroll
-        for (int i = 0; i < HL; ++i) o[i] = fmaf(w, to_f(ld_act(kr + a.plane + d0 + lane + 32 * i)), o[i]);
+        for (int i = 0; i < HL; ++i) o[i] = fmaf(w, to_f(ld_act(kr + a.plane + d0 + lane % (D / 4) + 32 * i)), o[i]);
       }
     }
   }
 #pragma unroll
   for (int i = 0; i < HL; ++i) {
+    if (lane >= D / 4) continue;
     if (to_f32) to_f32[d0 + lane + 32 * i] = o[i];
     else to_bf16[d0 + lane + 32 * i] = __float2bfloat16_rn(o[i] * k);
   }
@@ -574,9 +609,8 @@ __device__ __forceinline__ void put_parts(const PrefixAttn& a, int2 info, int ti
 template <int D>
 __global__ void __launch_bounds__(THREADS, 1)
 prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ CUtensorMap qmap,
-                           const PrefixAttn a) {
+                           const __grid_constant__ PrefixAttn a) {
   using C = Cfg<D>;
-  constexpr int TILE = C::TILE, UNITS = C::UNITS, HALF = TILE / 2;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = tc::smem_u32(smem_raw), sm = (raw + 1023u) & ~1023u;
   uint8_t* gen = smem_raw + (sm - raw);
@@ -584,20 +618,25 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid
   int* units_s = reinterpret_cast<int*>(gen + C::units);
   int2* info = reinterpret_cast<int2*>(gen + C::info);
   int* seq_s = reinterpret_cast<int*>(gen + C::seq);
-  int* ql_s = reinterpret_cast<int*>(gen + C::ql);
+  uint16_t* ql_s = reinterpret_cast<uint16_t*>(gen + C::ql);
   int* pre_s = reinterpret_cast<int*>(gen + C::pre);
   int* cum = reinterpret_cast<int*>(gen + C::cum);
   int4* meta = reinterpret_cast<int4*>(gen + C::meta);
   float* pair_s = reinterpret_cast<float*>(gen + C::pairs);
+  float* ref_s = reinterpret_cast<float*>(gen + C::refs);
+  float* sum_s = reinterpret_cast<float*>(gen + C::sums);
   auto bar = [&](int i) { return sm + C::bars + 8 * i; };
   auto full = [&](int s) { return bar(s); };
   auto freed = [&](int s) { return bar(C::STAGES + s); };
-  auto meta_full = [&](int s) { return bar(2 * C::STAGES + s); };
-  constexpr int B0 = 2 * C::STAGES + META;
-  auto s_full = [&](int s) { return bar(B0 + s); };
-  auto p_full = [&](int s) { return bar(B0 + 2 + s); };
-  const uint32_t o_done = bar(B0 + 4), q_tmem = bar(B0 + 5), drained = bar(B0 + 6);
-  auto pair = [&](int q) { return bar(B0 + 8 + q); };
+  constexpr int B0 = 2 * C::STAGES;
+  auto s_full = [&](int s) { return bar(B0 + s); };      // scores of a set's tile
+  auto p_full = [&](int s) { return bar(B0 + 2 + s); };  // weights of a set's tile
+  auto added = [&](int s) { return bar(B0 + 4 + s); };   // a set's tile is in O
+  const uint32_t s_free = bar(B0 + 6), q_tmem = bar(B0 + 7), q_free = bar(B0 + 8), o_free = bar(B0 + 9);
+  auto drained = [&](int w) { return bar(B0 + 10 + w); };
+  auto pair = [&](int set, int q) { return bar(B0 + 12 + 4 * set + q); };
+  auto decided = [&](int set, int q) { return bar(B0 + 20 + 4 * set + q); };
+  auto summed = [&](int q) { return bar(B0 + 28 + q); };
   uint32_t* slot = reinterpret_cast<uint32_t*>(gen + C::misc);
   volatile int* stop = reinterpret_cast<volatile int*>(slot + 1);
   auto held = [&](uint32_t b, uint32_t parity) { return wait(b, parity, stop, a.polls); };
@@ -608,18 +647,26 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid
       tc::mbar_init(full(s), 1);
       tc::mbar_init(freed(s), 1);
     }
-    for (int s = 0; s < META; ++s) tc::mbar_init(meta_full(s), 1);
     for (int s = 0; s < 2; ++s) {
       tc::mbar_init(s_full(s), 1);
-      tc::mbar_init(p_full(s), SOFT / 32);
+      tc::mbar_init(p_full(s), SETW);
+      tc::mbar_init(added(s), 1);
+      for (int q = 0; q < 4; ++q) {
+        tc::mbar_init(pair(s, q), 2);
+        tc::mbar_init(decided(s, q), 2);
+      }
     }
-    tc::mbar_init(o_done, 1);
-    tc::mbar_init(q_tmem, SOFT / 32);
-    tc::mbar_init(drained, 1);
-    for (int q = 0; q < 4; ++q) tc::mbar_init(pair(q), 2);
+    for (int q = 0; q < 4; ++q) tc::mbar_init(summed(q), 4);
+    tc::mbar_init(s_free, SETW);
+    tc::mbar_init(q_tmem, SETW);
+    tc::mbar_init(q_free, 1);
+    tc::mbar_init(o_free, 2 * SETW);
+    tc::mbar_init(drained(0), 1);
+    tc::mbar_init(drained(1), 1);
     *stop = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&map) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&qmap) : "memory");
   }
   if (warp == THREADS / 32 - 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc::smem_u32(slot)),
@@ -632,20 +679,27 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid
 
   // ---------------------------------------------------------------- the tiles and their units
   {
+    static_assert(THREADS > kMaxTiles);  // a thread a sequence, group and tile
     int* g_start = reinterpret_cast<int*>(gen);           // [groups + 1]
     int* g_tile = reinterpret_cast<int*>(gen) + kMaxTiles + 1;
-    for (int i = tid; i < a.tiles; i += THREADS) {
-      info[i] = make_int2(0, 0);
-      units_s[i] = 0;
+    int seq = 0, ql = 0, start = 0, P = 0;
+    if (tid < a.B) {
+      seq = ld_act(a.seq_lens + tid);
+      ql = a.q_lens ? ld_act(a.q_lens + tid) : a.T;
     }
-    for (int b = tid; b < a.B; b += THREADS) {
-      seq_s[b] = ld_act(a.seq_lens + b);
-      ql_s[b] = new_tokens(a, b);
+    if (tid <= a.groups) start = ld_act(a.starts + tid);
+    if (tid < a.groups) P = ld_act(a.prefixes + tid);
+    if (tid < a.tiles) {
+      info[tid] = make_int2(0, 0);
+      units_s[tid] = 0;
     }
-    for (int g = tid; g <= a.groups; g += THREADS) {
-      g_start[g] = clamped(ld_act(a.starts + g), a.B);
-      if (g < a.groups) pre_s[g] = prefix_of(a, g);
+    ql = clamped(ql, a.T);
+    if (tid < a.B) {
+      seq_s[tid] = seq;
+      ql_s[tid] = (uint16_t)ql;  // (as many as fit the tiles that there may be)
     }
+    if (tid <= a.groups) g_start[tid] = clamped(start, a.B);
+    if (tid < a.groups) pre_s[tid] = clamped(P, a.cap);
     __syncthreads();
     if (warp == 0) {
       int before = 0, nm = -1;  // nm: tiles of every group; 0: not the same for all
@@ -662,37 +716,41 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid
         if (g < a.groups) g_tile[g] = before + incl - n;
         before += __shfl_sync(0xffffffffu, incl, 31);
       }
-      if (lane == 0) pref[0] = nm > 1 && nm <= kMaxTeam && nm * 4 <= (int)gridDim.x && !a.whole ? nm : 1;
+      if (lane == 0) slot[3] = nm > 1 && nm <= kMaxTeam && nm * 4 <= (int)gridDim.x && !a.whole ? nm : 1;
     }
-    __syncthreads();
-    for (int b = tid; b < a.B; b += THREADS) {
-      int g = 0, n = a.groups;
-      while (n > 1) {  // the last group that starts at or before b
+    int g = 0, s = 0, e = 0;
+    if (tid < a.B) {
+      int n = a.groups;
+      while (n > 1) {  // the last group that starts at or before the sequence
         const int half = n / 2;
-        if (g_start[g + half] <= b) g += half, n -= half;
+        if (g_start[g + half] <= tid) g += half, n -= half;
         else n = half;
       }
-      const int s = g_start[g], e = g_start[g + 1];
-      if (b < s || b >= e) continue;  // starts that are not ascending from 0 to B
-      const int P = pre_s[g], tail = tail_units(a, seq_s[b], ql_s[b], P), k = b - s;
+      s = g_start[g];
+      e = g_start[g + 1];
+      P = pre_s[g];
+    }
+    __syncthreads();
+    if (tid >= s && tid < e) {  // (starts that ascend from 0 to B have every sequence in a group)
+      const int tail = tail_units(a, seq, ql, P), k = tid - s;
       const int t0 = g_tile[g] + (a.tps > 1 ? k * a.tps : k / a.spt);
       const bool lead = a.tps > 1 || k % a.spt == 0;
-      for (int p = 0; p < a.tps; ++p) {
-        if (t0 + p >= a.tiles) break;
+      for (int p = 0; p < a.tps && t0 + p < a.tiles; ++p) {
         atomicAdd(&units_s[t0 + p], tail + (lead ? prefix_units(P) : 0));
-        if (lead) info[t0 + p] = make_int2(b | (a.tps > 1 ? p : min(a.spt, e - b)) << 16, g | s << 16);
+        if (lead) info[t0 + p] = make_int2(tid | (a.tps > 1 ? p : min(a.spt, e - tid)) << 16, g | s << 16);
       }
     }
     __syncthreads();
     if (warp == 0) {
-      const int nm = pref[0], lists = nm > 1 ? a.groups : a.tiles;
+      const int nm = slot[3], lists = nm > 1 ? a.groups : a.tiles;
       int before = 0;
-      __syncwarp();
       for (int t0 = 0; t0 < lists; t0 += 32) {
         const int t = t0 + lane;
         int n = 0;
-        if (t < lists)
+        if (t < lists) {
           for (int i = 0; i < nm; ++i) n = max(n, units_s[t * nm + i]);
+          if (n > 0) n += kStart;
+        }
         int incl = n;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -702,10 +760,7 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid
         if (t < lists) pref[1 + t] = before + incl;
         before += __shfl_sync(0xffffffffu, incl, 31);
       }
-      if (lane == 0) {
-        pref[0] = 0;
-        slot[3] = nm;
-      }
+      if (lane == 0) pref[0] = 0;
     }
     for (int t = blockIdx.x; t < a.tiles; t += gridDim.x) {  // rows that see nothing
       if (units_s[t] != 0) continue;
@@ -725,127 +780,127 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid
   Shares sh;
   sh.nm = slot[3];
   const int lists = sh.nm > 1 ? a.groups : a.tiles;
-  sh.all = (int64_t)pref[lists] * a.hkv;
+  sh.all = pref[lists] * a.hkv;
   sh.whole = a.whole;
-  sh.runs = (int)max((int64_t)1, min((int64_t)((int)gridDim.x / sh.nm), sh.whole ? (int64_t)lists * a.hkv
-                                                                                   : (sh.all + kMinUnits - 1) / kMinUnits));
+  sh.runs = max(1, min((int)gridDim.x / sh.nm, sh.whole ? lists * a.hkv : (sh.all - kStart * lists * a.hkv) / kMinUnits));
   Walk walk(a, sh, pref, lists);
   Segment sg;
   const float c = fmaxf(fabsf(a.scale) * 1.4426950408889634f, 1e-38f);  // not 0: keeps the mask's infinity an infinity
   int jg = 0;  // tiles before this segment
 
-  if (warp < SOFT / 32) {
+  if (warp < 2 * SETW) {
     // -------------------------------------------------------------- rows
-    const int quad = warp & 3, half = warp >> 2;  // TMEM lanes 32 quad .., positions HALF half .. of a tile
-    const int r = quad * 32 + lane;
+    const int quad = warp & 3, half = warp >> 2 & 1, set = warp / SETW;
+    const int r = quad * 32 + lane;               // TMEM lanes 32 quad .., positions HALF half .. of a tile
     const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16);
     int swaps = 0, n = 0;  // n: stages filled before
     bool ok = true;
-    // the row's two threads swap a number; false when the CTA gives up
-    auto swap = [&](float& x) {
-      float* at = pair_s + (swaps & 1) * 2 * ROWS;
-      at[half * ROWS + r] = x;
-      __syncwarp();
-      if (lane == 0) tc::mbar_arrive(pair(quad));
-      if (!held(pair(quad), swaps & 1)) return false;
-      x = at[(half ^ 1) * ROWS + r];
-      ++swaps;
-      return true;
-    };
     for (int seg = 0; walk.next(a, sh, pref, units_s, info, sg); ++seg) {
-      const int tiles = (sg.hi - sg.lo + UNITS - 1) / UNITS;
+      const int tiles = (sg.hi - sg.lo + UNITS - 1) / UNITS, last = jg + tiles - 1;
       const RowAt w = row_at<D>(a, sg.rows, sg.head, r, a.tile_rows, seq_s, ql_s);
-      if (sg.lo == 0 && warp == 0)
+      if (sg.lo == 0 && warp == SETW)
         put_parts(a, info[sg.tile], sg.tile, sg.head, 2 * (int)blockIdx.x + 1, sg.parts, 2 * sh.nm, lane, 32);
       const bool real = w.pos >= 0;
       const bool busy = __any_sync(0xffffffffu, real);
-      // this thread's half of its row of Q out of the ring into TMEM (rows that are not there may hold anything)
+      if (set == 1) {
+        // this thread's half of its row of Q out of the ring into TMEM (rows that are not there may hold anything)
+        ok = ok && (seg == 0 || held(q_free, (seg - 1) & 1)) && held(full(n % C::STAGES), (n / C::STAGES) & 1);
+        if (ok) {
+          tc::tc_fence_after();
+          const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
 #pragma unroll
-      for (int h = 0; h < C::QST; ++h) ok = ok && held(full((n + h) % C::STAGES), ((n + h) / C::STAGES) & 1);
-      if (ok) {
-        constexpr int CH = D / 64;  // lines of 64 dims; ROWS of them a chunk, CH / QST chunks a stage
-        const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
+          for (int i = 0; i < D / 64; ++i) {  // 32 dims at a time: 4 pieces of 16 bytes
+            const int dim = half * (D / 2) + 32 * i;
+            const uint32_t line = sm + (n % C::STAGES) * C::KV + dim / 64 * (ROWS * 128) + r * 128;
+            uint32_t y[16];
 #pragma unroll
-        for (int i = 0; i < D / 32; i += 2) {  // 32 dims at a time: 4 pieces of 16 bytes
-          const int dim = half * (D / 2) + 16 * i;
-          const int ch = dim / 64, st = (n + ch / (CH / C::QST)) % C::STAGES;
-          const uint32_t line = sm + st * C::KV + (ch % (CH / C::QST)) * (ROWS * 128) + r * 128;
-          uint32_t y[16];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const uint4 v = lds128(line + ((((dim % 64) / 8 + k) ^ (r & 7)) << 4));
-            y[4 * k] = v.x ^ flip;
-            y[4 * k + 1] = v.y ^ flip;
-            y[4 * k + 2] = v.z ^ flip;
-            y[4 * k + 3] = v.w ^ flip;
+            for (int k = 0; k < 4; ++k) {
+              const uint4 v = lds128(line + ((((dim % 64) / 8 + k) ^ (r & 7)) << 4));
+              y[4 * k] = v.x ^ flip;
+              y[4 * k + 1] = v.y ^ flip;
+              y[4 * k + 2] = v.z ^ flip;
+              y[4 * k + 3] = v.w ^ flip;
+            }
+            tc::tmem_store16(lanes + C::q_col + dim / 2, y);
           }
-          tc::tmem_store16(lanes + C::q_col + dim / 2, y);
+          asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+          tc::tc_fence_before();
+          __syncwarp();
+          if (lane == 0) tc::mbar_arrive(q_tmem);
         }
-        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-        tc::tc_fence_before();
-        __syncwarp();
-        if (lane == 0) tc::mbar_arrive(q_tmem);
       }
-      n += C::QST + 2 * tiles;
-      // M: what the weights are relative to; -1e38 where nothing has been seen
-      float M = -1e38f, l = 0.f;
+      n += 2 + 2 * tiles;
+      // M: what the weights are relative to
+      float M = kNothing, l = 0.f;
 #pragma unroll 1
-      for (int j = 0; ok && j < tiles; ++j) {
-        const int jt = jg + j, buf = jt & 1;
-        ok = held(s_full(buf), (jt >> 1) & 1) && held(meta_full(jt % META), (jt / META) & 1);
+      for (int jt = jg + ((jg ^ set) & 1); ok && jt <= last; jt += 2) {
+        const bool first = jt == jg;
+        ok = held(s_full(set), (jt >> 1) & 1);  // (and the tile's units are described: that was before K came in)
         if (!ok) break;
         tc::tc_fence_after();
+        uint32_t x[HALF];
+        uint32_t see = 0;
+        bool none = true;
+        float m = kNothing;
         if (busy) {
-          uint32_t x[HALF];
-#pragma unroll
-          for (int i = 0; i < HALF; i += 32) tc::tmem_load32(lanes + buf * TILE + half * HALF + i, x + i);
+          tc::tmem_load32(lanes + half * HALF, x);
           // which of this thread's positions its row sees
-          uint32_t see[HALF / 32];
           const int4* mt = meta + (jt % META) * UNITS + half * (UNITS / 2);
-          bool all_seen = true, none = true;
 #pragma unroll
           for (int u = 0; u < UNITS / 2; ++u) {
-            const int4 m = mt[u];  // first position, positions from, to, whose (-1: every row's)
-            const int to = min(min(m.z, w.pos + 1) - m.x, 16), from = max(m.y - m.x, 0);
+            const int4 d = mt[u];  // first position, positions from, to, whose (-1: every row's)
+            const int to = min(min(d.z, w.pos + 1) - d.x, 16), from = max(d.y - d.x, 0);
             uint32_t bits = to > from ? (0xffffu >> (16 - to)) & (0xffffu << from) : 0u;
-            if (m.w >= 0 && m.w != w.seq) bits = 0;
-            if (u & 1) see[u >> 1] |= bits << 16;
-            else see[u >> 1] = bits;
+            if (d.w >= 0 && d.w != w.seq) bits = 0;
+            see |= bits << (16 * u);
           }
-#pragma unroll
-          for (int i = 0; i < HALF / 32; ++i) {
-            all_seen &= see[i] == 0xffffffffu;
-            none &= see[i] == 0;
-          }
-          all_seen = __all_sync(0xffffffffu, all_seen);
-          none = __all_sync(0xffffffffu, none);
-#pragma unroll
-          for (int i = 0; i < HALF; i += 32) tc::tmem_ready(x + i);
-          float m = -INFINITY;
+          if (!real) see = 0xffffffffu;  // nobody asks for the row: no reason to mask
+          const bool all_seen = __all_sync(0xffffffffu, see == 0xffffffffu);
+          none = !all_seen && __all_sync(0xffffffffu, see == 0 || !real);
+          tc::tmem_ready(x);
+          tc::tc_fence_before();
+          __syncwarp();
+          if (lane == 0) tc::mbar_arrive(s_free);
           if (!none) {
             if (!all_seen) {
 #pragma unroll
               for (int i = 0; i < HALF; ++i)
-                if (!(see[i / 32] >> (i % 32) & 1)) x[i] = 0xff800000u;
+                if (!(see >> i & 1)) x[i] = 0xff800000u;
             }
-            float m2 = -INFINITY;
+            float m0 = -INFINITY, m1 = -INFINITY, m2 = -INFINITY, m3 = -INFINITY;
 #pragma unroll
-            for (int i = 0; i < HALF; i += 4) {
-              m = fmaxf(m, fmaxf(__uint_as_float(x[i]), __uint_as_float(x[i + 1])));
-              m2 = fmaxf(m2, fmaxf(__uint_as_float(x[i + 2]), __uint_as_float(x[i + 3])));
+            for (int i = 0; i < HALF; i += 8) {
+              m0 = fmaxf(m0, fmaxf(__uint_as_float(x[i]), __uint_as_float(x[i + 1])));
+              m1 = fmaxf(m1, fmaxf(__uint_as_float(x[i + 2]), __uint_as_float(x[i + 3])));
+              m2 = fmaxf(m2, fmaxf(__uint_as_float(x[i + 4]), __uint_as_float(x[i + 5])));
+              m3 = fmaxf(m3, fmaxf(__uint_as_float(x[i + 6]), __uint_as_float(x[i + 7])));
             }
-            m = fmaxf(m, m2);
+            m = fmaxf(fmaxf(m0, m1), fmaxf(m2, m3));
+            m = fmaxf(m * c, kNothing);  // a NaN score counts as the lowest value here and spoils the sums
           }
-          m = fmaxf(m * c, -1e38f);  // a NaN score counts as the lowest value here and spoils the sums
-          float mo = m, f = 1.f;
-          ok = swap(mo);
-          if (!ok) break;
-          m = fmaxf(m, mo);
-          if (m > M + kSpan) {
-            // (a row that has seen nothing has zeros in O, or what it is worked out again for: nothing to rescale)
-            if (M > -1e38f) f = ex2(M - m);
-            M = m;
-            l *= f;
+        }
+        if (!busy && lane == 0) tc::mbar_arrive(s_free);
+        float* at = pair_s + (set * 2 + (swaps & 1)) * 2 * ROWS;
+        at[half * ROWS + r] = m;
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(pair(set, quad));
+        // the other half's maxima; the tile before's M; and the weights of two tiles before have been used (`decided`
+        // says that too).  A barrier in its first phase has no phase before that: waits for parity 1 are over.
+        ok = wait3(pair(set, quad), swaps & 1, first ? pair(set, quad) : decided(set ^ 1, quad),
+                   first ? swaps & 1 : ((jt - 1) >> 1) & 1, added(set), ((jt >> 1) - 1) & 1, stop, a.polls);
+        if (!ok) break;
+        ++swaps;
+        const float before = first ? kNothing : ref_s[((jt - 1) & 1) * ROWS + r];
+        m = fmaxf(m, at[(half ^ 1) * ROWS + r]);
+        const bool moved = real && m > before + kSpan;
+        const float now = moved ? m : before;
+        if (half == 0) ref_s[(jt & 1) * ROWS + r] = now;
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(decided(set, quad));
+        if (busy) {
+          if (now != M) {
+            l *= ex2(M - now);
+            M = now;
           }
           uint32_t p[HALF / 2];
           if (none) {
@@ -867,12 +922,15 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid
             }
             l += (s0.x + s0.y) + (s1.x + s1.y);
           }
-          if constexpr (HALF == 32) tc::tmem_store16(lanes + buf * TILE + half * (HALF / 2), p);
-          else tc::tmem_store32(lanes + buf * TILE + half * (HALF / 2), p);
-          if (j > 0 && __any_sync(0xffffffffu, f != 1.f)) {  // half of O each, once the tile before has been added
-            ok = held(o_done, (jt - 1) & 1);
+          tc::tc_fence_after();
+          tc::tmem_store16(lanes + C::p_col + set * (TILE / 2) + half * (HALF / 2), p);
+          // (a row that has seen nothing has zeros in O, or what it is worked out again for: nothing to rescale)
+          const bool shift = moved && before > kNothing;
+          if (__any_sync(0xffffffffu, shift)) {  // half of O each, once the tile before has been added
+            ok = held(added(set ^ 1), ((jt - 1) >> 1) & 1);
             if (!ok) break;
             tc::tc_fence_after();
+            const float f = shift ? ex2(before - now) : 1.f;
 #pragma unroll 1
             for (int i = half * (D / 2); i < (half + 1) * (D / 2); i += 32) {
               uint32_t y[32];
@@ -887,104 +945,98 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid
         }
         tc::tc_fence_before();
         __syncwarp();
-        if (lane == 0) tc::mbar_arrive(p_full(buf));
+        if (lane == 0) tc::mbar_arrive(p_full(set));
       }
-      if (ok && busy) {
-        float lo = l;
-        ok = swap(lo);
-        l += lo;
+      if (ok) {
+        // the row's four threads add up what they have, relative to the last tile's M
+        if ((last & 1) != set) ok = held(decided(set ^ 1, quad), (last >> 1) & 1);
+        const float now = ok ? ref_s[(last & 1) * ROWS + r] : M;
+        float* to = sum_s + (seg & 1) * 4 * ROWS + r;
+        to[(2 * set + half) * ROWS] = l == 0.f ? 0.f : l * ex2(M - now);
+        M = now;
+        __syncwarp();
+        if (ok && lane == 0) tc::mbar_arrive(summed(quad));
+        ok = ok && held(summed(quad), seg & 1);
+        l = (to[0] + to[ROWS]) + (to[2 * ROWS] + to[3 * ROWS]);
       }
-      ok = ok && held(o_done, (jg + tiles - 1) & 1);
-      tc::tc_fence_after();
       jg += tiles;
+      ok = ok && held(added(last & 1), (last >> 1) & 1);
+      tc::tc_fence_after();
       const float nan = __int_as_float(0x7fc00000);
       const bool direct = sg.slot < 0;
-      const int64_t po = (int64_t)max(sg.slot, 0) * ROWS + r;
-      if (!direct && half == 0) a.ws_ml[po] = make_float2(M, !real ? 0.f : ok ? l : nan);
-      bf16* out = reinterpret_cast<bf16*>(a.out) + w.at;
+      const int po = max(sg.slot, 0) * ROWS + quad * 32;
+      if (!direct && half == 0 && set == 0) a.ws_ml[po + lane] = make_float2(M, !real ? 0.f : ok ? l : nan);
+      const bool any = real && l != 0.f;  // l is NaN, not 0, where a seen score is
+      // a row's scale; -1: nothing to write
+      float k = any ? 1.f / l : 0.f;
       if (!ok) {
         if (lane == 0) atomicExch(&gave_up, 1u);
-        if (direct && w.at >= 0)
-#pragma unroll 1
-          for (int d = half * (D / 2); d < (half + 1) * (D / 2); ++d) out[d] = __float2bfloat16_rn(real ? nan : 0.f);
-        continue;
+        k = real ? nan : 0.f;
       }
-      const bool any = real && l != 0.f;  // l is NaN, not 0, where a seen score is
-      const float k = any ? 1.f / l : 0.f;
-      // A warp's 32 rows by 64 bytes go through shared memory, so that a store covers 8 rows of 64 bytes, not 32 of 16.
-      const uint32_t seen = __ballot_sync(0xffffffffu, any), exist = __ballot_sync(0xffffffffu, w.at >= 0);
-      const uint32_t box = sm + C::stage + warp * 2048, mine = box + lane * 64;
-      const int q4 = lane & 3;
-      int64_t at4[4];  // of the rows that this lane stores a quarter of
-      uint32_t put4 = 0;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int row = 8 * i + (lane >> 2);
-        at4[i] = direct ? __shfl_sync(0xffffffffu, w.at, row) : (po - lane + row) * D;
-        put4 |= ((direct ? exist : seen) >> row & 1u) << i;
-      }
-      auto send = [&](const uint32_t* y, char* base, int size, int d) {  // 16 words of each row, dims d ..
-        __syncwarp();
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          sts128(mine + ((i ^ (lane >> 1 & 3)) << 4), make_uint4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]));
-        __syncwarp();
-        uint4 v[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int row = 8 * i + (lane >> 2);
-          v[i] = lds128(box + row * 64 + ((q4 ^ (row >> 1 & 3)) << 4));
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (put4 >> i & 1) *reinterpret_cast<uint4*>(base + (at4[i] + d) * size + 16 * q4) = v[i];
-      };
-      float odd0 = 0.f, odd1 = 0.f;  // NaN once an element is not finite
-      if (busy || (direct && exist)) {
-        uint32_t y[32];
-        const int d0 = half * (D / 2);
-        if (busy) tc::tmem_load32(lanes + C::o_col + d0, y);
+      // A warp takes D / 4 dims of its 32 rows, fragments of 8 rows by 8 dims: a row's 8 dims lie in 4 lanes.
+      const int exist = w.at >= 0 ? (int)(w.at / D) : -1, q4 = 2 * (lane & 3), d0 = (2 * half + set) * (D / 4);
+      uint32_t bad = 0;  // rows that hold an infinity or NaN
 #pragma unroll 1
-        for (int d = d0; d < d0 + D / 2; d += 32) {
-          uint32_t z[32];
-          if (busy) {
-            tc::tmem_ready(y);
+      for (int h = 0; h < 32; h += 16) {
+        const int r0 = h + (lane >> 2), r1 = r0 + 8;
+        const float k0 = __shfl_sync(0xffffffffu, k, r0), k1 = __shfl_sync(0xffffffffu, k, r1);
+        const int e0 = __shfl_sync(0xffffffffu, exist, r0), e1 = __shfl_sync(0xffffffffu, exist, r1);
+        float odd0 = 0.f, odd1 = 0.f;  // NaN once an element is not finite
+#pragma unroll 1
+        for (int d = d0; d < d0 + D / 4; d += 16) {
+          uint32_t y[8];
+          if (ok && busy) {
+            tmem_load_16x16(lanes + ((uint32_t)h << 16) + C::o_col + d, y);
 #pragma unroll
-            for (int i = 0; i < 32; ++i) z[i] = y[i];
-            if (d + 32 < d0 + D / 2) tc::tmem_load32(lanes + C::o_col + d + 32, y);
+            for (int i = 0; i < 2; ++i) {
+              odd0 = fmaf(__uint_as_float(y[4 * i]), 0.f, fmaf(__uint_as_float(y[4 * i + 1]), 0.f, odd0));
+              odd1 = fmaf(__uint_as_float(y[4 * i + 2]), 0.f, fmaf(__uint_as_float(y[4 * i + 3]), 0.f, odd1));
+            }
           } else {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) z[i] = 0;
-          }
-#pragma unroll
-          for (int i = 0; i < 32; i += 2) {
-            odd0 = fmaf(__uint_as_float(z[i]), 0.f, odd0);
-            odd1 = fmaf(__uint_as_float(z[i + 1]), 0.f, odd1);
+            for (int i = 0; i < 8; ++i) y[i] = 0x3f800000u;
           }
           if (direct) {
-            uint32_t p[16];
+            bf16* to = reinterpret_cast<bf16*>(a.out) + d + q4;
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-              p[i] = any ? pack_bf16(__uint_as_float(z[2 * i]) * k, __uint_as_float(z[2 * i + 1]) * k) : 0u;
-            send(p, reinterpret_cast<char*>(a.out), 2, d);
+            for (int i = 0; i < 2; ++i) {
+              // (O may be anything where a row sees nothing)
+              const uint32_t z0 = k0 == 0.f ? 0u : pack_bf16(__uint_as_float(y[4 * i]) * k0, __uint_as_float(y[4 * i + 1]) * k0);
+              const uint32_t z1 = k1 == 0.f ? 0u : pack_bf16(__uint_as_float(y[4 * i + 2]) * k1, __uint_as_float(y[4 * i + 3]) * k1);
+              if (e0 >= 0) *reinterpret_cast<uint32_t*>(to + (int64_t)e0 * D + 8 * i) = z0;
+              if (e1 >= 0) *reinterpret_cast<uint32_t*>(to + (int64_t)e1 * D + 8 * i) = z1;
+            }
           } else {
-            send(z, reinterpret_cast<char*>(a.ws_o), 4, d);
-            send(z + 16, reinterpret_cast<char*>(a.ws_o), 4, d + 16);
+            float* to = a.ws_o + (int64_t)po * D + d + q4;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              if (k0 != 0.f) *reinterpret_cast<uint2*>(to + r0 * D + 8 * i) = make_uint2(y[4 * i], y[4 * i + 1]);
+              if (k1 != 0.f) *reinterpret_cast<uint2*>(to + r1 * D + 8 * i) = make_uint2(y[4 * i + 2], y[4 * i + 3]);
+            }
           }
         }
+        // the lanes of a row are four in a row
+        const uint32_t b0 = __ballot_sync(0xffffffffu, odd0 != 0.f), b1 = __ballot_sync(0xffffffffu, odd1 != 0.f);
+        if (b0 | b1)
+          for (int i = 0; i < 8; ++i) {
+            if (b0 >> (4 * i) & 15u) bad |= 1u << (h + i);
+            if (b1 >> (4 * i) & 15u) bad |= 1u << (h + 8 + i);
+          }
       }
-      const bool odd = any && odd0 + odd1 != 0.f;
       // rows that V's infinities or NaN have reached: seen ones come out as they are, others are taken out
-      for (uint32_t left = __ballot_sync(0xffffffffu, odd && l == l); left; left &= left - 1) {
+      for (uint32_t left = __ballot_sync(0xffffffffu, any && l == l && (bad >> lane & 1)); left; left &= left - 1) {
         const int from = __ffs(left) - 1;
-        const int64_t at = __shfl_sync(0xffffffffu, w.at, from), pr = __shfl_sync(0xffffffffu, po, from);
+        const int64_t at = __shfl_sync(0xffffffffu, w.at, from);
         row_again<D>(a, sg, __shfl_sync(0xffffffffu, w.seq, from), __shfl_sync(0xffffffffu, w.pos, from), at, c,
-                     __shfl_sync(0xffffffffu, M, from), half * (D / 2), __shfl_sync(0xffffffffu, k, from),
-                     direct ? nullptr : a.ws_o + pr * D, direct ? reinterpret_cast<bf16*>(a.out) + at : nullptr);
+                     __shfl_sync(0xffffffffu, M, from), d0, __shfl_sync(0xffffffffu, k, from),
+                     direct ? nullptr : a.ws_o + (int64_t)(po + from) * D,
+                     direct ? reinterpret_cast<bf16*>(a.out) + at : nullptr);
       }
       tc::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) tc::mbar_arrive(o_free);
     }
-  } else if (warp == SOFT / 32) {
+  } else if (warp == 2 * SETW) {
     // -------------------------------------------------------------- pages
     const int64_t rows_plane = (int64_t)a.num_layers * a.num_blocks * a.block_size;
     const int64_t row_layer = (int64_t)a.layer_no * a.num_blocks * a.block_size;
@@ -1046,25 +1098,21 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid
         vrow[0] = row;
       };
       look(0);
-      // Q: rows of all of the tile's tokens and heads, a box of 64 dims at a time
+      // Q: rows of all of the tile's tokens and heads, a box of 64 dims at a time, into two stages that lie side by side
 #pragma unroll
-      for (int h = 0; h < C::QST; ++h) {
-        const int s = n % C::STAGES;
-        if (n >= C::STAGES && !held(freed(s), (n / C::STAGES - 1) & 1)) {
-          ok = false;
-          break;
-        }
-        if (lead) {
-          constexpr int CS = D / 64 / C::QST;
-          tc::mbar_expect_tx(full(s), CS * a.q_box * 128);
+      for (int h = 0; h < 2; ++h) ok = ok && (n + h < C::STAGES || held(freed((n + h) % C::STAGES), ((n + h) / C::STAGES - 1) & 1));
+      if (!ok) break;
+      if (lead) {
+        const int st = n % C::STAGES;
+        tc::mbar_expect_tx(full(st), D / 64 * a.q_box * 128);
+        tc::mbar_arrive(full(st + 1));
 #pragma unroll
-          for (int ch = 0; ch < CS; ++ch)
-            tma_rows(sm + s * C::KV + ch * (ROWS * 128), &qmap, full(s), h * CS + ch, sg.head * a.G,
-                     sg.rows.seq0 * a.T + sg.rows.part * (a.tile_rows / a.G));
-        }
-        __syncwarp();
-        ++n;
+        for (int ch = 0; ch < D / 64; ++ch)
+          tma_rows(sm + st * C::KV + ch * (ROWS * 128), &qmap, full(st), ch, sg.head * a.G,
+                   sg.rows.seq0 * a.T + sg.rows.part * (a.tile_rows / a.G));
       }
+      __syncwarp();
+      n += 2;
       auto fetch = [&](int row_of_lane, int in_batch, int64_t base, int plane) {
         const int s = n % C::STAGES;
         if (n >= C::STAGES && !held(freed(s), (n / C::STAGES - 1) & 1)) return false;
@@ -1084,7 +1132,7 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid
         ++n;
         return true;
       };
-      for (int j = 0; ok && j <= tiles; ++j) {
+      for (int j = 0; ok && j < tiles + 2; ++j) {  // K of tile j, V of tile j - 2: the order of the products
         if (j < tiles) {
           if (j % BATCH == 0) {
             advance();
@@ -1093,10 +1141,10 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid
           const int jt = jg + j;
           if (lane / UNITS == j % BATCH) meta[(jt % META) * UNITS + lane % UNITS] = m;
           __syncwarp();
-          if (lane == 0) tc::mbar_arrive(meta_full(jt % META));
           ok = fetch(vrow[0], j % BATCH, row_layer, 0);
         }
-        if (ok && j > 0) ok = fetch(j < tiles && j % BATCH == 0 ? vrow[1] : vrow[0], (j - 1) % BATCH, row_layer, 1);
+        if (ok && j >= 2 && j - 2 < tiles)
+          ok = fetch((j - 2) / BATCH == min(j, tiles - 1) / BATCH ? vrow[0] : vrow[1], (j - 2) % BATCH, row_layer, 1);
       }
       jg += tiles;
     }
@@ -1111,61 +1159,65 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid
     // registers.
     uint32_t lead;
     asm volatile("{.reg .pred p; elect.sync _|p, 0xffffffff; selp.u32 %0, 1, 0, p;}" : "=r"(lead));
-    int n = 0;
+    int n = 0;  // stages before this segment's
     bool ok = true;
     auto ready = [&](uint32_t b, uint32_t parity) {
       const bool yes = held(b, parity);
       tc::tc_fence_after();
       return yes;
     };
-    auto scores = [&](int jt) {
-      const int s = n % C::STAGES;
-      if (!ready(full(s), (n / C::STAGES) & 1)) return false;
-      const uint64_t kd = tc::sw128_desc(sm + s * C::KV);
-      if (lead) {
-#pragma unroll
-        for (int d = 0; d < D / 64; ++d)
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            tc::umma_ts(tmem + (jt & 1) * TILE, tmem + C::q_col + d * 32 + 8 * k, kd + d * ((TILE * 128) >> 4) + 2 * k,
-                        idesc<TILE, false>(), d || k);
-        tc::umma_commit(freed(s));
-        tc::umma_commit(s_full(jt & 1));
-      }
-      ++n;
-      return true;
-    };
     for (int seg = 0; ok && walk.next(a, sh, pref, units_s, info, sg); ++seg) {
       const int tiles = (sg.hi - sg.lo + UNITS - 1) / UNITS;
-      ok = ready(q_tmem, seg & 1);
-      if (!ok) break;
-#pragma unroll
-      for (int h = 0; h < C::QST; ++h, ++n)
-        if (lead) tc::mbar_arrive(freed(n % C::STAGES));  // Q has left the ring
-      ok = scores(jg);
-#pragma unroll 1
-      for (int j = 0; ok && j < tiles; ++j) {
-        const int jt = jg + j;
-        if (j + 1 < tiles) ok = scores(jt + 1);
-        const int s = n % C::STAGES;
-        ok = ok && ready(p_full(jt & 1), (jt >> 1) & 1) && ready(full(s), (n / C::STAGES) & 1);
+      if (warp == 2 * SETW + 1) {
+        ok = ready(q_tmem, seg & 1);
         if (!ok) break;
-        const uint64_t vd = tc::mn128_desc<TILE>(sm + s * C::KV);
-        if (lead) {
-#pragma unroll
-          for (int k = 0; k < TILE / 16; ++k)  // 16 positions: 8 columns of P, two groups of 8 rows of V
-            tc::umma_ts(tmem + C::o_col, tmem + (jt & 1) * TILE + 8 * k, vd + (2048 >> 4) * k, idesc<D, true>(),
-                        j || k);
-          tc::umma_commit(freed(s));
-          tc::umma_commit(o_done);
+        if (lead) {  // Q has left the ring
+          tc::mbar_arrive(freed(n % C::STAGES));
+          tc::mbar_arrive(freed(n % C::STAGES + 1));
         }
-        ++n;
+#pragma unroll 1
+        for (int j = 0; j < tiles; ++j) {
+          const int jt = jg + j, at = n + (j < 2 ? j + 2 : 2 * j), s = at % C::STAGES;
+          ok = ready(full(s), (at / C::STAGES) & 1) && (jt == 0 || ready(s_free, (jt - 1) & 1));
+          if (!ok) break;
+          const uint64_t kd = tc::sw128_desc(sm + s * C::KV);
+          if (lead) {
+#pragma unroll
+            for (int d = 0; d < D / 64; ++d)
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                tc::umma_ts(tmem, tmem + C::q_col + d * 32 + 8 * k, kd + d * ((TILE * 128) >> 4) + 2 * k,
+                            idesc<TILE, false>(), d || k);
+            tc::umma_commit(s_full(jt & 1));
+            tc::umma_commit(freed(s));
+            if (j == tiles - 1) tc::umma_commit(q_free);
+          }
+        }
+      } else {
+        ok = seg == 0 || ready(o_free, (seg - 1) & 1);
+#pragma unroll 1
+        for (int j = 0; ok && j < tiles; ++j) {
+          const int jt = jg + j, at = n + 2 * j + 3 + min(tiles - 1 - j, 2), s = at % C::STAGES;
+          ok = ready(full(s), (at / C::STAGES) & 1) && ready(p_full(jt & 1), (jt >> 1) & 1);
+          if (!ok) break;
+          const uint64_t vd = tc::mn128_desc<TILE>(sm + s * C::KV);
+          if (lead) {
+#pragma unroll
+            for (int k = 0; k < TILE / 16; ++k)  // 16 positions: 8 columns of P, two groups of 8 rows of V
+              tc::umma_ts(tmem + C::o_col, tmem + C::p_col + (jt & 1) * (TILE / 2) + 8 * k, vd + (2048 >> 4) * k,
+                          idesc<D, true>(), j || k);
+            tc::umma_commit(added(jt & 1));
+            tc::umma_commit(freed(s));
+          }
+        }
       }
+      n += 2 + 2 * tiles;
       jg += tiles;
     }
     if (!ok) {  // let the products issued so far end before TMEM goes back
-      if (lead) tc::umma_commit(drained);
-      for (uint32_t i = 0; i < kPolls && !tc::mbar_try_wait(drained, 0); ++i) {}
+      const uint32_t mine = drained(warp & 1);
+      if (lead) tc::umma_commit(mine);
+      for (uint32_t i = 0; i < kPolls && !tc::mbar_try_wait(mine, 0); ++i) {}
     }
     __syncwarp();
   }
@@ -1308,7 +1360,9 @@ PrefixLayout prefix_layout(int dtype, int B, int T, int hq, int hkv, int D, int 
   const int G = hq / hkv;
   if (dtype == SSD_DTYPE_BF16 && block_size % 16 == 0 && G <= tile::ROWS) {
     tiles_of(tile::ROWS / G * G);  // whole tokens
-    L.tc = L.tiles <= tile::kMaxTiles && B <= tile::kMaxTiles && groups <= tile::kMaxTiles;
+    // (the units are counted in 32 bits)
+    L.tc = L.tiles <= tile::kMaxTiles && B <= tile::kMaxTiles && groups <= tile::kMaxTiles &&
+           (((int64_t)max_seq_len + 15) / 16 + tile::kStart) * (L.tiles + B) * hkv < (1 << 30);
   }
   const int64_t units = ((int64_t)max_seq_len + 15) / 16;  // of a sequence
   if (L.tc) {
