@@ -344,9 +344,8 @@ __global__ void __launch_bounds__(kChunkC) prefix_attention_cc_kernel(const Pref
 //               tile's positions each: scores out of TMEM, maxima (exchanged between the two), weights, rescaling of
 //               O (only when a row's reference has to move).  Set 0 also writes results, set 1 brings Q into TMEM.
 //   warp 16     walks the tables and fetches Q and units by TMA into a ring of stages
-//   warp 17     issues the products S: S has one place in TMEM, free again as soon as the scores have been read
-//   warp 18     issues the products with V: the weights have two places, so the tensor cores run while both sets are
-//               at work.  (Two warps: a product's issue and each wait take long enough to hold up the other's.)
+//   warp 17     issues the products in the order S(j + 2), O(j): S has one place in TMEM, free again as soon as the
+//               scores have been read (O(j) runs meanwhile), and the weights two
 // The sets share a row's reference M through shared memory: tile j decides on it once tile j - 1 has (`decided`), which
 // is early in a tile's work; the weights themselves overlap.
 // A product with weight zero still spreads infinities and NaN of V over rows that do not see them.  Then a row's O is
@@ -362,7 +361,7 @@ constexpr int UNITS = TILE / 16;
 constexpr int HALF = TILE / 2;         // positions of a thread
 constexpr int SET = 256;               // threads of a set of row warps
 constexpr int SETW = SET / 32;
-constexpr int THREADS = 2 * SET + 96;
+constexpr int THREADS = 2 * SET + 64;
 constexpr int META = 16;               // tiles whose units are described: more than there are between fetch and use
 constexpr int kMaxTiles = 256;         // also sequences and groups: their numbers are kept in shared memory
 constexpr int kMinUnits = 8;           // of a run: shorter ones cost more in prologues and joins than they save
@@ -406,14 +405,35 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-// 16 TMEM lanes by 16 fp32 columns: lane L holds columns 2 (L % 4), + 1 of row L / 4 and of row L / 4 + 8, then the same 8
-// columns further on.
-__device__ __forceinline__ void tmem_load_16x16(uint32_t addr, uint32_t* r) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];\n\ttcgen05.wait::ld.sync.aligned;"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
-      : "r"(addr)
-      : "memory");
+// 16 TMEM lanes by N fp32 columns (16, 32 or 64): lane L holds, of every 8 columns, 2 (L % 4) and the one behind it of row
+// L / 4 (r[0], r[1]) and of row L / 4 + 8 (r[2], r[3]).
+template <int N>
+__device__ __forceinline__ void tmem_fragments(uint32_t addr, uint32_t* r) {
+  if constexpr (N == 16) {
+    asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];\n\ttcgen05.wait::ld.sync.aligned;"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7])
+                 : "r"(addr)
+                 : "memory");
+  } else if constexpr (N == 32) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(addr)
+        : "memory");
+  } else {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(addr)
+        : "memory");
+  }
 }
 __device__ __forceinline__ uint4 lds128(uint32_t p) {
   uint4 v;
@@ -425,27 +445,45 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
-// For whole warps: true in every lane, or false in every lane.
-__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile int* stop, uint32_t polls) {
-  bool ok = false;
-  for (uint32_t i = 0; i < polls; ++i) {
-    ok = tc::mbar_try_wait(bar, parity);
-    if (ok || ((i & 255u) == 255u && *stop)) break;
-  }
-  if (!ok) *stop = 1;
-  return __all_sync(0xffffffffu, ok);
+// Two or three waits at once, as a rule over: the polls stand in one block so that their latencies overlap.
+__device__ __forceinline__ bool try2(uint32_t b0, uint32_t p0, uint32_t b1, uint32_t p1) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 q, [%3], %4;\n\t"
+      "and.pred p, p, q;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(b0), "r"(p0), "r"(b1), "r"(p1)
+      : "memory");
+  return ok != 0;
 }
-// Three waits at once: as a rule all are over.
-__device__ __forceinline__ bool wait3(uint32_t b0, uint32_t p0, uint32_t b1, uint32_t p1, uint32_t b2, uint32_t p2,
-                                      volatile int* stop, uint32_t polls) {
-  bool ok = false;
-  for (uint32_t i = 0; i < polls; ++i) {
-    const bool x = tc::mbar_try_wait(b0, p0), y = tc::mbar_try_wait(b1, p1), z = tc::mbar_try_wait(b2, p2);
-    ok = x && y && z;
-    if (ok || ((i & 255u) == 255u && *stop)) break;
+__device__ __forceinline__ bool try3(uint32_t b0, uint32_t p0, uint32_t b1, uint32_t p1, uint32_t b2, uint32_t p2) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p, q, r;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 q, [%3], %4;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 r, [%5], %6;\n\t"
+      "and.pred p, p, q;\n\t"
+      "and.pred p, p, r;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(b0), "r"(p0), "r"(b1), "r"(p1), "r"(b2), "r"(p2)
+      : "memory");
+  return ok != 0;
+}
+// For whole warps: true in every lane, or false in every lane (the branches are uniform: a wait that is over costs
+// little more than its poll).
+template <typename Poll>
+__device__ __forceinline__ bool wait_for(Poll poll, volatile int* stop, uint32_t polls) {
+  for (uint32_t i = 0;; ++i) {
+    if (__all_sync(0xffffffffu, poll())) return true;
+    if (i >= polls || ((i & 255u) == 255u && __any_sync(0xffffffffu, *stop))) break;
   }
-  if (!ok) *stop = 1;
-  return __all_sync(0xffffffffu, ok);
+  *stop = 1;
+  return false;
 }
 // bf16 operands, fp32 accumulator, M = 128; B's long side contiguous (MN-major) or not.
 template <int N, bool B_MN>
@@ -632,14 +670,16 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid
   auto s_full = [&](int s) { return bar(B0 + s); };      // scores of a set's tile
   auto p_full = [&](int s) { return bar(B0 + 2 + s); };  // weights of a set's tile
   auto added = [&](int s) { return bar(B0 + 4 + s); };   // a set's tile is in O
-  const uint32_t s_free = bar(B0 + 6), q_tmem = bar(B0 + 7), q_free = bar(B0 + 8), o_free = bar(B0 + 9);
-  auto drained = [&](int w) { return bar(B0 + 10 + w); };
+  const uint32_t s_free = bar(B0 + 6), q_tmem = bar(B0 + 7), q_free = bar(B0 + 8), o_free = bar(B0 + 9),
+                 drained = bar(B0 + 10);
   auto pair = [&](int set, int q) { return bar(B0 + 12 + 4 * set + q); };
   auto decided = [&](int set, int q) { return bar(B0 + 20 + 4 * set + q); };
   auto summed = [&](int q) { return bar(B0 + 28 + q); };
   uint32_t* slot = reinterpret_cast<uint32_t*>(gen + C::misc);
   volatile int* stop = reinterpret_cast<volatile int*>(slot + 1);
-  auto held = [&](uint32_t b, uint32_t parity) { return wait(b, parity, stop, a.polls); };
+  auto held = [&](uint32_t b, uint32_t parity) {
+    return wait_for([&] { return tc::mbar_try_wait(b, parity); }, stop, a.polls);
+  };
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   if (tid == 0) {
@@ -661,8 +701,7 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid
     tc::mbar_init(q_tmem, SETW);
     tc::mbar_init(q_free, 1);
     tc::mbar_init(o_free, 2 * SETW);
-    tc::mbar_init(drained(0), 1);
-    tc::mbar_init(drained(1), 1);
+    tc::mbar_init(drained, 1);
     *stop = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&map) : "memory");
@@ -886,8 +925,9 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid
         if (lane == 0) tc::mbar_arrive(pair(set, quad));
         // the other half's maxima; the tile before's M; and the weights of two tiles before have been used (`decided`
         // says that too).  A barrier in its first phase has no phase before that: waits for parity 1 are over.
-        ok = wait3(pair(set, quad), swaps & 1, first ? pair(set, quad) : decided(set ^ 1, quad),
-                   first ? swaps & 1 : ((jt - 1) >> 1) & 1, added(set), ((jt >> 1) - 1) & 1, stop, a.polls);
+        const uint32_t b0 = pair(set, quad), b1 = first ? b0 : decided(set ^ 1, quad), p0 = swaps & 1,
+                       p1 = first ? p0 : ((jt - 1) >> 1) & 1;
+        ok = wait_for([&] { return try3(b0, p0, b1, p1, added(set), ((jt >> 1) - 1) & 1); }, stop, a.polls);
         if (!ok) break;
         ++swaps;
         const float before = first ? kNothing : ref_s[((jt - 1) & 1) * ROWS + r];
@@ -982,37 +1022,45 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid
         const float k0 = __shfl_sync(0xffffffffu, k, r0), k1 = __shfl_sync(0xffffffffu, k, r1);
         const int e0 = __shfl_sync(0xffffffffu, exist, r0), e1 = __shfl_sync(0xffffffffu, exist, r1);
         float odd0 = 0.f, odd1 = 0.f;  // NaN once an element is not finite
-#pragma unroll 1
-        for (int d = d0; d < d0 + D / 4; d += 16) {
-          uint32_t y[8];
-          if (ok && busy) {
-            tmem_load_16x16(lanes + ((uint32_t)h << 16) + C::o_col + d, y);
+        constexpr int NF = D / 32;  // fragments of 8 dims
+        uint32_t y[4 * NF];
+        if (ok && busy) {
+          tmem_fragments<D / 4>(lanes + ((uint32_t)h << 16) + C::o_col + d0, y);
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              odd0 = fmaf(__uint_as_float(y[4 * i]), 0.f, fmaf(__uint_as_float(y[4 * i + 1]), 0.f, odd0));
-              odd1 = fmaf(__uint_as_float(y[4 * i + 2]), 0.f, fmaf(__uint_as_float(y[4 * i + 3]), 0.f, odd1));
-            }
-          } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) y[i] = 0x3f800000u;
+          for (int i = 0; i < NF; ++i) {
+            odd0 = fmaf(__uint_as_float(y[4 * i]), 0.f, fmaf(__uint_as_float(y[4 * i + 1]), 0.f, odd0));
+            odd1 = fmaf(__uint_as_float(y[4 * i + 2]), 0.f, fmaf(__uint_as_float(y[4 * i + 3]), 0.f, odd1));
           }
-          if (direct) {
-            bf16* to = reinterpret_cast<bf16*>(a.out) + d + q4;
+        } else {
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              // (O may be anything where a row sees nothing)
-              const uint32_t z0 = k0 == 0.f ? 0u : pack_bf16(__uint_as_float(y[4 * i]) * k0, __uint_as_float(y[4 * i + 1]) * k0);
-              const uint32_t z1 = k1 == 0.f ? 0u : pack_bf16(__uint_as_float(y[4 * i + 2]) * k1, __uint_as_float(y[4 * i + 3]) * k1);
-              if (e0 >= 0) *reinterpret_cast<uint32_t*>(to + (int64_t)e0 * D + 8 * i) = z0;
-              if (e1 >= 0) *reinterpret_cast<uint32_t*>(to + (int64_t)e1 * D + 8 * i) = z1;
-            }
-          } else {
-            float* to = a.ws_o + (int64_t)po * D + d + q4;
+          for (int i = 0; i < 4 * NF; ++i) y[i] = 0x3f800000u;
+        }
+        if (direct) {
+          // (O may be anything where a row sees nothing)
+          bf16* to = reinterpret_cast<bf16*>(a.out) + d0 + q4;
+          if (e0 >= 0) {
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              if (k0 != 0.f) *reinterpret_cast<uint2*>(to + r0 * D + 8 * i) = make_uint2(y[4 * i], y[4 * i + 1]);
-              if (k1 != 0.f) *reinterpret_cast<uint2*>(to + r1 * D + 8 * i) = make_uint2(y[4 * i + 2], y[4 * i + 3]);
-            }
+            for (int i = 0; i < NF; ++i)
+              *reinterpret_cast<uint32_t*>(to + (int64_t)e0 * D + 8 * i) =
+                  k0 == 0.f ? 0u : pack_bf16(__uint_as_float(y[4 * i]) * k0, __uint_as_float(y[4 * i + 1]) * k0);
+          }
+          if (e1 >= 0) {
+#pragma unroll
+            for (int i = 0; i < NF; ++i)
+              *reinterpret_cast<uint32_t*>(to + (int64_t)e1 * D + 8 * i) =
+                  k1 == 0.f ? 0u : pack_bf16(__uint_as_float(y[4 * i + 2]) * k1, __uint_as_float(y[4 * i + 3]) * k1);
+          }
+        } else {
+          float* to = a.ws_o + (int64_t)po * D + d0 + q4;
+          if (k0 != 0.f) {
+#pragma unroll
+            for (int i = 0; i < NF; ++i)
+              *reinterpret_cast<uint2*>(to + r0 * D + 8 * i) = make_uint2(y[4 * i], y[4 * i + 1]);
+          }
+          if (k1 != 0.f) {
+#pragma unroll
+            for (int i = 0; i < NF; ++i)
+              *reinterpret_cast<uint2*>(to + r1 * D + 8 * i) = make_uint2(y[4 * i + 2], y[4 * i + 3]);
           }
         }
         // the lanes of a row are four in a row
@@ -1159,65 +1207,65 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid
     // registers.
     uint32_t lead;
     asm volatile("{.reg .pred p; elect.sync _|p, 0xffffffff; selp.u32 %0, 1, 0, p;}" : "=r"(lead));
-    int n = 0;  // stages before this segment's
+    int n = 0;
     bool ok = true;
-    auto ready = [&](uint32_t b, uint32_t parity) {
-      const bool yes = held(b, parity);
+    auto ready = [&](uint32_t b0, uint32_t p0, uint32_t b1, uint32_t p1) {
+      const bool yes = wait_for([&] { return try2(b0, p0, b1, p1); }, stop, a.polls);
       tc::tc_fence_after();
       return yes;
     };
+    auto scores = [&](int jt, bool is_last) {
+      const int s = n % C::STAGES;
+      // (no scores before the first ones: a wait for parity 1 of a barrier in its first phase is over)
+      if (!ready(full(s), (n / C::STAGES) & 1, s_free, (jt - 1) & 1)) return false;
+      const uint64_t kd = tc::sw128_desc(sm + s * C::KV);
+      if (lead) {
+#pragma unroll
+        for (int d = 0; d < D / 64; ++d)
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            tc::umma_ts(tmem, tmem + C::q_col + d * 32 + 8 * k, kd + d * ((TILE * 128) >> 4) + 2 * k,
+                        idesc<TILE, false>(), d || k);
+        tc::umma_commit(s_full(jt & 1));
+        tc::umma_commit(freed(s));
+        if (is_last) tc::umma_commit(q_free);
+      }
+      ++n;
+      return true;
+    };
     for (int seg = 0; ok && walk.next(a, sh, pref, units_s, info, sg); ++seg) {
       const int tiles = (sg.hi - sg.lo + UNITS - 1) / UNITS;
-      if (warp == 2 * SETW + 1) {
-        ok = ready(q_tmem, seg & 1);
-        if (!ok) break;
-        if (lead) {  // Q has left the ring
-          tc::mbar_arrive(freed(n % C::STAGES));
-          tc::mbar_arrive(freed(n % C::STAGES + 1));
-        }
-#pragma unroll 1
-        for (int j = 0; j < tiles; ++j) {
-          const int jt = jg + j, at = n + (j < 2 ? j + 2 : 2 * j), s = at % C::STAGES;
-          ok = ready(full(s), (at / C::STAGES) & 1) && (jt == 0 || ready(s_free, (jt - 1) & 1));
-          if (!ok) break;
-          const uint64_t kd = tc::sw128_desc(sm + s * C::KV);
-          if (lead) {
-#pragma unroll
-            for (int d = 0; d < D / 64; ++d)
-#pragma unroll
-              for (int k = 0; k < 4; ++k)
-                tc::umma_ts(tmem, tmem + C::q_col + d * 32 + 8 * k, kd + d * ((TILE * 128) >> 4) + 2 * k,
-                            idesc<TILE, false>(), d || k);
-            tc::umma_commit(s_full(jt & 1));
-            tc::umma_commit(freed(s));
-            if (j == tiles - 1) tc::umma_commit(q_free);
-          }
-        }
-      } else {
-        ok = seg == 0 || ready(o_free, (seg - 1) & 1);
-#pragma unroll 1
-        for (int j = 0; ok && j < tiles; ++j) {
-          const int jt = jg + j, at = n + 2 * j + 3 + min(tiles - 1 - j, 2), s = at % C::STAGES;
-          ok = ready(full(s), (at / C::STAGES) & 1) && ready(p_full(jt & 1), (jt >> 1) & 1);
-          if (!ok) break;
-          const uint64_t vd = tc::mn128_desc<TILE>(sm + s * C::KV);
-          if (lead) {
-#pragma unroll
-            for (int k = 0; k < TILE / 16; ++k)  // 16 positions: 8 columns of P, two groups of 8 rows of V
-              tc::umma_ts(tmem + C::o_col, tmem + C::p_col + (jt & 1) * (TILE / 2) + 8 * k, vd + (2048 >> 4) * k,
-                          idesc<D, true>(), j || k);
-            tc::umma_commit(added(jt & 1));
-            tc::umma_commit(freed(s));
-          }
-        }
+      ok = ready(q_tmem, seg & 1, q_tmem, seg & 1);
+      if (!ok) break;
+      if (lead) {  // Q has left the ring
+        tc::mbar_arrive(freed(n % C::STAGES));
+        tc::mbar_arrive(freed(n % C::STAGES + 1));
       }
-      n += 2 + 2 * tiles;
+      n += 2;
+      ok = scores(jg, tiles == 1) && (tiles < 2 || scores(jg + 1, tiles == 2)) && ready(o_free, (seg - 1) & 1, o_free, (seg - 1) & 1);
+#pragma unroll 1
+      for (int j = 0; ok && j < tiles; ++j) {
+        const int jt = jg + j;
+        if (j + 2 < tiles) ok = scores(jt + 2, j + 3 == tiles);
+        const int s = n % C::STAGES;
+        ok = ok && ready(full(s), (n / C::STAGES) & 1, p_full(jt & 1), (jt >> 1) & 1);
+        if (!ok) break;
+        const uint64_t vd = tc::mn128_desc<TILE>(sm + s * C::KV);
+        if (lead) {
+#pragma unroll
+          for (int k = 0; k < TILE / 16; ++k)  // 16 positions: 8 columns of P, two groups of 8 rows of V
+            tc::umma_ts(tmem + C::o_col, tmem + C::p_col + (jt & 1) * (TILE / 2) + 8 * k, vd + (2048 >> 4) * k,
+                        idesc<D, true>(), j || k);
+          tc::umma_commit(added(jt & 1));
+          tc::umma_commit(freed(s));
+        }
+        ++n;
+      }
       jg += tiles;
     }
     if (!ok) {  // let the products issued so far end before TMEM goes back
-      const uint32_t mine = drained(warp & 1);
-      if (lead) tc::umma_commit(mine);
-      for (uint32_t i = 0; i < kPolls && !tc::mbar_try_wait(mine, 0); ++i) {}
+      if (lead) tc::umma_commit(drained);
+      for (uint32_t i = 0; i < kPolls && !tc::mbar_try_wait(drained, 0); ++i) {}
     }
     __syncwarp();
   }
