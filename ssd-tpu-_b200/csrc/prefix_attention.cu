@@ -36,6 +36,7 @@ struct PrefixAttn {
   int cap;               // positions of a sequence that may be read
   int R;                 // query rows of a sequence and KV head: G * T
   int tile_rows;         // query rows of a row tile
+  int spt_inv;           // 65536 / spt + 1
   int spt, tps;          // sequences of a row tile (R <= its rows), else tiles of a sequence
   int tiles;             // bound on the row tiles of all groups
   int num_layers, layer_no;
@@ -365,7 +366,7 @@ constexpr int THREADS = 2 * SET + 64;
 constexpr int META = 16;               // tiles whose units are described: more than there are between fetch and use
 constexpr int kMaxTiles = 256;         // also sequences and groups: their numbers are kept in shared memory
 constexpr int kMinUnits = 8;           // of a run: shorter ones cost more in prologues and joins than they save
-constexpr int kStart = 24;             // units that the start of a list is worth
+constexpr int kStart = 40;             // units that the start of a list is worth
 constexpr int kWhole = 64;             // lists of at most so many units are not cut
 constexpr int kMaxTeam = 8;            // CTAs that walk a group's lists side by side
 constexpr float kSpan = 8.f;           // weights are at most 2^8
@@ -384,7 +385,8 @@ struct Cfg {
   static constexpr uint32_t seq = info + 8 * kMaxTiles;               // int [kMaxTiles]: lengths,
   static constexpr uint32_t ql = seq + 4 * kMaxTiles;                 // uint16: new tokens of the sequences,
   static constexpr uint32_t pre = ql + 2 * kMaxTiles;                 // prefixes of the groups
-  static constexpr uint32_t cum = pre + 4 * kMaxTiles;                // int [ROWS + 4]: units before a sequence's tail
+  static constexpr uint32_t first = pre + 4 * kMaxTiles;              // int [kMaxTiles + 1]: first sequences
+  static constexpr uint32_t cum = first + 4 * (kMaxTiles + 4);        // int [ROWS + 4]: units before a sequence's tail
   static constexpr uint32_t meta = cum + 4 * (ROWS + 4);              // int4 [META][UNITS]
   static constexpr uint32_t pairs = meta + 16 * META * UNITS;         // float [set][turn][half][ROWS]: maxima
   static constexpr uint32_t refs = pairs + 4 * 8 * ROWS;              // float [tile parity][ROWS]: M
@@ -396,8 +398,6 @@ struct Cfg {
   static constexpr uint32_t p_col = TILE, q_col = 2 * TILE, o_col = q_col + D / 2, tmem_cols = D == 64 ? 256 : 512;
   static_assert(o_col + D <= tmem_cols);
   static_assert(smem <= 227 * 1024);
-  // planning, in the ring's place: group starts, their first tiles
-  static_assert(ring >= 8 * (kMaxTiles + 1));
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -522,6 +522,12 @@ struct Shares {
     return run * q + run * (all - q * runs) / runs;
   }
 };
+// Tile m of the group that starts with sequence `first`.
+__device__ __forceinline__ int team_tile(const PrefixAttn& a, int first, int m) {
+  return a.tps > 1 ? first * a.tps + m : first + m * a.spt;
+}
+// x / spt (x < 512).
+__device__ __forceinline__ int by_spt(const PrefixAttn& a, int x) { return (x * a.spt_inv) >> 16; }
 struct Walk {
   int pos, end;
   int at;           // tile (group, where there are teams) that pos is in
@@ -548,13 +554,13 @@ struct Walk {
     }
   }
   __device__ bool next(const PrefixAttn& a, const Shares& sh, const int* pref, const int* units_s, const int2* info,
-                       Segment& s) {
+                       const int* first_s, Segment& s) {
     while (pos < end) {
       while (pref[at + 1] * a.hkv <= pos) ++at;
       const int list = pref[at + 1] - pref[at], first = pref[at] * a.hkv;
       s.head = (pos - first) / list;
       const int base = first + s.head * list + kStart;  // of the list's first unit
-      s.tile = at * sh.nm + (int)blockIdx.x % sh.nm;
+      s.tile = sh.nm > 1 ? team_tile(a, first_s[at], (int)blockIdx.x % sh.nm) : at;
       const int units = units_s[s.tile];
       s.lo = max(pos - base, 0);
       s.hi = min(min(base - kStart + list, end) - base, units);
@@ -658,6 +664,7 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid
   int* seq_s = reinterpret_cast<int*>(gen + C::seq);
   uint16_t* ql_s = reinterpret_cast<uint16_t*>(gen + C::ql);
   int* pre_s = reinterpret_cast<int*>(gen + C::pre);
+  int* first_s = reinterpret_cast<int*>(gen + C::first);
   int* cum = reinterpret_cast<int*>(gen + C::cum);
   int4* meta = reinterpret_cast<int4*>(gen + C::meta);
   float* pair_s = reinterpret_cast<float*>(gen + C::pairs);
@@ -713,104 +720,113 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
+  // parameters come into the constant cache where they are first used: what comes next, all at once
+  asm volatile("" ::"r"(a.B), "r"(a.T), "r"(a.groups), "r"(a.tiles), "r"(a.spt), "r"(a.hkv), "r"(a.block_size), "l"(a.tables),
+               "l"(a.parts), "l"(a.starts));
   pdl_wait();
   pdl_trigger();
 
   // ---------------------------------------------------------------- the tiles and their units
+  // A tile goes by the number of its first sequence (times tps, plus its slice, where a sequence has several): numbers in
+  // between stand for nothing.
   {
     static_assert(THREADS > kMaxTiles);  // a thread a sequence, group and tile
-    int* g_start = reinterpret_cast<int*>(gen);           // [groups + 1]
-    int* g_tile = reinterpret_cast<int*>(gen) + kMaxTiles + 1;
-    int seq = 0, ql = 0, start = 0, P = 0;
+    int seq = 0, ql = 0, start = 0, end = 0, P = 0;
     if (tid < a.B) {
       seq = ld_act(a.seq_lens + tid);
       ql = a.q_lens ? ld_act(a.q_lens + tid) : a.T;
     }
-    if (tid <= a.groups) start = ld_act(a.starts + tid);
-    if (tid < a.groups) P = ld_act(a.prefixes + tid);
+    if (tid < a.groups) {
+      start = ld_act(a.starts + tid);
+      end = ld_act(a.starts + tid + 1);
+      P = ld_act(a.prefixes + tid);
+    }
     if (tid < a.tiles) {
-      info[tid] = make_int2(0, 0);
+      info[tid] = make_int2(-1, 0);
       units_s[tid] = 0;
     }
     ql = clamped(ql, a.T);
+    start = clamped(start, a.B);
+    end = clamped(end, a.B);
     if (tid < a.B) {
       seq_s[tid] = seq;
       ql_s[tid] = (uint16_t)ql;  // (as many as fit the tiles that there may be)
     }
-    if (tid <= a.groups) g_start[tid] = clamped(start, a.B);
-    if (tid < a.groups) pre_s[tid] = clamped(P, a.cap);
-    __syncthreads();
-    if (warp == 0) {
-      int before = 0, nm = -1;  // nm: tiles of every group; 0: not the same for all
-      for (int g0 = 0; g0 < a.groups; g0 += 32) {
-        const int g = g0 + lane, n = g < a.groups ? group_tiles(a, g_start[g + 1] - g_start[g]) : 0;
-        if (nm < 0) nm = __shfl_sync(0xffffffffu, n, 0);
-        if (__any_sync(0xffffffffu, g < a.groups && n != nm)) nm = 0;
-        int incl = n;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const int y = __shfl_up_sync(0xffffffffu, incl, o);
-          if (lane >= o) incl += y;
-        }
-        if (g < a.groups) g_tile[g] = before + incl - n;
-        before += __shfl_sync(0xffffffffu, incl, 31);
-      }
-      if (lane == 0) slot[3] = nm > 1 && nm <= kMaxTeam && nm * 4 <= (int)gridDim.x && !a.whole ? nm : 1;
+    if (tid < a.groups) {
+      first_s[tid] = start;
+      pre_s[tid] = clamped(P, a.cap);
+      if (tid == a.groups - 1) first_s[a.groups] = end;
+      if (tid == 0) slot[3] = a.tps > 1 ? (end - start) * a.tps : by_spt(a, end - start + a.spt - 1);
     }
+    __syncthreads();
+    const int nm = slot[3];  // tiles of the first group: of all, if there are to be teams
+    const bool same = tid >= a.groups || nm == (a.tps > 1 ? (end - start) * a.tps : by_spt(a, end - start + a.spt - 1));
     int g = 0, s = 0, e = 0;
     if (tid < a.B) {
       int n = a.groups;
       while (n > 1) {  // the last group that starts at or before the sequence
         const int half = n / 2;
-        if (g_start[g + half] <= tid) g += half, n -= half;
+        if (first_s[g + half] <= tid) g += half, n -= half;
         else n = half;
       }
-      s = g_start[g];
-      e = g_start[g + 1];
-      P = pre_s[g];
+      s = first_s[g];
+      e = first_s[g + 1];
     }
-    __syncthreads();
     if (tid >= s && tid < e) {  // (starts that ascend from 0 to B have every sequence in a group)
-      const int tail = tail_units(a, seq, ql, P), k = tid - s;
-      const int t0 = g_tile[g] + (a.tps > 1 ? k * a.tps : k / a.spt);
-      const bool lead = a.tps > 1 || k % a.spt == 0;
-      for (int p = 0; p < a.tps && t0 + p < a.tiles; ++p) {
-        atomicAdd(&units_s[t0 + p], tail + (lead ? prefix_units(P) : 0));
-        if (lead) info[t0 + p] = make_int2(tid | (a.tps > 1 ? p : min(a.spt, e - tid)) << 16, g | s << 16);
+      const int own = pre_s[g], tail = tail_units(a, seq, ql, own), k = tid - s;
+      const int seq0 = a.tps > 1 ? tid : s + by_spt(a, k) * a.spt;
+      const bool lead = seq0 == tid;
+      for (int p = 0; p < a.tps; ++p) {
+        const int t = seq0 * a.tps + p;
+        atomicAdd(&units_s[t], tail + (lead ? prefix_units(own) : 0));
+        if (lead) info[t] = make_int2(tid | (a.tps > 1 ? p : min(a.spt, e - tid)) << 16, g | s << 16);
       }
     }
-    __syncthreads();
+    const bool team = __syncthreads_and(same) && nm > 1 && nm <= kMaxTeam && nm * 4 <= (int)gridDim.x && !a.whole;
     if (warp == 0) {
-      const int nm = slot[3], lists = nm > 1 ? a.groups : a.tiles;
-      int before = 0;
-      for (int t0 = 0; t0 < lists; t0 += 32) {
-        const int t = t0 + lane;
+      const int lists = team ? a.groups : a.tiles, per = (lists + 31) / 32;
+      int sum = 0, starts = 0;
+      for (int i = 0; i < per; ++i) {
+        const int t = lane * per + i;
         int n = 0;
         if (t < lists) {
-          for (int i = 0; i < nm; ++i) n = max(n, units_s[t * nm + i]);
-          if (n > 0) n += kStart;
+          if (team) {
+            for (int m = 0; m < nm; ++m) n = max(n, units_s[team_tile(a, first_s[t], m)]);
+          } else {
+            n = units_s[t];
+          }
+          if (n > 0) n += kStart, ++starts;
+          pref[1 + t] = n;
         }
-        int incl = n;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const int y = __shfl_up_sync(0xffffffffu, incl, o);
-          if (lane >= o) incl += y;
-        }
-        if (t < lists) pref[1 + t] = before + incl;
-        before += __shfl_sync(0xffffffffu, incl, 31);
+        sum += n;
       }
-      if (lane == 0) pref[0] = 0;
+      int incl = sum;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += y;
+      }
+      int before = incl - sum;
+      for (int i = 0; i < per; ++i) {
+        const int t = lane * per + i;
+        if (t < lists) pref[1 + t] = before += pref[1 + t];
+      }
+      starts = __reduce_add_sync(0xffffffffu, starts);
+      if (lane == 0) {
+        pref[0] = 0;
+        slot[2] = starts;
+        slot[3] = team ? nm : 1;
+      }
     }
     for (int t = blockIdx.x; t < a.tiles; t += gridDim.x) {  // rows that see nothing
-      if (units_s[t] != 0) continue;
       const int2 in = info[t];
+      if (in.x < 0 || units_s[t] != 0) continue;
       const int seq0 = in.x & 0xffff, n = a.tps > 1 ? (in.x >> 16 ? 0 : 1) : in.x >> 16;
       const int64_t row = (int64_t)a.T * a.hq * D / 8;
       for (int64_t i = tid; i < n * row; i += THREADS)
         reinterpret_cast<uint4*>(a.out)[seq0 * row + i] = make_uint4(0, 0, 0, 0);
       for (int h = tid; h < a.hkv; h += THREADS) put_parts(a, in, t, h, 0, 1, 0, 0, 1);
     }
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the ring was written by threads
   }
   tc::tc_fence_before();
   __syncthreads();
@@ -821,7 +837,7 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid
   const int lists = sh.nm > 1 ? a.groups : a.tiles;
   sh.all = pref[lists] * a.hkv;
   sh.whole = a.whole;
-  sh.runs = max(1, min((int)gridDim.x / sh.nm, sh.whole ? lists * a.hkv : (sh.all - kStart * lists * a.hkv) / kMinUnits));
+  sh.runs = max(1, min((int)gridDim.x / sh.nm, sh.whole ? lists * a.hkv : (sh.all - kStart * (int)slot[2] * a.hkv) / kMinUnits));
   Walk walk(a, sh, pref, lists);
   Segment sg;
   const float c = fmaxf(fabsf(a.scale) * 1.4426950408889634f, 1e-38f);  // not 0: keeps the mask's infinity an infinity
@@ -834,7 +850,7 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid
     const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16);
     int swaps = 0, n = 0;  // n: stages filled before
     bool ok = true;
-    for (int seg = 0; walk.next(a, sh, pref, units_s, info, sg); ++seg) {
+    for (int seg = 0; walk.next(a, sh, pref, units_s, info, first_s, sg); ++seg) {
       const int tiles = (sg.hi - sg.lo + UNITS - 1) / UNITS, last = jg + tiles - 1;
       const RowAt w = row_at<D>(a, sg.rows, sg.head, r, a.tile_rows, seq_s, ql_s);
       if (sg.lo == 0 && warp == SETW)
@@ -1092,7 +1108,7 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid
     asm volatile("{.reg .pred p; elect.sync _|p, 0xffffffff; selp.u32 %0, 1, 0, p;}" : "=r"(lead));
     int n = 0;        // stages filled
     bool ok = true;
-    for (int seg = 0; ok && walk.next(a, sh, pref, units_s, info, sg); ++seg) {
+    for (int seg = 0; ok && walk.next(a, sh, pref, units_s, info, first_s, sg); ++seg) {
       const int tiles = (sg.hi - sg.lo + UNITS - 1) / UNITS;
       const int P = pre_s[sg.rows.group], pu = prefix_units(P);
       int before = pu;
@@ -1233,7 +1249,7 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid
       ++n;
       return true;
     };
-    for (int seg = 0; ok && walk.next(a, sh, pref, units_s, info, sg); ++seg) {
+    for (int seg = 0; ok && walk.next(a, sh, pref, units_s, info, first_s, sg); ++seg) {
       const int tiles = (sg.hi - sg.lo + UNITS - 1) / UNITS;
       ok = ready(q_tmem, seg & 1, q_tmem, seg & 1);
       if (!ok) break;
@@ -1408,8 +1424,9 @@ PrefixLayout prefix_layout(int dtype, int B, int T, int hq, int hkv, int D, int 
   const int G = hq / hkv;
   if (dtype == SSD_DTYPE_BF16 && block_size % 16 == 0 && G <= tile::ROWS) {
     tiles_of(tile::ROWS / G * G);  // whole tokens
+    L.tiles = (int)std::min<int64_t>((int64_t)B * L.tps, 0x7fffffff);  // (numbers of tiles, see the kernel)
     // (the units are counted in 32 bits)
-    L.tc = L.tiles <= tile::kMaxTiles && B <= tile::kMaxTiles && groups <= tile::kMaxTiles &&
+    L.tc = L.tiles <= tile::kMaxTiles && groups <= tile::kMaxTiles &&
            (((int64_t)max_seq_len + 15) / 16 + tile::kStart) * (L.tiles + B) * hkv < (1 << 30);
   }
   const int64_t units = ((int64_t)max_seq_len + 15) / 16;  // of a sequence
@@ -1538,6 +1555,7 @@ extern "C" int ssd_shared_prefix_attention(ssd_stream_t stream, const void* q, c
   a.tile_rows = L.tile_rows;
   a.q_box = tile::ROWS / a.G * a.G;
   a.spt = L.spt;
+  a.spt_inv = 65536 / L.spt + 1;
   a.tps = L.tps;
   a.tiles = L.tiles;
   a.nsplit = L.nsplit;
