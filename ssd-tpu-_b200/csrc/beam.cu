@@ -8,7 +8,7 @@
 //                 largest logits.  One pass over the data; beams that offer one candidate or none are not read.
 //   merge kernel  a CTA a request: the slices' statistics become lse_w, the slices' candidates are ranked in 64
 //                 bits, the W best are written in order.
-// The W largest of a CTA: each half warp's maximum, the W-th largest of these 32 as a bound that at least W values
+// The W largest of a CTA: the maxima of 32 groups of threads, the W-th largest of these as a bound that at least W values
 // reach (and seldom more than a few times W), those values to shared memory, and each one's rank by counting the
 // larger ones.  Where more values reach the bound than fit (long runs of equal logits, sorted rows), W rounds of a
 // maximum over the CTA.  Order never depends on which thread comes first: equal values rank by their index.
@@ -18,8 +18,8 @@ namespace ssd {
 namespace {
 
 constexpr int kMaxBeams = 32;
-constexpr int kThreads = 512;          // 32 half warps
-constexpr int kList = 512;             // candidates that reach the bound
+constexpr int kRowThreads = 256, kMergeThreads = 512;
+constexpr int kList = 256;             // candidates that reach the bound
 constexpr unsigned kAll = 0xffffffffu;
 
 // Lane's rank among the warp's 32 values (largest first, lower lanes before equal ones).
@@ -35,15 +35,17 @@ __device__ __forceinline__ int lane_rank(T v) {
   return rank;
 }
 
-// The W-th largest of the 32 half warps' maxima, for every thread; `maxima` and `bound` are shared memory.
-template <typename T>
+// The W-th largest of the maxima of 32 groups of THREADS / 32 threads, for every thread; `maxima` and `bound` are shared
+// memory.
+template <int THREADS, typename T>
 __device__ __forceinline__ T select_bound(T mine, int W, T* maxima, T* bound) {
+  constexpr int N = THREADS / 32;
 #pragma unroll
-  for (int o = 8; o > 0; o >>= 1) {
+  for (int o = N / 2; o > 0; o >>= 1) {
     const T y = __shfl_xor_sync(kAll, mine, o);
     mine = y > mine ? y : mine;
   }
-  if ((threadIdx.x & 15) == 0) maxima[threadIdx.x >> 4] = mine;
+  if (threadIdx.x % N == 0) maxima[threadIdx.x / N] = mine;
   __syncthreads();
   if (threadIdx.x < 32) {
     const T v = maxima[threadIdx.x];
@@ -71,10 +73,10 @@ __device__ __forceinline__ bool reads_logits(const float* scores, const uint8_t*
 }
 
 template <int ITEMS, bool VEC>
-__global__ void __launch_bounds__(kThreads, 2) beam_rows_kernel(const BeamRows a) {
+__global__ void __launch_bounds__(kRowThreads, 4) beam_rows_kernel(const BeamRows a) {
   __shared__ unsigned long long list[kList];
   __shared__ float maxima[32];
-  __shared__ float2 ms[kThreads / 32];
+  __shared__ float2 ms[kRowThreads / 32];
   __shared__ float bound_s;
   __shared__ int count;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -82,10 +84,10 @@ __global__ void __launch_bounds__(kThreads, 2) beam_rows_kernel(const BeamRows a
   pdl_wait();
   pdl_trigger();
   if (!reads_logits(a.scores, a.finished, row)) return;
-  const int v0 = slice * (ITEMS * kThreads), n = min(ITEMS * kThreads, a.V - v0);
+  const int v0 = slice * (ITEMS * kRowThreads), n = min(ITEMS * kRowThreads, a.V - v0);
   const float* x = a.logits + row * a.ld + v0;
   float v[ITEMS];
-  auto index = [&](int i) { return VEC ? ((i >> 2) * kThreads + tid) * 4 + (i & 3) : i * kThreads + tid; };
+  auto index = [&](int i) { return VEC ? ((i >> 2) * kRowThreads + tid) * 4 + (i & 3) : i * kRowThreads + tid; };
   if constexpr (VEC) {
 #pragma unroll
     for (int i = 0; i < ITEMS; i += 4) {
@@ -104,7 +106,7 @@ __global__ void __launch_bounds__(kThreads, 2) beam_rows_kernel(const BeamRows a
   float m = -INFINITY;
 #pragma unroll
   for (int i = 0; i < ITEMS; ++i) m = fmaxf(m, v[i]);
-  const float t = select_bound(m, a.W, maxima, &bound_s);
+  const float t = select_bound<kRowThreads>(m, a.W, maxima, &bound_s);
   // statistics: the thread's own maximum as reference, 0 where nothing is left of its part
   float s = 0.f;
   const float ref = m == -INFINITY ? 0.f : m;
@@ -125,7 +127,7 @@ __global__ void __launch_bounds__(kThreads, 2) beam_rows_kernel(const BeamRows a
   __syncthreads();
   const int64_t out = (int64_t)row * a.slices + slice;
   if (warp == 0) {
-    const float2 w = lane < kThreads / 32 ? ms[lane] : make_float2(-INFINITY, 0.f);
+    const float2 w = lane < kRowThreads / 32 ? ms[lane] : make_float2(-INFINITY, 0.f);
     const float M = warp_max(w.x), R = M == -INFINITY ? 0.f : M;
     const float S = warp_sum(w.x == -INFINITY ? w.y : w.y * __expf(w.x - R));
     if (lane == 0) a.stats[out] = make_float2(M, S);
@@ -154,7 +156,7 @@ __global__ void __launch_bounds__(kThreads, 2) beam_rows_kernel(const BeamRows a
     best = block_reduce(best, list, OpMax());
     if (tid == 0) keys[k] = best;
     if (best == 0) {
-      for (int i = k + 1 + tid; i < a.W; i += kThreads) keys[i] = 0;
+      for (int i = k + 1 + tid; i < a.W; i += kRowThreads) keys[i] = 0;
       return;
     }
     last = best;
@@ -184,19 +186,19 @@ __device__ __forceinline__ bool better(unsigned long long ka, uint32_t fa, unsig
   return ka > kb || (ka == kb && fa < fb);
 }
 
-__global__ void __launch_bounds__(kThreads) beam_merge_kernel(const BeamMerge a) {
+__global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamMerge a) {
   __shared__ unsigned long long maxima[32], bound_s;
   __shared__ unsigned long long list_k[kList];
   __shared__ uint32_t list_f[kList];
   __shared__ double lse[kMaxBeams], base[kMaxBeams], norm[kMaxBeams];
   __shared__ int kind[kMaxBeams];  // 0: offers nothing, 1: its tokens, 2: itself
   __shared__ int count;
-  __shared__ unsigned long long red_k[kThreads / 32];
-  __shared__ uint32_t red_f[kThreads / 32];
+  __shared__ unsigned long long red_k[kMergeThreads / 32];
+  __shared__ uint32_t red_f[kMergeThreads / 32];
   const BeamRows& r = a.r;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = blockIdx.x, W = r.W;
   pdl_wait();
-  for (int w = warp; w < W; w += kThreads / 32) {
+  for (int w = warp; w < W; w += kMergeThreads / 32) {
     const int row = g * W + w;
     const float sc = ld_act(r.scores + row);
     const bool done = r.finished && ld_act(r.finished + row);
@@ -250,9 +252,9 @@ __global__ void __launch_bounds__(kThreads) beam_merge_kernel(const BeamMerge a)
     return c;
   };
   unsigned long long best = 0;
-  for (int i = tid; i < total; i += kThreads) best = max(best, cand(i).key);
-  const unsigned long long t = select_bound(best, W, maxima, &bound_s);
-  for (int i = tid; i < total; i += kThreads) {
+  for (int i = tid; i < total; i += kMergeThreads) best = max(best, cand(i).key);
+  const unsigned long long t = select_bound<kMergeThreads>(best, W, maxima, &bound_s);
+  for (int i = tid; i < total; i += kMergeThreads) {
     const Cand c = cand(i);
     if (c.key != 0 && c.key >= t) {
       const int at = atomicAdd(&count, 1);
@@ -303,7 +305,7 @@ __global__ void __launch_bounds__(kThreads) beam_merge_kernel(const BeamMerge a)
     for (int k = 0; k < W; ++k) {
       unsigned long long bk = 0;
       uint32_t bf = 0xffffffffu;
-      for (int i = tid; i < total; i += kThreads) {
+      for (int i = tid; i < total; i += kMergeThreads) {
         const Cand c = cand(i);
         if (c.key != 0 && better(last_k, last_f, c.key, c.flat) && better(c.key, c.flat, bk, bf)) {
           bk = c.key;
@@ -319,7 +321,7 @@ __global__ void __launch_bounds__(kThreads) beam_merge_kernel(const BeamMerge a)
       __syncthreads();
       if (lane == 0) { red_k[warp] = bk; red_f[warp] = bf; }
       __syncthreads();
-      for (int i = 0; i < kThreads / 32; ++i)
+      for (int i = 0; i < kMergeThreads / 32; ++i)
         if (better(red_k[i], red_f[i], bk, bf)) { bk = red_k[i]; bf = red_f[i]; }
       if (tid == 0) put(k, bk, bf);
       last_k = bk;
@@ -339,8 +341,8 @@ struct BeamLayout {
 BeamLayout beam_layout(int G, int W, int V) {
   BeamLayout L;
   const int64_t rows = (int64_t)G * W;
-  L.items = rows * ((V + kManyItems * kThreads - 1) / (kManyItems * kThreads)) >= 2 * 148 ? kManyItems : kFewItems;
-  L.slices = (V + L.items * kThreads - 1) / (L.items * kThreads);
+  L.items = rows * ((V + kManyItems * kRowThreads - 1) / (kManyItems * kRowThreads)) >= 2 * 148 ? kManyItems : kFewItems;
+  L.slices = (V + L.items * kRowThreads - 1) / (L.items * kRowThreads);
   L.off_keys = (sizeof(float2) * (size_t)rows * L.slices + 255) & ~size_t(255);
   L.total = L.off_keys + sizeof(unsigned long long) * (size_t)rows * L.slices * W;
   return L;
@@ -379,14 +381,14 @@ extern "C" int ssd_beam_select(ssd_stream_t stream, const float* logits, int64_t
   const dim3 grid(L.slices, G * W);
   const bool vec = !(reinterpret_cast<uintptr_t>(logits) & 15) && ld % 4 == 0 && V % 4 == 0;
   if (L.items == kManyItems) {
-    if (vec) SSD_PDL((beam_rows_kernel<kManyItems, true>), grid, kThreads, 0, stream, r);
-    else SSD_PDL((beam_rows_kernel<kManyItems, false>), grid, kThreads, 0, stream, r);
+    if (vec) SSD_PDL((beam_rows_kernel<kManyItems, true>), grid, kRowThreads, 0, stream, r);
+    else SSD_PDL((beam_rows_kernel<kManyItems, false>), grid, kRowThreads, 0, stream, r);
   } else {
-    if (vec) SSD_PDL((beam_rows_kernel<kFewItems, true>), grid, kThreads, 0, stream, r);
-    else SSD_PDL((beam_rows_kernel<kFewItems, false>), grid, kThreads, 0, stream, r);
+    if (vec) SSD_PDL((beam_rows_kernel<kFewItems, true>), grid, kRowThreads, 0, stream, r);
+    else SSD_PDL((beam_rows_kernel<kFewItems, false>), grid, kRowThreads, 0, stream, r);
   }
   const BeamMerge m{r, lengths, eos, (double)length_penalty, out_scores, out_parents, out_tokens, out_lengths,
                     out_finished};
-  SSD_PDL(beam_merge_kernel, G, kThreads, 0, stream, m);
+  SSD_PDL(beam_merge_kernel, G, kMergeThreads, 0, stream, m);
   return SSD_OK;
 }

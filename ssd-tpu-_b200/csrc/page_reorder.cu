@@ -4,21 +4,25 @@
 // for the others, and pages that no row refers to any more go back on the free list.  Nothing of a whole page moves, so
 // what a step cannot do without is the tables' entries, once read and once written, and the copied rows.
 //
-//   reorder kernel  one cluster of CTAs (hardware barriers between its phases, no second launch): reference counts
-//                   change by (children - 1) for each entry; entries whose count has come to nothing are marked; the
-//                   tables are permuted in place, a stripe of columns at a time through shared memory; the marked
-//                   blocks are pushed in ascending order and the fresh ones popped in row order, so that the free
-//                   list does not depend on which thread came first.
+//   reorder kernel  one cluster of CTAs (hardware barriers between its phases, no second launch), or one CTA for small
+//                   tables.  A thread takes one column of one request at a time, its W entries in registers: reference
+//                   counts change by (children - 1) for each, summed up first where all rows hold one page (a shared
+//                   prompt: no atomics).  Then entries whose count has come to nothing are marked and the columns
+//                   written in their new order.  The marked blocks are pushed in ascending order and the fresh ones
+//                   popped in row order, so that the free list does not depend on which thread came first.
 //   row copy kernel the first rows of a page in all planes, a CTA a piece of one plane of one pair.
+#include <algorithm>
+
 #include "kv8.cuh"
 
 namespace ssd {
 namespace {
 
 constexpr int kMaxReorder = 1024;   // rows
-constexpr int kReorderThreads = 512;
+constexpr int kMaxBeams = 32;       // of a request
+constexpr int kReorderThreads = 1024;
 constexpr int kCluster = 8;
-constexpr int kStripe = 4096;       // table entries of a stripe
+constexpr int kOneCta = 4096;       // columns of all requests that one CTA takes alone
 constexpr int kGone = 1 << 30;      // in a reference count's place: nobody refers to the block any more
 
 struct Reorder {
@@ -27,26 +31,13 @@ struct Reorder {
   int32_t *free_list, *free_top, *refs;
   int num_blocks;
   const int32_t *parents, *held;
-  int B, W, block_size;
+  int G, W, block_size;
   uint8_t* ok;
   int32_t *src, *dst, *rows;        // the copies: pages and how many rows of them; -1: none
 };
 
 __device__ __forceinline__ void cluster_barrier() {
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-__device__ __forceinline__ int cluster_rank() {
-  uint32_t r;
-  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return (int)r;
-}
-// Reads an int of CTA `rank`'s shared memory.
-__device__ __forceinline__ int ld_cluster(const int* p, int rank) {
-  uint32_t a = (uint32_t)__cvta_generic_to_shared(p), b;
-  int v;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(b) : "r"(a), "r"(rank));
-  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(b) : "memory");
-  return v;
 }
 
 // Exclusive sum over the CTA; `tmp` holds a number a warp.
@@ -61,48 +52,57 @@ __device__ __forceinline__ int block_scan(int v, int* tmp, int* total) {
   __syncthreads();
   if (lane == 31) tmp[warp] = x;
   __syncthreads();
-  int before = 0, all = 0;
-  for (int w = 0; w < (int)blockDim.x / 32; ++w) {
-    if (w < warp) before += tmp[w];
-    all += tmp[w];
+  const int mine = tmp[lane];  // 32 warps
+  int y = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int z = __shfl_up_sync(0xffffffffu, y, o);
+    if (lane >= o) y += z;
   }
-  *total = all;
-  return before + x - v;
+  *total = __shfl_sync(0xffffffffu, y, 31);
+  return __shfl_sync(0xffffffffu, y - mine, warp) + x - v;
 }
 
+// WM: at least W.
+template <int WM>
 __global__ void __launch_bounds__(kReorderThreads) page_reorder_kernel(const Reorder a) {
-  __shared__ int stripe[kStripe];
   __shared__ int16_t parent_s[kMaxReorder];            // -1: the row is emptied
   __shared__ int children[kMaxReorder], first[kMaxReorder];
   __shared__ int need_s[kMaxReorder], len_s[kMaxReorder];  // blocks that a row's tokens take, and that it has
   __shared__ int part_s[kMaxReorder];                  // index of the partial page (-1: none)
-  __shared__ int tmp[kReorderThreads / 32], mine_s, top_s;
-  const int tid = threadIdx.x, rank = cluster_rank();
+  __shared__ int used_s, tmp[32];
+  const int tid = threadIdx.x, B = a.G * a.W;
   pdl_wait();
-  for (int i = tid; i < a.B; i += kReorderThreads) {
-    children[i] = 0;
-    first[i] = a.B;
-    const int len = min(max(ld_act(a.lens + i), 0), a.max_blocks), n = max(ld_act(a.held + i), 0);
-    const int full = min(n / a.block_size, len);
-    const bool part = full < len && n % a.block_size != 0;
-    need_s[i] = full + part;
-    len_s[i] = len;
-    part_s[i] = part ? full : -1;
+  int parent = 0, len = 0, held = 0;
+  if (tid < B) {
+    parent = ld_act(a.parents + tid);
+    len = ld_act(a.lens + tid);
+    held = ld_act(a.held + tid);
   }
-  if (tid == 0) top_s = ld_act(a.free_top);
+  const int top = min(max(ld_act(a.free_top), 0), a.num_blocks);
+  if (tid == 0) used_s = 0;
+  children[tid] = 0;
+  first[tid] = B;
   __syncthreads();
-  for (int i = tid; i < a.B; i += kReorderThreads) {
-    const int p = ld_act(a.parents + i);
-    const int at = (unsigned)p < (unsigned)a.W ? i / a.W * a.W + p : -1;
-    parent_s[i] = (int16_t)at;
-    if (at >= 0) {
-      atomicAdd(&children[at], 1);
-      atomicMin(&first[at], i);
+  len = min(max(len, 0), a.max_blocks);
+  held = max(held, 0);
+  parent = tid < B && (unsigned)parent < (unsigned)a.W ? tid / a.W * a.W + parent : -1;
+  const int full = min(held / a.block_size, len);
+  const bool part = full < len && held % a.block_size != 0;
+  if (tid < B) {
+    need_s[tid] = full + part;
+    len_s[tid] = len;
+    part_s[tid] = part ? full : -1;
+    parent_s[tid] = (int16_t)parent;
+    if (parent >= 0) {
+      atomicAdd(&children[parent], 1);
+      atomicMin(&first[parent], tid);
     }
   }
+  const int longest = __reduce_max_sync(0xffffffffu, tid < B ? len : 0);
+  if ((tid & 31) == 0 && longest > 0) atomicMax(&used_s, longest);
   __syncthreads();
-  int used = 0;
-  for (int i = 0; i < a.B; ++i) used = max(used, len_s[i]);
+  const int used = used_s, items = a.G * used;
   // change of a block's count for entry j of row b
   auto change = [&](int b, int j) {
     if (j >= len_s[b]) return 0;
@@ -110,112 +110,132 @@ __global__ void __launch_bounds__(kReorderThreads) page_reorder_kernel(const Reo
     const int c = children[b];
     return j == part_s[b] ? (c > 0 ? 0 : -1) : c - 1;
   };
-  const int cols = max(1, kStripe / a.B);  // columns of a stripe
-  const int stripes = (used + cols - 1) / cols;
-  for (int s = rank; s < stripes; s += kCluster) {
-    for (int e = tid; e < a.B * cols; e += kReorderThreads) {
-      const int b = e / cols, j = s * cols + e % cols, d = change(b, j);
-      if (d == 0) continue;
-      const int blk = ld_act(a.tables + (int64_t)b * a.max_blocks + j);
-      if ((unsigned)blk < (unsigned)a.num_blocks) atomicAdd(a.refs + blk, d);
+  auto entries = [&](int g, int j, int* e) {
+#pragma unroll
+    for (int w = 0; w < WM; ++w) {
+      e[w] = -1;
+      if (w < a.W && j < len_s[g * a.W + w]) e[w] = ld_act(a.tables + (int64_t)(g * a.W + w) * a.max_blocks + j);
     }
-  }
-  cluster_barrier();
-  for (int s = rank; s < stripes; s += kCluster) {
-    __syncthreads();
-    for (int e = tid; e < a.B * cols; e += kReorderThreads) {
-      const int b = e / cols, j = s * cols + e % cols;
-      int blk = -1;
-      if (j < len_s[b]) blk = ld_act(a.tables + (int64_t)b * a.max_blocks + j);
-      stripe[e] = blk;
-      if ((unsigned)blk < (unsigned)a.num_blocks && change(b, j) < 0 && ld_act(a.refs + blk) <= 0)
-        __stcg(a.refs + blk, kGone);
-    }
-    __syncthreads();
-    for (int e = tid; e < a.B * cols; e += kReorderThreads) {
-      const int b = e / cols, j = s * cols + e % cols, p = parent_s[b];
-      if (p == b && need_s[b] == len_s[b] && (part_s[b] < 0 || first[b] == b)) continue;
-      const int had = len_s[b], has = p >= 0 ? need_s[p] : 0;
-      if (j >= max(had, has) || j >= a.max_blocks) continue;
-      int blk = -1;
-      if (j < has && (j != part_s[p] || first[p] == b)) blk = stripe[p * cols + (e % cols)];
-      else if (j < has) blk = -2 - stripe[p * cols + (e % cols)];  // a copy is wanted; the page it is of
-      a.tables[(int64_t)b * a.max_blocks + j] = blk;
-    }
-  }
-  cluster_barrier();
-  // the blocks that are gone: each CTA a run of blocks, in ascending order
-  const int run = (a.num_blocks + kCluster - 1) / kCluster, lo = min(rank * run, a.num_blocks),
-            hi = min(lo + run, a.num_blocks);
-  const int per = (hi - lo + kReorderThreads - 1) / kReorderThreads;
-  const int my0 = min(lo + tid * per, hi), my1 = min(my0 + per, hi);
-  int n = 0;
-  for (int i = my0; i < my1; ++i) n += ld_act(a.refs + i) == kGone;
-  int total;
-  int at = block_scan(n, tmp, &total);
-  if (tid == 0) mine_s = total;
-  cluster_barrier();
-  int freed = 0;
-  for (int r = 0; r < kCluster; ++r) {
-    const int x = ld_cluster(&mine_s, r);
-    if (r < rank) at += x;
-    freed += x;
-  }
-  const int top = min(max(top_s, 0), a.num_blocks);
-  at += top;
-  for (int i = my0; i < my1; ++i) {
-    if (ld_act(a.refs + i) != kGone) continue;
-    __stcg(a.refs + i, 0);
-    if (at < a.num_blocks) __stcg(a.free_list + at, i);
-    ++at;
-  }
-  cluster_barrier();  // (also: no CTA leaves while another may read its shared memory)
-  if (rank != 0) return;
-  // fresh pages, popped in row order
-  int avail = min(top + freed, a.num_blocks);
-  for (int b0 = 0; b0 < a.B; b0 += kReorderThreads) {
-    const int b = b0 + tid, p = b < a.B ? parent_s[b] : -1;
-    const bool take = p >= 0 && part_s[p] >= 0 && first[p] != b;
-    int all;
-    const int nth = block_scan(take, tmp, &all), slot = avail - 1 - nth;
-    if (b < a.B) {
-      int src = -1, dst = -1, rows = 0;
-      bool ok = true;
-      int len = p >= 0 ? need_s[p] : 0;
-      if (take) {
-        int32_t* row = a.tables + (int64_t)b * a.max_blocks;
-        const int full = part_s[p];
-        src = -2 - __ldcg(row + full);
-        dst = slot >= 0 ? __ldcg(a.free_list + slot) : -1;
-        if ((unsigned)dst < (unsigned)a.num_blocks) {
-          __stcg(a.free_list + slot, -1);
-          a.refs[dst] = 1;
-          row[full] = dst;
-          rows = ld_act(a.held + p) % a.block_size;
-        } else {  // no page left: the row is left empty (its siblings keep the shared pages alive)
-          ok = false;
-          for (int j = 0; j < len; ++j) {
-            const int blk = __ldcg(row + j);
-            if (j < full && (unsigned)blk < (unsigned)a.num_blocks) atomicSub(a.refs + blk, 1);
-            row[j] = -1;
-          }
-          src = dst = -1;
-          len = 0;
-        }
+  };
+  const int step = gridDim.x * kReorderThreads;
+  for (int i = blockIdx.x * kReorderThreads + tid; i < items; i += step) {
+    const int g = i / used, j = i - g * used;
+    int e[WM], net = 0;
+    entries(g, j, e);
+    bool one = true;
+#pragma unroll
+    for (int w = 0; w < WM; ++w)
+      if (w < a.W) {
+        one &= e[w] == e[0];
+        net += change(g * a.W + w, j);
       }
-      a.lens[b] = len;
-      if (a.ok) a.ok[b] = ok;
-      a.src[b] = src;
-      a.dst[b] = dst;
-      a.rows[b] = rows;
+    if (one) {
+      if (net != 0 && (unsigned)e[0] < (unsigned)a.num_blocks) atomicAdd(a.refs + e[0], net);
+      continue;
     }
-    avail = max(avail - all, 0);
+#pragma unroll
+    for (int w = 0; w < WM; ++w)
+      if (w < a.W && (unsigned)e[w] < (unsigned)a.num_blocks) {
+        const int d = change(g * a.W + w, j);
+        if (d != 0) atomicAdd(a.refs + e[w], d);
+      }
   }
-  if (tid == 0) *a.free_top = avail;
+  cluster_barrier();
+  for (int i = blockIdx.x * kReorderThreads + tid; i < items; i += step) {
+    const int g = i / used, j = i - g * used;
+    int e[WM], refs[WM];
+    entries(g, j, e);
+#pragma unroll
+    for (int w = 0; w < WM; ++w)
+      refs[w] = w < a.W && (unsigned)e[w] < (unsigned)a.num_blocks && change(g * a.W + w, j) < 0 ? ld_act(a.refs + e[w]) : 1;
+#pragma unroll
+    for (int w = 0; w < WM; ++w)
+      if (refs[w] <= 0) __stcg(a.refs + e[w], kGone);
+#pragma unroll
+    for (int w = 0; w < WM; ++w) {
+      if (w >= a.W) continue;
+      const int b = g * a.W + w, p = parent_s[b], has = p >= 0 ? need_s[p] : 0;
+      if (j >= max(len_s[b], has)) continue;
+      int blk = -1;
+      if (j < has) {
+        const int from = p - g * a.W;
+#pragma unroll
+        for (int x = 0; x < WM; ++x)
+          if (x == from) blk = e[x];
+        if (j == part_s[p] && first[p] != b) blk = -2 - blk;  // a copy is wanted; the page it is of
+      }
+      if (blk != e[w]) __stcg(a.tables + (int64_t)b * a.max_blocks + j, blk);
+    }
+  }
+  cluster_barrier();
+  if (blockIdx.x != 0) return;
+  // the blocks that are gone, pushed in ascending order: a run of them a thread
+  const int run = (a.num_blocks + kReorderThreads - 1) / kReorderThreads, lo = min(tid * run, a.num_blocks),
+            hi = min(lo + run, a.num_blocks);
+  int n = 0;
+#pragma unroll 8
+  for (int i = lo; i < hi; ++i) n += ld_act(a.refs + i) == kGone;
+  int freed;
+  int at = top + block_scan(n, tmp, &freed);
+  if (n > 0)
+    for (int i = lo; i < hi; ++i) {
+      if (ld_act(a.refs + i) != kGone) continue;
+      __stcg(a.refs + i, 0);
+      if (at < a.num_blocks) __stcg(a.free_list + at, i);
+      ++at;
+    }
+  // fresh pages, popped in row order
+  const int avail = min(top + freed, a.num_blocks);
+  const int b = tid, p = parent;
+  const bool take = p >= 0 && part_s[p] >= 0 && first[p] != b;
+  int all;
+  const int nth = block_scan(take, tmp, &all), slot = avail - 1 - nth;  // (its barriers: the pushes are there)
+  if (b < B) {
+    int src = -1, dst = -1, rows = 0;
+    bool ok = true;
+    int now = p >= 0 ? need_s[p] : 0;
+    if (take) {
+      int32_t* row = a.tables + (int64_t)b * a.max_blocks;
+      const int at_part = part_s[p];
+      src = -2 - __ldcg(row + at_part);
+      dst = slot >= 0 ? __ldcg(a.free_list + slot) : -1;
+      if ((unsigned)dst < (unsigned)a.num_blocks) {
+        __stcg(a.free_list + slot, -1);
+        a.refs[dst] = 1;
+        row[at_part] = dst;
+        rows = ld_act(a.held + p) % a.block_size;
+      } else {  // no page left: the row is left empty (its siblings keep the shared pages alive)
+        ok = false;
+        for (int j = 0; j < now; ++j) {
+          const int blk = __ldcg(row + j);
+          if (j < at_part && (unsigned)blk < (unsigned)a.num_blocks) atomicSub(a.refs + blk, 1);
+          row[j] = -1;
+        }
+        src = dst = -1;
+        now = 0;
+      }
+    }
+    a.lens[b] = now;
+    if (a.ok) a.ok[b] = ok;
+    a.src[b] = src;
+    a.dst[b] = dst;
+    a.rows[b] = rows;
+  }
+  if (tid == 0) *a.free_top = max(avail - all, 0);
   pdl_trigger();
 }
 
-constexpr int kRowsThreads = 256, kRowsItems = 4;
+template <int WM>
+int launch_reorder(cudaStream_t st, const Reorder& a) {
+  const unsigned ctas = (int64_t)a.G * a.max_blocks <= kOneCta ? 1 : kCluster;
+  if (launch_pdl_cluster(page_reorder_kernel<WM>, dim3(ctas), dim3(kReorderThreads), 0, st, ctas, a) != cudaSuccess) {
+    (void)cudaGetLastError();
+    return SSD_ERR_LAUNCH;
+  }
+  return SSD_OK;
+}
+
+constexpr int kRowsThreads = 128, kRowsItems = 8;
 
 struct RowCopy {
   char* pages;
@@ -265,15 +285,11 @@ extern "C" int ssd_page_reorder(ssd_stream_t stream, int32_t* block_tables, int3
   if (!block_tables || !table_lens || !free_list || !free_top || !ref_counts || !parents || !num_tokens || !copy_src ||
       !copy_dst || !copy_rows)
     return SSD_ERR_INVALID;
-  if ((int64_t)G * W > kMaxReorder || num_blocks >= kGone) return SSD_ERR_UNSUPPORTED;
+  if (W > kMaxBeams || (int64_t)G * W > kMaxReorder || num_blocks >= kGone) return SSD_ERR_UNSUPPORTED;
   const Reorder a{block_tables, table_lens, max_blocks, free_list, free_top, ref_counts, num_blocks, parents, num_tokens,
-                  G * W, W, block_size, ok, copy_src, copy_dst, copy_rows};
-  if (launch_pdl_cluster(page_reorder_kernel, dim3(kCluster), dim3(kReorderThreads), 0, (cudaStream_t)stream, kCluster,
-                         a) != cudaSuccess) {
-    (void)cudaGetLastError();
-    return SSD_ERR_LAUNCH;
-  }
-  return SSD_OK;
+                  G, W, block_size, ok, copy_src, copy_dst, copy_rows};
+  cudaStream_t st = (cudaStream_t)stream;
+  return W <= 8 ? launch_reorder<8>(st, a) : launch_reorder<kMaxBeams>(st, a);
 }
 
 extern "C" int ssd_page_copy_rows(ssd_stream_t stream, void* pages, float* scales, int num_blocks, int block_size,

@@ -81,7 +81,7 @@ def reorder(**kw):
 @pytest.mark.parametrize("kw,rc", [(dict(G=0), OK)] + [(dict([(k, None)]), INVALID) for k in (
     "tables", "lens", "free", "top", "refs", "parents", "held", "src", "dst", "rows")] + [
     (dict(W=0), INVALID), (dict(G=-1), INVALID), (dict(bs=0), INVALID), (dict(max_blocks=0), INVALID),
-    (dict(num_blocks=0), INVALID), (dict(G=257), UNSUPPORTED), (dict(num_blocks=1 << 30), UNSUPPORTED)])
+    (dict(num_blocks=0), INVALID), (dict(G=257), UNSUPPORTED), (dict(G=1, W=33), UNSUPPORTED), (dict(num_blocks=1 << 30), UNSUPPORTED)])
 def test_reorder_refusals(kw, rc):
     assert reorder(**kw) == rc
 
