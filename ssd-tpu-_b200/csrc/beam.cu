@@ -12,7 +12,7 @@
 // reach (and seldom more than a few times W), those values to shared memory, and each one's rank by counting the
 // larger ones.  Where more values reach the bound than fit (long runs of equal logits, sorted rows), W rounds of a
 // maximum over the CTA.  Order never depends on which thread comes first: equal values rank by their index.
-#include "common.cuh"
+#include "tcgen05.cuh"
 
 namespace ssd {
 namespace {
@@ -57,6 +57,13 @@ __device__ __forceinline__ T select_bound(T mine, int W, T* maxima, T* bound) {
 
 // Zeros of either sign are one value.
 __device__ __forceinline__ unsigned long long logit_key(float x, uint32_t i) { return argmax_key(x + 0.f, i); }
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+constexpr float kLog2e = 1.4426950408889634f;
 
 struct BeamRows {
   const float* logits;
@@ -107,21 +114,30 @@ __global__ void __launch_bounds__(kRowThreads, 4) beam_rows_kernel(const BeamRow
 #pragma unroll
   for (int i = 0; i < ITEMS; ++i) m = fmaxf(m, v[i]);
   const float t = select_bound<kRowThreads>(m, a.W, maxima, &bound_s);
-  // statistics: the thread's own maximum as reference, 0 where nothing is left of its part
-  float s = 0.f;
+  // statistics: the thread's own maximum as reference, 0 where nothing is left of its part.  e^(x - m) as 2^((x - m) log2 e):
+  // the difference first, which is exact where it counts.
   const float ref = m == -INFINITY ? 0.f : m;
-#pragma unroll
-  for (int i = 0; i < ITEMS; ++i) s += __expf(v[i] - ref);
   {
+    float2 s2 = make_float2(0.f, 0.f);
+    const float2 l2 = make_float2(kLog2e, kLog2e), r2 = make_float2(-ref, -ref), none = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < ITEMS; i += 2) {
+      const float2 e = tc::fma2(tc::add2(make_float2(v[i], v[i + 1]), r2), l2, none);
+      s2 = tc::add2(s2, make_float2(ex2(e.x), ex2(e.y)));
+    }
+    const float s = s2.x + s2.y;
     const float M = warp_max(m), R = M == -INFINITY ? 0.f : M;
-    const float S = warp_sum(m == -INFINITY ? s : s * __expf(m - R));
+    const float S = warp_sum(m == -INFINITY ? s : s * ex2((m - R) * kLog2e));
     if (lane == 0) ms[warp] = make_float2(M, S);
   }
+  const float least = fmaxf(t, -3.402823466e38f);  // -inf is never taken
+  if (m >= least) {
 #pragma unroll
-  for (int i = 0; i < ITEMS; ++i) {
-    if (v[i] >= t && v[i] > -INFINITY) {
-      const int at = atomicAdd(&count, 1);
-      if (at < kList) list[at] = logit_key(v[i], (uint32_t)(v0 + index(i)));
+    for (int i = 0; i < ITEMS; ++i) {
+      if (v[i] >= least) {
+        const int at = atomicAdd(&count, 1);
+        if (at < kList) list[at] = logit_key(v[i], (uint32_t)(v0 + index(i)));
+      }
     }
   }
   __syncthreads();
@@ -129,7 +145,7 @@ __global__ void __launch_bounds__(kRowThreads, 4) beam_rows_kernel(const BeamRow
   if (warp == 0) {
     const float2 w = lane < kRowThreads / 32 ? ms[lane] : make_float2(-INFINITY, 0.f);
     const float M = warp_max(w.x), R = M == -INFINITY ? 0.f : M;
-    const float S = warp_sum(w.x == -INFINITY ? w.y : w.y * __expf(w.x - R));
+    const float S = warp_sum(w.x == -INFINITY ? w.y : w.y * ex2((w.x - R) * kLog2e));
     if (lane == 0) a.stats[out] = make_float2(M, S);
   }
   unsigned long long* keys = a.keys + out * a.W;
@@ -190,7 +206,7 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamMer
   __shared__ unsigned long long maxima[32], bound_s;
   __shared__ unsigned long long list_k[kList];
   __shared__ uint32_t list_f[kList];
-  __shared__ double lse[kMaxBeams], base[kMaxBeams], norm[kMaxBeams];
+  __shared__ double lse[kMaxBeams], base[kMaxBeams], inv[kMaxBeams];
   __shared__ int kind[kMaxBeams];  // 0: offers nothing, 1: its tokens, 2: itself
   __shared__ int count;
   __shared__ unsigned long long red_k[kMergeThreads / 32];
@@ -224,45 +240,63 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamMer
       lse[w] = l;
       base[w] = sc;
       kind[w] = k;
-      norm[w] = a.alpha == 0.0 ? 1.0 : pow((double)(k == 2 ? max(len, 1) : len + 1), a.alpha);
+      inv[w] = a.alpha == 0.0 ? 1.0 : pow((double)(k == 2 ? max(len, 1) : len + 1), -a.alpha);
     }
   }
   if (tid == 0) count = 0;
   __syncthreads();
-  const int per = r.slices * W, total = W * per;
-  // candidate i: of beam i / per (its first one stands for a finished beam)
-  auto cand = [&](int i) {
+  // A beam's candidates go to T threads of the CTA, the first of them also standing for a finished beam.
+  const int per = r.slices * W;
+  int shift = 9;  // log2 of T
+  while (kMergeThreads >> shift < W) --shift;
+  const int w = tid >> shift, i0 = tid & ((1 << shift) - 1), step = 1 << shift;
+  const int mine = w < W ? kind[w] : 0;
+  auto cand = [&](unsigned long long key) {
     Cand c{0, 0xffffffffu};
-    const int w = i / per;
-    if (kind[w] == 0 || (kind[w] == 2 && i != w * per)) return c;
-    double rank;
-    uint32_t token;
-    if (kind[w] == 2) {
-      rank = base[w] / norm[w];
-      token = (uint32_t)a.eos;
-    } else {
-      const unsigned long long key = __ldcg(r.keys + (int64_t)g * total + i);
-      if (key == 0) return c;
-      token = argmax_key_index(key);
-      rank = (base[w] + ((double)argmax_key_value(key) - lse[w])) / norm[w];
-    }
+    if (key == 0) return c;
+    const uint32_t token = argmax_key_index(key);
+    const double rank = (base[w] + ((double)argmax_key_value(key) - lse[w])) * inv[w];
     if (!(rank > -INFINITY)) return c;  // NaN too
     c.key = double_key(rank + 0.0);
     c.flat = (uint32_t)w * (uint32_t)r.V + token;
     return c;
   };
-  unsigned long long best = 0;
-  for (int i = tid; i < total; i += kMergeThreads) best = max(best, cand(i).key);
+  const unsigned long long* keys = r.keys + ((int64_t)g * W + w) * per;
+  Cand self{0, 0xffffffffu};
+  if (mine == 2 && i0 == 0) {
+    const double rank = base[w] * inv[w];
+    if (rank > -INFINITY) self = Cand{double_key(rank + 0.0), (uint32_t)w * (uint32_t)r.V + (uint32_t)a.eos};
+  }
+  // the thread's first candidates stay in registers
+  constexpr int HELD = 4;
+  Cand held[HELD];
+  unsigned long long best = self.key, raw[HELD];
+#pragma unroll
+  for (int k = 0; k < HELD; ++k) {
+    const int i = i0 + k * step;
+    raw[k] = mine == 1 && i < per ? __ldcg(keys + i) : 0;
+  }
+#pragma unroll
+  for (int k = 0; k < HELD; ++k) {
+    held[k] = cand(raw[k]);
+    best = max(best, held[k].key);
+  }
+  const int more = mine == 1 ? per : 0;
+  for (int i = i0 + HELD * step; i < more; i += step) best = max(best, cand(__ldcg(keys + i)).key);
   const unsigned long long t = select_bound<kMergeThreads>(best, W, maxima, &bound_s);
-  for (int i = tid; i < total; i += kMergeThreads) {
-    const Cand c = cand(i);
-    if (c.key != 0 && c.key >= t) {
-      const int at = atomicAdd(&count, 1);
-      if (at < kList) {
-        list_k[at] = c.key;
-        list_f[at] = c.flat;
-      }
+  auto take = [&](const Cand& c) {
+    if (c.key == 0 || c.key < t) return;
+    const int at = atomicAdd(&count, 1);
+    if (at < kList) {
+      list_k[at] = c.key;
+      list_f[at] = c.flat;
     }
+  };
+  if (best >= t) {
+    take(self);
+#pragma unroll
+    for (int k = 0; k < HELD; ++k) take(held[k]);
+    for (int i = i0 + HELD * step; i < more; i += step) take(cand(__ldcg(keys + i)));
   }
   __syncthreads();
   auto put = [&](int k, unsigned long long key, uint32_t flat) {
@@ -305,13 +339,14 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamMer
     for (int k = 0; k < W; ++k) {
       unsigned long long bk = 0;
       uint32_t bf = 0xffffffffu;
-      for (int i = tid; i < total; i += kMergeThreads) {
-        const Cand c = cand(i);
+      auto next = [&](const Cand& c) {
         if (c.key != 0 && better(last_k, last_f, c.key, c.flat) && better(c.key, c.flat, bk, bf)) {
           bk = c.key;
           bf = c.flat;
         }
-      }
+      };
+      next(self);
+      for (int i = i0; i < more; i += step) next(cand(__ldcg(keys + i)));
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) {
         const unsigned long long ok = __shfl_xor_sync(kAll, bk, o);
