@@ -643,6 +643,14 @@ typedef struct {
    * kv_scales its scales [2, L, num_blocks, Hkv]: K and V enter by ssd_kv8_rope_append and the
    * attention is ssd_kv8_attention.  Not with qk_pairs weights. */
   float* kv_scales;
+  /* Rows that share prefixes (NULL: none): groups of rows and their prefixes as for ssd_shared_prefix_attention,
+   * which is the attention then, with this workspace (ssd_shared_prefix_attention_workspace_size for max_seq_len and
+   * the weights' dtype, 16-byte aligned).  An 8-bit cache is read row by row all the same. */
+  const int32_t* group_starts;     /* [num_groups + 1] */
+  const int32_t* prefix_lens;      /* [num_groups] */
+  int num_groups;
+  void* prefix_workspace;
+  size_t prefix_workspace_bytes;
 } ssd_gemma_batch;
 
 size_t ssd_gemma_scratch_size(const ssd_gemma_weights* w, int B, int T, int max_seq_len);

@@ -315,6 +315,12 @@ extern "C" int ssd_gemma_forward(ssd_stream_t stream, const ssd_gemma_weights* w
   if (bt->max_seq_len > w->rope_max_pos) return SSD_ERR_INVALID;
   if (w->tp_world > 1 && !bt->comm) return SSD_ERR_INVALID;
   if (bt->kv_scales && w->qk_pairs) return SSD_ERR_INVALID;
+  if (bt->group_starts && (!bt->prefix_lens || bt->num_groups <= 0)) return SSD_ERR_INVALID;
+  if (bt->group_starts && !bt->kv_scales) {  // before anything is launched
+    const size_t need = ssd_shared_prefix_attention_workspace_size(w->dtype, B, T, w->num_heads, w->num_kv_heads, w->head_dim,
+                                                                   bt->block_size, bt->num_groups, bt->max_seq_len);
+    if (!bt->prefix_workspace || bt->prefix_workspace_bytes < need) return SSD_ERR_WORKSPACE;
+  }
   if (bt->comm) {
     const ssd_comm* c = bt->comm;
     if (c->world != std::max(w->tp_world, 1) || c->rank != w->tp_rank || w->dtype != SSD_DTYPE_BF16 ||
@@ -423,6 +429,11 @@ extern "C" int ssd_gemma_forward(ssd_stream_t stream, const ssd_gemma_weights* w
                                 l, bt->block_tables, bt->max_blocks, s.seq_after, s.qlen, s.attn, scale, B, T, hq,
                                 bt->max_seq_len, reinterpret_cast<char*>(s.attn_ws) + kKv8WsOffset,
                                 s.attn_ws_bytes - kKv8WsOffset));
+    else if (bt->group_starts)
+      SSD_TRY(ssd_shared_prefix_attention(stream, s.q, bt->kv_pages, dt, L, bt->num_blocks, bt->block_size, hkv, D, l,
+                                          bt->block_tables, bt->max_blocks, s.seq_after, s.qlen, bt->group_starts,
+                                          bt->prefix_lens, bt->num_groups, s.attn, scale, B, T, hq, bt->max_seq_len,
+                                          bt->prefix_workspace, bt->prefix_workspace_bytes));
     else
     // early = 1: the kernel before it (RoPE + K/V write, or the QKV projection that
     // does them) writes only q and the new rows

@@ -131,6 +131,8 @@ class GemmaBatchC(C.Structure):
         ("prof_kind", C.POINTER(_i)),
         ("comm", C.POINTER(CommC)),
         ("kv_scales", _p),
+        ("group_starts", _p), ("prefix_lens", _p), ("num_groups", _i),
+        ("prefix_workspace", _p), ("prefix_workspace_bytes", _sz),
     ]
 
 

@@ -35,7 +35,7 @@ import torch
 
 from .. import _lib
 from .._lib import GemmaBatchC, GemmaWeightsC, check, dtype_code, lib, ptr, stream_ptr
-from ..kernels.kv8_cache import KV8CacheState
+from ..kernels.kv8_cache import KV8CacheState, ints
 from ..kernels.kv_cache import KVCacheState
 
 
@@ -311,9 +311,22 @@ class GemmaRunner:
             self._scratch[key] = buf
         return buf
 
+    def _prefix_workspace(self, b: int, t: int, block_size: int, groups: int) -> torch.Tensor:
+        key = (b, t, block_size, groups)
+        buf = self._scratch.get(key)
+        if buf is None:
+            s = self.w.shape
+            n = lib().ssd_shared_prefix_attention_workspace_size(
+                dtype_code(self.w.dtype), b, t, s.num_heads, s.num_kv_heads, s.head_dim, block_size, groups, self.max_seq_len)
+            buf = self._scratch[key] = torch.empty(max(n, 16), dtype=torch.uint8, device=self.w.device)
+        return buf
+
     def forward(self, tokens: torch.Tensor, seq_lens_before: torch.Tensor, pages,
                 block_tables: torch.Tensor, logits: torch.Tensor | None, q_lens: torch.Tensor | None = None,
-                last_only: bool = False, stream=None, prof: "ProjectionTimer | None" = None) -> torch.Tensor:
+                last_only: bool = False, stream=None, prof: "ProjectionTimer | None" = None,
+                groups: tuple[torch.Tensor, torch.Tensor] | None = None) -> torch.Tensor:
+        """``groups``: (group_starts, prefix_lens) as ``shared_prefix_attention`` takes them, for rows that share
+        prefixes (an 8-bit cache is read row by row all the same)."""
         b, t = tokens.shape
         sc = self.scratch(b, t)
         scales = None
@@ -335,6 +348,14 @@ class GemmaRunner:
         bt.logits, bt.logits_last_only = ptr(logits), int(bool(last_only))
         bt.scratch, bt.scratch_bytes = ptr(sc), sc.numel()
         bt.comm = self._comm_ptr
+        if groups is not None:
+            starts, prefixes = groups
+            n = prefixes.shape[0]
+            dev = tokens.get_device()
+            bt.group_starts, bt.prefix_lens = ints(starts, (n + 1,), "group_starts", dev), ints(prefixes, (n,), "prefix_lens", dev)
+            bt.num_groups = n
+            ws = self._prefix_workspace(b, t, pages.shape[3], n)
+            bt.prefix_workspace, bt.prefix_workspace_bytes = ptr(ws), ws.numel()
         if prof is not None:
             prof.attach(bt)
         check(lib().ssd_gemma_forward(stream_ptr(stream), C.byref(self.w.cstruct()), C.byref(bt)),

@@ -1,6 +1,7 @@
 """LLM inference engine: AR, SD, SSD modes (drop-in for jax_ssd/runtime/engine.py:33-333).
 
-* ``ar``  -- target-only greedy decode (``GreedyDecoder``);
+* ``ar``  -- target-only greedy decode (``GreedyDecoder``), or beam search (``BeamSearchDecoder``) where the sampling
+  parameters ask for ``num_beams`` > 1: the best beam of each prompt;
 * ``sd``  -- speculative decoding on the device-resident step of
   ``SpeculativeDecoder`` (one greedy prompt: draft k tokens, verify k+1, fused
   acceptance, page rollback, CUDA-graph replay -- the hot path this package
@@ -111,6 +112,8 @@ class LLMEngine:
         collector = MetricsCollector(mode=self.config.mode.value)
         collector.start()
         mode = self.config.mode
+        if sampling.num_beams > 1:
+            return self._run_beams(prompts, sampling, on_token, collector)
         batched = mode == DecodeMode.SD and (len(prompts) > 1 or sampling.temperature > 0)
         # the batched decoder's rows are the slots; the other paths take one prompt at a time
         sched = Scheduler(num_slots=self._num_slots(len(prompts)) if batched else 1)
@@ -194,6 +197,40 @@ class LLMEngine:
         collector.record_first_token()
         n = self._emit(seq, out, sampling.max_new_tokens, on_token)
         collector.record_step(StepMetrics(target_verify_ms=(time.perf_counter() - t0) * 1000, accepted_tokens=n))
+
+    def _run_beams(self, prompts, sampling, on_token, collector) -> tuple[list[list[int]], RunMetrics]:
+        """Beam search: the best beam of each prompt; as many prompts at a time as the rows of a forward take."""
+        W = int(sampling.num_beams)
+        if self.config.mode != DecodeMode.AR:
+            raise ValueError("num_beams > 1 needs ar mode")
+        if sampling.temperature > 0:
+            raise ValueError("num_beams > 1 needs temperature 0")
+        if not prompts:
+            return [], collector.finish()
+        dtype = torch.float32 if self.target_preset.startswith("toy") else torch.bfloat16
+        requests = min(len(prompts), max_tokens_per_forward(dtype) // W)
+        if requests < 1:
+            raise ValueError(f"num_beams {W} exceeds one forward ({max_tokens_per_forward(dtype)} rows)")
+        sched = Scheduler(num_slots=len(prompts))
+        seqs = [sched.add_request(p) for p in prompts]
+        max_len = self._max_len(max(len(s.prompt_token_ids) for s in seqs), sampling)
+        self.ranks.call("begin")
+        t0 = time.perf_counter()
+        try:
+            out = self.ranks.call("beam_generate", [list(s.prompt_token_ids) for s in seqs], W, requests,
+                                  sampling.max_new_tokens, max_len, self.config.block_size,
+                                  float(sampling.length_penalty),
+                                  None if sampling.ignore_eos else sampling.eos_token_id)[0]
+        finally:
+            status = self.ranks.call("end")
+        if any(status):
+            raise RuntimeError(f"a collective or another device-side wait timed out (rank statuses {status})")
+        collector.record_first_token()
+        n = sum(self._emit(s, beams[0][0] if beams else [], sampling.max_new_tokens, on_token)
+                for s, beams in zip(seqs, out))
+        collector.record_step(StepMetrics(target_verify_ms=(time.perf_counter() - t0) * 1000, accepted_tokens=n,
+                                          sequences=len(seqs)))
+        return [s.completion_token_ids for s in seqs], collector.finish()
 
     def _run_sd(self, seq, sampling, on_token, collector) -> None:
         k = self.config.speculate_k

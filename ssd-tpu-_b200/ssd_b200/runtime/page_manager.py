@@ -23,7 +23,7 @@ import torch
 
 from .._lib import check, lib, ptr, stream_ptr
 from ..kernels.kv8_cache import KV8CacheState
-from ..kernels.page_moves import compact_pages, copy_pages
+from ..kernels.page_moves import compact_pages, copy_pages, reorder_pages
 from .sequence import Sequence
 
 
@@ -164,6 +164,14 @@ class PageManager:
             # the partial page and its scales; a row that got no block has -1 there
             copy_pages(cache, self.tables[src_row, full:full + 1].expand(n), self.tables[dst_row0:dst_row0 + n, full])
         return ok[:n]
+
+    def reorder_rows(self, row0: int, parents: torch.Tensor, num_tokens: torch.Tensor, cache) -> torch.Tensor:
+        """Rows row0 .. row0 + G*W - 1 follow their parents [G, W] (beam search, ``page_moves.reorder_pages``): row g*W + i
+        becomes what row g*W + parents[g, i] was (-1: empty) for its first ``num_tokens`` [G*W] tokens.  ``cache``: the
+        cache, or every cache that uses this manager's blocks.  Returns ok [G*W] uint8 (device)."""
+        n = parents.numel()
+        return reorder_pages(cache, self.tables[row0:row0 + n], self.lens[row0:row0 + n], self.ref_counts_dev,
+                             self.free_list, self.free_top, parents, num_tokens)
 
     def compact(self, cache) -> torch.Tensor:
         """Move the blocks in use to the front of the pool (``page_moves.compact_pages``): tables, counts

@@ -68,6 +68,7 @@ class RankState:
         self.target = None  # GemmaAdapter of the ssd loop
         self.dec = None
         self._mark = None
+        self._beams = False  # beam search since the last ``end``
         if cfg.get("target_adapter"):
             self._adapter()  # its heap buffers are allocated before any generate call's mark
 
@@ -78,7 +79,7 @@ class RankState:
 
     def end(self) -> int:
         """End of a generate call: drop its decoders, free their heap buffers; the status of the device-side waits (the
-        collectives', and the 8-bit cache attention's)."""
+        collectives', and the attention kernels')."""
         torch.cuda.current_stream().synchronize()
         self.dec = None
         status = 0
@@ -88,6 +89,9 @@ class RankState:
                 self.comm.release(self._mark)
         if self.kv_cache_dtype == "fp8":
             status = lib().ssd_kv8_attention_status(stream_ptr()) or status
+        if self._beams:
+            self._beams = False
+            status = lib().ssd_shared_prefix_attention_status(stream_ptr()) or status
         return status
 
     # ------------------------------------------------------------ ar
@@ -96,6 +100,20 @@ class RankState:
 
         return GreedyDecoder(self.target_w, max_seq_len=max_len, block_size=block_size, comm=self.comm,
                              kv_cache_dtype=self.kv_cache_dtype).generate(prompt, max_new)
+
+    def beam_generate(self, prompts: list[list[int]], num_beams: int, requests: int, max_new: int, max_len: int,
+                      block_size: int, length_penalty: float, eos: int | None) -> list[list[tuple[list[int], float]]]:
+        from .beam import BeamSearchDecoder
+
+        self._beams = True
+        # one decoder for every batch of the call: its cache and scratch are the same for all
+        dec = BeamSearchDecoder(self.target_w, num_beams, requests, max_seq_len=max_len, block_size=block_size,
+                                comm=self.comm, kv_cache_dtype=self.kv_cache_dtype, length_penalty=length_penalty,
+                                eos_token_id=eos)
+        out = []
+        for i in range(0, len(prompts), requests):
+            out += dec.generate(prompts[i:i + requests], max_new)
+        return out
 
     # ------------------------------------------------------------ sd, one sequence (graph-replayed step)
     def sd_start(self, prompt: list[int], k: int, max_len: int, block_size: int) -> int:
