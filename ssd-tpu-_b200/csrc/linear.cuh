@@ -63,6 +63,7 @@ bool linear_tc_supported(int M, int N, int K);
 // page of one head, 64 dims wide (128-byte swizzle); D % 64 == 0.
 bool make_kv_page_map(CUtensorMap* m, const void* pages, int plane_pages, int block_size, int hkv, int D);
 bool make_kv_row_map(CUtensorMap* m, const void* base, int64_t rows, int heads, int D, int box_heads, int box_rows);
+bool make_kv_unit_map(CUtensorMap* m, const void* base, int64_t rows, int heads, int D);
 
 // ssd_paged_verify_attention with `early`: nonzero when the previous kernel in
 // the stream writes only q and this step's new K/V rows (the decoder forward),

@@ -1191,6 +1191,19 @@ bool make_kv_row_map(CUtensorMap* m, const void* base, int64_t rows, int heads, 
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+bool make_kv_unit_map(CUtensorMap* m, const void* base, int64_t rows, int heads, int D) {
+  // the same rows in 4-D (d % 64, row, d / 64, head): one box = 16 rows of one head, 64 dims after 64 dims
+  tc::EncodeFn fn = tc::encode_fn();
+  if (!fn || D % 64 || rows > 0x7fffffff) return false;
+  cuuint64_t dims[4] = {64, (cuuint64_t)rows, (cuuint64_t)(D / 64), (cuuint64_t)heads};
+  cuuint64_t strides[3] = {(cuuint64_t)heads * D * 2, 128, (cuuint64_t)D * 2};
+  cuuint32_t box[4] = {64, 16, (cuuint32_t)(D / 64), 1};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, box, estr,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 bool linear_tc_supported(int M, int N, int K) {
   return M >= 1 && M <= 256 && N >= 1 && K >= 64 && (K % 8) == 0 && (N + tc::BM - 1) / tc::BM <= kCounterCap &&
          tc::encode_fn() != nullptr;

@@ -344,7 +344,10 @@ __global__ void __launch_bounds__(kChunkC) prefix_attention_cc_kernel(const Pref
 //   warps 0-15  two sets of eight that take tiles of positions in turn, in each two threads a query row with half a
 //               tile's positions each: scores out of TMEM, maxima (exchanged between the two), weights, rescaling of
 //               O (only when a row's reference has to move).  Set 0 also writes results, set 1 brings Q into TMEM.
-//   warp 16     walks the tables and fetches Q and units by TMA into a ring of stages
+//   warp 16     walks the tables and fetches Q and the units of K by TMA into a ring of stages: a line of 64 dims of
+//               a unit's 16 rows at a time, which is what lays all of a tile's lines out as one operand
+//   warp 18     does the same for V, whole units at a time (each is an operand of its own); a warp alone would be
+//               held up by the issue of the copies, some 45 cycles each
 //   warp 17     issues the products in the order S(j + 2), O(j): S has one place in TMEM, free again as soon as the
 //               scores have been read (O(j) runs meanwhile), and the weights two
 // The sets share a row's reference M through shared memory: tile j decides on it once tile j - 1 has (`decided`), which
@@ -362,11 +365,11 @@ constexpr int UNITS = TILE / 16;
 constexpr int HALF = TILE / 2;         // positions of a thread
 constexpr int SET = 256;               // threads of a set of row warps
 constexpr int SETW = SET / 32;
-constexpr int THREADS = 2 * SET + 64;
+constexpr int THREADS = 2 * SET + 96;
 constexpr int META = 16;               // tiles whose units are described: more than there are between fetch and use
 constexpr int kMaxTiles = 256;         // also sequences and groups: their numbers are kept in shared memory
 constexpr int kMinUnits = 8;           // of a run: shorter ones cost more in prologues and joins than they save
-constexpr int kStart = 40;             // units that the start of a list is worth
+constexpr int kStart = 48;             // units that the start of a list is worth
 constexpr int kWhole = 64;             // lists of at most so many units are not cut
 constexpr int kMaxTeam = 8;            // CTAs that walk a group's lists side by side
 constexpr float kSpan = 8.f;           // weights are at most 2^8
@@ -376,9 +379,12 @@ __device__ uint32_t gave_up;           // 1 once a CTA's wait ran out
 
 template <int D>
 struct Cfg {
-  static constexpr int STAGES = D == 256 ? 6 : D == 128 ? 12 : 16;
-  static constexpr uint32_t KV = TILE * D * 2;  // bytes of a stage: one tile's K or V; Q takes two
-  static constexpr uint32_t ring = STAGES * KV;
+  static constexpr int STAGES = D == 256 ? 3 : 6;  // of K (and Q), and of V
+  static constexpr uint32_t KV = TILE * D * 2;     // bytes of one tile's K or V
+  static constexpr uint32_t KS = KV < 16384 ? 16384 : KV;  // of a stage of K
+  static constexpr int QST = ROWS * D * 2 / KS;    // stages that Q takes: lines of 64 dims, ROWS of them to a chunk
+  static constexpr int CPS = KS / 16384;           // chunks of a stage
+  static constexpr uint32_t v = STAGES * KS, ring = v + STAGES * KV;
   static constexpr uint32_t pref = ring;                              // int [kMaxTiles + 1], see Walk
   static constexpr uint32_t units = pref + 4 * (kMaxTiles + 4);       // int [kMaxTiles]: units of each tile
   static constexpr uint32_t info = units + 4 * kMaxTiles;             // int2 [kMaxTiles]
@@ -386,13 +392,14 @@ struct Cfg {
   static constexpr uint32_t ql = seq + 4 * kMaxTiles;                 // uint16: new tokens of the sequences,
   static constexpr uint32_t pre = ql + 2 * kMaxTiles;                 // prefixes of the groups
   static constexpr uint32_t first = pre + 4 * kMaxTiles;              // int [kMaxTiles + 1]: first sequences
-  static constexpr uint32_t cum = first + 4 * (kMaxTiles + 4);        // int [ROWS + 4]: units before a sequence's tail
-  static constexpr uint32_t meta = cum + 4 * (ROWS + 4);              // int4 [META][UNITS]
+  static constexpr uint32_t spt = first + 4 * (kMaxTiles + 4);        // int [kMaxTiles]: sequences of a group's tiles
+  static constexpr uint32_t cum = spt + 4 * kMaxTiles;                       // int [2][ROWS + 4]: units before a sequence's tail, for either fetching warp
+  static constexpr uint32_t meta = cum + 8 * (ROWS + 4);              // int4 [META][UNITS]
   static constexpr uint32_t pairs = meta + 16 * META * UNITS;         // float [set][turn][half][ROWS]: maxima
   static constexpr uint32_t refs = pairs + 4 * 8 * ROWS;              // float [tile parity][ROWS]: M
   static constexpr uint32_t sums = refs + 4 * 2 * ROWS;               // float [segment parity][set, half][ROWS]
   static constexpr uint32_t bars = sums + 4 * 8 * ROWS;
-  static constexpr uint32_t misc = bars + 8 * (2 * STAGES + 32);
+  static constexpr uint32_t misc = bars + 8 * (4 * STAGES + 32);
   static constexpr size_t smem = 1024 + misc + 32;
   // TMEM columns: scores, two tiles' weights (two bf16 to a column), Q (likewise), O
   static constexpr uint32_t p_col = TILE, q_col = 2 * TILE, o_col = q_col + D / 2, tmem_cols = D == 64 ? 256 : 512;
@@ -499,6 +506,13 @@ __device__ __forceinline__ void tma_rows(uint32_t dst, const CUtensorMap* map, u
       : "memory");
 }
 
+__device__ __forceinline__ void tma_unit(uint32_t dst, const CUtensorMap* map, uint32_t bar, int row, int head) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::
+          "r"(dst), "l"(map), "r"(bar), "r"(0), "r"(row), "r"(0), "r"(head)
+      : "memory");
+}
+
 // A run of units of one tile and head.
 struct Segment {
   int tile, head, lo, hi;   // units [lo, hi) of the tile's list
@@ -522,9 +536,9 @@ struct Shares {
     return run * q + run * (all - q * runs) / runs;
   }
 };
-// Tile m of the group that starts with sequence `first`.
-__device__ __forceinline__ int team_tile(const PrefixAttn& a, int first, int m) {
-  return a.tps > 1 ? first * a.tps + m : first + m * a.spt;
+// Tile m of the group that starts with sequence `first` and has `spt` of them to a tile.
+__device__ __forceinline__ int team_tile(const PrefixAttn& a, int first, int spt, int m) {
+  return a.tps > 1 ? first * a.tps + m : first + m * spt;
 }
 // x / spt (x < 512).
 __device__ __forceinline__ int by_spt(const PrefixAttn& a, int x) { return (x * a.spt_inv) >> 16; }
@@ -554,13 +568,13 @@ struct Walk {
     }
   }
   __device__ bool next(const PrefixAttn& a, const Shares& sh, const int* pref, const int* units_s, const int2* info,
-                       const int* first_s, Segment& s) {
+                       const int* first_s, const int* spt_s, Segment& s) {
     while (pos < end) {
       while (pref[at + 1] * a.hkv <= pos) ++at;
       const int list = pref[at + 1] - pref[at], first = pref[at] * a.hkv;
       s.head = (pos - first) / list;
       const int base = first + s.head * list + kStart;  // of the list's first unit
-      s.tile = sh.nm > 1 ? team_tile(a, first_s[at], (int)blockIdx.x % sh.nm) : at;
+      s.tile = sh.nm > 1 ? team_tile(a, first_s[at], spt_s[at], (int)blockIdx.x % sh.nm) : at;
       const int units = units_s[s.tile];
       s.lo = max(pos - base, 0);
       s.hi = min(min(base - kStart + list, end) - base, units);
@@ -652,7 +666,8 @@ __device__ __forceinline__ void put_parts(const PrefixAttn& a, int2 info, int ti
 
 template <int D>
 __global__ void __launch_bounds__(THREADS, 1)
-prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ CUtensorMap qmap,
+prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ CUtensorMap vmap,
+                           const __grid_constant__ CUtensorMap qmap,
                            const __grid_constant__ PrefixAttn a) {
   using C = Cfg<D>;
   extern __shared__ uint8_t smem_raw[];
@@ -665,7 +680,7 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid
   uint16_t* ql_s = reinterpret_cast<uint16_t*>(gen + C::ql);
   int* pre_s = reinterpret_cast<int*>(gen + C::pre);
   int* first_s = reinterpret_cast<int*>(gen + C::first);
-  int* cum = reinterpret_cast<int*>(gen + C::cum);
+  int* spt_s = reinterpret_cast<int*>(gen + C::spt);
   int4* meta = reinterpret_cast<int4*>(gen + C::meta);
   float* pair_s = reinterpret_cast<float*>(gen + C::pairs);
   float* ref_s = reinterpret_cast<float*>(gen + C::refs);
@@ -673,7 +688,9 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid
   auto bar = [&](int i) { return sm + C::bars + 8 * i; };
   auto full = [&](int s) { return bar(s); };
   auto freed = [&](int s) { return bar(C::STAGES + s); };
-  constexpr int B0 = 2 * C::STAGES;
+  auto v_full = [&](int s) { return bar(2 * C::STAGES + s); };
+  auto v_freed = [&](int s) { return bar(3 * C::STAGES + s); };
+  constexpr int B0 = 4 * C::STAGES;
   auto s_full = [&](int s) { return bar(B0 + s); };      // scores of a set's tile
   auto p_full = [&](int s) { return bar(B0 + 2 + s); };  // weights of a set's tile
   auto added = [&](int s) { return bar(B0 + 4 + s); };   // a set's tile is in O
@@ -693,6 +710,8 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid
     for (int s = 0; s < C::STAGES; ++s) {
       tc::mbar_init(full(s), 1);
       tc::mbar_init(freed(s), 1);
+      tc::mbar_init(v_full(s), 1);
+      tc::mbar_init(v_freed(s), 1);
     }
     for (int s = 0; s < 2; ++s) {
       tc::mbar_init(s_full(s), 1);
@@ -712,6 +731,7 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid
     *stop = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&map) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&vmap) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&qmap) : "memory");
   }
   if (warp == THREADS / 32 - 1) {
@@ -756,11 +776,16 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid
       first_s[tid] = start;
       pre_s[tid] = clamped(P, a.cap);
       if (tid == a.groups - 1) first_s[a.groups] = end;
-      if (tid == 0) slot[3] = a.tps > 1 ? (end - start) * a.tps : by_spt(a, end - start + a.spt - 1);
+    }
+    // tiles of the group, and sequences of each: as even as they come
+    const int of_group = a.tps > 1 ? (end - start) * a.tps : by_spt(a, max(end - start, 0) + a.spt - 1);
+    if (tid < a.groups) {
+      spt_s[tid] = a.tps > 1 || of_group < 1 ? 1 : (end - start + of_group - 1) / of_group;
+      if (tid == 0) slot[3] = of_group;
     }
     __syncthreads();
     const int nm = slot[3];  // tiles of the first group: of all, if there are to be teams
-    const bool same = tid >= a.groups || nm == (a.tps > 1 ? (end - start) * a.tps : by_spt(a, end - start + a.spt - 1));
+    const bool same = tid >= a.groups || nm == of_group;
     int g = 0, s = 0, e = 0;
     if (tid < a.B) {
       int n = a.groups;
@@ -774,12 +799,12 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid
     }
     if (tid >= s && tid < e) {  // (starts that ascend from 0 to B have every sequence in a group)
       const int own = pre_s[g], tail = tail_units(a, seq, ql, own), k = tid - s;
-      const int seq0 = a.tps > 1 ? tid : s + by_spt(a, k) * a.spt;
+      const int spt = spt_s[g], seq0 = s + k / spt * spt;
       const bool lead = seq0 == tid;
       for (int p = 0; p < a.tps; ++p) {
         const int t = seq0 * a.tps + p;
         atomicAdd(&units_s[t], tail + (lead ? prefix_units(own) : 0));
-        if (lead) info[t] = make_int2(tid | (a.tps > 1 ? p : min(a.spt, e - tid)) << 16, g | s << 16);
+        if (lead) info[t] = make_int2(tid | (a.tps > 1 ? p : min(spt, e - tid)) << 16, g | s << 16);
       }
     }
     const bool team = __syncthreads_and(same) && nm > 1 && nm <= kMaxTeam && nm * 4 <= (int)gridDim.x && !a.whole;
@@ -791,7 +816,7 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid
         int n = 0;
         if (t < lists) {
           if (team) {
-            for (int m = 0; m < nm; ++m) n = max(n, units_s[team_tile(a, first_s[t], m)]);
+            for (int m = 0; m < nm; ++m) n = max(n, units_s[team_tile(a, first_s[t], spt_s[t], m)]);
           } else {
             n = units_s[t];
           }
@@ -848,9 +873,9 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid
     const int quad = warp & 3, half = warp >> 2 & 1, set = warp / SETW;
     const int r = quad * 32 + lane;               // TMEM lanes 32 quad .., positions HALF half .. of a tile
     const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16);
-    int swaps = 0, n = 0;  // n: stages filled before
+    int swaps = 0, n = 0;  // n: stages of K filled before
     bool ok = true;
-    for (int seg = 0; walk.next(a, sh, pref, units_s, info, first_s, sg); ++seg) {
+    for (int seg = 0; walk.next(a, sh, pref, units_s, info, first_s, spt_s, sg); ++seg) {
       const int tiles = (sg.hi - sg.lo + UNITS - 1) / UNITS, last = jg + tiles - 1;
       const RowAt w = row_at<D>(a, sg.rows, sg.head, r, a.tile_rows, seq_s, ql_s);
       if (sg.lo == 0 && warp == SETW)
@@ -859,14 +884,16 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid
       const bool busy = __any_sync(0xffffffffu, real);
       if (set == 1) {
         // this thread's half of its row of Q out of the ring into TMEM (rows that are not there may hold anything)
-        ok = ok && (seg == 0 || held(q_free, (seg - 1) & 1)) && held(full(n % C::STAGES), (n / C::STAGES) & 1);
+        ok = ok && (seg == 0 || held(q_free, (seg - 1) & 1)) && held(full(n % C::STAGES), (n / C::STAGES) & 1) &&
+             (C::QST == 1 || held(full((n + 1) % C::STAGES), ((n + 1) / C::STAGES) & 1));
         if (ok) {
           tc::tc_fence_after();
           const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
 #pragma unroll
           for (int i = 0; i < D / 64; ++i) {  // 32 dims at a time: 4 pieces of 16 bytes
             const int dim = half * (D / 2) + 32 * i;
-            const uint32_t line = sm + (n % C::STAGES) * C::KV + dim / 64 * (ROWS * 128) + r * 128;
+            const int ch = dim / 64;
+            const uint32_t line = sm + (n + ch / C::CPS) % C::STAGES * C::KS + ch % C::CPS * (ROWS * 128) + r * 128;
             uint32_t y[16];
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
@@ -884,7 +911,7 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid
           if (lane == 0) tc::mbar_arrive(q_tmem);
         }
       }
-      n += 2 + 2 * tiles;
+      n += C::QST + tiles;
       // M: what the weights are relative to
       float M = kNothing, l = 0.f;
 #pragma unroll 1
@@ -1100,15 +1127,19 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid
       __syncwarp();
       if (lane == 0) tc::mbar_arrive(o_free);
     }
-  } else if (warp == 2 * SETW) {
+  } else if (warp != 2 * SETW + 1) {
     // -------------------------------------------------------------- pages
-    const int64_t rows_plane = (int64_t)a.num_layers * a.num_blocks * a.block_size;
-    const int64_t row_layer = (int64_t)a.layer_no * a.num_blocks * a.block_size;
     uint32_t lead;    // one lane issues: operands of the copies then stay in uniform registers
     asm volatile("{.reg .pred p; elect.sync _|p, 0xffffffff; selp.u32 %0, 1, 0, p;}" : "=r"(lead));
+    const bool is_v = warp != 2 * SETW;
+    const uint32_t ring = sm + (is_v ? C::v : 0u);
+    int* cum = reinterpret_cast<int*>(gen + C::cum) + (is_v ? ROWS + 4 : 0);
+    auto filled = [&](int s) { return is_v ? v_full(s) : full(s); };
+    auto emptied = [&](int s) { return is_v ? v_freed(s) : freed(s); };
+    const int plane_row = ((is_v ? a.num_layers : 0) + a.layer_no) * a.num_blocks * a.block_size;
     int n = 0;        // stages filled
     bool ok = true;
-    for (int seg = 0; ok && walk.next(a, sh, pref, units_s, info, first_s, sg); ++seg) {
+    for (int seg = 0; ok && walk.next(a, sh, pref, units_s, info, first_s, spt_s, sg); ++seg) {
       const int tiles = (sg.hi - sg.lo + UNITS - 1) / UNITS;
       const int P = pre_s[sg.rows.group], pu = prefix_units(P);
       int before = pu;
@@ -1150,7 +1181,7 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid
         }
       };
       int4 m;
-      int vrow[2] = {0, 0};  // rows of this lane's unit, of this batch and of the one before
+      int vrow = 0;  // rows of this lane's unit
       auto advance = [&] {
         const bool there = (unsigned)next_blk < (unsigned)a.num_blocks;
         m = there ? next_m : make_int4(0, 0, 0, -1);
@@ -1158,63 +1189,56 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid
         // units that are not there fetch the batch's first rows: finite values as a rule, and no bytes of DRAM
         const int first = __shfl_sync(0xffffffffu, row, 0);
         if (!there) row = first;
-        vrow[1] = vrow[0];
-        vrow[0] = row;
+        vrow = row;
       };
       look(0);
-      // Q: rows of all of the tile's tokens and heads, a box of 64 dims at a time, into two stages that lie side by side
-#pragma unroll
-      for (int h = 0; h < 2; ++h) ok = ok && (n + h < C::STAGES || held(freed((n + h) % C::STAGES), ((n + h) / C::STAGES - 1) & 1));
-      if (!ok) break;
-      if (lead) {
+      // Q: rows of all of the tile's tokens and heads, 64 dims at a time
+      for (int h = 0; ok && !is_v && h < C::QST; ++h, ++n) {
         const int st = n % C::STAGES;
-        tc::mbar_expect_tx(full(st), D / 64 * a.q_box * 128);
-        tc::mbar_arrive(full(st + 1));
+        ok = n < C::STAGES || held(freed(st), (n / C::STAGES - 1) & 1);
+        if (ok && lead) {
+          tc::mbar_expect_tx(full(st), C::CPS * a.q_box * 128);
 #pragma unroll
-        for (int ch = 0; ch < D / 64; ++ch)
-          tma_rows(sm + st * C::KV + ch * (ROWS * 128), &qmap, full(st), ch, sg.head * a.G,
-                   sg.rows.seq0 * a.T + sg.rows.part * (a.tile_rows / a.G));
-      }
-      __syncwarp();
-      n += 2;
-      auto fetch = [&](int row_of_lane, int in_batch, int64_t base, int plane) {
-        const int s = n % C::STAGES;
-        if (n >= C::STAGES && !held(freed(s), (n / C::STAGES - 1) & 1)) return false;
-        int rows[UNITS];
-#pragma unroll
-        for (int u = 0; u < UNITS; ++u)
-          rows[u] = (int)(plane * rows_plane + base) + __shfl_sync(0xffffffffu, row_of_lane, (in_batch * UNITS + u) & 31);
-        if (lead) {
-          tc::mbar_expect_tx(full(s), C::KV);
-#pragma unroll
-          for (int u = 0; u < UNITS; ++u)
-#pragma unroll
-            for (int ch = 0; ch < D / 64; ++ch)
-              tma_rows(sm + s * C::KV + ch * (TILE * 128) + u * 2048, &map, full(s), ch, sg.head, rows[u]);
+          for (int ch = 0; ch < C::CPS; ++ch)
+            tma_rows(sm + st * C::KS + ch * (ROWS * 128), &qmap, full(st), h * C::CPS + ch, sg.head * a.G,
+                     sg.rows.seq0 * a.T + sg.rows.part * (a.tile_rows / a.G));
         }
         __syncwarp();
-        ++n;
-        return true;
-      };
-      for (int j = 0; ok && j < tiles + 2; ++j) {  // K of tile j, V of tile j - 2: the order of the products
-        if (j < tiles) {
-          if (j % BATCH == 0) {
-            advance();
-            look(j + BATCH);
-          }
-          const int jt = jg + j;
-          if (lane / UNITS == j % BATCH) meta[(jt % META) * UNITS + lane % UNITS] = m;
-          __syncwarp();
-          ok = fetch(vrow[0], j % BATCH, row_layer, 0);
+      }
+      for (int j = 0; ok && j < tiles; ++j, ++n) {
+        if (j % BATCH == 0) {
+          advance();
+          look(j + BATCH);
         }
-        if (ok && j >= 2 && j - 2 < tiles)
-          ok = fetch((j - 2) / BATCH == min(j, tiles - 1) / BATCH ? vrow[0] : vrow[1], (j - 2) % BATCH, row_layer, 1);
+        const int jt = jg + j, st = n % C::STAGES;
+        if (!is_v && lane / UNITS == j % BATCH) meta[(jt % META) * UNITS + lane % UNITS] = m;
+        ok = n < C::STAGES || held(emptied(st), (n / C::STAGES - 1) & 1);
+        if (!ok) break;
+        int rows[UNITS];
+#pragma unroll
+        for (int u = 0; u < UNITS; ++u) rows[u] = plane_row + __shfl_sync(0xffffffffu, vrow, (j % BATCH) * UNITS + u);
+        __syncwarp();
+        if (lead) {
+          const uint32_t to = ring + st * (is_v ? C::KV : C::KS);
+          tc::mbar_expect_tx(filled(st), C::KV);
+          if (is_v) {
+#pragma unroll
+            for (int u = 0; u < UNITS; ++u) tma_unit(to + u * (16 * D * 2), &vmap, filled(st), rows[u], sg.head);
+          } else {
+#pragma unroll
+            for (int u = 0; u < UNITS; ++u)
+#pragma unroll
+              for (int ch = 0; ch < D / 64; ++ch)
+                tma_rows(to + ch * (TILE * 128) + u * 2048, &map, filled(st), ch, sg.head, rows[u]);
+          }
+        }
+        __syncwarp();
       }
       jg += tiles;
     }
     if (!ok) {  // copies in flight land before shared memory goes
       for (int i = max(0, n - C::STAGES); i < n; ++i)
-        for (uint32_t p = 0; p < kPolls && !tc::mbar_try_wait(full(i % C::STAGES), (i / C::STAGES) & 1); ++p) {}
+        for (uint32_t p = 0; p < kPolls && !tc::mbar_try_wait(filled(i % C::STAGES), (i / C::STAGES) & 1); ++p) {}
     }
     __syncwarp();
   } else {
@@ -1223,7 +1247,7 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid
     // registers.
     uint32_t lead;
     asm volatile("{.reg .pred p; elect.sync _|p, 0xffffffff; selp.u32 %0, 1, 0, p;}" : "=r"(lead));
-    int n = 0;
+    int n = 0, nv = 0;  // stages of K, of V used
     bool ok = true;
     auto ready = [&](uint32_t b0, uint32_t p0, uint32_t b1, uint32_t p1) {
       const bool yes = wait_for([&] { return try2(b0, p0, b1, p1); }, stop, a.polls);
@@ -1234,7 +1258,7 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid
       const int s = n % C::STAGES;
       // (no scores before the first ones: a wait for parity 1 of a barrier in its first phase is over)
       if (!ready(full(s), (n / C::STAGES) & 1, s_free, (jt - 1) & 1)) return false;
-      const uint64_t kd = tc::sw128_desc(sm + s * C::KV);
+      const uint64_t kd = tc::sw128_desc(sm + s * C::KS);
       if (lead) {
 #pragma unroll
         for (int d = 0; d < D / 64; ++d)
@@ -1249,33 +1273,30 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid
       ++n;
       return true;
     };
-    for (int seg = 0; ok && walk.next(a, sh, pref, units_s, info, first_s, sg); ++seg) {
+    for (int seg = 0; ok && walk.next(a, sh, pref, units_s, info, first_s, spt_s, sg); ++seg) {
       const int tiles = (sg.hi - sg.lo + UNITS - 1) / UNITS;
       ok = ready(q_tmem, seg & 1, q_tmem, seg & 1);
       if (!ok) break;
-      if (lead) {  // Q has left the ring
-        tc::mbar_arrive(freed(n % C::STAGES));
-        tc::mbar_arrive(freed(n % C::STAGES + 1));
-      }
-      n += 2;
+      for (int h = 0; h < C::QST; ++h, ++n)
+        if (lead) tc::mbar_arrive(freed(n % C::STAGES));  // Q has left the ring
       ok = scores(jg, tiles == 1) && (tiles < 2 || scores(jg + 1, tiles == 2)) && ready(o_free, (seg - 1) & 1, o_free, (seg - 1) & 1);
 #pragma unroll 1
       for (int j = 0; ok && j < tiles; ++j) {
         const int jt = jg + j;
         if (j + 2 < tiles) ok = scores(jt + 2, j + 3 == tiles);
-        const int s = n % C::STAGES;
-        ok = ok && ready(full(s), (n / C::STAGES) & 1, p_full(jt & 1), (jt >> 1) & 1);
+        const int s = nv % C::STAGES;
+        ok = ok && ready(v_full(s), (nv / C::STAGES) & 1, p_full(jt & 1), (jt >> 1) & 1);
         if (!ok) break;
-        const uint64_t vd = tc::mn128_desc<TILE>(sm + s * C::KV);
+        const uint64_t vd = tc::mn128_desc<16>(sm + C::v + s * C::KV);
         if (lead) {
 #pragma unroll
-          for (int k = 0; k < TILE / 16; ++k)  // 16 positions: 8 columns of P, two groups of 8 rows of V
-            tc::umma_ts(tmem + C::o_col, tmem + C::p_col + (jt & 1) * (TILE / 2) + 8 * k, vd + (2048 >> 4) * k,
+          for (int k = 0; k < UNITS; ++k)  // 16 positions: 8 columns of P, a unit of V
+            tc::umma_ts(tmem + C::o_col, tmem + C::p_col + (jt & 1) * (TILE / 2) + 8 * k, vd + ((16 * D * 2) >> 4) * k,
                         idesc<D, true>(), j || k);
           tc::umma_commit(added(jt & 1));
-          tc::umma_commit(freed(s));
+          tc::umma_commit(v_freed(s));
         }
-        ++n;
+        ++nv;
       }
       jg += tiles;
     }
@@ -1454,15 +1475,16 @@ PrefixLayout prefix_layout(int dtype, int B, int T, int hq, int hkv, int D, int 
 
 template <int D>
 int launch_tc(cudaStream_t st, const PrefixAttn& a, int ctas) {
-  CUtensorMap map, qmap;
+  CUtensorMap map, vmap, qmap;
   if (!make_kv_row_map(&map, a.pages, (int64_t)2 * a.num_layers * a.num_blocks * a.block_size, a.hkv, D, 1, 16) ||
+      !make_kv_unit_map(&vmap, a.pages, (int64_t)2 * a.num_layers * a.num_blocks * a.block_size, a.hkv, D) ||
       !make_kv_row_map(&qmap, a.q, (int64_t)a.B * a.T, a.hq, D, a.G, tile::ROWS / a.G))
     return SSD_ERR_LAUNCH;
   auto kern = tile::prefix_attention_tc_kernel<D>;
   constexpr size_t smem = tile::Cfg<D>::smem;
   static std::atomic<uint64_t> ready{0};
   if (!allow_smem(ready, kern, (int)smem)) return SSD_ERR_LAUNCH;
-  SSD_PDL(kern, ctas, tile::THREADS, smem, st, map, qmap, a);
+  SSD_PDL(kern, ctas, tile::THREADS, smem, st, map, vmap, qmap, a);
   const int64_t rows = (int64_t)a.B * a.T * a.hq;
   if (a.whole) return SSD_OK;
   SSD_PDL((prefix_join_kernel<bf16, D, tile::ROWS, true>), (unsigned)rows, 32 * kJoinWarps, 0, st, a);
