@@ -1316,19 +1316,23 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid
 }  // namespace tile
 
 // ------------------------------------------------------------------ join
-// out = sum_i w_i o_i / sum_i w_i l_i over a row's parts, w_i = e^(m_i - M).  Four warps a query row, each every fourth
-// part, a lane D / 32 dims.  Bound by latency: where the parts are, their statistics and sums at once, the
-// exchange between the warps.
-constexpr int kJoinWarps = 4, kJoinParts = 256;
+// out = sum_i w_i o_i / sum_i w_i l_i over a row's parts, w_i = e^(m_i - M).  NW warps a query row, each every NW-th part,
+// a lane D / 32 dims.  Bound by latency: where the parts are, then their statistics and sums at once, then (NW = 4)
+// the exchange between the warps.
+constexpr int kJoinParts = 160;
+// Rows up to which four warps take a row: so many CTAs are there at once (480 rows of some 9 parts: 21.2 against 22.9 us for
+// the whole call; 3584 rows of 4 or 5: 80.5 against 78.2).
+constexpr int64_t kJoinFew = 148 * 16;
 
-template <typename T, int D, int ROWS, bool LOG2>
-__global__ void __launch_bounds__(32 * kJoinWarps) prefix_join_kernel(const PrefixAttn a) {
-  constexpr int PL = D / 32, AHEAD = 4;
-  __shared__ float2 ml_s[kJoinParts];
-  __shared__ __align__(16) float o_s[kJoinWarps - 1][D];
-  __shared__ float sum_s[kJoinWarps];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t row = blockIdx.x;
+template <typename T, int D, int ROWS, bool LOG2, int NW>
+__global__ void __launch_bounds__(128) prefix_join_kernel(const PrefixAttn a) {
+  constexpr int PL = D / 32, VL = PL < 4 ? PL : 4, NV = PL / VL, AHEAD = NW == 1 ? 6 : 4;
+  __shared__ float2 ml_s[4 / NW][kJoinParts];
+  __shared__ __align__(16) float o_s[NW == 1 ? 1 : NW - 1][D];
+  __shared__ float sum_s[4];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = warp % NW, mine = warp / NW;
+  const int64_t row = (int64_t)blockIdx.x * (4 / NW) + mine;
+  if (row >= (int64_t)a.B * a.T * a.hq) return;  // (NW = 1: whole warps, which do not wait for one another)
   const int h = (int)(row % a.hq), t = (int)(row / a.hq % a.T), b = (int)(row / a.hq / a.T);
   const int head = h / a.G;
   const int in = t * a.G + h % a.G;  // among the sequence's rows of this KV head
@@ -1337,44 +1341,43 @@ __global__ void __launch_bounds__(32 * kJoinWarps) prefix_join_kernel(const Pref
   const int r = a.tps > 1 ? in % a.tile_rows : at.w + in;
   if (at.y == 1 || (unsigned)at.y > (unsigned)kJoinParts || (unsigned)r >= (unsigned)ROWS) return;
   auto part = [&](int i) { return (int64_t)(i == 0 ? at.x : (LOG2 ? at.x & ~1 : at.x) + i * at.z) * ROWS + r; };
+  auto sums = [&](int i, float* v) {
+    const float* from = a.ws_o + part(i) * D + lane * VL;
+#pragma unroll
+    for (int x = 0; x < NV; ++x) {
+      if constexpr (VL == 4) {
+        const float4 y = __ldcg(reinterpret_cast<const float4*>(from + x * 128));
+        v[4 * x] = y.x; v[4 * x + 1] = y.y; v[4 * x + 2] = y.z; v[4 * x + 3] = y.w;
+      } else {
+        const float2 y = __ldcg(reinterpret_cast<const float2*>(from));
+        v[0] = y.x; v[1] = y.y;
+      }
+    }
+  };
   float v[AHEAD][PL];
 #pragma unroll
-  for (int k = 0; k < AHEAD; ++k) {  // the first parts' sums before anything is known of their weights
-    const int i = warp + k * kJoinWarps;
-    if (i < at.y)
-#pragma unroll
-      for (int x = 0; x < PL; x += 2) {
-        const float2 y = __ldcg(reinterpret_cast<const float2*>(a.ws_o + part(i) * D + lane * 2 + x * 32));
-        v[k][x] = y.x;
-        v[k][x + 1] = y.y;
-      }
-  }
+  for (int k = 0; k < AHEAD; ++k)  // the first parts' sums before anything is known of their weights
+    if (sub + k * NW < at.y) sums(sub + k * NW, v[k]);
+  for (int i = lane + 32 * sub; i < at.y; i += 32 * NW) ml_s[mine][i] = __ldcg(a.ws_ml + part(i));
+  if constexpr (NW == 1) __syncwarp();
+  else __syncthreads();
   float M = -INFINITY;
-  for (int i = threadIdx.x; i < at.y; i += 32 * kJoinWarps) ml_s[i] = __ldcg(a.ws_ml + part(i));
-  __syncthreads();
-  for (int i = lane; i < at.y; i += 32) M = fmaxf(M, ml_s[i].x);
+  for (int i = lane; i < at.y; i += 32) M = fmaxf(M, ml_s[mine][i].x);
   M = warp_max(M);
   float o[PL], L = 0.f;
 #pragma unroll
   for (int x = 0; x < PL; ++x) o[x] = 0.f;
-  for (int i0 = warp; i0 < at.y; i0 += AHEAD * kJoinWarps) {
-    if (i0 != warp)
+  for (int i0 = sub; i0 < at.y; i0 += AHEAD * NW) {
+    if (i0 != sub) {
 #pragma unroll
-      for (int k = 0; k < AHEAD; ++k) {
-        const int i = i0 + k * kJoinWarps;
-        if (i < at.y)
-#pragma unroll
-          for (int x = 0; x < PL; x += 2) {
-            const float2 y = __ldcg(reinterpret_cast<const float2*>(a.ws_o + part(i) * D + lane * 2 + x * 32));
-            v[k][x] = y.x;
-            v[k][x + 1] = y.y;
-          }
-      }
+      for (int k = 0; k < AHEAD; ++k)
+        if (i0 + k * NW < at.y) sums(i0 + k * NW, v[k]);
+    }
 #pragma unroll
     for (int k = 0; k < AHEAD; ++k) {
-      const int i = i0 + k * kJoinWarps;
+      const int i = i0 + k * NW;
       if (i >= at.y) break;
-      const float2 ml = ml_s[i];
+      const float2 ml = ml_s[mine][i];
       if (ml.y == 0.f) continue;  // a part that the row sees nothing of is passed over, whatever it left
       const float w = LOG2 ? exp2f(ml.x - M) : expf(ml.x - M);
       L = fmaf(w, ml.y, L);
@@ -1382,33 +1385,31 @@ __global__ void __launch_bounds__(32 * kJoinWarps) prefix_join_kernel(const Pref
       for (int x = 0; x < PL; ++x) o[x] = fmaf(w, v[k][x], o[x]);
     }
   }
-  if (warp > 0) {
+  if constexpr (NW > 1) {
+    if (sub > 0) {
 #pragma unroll
-    for (int x = 0; x < PL; x += 2)
-      *reinterpret_cast<float2*>(&o_s[warp - 1][lane * 2 + x * 32]) = make_float2(o[x], o[x + 1]);
-    if (lane == 0) sum_s[warp] = L;
-  }
-  __syncthreads();
-  if (warp > 0) return;
+      for (int x = 0; x < PL; ++x) o_s[sub - 1][lane * VL + x % VL + x / VL * 128] = o[x];
+      if (lane == 0) sum_s[sub] = L;
+    }
+    __syncthreads();
+    if (sub > 0) return;
 #pragma unroll
-  for (int k = 1; k < kJoinWarps; ++k) {
-    L += sum_s[k];
+    for (int k = 1; k < NW; ++k) {
+      L += sum_s[k];
 #pragma unroll
-    for (int x = 0; x < PL; x += 2) {
-      const float2 y = *reinterpret_cast<const float2*>(&o_s[k - 1][lane * 2 + x * 32]);
-      o[x] += y.x;
-      o[x + 1] += y.y;
+      for (int x = 0; x < PL; ++x) o[x] += o_s[k - 1][lane * VL + x % VL + x / VL * 128];
     }
   }
   const float k = L != 0.f ? 1.f / L : 0.f;
-  T* out = reinterpret_cast<T*>(a.out) + row * D + lane * 2;
+  T* out = reinterpret_cast<T*>(a.out) + row * D + lane * VL;
 #pragma unroll
   for (int x = 0; x < PL; x += 2) {
     const float y0 = L != 0.f ? o[x] * k : 0.f, y1 = L != 0.f ? o[x + 1] * k : 0.f;
+    T* to = out + x % VL + x / VL * 128;
     if constexpr (sizeof(T) == 2)
-      *reinterpret_cast<__nv_bfloat162*>(out + x * 32) = __floats2bfloat162_rn(y0, y1);
+      *reinterpret_cast<__nv_bfloat162*>(to) = __floats2bfloat162_rn(y0, y1);
     else
-      *reinterpret_cast<float2*>(out + x * 32) = make_float2(y0, y1);
+      *reinterpret_cast<float2*>(to) = make_float2(y0, y1);
   }
 }
 
@@ -1487,7 +1488,10 @@ int launch_tc(cudaStream_t st, const PrefixAttn& a, int ctas) {
   SSD_PDL(kern, ctas, tile::THREADS, smem, st, map, vmap, qmap, a);
   const int64_t rows = (int64_t)a.B * a.T * a.hq;
   if (a.whole) return SSD_OK;
-  SSD_PDL((prefix_join_kernel<bf16, D, tile::ROWS, true>), (unsigned)rows, 32 * kJoinWarps, 0, st, a);
+  if (rows > kJoinFew)
+    SSD_PDL((prefix_join_kernel<bf16, D, tile::ROWS, true, 1>), (unsigned)((rows + 3) / 4), 128, 0, st, a);
+  else
+    SSD_PDL((prefix_join_kernel<bf16, D, tile::ROWS, true, 4>), (unsigned)rows, 128, 0, st, a);
   return SSD_OK;
 }
 
@@ -1496,7 +1500,7 @@ int launch_cc(cudaStream_t st, const PrefixAttn& a) {
   SSD_PDL((prefix_attention_cc_kernel<T, D>), dim3(a.nsplit, a.hkv, a.tiles), kChunkC, 0, st, a);
   if (a.nsplit == 1) return SSD_OK;
   const int64_t rows = (int64_t)a.B * a.T * a.hq;
-  SSD_PDL((prefix_join_kernel<T, D, kRowsC, false>), (unsigned)rows, 32 * kJoinWarps, 0, st, a);
+  SSD_PDL((prefix_join_kernel<T, D, kRowsC, false, 4>), (unsigned)rows, 128, 0, st, a);
   return SSD_OK;
 }
 
