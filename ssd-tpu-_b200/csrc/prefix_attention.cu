@@ -874,7 +874,7 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid
     const int r = quad * 32 + lane;               // TMEM lanes 32 quad .., positions HALF half .. of a tile
     const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16);
     int swaps = 0, n = 0;  // n: stages of K filled before
-    bool ok = true;
+    bool ok = a.polls > 0;  // (0: gives up before the first wait)
     for (int seg = 0; walk.next(a, sh, pref, units_s, info, first_s, spt_s, sg); ++seg) {
       const int tiles = (sg.hi - sg.lo + UNITS - 1) / UNITS, last = jg + tiles - 1;
       const RowAt w = row_at<D>(a, sg.rows, sg.head, r, a.tile_rows, seq_s, ql_s);
@@ -1032,8 +1032,10 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid
       }
       if (ok) {
         // the row's four threads add up what they have, relative to the last tile's M
-        if ((last & 1) != set) ok = held(decided(set ^ 1, quad), (last >> 1) & 1);
-        const float now = ok ? ref_s[(last & 1) * ROWS + r] : M;
+        // (of its own last tile a thread has M; the other half may not have written it down yet)
+        const bool other = (last & 1) != set;
+        if (other) ok = held(decided(set ^ 1, quad), (last >> 1) & 1);
+        const float now = ok && other ? ref_s[(last & 1) * ROWS + r] : M;
         float* to = sum_s + (seg & 1) * 4 * ROWS + r;
         to[(2 * set + half) * ROWS] = l == 0.f ? 0.f : l * ex2(M - now);
         M = now;
@@ -1076,7 +1078,7 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid
           }
         } else {
 #pragma unroll
-          for (int i = 0; i < 4 * NF; ++i) y[i] = 0x3f800000u;
+          for (int i = 0; i < 4 * NF; ++i) y[i] = 0x7fc00000u;  // (not `busy`: nobody reads it)
         }
         if (direct) {
           // (O may be anything where a row sees nothing)
@@ -1138,7 +1140,7 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid
     auto emptied = [&](int s) { return is_v ? v_freed(s) : freed(s); };
     const int plane_row = ((is_v ? a.num_layers : 0) + a.layer_no) * a.num_blocks * a.block_size;
     int n = 0;        // stages filled
-    bool ok = true;
+    bool ok = a.polls > 0;
     for (int seg = 0; ok && walk.next(a, sh, pref, units_s, info, first_s, spt_s, sg); ++seg) {
       const int tiles = (sg.hi - sg.lo + UNITS - 1) / UNITS;
       const int P = pre_s[sg.rows.group], pu = prefix_units(P);
@@ -1196,7 +1198,8 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid
       for (int h = 0; ok && !is_v && h < C::QST; ++h, ++n) {
         const int st = n % C::STAGES;
         ok = n < C::STAGES || held(freed(st), (n / C::STAGES - 1) & 1);
-        if (ok && lead) {
+        if (!ok) break;
+        if (lead) {
           tc::mbar_expect_tx(full(st), C::CPS * a.q_box * 128);
 #pragma unroll
           for (int ch = 0; ch < C::CPS; ++ch)
@@ -1236,7 +1239,7 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid
       }
       jg += tiles;
     }
-    if (!ok) {  // copies in flight land before shared memory goes
+    {  // copies in flight land before shared memory goes, whoever has given up
       for (int i = max(0, n - C::STAGES); i < n; ++i)
         for (uint32_t p = 0; p < kPolls && !tc::mbar_try_wait(filled(i % C::STAGES), (i / C::STAGES) & 1); ++p) {}
     }
@@ -1248,7 +1251,7 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid
     uint32_t lead;
     asm volatile("{.reg .pred p; elect.sync _|p, 0xffffffff; selp.u32 %0, 1, 0, p;}" : "=r"(lead));
     int n = 0, nv = 0;  // stages of K, of V used
-    bool ok = true;
+    bool ok = a.polls > 0;
     auto ready = [&](uint32_t b0, uint32_t p0, uint32_t b1, uint32_t p1) {
       const bool yes = wait_for([&] { return try2(b0, p0, b1, p1); }, stop, a.polls);
       tc::tc_fence_after();

@@ -17,7 +17,7 @@ from functools import lru_cache
 import torch
 
 from .._lib import dtype_code, lib
-from .kv8_cache import _rows, _tables, ints, launch
+from .kv8_cache import _current_device, _rows, _tables, ints, launch
 from .kv_cache import KVCacheState
 
 
@@ -65,3 +65,10 @@ def shared_prefix_attention(q: torch.Tensor, cache: KVCacheState, layer: int, bl
            groups, out.data_ptr(), hd ** -0.5 if scale is None else float(scale), b, t, hq, max_seq_len,
            None if ws is None else ws.data_ptr(), need)
     return out
+
+
+def check_shared_prefix_attention(device=None) -> None:
+    """Wait for the current stream of the GPU (None: the current one) and raise if a ``shared_prefix_attention`` there gave
+    up a device-side wait since the last check (``ssd_shared_prefix_attention_status``); its unfinished rows are NaN."""
+    dev = torch.device("cuda" if device is None else device)
+    launch("ssd_shared_prefix_attention_status", _current_device() if dev.index is None else dev.index)

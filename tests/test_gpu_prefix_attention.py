@@ -234,6 +234,81 @@ def test_graphs_and_streams(cuda):
     assert torch.equal(o1, shared_prefix_attention(**c1))
 
 
+WIDE = [  # more than a row tile, or than the tensor-core kernel's plan, holds; heads that fill no tile
+    (([300], [70], [1 + i % 9 for i in range(300)], 1, 8, 1, 64), 16),
+    (([1] * 270, [i % 40 for i in range(270)], [2] * 270, 2, 4, 2, 64), 16),
+    (([256], [33], [1 + i % 5 for i in range(256)], 1, 4, 4, 64), 16),
+    (([5, 2], [90, 17], [3, 4, 30, 6, 7, 3, 50], 3, 6, 2, 128), 48),
+    (([3], [200], [13, 40, 90], 13, 20, 2, 256), 32),
+    (([2], [100], [300, 310], 300, 8, 1, 64), 16),
+    (([3, 2], [40, 20], [1, 2, 3, 4, 5], 1, 256, 1, 64), 16),
+    (([2, 3], [2000, 40], [1, 900, 3, 1500, 8], 1, 130, 1, 128), 16),
+]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("shape,bs", WIDE, ids=range(len(WIDE)))
+def test_wide_batches_and_odd_heads(cuda, shape, bs, dtype):
+    check(case(41, *shape, bs, dtype))
+
+
+@pytest.mark.parametrize("dtype,bs", [("bf16", 16), ("bf16", 4), ("f32", 16)])
+def test_lengths_past_their_bounds_count_as_the_bounds(cuda, dtype, bs):
+    """q_lens above T are T; positions from max_seq_len on are not read, whatever lengths and prefixes say."""
+    import torch
+
+    from ssd_b200.kernels.prefix_attention import shared_prefix_attention
+
+    c = case(42, [3, 1], [64, 40], [9, 8, 20, 5], 2, 8, 2, 64, bs, dtype)
+    want = shared_prefix_attention(**c)
+    assert torch.equal(shared_prefix_attention(**{**c, "q_lens": torch.full_like(c["seq_lens"], 9)}), want)
+    short = shared_prefix_attention(**c, max_seq_len=48).double().cpu().numpy()
+    keys = {**c, "block_tables": c["block_tables"].clone()}
+    keys["block_tables"][:, 48 // bs:] = -1  # the same positions missing
+    w, size, slack = oracle(keys)
+    assert (np.abs(short - w) <= bound(keys, w, size, slack)).all()
+
+
+@pytest.mark.parametrize("hq,hkv,d,prefix", [(8, 1, 256, 40), (8, 1, 256, 3000), (16, 4, 64, 700), (4, 2, 128, 1500)])
+def test_a_wait_that_runs_out_is_reported(cuda, hq, hkv, d, prefix):
+    """No polls allowed: every CTA gives up at its first wait.  Rows are NaN (those past q_lens zeros), the status says so
+    once, and the next call is right."""
+    from ssd_b200._lib import SSDError, lib
+    from ssd_b200.kernels.prefix_attention import check_shared_prefix_attention, shared_prefix_attention
+
+    c = case(43, [3, 2], [prefix, 20], [9, 8, 20, 30, 6], 2, hq, hkv, d, 16, q_lens=[2, 1, 2, 2, 0])
+    check_shared_prefix_attention()
+    assert lib().ssd_shared_prefix_attention_set_polls(-2) == 1
+    try:
+        assert lib().ssd_shared_prefix_attention_set_polls(0) == 0
+        got = shared_prefix_attention(**c).float().cpu().numpy()
+    finally:
+        assert lib().ssd_shared_prefix_attention_set_polls(-1) == 0
+    with pytest.raises(SSDError, match="timed out"):
+        check_shared_prefix_attention()
+    check_shared_prefix_attention("cuda")
+    for b, n in enumerate([2, 1, 2, 2, 0]):
+        assert np.isnan(got[b, :n]).all() and (got[b, n:] == 0).all()
+    check(c)
+    check_shared_prefix_attention()
+
+
+@pytest.mark.parametrize("shape", [SHAPES[3], SHAPES[4], SHAPES[7], ([2, 1], [3000, 1000], [70, 8, 5], 2, 8, 2, 256)],
+                         ids=range(4))
+def test_repeats_are_equal_to_the_bit(cuda, shape):
+    """Sums are taken in one order: threads that came in another would show in a few of many calls."""
+    import torch
+
+    from ssd_b200.kernels.prefix_attention import shared_prefix_attention
+
+    c = case(44, *shape, 16)
+    want = shared_prefix_attention(**c)
+    differ = torch.zeros((), dtype=torch.int64, device="cuda")
+    for _ in range(2500):
+        differ += (shared_prefix_attention(**c) != want).any()
+    assert int(differ) == 0
+
+
 def test_nothing_to_do(cuda):
     import torch
 
