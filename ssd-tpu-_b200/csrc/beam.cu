@@ -12,6 +12,8 @@
 // reach (and seldom more than a few times W), those values to shared memory, and each one's rank by counting the
 // larger ones.  Where more values reach the bound than fit (long runs of equal logits, sorted rows), W rounds of a
 // maximum over the CTA.  Order never depends on which thread comes first: equal values rank by their index.
+#include <algorithm>
+
 #include "tcgen05.cuh"
 
 namespace ssd {
@@ -19,26 +21,14 @@ namespace {
 
 constexpr int kMaxBeams = 32;
 constexpr int kRowThreads = 256, kMergeThreads = 512;
-constexpr int kList = 256;             // candidates that reach the bound
+constexpr int kList = 256;             // candidates that there is room for
+constexpr int kFewItems = 16, kManyItems = 32;  // logits of a thread
 constexpr unsigned kAll = 0xffffffffu;
 
-// Lane's rank among the warp's 32 values (largest first, lower lanes before equal ones).
-template <typename T>
-__device__ __forceinline__ int lane_rank(T v) {
-  const int lane = threadIdx.x & 31;
-  int rank = 0;
-#pragma unroll
-  for (int i = 0; i < 32; ++i) {
-    const T o = __shfl_sync(kAll, v, i);
-    rank += o > v || (o == v && i < lane);
-  }
-  return rank;
-}
-
-// The W-th largest of the maxima of 32 groups of THREADS / 32 threads, for every thread; `maxima` and `bound` are shared
-// memory.
+// The largest value that at least W of the maxima of 32 groups of THREADS / 32 threads reach; `maxima` is shared memory.
+// Every warp finds it for itself, which takes one barrier.
 template <int THREADS, typename T>
-__device__ __forceinline__ T select_bound(T mine, int W, T* maxima, T* bound) {
+__device__ __forceinline__ T select_bound(T mine, int W, T* maxima) {
   constexpr int N = THREADS / 32;
 #pragma unroll
   for (int o = N / 2; o > 0; o >>= 1) {
@@ -47,12 +37,12 @@ __device__ __forceinline__ T select_bound(T mine, int W, T* maxima, T* bound) {
   }
   if (threadIdx.x % N == 0) maxima[threadIdx.x / N] = mine;
   __syncthreads();
-  if (threadIdx.x < 32) {
-    const T v = maxima[threadIdx.x];
-    if (lane_rank(v) == W - 1) *bound = v;
-  }
-  __syncthreads();
-  return *bound;
+  const T v = maxima[threadIdx.x & 31];
+  int reach = 0;
+#pragma unroll
+  for (int i = 0; i < 32; ++i) reach += maxima[i] >= v;
+  const int least = __reduce_min_sync(kAll, reach >= W ? reach : 33);
+  return __shfl_sync(kAll, v, __ffs(__ballot_sync(kAll, reach == least)) - 1);
 }
 
 // Zeros of either sign are one value.
@@ -65,27 +55,60 @@ __device__ __forceinline__ float ex2(float x) {
 }
 constexpr float kLog2e = 1.4426950408889634f;
 
+// What a sum of e^(x - m) is worth relative to M >= m (not both -inf).  e^(x - m) as 2^((x - m) log2 e): the difference first,
+// which is exact where it counts.
+__device__ __forceinline__ float to_larger(float m, float M) { return ex2((m - M) * kLog2e); }
+
 struct BeamRows {
   const float* logits;
   int64_t ld;
   const float* scores;
   const uint8_t* finished;
-  int W, V, slices;
+  int W, V, slices;              // slices of a row
   float2* stats;                 // [row][slice] maximum, sum of e^(x - maximum)
   unsigned long long* keys;      // [row][slice][W] argmax_key, largest first; 0: none
 };
 
 __device__ __forceinline__ bool reads_logits(const float* scores, const uint8_t* finished, int row) {
-  return ld_act(scores + row) > -INFINITY && !(finished && ld_act(finished + row));
+  const float score = ld_act(scores + row);
+  const uint8_t done = finished ? ld_act(finished + row) : 0;  // (both loads at once)
+  return score > -INFINITY && !done;
+}
+
+struct RowShared {
+  unsigned long long list[kList];  // candidates of the part so far
+  unsigned long long red[32];
+  float maxima[32];
+  float sums[kRowThreads / 32];
+  int count;
+};
+
+// More of a slice reaches its bound than there is room for (runs of equal logits): the W best, one after another.  The logits
+// are read again.  Returns how many there are.
+__device__ __noinline__ int crowded(RowShared& sh, const float* x, int n, int v0, int W) {
+  unsigned long long last = ~0ull;
+  int found = 0;
+#pragma unroll 1
+  for (; found < W; ++found) {
+    unsigned long long best = 0;
+#pragma unroll 1
+    for (int i = threadIdx.x; i < n; i += kRowThreads) {
+      const float y = ld_act(x + i);
+      const unsigned long long key = logit_key(y, (uint32_t)(v0 + i));
+      if (y > -INFINITY && key < last && key > best) best = key;
+    }
+    best = block_reduce(best, sh.red, OpMax());
+    if (best == 0) break;
+    if (threadIdx.x == 0) sh.list[found] = best;
+    last = best;
+  }
+  __syncthreads();
+  return found;
 }
 
 template <int ITEMS, bool VEC>
-__global__ void __launch_bounds__(kRowThreads, 4) beam_rows_kernel(const BeamRows a) {
-  __shared__ unsigned long long list[kList];
-  __shared__ float maxima[32];
-  __shared__ float2 ms[kRowThreads / 32];
-  __shared__ float bound_s;
-  __shared__ int count;
+__global__ void __launch_bounds__(kRowThreads, ITEMS == kManyItems ? 4 : 6) beam_rows_kernel(const BeamRows a) {
+  __shared__ RowShared sh;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int slice = blockIdx.x, row = blockIdx.y;
   pdl_wait();
@@ -93,13 +116,13 @@ __global__ void __launch_bounds__(kRowThreads, 4) beam_rows_kernel(const BeamRow
   if (!reads_logits(a.scores, a.finished, row)) return;
   const int v0 = slice * (ITEMS * kRowThreads), n = min(ITEMS * kRowThreads, a.V - v0);
   const float* x = a.logits + row * a.ld + v0;
+  auto at = [&](int i) { return VEC ? ((i >> 2) * kRowThreads + tid) * 4 + (i & 3) : i * kRowThreads + tid; };
   float v[ITEMS];
-  auto index = [&](int i) { return VEC ? ((i >> 2) * kRowThreads + tid) * 4 + (i & 3) : i * kRowThreads + tid; };
   if constexpr (VEC) {
 #pragma unroll
     for (int i = 0; i < ITEMS; i += 4) {
       uint4 u = make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u);
-      if (index(i) < n) u = ld_act_v4(x + index(i));  // n is a multiple of 4
+      if (at(i) < n) u = ld_act_v4(x + at(i));  // n is a multiple of 4
       v[i] = __uint_as_float(u.x);
       v[i + 1] = __uint_as_float(u.y);
       v[i + 2] = __uint_as_float(u.z);
@@ -107,75 +130,64 @@ __global__ void __launch_bounds__(kRowThreads, 4) beam_rows_kernel(const BeamRow
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < ITEMS; ++i) v[i] = index(i) < n ? ld_act(x + index(i)) : -INFINITY;
+    for (int i = 0; i < ITEMS; ++i) v[i] = at(i) < n ? ld_act(x + at(i)) : -INFINITY;
   }
-  if (tid == 0) count = 0;
-  float m = -INFINITY;
+  if (tid == 0) sh.count = 0;
+  float m = -INFINITY, most[ITEMS / 8];
 #pragma unroll
-  for (int i = 0; i < ITEMS; ++i) m = fmaxf(m, v[i]);
-  const float t = select_bound<kRowThreads>(m, a.W, maxima, &bound_s);
-  // statistics: the thread's own maximum as reference, 0 where nothing is left of its part.  e^(x - m) as 2^((x - m) log2 e):
-  // the difference first, which is exact where it counts.
+  for (int k = 0; k < ITEMS / 8; ++k) {
+    most[k] = v[8 * k];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) most[k] = fmaxf(most[k], v[8 * k + i]);
+    m = fmaxf(m, most[k]);  // (NaN counts as -inf)
+  }
+  const float bound = fmaxf(select_bound<kRowThreads>(m, a.W, sh.maxima), -3.402823466e38f);  // -inf is never taken
+  if (m >= bound) {
+#pragma unroll
+    for (int k = 0; k < ITEMS / 8; ++k) {
+      if (!(most[k] >= bound)) continue;
+#pragma unroll
+      for (int i = 8 * k; i < 8 * k + 8; ++i) {
+        if (v[i] >= bound) {
+          const int place = atomicAdd(&sh.count, 1);
+          if (place < kList) sh.list[place] = logit_key(v[i], (uint32_t)(v0 + at(i)));
+        }
+      }
+    }
+  }
+  // the thread's sum, relative to its maximum (0 where nothing is left of its part)
   const float ref = m == -INFINITY ? 0.f : m;
+  float2 s2 = make_float2(0.f, 0.f);
   {
-    float2 s2 = make_float2(0.f, 0.f);
     const float2 l2 = make_float2(kLog2e, kLog2e), r2 = make_float2(-ref, -ref), none = make_float2(0.f, 0.f);
 #pragma unroll
     for (int i = 0; i < ITEMS; i += 2) {
       const float2 e = tc::fma2(tc::add2(make_float2(v[i], v[i + 1]), r2), l2, none);
       s2 = tc::add2(s2, make_float2(ex2(e.x), ex2(e.y)));
     }
-    const float s = s2.x + s2.y;
-    const float M = warp_max(m), R = M == -INFINITY ? 0.f : M;
-    const float S = warp_sum(m == -INFINITY ? s : s * ex2((m - R) * kLog2e));
-    if (lane == 0) ms[warp] = make_float2(M, S);
-  }
-  const float least = fmaxf(t, -3.402823466e38f);  // -inf is never taken
-  if (m >= least) {
-#pragma unroll
-    for (int i = 0; i < ITEMS; ++i) {
-      if (v[i] >= least) {
-        const int at = atomicAdd(&count, 1);
-        if (at < kList) list[at] = logit_key(v[i], (uint32_t)(v0 + index(i)));
-      }
-    }
   }
   __syncthreads();
-  const int64_t out = (int64_t)row * a.slices + slice;
-  if (warp == 0) {
-    const float2 w = lane < kRowThreads / 32 ? ms[lane] : make_float2(-INFINITY, 0.f);
-    const float M = warp_max(w.x), R = M == -INFINITY ? 0.f : M;
-    const float S = warp_sum(w.x == -INFINITY ? w.y : w.y * ex2((w.x - R) * kLog2e));
-    if (lane == 0) a.stats[out] = make_float2(M, S);
+  // the candidates in order, and the sums relative to the largest of them
+  int found = sh.count;
+  if (found > kList) found = crowded(sh, x, n, v0, a.W);
+  unsigned long long* keys = a.keys + ((int64_t)row * a.slices + slice) * a.W;
+  if (tid < found) {
+    const unsigned long long mine = sh.list[tid];
+    int rank = 0;
+#pragma unroll 4
+    for (int i = 0; i < found; ++i) rank += sh.list[i] > mine;
+    if (rank < a.W) keys[rank] = mine;
   }
-  unsigned long long* keys = a.keys + out * a.W;
-  const int found = count;
-  if (found <= kList) {
-    if (tid < found) {
-      const unsigned long long mine = list[tid];
-      int rank = 0;
-      for (int i = 0; i < found; ++i) rank += list[i] > mine;
-      if (rank < a.W) keys[rank] = mine;
-    }
-    if (tid >= found && tid < a.W) keys[tid] = 0;
-    return;
-  }
-  unsigned long long last = ~0ull;
-  for (int k = 0; k < a.W; ++k) {
-    unsigned long long best = 0;
+  if (tid >= found && tid < a.W) keys[tid] = 0;
+  const float M = key_float(__reduce_max_sync(kAll, float_key(sh.maxima[lane])));
+  const float S = warp_sum(m == -INFINITY ? s2.x + s2.y : (s2.x + s2.y) * to_larger(m, M));
+  if (lane == 0) sh.sums[warp] = S;
+  __syncthreads();
+  if (tid == 0) {
+    float total = sh.sums[0];
 #pragma unroll
-    for (int i = 0; i < ITEMS; ++i) {
-      if (!(v[i] > -INFINITY)) continue;
-      const unsigned long long key = logit_key(v[i], (uint32_t)(v0 + index(i)));
-      if (key < last && key > best) best = key;
-    }
-    best = block_reduce(best, list, OpMax());
-    if (tid == 0) keys[k] = best;
-    if (best == 0) {
-      for (int i = k + 1 + tid; i < a.W; i += kRowThreads) keys[i] = 0;
-      return;
-    }
-    last = best;
+    for (int i = 1; i < kRowThreads / 32; ++i) total += sh.sums[i];
+    a.stats[(int64_t)row * a.slices + slice] = make_float2(M, total);
   }
 }
 
@@ -203,54 +215,62 @@ __device__ __forceinline__ bool better(unsigned long long ka, uint32_t fa, unsig
 }
 
 __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamMerge a) {
-  __shared__ unsigned long long maxima[32], bound_s;
+  __shared__ unsigned long long maxima[32];
   __shared__ unsigned long long list_k[kList];
   __shared__ uint32_t list_f[kList];
+  __shared__ float list_x[kList];
   __shared__ double lse[kMaxBeams], base[kMaxBeams], inv[kMaxBeams];
-  __shared__ int kind[kMaxBeams];  // 0: offers nothing, 1: its tokens, 2: itself
+  __shared__ int kind[kMaxBeams], len_s[kMaxBeams];  // 0: offers nothing, 1: its tokens, 2: itself
   __shared__ int count;
   __shared__ unsigned long long red_k[kMergeThreads / 32];
   __shared__ uint32_t red_f[kMergeThreads / 32];
   const BeamRows& r = a.r;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = blockIdx.x, W = r.W;
   pdl_wait();
-  for (int w = warp; w < W; w += kMergeThreads / 32) {
-    const int row = g * W + w;
+  // two tasks a beam, a warp each: log sum e^x, and length^-alpha
+  for (int task = warp; task < 2 * W; task += kMergeThreads / 32) {
+    const int w = task < W ? task : task - W, row = g * W + w;
     const float sc = ld_act(r.scores + row);
     const bool done = r.finished && ld_act(r.finished + row);
-    const int len = a.lengths ? ld_act(a.lengths + row) : 0;
     const int k = sc > -INFINITY ? (done ? 2 : 1) : 0;
+    if (task >= W) {
+      const int len = a.lengths ? ld_act(a.lengths + row) : 0;
+      const double y = a.alpha == 0.0 ? 1.0 : pow((double)(k == 2 ? max(len, 1) : len + 1), -a.alpha);
+      if (lane == 0) {
+        inv[w] = y;
+        len_s[w] = len;
+      }
+      continue;
+    }
     double l = 0.0;
     if (k == 1) {
       const float2* st = r.stats + (int64_t)row * r.slices;
+      const int n = r.slices;
       float M = -INFINITY;
-      for (int i = lane; i < r.slices; i += 32) M = fmaxf(M, __ldcg(st + i).x);
+      for (int i = lane; i < n; i += 32) M = fmaxf(M, __ldcg(st + i).x);
       M = warp_max(M);
-      const float R = M == -INFINITY ? 0.f : M;
       double S = 0.0;
-      for (int i = lane; i < r.slices; i += 32) {
+      for (int i = lane; i < n; i += 32) {
         const float2 y = __ldcg(st + i);
-        S += y.x == -INFINITY ? (double)y.y : (double)y.y * exp((double)y.x - (double)R);
+        S += (double)(y.x == -INFINITY ? y.y : y.y * to_larger(y.x, M));
       }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) S += __shfl_xor_sync(kAll, S, o);
-      l = (double)R + log(S);
+      l = (M == -INFINITY ? 0.0 : (double)M) + log(S);
     }
     if (lane == 0) {
       lse[w] = l;
       base[w] = sc;
       kind[w] = k;
-      inv[w] = a.alpha == 0.0 ? 1.0 : pow((double)(k == 2 ? max(len, 1) : len + 1), -a.alpha);
     }
   }
   if (tid == 0) count = 0;
   __syncthreads();
   // A beam's candidates go to T threads of the CTA, the first of them also standing for a finished beam.
-  const int per = r.slices * W;
   int shift = 9;  // log2 of T
   while (kMergeThreads >> shift < W) --shift;
   const int w = tid >> shift, i0 = tid & ((1 << shift) - 1), step = 1 << shift;
-  const int mine = w < W ? kind[w] : 0;
+  const int mine = w < W ? kind[w] : 0, per = mine == 1 ? r.slices * W : 0;
   auto cand = [&](unsigned long long key) {
     Cand c{0, 0xffffffffu};
     if (key == 0) return c;
@@ -261,7 +281,7 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamMer
     c.flat = (uint32_t)w * (uint32_t)r.V + token;
     return c;
   };
-  const unsigned long long* keys = r.keys + ((int64_t)g * W + w) * per;
+  const unsigned long long* keys = r.keys + ((int64_t)g * W + w) * r.slices * W;
   Cand self{0, 0xffffffffu};
   if (mine == 2 && i0 == 0) {
     const double rank = base[w] * inv[w];
@@ -274,44 +294,46 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamMer
 #pragma unroll
   for (int k = 0; k < HELD; ++k) {
     const int i = i0 + k * step;
-    raw[k] = mine == 1 && i < per ? __ldcg(keys + i) : 0;
+    raw[k] = i < per ? __ldcg(keys + i) : 0;
   }
 #pragma unroll
   for (int k = 0; k < HELD; ++k) {
     held[k] = cand(raw[k]);
     best = max(best, held[k].key);
   }
-  const int more = mine == 1 ? per : 0;
-  for (int i = i0 + HELD * step; i < more; i += step) best = max(best, cand(__ldcg(keys + i)).key);
-  const unsigned long long t = select_bound<kMergeThreads>(best, W, maxima, &bound_s);
-  auto take = [&](const Cand& c) {
+  for (int i = i0 + HELD * step; i < per; i += step) best = max(best, cand(__ldcg(keys + i)).key);
+  const unsigned long long t = select_bound<kMergeThreads>(best, W, maxima);
+  auto take = [&](const Cand& c, float x) {
     if (c.key == 0 || c.key < t) return;
     const int at = atomicAdd(&count, 1);
     if (at < kList) {
       list_k[at] = c.key;
       list_f[at] = c.flat;
+      list_x[at] = x;
     }
   };
   if (best >= t) {
-    take(self);
+    take(self, 0.f);
 #pragma unroll
-    for (int k = 0; k < HELD; ++k) take(held[k]);
-    for (int i = i0 + HELD * step; i < more; i += step) take(cand(__ldcg(keys + i)));
+    for (int k = 0; k < HELD; ++k) take(held[k], argmax_key_value(raw[k]));
+    for (int i = i0 + HELD * step; i < per; i += step) {
+      const unsigned long long key = __ldcg(keys + i);
+      take(cand(key), argmax_key_value(key));
+    }
   }
   __syncthreads();
-  auto put = [&](int k, unsigned long long key, uint32_t flat) {
+  auto put = [&](int k, unsigned long long key, uint32_t flat, float x) {
     const int at = g * W + k;
     float score = -INFINITY;
     int parent = -1, token = -1, len = 0, fin = 1;
     if (key != 0) {
       parent = (int)(flat / (uint32_t)r.V);
       token = (int)(flat - (uint32_t)parent * (uint32_t)r.V);
-      const int before = a.lengths ? ld_act(a.lengths + g * W + parent) : 0;
+      const int before = len_s[parent];
       if (kind[parent] == 2) {
         score = (float)base[parent];
         len = before;
       } else {
-        const float x = ld_act(r.logits + (int64_t)(g * W + parent) * r.ld + token);
         score = (float)(base[parent] + ((double)x - lse[parent]));
         len = before + 1;
         fin = token == a.eos;
@@ -330,9 +352,9 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamMer
       const uint32_t flat = list_f[tid];
       int rank = 0;
       for (int i = 0; i < found; ++i) rank += better(list_k[i], list_f[i], key, flat);
-      if (rank < W) put(rank, key, flat);
+      if (rank < W) put(rank, key, flat, list_x[tid]);
     }
-    if (tid >= found && tid < W) put(tid, 0, 0);
+    if (tid >= found && tid < W) put(tid, 0, 0, 0.f);
   } else {
     unsigned long long last_k = ~0ull;
     uint32_t last_f = 0;
@@ -346,7 +368,7 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamMer
         }
       };
       next(self);
-      for (int i = i0; i < more; i += step) next(cand(__ldcg(keys + i)));
+      for (int i = i0; i < per; i += step) next(cand(__ldcg(keys + i)));
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) {
         const unsigned long long ok = __shfl_xor_sync(kAll, bk, o);
@@ -358,15 +380,16 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamMer
       __syncthreads();
       for (int i = 0; i < kMergeThreads / 32; ++i)
         if (better(red_k[i], red_f[i], bk, bf)) { bk = red_k[i]; bf = red_f[i]; }
-      if (tid == 0) put(k, bk, bf);
+      if (tid == 0) {
+        const uint32_t parent = bf / (uint32_t)r.V;
+        put(k, bk, bf, bk ? ld_act(r.logits + (int64_t)(g * W + parent) * r.ld + (bf - parent * (uint32_t)r.V)) : 0.f);
+      }
       last_k = bk;
       last_f = bf;
     }
   }
   pdl_trigger();
 }
-
-constexpr int kFewItems = 16, kManyItems = 32;
 
 struct BeamLayout {
   int items, slices;
@@ -411,8 +434,8 @@ extern "C" int ssd_beam_select(ssd_stream_t stream, const float* logits, int64_t
   if (!workspace || workspace_bytes < L.total) return SSD_ERR_WORKSPACE;
   if (reinterpret_cast<uintptr_t>(workspace) & 15) return SSD_ERR_UNSUPPORTED;
   char* w = reinterpret_cast<char*>(workspace);
-  BeamRows r{logits, ld, scores, finished, W, V, L.slices, reinterpret_cast<float2*>(w),
-             reinterpret_cast<unsigned long long*>(w + L.off_keys)};
+  const BeamRows r{logits, ld, scores, finished, W, V, L.slices, reinterpret_cast<float2*>(w),
+                   reinterpret_cast<unsigned long long*>(w + L.off_keys)};
   const dim3 grid(L.slices, G * W);
   const bool vec = !(reinterpret_cast<uintptr_t>(logits) & 15) && ld % 4 == 0 && V % 4 == 0;
   if (L.items == kManyItems) {

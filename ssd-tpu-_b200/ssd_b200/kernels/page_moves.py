@@ -155,8 +155,8 @@ def reorder_pages(cache, tables: torch.Tensor, lens: torch.Tensor, ref_counts: t
     n, cols = tables.shape
     if n != g * w:
         raise ValueError(f"{list(parents.shape)} parents do not fit {n} rows")
-    work = parents.new_empty((3, max(n, 1)))  # the copies: sources, targets, rows
-    ok = parents.new_empty((n,), dtype=torch.uint8)
+    work = parents.new_empty(3 * max(n, 1))  # the copies: sources, targets, rows
+    ok = parents.new_empty(n, dtype=torch.uint8)
     src, step = work.data_ptr(), 4 * max(n, 1)
     launch("ssd_page_reorder", dev, ints(tables, (n, cols), "tables", dev), ints(lens, (n,), "lens", dev), cols,
            ints(free_list, (nb,), "free_list", dev), ints(free_top, (1,), "free_top", dev),

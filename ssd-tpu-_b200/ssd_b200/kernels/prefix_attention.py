@@ -58,7 +58,7 @@ def shared_prefix_attention(q: torch.Tensor, cache: KVCacheState, layer: int, bl
     dtype = dtype_code(q.dtype)
     # a workspace of its own for every call: calls on other streams or in captured graphs share nothing
     need = _workspace_size(dtype, b, t, hq, hkv, hd, bs, groups, max_seq_len)
-    ws = q.new_empty((need,), dtype=torch.uint8) if need else None
+    ws = q.new_empty(need, dtype=torch.uint8) if need else None
     launch("ssd_shared_prefix_attention", dev, at, p.data_ptr(), dtype, nl, nb, bs, hkv, hd, layer, tab, cols,
            ints(seq_lens, (b,), "seq_lens", dev), ints(q_lens, (b,), "q_lens", dev),
            ints(group_starts, (groups + 1,), "group_starts", dev), ints(prefix_lens, (groups,), "prefix_lens", dev),
