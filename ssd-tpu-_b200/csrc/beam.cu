@@ -107,7 +107,7 @@ __device__ __noinline__ int crowded(RowShared& sh, const float* x, int n, int v0
 }
 
 template <int ITEMS, bool VEC>
-__global__ void __launch_bounds__(kRowThreads, ITEMS == kManyItems ? 4 : 6) beam_rows_kernel(const BeamRows a) {
+__global__ void __launch_bounds__(kRowThreads, ITEMS == kManyItems ? 5 : 8) beam_rows_kernel(const BeamRows a) {
   __shared__ RowShared sh;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int slice = blockIdx.x, row = blockIdx.y;
@@ -227,6 +227,7 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamMer
   const BeamRows& r = a.r;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = blockIdx.x, W = r.W;
   pdl_wait();
+  pdl_trigger();
   // two tasks a beam, a warp each: log sum e^x, and length^-alpha
   for (int task = warp; task < 2 * W; task += kMergeThreads / 32) {
     const int w = task < W ? task : task - W, row = g * W + w;
@@ -388,7 +389,6 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamMer
       last_f = bf;
     }
   }
-  pdl_trigger();
 }
 
 struct BeamLayout {

@@ -39,6 +39,10 @@ struct Reorder {
 };
 
 __device__ __forceinline__ void cluster_barrier() {
+  if (gridDim.x == 1) {
+    __syncthreads();
+    return;
+  }
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
@@ -75,6 +79,7 @@ __global__ void __launch_bounds__(kReorderThreads) page_reorder_kernel(const Reo
   __shared__ int used_s, tmp[32];
   const int tid = threadIdx.x, B = a.G * a.W;
   pdl_wait();
+  pdl_trigger();
   int parent = 0, len = 0, held = 0;
   if (tid < B) {
     parent = ld_act(a.parents + tid);
@@ -224,7 +229,6 @@ __global__ void __launch_bounds__(kReorderThreads) page_reorder_kernel(const Reo
     a.rows[b] = rows;
   }
   if (tid == 0) *a.free_top = max(avail - all, 0);
-  pdl_trigger();
 }
 
 bool allow_cluster(std::atomic<uint64_t>& ready, void (*kern)(Reorder)) {
