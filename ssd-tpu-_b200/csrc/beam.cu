@@ -22,7 +22,8 @@ namespace {
 constexpr int kMaxBeams = 32;
 constexpr int kRowThreads = 256, kMergeThreads = 512;
 constexpr int kList = 256;             // candidates that there is room for
-constexpr int kFewItems = 16, kManyItems = 32;  // logits of a thread
+constexpr int kItems = 32;             // logits of a thread
+constexpr int kSlice = kItems * kRowThreads;
 constexpr unsigned kAll = 0xffffffffu;
 
 // The largest value that at least W of the maxima of 32 groups of THREADS / 32 threads reach; `maxima` is shared memory.
@@ -106,21 +107,21 @@ __device__ __noinline__ int crowded(RowShared& sh, const float* x, int n, int v0
   return found;
 }
 
-template <int ITEMS, bool VEC>
-__global__ void __launch_bounds__(kRowThreads, ITEMS == kManyItems ? 5 : 8) beam_rows_kernel(const BeamRows a) {
+template <bool VEC>
+__global__ void __launch_bounds__(kRowThreads, 5) beam_rows_kernel(const BeamRows a) {
   __shared__ RowShared sh;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int slice = blockIdx.x, row = blockIdx.y;
   pdl_wait();
   pdl_trigger();
   if (!reads_logits(a.scores, a.finished, row)) return;
-  const int v0 = slice * (ITEMS * kRowThreads), n = min(ITEMS * kRowThreads, a.V - v0);
+  const int v0 = slice * kSlice, n = min(kSlice, a.V - v0);
   const float* x = a.logits + row * a.ld + v0;
   auto at = [&](int i) { return VEC ? ((i >> 2) * kRowThreads + tid) * 4 + (i & 3) : i * kRowThreads + tid; };
-  float v[ITEMS];
+  float v[kItems];
   if constexpr (VEC) {
 #pragma unroll
-    for (int i = 0; i < ITEMS; i += 4) {
+    for (int i = 0; i < kItems; i += 4) {
       uint4 u = make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u);
       if (at(i) < n) u = ld_act_v4(x + at(i));  // n is a multiple of 4
       v[i] = __uint_as_float(u.x);
@@ -130,12 +131,12 @@ __global__ void __launch_bounds__(kRowThreads, ITEMS == kManyItems ? 5 : 8) beam
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < ITEMS; ++i) v[i] = at(i) < n ? ld_act(x + at(i)) : -INFINITY;
+    for (int i = 0; i < kItems; ++i) v[i] = at(i) < n ? ld_act(x + at(i)) : -INFINITY;
   }
   if (tid == 0) sh.count = 0;
-  float m = -INFINITY, most[ITEMS / 8];
+  float m = -INFINITY, most[kItems / 8];
 #pragma unroll
-  for (int k = 0; k < ITEMS / 8; ++k) {
+  for (int k = 0; k < kItems / 8; ++k) {
     most[k] = v[8 * k];
 #pragma unroll
     for (int i = 1; i < 8; ++i) most[k] = fmaxf(most[k], v[8 * k + i]);
@@ -144,7 +145,7 @@ __global__ void __launch_bounds__(kRowThreads, ITEMS == kManyItems ? 5 : 8) beam
   const float bound = fmaxf(select_bound<kRowThreads>(m, a.W, sh.maxima), -3.402823466e38f);  // -inf is never taken
   if (m >= bound) {
 #pragma unroll
-    for (int k = 0; k < ITEMS / 8; ++k) {
+    for (int k = 0; k < kItems / 8; ++k) {
       if (!(most[k] >= bound)) continue;
 #pragma unroll
       for (int i = 8 * k; i < 8 * k + 8; ++i) {
@@ -161,7 +162,7 @@ __global__ void __launch_bounds__(kRowThreads, ITEMS == kManyItems ? 5 : 8) beam
   {
     const float2 l2 = make_float2(kLog2e, kLog2e), r2 = make_float2(-ref, -ref), none = make_float2(0.f, 0.f);
 #pragma unroll
-    for (int i = 0; i < ITEMS; i += 2) {
+    for (int i = 0; i < kItems; i += 2) {
       const float2 e = tc::fma2(tc::add2(make_float2(v[i], v[i + 1]), r2), l2, none);
       s2 = tc::add2(s2, make_float2(ex2(e.x), ex2(e.y)));
     }
@@ -392,17 +393,16 @@ __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamMer
 }
 
 struct BeamLayout {
-  int items, slices;
+  int slices;
   size_t off_keys, total;
 };
 
 BeamLayout beam_layout(int G, int W, int V) {
   BeamLayout L;
-  const int64_t rows = (int64_t)G * W;
-  L.items = rows * ((V + kManyItems * kRowThreads - 1) / (kManyItems * kRowThreads)) >= 2 * 148 ? kManyItems : kFewItems;
-  L.slices = (V + L.items * kRowThreads - 1) / (L.items * kRowThreads);
-  L.off_keys = (sizeof(float2) * (size_t)rows * L.slices + 255) & ~size_t(255);
-  L.total = L.off_keys + sizeof(unsigned long long) * (size_t)rows * L.slices * W;
+  const size_t rows = (size_t)G * W;
+  L.slices = (int)(((int64_t)V + kSlice - 1) / kSlice);
+  L.off_keys = (sizeof(float2) * rows * L.slices + 255) & ~size_t(255);
+  L.total = L.off_keys + sizeof(unsigned long long) * rows * L.slices * W;
   return L;
 }
 
@@ -438,13 +438,8 @@ extern "C" int ssd_beam_select(ssd_stream_t stream, const float* logits, int64_t
                    reinterpret_cast<unsigned long long*>(w + L.off_keys)};
   const dim3 grid(L.slices, G * W);
   const bool vec = !(reinterpret_cast<uintptr_t>(logits) & 15) && ld % 4 == 0 && V % 4 == 0;
-  if (L.items == kManyItems) {
-    if (vec) SSD_PDL((beam_rows_kernel<kManyItems, true>), grid, kRowThreads, 0, stream, r);
-    else SSD_PDL((beam_rows_kernel<kManyItems, false>), grid, kRowThreads, 0, stream, r);
-  } else {
-    if (vec) SSD_PDL((beam_rows_kernel<kFewItems, true>), grid, kRowThreads, 0, stream, r);
-    else SSD_PDL((beam_rows_kernel<kFewItems, false>), grid, kRowThreads, 0, stream, r);
-  }
+  if (vec) SSD_PDL(beam_rows_kernel<true>, grid, kRowThreads, 0, stream, r);
+  else SSD_PDL(beam_rows_kernel<false>, grid, kRowThreads, 0, stream, r);
   const BeamMerge m{r, lengths, eos, (double)length_penalty, out_scores, out_parents, out_tokens, out_lengths,
                     out_finished};
   SSD_PDL(beam_merge_kernel, G, kMergeThreads, 0, stream, m);
