@@ -10,8 +10,10 @@
 //                 bits, the W best are written in order.
 // The W largest of a CTA: the maxima of 32 groups of threads, the W-th largest of these as a bound that at least W values
 // reach (and seldom more than a few times W), those values to shared memory, and each one's rank by counting the
-// larger ones.  Where more values reach the bound than fit (long runs of equal logits, sorted rows), W rounds of a
-// maximum over the CTA.  Order never depends on which thread comes first: equal values rank by their index.
+// larger ones.  Where more values reach the bound than fit (long runs of equal logits), W rounds of a maximum over the
+// CTA.  Order never depends on which thread comes first: equal values rank by their index.
+// Bound by DRAM for many rows: 256 rows of 256000 logits take 51 us, the rows kernel 46 of them (262 MB, 5.7 TB/s), 32
+// rows 11.6 us; few rows by the two kernels' chains of reads and barriers: one row of 256000 logits 6.6 us.
 #include <algorithm>
 
 #include "tcgen05.cuh"
@@ -22,7 +24,10 @@ namespace {
 constexpr int kMaxBeams = 32;
 constexpr int kRowThreads = 256, kMergeThreads = 512;
 constexpr int kList = 256;             // candidates that there is room for
-constexpr int kItems = 32;             // logits of a thread
+// Logits of a thread.  16: 71 us instead of 51 for 256 rows of 256000, 7.0 instead of 6.6 for one: what a CTA does once, some
+// 2 us of it, is worth more than the second wave that small slices save.  Slices fetched ahead into shared memory by CTAs
+// that stay (one pass, a running bound) came out at 60 us: the slices' barriers leave less in flight than CTAs that come and go.
+constexpr int kItems = 32;
 constexpr int kSlice = kItems * kRowThreads;
 constexpr unsigned kAll = 0xffffffffu;
 
@@ -107,6 +112,8 @@ __device__ __noinline__ int crowded(RowShared& sh, const float* x, int n, int v0
   return found;
 }
 
+// VEC: 16 bytes a load, where the rows' alignment allows it (256 rows of 256000 logits 53 us, of 255999 58).  Five CTAs an
+// SM (48 registers): 51 us, four 56, six 52.
 template <bool VEC>
 __global__ void __launch_bounds__(kRowThreads, 5) beam_rows_kernel(const BeamRows a) {
   __shared__ RowShared sh;
@@ -215,6 +222,8 @@ __device__ __forceinline__ bool better(unsigned long long ka, uint32_t fa, unsig
   return ka > kb || (ka == kb && fa < fb);
 }
 
+// A CTA a request: bound by latency, of the fp64 logarithms and powers and a handful of barriers (some 4 us; 32 requests of 8
+// beams, 2048 candidates each, 5 us).
 __global__ void __launch_bounds__(kMergeThreads) beam_merge_kernel(const BeamMerge a) {
   __shared__ unsigned long long maxima[32];
   __shared__ unsigned long long list_k[kList];
