@@ -251,9 +251,12 @@ bool allow_cluster(std::atomic<uint64_t>& ready, void (*kern)(Reorder)) {
 template <int WM>
 int launch_reorder(cudaStream_t st, const Reorder& a) {
   static std::atomic<uint64_t> ready{0};  // devices whose limit is raised
-  const unsigned ctas = (int64_t)a.G * a.max_blocks <= kOneCta ? 1 : kCluster;
-  if (ctas > 1 && !allow_cluster(ready, page_reorder_kernel<WM>)) return SSD_ERR_LAUNCH;
-  if (launch_pdl_cluster(page_reorder_kernel<WM>, dim3(ctas), dim3(kReorderThreads), 0, st, ctas, a) != cudaSuccess) {
+  if ((int64_t)a.G * a.max_blocks <= kOneCta) {
+    SSD_PDL(page_reorder_kernel<WM>, 1, kReorderThreads, 0, st, a);
+    return SSD_OK;
+  }
+  if (!allow_cluster(ready, page_reorder_kernel<WM>)) return SSD_ERR_LAUNCH;
+  if (launch_pdl_cluster(page_reorder_kernel<WM>, dim3(kCluster), dim3(kReorderThreads), 0, st, kCluster, a) != cudaSuccess) {
     (void)cudaGetLastError();
     return SSD_ERR_LAUNCH;
   }

@@ -143,12 +143,12 @@ def reorder_pages(cache, tables: torch.Tensor, lens: torch.Tensor, ref_counts: t
     pools = [_pool(c) for c in cache] if isinstance(cache, (list, tuple)) else [_pool(cache)]
     if not pools:
         raise ValueError("reorder_pages wants a cache")
-    dev, nb = pools[0][0], pools[0][3]
-    bs = pools[0][7][1]
-    if any(p[0] != dev or p[3] != nb or p[7][1] != bs for p in pools):
-        raise ValueError("the caches of one pool have the same blocks, block size and device")
-    if any(p[5] > _MAX_PAGE for p in pools):  # before the tables change: the copies would be refused
-        raise ValueError(f"a page of one plane may hold {_MAX_PAGE} bytes at most")
+    dev, _, _, nb, _, _, _, (_, bs, _, _) = pools[0]
+    for p in pools:
+        if p[0] != dev or p[3] != nb or p[7][1] != bs:
+            raise ValueError("the caches of one pool have the same blocks, block size and device")
+        if p[5] > _MAX_PAGE:  # before the tables change: the copies would be refused
+            raise ValueError(f"a page of one plane may hold {_MAX_PAGE} bytes at most")
     if parents.dim() != 2 or tables.dim() != 2:
         raise ValueError(f"parents are [G, W] and tables [G*W, max_blocks], got {list(parents.shape)} and {list(tables.shape)}")
     g, w = parents.shape
