@@ -81,6 +81,7 @@ __global__ void __launch_bounds__(kReorderThreads) page_reorder_kernel(const Reo
   __shared__ int children[kMaxReorder], first[kMaxReorder];
   __shared__ int need_s[kMaxReorder], len_s[kMaxReorder];  // blocks that a row's tokens take, and that it has
   __shared__ int part_s[kMaxReorder];                  // index of the partial page (-1: none)
+  __shared__ int whole_s[kMaxReorder];                 // of a request: columns that are whole pages of all its rows
   __shared__ int used_s, tmp[32];
   const int tid = threadIdx.x, B = a.G * a.W;
   pdl_wait();
@@ -95,6 +96,7 @@ __global__ void __launch_bounds__(kReorderThreads) page_reorder_kernel(const Reo
   if (tid == 0) used_s = 0;
   children[tid] = 0;
   first[tid] = B;
+  whole_s[tid] = a.max_blocks;
   __syncthreads();
   len = min(max(len, 0), a.max_blocks);
   held = max(held, 0);
@@ -106,6 +108,7 @@ __global__ void __launch_bounds__(kReorderThreads) page_reorder_kernel(const Reo
     len_s[tid] = len;
     part_s[tid] = part ? full : -1;
     parent_s[tid] = (int16_t)parent;
+    atomicMin(&whole_s[tid / a.W], parent >= 0 ? full : 0);
     if (parent >= 0) {
       atomicAdd(&children[parent], 1);
       atomicMin(&first[parent], tid);
@@ -129,18 +132,30 @@ __global__ void __launch_bounds__(kReorderThreads) page_reorder_kernel(const Reo
       if (w < a.W && j < len_s[g * a.W + w]) e[w] = ld_act(a.tables + (int64_t)(g * a.W + w) * a.max_blocks + j);
     }
   };
-  const int step = gridDim.x * kReorderThreads;
-  for (int i = blockIdx.x * kReorderThreads + tid; i < items; i += step) {
+  const int step = gridDim.x * kReorderThreads, i0 = blockIdx.x * kReorderThreads + tid;
+  int kept[WM <= 8 ? WM : 1];  // the thread's first column (registers that the larger kernel has not got)
+  uint32_t same = 0;           // bit k: the k-th column stays as it is
+  for (int i = i0, k = 0; i < items; i += step, ++k) {
     const int g = i / used, j = i - g * used;
     int e[WM], net = 0;
     entries(g, j, e);
+    if constexpr (WM <= 8) {
+      if (k == 0) {
+#pragma unroll
+        for (int w = 0; w < WM; ++w) kept[w] = e[w];
+      }
+    }
     bool one = true;
 #pragma unroll
     for (int w = 0; w < WM; ++w)
-      if (w < a.W) {
-        one &= e[w] == e[0];
-        net += change(g * a.W + w, j);
-      }
+      if (w < a.W) one &= e[w] == e[0];
+    if (one && j < whole_s[g]) {  // the prompt's pages: shared by the parents, shared by the children
+      if (k < 32) same |= 1u << k;
+      continue;
+    }
+#pragma unroll
+    for (int w = 0; w < WM; ++w)
+      if (w < a.W) net += change(g * a.W + w, j);
     if (one) {
       if (net != 0 && (unsigned)e[0] < (unsigned)a.num_blocks) atomicAdd(a.refs + e[0], net);
       continue;
@@ -153,10 +168,16 @@ __global__ void __launch_bounds__(kReorderThreads) page_reorder_kernel(const Reo
       }
   }
   cluster_barrier();
-  for (int i = blockIdx.x * kReorderThreads + tid; i < items; i += step) {
+  for (int i = i0, k = 0; i < items; i += step, ++k) {
+    if (k < 32 && (same >> k & 1)) continue;
     const int g = i / used, j = i - g * used;
     int e[WM], refs[WM];
-    entries(g, j, e);
+    if (WM <= 8 && k == 0) {
+#pragma unroll
+      for (int w = 0; w < WM; ++w) e[w] = kept[WM <= 8 ? w : 0];
+    } else {
+      entries(g, j, e);
+    }
 #pragma unroll
     for (int w = 0; w < WM; ++w)
       refs[w] = w < a.W && (unsigned)e[w] < (unsigned)a.num_blocks && change(g * a.W + w, j) < 0 ? ld_act(a.refs + e[w]) : 1;
@@ -185,17 +206,29 @@ __global__ void __launch_bounds__(kReorderThreads) page_reorder_kernel(const Reo
   const int run = (a.num_blocks + kReorderThreads - 1) / kReorderThreads, lo = min(tid * run, a.num_blocks),
             hi = min(lo + run, a.num_blocks);
   int n = 0;
-#pragma unroll 8
-  for (int i = lo; i < hi; ++i) n += ld_act(a.refs + i) == kGone;
+  uint32_t which = 0;  // of the first 32 (runs are seldom longer)
+  constexpr int AT_ONCE = 8;
+  for (int i = lo; i < hi; i += AT_ONCE) {
+    int refs[AT_ONCE];
+#pragma unroll
+    for (int k = 0; k < AT_ONCE; ++k) refs[k] = i + k < hi ? ld_act(a.refs + i + k) : 0;
+#pragma unroll
+    for (int k = 0; k < AT_ONCE; ++k)
+      if (refs[k] == kGone) {
+        ++n;
+        if (i + k - lo < 32) which |= 1u << (i + k - lo);
+      }
+  }
   int freed;
   int at = top + block_scan(n, tmp, &freed);
-  if (n > 0)
-    for (int i = lo; i < hi; ++i) {
-      if (ld_act(a.refs + i) != kGone) continue;
-      __stcg(a.refs + i, 0);
-      if (at < a.num_blocks) __stcg(a.free_list + at, i);
-      ++at;
-    }
+  auto push = [&](int i) {
+    __stcg(a.refs + i, 0);
+    if (at < a.num_blocks) __stcg(a.free_list + at, i);
+    ++at;
+  };
+  for (; which; which &= which - 1) push(lo + __ffs(which) - 1);
+  for (int i = lo + 32; i < hi; ++i)
+    if (ld_act(a.refs + i) == kGone) push(i);
   // fresh pages, popped in row order
   const int avail = min(top + freed, a.num_blocks);
   const int b = tid, p = parent;
