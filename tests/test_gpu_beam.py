@@ -61,6 +61,12 @@ def test_select_matches(cuda, G, W, V):
     select(x, s, n, f, 0, -0.5)
 
 
+@pytest.mark.parametrize("G,W,V", [(1, 2, 3000001), (2, 31, 70000), (60, 17, 9000)])
+def test_select_large(cuda, G, W, V):
+    x, s, n, f = inputs(G * 1000 + W, G, W, V)
+    select(x, s, n, f, V // 2, 0.7)
+
+
 def test_select_first_step_and_dead_beams(cuda):
     x, s, n, f = inputs(1, 3, 6, 5000)
     s[:] = float("-inf")
@@ -275,6 +281,17 @@ def test_reorder_matches(cuda, kind, G, W, bs, lo, hi):
     for step in range(4):
         parents = rng.integers(0, W, (G, W)) if step else np.tile(np.arange(W), (G, 1))
         held = reorder(c, pm, held, parents)
+
+
+@pytest.mark.parametrize("G,W,bs,lo,hi,free", [
+    (3, 9, 16, 1, 120, 40), (2, 16, 4, 30, 90, 90), (32, 32, 16, 1, 70, 2100), (5, 32, 8, 200, 900, 400),  # many beams
+    (4, 3, 4, 100, 400, 40000), (20, 8, 1, 200, 700, 33000),  # pools of which a thread looks through many blocks
+    (1024, 1, 1, 500, 560, 8)])                               # more columns than fit a thread's marks
+def test_reorder_wide_and_large(cuda, G, W, bs, lo, hi, free):
+    c, pm, held = pool(G + W + bs, G, W, bs, lo, hi, free, layers=1, hkv=1)
+    rng = np.random.default_rng(G)
+    for step in range(2):
+        held = reorder(c, pm, held, rng.integers(-1 if step else 0, W, (G, W)))
 
 
 def test_reorder_all_children_of_one_and_back(cuda):
