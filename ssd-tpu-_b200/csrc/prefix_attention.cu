@@ -289,27 +289,35 @@ __global__ void __launch_bounds__(kChunkC) prefix_attention_cc_kernel(const Pref
 #pragma unroll
       for (int x = 0; x < 4; ++x) o[r][x] *= fac[r];
     const int n = min(kChunkC, hi - c0);
-#pragma unroll 4
-    for (int j = pg; j < n; j += PG) {
-      const int64_t vo = v_s[j];
-      if (vo < 0) continue;
-      float v[4];
-      load4(pages + vo + 4 * dg, v);
-      const float4 pa = p_s[j][0], pb = p_s[j][1];
-      const float pr[8] = {pa.x, pa.y, pa.z, pa.w, pb.x, pb.y, pb.z, pb.w};
-      if (fabsf(v[0]) + fabsf(v[1]) + fabsf(v[2]) + fabsf(v[3]) <= FLT_MAX) {
+    constexpr int AT_ONCE = 4;  // V rows on their way
+#pragma unroll 1
+    for (int j0 = pg; j0 < n; j0 += AT_ONCE * PG) {
+      float v[AT_ONCE][4];
 #pragma unroll
-        for (int r = 0; r < kRowsC; ++r)
+      for (int k = 0; k < AT_ONCE; ++k) {
+        const int64_t vo = j0 + k * PG < n ? v_s[j0 + k * PG] : -1;
+        v[k][0] = v[k][1] = v[k][2] = v[k][3] = 0.f;
+        if (vo >= 0) load4(pages + vo + 4 * dg, v[k]);
+      }
 #pragma unroll
-          for (int x = 0; x < 4; ++x) o[r][x] = fmaf(pr[r], v[x], o[r][x]);
-      } else {  // an infinity or NaN (or a sum past fp32) reaches the rows that see the position, no others
-        const uint32_t in = see_s[j];
+      for (int k = 0; k < AT_ONCE; ++k) {
+        const int j = min(j0 + k * PG, kChunkC - 1);  // (past n: zeros)
+        const float4 pa = p_s[j][0], pb = p_s[j][1];
+        const float pr[8] = {pa.x, pa.y, pa.z, pa.w, pb.x, pb.y, pb.z, pb.w};
+        if (fabsf(v[k][0]) + fabsf(v[k][1]) + fabsf(v[k][2]) + fabsf(v[k][3]) <= FLT_MAX) {
 #pragma unroll
-        for (int r = 0; r < kRowsC; ++r)
-          if (in >> r & 1) {
+          for (int r = 0; r < kRowsC; ++r)
 #pragma unroll
-            for (int x = 0; x < 4; ++x) o[r][x] = fmaf(pr[r], v[x], o[r][x]);
-          }
+            for (int x = 0; x < 4; ++x) o[r][x] = fmaf(pr[r], v[k][x], o[r][x]);
+        } else {  // an infinity or NaN (or a sum past fp32) reaches the rows that see the position, no others
+          const uint32_t in = see_s[j];
+#pragma unroll
+          for (int r = 0; r < kRowsC; ++r)
+            if (in >> r & 1) {
+#pragma unroll
+              for (int x = 0; x < 4; ++x) o[r][x] = fmaf(pr[r], v[k][x], o[r][x]);
+            }
+        }
       }
     }
   }
