@@ -126,8 +126,8 @@ __device__ __forceinline__ RowAt row_at(const PrefixAttn& a, const RowTile& tl, 
   w.at = -1;
   if (tl.group >= 0 && r < rows && w.seq < tl.nseq && in < a.R) {
     w.at = (((int64_t)w.b * a.T + w.t) * a.hq + head * a.G + (in - w.t * a.G)) * D;
-    const int ql = ql_s ? ql_s[w.b] : new_tokens(a, w.b);
-    if (w.t < ql) w.pos = max((seq_s ? seq_s[w.b] : ld_act(a.seq_lens + w.b)) - ql + w.t, -1);
+    const int seq = seq_s ? seq_s[w.b] : ld_act(a.seq_lens + w.b), ql = ql_s ? ql_s[w.b] : new_tokens(a, w.b);
+    if (w.t < ql) w.pos = max(seq - ql + w.t, -1);
   }
   return w;
 }
@@ -174,15 +174,17 @@ __global__ void __launch_bounds__(kChunkC) prefix_attention_cc_kernel(const Pref
   const RowTile tl = find_tile(a, tile);
   if (tl.group < 0) return;
   const int P = prefix_of(a, tl.group);
-  if (tid < kRowsC) {
-    row_s[tid] = row_at<D>(a, tl, head, tid, kRowsC);
-    run[tid] = -INFINITY;
-    sum[tid] = 0.f;
+  if (warp == 1 && lane < kRowsC) {
+    row_s[lane] = row_at<D>(a, tl, head, lane, kRowsC);
+    run[lane] = -INFINITY;
+    sum[lane] = 0.f;
   }
   if (warp == 0) {
     int tail = 0;
-    if (lane < tl.nseq && new_tokens(a, tl.seq0 + lane) > 0)
-      tail = max(min(ld_act(a.seq_lens + tl.seq0 + lane), a.cap) - P, 0);
+    if (lane < tl.nseq) {
+      const int seq = ld_act(a.seq_lens + tl.seq0 + lane), ql = new_tokens(a, tl.seq0 + lane);
+      if (ql > 0) tail = max(min(seq, a.cap) - P, 0);
+    }
     int incl = tail;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
