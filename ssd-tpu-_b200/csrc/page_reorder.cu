@@ -12,8 +12,8 @@
 //                   popped in row order, so that the free list does not depend on which thread came first.
 //   row copy kernel the first rows of a page in all planes, a CTA a piece of one plane of one pair.
 // Bound by latency: for four beams a chain of eight or so trips to L2 with barriers between them (4.5 us), then the copies
-// (28 layers, 16 heads of 256: 22 MB in 9 us); 256 rows with 200 to 4000 tokens 25 us, 16 of them scattered counts and the last CTA's
-// walk over the free list, 9 the copies (13 MB each way).
+// (28 layers, 16 heads of 256: 22 MB in 9 us); 256 rows with 200 to 4000 tokens 22 us, 13 of them the tables, scattered counts
+// and one CTA's walk over all of them, 9 the copies (13 MB each way).
 #include <algorithm>
 
 #include "kv8.cuh"
@@ -24,11 +24,11 @@ namespace {
 constexpr int kMaxReorder = 1024;   // rows
 constexpr int kMaxBeams = 32;       // of a request
 constexpr int kReorderThreads = 1024;
-// 16 CTAs: 32 requests of 8 beams with 200 to 4000 tokens 25.6 us, 8 CTAs 28.7, the copies included: most of it is
+// 16 CTAs: 32 requests of 8 beams with 200 to 4000 tokens 21.9 us, 8 CTAs 27.1, the copies included: most of it is
 // scattered reads and atomics of the counts, which each SM takes one after another.
 constexpr int kCluster = 16;
-// Columns of all requests that one CTA takes alone (a cluster for the toy pair's 4 rows 9.4 us instead of 8.4, for four beams of
-// 530 tokens 15.8 instead of 14.8; one CTA for 256 rows 71 instead of 25).
+// Columns of all requests that one CTA takes alone (a cluster for the toy pair's 4 rows 9.5 us instead of 8.7, for four beams of
+// 530 tokens 15.8 instead of 14.8; one CTA for 256 rows 49 instead of 22).
 constexpr int kOneCta = 4096;
 constexpr int kGone = 1 << 30;      // in a reference count's place: nobody refers to the block any more
 
