@@ -138,7 +138,7 @@ __device__ __forceinline__ RowAt row_at(const PrefixAttn& a, const RowTile& tl, 
 // memory), the rows' maxima and sums are taken over the CTA, and for P V a thread holds 4 dims of all rows over
 // every PG-th position.  Bound by its FMAs on long contexts, by the chain of reads (lengths, table, page) and barriers of one
 // chunk on short ones: two groups of 3 and 4 fp32 rows with at most 120 positions take 9.0 us, 8
-// rows of 8000 positions and 4 KV heads of 256 51 us (131 MB, 2.6 TB/s).
+// rows of 8000 positions and 4 KV heads of 256 51 us (66 MB, which two row tiles read).
 constexpr int kRowsC = 8, kChunkC = 256, kWarpsC = kChunkC / 32;
 constexpr int kMaxSplitC = 32;
 
