@@ -129,3 +129,8 @@ def test_oracle_attention_equals_plain_attention():
         k, v = (pages[x, tables[b]].reshape(12, 8)[:n] for x in (0, 1))
         w = np.exp(q[b, 0] @ k.T * 0.5)
         assert np.allclose(out[b, 0], w @ v / w.sum(1, keepdims=True))
+
+
+def test_polls_below_the_default_mark_are_refused():
+    assert lib().ssd_shared_prefix_attention_set_polls(-2) == INVALID
+    assert lib().ssd_shared_prefix_attention_set_polls(-1) == OK
