@@ -45,7 +45,7 @@ struct PrefixAttn {
   int nsplit;            // parts of a tile's list (CUDA-core kernel)
   float* ws_o;           // [part][row][D] unnormalised sums
   float2* ws_ml;         // [part][row] what they are relative to, sum of weights
-  // [sequence, or tile where a sequence has several][head]: first part, parts (1: the kernel has
+  // [sequence, or slice of one where it takes several tiles][head]: first part, parts (1: the kernel has
   // written the rows itself), step from part to part, the sequence's first row
   int4* parts;
   bool whole;            // lists are not cut
@@ -154,6 +154,25 @@ __device__ __forceinline__ void load4(const KV* p, float* f) {
   }
 }
 
+// The sequences before the first group and behind the last: zeros in a head's rows, and nothing to join.  For a whole warp.
+template <typename KV, int D>
+__device__ __forceinline__ void rows_of_no_group(const PrefixAttn& a, int head) {
+  const int lane = threadIdx.x & 31;
+  int end = 0;
+  for (int g = lane; g <= a.groups; g += 32) end = max(end, clamped(ld_act(a.starts + g), a.B));
+  end = __reduce_max_sync(0xffffffffu, end);
+  const int first = clamped(ld_act(a.starts), a.B), n = first + a.B - end;
+  for (int k = 0; k < n; ++k) {
+    const int b = k < first ? k : end + k - first;
+    for (int t = 0; t < a.T; ++t) {
+      KV* to = reinterpret_cast<KV*>(a.out) + (((int64_t)b * a.T + t) * a.hq + head * a.G) * D;
+      for (int i = lane; i < a.G * D; i += 32) to[i] = from_f<KV>(0.f);
+    }
+    if (a.nsplit > 1)
+      for (int p = lane; p < a.tps; p += 32) a.parts[((int64_t)b * a.tps + p) * a.hkv + head] = make_int4(0, 1, 0, 0);
+  }
+}
+
 template <typename KV, int D>
 __global__ void __launch_bounds__(kChunkC) prefix_attention_cc_kernel(const PrefixAttn a) {
   constexpr int DG = D / 4, PG = kChunkC / DG;
@@ -173,6 +192,7 @@ __global__ void __launch_bounds__(kChunkC) prefix_attention_cc_kernel(const Pref
   pdl_wait();
   pdl_trigger();
   const RowTile tl = find_tile(a, tile);
+  if (tile == 0 && split == 0 && warp == kWarpsC - 1) rows_of_no_group<KV, D>(a, head);
   if (tl.group < 0) return;
   const int P = prefix_of(a, tl.group);
   if (warp == 1 && lane < kRowsC) {
@@ -206,7 +226,7 @@ __global__ void __launch_bounds__(kChunkC) prefix_attention_cc_kernel(const Pref
   const int per = max(1, (chunks + a.nsplit - 1) / a.nsplit);
   const int parts = max(1, (chunks + per - 1) / per);
   if (a.nsplit > 1 && split == 0 && tid < tl.nseq)
-    a.parts[(int64_t)(a.tps > 1 ? tile : tl.seq0 + tid) * a.hkv + head] =
+    a.parts[(int64_t)(a.tps > 1 ? tl.seq0 * a.tps + tl.part : tl.seq0 + tid) * a.hkv + head] =
         make_int4((tile * a.hkv + head) * a.nsplit, parts, 1, a.tps > 1 ? 0 : tid * a.R);
   if (split >= parts) return;
   const int lo = split * per * kChunkC, hi = min(len, lo + per * kChunkC);
@@ -819,7 +839,7 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid
       s = first_s[g];
       e = first_s[g + 1];
     }
-    if (tid >= s && tid < e) {  // (starts that ascend from 0 to B have every sequence in a group)
+    if (tid >= s && tid < e) {
       const int own = pre_s[g], tail = tail_units(a, seq, ql, own), k = tid - s;
       const int spt = spt_s[g], seq0 = s + k / spt * spt;
       const bool lead = seq0 == tid;
@@ -828,6 +848,8 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid
         atomicAdd(&units_s[t], tail + (lead ? prefix_units(own) : 0));
         if (lead) info[t] = make_int2(tid | (a.tps > 1 ? p : min(spt, e - tid)) << 16, g | s << 16);
       }
+    } else if (tid < a.B) {  // before the first group or behind the last: a tile of its own that sees nothing
+      for (int p = 0; p < a.tps; ++p) info[tid * a.tps + p] = make_int2(tid | (a.tps > 1 ? p : 1) << 16, 0);
     }
     const bool team = __syncthreads_and(same) && nm > 1 && nm <= kMaxTeam && nm * 4 <= (int)gridDim.x && !a.whole;
     if (warp == 0) {

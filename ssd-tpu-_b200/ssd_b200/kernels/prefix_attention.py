@@ -32,7 +32,8 @@ def shared_prefix_attention(q: torch.Tensor, cache: KVCacheState, layer: int, bl
                             max_seq_len: int | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """Attention of q [B,T,Hq,D] against each row's pages, shared prefixes read once (``ssd_shared_prefix_attention``).
 
-    ``group_starts`` int32 [groups + 1], ascending from 0 to B: rows group_starts[g] .. group_starts[g+1]-1 are group g.
+    ``group_starts`` int32 [groups + 1], ascending from 0 to B: rows group_starts[g] .. group_starts[g+1]-1 are group g;
+    rows before the first group or behind the last come back as zeros.
     ``prefix_lens`` int32 [groups]: leading positions in which the group's rows agree, read through the table of its
     first row (0: nothing is shared).  The other arguments and the result are those of ``paged_verify_attention``:
     seq_lens [B] counts cached tokens INCLUDING the new ones, new token t of row b sits at position seq_lens[b] -

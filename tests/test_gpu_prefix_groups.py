@@ -1,0 +1,69 @@
+"""GPU: the groups of the shared-prefix attention where they do not cover the batch in order."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+
+from test_gpu_prefix_attention import case, check
+
+pytestmark = pytest.mark.gpu
+
+KINDS = [("bf16", 16), ("bf16", 4), ("f32", 16)]
+
+
+def poison():
+    """What a later allocation finds in its memory: large numbers, as addresses and as sums."""
+    import torch
+
+    for n in (1 << 16, 1 << 20, 1 << 24):
+        torch.full((n,), 0x70707070, dtype=torch.int32, device="cuda")
+
+
+PARTIAL = [  # sizes, prefixes, tails, T, hq, hkv, D
+    ([3, 2, 2], [20, 40, 7], [6, 4, 9, 4, 5, 8, 3], 2, 8, 2, 64),                      # lists that are not cut
+    ([3, 2, 2], [300, 2500, 90], [5, 700, 90, 300, 33, 8, 9], 2, 4, 2, 128),           # joined parts
+    ([2, 1, 2], [100, 1000, 30], [50, 60, 70, 41, 45], 40, 8, 1, 256),                 # several tiles a sequence
+    ([5, 32, 2], [64, 1500, 9], [3 + i % 40 for i in range(39)], 4, 16, 2, 64),        # two tiles a group: a team
+]
+
+
+@pytest.mark.parametrize("dtype,bs", KINDS)
+@pytest.mark.parametrize("shape", PARTIAL, ids=range(len(PARTIAL)))
+def test_rows_of_no_group_are_zeros(cuda, shape, dtype, bs):
+    """Groups that begin above row 0 and end below the last one, and that hold no rows at all."""
+    import torch
+
+    c = case(21, *shape, bs, dtype)
+    sizes = shape[0]
+    starts = c["group_starts"]
+    out = torch.full_like(c["q"], float("nan"))
+    for lo, hi in ((1, 2), (1, 3), (0, 2)):
+        part = {**c, "group_starts": starts[lo:hi + 1].contiguous(), "prefix_lens": c["prefix_lens"][lo:hi].contiguous()}
+        poison()
+        got = check(part, out=out.fill_(float("nan")))
+        first, end = sum(sizes[:lo]), sum(sizes[:hi])
+        assert (got[:first] == 0).all() and (got[end:] == 0).all()
+    none = {**c, "group_starts": torch.tensor([2, 2, 2], dtype=torch.int32, device="cuda"), "prefix_lens": c["prefix_lens"][:2]}
+    poison()
+    assert (check(none, out=out.fill_(float("nan"))) == 0).all()
+
+
+def test_rows_of_no_group_in_a_replayed_graph(cuda):
+    """The groups shrink between replays of one captured call."""
+    import torch
+
+    from ssd_b200.kernels.prefix_attention import shared_prefix_attention
+
+    c = case(22, *PARTIAL[1], 16)
+    g = torch.cuda.CUDAGraph()
+    shared_prefix_attention(**c)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g):
+        o = shared_prefix_attention(**c)
+    c["group_starts"].copy_(torch.tensor([3, 5, 5, 5], dtype=torch.int32))
+    c["prefix_lens"].copy_(torch.tensor([2500, 0, 0], dtype=torch.int32))
+    g.replay()
+    torch.cuda.synchronize()
+    assert np.array_equal(o.double().cpu().numpy(), check(c))
+    assert (o[:3] == 0).all() and (o[5:] == 0).all()
