@@ -262,7 +262,8 @@ int ssd_paged_verify_attention(ssd_stream_t stream, const void* q, const void* p
  * The same over rows that share prefixes (no counterpart in the reference, which decodes one sequence at a
  * time): beams, branches or samples of one prompt after ssd_page_fork, or a batch under one system prompt.
  *   group_starts [num_groups + 1] ascending, 0 .. B: rows group_starts[g] .. group_starts[g+1]-1 form group g;
- *                rows before the first group or behind the last come back as zeros
+ *                rows before the first group or behind the last come back as zeros, and a start below one before
+ *                it counts as that one
  *   prefix_lens  [num_groups] leading positions in which a group's rows agree (0: none; any number, a partial
  *                page that every row holds a copy of included).  They are read through the table of the group's
  *                first row, once for as many of its rows as fit a tile

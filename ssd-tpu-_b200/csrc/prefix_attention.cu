@@ -63,17 +63,25 @@ __device__ __forceinline__ int group_tiles(const PrefixAttn& a, int rows) {
 }
 __device__ __forceinline__ int clamped(int x, int hi) { return min(max(x, 0), hi); }
 
-// Tile `tile` of the batch: groups in order, their tiles in order.  For whole warps.
+// Tile `tile` of the batch: groups in order, their tiles in order.  A start below one before it counts as that one, so that
+// no row is in two groups.  For whole warps.
 __device__ __forceinline__ RowTile find_tile(const PrefixAttn& a, int tile) {
   const int lane = threadIdx.x & 31;
-  int before = 0;
+  int before = 0, high = 0;  // high: the largest start so far
   for (int g0 = 0; g0 < a.groups; g0 += 32) {
     const int g = g0 + lane;
-    int s = 0, e = 0;
+    int s = high, e = high;
     if (g < a.groups) {
       s = clamped(ld_act(a.starts + g), a.B);
       e = clamped(ld_act(a.starts + g + 1), a.B);
     }
+    if (__any_sync(0xffffffffu, e < s || s < high)) {
+      s = max(s, high);
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) s = max(s, __shfl_up_sync(0xffffffffu, s, o));  // (lane 0 .. o-1: its own)
+      e = max(s, e);
+    }
+    high = __shfl_sync(0xffffffffu, e, 31);
     const int n = group_tiles(a, e - s);
     int incl = n;
 #pragma unroll
@@ -820,12 +828,28 @@ prefix_attention_tc_kernel(const __grid_constant__ CUtensorMap map, const __grid
       if (tid == a.groups - 1) first_s[a.groups] = end;
     }
     // tiles of the group, and sequences of each: as even as they come
-    const int of_group = a.tps > 1 ? (end - start) * a.tps : by_spt(a, max(end - start, 0) + a.spt - 1);
-    if (tid < a.groups) {
-      spt_s[tid] = a.tps > 1 || of_group < 1 ? 1 : (end - start + of_group - 1) / of_group;
-      if (tid == 0) slot[3] = of_group;
+    int of_group;
+    auto even = [&] {
+      of_group = a.tps > 1 ? (end - start) * a.tps : by_spt(a, end - start + a.spt - 1);
+      if (tid < a.groups) {
+        spt_s[tid] = a.tps > 1 || of_group < 1 ? 1 : (end - start + of_group - 1) / of_group;
+        if (tid == 0) slot[3] = of_group;
+      }
+    };
+    const bool ascends = start <= end;
+    end = max(start, end);
+    even();
+    if (!__syncthreads_and(ascends)) {  // a start below one before it counts as that one: no row is in two groups
+      if (tid == 0)
+        for (int g = 1; g <= a.groups; ++g) first_s[g] = max(first_s[g], first_s[g - 1]);
+      __syncthreads();
+      if (tid < a.groups) {
+        start = first_s[tid];
+        end = first_s[tid + 1];
+      }
+      even();
+      __syncthreads();
     }
-    __syncthreads();
     const int nm = slot[3];  // tiles of the first group: of all, if there are to be teams
     const bool same = tid >= a.groups || nm == of_group;
     int g = 0, s = 0, e = 0;

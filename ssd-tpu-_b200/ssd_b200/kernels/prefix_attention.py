@@ -33,7 +33,7 @@ def shared_prefix_attention(q: torch.Tensor, cache: KVCacheState, layer: int, bl
     """Attention of q [B,T,Hq,D] against each row's pages, shared prefixes read once (``ssd_shared_prefix_attention``).
 
     ``group_starts`` int32 [groups + 1], ascending from 0 to B: rows group_starts[g] .. group_starts[g+1]-1 are group g;
-    rows before the first group or behind the last come back as zeros.
+    rows before the first group or behind the last come back as zeros, and a start below one before it counts as that one.
     ``prefix_lens`` int32 [groups]: leading positions in which the group's rows agree, read through the table of its
     first row (0: nothing is shared).  The other arguments and the result are those of ``paged_verify_attention``:
     seq_lens [B] counts cached tokens INCLUDING the new ones, new token t of row b sits at position seq_lens[b] -

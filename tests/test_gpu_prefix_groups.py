@@ -67,3 +67,42 @@ def test_rows_of_no_group_in_a_replayed_graph(cuda):
     torch.cuda.synchronize()
     assert np.array_equal(o.double().cpu().numpy(), check(c))
     assert (o[:3] == 0).all() and (o[5:] == 0).all()
+
+
+@pytest.mark.parametrize("dtype,bs", KINDS)
+@pytest.mark.parametrize("starts", [[0, 5, 3, 7], [4, 0, 2, 7], [0, 3, 7, 5], [7, 3, 1, 0], [-4, 2, 1, 90], [0, 2, -1, 7]])
+@pytest.mark.parametrize("shape", PARTIAL[:3], ids=range(3))
+def test_starts_that_descend_count_as_the_largest_before(cuda, shape, starts, dtype, bs):
+    """No row is in two groups, whatever the starts say: the same bits as with ascending ones."""
+    import torch
+
+    from ssd_b200.kernels.prefix_attention import shared_prefix_attention
+
+    c = case(23, *shape, bs, dtype)
+    B = c["q"].shape[0]
+    c["prefix_lens"][:] = torch.tensor([3, 0, 5], dtype=torch.int32)
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    upright = np.maximum.accumulate(np.clip(starts, 0, B)).tolist()
+    poison()
+    got = shared_prefix_attention(**{**c, "group_starts": i32(starts)})
+    assert torch.equal(got, shared_prefix_attention(**{**c, "group_starts": i32(upright)}))
+    check({**c, "group_starts": i32(upright)})
+
+
+def test_many_starts_that_descend(cuda):
+    """More groups than a warp takes at once, with steps back inside and between its batches."""
+    import torch
+
+    from ssd_b200.kernels.prefix_attention import shared_prefix_attention
+
+    rng = np.random.default_rng(24)
+    for dtype, bs in KINDS:
+        c = case(25, [1] * 90, [0] * 90, [1 + i % 50 for i in range(90)], 1, 4, 2, 64, bs, dtype)
+        for _ in range(4):
+            starts = np.sort(rng.integers(0, 91, 91))
+            starts[rng.integers(0, 91, 12)] = rng.integers(-5, 99, 12)
+            upright = np.maximum.accumulate(np.clip(starts, 0, 90))
+            i32 = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+            got = shared_prefix_attention(**{**c, "group_starts": i32(starts)})
+            assert torch.equal(got, shared_prefix_attention(**{**c, "group_starts": i32(upright)}))
+            check({**c, "group_starts": i32(upright)})
