@@ -30,6 +30,7 @@ constexpr int kCluster = 16;
 // Columns of all requests that one CTA takes alone (a cluster for the toy pair's 4 rows 9.5 us instead of 8.7, for four beams of
 // 530 tokens 15.8 instead of 14.8; one CTA for 256 rows 49 instead of 22).
 constexpr int kOneCta = 4096;
+constexpr int kMaxColumns = 1 << 30;  // of all requests: counted in 32 bits, a step of all threads behind the last included
 constexpr int kGone = 1 << 30;      // in a reference count's place: nobody refers to the block any more
 
 struct Reorder {
@@ -346,7 +347,8 @@ extern "C" int ssd_page_reorder(ssd_stream_t stream, int32_t* block_tables, int3
   if (!block_tables || !table_lens || !free_list || !free_top || !ref_counts || !parents || !num_tokens || !copy_src ||
       !copy_dst || !copy_rows)
     return SSD_ERR_INVALID;
-  if (W > kMaxBeams || (int64_t)G * W > kMaxReorder || num_blocks >= kGone) return SSD_ERR_UNSUPPORTED;
+  if (W > kMaxBeams || (int64_t)G * W > kMaxReorder || num_blocks >= kGone || (int64_t)G * max_blocks > kMaxColumns)
+    return SSD_ERR_UNSUPPORTED;
   const Reorder a{block_tables, table_lens, max_blocks, free_list, free_top, ref_counts, num_blocks, parents, num_tokens,
                   G, W, block_size, ok, copy_src, copy_dst, copy_rows};
   cudaStream_t st = (cudaStream_t)stream;

@@ -16,3 +16,16 @@ def test_attention_workspace_of_very_long_contexts():
     assert size(8, 1 << 28) == 2 * per_tile + 256     # 7 sequences a tile
     assert size(8, 1 << 29) == 3 * per_tile + 256     # 3
     assert size(8, 1 << 30) == 8 * per_tile + 256     # 1
+
+
+def test_reorder_refuses_more_columns_than_it_counts():
+    """G * max_blocks columns are counted in 32 bits; refused before any address is looked at."""
+    from ssd_b200 import _lib
+
+    p = 1 << 20  # an address that no refused call touches
+
+    def call(g, max_blocks):
+        return _lib.lib().ssd_page_reorder(None, p, p, max_blocks, p, p, p, 64, p, p, 16, None, p, p, p, g, 1)
+
+    for g, cols in ((1024, (1 << 20) + 1), (2, (1 << 29) + 1), (1, (1 << 30) + 1), (3, 0x7fffffff)):
+        assert call(g, cols) == 4
