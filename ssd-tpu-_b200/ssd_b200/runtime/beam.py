@@ -23,16 +23,28 @@ from .page_manager import PageManager
 _CHECK_EVERY = 16  # steps between looks at whether every beam has finished
 
 
+def blocks_per_request(num_beams: int, max_seq_len: int, max_new: int, block_size: int) -> int:
+    """Blocks that one request's beams hold at most, whatever its prompt (prompt + max_new - 1 tokens within max_seq_len).
+
+    The n // block_size whole blocks of a prompt of n tokens are shared by all beams; from the block of the prompt's end on
+    each beam may have its own, at most (max_new + 2 block_size - 3) // block_size of them.
+    """
+    every = -(-max_seq_len // block_size)
+    own = min((max(max_new, 1) + 2 * block_size - 3) // block_size, every)
+    return every - own + num_beams * own
+
+
 class BeamSearchDecoder:
     """Beam search with ``num_beams`` beams for up to ``requests`` prompts at a time.
 
     ``length_penalty``: beams are ranked by score / length ** length_penalty.  ``eos_token_id``: a beam that emits it
-    has finished and keeps its place and score (None: none ever does).
+    has finished and keeps its place and score (None: none ever does).  ``max_new``: the most tokens that ``generate`` will
+    be asked for (None: up to max_seq_len); the cache holds a prompt's blocks once and the beams' own blocks for so many.
     """
 
     def __init__(self, target: GemmaWeights, num_beams: int, requests: int = 1, max_seq_len: int = 1024,
                  block_size: int = 16, comm=None, kv_cache_dtype: str = "auto", length_penalty: float = 0.0,
-                 eos_token_id: int | None = None):
+                 eos_token_id: int | None = None, max_new: int | None = None):
         G, W = self.G, self.W = int(requests), int(num_beams)
         if not 1 <= W <= MAX_BEAMS or G < 1:
             raise ValueError(f"1 to {MAX_BEAMS} beams and at least one request are needed, got {W} and {G}")
@@ -43,9 +55,12 @@ class BeamSearchDecoder:
             raise ValueError(f"eos_token_id {eos_token_id} is outside the vocabulary of {target.shape.vocab}")
         self.dev = dev = target.device
         self.max_seq_len = int(max_seq_len)
+        self.max_new = self.max_seq_len if max_new is None else int(max_new)
+        if not 0 <= self.max_new <= self.max_seq_len:
+            raise ValueError(f"max_new must be 0 to {self.max_seq_len}, got {max_new}")
         self.length_penalty, self.eos = float(length_penalty), eos_token_id
         blocks = (self.max_seq_len + block_size - 1) // block_size + 1
-        num_blocks = B * blocks + 2
+        num_blocks = G * blocks_per_request(W, self.max_seq_len, self.max_new, block_size) + 2
         self.cache = allocate_kv_cache(target, num_blocks, block_size, kv_cache_dtype)
         self.pm = PageManager(block_size, num_blocks, max_seqs=B, max_blocks_per_seq=blocks, device=dev)
         self.runner = GemmaRunner(target, B, 64, self.max_seq_len, comm=comm)
@@ -79,6 +94,8 @@ class BeamSearchDecoder:
             raise ValueError("empty prompt")
         if max_new < 1:
             return [[([], 0.0)] for _ in prompts]
+        if max_new > self.max_new:
+            raise ValueError(f"{max_new} new tokens were asked for, the decoder's cache was made for {self.max_new}")
         if max(len(p) for p in prompts) + max_new - 1 > self.max_seq_len:
             raise ValueError("prompt + max_new exceeds max_seq_len")
         self.pm.free_rows(0, B)

@@ -109,7 +109,7 @@ class RankState:
         # one decoder for every batch of the call: its cache and scratch are the same for all
         dec = BeamSearchDecoder(self.target_w, num_beams, requests, max_seq_len=max_len, block_size=block_size,
                                 comm=self.comm, kv_cache_dtype=self.kv_cache_dtype, length_penalty=length_penalty,
-                                eos_token_id=eos)
+                                eos_token_id=eos, max_new=max(max_new, 0))
         out = []
         for i in range(0, len(prompts), requests):
             out += dec.generate(prompts[i:i + requests], max_new)

@@ -29,3 +29,64 @@ def test_reorder_refuses_more_columns_than_it_counts():
 
     for g, cols in ((1024, (1 << 20) + 1), (2, (1 << 29) + 1), (1, (1 << 30) + 1), (3, 0x7fffffff)):
         assert call(g, cols) == 4
+
+
+def _peak(num_beams, prompt, max_new, block_size, rng, apart):
+    """Blocks in use at most while beams follow random parents, or (``apart``) each goes on for itself, which shares least:
+    tables as page lists, as ``PageManager`` keeps them."""
+    import numpy as np
+
+    from oracle import beams
+
+    W, pages = num_beams, -(-prompt // block_size)
+    supply = iter(range(pages, 1 << 30))
+    tables = [list(range(pages))] + [[] for _ in range(W - 1)]
+    refs = {b: 1 for b in range(pages)}
+    free, peak, held = [], pages, [prompt] + [0] * (W - 1)
+    for step in range(max_new - 1):
+        # blocks that nobody holds are taken first; new ones only where the list is empty
+        free = free + [next(supply) for _ in range(2 * W)]
+        parents = rng.integers(0, W, (1, W)) if step else np.zeros((1, W), int)
+        if step and (apart or rng.random() < 0.3):
+            parents[:] = rng.permutation(W)
+        tables, refs, free, ok, _ = beams.reorder(tables, [len(t) for t in tables], refs, free, parents, held, block_size)
+        assert all(ok)
+        held = [prompt + step] * W
+        for t in tables:
+            for _ in range(-(-(held[0] + 1) // block_size) - len(t)):
+                b = free.pop()
+                t.append(b)
+                refs[b] = 1
+        held = [h + 1 for h in held]
+        peak = max(peak, len(refs))
+    return peak
+
+
+def test_a_requests_blocks_suffice():
+    """No search holds more blocks than its share of the pool, and the worst prompts hold about as many."""
+    import numpy as np
+
+    from ssd_b200.runtime.beam import blocks_per_request
+
+    rng = np.random.default_rng(0)
+    for W, bs, max_seq_len, max_new in [(4, 16, 64, 20), (3, 1, 12, 5), (1, 4, 30, 9), (8, 4, 40, 40), (2, 16, 50, 1),
+                                        (5, 3, 31, 2), (4, 5, 60, 17)]:
+        most = 0
+        for prompt in range(1, max_seq_len + 1):
+            new = min(max_new, max_seq_len - prompt + 1)
+            most = max(most, _peak(W, prompt, new, bs, rng, True))
+            if prompt % 3 == 0:
+                most = max(most, _peak(W, prompt, new, bs, rng, False),
+                           _peak(W, prompt, int(rng.integers(1, new + 1)), bs, rng, True))
+        bound = blocks_per_request(W, max_seq_len, max_new, bs)
+        assert most <= bound <= most + W + 1, (W, bs, max_seq_len, max_new, most, bound)
+
+
+def test_the_prompts_blocks_are_held_once():
+    from ssd_b200.runtime.beam import blocks_per_request
+
+    # 4 beams of 64 new tokens behind up to 1437 prompt tokens: 4 times 5 blocks, and the prompt's
+    assert blocks_per_request(4, 1500, 64, 16) == 94 - 5 + 4 * 5
+    assert blocks_per_request(4, 1500, 1500, 16) == 4 * 94
+    assert blocks_per_request(1, 1500, 64, 16) == 94
+    assert blocks_per_request(4, 10, 0, 1) == 10 and blocks_per_request(4, 10, 1, 1) == 10
