@@ -34,6 +34,15 @@ def blocks_per_request(num_beams: int, max_seq_len: int, max_new: int, block_siz
     return every - own + num_beams * own
 
 
+def requests_that_fit(shape, elem: int, num_beams: int, requests: int, max_seq_len: int, max_new: int, block_size: int,
+                      free_bytes: int) -> int:
+    """How many of ``requests`` searches fit side by side in ``free_bytes``, one at least (which may be refused its memory
+    then): their blocks of ``elem`` bytes an element, and their logits."""
+    blocks = blocks_per_request(num_beams, max_seq_len, max_new, block_size)
+    each = blocks * block_size * shape.kv_bytes_per_token(elem) + 4 * num_beams * shape.vocab
+    return max(1, min(requests, free_bytes // each))
+
+
 class BeamSearchDecoder:
     """Beam search with ``num_beams`` beams for up to ``requests`` prompts at a time.
 

@@ -199,7 +199,8 @@ class LLMEngine:
         collector.record_step(StepMetrics(target_verify_ms=(time.perf_counter() - t0) * 1000, accepted_tokens=n))
 
     def _run_beams(self, prompts, sampling, on_token, collector) -> tuple[list[list[int]], RunMetrics]:
-        """Beam search: the best beam of each prompt; as many prompts at a time as the rows of a forward take."""
+        """Beam search: the best beam of each prompt; as many prompts at a time as the rows of a forward and the free memory
+        take, at most max(batch_buckets)."""
         W = int(sampling.num_beams)
         if self.config.mode != DecodeMode.AR:
             raise ValueError("num_beams > 1 needs ar mode")
@@ -211,12 +212,16 @@ class LLMEngine:
         requests = min(len(prompts), max_tokens_per_forward(dtype) // W)
         if requests < 1:
             raise ValueError(f"num_beams {W} exceeds one forward ({max_tokens_per_forward(dtype)} rows)")
+        requests = max(1, min(requests, max(self.config.batch_buckets)))
         sched = Scheduler(num_slots=len(prompts))
         seqs = [sched.add_request(p) for p in prompts]
         max_len = self._max_len(max(len(s.prompt_token_ids) for s in seqs), sampling)
         self.ranks.call("begin")
         t0 = time.perf_counter()
         try:
+            # the same number on every rank
+            requests = min(self.ranks.call("beam_requests", W, requests, sampling.max_new_tokens, max_len,
+                                           self.config.block_size))
             out = self.ranks.call("beam_generate", [list(s.prompt_token_ids) for s in seqs], W, requests,
                                   sampling.max_new_tokens, max_len, self.config.block_size,
                                   float(sampling.length_penalty),

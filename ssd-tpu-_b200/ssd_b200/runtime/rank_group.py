@@ -101,6 +101,16 @@ class RankState:
         return GreedyDecoder(self.target_w, max_seq_len=max_len, block_size=block_size, comm=self.comm,
                              kv_cache_dtype=self.kv_cache_dtype).generate(prompt, max_new)
 
+    def beam_requests(self, num_beams: int, requests: int, max_new: int, max_len: int, block_size: int) -> int:
+        """How many of the requests' searches fit side by side in this rank's free memory."""
+        from .beam import requests_that_fit
+
+        free = torch.cuda.mem_get_info(self.dev)[0]
+        free += torch.cuda.memory_reserved(self.dev) - torch.cuda.memory_allocated(self.dev)
+        elem = 1 if self.kv_cache_dtype == "fp8" else self.target_w.dtype.itemsize
+        # a tenth for the forward's scratch, the workspaces and the 8-bit cache's scales
+        return requests_that_fit(self.target_w.shape, elem, num_beams, requests, max_len, max_new, block_size, free * 9 // 10)
+
     def beam_generate(self, prompts: list[list[int]], num_beams: int, requests: int, max_new: int, max_len: int,
                       block_size: int, length_penalty: float, eos: int | None) -> list[list[tuple[list[int], float]]]:
         from .beam import BeamSearchDecoder

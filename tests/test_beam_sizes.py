@@ -90,3 +90,15 @@ def test_the_prompts_blocks_are_held_once():
     assert blocks_per_request(4, 1500, 1500, 16) == 4 * 94
     assert blocks_per_request(1, 1500, 64, 16) == 94
     assert blocks_per_request(4, 10, 0, 1) == 10 and blocks_per_request(4, 10, 1, 1) == 10
+
+
+def test_requests_go_by_the_memory_that_is_there():
+    from ssd_b200.models.gemma import PRESETS
+    from ssd_b200.runtime.beam import blocks_per_request, requests_that_fit
+
+    s = PRESETS["gemma-7b"]
+    fit = lambda free, elem=2: requests_that_fit(s, elem, 4, 64, 1500, 64, 16, free)  # noqa: E731
+    each = blocks_per_request(4, 1500, 64, 16) * 16 * 2 * 2 * 28 * 16 * 256 + 4 * 4 * 256000
+    assert fit(180 << 30) == 64
+    assert fit(10 * each) == 10 and fit(10 * each - 1) == 9 and fit(10 * each, 1) in (19, 20)
+    assert fit(0) == 1 and fit(each // 2) == 1

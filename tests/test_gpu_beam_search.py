@@ -38,3 +38,40 @@ def test_a_search_in_its_own_share_of_blocks(cuda, W, G, bs, max_seq_len, max_ne
     for bad in (-1, max_seq_len + 1):
         with pytest.raises(ValueError):
             BeamSearchDecoder(w, W, G, max_seq_len=max_seq_len, block_size=bs, max_new=bad)
+
+
+def test_the_engine_takes_as_many_requests_as_fit(cuda, monkeypatch):
+    """Bounded by batch_buckets and by the free memory: more prompts go through one after another."""
+    import torch
+
+    from ssd_b200 import LLM, DecodeMode, SamplingParams
+    from ssd_b200.runtime import beam
+
+    llm = LLM.from_mode(DecodeMode.AR)
+    try:
+        seen = []
+        make = beam.BeamSearchDecoder.__init__
+
+        def spy(self, target, num_beams, requests=1, *args, **kw):
+            seen.append(requests)
+            make(self, target, num_beams, requests, *args, **kw)
+
+        monkeypatch.setattr(beam.BeamSearchDecoder, "__init__", spy)
+        prompts = [[1, 2, 3, 4, 5], [9, 8, 7], [5] * 20, [6, 6], [30, 31, 32], [7]]
+        sampling = SamplingParams(max_new_tokens=6, num_beams=4)
+        out, metrics = llm.generate(prompts, sampling)
+        assert seen == [4] and metrics.total_tokens == 36  # 16 rows a forward
+        llm._engine.config.batch_buckets = (1, 3)
+        few, _ = llm.generate(prompts, sampling)
+        assert seen == [4, 3] and [len(t) for t in few] == [6] * 6
+        state = llm._engine.ranks.state
+        shape, max_len = state.target_w.shape, 20 + 6 + 2 * 5 + 16
+        each = beam.blocks_per_request(4, max_len, 6, 16) * 16 * shape.kv_bytes_per_token(4) + 4 * 4 * shape.vocab
+        monkeypatch.setattr(torch.cuda, "memory_reserved", lambda d=None: 0)
+        monkeypatch.setattr(torch.cuda, "memory_allocated", lambda d=None: 0)
+        for free, want in ((each * 10 // 9 * 2 + 100, 2), (each, 1), (0, 1)):
+            monkeypatch.setattr(torch.cuda, "mem_get_info", lambda d=None, f=free: (f, 1 << 37))
+            one, _ = llm.generate(prompts, sampling)
+            assert seen[-1] == want and [len(t) for t in one] == [6] * 6
+    finally:
+        llm.shutdown()
