@@ -27,7 +27,7 @@ device split (connect/mesh_allocator.py:47-61).
 Greedy decoding is the default, as in the reference (whose sd/ssd paths never
 read ``SamplingParams.temperature``, engine.py:235,292); here a temperature > 0
 selects rejection sampling on the batched path.  Outputs are truncated to
-``max_new_tokens``.
+``max_new_tokens``, and end with ``eos_token_id`` where one is given (and ``ignore_eos`` is not set).
 """
 
 from __future__ import annotations
@@ -112,6 +112,9 @@ class LLMEngine:
         collector = MetricsCollector(mode=self.config.mode.value)
         collector.start()
         mode = self.config.mode
+        eos = self._eos(sampling)
+        if eos is not None and not 0 <= eos < self.vocab_size:
+            raise ValueError(f"eos_token_id {eos} is outside the vocabulary of {self.vocab_size}")
         if sampling.num_beams > 1:
             return self._run_beams(prompts, sampling, on_token, collector)
         batched = mode == DecodeMode.SD and (len(prompts) > 1 or sampling.temperature > 0)
@@ -171,10 +174,17 @@ class LLMEngine:
         cap = max_tokens_per_forward(dtype) // (self.config.speculate_k + 1)
         return max(1, min(n, max(self.config.batch_buckets), cap))
 
-    def _emit(self, seq: Sequence, toks: list[int], limit: int, on_token) -> int:
+    @staticmethod
+    def _eos(sampling: SamplingParams) -> int | None:
+        return None if sampling.ignore_eos else sampling.eos_token_id
+
+    def _done(self, seq: Sequence, sampling: SamplingParams) -> bool:
+        return seq.is_finished(self._eos(sampling), sampling.max_new_tokens)
+
+    def _emit(self, seq: Sequence, toks: list[int], sampling: SamplingParams, on_token) -> int:
         n = 0
         for t in toks:
-            if seq.num_completion_tokens >= limit:
+            if self._done(seq, sampling):
                 break
             seq.append_token(t)
             n += 1
@@ -195,7 +205,7 @@ class LLMEngine:
         out = self.ranks.call("ar_generate", list(seq.prompt_token_ids), sampling.max_new_tokens, max_len,
                               self.config.block_size)[0]
         collector.record_first_token()
-        n = self._emit(seq, out, sampling.max_new_tokens, on_token)
+        n = self._emit(seq, out, sampling, on_token)
         collector.record_step(StepMetrics(target_verify_ms=(time.perf_counter() - t0) * 1000, accepted_tokens=n))
 
     def _run_beams(self, prompts, sampling, on_token, collector) -> tuple[list[list[int]], RunMetrics]:
@@ -225,13 +235,13 @@ class LLMEngine:
             out = self.ranks.call("beam_generate", [list(s.prompt_token_ids) for s in seqs], W, requests,
                                   sampling.max_new_tokens, max_len, self.config.block_size,
                                   float(sampling.length_penalty),
-                                  None if sampling.ignore_eos else sampling.eos_token_id)[0]
+                                  self._eos(sampling))[0]
         finally:
             status = self.ranks.call("end")
         if any(status):
             raise RuntimeError(f"a collective or another device-side wait timed out (rank statuses {status})")
         collector.record_first_token()
-        n = sum(self._emit(s, beams[0][0] if beams else [], sampling.max_new_tokens, on_token)
+        n = sum(self._emit(s, beams[0][0] if beams else [], sampling, on_token)
                 for s, beams in zip(seqs, out))
         collector.record_step(StepMetrics(target_verify_ms=(time.perf_counter() - t0) * 1000, accepted_tokens=n,
                                           sequences=len(seqs)))
@@ -241,12 +251,12 @@ class LLMEngine:
         k = self.config.speculate_k
         max_len = self._max_len(len(seq.prompt_token_ids), sampling)
         first = self.ranks.call("sd_start", list(seq.prompt_token_ids), k, max_len, self.config.block_size)[0]
-        self._emit(seq, [first], sampling.max_new_tokens, on_token)
+        self._emit(seq, [first], sampling, on_token)
         collector.record_first_token()
-        while not seq.is_finished(None, sampling.max_new_tokens):
+        while not self._done(seq, sampling):
             t0 = time.perf_counter()
             new, verify_ms, acc = self.ranks.call("sd_step")[0]
-            n = self._emit(seq, new, sampling.max_new_tokens, on_token)
+            n = self._emit(seq, new, sampling, on_token)
             collector.record_step(StepMetrics(target_verify_ms=(time.perf_counter() - t0) * 1000, accepted_tokens=n,
                                               verify_device_ms=verify_ms))
             collector.record_accepts([acc])
@@ -258,19 +268,18 @@ class LLMEngine:
         temp = float(sampling.temperature)
         self.ranks.call("batch_open", sched.num_slots, k, max_len, self.config.block_size, temp,
                         float(sampling.top_p) if temp > 0 else 1.0, self.config.sampler_x, self.config.seed)
-        limit = sampling.max_new_tokens
         first_done = False
         while sched.has_work():
             placed = sched.admit()
             if placed:
                 firsts = self.ranks.call("batch_admit", [(slot, s.prompt_token_ids) for slot, s in placed])[0]
                 for (slot, seq), f in zip(placed, firsts):
-                    self._emit(seq, [f], limit, on_token)
+                    self._emit(seq, [f], sampling, on_token)
                 if not first_done:
                     collector.record_first_token()
                     first_done = True
             for slot, seq in sched.slots():
-                if seq.is_finished(None, limit):
+                if self._done(seq, sampling):
                     sched.retire(slot)
                     if not sched.waiting:
                         self.ranks.call("batch_park", slot)
@@ -279,7 +288,7 @@ class LLMEngine:
             t0 = time.perf_counter()
             new, verify_ms, accepts = self.ranks.call("batch_step")[0]
             active = sched.slots()
-            emitted = sum(self._emit(seq, new[slot], limit, on_token) for slot, seq in active)
+            emitted = sum(self._emit(seq, new[slot], sampling, on_token) for slot, seq in active)
             collector.record_step(StepMetrics(target_verify_ms=(time.perf_counter() - t0) * 1000,
                                               accepted_tokens=emitted, verify_device_ms=verify_ms,
                                               sequences=len(active)))
@@ -289,11 +298,11 @@ class LLMEngine:
         assert self.draft_worker is not None
         recovery = self.ranks.call("target_prefill", list(seq.prompt_token_ids))[0]
         seq.recovery_token = recovery
-        self._emit(seq, [recovery], sampling.max_new_tokens, on_token)
+        self._emit(seq, [recovery], sampling, on_token)
         collector.record_first_token()
         acc = 0
         commit: list[int] | None = None
-        while not seq.is_finished(None, sampling.max_new_tokens):
+        while not self._done(seq, sampling):
             t0 = time.perf_counter()
             key = torch.tensor([[seq.seq_id, acc, recovery]], dtype=torch.int32)
             self.draft_worker.submit(DraftRequest(DraftCommand.SERVE, key, torch.tensor([seq.num_tokens]),
@@ -309,7 +318,7 @@ class LLMEngine:
                 raise RuntimeError(f"tensor-parallel ranks disagree on the verify outcome: {outcomes}")
             acc, recovery, verify_ms = outcomes[0]
             commit = spec[:acc] + [recovery]
-            n = self._emit(seq, commit, sampling.max_new_tokens, on_token)
+            n = self._emit(seq, commit, sampling, on_token)
             collector.record_step(StepMetrics(target_verify_ms=(time.perf_counter() - t0) * 1000,
                                               draft_step_ms=(t1 - t0) * 1000, cache_hit=bool(resp.cache_hit[0]),
                                               accepted_tokens=n, verify_device_ms=verify_ms))

@@ -75,3 +75,27 @@ def test_the_engine_takes_as_many_requests_as_fit(cuda, monkeypatch):
             assert seen[-1] == want and [len(t) for t in one] == [6] * 6
     finally:
         llm.shutdown()
+
+
+@pytest.mark.parametrize("mode,prompts,temperature", [("ar", 2, 0.0), ("sd", 1, 0.0), ("sd", 3, 0.0), ("sd", 2, 0.8), ("ssd", 1, 0.0)])
+def test_eos_ends_an_output_in_every_mode(cuda, mode, prompts, temperature):
+    from ssd_b200 import LLM, DecodeMode, SamplingParams
+
+    llm = LLM.from_mode(DecodeMode(mode))
+    try:
+        given = [[1, 2, 3, 4, 5], [9, 8, 7], [5] * 20][:prompts]
+        make = lambda **kw: SamplingParams(max_new_tokens=12, temperature=temperature, **kw)  # noqa: E731
+        full, _ = llm.generate(given, make())
+        assert [len(t) for t in full] == [12] * prompts
+        for stop in {full[0][0], full[0][5], full[-1][11]}:
+            got, _ = llm.generate(given, make(eos_token_id=stop))
+            if temperature == 0:
+                assert got == [t[:t.index(stop) + 1] if stop in t else t for t in full]
+            for t in got:
+                assert stop not in t[:-1] and (len(t) == 12 or t[-1] == stop)
+            assert [len(t) for t in llm.generate(given, make(eos_token_id=stop, ignore_eos=True))[0]] == [12] * prompts
+        for bad in (dict(eos_token_id=llm._engine.vocab_size), dict(eos_token_id=-1)):
+            with pytest.raises(ValueError):
+                llm.generate(given, make(**bad))
+    finally:
+        llm.shutdown()
