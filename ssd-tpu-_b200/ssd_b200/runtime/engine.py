@@ -112,6 +112,8 @@ class LLMEngine:
         collector = MetricsCollector(mode=self.config.mode.value)
         collector.start()
         mode = self.config.mode
+        if sampling.num_beams < 1:
+            raise ValueError(f"num_beams must be at least 1, got {sampling.num_beams}")
         eos = self._eos(sampling)
         if eos is not None and not 0 <= eos < self.vocab_size:
             raise ValueError(f"eos_token_id {eos} is outside the vocabulary of {self.vocab_size}")

@@ -99,3 +99,16 @@ def test_eos_ends_an_output_in_every_mode(cuda, mode, prompts, temperature):
                 llm.generate(given, make(**bad))
     finally:
         llm.shutdown()
+
+
+@pytest.mark.parametrize("mode", ["ar", "sd", "ssd"])
+def test_fewer_than_one_beam_is_refused(cuda, mode):
+    from ssd_b200 import LLM, DecodeMode, SamplingParams
+
+    llm = LLM.from_mode(DecodeMode(mode))
+    try:
+        for n in (0, -3):
+            with pytest.raises(ValueError):
+                llm.generate([[1, 2]], SamplingParams(max_new_tokens=4, num_beams=n))
+    finally:
+        llm.shutdown()
