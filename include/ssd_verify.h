@@ -450,6 +450,8 @@ int ssd_beam_select(ssd_stream_t stream, const float* logits, int64_t ld, const 
  * belongs to one row.  Blocks that no row refers to any more are pushed on the free list before, in ascending
  * order.  A row whose parent is out of range (-1) is emptied; one that cannot get its block is emptied with
  * ok = 0 (ok [G*W] may be NULL).  W <= 32, G*W <= 1024, G * max_blocks <= 2^30 (else SSD_ERR_UNSUPPORTED).
+ * Where G * max_blocks is above 4096 the kernel is one cluster of 16 CTAs: on a device, or a part of one, that has no
+ * room for that, SSD_ERR_LAUNCH, and nothing has changed.
  */
 int ssd_page_reorder(ssd_stream_t stream, int32_t* block_tables, int32_t* table_lens, int max_blocks,
                      int32_t* free_list, int32_t* free_top, int32_t* ref_counts, int num_blocks,

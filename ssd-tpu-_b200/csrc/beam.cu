@@ -9,11 +9,17 @@
 //   merge kernel  a CTA a request: the slices' statistics become lse_w, the slices' candidates are ranked in 64
 //                 bits, the W best are written in order.
 // The W largest of a CTA: the maxima of 32 groups of threads, the W-th largest of these as a bound that at least W values
-// reach (and seldom more than a few times W), those values to shared memory, and each one's rank by counting the
-// larger ones.  Where more values reach the bound than fit (long runs of equal logits), W rounds of a maximum over the
-// CTA.  Order never depends on which thread comes first: equal values rank by their index.
+// reach (and of a slice's logits seldom more than a few times W), those values to shared memory, and each one's rank by
+// counting the larger ones.  Where more values reach the bound than fit, W rounds of a maximum over the CTA.  Order never
+// depends on which thread comes first: equal values rank by their index.
+// More than fit are long runs of equal logits in the rows kernel.  In the merge a beam has 512 / W of the threads (W rounded up
+// to a power of two), so the bound is as low as the worst beam's best candidate, and there is none where fewer than W
+// groups hold a candidate, as at a first step, where one beam is live: all its slices * W candidates are taken then.  From 9
+// beams over 256000 tokens on these do not fit, and the rounds, in which 16 or 32 threads read and rank every candidate
+// again, make up most of the call: one request's first step takes 12.6 us with 8 beams, 110 with 16, 705 with 32, a
+// step in mid-flight (scores within 5 of each other) 9.2, 21 and 950 us.
 // Bound by DRAM for many rows: 256 rows of 256000 logits take 51 us, the rows kernel 46 of them (262 MB, 5.7 TB/s), 32
-// rows 11.6 us; few rows by the two kernels' chains of reads and barriers: one row of 256000 logits 6.6 us.
+// rows 11.7 us; few rows by the two kernels' chains of reads and barriers: one row of 256000 logits 7 us.
 #include <algorithm>
 
 #include "tcgen05.cuh"

@@ -144,9 +144,11 @@ __device__ __forceinline__ RowAt row_at(const PrefixAttn& a, const RowTile& tl, 
 // fp32 caches, and bf16 ones whose pages are no whole runs of 16 rows.  A CTA takes 8 query rows of one KV head and a
 // part of their list, 256 positions at a time: a thread scores one position against all rows (q broadcast from shared
 // memory), the rows' maxima and sums are taken over the CTA, and for P V a thread holds 4 dims of all rows over
-// every PG-th position.  Bound by its FMAs on long contexts, by the chain of reads (lengths, table, page) and barriers of one
-// chunk on short ones: two groups of 3 and 4 fp32 rows with at most 120 positions take 9.0 us, 8
-// rows of 8000 positions and 4 KV heads of 256 51 us (66 MB, which two row tiles read).
+// every PG-th position.  Bound on long contexts by waiting for its loads: 8 sequences of 8000 fp32 positions and 8 query heads
+// over 4 KV heads of 256 take 53.5 us (66 MB, which two row tiles read: L2 sends 219 MB, since a thread's 16 bytes of its own K
+// row leave half a sector for later; FMAs 18 % busy), in bf16 over pages of 4 rows 49.2 us.  Bound by the chain of reads
+// (lengths, table, page) and barriers of one chunk on short ones: two groups of 3 and 4 fp32 rows with at most 120 positions
+// take 9.1 us.
 constexpr int kRowsC = 8, kChunkC = 256, kWarpsC = kChunkC / 32;
 constexpr int kMaxSplitC = 32;
 // Positions of a tile's list: counted in 32 bits, the chunks that the last part may have behind the list's end included.  The
@@ -399,7 +401,7 @@ __global__ void __launch_bounds__(kChunkC) prefix_attention_cc_kernel(const Pref
 // not finite although its sum of weights is, and the row is worked out again by itself, from the pages.
 // Bound by DRAM on long contexts: 32 rows of 7 tokens under a prompt of 8000, 16 KV heads of 256, take 79 us for 334 MB (4.2 TB/s
 // over the call; 5.9 TB/s in the loop, before it 3 us of plan, behind it 4 of partial sums and 8 of joining them).  Eight prompts
-// of 1000 to 8190 positions with 4 to 8 rows of one KV head take 25 us for 41 MB: 8 tiles a CTA, fewer than its start, end and
+// of 1000 to 8190 positions with 4 to 8 rows of one KV head take 24 to 29 us for 41 MB: 8 tiles a CTA, fewer than its start, end and
 // join are worth.
 // All waits are bounded, and a warp's lanes give up together.  A CTA that gives up raises `gave_up`, lets its copies and
 // products end, frees its TMEM and leaves NaN in the rows that it has not finished.  (A wait for a phase of a barrier is
@@ -420,7 +422,7 @@ constexpr int kMinUnits = 8;           // of a run, so that short batches are no
 // 48: 28.2, 21.1 and 21.2 us for 15 rows under a prompt of 2000, 87.8, 83.6 and 79.2 for 32 of 7 tokens under one of 8000.
 constexpr int kStart = 48;
 // Lists of at most so many units are not cut: the results go straight out and nothing is joined (four beams of 530
-// positions 11.8 us, cut and joined 13.4).
+// positions 11.8 us, cut and joined 13.4, both before the groups' order was looked at, which costs 0.1).
 constexpr int kWhole = 64;
 // CTAs that walk a group's lists side by side, so that a prefix comes from DRAM once however many tiles read it (two
 // tiles under the prompt of 8000: 79.2 us, each by itself 93.1).

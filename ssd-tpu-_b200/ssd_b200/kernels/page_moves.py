@@ -135,8 +135,8 @@ def reorder_pages(cache, tables: torch.Tensor, lens: torch.Tensor, ref_counts: t
 
     ``tables`` [G*W, max_blocks] with ``lens``, ``ref_counts``, ``free_list`` and ``free_top`` are the arrays of
     ``PageManager``; ``parents`` int32 [G, W] (-1: the row is emptied), ``num_tokens`` int32 [G*W] the tokens that each
-    old row holds.  Whole blocks are shared, a partial last block stays with the lowest of its parent's children and is
-    copied for the others, in ``cache`` (one cache, or a sequence of caches that share the pool's block ids); blocks
+    old row holds.  Whole blocks are shared, a partial last block (which has to be its row's alone) stays with the lowest of
+    its parent's children and is copied for the others, in ``cache`` (one cache, or a sequence of caches that share the pool's block ids); blocks
     that no row holds any more return to the free list.  Returns ok uint8 [G*W]: 0 where no block was left for a
     copy and the row is empty.  Nothing synchronises.  ``ssd_page_reorder`` and ``ssd_page_copy_rows``.
     """
