@@ -269,11 +269,11 @@ int ssd_paged_verify_attention(ssd_stream_t stream, const void* q, const void* p
  *                first row, once for as many of its rows as fit a tile
  * Rows, positions, lengths and zero rows as in ssd_paged_verify_attention, whatever the groups: a row sees the
  * positions up to its own.  What it does not see does not reach it, infinities and NaN included; positions
- * whose table entry is no block hold nothing.  Statistics and sums in fp32.  A row's bits depend on the rows
- * beside it and on the lengths, by which the positions are split.  max_seq_len (at most 2^30) bounds seq_lens;
- * B and num_groups are at most 1024, head_dim is 64, 128 or 256, q, pages, out and the workspace are 16-byte
- * aligned (else SSD_ERR_UNSUPPORTED).  B = 0 or T = 0 does nothing.  The workspace needs no initial content and
- * keeps none.
+ * whose table entry is no block hold nothing; a row whose scores are all -inf is zeros.  Statistics and sums in
+ * fp32.  A row's bits depend on the rows beside it and on the lengths, by which the positions are split.
+ * max_seq_len (at most 2^30) bounds seq_lens; B and num_groups are at most 1024, head_dim is 64, 128 or 256, q,
+ * pages, out and the workspace are 16-byte aligned (else SSD_ERR_UNSUPPORTED); out is not q.  B = 0 or T = 0 does
+ * nothing.  The workspace needs no initial content and keeps none.
  */
 size_t ssd_shared_prefix_attention_workspace_size(int dtype, int B, int T, int num_heads, int num_kv_heads,
                                                   int head_dim, int block_size, int num_groups, int max_seq_len);

@@ -106,3 +106,22 @@ def test_many_starts_that_descend(cuda):
             got = shared_prefix_attention(**{**c, "group_starts": i32(starts)})
             assert torch.equal(got, shared_prefix_attention(**{**c, "group_starts": i32(upright)}))
             check({**c, "group_starts": i32(upright)})
+
+
+@pytest.mark.parametrize("dtype,bs", KINDS)
+@pytest.mark.parametrize("prefix", [0, 37, 1200])
+def test_scores_of_minus_infinity_weigh_nothing(cuda, prefix, dtype, bs):
+    """Some of a row's scores -inf: the others make the row.  All of them: zeros, as where nothing is seen."""
+    import torch
+
+    from ssd_b200.kernels.prefix_attention import shared_prefix_attention
+
+    c = case(26, [2, 1], [prefix, 20], [9, 300, 5], 1, 4, 2, 64, bs, dtype)
+    c["q"][..., 0] = 1.0
+    keys = c["cache"].pages[0]
+    for j in range(prefix, prefix + 9, 2):       # every second one of row 0's tail
+        keys[:, c["block_tables"][0, j // bs].long(), j % bs, :, 0] = float("-inf")
+    keys[:, c["block_tables"][2, :-(-25 // bs)].long(), :, :, 0] = float("-inf")  # all that row 2 sees
+    got = shared_prefix_attention(**c)
+    assert (got[2] == 0).all()
+    check({**c, "group_starts": c["group_starts"][:2].contiguous(), "prefix_lens": c["prefix_lens"][:1]})
