@@ -1629,6 +1629,7 @@ extern "C" int ssd_shared_prefix_attention(ssd_stream_t stream, const void* q, c
   if (L.tiles > 65535) return SSD_ERR_UNSUPPORTED;
   if (!workspace || workspace_bytes < L.total) return SSD_ERR_WORKSPACE;
   if (!kv8_aligned(workspace)) return SSD_ERR_UNSUPPORTED;
+  if (out == q) return SSD_ERR_INVALID;
   char* w = reinterpret_cast<char*>(workspace);
   PrefixAttn a{};
   a.q = q;

@@ -37,7 +37,7 @@ def shared_prefix_attention(q: torch.Tensor, cache: KVCacheState, layer: int, bl
     ``prefix_lens`` int32 [groups]: leading positions in which the group's rows agree, read through the table of its
     first row (0: nothing is shared).  The other arguments and the result are those of ``paged_verify_attention``:
     seq_lens [B] counts cached tokens INCLUDING the new ones, new token t of row b sits at position seq_lens[b] -
-    q_lens[b] + t and sees the positions up to it, rows past q_lens[b] come back as zeros.
+    q_lens[b] + t and sees the positions up to it, rows past q_lens[b] come back as zeros.  ``out`` may not be q.
     """
     p = cache.pages
     if len(p.shape) != 6 or p.shape[0] != 2 or not p.is_contiguous():

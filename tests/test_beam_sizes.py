@@ -102,3 +102,16 @@ def test_requests_go_by_the_memory_that_is_there():
     assert fit(180 << 30) == 64
     assert fit(10 * each) == 10 and fit(10 * each - 1) == 9 and fit(10 * each, 1) in (19, 20)
     assert fit(0) == 1 and fit(each // 2) == 1
+
+
+def test_attention_refuses_its_queries_as_output():
+    """Rows that V's infinities reach are worked out again from q, after others of the row's warps have written theirs."""
+    from ssd_b200 import _lib
+
+    p = 1 << 20  # an aligned address that no refused call touches
+
+    def call(out, ws):
+        return _lib.lib().ssd_shared_prefix_attention(None, p, p, 0, 2, 64, 16, 2, 64, 1, p, 8, p, None, p, p, 2, out, 0.1, 4,
+                                                      2, 8, 128, ws, 0 if ws is None else 1 << 40)
+
+    assert call(p, 4 * p) == 1 and call(2 * p, None) == 5
